@@ -68,7 +68,7 @@ class Glif3Bwd(C.Structure):
 
 
 EVENTS_INCONSISTENT = 1     # BMTK_EVENTS_INCONSISTENT
-ABI_VERSION = 37  # BMTK_AMD_ABI_VERSION of include/bmtk_amd.h that the mirrors above were written for
+ABI_VERSION = 38  # BMTK_AMD_ABI_VERSION of include/bmtk_amd.h that the mirrors above were written for
 
 # name -> (restype, argtypes); every symbol include/bmtk_amd.h declares
 SIGNATURES = {
@@ -129,6 +129,17 @@ SIGNATURES = {
     "bmtk_microbench_atomics": (c_int32, [c_void_p, c_int64, c_int32, c_int32, c_int32, c_void_p]),
     "bmtk_microbench_hop": (c_int32, [c_void_p, c_void_p, c_int32, c_int32, c_int32, C.c_uint32, c_void_p]),
     "bmtk_spike_counts": (c_int32, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p]),
+    "bmtk_spike_readout_workspace_bytes": (c_int64, [c_int64, c_int64, c_int32, c_int32]),
+    "bmtk_spike_readout_fwd": (c_int32, [c_void_p, c_int64, c_int64, c_int64, c_int32, c_void_p, c_int32, c_int32, c_void_p, c_void_p, c_void_p]),
+    "bmtk_spike_readout_bwd_weight": (c_int32, [c_void_p, c_int64, c_int64, c_int64, c_int32, c_void_p, c_int32, c_int32, c_void_p, c_void_p]),
+    "bmtk_spike_readout_bwd_spikes": (c_int32, [c_void_p, c_void_p, c_int64, c_int64, c_int32, c_int32, c_int32, c_void_p, c_void_p]),
+    "bmtk_gated_scan_workspace_bytes": (c_int64, [c_int64, c_int64, c_int32, c_int32, c_int32]),
+    "bmtk_gated_scan_fwd": (c_int32, [c_int64, c_int64] + [c_int32] * 4 + [c_void_p, c_int64, c_int64] * 2 + [c_void_p] * 7),
+    "bmtk_gated_scan_bwd": (c_int32, [c_int64, c_int64] + [c_int32] * 4 + [c_void_p, c_int64, c_int64] * 2 + [c_void_p] * 2 +
+                            [c_void_p, c_int64, c_int64] + [c_void_p] * 6),
+    "bmtk_token_logprobs_workspace_bytes": (c_int64, [c_int64, c_int32, c_int32, c_int32]),
+    "bmtk_token_logprobs_fwd": (c_int32, [c_int64, c_int32, c_int32, c_void_p, c_int64, c_void_p, c_int64, c_int32] + [c_void_p] * 7),
+    "bmtk_token_logprobs_bwd": (c_int32, [c_int64, c_int32, c_int32, c_void_p, c_int64, c_void_p, c_int64] + [c_void_p] * 5 + [c_int64, c_void_p]),
     "bmtk_rate_mse": (c_int32, [c_void_p, c_int64, c_int32, c_int64, c_void_p, c_int64] + [c_void_p] * 5),
 }
 
@@ -137,6 +148,8 @@ RES_SYNC_WORDS = (1 + 64 * 8) * 1088  # BMTK_RES_SYNC_WORDS
 COMPACT_NOALLOC_MAX_N = 1 << 24       # BMTK_COMPACT_NOALLOC_MAX_N
 RECORD_COUNT_STRIDE = 16
 RES_FIRED_SLOTS = 16              # BMTK_RES_FIRED_SLOTS
+SCAN_MARK = 16                    # BMTK_SCAN_MARK
+LOGPROBS_MAX_TOP = 64             # BMTK_LOGPROBS_MAX_TOP
 
 
 class LibraryMissing(RuntimeError):

@@ -1,0 +1,484 @@
+// Log probabilities of given tokens, the entropy and the most probable alternatives of each row, and the gradient by the logits.
+#include <math.h>
+
+#include "readout.hpp"
+
+namespace bmtk {
+namespace {
+
+constexpr float kLog2e = 1.44269504088896340736f;
+
+// Sums over a part of a row: maximum m, s = sum of e^(x - m), u = sum of (x - m) e^(x - m).  Then the logarithm of the whole sum is
+// m + log s and the entropy log s - u / s: no term of it is below zero, so nothing cancels.
+struct Sums {
+    float m, s, u;
+};
+
+// e^(x - m); the difference first, so that logits at the end of the type's range stay in it
+__device__ __forceinline__ float exp_diff(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
+
+// maximum with NaN as the largest value: a row with one shows it
+__device__ __forceinline__ float max_nan(float a, float b) { return a >= b || a != a ? a : b; }
+
+// a part's sums under the maximum m of several (one whose logits are all -inf, or too far below to count, adds nothing)
+__device__ __forceinline__ void raise_to(Sums &q, float m)
+{
+    const float d = q.m - m, e = q.m == -INFINITY ? 0.0f : exp_diff(d);
+    q.u = e == 0.0f ? 0.0f : (q.u + d * q.s) * e;
+    q.s *= e;
+    q.m = m;
+}
+// what two parts are together
+__device__ __forceinline__ Sums join(Sums a, Sums b)
+{
+    const float m = max_nan(a.m, b.m);
+    raise_to(a, m);
+    raise_to(b, m);
+    return Sums{m, a.s + b.s, a.u + b.u};
+}
+// log probability of a logit.  (Sums of a row with NaN or +inf are NaN.)
+__device__ __forceinline__ float logp_of(const Sums &q, float x) { return x == -INFINITY && q.s == q.s ? -INFINITY : (x - q.m) - logf(q.s); }
+
+// Order of the alternatives: the larger logit first (NaN before all), of equal ones the lower index.  One whole number for both;
+// 0 is below every real one.
+__device__ __forceinline__ uint64_t rank_of(float x, uint32_t index)
+{
+    uint32_t b = __float_as_uint(x + 0.0f);   // (-0 is 0)
+    if (x != x) b = 0x7fffffffu;
+    b = (int32_t)b < 0 ? ~b : b | 0x80000000u;
+    return ((uint64_t)b << 32) | (uint32_t)~index;
+}
+__device__ __forceinline__ uint32_t index_of(uint64_t rank) { return ~(uint32_t)rank; }
+__device__ __forceinline__ float logit_of(uint64_t rank)
+{
+    const uint32_t b = (uint32_t)(rank >> 32);
+    return __uint_as_float((int32_t)b < 0 ? b & 0x7fffffffu : ~b);
+}
+
+__device__ __forceinline__ uint64_t lane_xor(uint64_t v, int m)
+{
+    return ((uint64_t)(uint32_t)__shfl_xor((int)(v >> 32), m) << 32) | (uint32_t)__shfl_xor((int)(uint32_t)v, m);
+}
+__device__ __forceinline__ uint64_t lane_get(uint64_t v, int src)
+{
+    return ((uint64_t)(uint32_t)__shfl((int)(v >> 32), src) << 32) | (uint32_t)__shfl((int)(uint32_t)v, src);
+}
+
+// one comparison of a sorting network over lanes: the lane keeps the larger of its own and its partner's, or the smaller
+__device__ __forceinline__ uint64_t exchange(uint64_t v, int m, bool larger)
+{
+    const uint64_t o = lane_xor(v, m);
+    return (o > v) == larger ? o : v;
+}
+// lanes of each group of W, the largest first (bitonic)
+template <int W>
+__device__ __forceinline__ uint64_t sort_lanes(uint64_t v)
+{
+    const int l = lane_id() & (W - 1);
+#pragma unroll
+    for (int k = 2; k <= W; k *= 2)
+#pragma unroll
+        for (int m = k / 2; m > 0; m /= 2) v = exchange(v, m, ((l & m) == 0) == ((l & k) == 0 || k == W));
+    return v;
+}
+// the 64 largest of two sorted lists, sorted: the larger of each pair (l, 63 - l) are those, and are bitonic
+__device__ __forceinline__ uint64_t merge_lanes(uint64_t a, uint64_t b)
+{
+    const int l = lane_id();
+    const uint64_t o = lane_get(b, kWave - 1 - l);
+    uint64_t v = a > o ? a : o;
+#pragma unroll
+    for (int m = kWave / 2; m > 0; m /= 2) v = exchange(v, m, (l & m) == 0);
+    return v;
+}
+
+template <int W>
+__device__ __forceinline__ Sums join_lanes(Sums a)
+{
+#pragma unroll
+    for (int m = W / 2; m > 0; m /= 2) a = join(a, Sums{__shfl_xor(a.m, m), __shfl_xor(a.s, m), __shfl_xor(a.u, m)});
+    return a;
+}
+
+struct Row {
+    const void *logits;
+    const int64_t *tokens;
+    int64_t rows, row_stride;
+    int32_t vocab, top;
+    int64_t ignore;
+    float *logp, *entropy, *lse, *top_logp;
+    int64_t *top_index;
+};
+
+// what is written of a row, by one lane: its token's logit is read again
+template <typename T>
+__device__ __forceinline__ void write_row(const Row &a, int64_t r, const Sums &q)
+{
+    const int64_t token = a.tokens[r];
+    float lp = 0.0f;
+    if (token != a.ignore) {
+        lp = NAN;   // a token outside the vocabulary
+        if (token >= 0 && token < a.vocab) lp = logp_of(q, (float)static_cast<const T *>(a.logits)[r * a.row_stride + token]);
+    }
+    a.logp[r] = lp;
+    a.lse[r] = q.m == -INFINITY ? -INFINITY : q.m + logf(q.s);
+    a.entropy[r] = q.m == -INFINITY ? 0.0f : logf(q.s) - q.u / q.s;
+}
+
+__device__ __forceinline__ void write_top(const Row &a, int64_t r, const Sums &q, int k, uint64_t rank)
+{
+    a.top_index[r * a.top + k] = (int64_t)index_of(rank);
+    a.top_logp[r * a.top + k] = logp_of(q, logit_of(rank));
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Rows of up to 64 logits: W lanes each, one logit a lane
+template <typename T, int W>
+__global__ void __launch_bounds__(kBlock) logprobs_short_kernel(const Row a)
+{
+    const int l = lane_id() & (W - 1);
+    const int64_t r = (int64_t)blockIdx.x * (kBlock / W) + threadIdx.x / W;
+    const bool in = r < a.rows && l < a.vocab;
+    const float x = in ? (float)static_cast<const T *>(a.logits)[r * a.row_stride + l] : -INFINITY;
+    Sums q{x, x == -INFINITY ? 0.0f : 1.0f, 0.0f};
+    q = join_lanes<W>(q);
+    if (r < a.rows && l == 0) write_row<T>(a, r, q);
+    if (a.top > 0) {
+        const uint64_t v = sort_lanes<W>(in ? rank_of(x, l) : 0);
+        if (r < a.rows && l < a.top) write_top(a, r, q, l, v);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Longer rows: a workgroup takes a row, or a slice of one, in one pass.
+
+// A wavefront's alternatives: the 64 best so far, sorted, one a lane, and a queue of those that may be among them.  A logit is
+// compared with the last that counts; what passes waits until 64 do, which are sorted and merged in at once.
+struct Alternatives {
+    uint64_t best;
+    uint64_t last;       // the last of the best `top`
+    float least;         // its logit
+    unsigned waiting;
+    uint64_t *queue;     // 128 places in LDS
+
+    __device__ __forceinline__ void start(uint64_t *q) { best = last = 0, least = -INFINITY, waiting = 0, queue = q; }
+    __device__ __forceinline__ void take(int top)
+    {
+        const int l = lane_id();
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        const unsigned n = waiting < kWave ? waiting : kWave;
+        // (the last ones, so that the rest stays where it is)
+        const uint64_t v = (unsigned)l < n ? queue[waiting - n + l] : 0;
+        waiting -= n;
+        best = merge_lanes(best, sort_lanes<kWave>(v));
+        last = bcast_u64(best, top - 1);
+        if (last != 0) least = logit_of(last);
+        __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+        __builtin_amdgcn_wave_barrier();
+    }
+    __device__ __forceinline__ void look(float x, uint32_t index, bool in, int top)
+    {
+        const uint64_t rank = rank_of(x, index);
+        const bool may = in && rank > last;
+        const uint64_t mask = __ballot(may);
+        if (mask == 0) return;
+        if (may) queue[waiting + lane_prefix(mask)] = rank;
+        waiting += (unsigned)__popcll(mask);
+        __builtin_amdgcn_wave_barrier();
+        if (waiting >= kWave) take(top);
+    }
+};
+
+// one logit into a lane's sums; m is the maximum already
+__device__ __forceinline__ void add_logit(Sums &q, float x)
+{
+    const float d = x - q.m, e = exp_diff(d);
+    q.s += e;
+    q.u += e == 0.0f ? 0.0f : d * e;
+}
+template <typename T, int N, bool kTop>
+__device__ __forceinline__ void take_logits(Sums &q, Alternatives &alt, const float (&x)[N], uint32_t index, bool in, int top)
+{
+    float m = x[0];
+#pragma unroll
+    for (int k = 1; k < N; ++k) m = max_nan(m, x[k]);
+    if (in && m != -INFINITY) {
+        if (!(m <= q.m)) raise_to(q, m);
+#pragma unroll
+        for (int k = 0; k < N; ++k) add_logit(q, x[k]);
+    }
+    // (equal ones are looked at, and a NaN, which comes before all)
+    if (kTop && __ballot(in && !(m < alt.least)) != 0)
+#pragma unroll
+        for (int k = 0; k < N; ++k) alt.look(x[k], index + k, in, top);
+}
+
+struct Slices {
+    int32_t count;
+    int32_t length;      // logits of a slice
+    float *sums;         // [rows][count][3]
+    uint64_t *best;      // [rows][count][top]
+};
+
+template <typename T, int kWaves, bool kTop>
+__global__ void __launch_bounds__(kWaves * kWave) logprobs_kernel(const Row a, const Slices sl)
+{
+    constexpr int N = 16 / sizeof(T);
+    __shared__ Sums wave_sums[kWaves];
+    __shared__ uint64_t queues[kTop ? kWaves : 1][2 * kWave];
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
+    const int64_t r = blockIdx.x;
+    const T *row = static_cast<const T *>(a.logits) + r * a.row_stride;
+    const int begin = (int)blockIdx.y * sl.length, end = min(a.vocab, begin + sl.length);
+    Sums q{-INFINITY, 0.0f, 0.0f};
+    Alternatives alt;
+    if (kTop) alt.start(queues[wave]);
+
+    // 16 bytes a lane and load from the first address that allows it; what lies before and behind, logit by logit
+    const int odd = (int)((reinterpret_cast<uintptr_t>(row + begin) & 15) / sizeof(T));
+    const int body = min(end, begin + (odd ? N - odd : 0));
+    const int packs = (end - body) / N, tail = body + packs * N;
+    if (wave == 0) {
+        const int at = lane < body - begin ? begin + lane : tail + lane - (body - begin);
+        const bool in = at < end;
+        const float x[1] = {in ? (float)row[at] : -INFINITY};
+        take_logits<T, 1, kTop>(q, alt, x, (uint32_t)at, in, a.top);
+    }
+    for (int p = wave * kWave; p < packs; p += kWaves * kWave) {
+        const bool in = p + lane < packs;
+        Pack<T, N> v{};
+        if (in) v = *reinterpret_cast<const Pack<T, N> *>(row + body + (p + lane) * N);
+        float x[N];
+#pragma unroll
+        for (int k = 0; k < N; ++k) x[k] = (float)v.v[k];
+        take_logits<T, N, kTop>(q, alt, x, (uint32_t)(body + (p + lane) * N), in, a.top);
+    }
+    if (kTop)
+        while (alt.waiting) alt.take(a.top);
+    q = join_lanes<kWave>(q);
+    if (kWaves > 1) {
+        if (lane == 0) wave_sums[wave] = q;
+        if (kTop) queues[wave][lane] = alt.best;
+        __syncthreads();
+        if (wave != 0) return;
+        for (int w = 1; w < kWaves; ++w) {
+            q = join(q, wave_sums[w]);
+            if (kTop) alt.best = merge_lanes(alt.best, queues[w][lane]);
+        }
+    }
+    if (sl.count > 1) {
+        const int64_t at = r * sl.count + blockIdx.y;
+        if (lane == 0) sl.sums[at * 3] = q.m, sl.sums[at * 3 + 1] = q.s, sl.sums[at * 3 + 2] = q.u;
+        if (kTop && lane < a.top) sl.best[at * a.top + lane] = alt.best;
+        return;
+    }
+    if (lane == 0) write_row<T>(a, r, q);
+    if (kTop && lane < a.top) write_top(a, r, q, lane, alt.best);
+}
+
+// the slices of a row together
+template <typename T, bool kTop>
+__global__ void __launch_bounds__(kWave) logprobs_join_kernel(const Row a, const Slices sl)
+{
+    const int lane = lane_id();
+    const int64_t r = blockIdx.x;
+    Sums q{-INFINITY, 0.0f, 0.0f};
+    uint64_t best = 0;
+    for (int k = lane; k < sl.count; k += kWave) {
+        const float *p = sl.sums + (r * sl.count + k) * 3;
+        q = join(q, Sums{p[0], p[1], p[2]});
+    }
+    q = join_lanes<kWave>(q);
+    if (kTop)
+        for (int k = 0; k < sl.count; ++k) {
+            const uint64_t v = lane < a.top ? sl.best[(r * sl.count + k) * a.top + lane] : 0;
+            best = merge_lanes(best, v);
+        }
+    if (lane == 0) write_row<T>(a, r, q);
+    if (kTop && lane < a.top) write_top(a, r, q, lane, best);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Backward: with p = e^(x - lse), log probability l = x - lse and entropy H,
+//   d x_j = d_logp (delta_j,token - p_j) - d_entropy p_j (l_j + H)
+struct RowBwd {
+    const void *logits;
+    void *d_logits;
+    const int64_t *tokens;
+    const float *lse, *entropy, *d_logp, *d_entropy;
+    int64_t rows, row_stride, out_stride;
+    int32_t vocab;
+    int64_t ignore;
+};
+struct Factors {
+    float lse, by_logp, by_entropy, entropy;
+    int64_t token;
+};
+__device__ __forceinline__ Factors factors_of(const RowBwd &a, int64_t r)
+{
+    Factors f;
+    f.lse = a.lse[r];
+    f.entropy = a.entropy[r];
+    f.token = a.tokens[r];
+    f.by_logp = f.token == a.ignore ? 0.0f : a.d_logp ? a.d_logp[r] : 0.0f;
+    f.by_entropy = a.d_entropy ? a.d_entropy[r] : 0.0f;
+    if (f.token != a.ignore && (f.token < 0 || f.token >= a.vocab)) f.by_logp = NAN;   // as its log probability is
+    if (f.lse == -INFINITY) f.lse = f.by_logp = f.by_entropy = 0.0f;                      // a row of nothing but -inf: nothing moves it
+    return f;
+}
+__device__ __forceinline__ float gradient(const Factors &f, float x, int j)
+{
+    const float l = x - f.lse, p = exp_diff(l);
+    float d = -(p * f.by_logp);
+    if (p != 0.0f) d -= p * f.by_entropy * (l + f.entropy);   // (of a logit of -inf there is nothing)
+    return j == f.token ? d + f.by_logp : d;
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kBlock) logprobs_bwd_kernel(const RowBwd a, int length, bool together)
+{
+    constexpr int N = 16 / sizeof(T);
+    const int64_t r = blockIdx.x;
+    const T *row = static_cast<const T *>(a.logits) + r * a.row_stride;
+    T *out = static_cast<T *>(a.d_logits) + r * a.out_stride;
+    const int begin = (int)blockIdx.y * length, end = min(a.vocab, begin + length);
+    const Factors f = factors_of(a, r);
+    const int odd = (int)((reinterpret_cast<uintptr_t>(row + begin) & 15) / sizeof(T));
+    const int body = !together ? end : min(end, begin + (odd ? N - odd : 0));
+    const int packs = (end - body) / N, tail = body + packs * N;
+    for (int p = threadIdx.x; p < packs; p += kBlock) {
+        Pack<T, N> v = *reinterpret_cast<const Pack<T, N> *>(row + body + p * N);
+#pragma unroll
+        for (int k = 0; k < N; ++k) v.v[k] = (T)gradient(f, (float)v.v[k], body + p * N + k);
+        *reinterpret_cast<Pack<T, N> *>(out + body + p * N) = v;
+    }
+    const int apart = (body - begin) + (end - tail);
+    for (int k = threadIdx.x; k < apart; k += kBlock) {
+        const int at = k < body - begin ? begin + k : tail + k - (body - begin);
+        out[at] = (T)gradient(f, (float)row[at], at);
+    }
+}
+
+// short rows: logit by logit
+template <typename T>
+__global__ void __launch_bounds__(kBlock) logprobs_bwd_short_kernel(const RowBwd a, FastDiv by_vocab)
+{
+    const int64_t block_rows = kBlock;   // a workgroup takes this many rows, so that numbers within it are small
+    const int64_t r0 = (int64_t)blockIdx.x * block_rows;
+    const int here = (int)min(block_rows, a.rows - r0);
+    for (int c = threadIdx.x; c < here * a.vocab; c += kBlock) {
+        const int k = (int)div_by((uint32_t)c, by_vocab), j = c - k * a.vocab;
+        const int64_t r = r0 + k;
+        const Factors f = factors_of(a, r);
+        static_cast<T *>(a.d_logits)[r * a.out_stride + j] = (T)gradient(f, (float)static_cast<const T *>(a.logits)[r * a.row_stride + j], j);
+    }
+}
+
+// Slices of a row: enough workgroups to fill the chip, four loads a lane at least, and a whole number of 64 loads
+void slices_of(int64_t rows, int32_t vocab, int32_t dtype, Slices &sl)
+{
+    const int64_t unit = 4 * kBlock * (16 / (int64_t)type_size(dtype));
+    int64_t s = 768 / rows, most = div_up(vocab, unit);
+    if (s > most) s = most;
+    if (s < 1) s = 1;
+    sl.length = (int32_t)(div_up(div_up(vocab, s), 64) * 64);
+    sl.count = (int32_t)div_up(vocab, sl.length);
+}
+
+int check_logprobs(const char *who, int64_t rows, int32_t vocab, int32_t dtype, int32_t top)
+{
+    BMTK_REQUIRE(rows > 0 && vocab > 0, "%s: sizes must be positive", who);
+    BMTK_REQUIRE(rows < (1ll << 24) && vocab < (1 << 30), "%s: rows must stay below 2^24 and vocab below 2^30", who);
+    BMTK_REQUIRE(dtype == BMTK_F32 || dtype == BMTK_BF16 || dtype == BMTK_F16, "%s: unknown type %d", who, dtype);
+    BMTK_REQUIRE(top >= 0 && top <= BMTK_LOGPROBS_MAX_TOP && top <= vocab, "%s: top must lie in 0..min(%d, vocab)", who, BMTK_LOGPROBS_MAX_TOP);
+    return BMTK_OK;
+}
+
+constexpr int kShort = 64;       // a logit a lane
+constexpr int kOneWave = 2048;   // rows up to this length: a wavefront each
+
+}  // namespace
+}  // namespace bmtk
+
+using namespace bmtk;
+
+extern "C" int64_t bmtk_token_logprobs_workspace_bytes(int64_t rows, int32_t vocab, int32_t dtype, int32_t top)
+{
+    if (check_logprobs("token_logprobs_workspace_bytes", rows, vocab, dtype, top) != BMTK_OK || vocab <= kOneWave) return 0;
+    Slices sl{};
+    slices_of(rows, vocab, dtype, sl);
+    return sl.count > 1 ? rows * sl.count * (int64_t)(top * sizeof(uint64_t) + 3 * sizeof(float)) : 0;
+}
+
+extern "C" int bmtk_token_logprobs_fwd(int64_t rows, int32_t vocab, int32_t dtype, const void *logits, int64_t row_stride, const int64_t *tokens,
+                                       int64_t ignore, int32_t top, float *logp, float *entropy, float *lse, float *top_logp, int64_t *top_index,
+                                       void *workspace, void *stream)
+{
+    BMTK_REQUIRE(logits && tokens && logp && entropy && lse, "token_logprobs_fwd: pointers must be non-null");
+    const int rc = check_logprobs("token_logprobs_fwd", rows, vocab, dtype, top);
+    if (rc != BMTK_OK) return rc;
+    BMTK_REQUIRE(top == 0 || (top_logp && top_index), "token_logprobs_fwd: the alternatives have nowhere to go");
+    Row a{logits, tokens, rows, row_stride, vocab, top, ignore, logp, entropy, lse, top_logp, top_index};
+    const hipStream_t st = (hipStream_t)stream;
+    if (vocab <= kShort) {
+#define BMTK_SHORT(W) hipLaunchKernelGGL((logprobs_short_kernel<T, W>), dim3((unsigned)div_up(rows, kBlock / W)), dim3(kBlock), 0, st, a)
+        BMTK_BY_TYPE(dtype, T, {
+            if (vocab <= 16) BMTK_SHORT(16);
+            else BMTK_SHORT(64);
+        });
+#undef BMTK_SHORT
+        BMTK_CHECK_LAUNCH("token_logprobs_fwd");
+        return BMTK_OK;
+    }
+    Slices sl{1, vocab, nullptr, nullptr};
+    if (vocab > kOneWave) slices_of(rows, vocab, dtype, sl);
+    if (sl.count > 1) {
+        BMTK_REQUIRE(workspace && aligned(workspace, 8), "token_logprobs_fwd: needs its workspace");
+        sl.best = static_cast<uint64_t *>(workspace);
+        sl.sums = reinterpret_cast<float *>(sl.best + rows * sl.count * (int64_t)top);
+    }
+    const dim3 grid((unsigned)rows, (unsigned)sl.count);
+#define BMTK_ROWS(W, TOP) hipLaunchKernelGGL((logprobs_kernel<T, W, TOP>), grid, dim3(W *kWave), 0, st, a, sl)
+    BMTK_BY_TYPE(dtype, T, {
+        if (vocab <= kOneWave) {
+            if (top) BMTK_ROWS(1, true);
+            else BMTK_ROWS(1, false);
+        } else {
+            if (top) BMTK_ROWS(4, true);
+            else BMTK_ROWS(4, false);
+        }
+        if (sl.count > 1) {
+            if (top) hipLaunchKernelGGL((logprobs_join_kernel<T, true>), dim3((unsigned)rows), dim3(kWave), 0, st, a, sl);
+            else hipLaunchKernelGGL((logprobs_join_kernel<T, false>), dim3((unsigned)rows), dim3(kWave), 0, st, a, sl);
+        }
+    });
+#undef BMTK_ROWS
+    BMTK_CHECK_LAUNCH("token_logprobs_fwd");
+    return BMTK_OK;
+}
+
+extern "C" int bmtk_token_logprobs_bwd(int64_t rows, int32_t vocab, int32_t dtype, const void *logits, int64_t row_stride, const int64_t *tokens,
+                                       int64_t ignore, const float *lse, const float *entropy, const float *d_logp, const float *d_entropy, void *d_logits,
+                                       int64_t out_stride, void *stream)
+{
+    BMTK_REQUIRE(logits && tokens && lse && entropy && d_logits, "token_logprobs_bwd: pointers must be non-null");
+    const int rc = check_logprobs("token_logprobs_bwd", rows, vocab, dtype, 0);
+    if (rc != BMTK_OK) return rc;
+    BMTK_REQUIRE(d_logp || d_entropy, "token_logprobs_bwd: no gradient to go on from");
+    const RowBwd a{logits, d_logits, tokens, lse, entropy, d_logp, d_entropy, rows, row_stride, out_stride, vocab, ignore};
+    const hipStream_t st = (hipStream_t)stream;
+    const size_t size = type_size(dtype);
+    // loads and stores of 16 bytes: both rows begin at the same place of such a piece
+    const bool together = ((reinterpret_cast<uintptr_t>(logits) ^ reinterpret_cast<uintptr_t>(d_logits)) & 15) == 0 && (((row_stride - out_stride) * (int64_t)size) & 15) == 0;
+    if (vocab < 512) {
+        const FastDiv by_vocab = fast_div((uint32_t)vocab);
+        BMTK_BY_TYPE(dtype, T, hipLaunchKernelGGL((logprobs_bwd_short_kernel<T>), dim3((unsigned)div_up(rows, kBlock)), dim3(kBlock), 0, st, a, by_vocab));
+    } else {
+        Slices sl{};
+        slices_of(rows, vocab, dtype, sl);
+        const dim3 grid((unsigned)rows, (unsigned)sl.count);
+        BMTK_BY_TYPE(dtype, T, hipLaunchKernelGGL((logprobs_bwd_kernel<T>), grid, dim3(kBlock), 0, st, a, sl.length, together));
+    }
+    BMTK_CHECK_LAUNCH("token_logprobs_bwd");
+    return BMTK_OK;
+}

@@ -1,0 +1,495 @@
+// Gated linear recurrence over the steps of many sequences, h[t] = a[t] h[t - 1] + x[t], and its backward pass.
+#include "readout.hpp"
+
+namespace bmtk {
+namespace {
+
+constexpr int kSteps = BMTK_SCAN_MARK;  // steps that a wavefront holds in registers; the state before each such block is kept
+constexpr int kMaxWaves = 8;
+
+// One column is one channel of one sequence: column q = sequence q / dim, channel q % dim.  A lane takes V neighbouring columns.
+struct ScanArgs {
+    const void *x, *a;
+    const float *state;
+    const int32_t *lengths;
+    void *h;
+    float *last, *marks;
+    const void *dh;
+    const float *d_last;
+    void *dx, *da;
+    float *d_state, *da_part;   // da_part: partial sums of the gates' gradient
+    float *sums;                // [splits][2][columns]: product of the gates and end state of a stretch, see scan_sums
+    int64_t n_steps, columns, split_steps;
+    int64_t x_t, x_b, a_t, a_b, dh_t, dh_b;   // strides of what is read, in elements; what is written is contiguous
+    int32_t dim, channels;      // channels of a gate
+    int32_t seg_lanes;          // lanes whose part of a gate's gradient is summed at once (0: nothing is summed)
+    int32_t groups, parts;      // gates of a step and sequence; entries of da_part of a step and sequence
+};
+
+template <typename T, int V>
+__device__ __forceinline__ void load_v(const T *p, bool there, float other, float (&v)[V])
+{
+    if (there) {
+        const Pack<T, V> q = *reinterpret_cast<const Pack<T, V> *>(p);
+#pragma unroll
+        for (int c = 0; c < V; ++c) v[c] = (float)q.v[c];
+    } else {
+#pragma unroll
+        for (int c = 0; c < V; ++c) v[c] = other;
+    }
+}
+
+template <typename T, int V>
+__device__ __forceinline__ void store_v(T *p, const float (&v)[V])
+{
+    Pack<T, V> q;
+#pragma unroll
+    for (int c = 0; c < V; ++c) q.v[c] = (T)v[c];
+    *reinterpret_cast<Pack<T, V> *>(p) = q;
+}
+
+// Gates: one per channel for all steps, one per channel and step, or one per step for several neighbouring channels
+enum { kConst = 0, kEach = 1, kShared = 2 };
+
+template <typename TA, int V, int G>
+__device__ __forceinline__ void load_gate(const TA *p, const int (&off)[V], bool there, float (&v)[V])
+{
+    if (G == kEach) {
+        load_v<TA, V>(p + off[0], there, 1.0f, v);
+    } else {
+#pragma unroll
+        for (int c = 0; c < V; ++c) v[c] = there ? (float)p[off[c]] : 1.0f;
+    }
+}
+
+// What a lane knows of its columns
+template <int V>
+struct Lane {
+    int64_t col;
+    bool in;
+    int32_t b, ch, len;
+    int gate[V];
+};
+template <int V, int G>
+__device__ __forceinline__ Lane<V> lane_of(const ScanArgs &s)
+{
+    Lane<V> l;
+    l.col = ((int64_t)blockIdx.x * kWave + lane_id()) * V;
+    l.in = l.col < s.columns;
+    const int64_t q = l.in ? l.col : 0;
+    l.b = (int32_t)(q / s.dim);
+    l.ch = (int32_t)(q - (int64_t)l.b * s.dim);
+    l.len = !l.in ? 0 : s.lengths ? min(max(s.lengths[l.b], 0), (int32_t)s.n_steps) : (int32_t)s.n_steps;
+#pragma unroll
+    for (int c = 0; c < V; ++c) l.gate[c] = G == kShared ? (l.ch + c) / s.channels : l.ch + c;
+    return l;
+}
+
+// What is left of a state behind several steps.  (Decays above 1 may have a product that 32 bits do not hold: it leaves nothing nothing.)
+__device__ __forceinline__ float passed(float product, float state) { return state == 0.0f ? 0.0f : product * state; }
+
+// State that a stretch begins with: the stretches before it, in order.  sums[k][0]: product of the gates of stretch k, [1]: where it ends from zero.
+template <int V>
+__device__ __forceinline__ void fold(const float *sums, int64_t columns, const Lane<V> &l, int first, int last, int by, float (&h)[V])
+{
+    if (!l.in) return;
+    for (int k = first; k != last; k += by) {
+        float p[V], e[V];
+        load_v<float, V>(sums + (int64_t)(2 * k) * columns + l.col, true, 0.0f, p);
+        load_v<float, V>(sums + (int64_t)(2 * k + 1) * columns + l.col, true, 0.0f, e);
+#pragma unroll
+        for (int c = 0; c < V; ++c) h[c] = passed(p[c], h[c]) + e[c];
+    }
+}
+
+// One pass over the steps of a stretch in rounds: each wavefront takes kSteps steps into registers, finds what they do to a state
+// that enters them, (product of the gates, end from zero), the wavefronts tell each other, and each then computes its steps from the
+// state that really enters.  Everything is read once.  kBack: in descending order of time, the state being c[t] = a[t] (dh[t] + c[t + 1]),
+// what a gradient that enters behind step t becomes before it.  kSumsOnly: only what the whole stretch does, for the stretches behind it.
+template <typename TX, typename TA, int V, int G, bool kBack, bool kSumsOnly>
+__global__ void __launch_bounds__(kMaxWaves * kWave) scan_kernel(const ScanArgs s)
+{
+    __shared__ float tell[2][kMaxWaves][2][V][kWave];
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), waves = blockDim.x / kWave;
+    const Lane<V> l = lane_of<V, G>(s);
+    const int64_t t_lo = (int64_t)blockIdx.y * s.split_steps, t_hi = min(s.n_steps, t_lo + s.split_steps);
+    const TX *x = static_cast<const TX *>(s.x) + (int64_t)l.b * s.x_b + l.ch;
+    const TA *a = static_cast<const TA *>(s.a) + (G == kConst ? 0 : (int64_t)l.b * s.a_b);
+    const TX *dh = static_cast<const TX *>(s.dh) + (kBack ? (int64_t)l.b * s.dh_b + l.ch : 0);
+    float a_const[V], d_const[V] = {};
+    if (G == kConst) load_gate<TA, V, kEach>(a, l.gate, l.in, a_const);
+
+    float enter[V], whole[V];   // the state that enters a round; kSumsOnly: product of the gates so far, too
+#pragma unroll
+    for (int c = 0; c < V; ++c) enter[c] = 0.0f, whole[c] = 1.0f;
+    if (!kSumsOnly) {
+        if (kBack) {
+            if (s.d_last && l.in) load_v<float, V>(s.d_last + l.col, true, 0.0f, enter);
+            fold<V>(s.sums, s.columns, l, gridDim.y - 1, blockIdx.y, -1, enter);
+        } else {
+            if (s.state && l.in) load_v<float, V>(s.state + l.col, true, 0.0f, enter);
+            fold<V>(s.sums, s.columns, l, 0, blockIdx.y, 1, enter);
+        }
+    }
+    const int64_t rounds = (t_hi - t_lo + (int64_t)waves * kSteps - 1) / ((int64_t)waves * kSteps);
+    for (int64_t round = 0; round < rounds; ++round) {
+        // a wavefront's block in the order in which the state passes: the last block first on the way back
+        const int64_t block = kBack ? rounds * waves - 1 - (round * waves + wave) : round * waves + wave;
+        const int64_t t0 = t_lo + block * kSteps;
+        float xv[kSteps][V], av[kSteps][V], gv[kBack ? kSteps : 1][V];
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+            const int64_t t = t0 + k;
+            const bool there = t < t_hi && t < l.len;
+            if (!(kBack && kSumsOnly)) load_v<TX, V>(x + t * s.x_t, there, 0.0f, xv[k]);
+            if (kBack) load_v<TX, V>(dh + t * s.dh_t, there, 0.0f, gv[k]);
+            if (G == kConst) {
+#pragma unroll
+                for (int c = 0; c < V; ++c) av[k][c] = there ? a_const[c] : 1.0f;
+            } else {
+                load_gate<TA, V, G>(a + t * s.a_t, l.gate, there, av[k]);
+            }
+        }
+        float p[V], e[V];
+#pragma unroll
+        for (int c = 0; c < V; ++c) {
+            p[c] = 1.0f, e[c] = 0.0f;
+            if (kBack) {
+#pragma unroll
+                for (int k = kSteps - 1; k >= 0; --k) e[c] = av[k][c] * (gv[k][c] + e[c]), p[c] *= av[k][c];
+            } else {
+#pragma unroll
+                for (int k = 0; k < kSteps; ++k) e[c] = av[k][c] * e[c] + xv[k][c], p[c] *= av[k][c];
+            }
+            tell[round & 1][wave][0][c][lane] = p[c];
+            tell[round & 1][wave][1][c][lane] = e[c];
+        }
+        // (two sets of places in turn: whoever writes the one of a round has passed the barrier behind the round before)
+        __syncthreads();
+        float mine[V];
+        for (int w = 0; w < waves; ++w) {
+            if (w == wave)
+#pragma unroll
+                for (int c = 0; c < V; ++c) mine[c] = enter[c];
+#pragma unroll
+            for (int c = 0; c < V; ++c) {
+                const float pw = tell[round & 1][w][0][c][lane];
+                enter[c] = passed(pw, enter[c]) + tell[round & 1][w][1][c][lane];
+                if (kSumsOnly) whole[c] *= pw;
+            }
+        }
+        if (kSumsOnly || t0 >= t_hi) continue;
+        if (!kBack) {
+            TX *h = static_cast<TX *>(s.h);
+            if (s.marks && l.in) store_v<float, V>(s.marks + t0 / kSteps * s.columns + l.col, mine);
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) {
+                float out[V];
+#pragma unroll
+                for (int c = 0; c < V; ++c) {
+                    mine[c] = av[k][c] * mine[c] + xv[k][c];
+                    out[c] = t0 + k < l.len ? mine[c] : 0.0f;
+                }
+                if (t0 + k < t_hi && l.in) store_v<TX, V>(h + (t0 + k) * s.columns + l.col, out);
+            }
+        } else {
+            // the states before each step, again from the kept one
+            float before[kSteps][V];
+            if (l.in) load_v<float, V>(s.marks + t0 / kSteps * s.columns + l.col, true, 0.0f, before[0]);
+            else
+#pragma unroll
+                for (int c = 0; c < V; ++c) before[0][c] = 0.0f;
+#pragma unroll
+            for (int k = 1; k < kSteps; ++k)
+#pragma unroll
+                for (int c = 0; c < V; ++c) before[k][c] = av[k - 1][c] * before[k - 1][c] + xv[k - 1][c];
+            TX *dx = static_cast<TX *>(s.dx);
+            TA *da = static_cast<TA *>(s.da);
+#pragma unroll
+            for (int k = kSteps - 1; k >= 0; --k) {
+                const int64_t t = t0 + k;
+                float g[V], d[V];
+#pragma unroll
+                for (int c = 0; c < V; ++c) {
+                    const float all = gv[k][c] + mine[c];
+                    g[c] = t < l.len ? all : 0.0f;   // (behind a sequence's end the gradient of its last state passes through)
+                    d[c] = t < l.len ? all * before[k][c] : 0.0f;
+                    mine[c] = av[k][c] * all;
+                    if (G == kConst) d_const[c] += d[c];
+                }
+                const bool write = t < t_hi && l.in;
+                if (write) store_v<TX, V>(dx + t * s.columns + l.col, g);
+                if (G == kEach && write) store_v<TA, V>(da + t * s.columns + l.col, d);
+                if (G == kShared) {
+                    float sum = d[0];
+                    if (V == 2 && s.seg_lanes) sum += d[1];
+                    for (int m = 1; m < s.seg_lanes; m *= 2) sum += __shfl_xor(sum, m);
+                    if (write) {
+                        // a gate's channels within the lanes: its gradient; else parts of it, to be joined
+                        const int64_t at = (t * (s.columns / s.dim) + l.b) * (int64_t)s.parts;
+                        if (s.da_part == nullptr) {
+                            if (lane % s.seg_lanes == 0) da[at + l.gate[0]] = (TA)sum;
+                        } else if (s.seg_lanes) {
+                            if (lane % s.seg_lanes == 0) s.da_part[at + l.ch / (V * s.seg_lanes)] = sum;
+                        } else {
+                            store_v<float, V>(s.da_part + at + l.ch, d);
+                        }
+                    }
+                }
+            }
+        }
+    }
+    if (!l.in) return;
+    if (kSumsOnly) {
+        if (wave == 0) {
+            store_v<float, V>(s.sums + (int64_t)(2 * blockIdx.y) * s.columns + l.col, whole);
+            store_v<float, V>(s.sums + (int64_t)(2 * blockIdx.y + 1) * s.columns + l.col, enter);
+        }
+        return;
+    }
+    if (!kBack) {
+        if (wave == 0 && blockIdx.y == gridDim.y - 1) store_v<float, V>(s.last + l.col, enter);
+        return;
+    }
+    if (wave == 0 && blockIdx.y == 0 && s.d_state) store_v<float, V>(s.d_state + l.col, enter);
+    if (G == kConst) store_v<float, V>(s.da_part + ((int64_t)blockIdx.y * waves + wave) * s.columns + l.col, d_const);
+}
+
+// One step: nothing to join
+template <typename TX, typename TA, int V, int G>
+__global__ void __launch_bounds__(kBlock) scan_one_kernel(const ScanArgs s)
+{
+    Lane<V> l;
+    l.col = ((int64_t)blockIdx.x * kBlock + threadIdx.x) * V;
+    if (l.col >= s.columns) return;
+    l.b = (int32_t)(l.col / s.dim);
+    l.ch = (int32_t)(l.col - (int64_t)l.b * s.dim);
+#pragma unroll
+    for (int c = 0; c < V; ++c) l.gate[c] = G == kShared ? (l.ch + c) / s.channels : l.ch + c;
+    const bool there = !s.lengths || s.lengths[l.b] > 0;
+    float x[V], a[V], h[V], out[V];
+    load_v<TX, V>(static_cast<const TX *>(s.x) + (int64_t)l.b * s.x_b + l.ch, there, 0.0f, x);
+    load_gate<TA, V, G == kShared ? kShared : kEach>(static_cast<const TA *>(s.a) + (G == kConst ? 0 : (int64_t)l.b * s.a_b), l.gate, there, a);
+    load_v<float, V>(s.state + l.col, s.state != nullptr, 0.0f, h);
+    if (s.marks) store_v<float, V>(s.marks + l.col, h);
+#pragma unroll
+    for (int c = 0; c < V; ++c) {
+        h[c] = a[c] * h[c] + x[c];
+        out[c] = there ? h[c] : 0.0f;
+    }
+    store_v<TX, V>(static_cast<TX *>(s.h) + l.col, out);
+    store_v<float, V>(s.last + l.col, h);
+}
+
+// Gradient of one decay per channel: its parts by stretch, wavefront and sequence, in order
+template <typename TA>
+__global__ void __launch_bounds__(kBlock) scan_join_const_kernel(const float *__restrict__ part, int64_t parts, int dim, TA *__restrict__ da)
+{
+    __shared__ float sum[kBlock];
+    const int lane = lane_id(), wave = threadIdx.x / kWave;
+    const int ch = blockIdx.x * kWave + lane;
+    float v = 0.0f;
+    if (ch < dim)
+        for (int64_t k = wave; k < parts; k += kBlock / kWave) v += part[k * dim + ch];
+    sum[threadIdx.x] = v;
+    __syncthreads();
+    if (wave == 0 && ch < dim) {
+        for (int w = 1; w < kBlock / kWave; ++w) v += sum[w * kWave + lane];
+        da[ch] = (TA)v;
+    }
+}
+
+// Gradient of a shared gate: n_part parts next to one another
+template <typename TA>
+__global__ void __launch_bounds__(kBlock) scan_join_shared_kernel(const float *__restrict__ part, int64_t gates, int n_part, TA *__restrict__ da)
+{
+    const int64_t g = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+    if (g >= gates) return;
+    float v = 0.0f;
+    for (int k = 0; k < n_part; ++k) v += part[g * n_part + k];
+    da[g] = (TA)v;
+}
+
+int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
+
+// How a call is laid out.  A lane takes two channels of a 16-bit type where rows and strides allow it (four bytes a lane and load).
+struct Plan {
+    int v, waves, seg_lanes, parts;
+    int64_t tiles, splits, split_steps;
+};
+
+Plan plan_of(int64_t n_steps, int64_t batch, int32_t dim, int32_t groups, int32_t dtype, bool pairs)
+{
+    Plan p;
+    p.v = dtype != BMTK_F32 && dim % 2 == 0 && pairs ? 2 : 1;
+    p.tiles = div_up(batch * dim, kWave * p.v);
+    int64_t w = div_up(n_steps, kSteps);
+    p.waves = (int)(w < kMaxWaves ? w : kMaxWaves);
+    // stretches of time: as many as fill the chip, of two rounds at least
+    int64_t s = 1024 / p.tiles, most = n_steps / (2 * kMaxWaves * kSteps);
+    if (s > most) s = most;
+    if (s > 64) s = 64;
+    if (s < 1) s = 1;
+    p.split_steps = div_up(div_up(n_steps, s), kSteps) * kSteps;
+    p.splits = div_up(n_steps, p.split_steps);
+    p.seg_lanes = p.parts = 0;
+    if (groups > 0 && groups != dim) {
+        const int channels = dim / groups, seg = gcd(channels, kWave * p.v);
+        p.seg_lanes = seg >= p.v ? seg / p.v : 0;
+        p.parts = p.seg_lanes ? dim / seg : dim;
+    }
+    return p;
+}
+
+int check_scan(const char *who, int64_t n_steps, int64_t batch, int32_t dim, int32_t groups, int32_t dtype, int32_t gate_dtype)
+{
+    BMTK_REQUIRE(n_steps > 0 && batch > 0 && dim > 0 && groups >= 0, "%s: sizes must be positive", who);
+    BMTK_REQUIRE(groups == 0 || dim % groups == 0, "%s: %d gates do not share %d channels evenly", who, groups, dim);
+    BMTK_REQUIRE(dtype == BMTK_F32 || dtype == BMTK_BF16 || dtype == BMTK_F16, "%s: unknown type %d", who, dtype);
+    BMTK_REQUIRE(gate_dtype == BMTK_F32 || gate_dtype == dtype, "%s: decays are in 32 bits or of the input's type", who);
+    BMTK_REQUIRE(n_steps < (1ll << 31) - 4096 && batch < (1ll << 31) && batch * (int64_t)dim < (1ll << 31), "%s: too many steps or columns", who);
+    return BMTK_OK;
+}
+
+}  // namespace
+}  // namespace bmtk
+
+using namespace bmtk;
+
+extern "C" int64_t bmtk_gated_scan_workspace_bytes(int64_t n_steps, int64_t batch, int32_t dim, int32_t groups, int32_t backward)
+{
+    if (check_scan("gated_scan_workspace_bytes", n_steps, batch, dim, groups, BMTK_F32, BMTK_F32) != BMTK_OK) return 0;
+    int64_t most = 0;
+    for (int pairs = 0; pairs < 2; ++pairs) {
+        const Plan p = plan_of(n_steps, batch, dim, groups, BMTK_BF16, pairs != 0);
+        int64_t floats = p.splits > 1 ? 2 * p.splits * batch * dim : 0;
+        if (backward && groups == 0) floats += p.splits * p.waves * batch * dim;
+        if (backward && groups > 0 && groups != dim && p.parts != groups) floats += n_steps * batch * p.parts;
+        most = floats > most ? floats : most;
+    }
+    return most * (int64_t)sizeof(float);
+}
+
+#define BMTK_SCAN_LAUNCH(BACK, SUMS)                                                                                                      \
+    do {                                                                                                                                  \
+        if (groups == 0) hipLaunchKernelGGL((scan_kernel<TX, TA, V, kConst, BACK, SUMS>), grid, dim3(p.waves *kWave), 0, st, s);           \
+        else if (groups == dim) hipLaunchKernelGGL((scan_kernel<TX, TA, V, kEach, BACK, SUMS>), grid, dim3(p.waves *kWave), 0, st, s);     \
+        else hipLaunchKernelGGL((scan_kernel<TX, TA, V, kShared, BACK, SUMS>), grid, dim3(p.waves *kWave), 0, st, s);                      \
+    } while (0)
+
+namespace {
+
+template <typename TX, typename TA, int V>
+void launch_fwd(const ScanArgs &s, const Plan &p, int groups, hipStream_t st)
+{
+    const int dim = s.dim;
+    if (s.n_steps == 1) {
+        const dim3 one((unsigned)div_up(s.columns, kBlock * V));
+        if (groups == 0) hipLaunchKernelGGL((scan_one_kernel<TX, TA, V, kConst>), one, dim3(kBlock), 0, st, s);
+        else if (groups == dim) hipLaunchKernelGGL((scan_one_kernel<TX, TA, V, kEach>), one, dim3(kBlock), 0, st, s);
+        else hipLaunchKernelGGL((scan_one_kernel<TX, TA, V, kShared>), one, dim3(kBlock), 0, st, s);
+        return;
+    }
+    dim3 grid((unsigned)p.tiles, (unsigned)p.splits);
+    if (p.splits > 1) BMTK_SCAN_LAUNCH(false, true);
+    BMTK_SCAN_LAUNCH(false, false);
+}
+
+template <typename TX, typename TA, int V>
+void launch_bwd(ScanArgs s, const Plan &p, int groups, hipStream_t st)
+{
+    const int dim = s.dim;
+    const int64_t batch = s.columns / dim;
+    dim3 grid((unsigned)p.tiles, (unsigned)p.splits);
+    if (p.splits > 1) BMTK_SCAN_LAUNCH(true, true);
+    BMTK_SCAN_LAUNCH(true, false);
+    if (groups == 0)
+        hipLaunchKernelGGL((scan_join_const_kernel<TA>), dim3((unsigned)div_up(dim, kWave)), dim3(kBlock), 0, st, s.da_part, p.splits * p.waves * batch, dim,
+                           (TA *)s.da);
+    else if (s.da_part)
+        hipLaunchKernelGGL((scan_join_shared_kernel<TA>), dim3((unsigned)div_up(s.n_steps * batch * groups, kBlock)), dim3(kBlock), 0, st, s.da_part,
+                           s.n_steps * batch * groups, p.parts / groups, (TA *)s.da);
+}
+
+}  // namespace
+
+// TX, TA and V for the call's types; V = 2 only for 16-bit types
+#define BMTK_SCAN_TYPES(DO)                                             \
+    do {                                                                \
+        if (dtype == BMTK_F32) DO(float, float, 1);                     \
+        else if (dtype == BMTK_BF16) {                                  \
+            if (gate_dtype == BMTK_F32) {                               \
+                if (p.v == 2) DO(bf16, float, 2);                       \
+                else DO(bf16, float, 1);                                \
+            } else {                                                    \
+                if (p.v == 2) DO(bf16, bf16, 2);                        \
+                else DO(bf16, bf16, 1);                                 \
+            }                                                           \
+        } else {                                                        \
+            if (gate_dtype == BMTK_F32) {                               \
+                if (p.v == 2) DO(f16, float, 2);                        \
+                else DO(f16, float, 1);                                 \
+            } else {                                                    \
+                if (p.v == 2) DO(f16, f16, 2);                          \
+                else DO(f16, f16, 1);                                   \
+            }                                                           \
+        }                                                               \
+    } while (0)
+
+// two neighbouring channels in one load
+static bool in_pairs(const void *p, int dtype, int64_t stride_t, int64_t stride_b)
+{
+    return aligned(p, 2 * type_size(dtype)) && stride_t % 2 == 0 && stride_b % 2 == 0;
+}
+
+extern "C" int bmtk_gated_scan_fwd(int64_t n_steps, int64_t batch, int32_t dim, int32_t groups, int32_t dtype, int32_t gate_dtype, const void *x, int64_t x_t,
+                                   int64_t x_b, const void *decay, int64_t a_t, int64_t a_b, const float *state, const int32_t *lengths, void *h, float *last,
+                                   float *marks, float *workspace, void *stream)
+{
+    BMTK_REQUIRE(x && decay && h && last, "gated_scan_fwd: pointers must be non-null");
+    const int rc = check_scan("gated_scan_fwd", n_steps, batch, dim, groups, dtype, gate_dtype);
+    if (rc != BMTK_OK) return rc;
+    bool pairs = in_pairs(x, dtype, x_t, x_b) && in_pairs(h, dtype, 0, 0) && aligned(state, 8) && aligned(last, 8) && aligned(marks, 8);
+    if (groups == dim || groups == 0) pairs = pairs && in_pairs(decay, gate_dtype, a_t, a_b);
+    const Plan p = plan_of(n_steps, batch, dim, groups, dtype, pairs);
+    BMTK_REQUIRE(p.splits == 1 || n_steps == 1 || workspace, "gated_scan_fwd: needs its workspace");
+    ScanArgs s{};
+    s.x = x, s.a = decay, s.state = state, s.lengths = lengths, s.h = h, s.last = last, s.marks = marks, s.sums = workspace;
+    s.n_steps = n_steps, s.columns = batch * dim, s.split_steps = p.split_steps;
+    s.x_t = x_t, s.x_b = x_b, s.a_t = a_t, s.a_b = a_b;
+    s.dim = dim, s.channels = groups > 0 ? dim / groups : 1, s.groups = groups;
+    const hipStream_t st = (hipStream_t)stream;
+#define BMTK_DO(TX, TA, V) launch_fwd<TX, TA, V>(s, p, groups, st)
+    BMTK_SCAN_TYPES(BMTK_DO);
+#undef BMTK_DO
+    BMTK_CHECK_LAUNCH("gated_scan_fwd");
+    return BMTK_OK;
+}
+
+extern "C" int bmtk_gated_scan_bwd(int64_t n_steps, int64_t batch, int32_t dim, int32_t groups, int32_t dtype, int32_t gate_dtype, const void *x, int64_t x_t,
+                                   int64_t x_b, const void *decay, int64_t a_t, int64_t a_b, const float *marks, const int32_t *lengths, const void *dh,
+                                   int64_t dh_t, int64_t dh_b, const float *d_last, void *dx, void *d_decay, float *d_state, float *workspace, void *stream)
+{
+    BMTK_REQUIRE(x && decay && marks && dh && dx && d_decay, "gated_scan_bwd: pointers must be non-null");
+    const int rc = check_scan("gated_scan_bwd", n_steps, batch, dim, groups, dtype, gate_dtype);
+    if (rc != BMTK_OK) return rc;
+    bool pairs = in_pairs(x, dtype, x_t, x_b) && in_pairs(dh, dtype, dh_t, dh_b) && in_pairs(dx, dtype, 0, 0) && aligned(marks, 8) && aligned(d_last, 8) &&
+                 aligned(d_state, 8) && aligned(workspace, 8);
+    if (groups == dim || groups == 0) pairs = pairs && in_pairs(decay, gate_dtype, a_t, a_b) && in_pairs(d_decay, gate_dtype, 0, 0);
+    const Plan p = plan_of(n_steps, batch, dim, groups, dtype, pairs);
+    const bool joined = groups == 0 || (groups != dim && p.parts != groups);
+    BMTK_REQUIRE((p.splits == 1 && !joined) || workspace, "gated_scan_bwd: needs its workspace");
+    ScanArgs s{};
+    s.x = x, s.a = decay, s.lengths = lengths, s.marks = const_cast<float *>(marks), s.dh = dh, s.d_last = d_last;
+    s.dx = dx, s.da = d_decay, s.d_state = d_state, s.sums = workspace;
+    if (joined) s.da_part = workspace + (p.splits > 1 ? 2 * p.splits * batch * dim : 0);
+    s.n_steps = n_steps, s.columns = batch * dim, s.split_steps = p.split_steps;
+    s.x_t = x_t, s.x_b = x_b, s.a_t = a_t, s.a_b = a_b, s.dh_t = dh_t, s.dh_b = dh_b;
+    s.dim = dim, s.channels = groups > 0 ? dim / groups : 1, s.groups = groups, s.seg_lanes = p.seg_lanes, s.parts = p.parts;
+    const hipStream_t st = (hipStream_t)stream;
+#define BMTK_DO(TX, TA, V) launch_bwd<TX, TA, V>(s, p, groups, st)
+    BMTK_SCAN_TYPES(BMTK_DO);
+#undef BMTK_DO
+    BMTK_CHECK_LAUNCH("gated_scan_bwd");
+    return BMTK_OK;
+}

@@ -1,0 +1,489 @@
+// Readout of spikes: y[t, b] = sum of the weight rows of the neurons that fired in step t of trial b, and its gradients.
+#include "readout.hpp"
+
+namespace bmtk {
+namespace {
+
+constexpr int kWaves = 4;
+constexpr int kQueue = 128;       // spikes found and not yet added: at most 63 left over and 64 new ones
+constexpr int kWordsPerLane = 4;  // spike words that a lane has under way at once
+constexpr int kRowLoads = 8;      // rows under way at once
+constexpr int kSumRows = 60;      // rows of 64 sums of a wavefront, in LDS: four wavefronts' and their queues are 64 KB
+
+// A wavefront's own queue is written and read by different lanes of it, in order: what the compiler must keep is that order.
+__device__ __forceinline__ void wave_order()
+{
+    __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
+    __builtin_amdgcn_wave_barrier();
+}
+
+__device__ __forceinline__ void lds_add(float *p, float v)
+{
+    __hip_atomic_fetch_add(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
+}
+
+template <typename T, int VW>
+__device__ __forceinline__ void load_row(const T *p, bool in, float (&v)[VW])
+{
+    Pack<T, VW> q{};
+    if (in) q = *reinterpret_cast<const Pack<T, VW> *>(p);
+#pragma unroll
+    for (int c = 0; c < VW; ++c) v[c] = (float)q.v[c];
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Forward.  A workgroup takes one step and a slice of its words of spike bits; a wavefront turns the set bits of 256 words at a
+// time into a queue of element numbers, works it off 64 spikes at a time (each lane divides one of them into neuron and trial),
+// and reads the weight rows, one per spike, 64 * VW channels by its 64 lanes.  The sums of a trial are the wavefront's own (in LDS, or
+// in registers for one trial), so their order is fixed; the wavefronts' sums are added in order at the end.
+template <typename T, int VW, bool kOne>
+__global__ void __launch_bounds__(kWaves * kWave)
+spike_fwd_kernel(const uint64_t *__restrict__ bits, int64_t stride, int64_t ne, FastDiv by_batch, int trials, int trial_tiles,
+                 const T *__restrict__ weight, int dim, int64_t slice_words, T *__restrict__ y, float *__restrict__ part)
+{
+    extern __shared__ float lds[];
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
+    const int64_t t = blockIdx.x;
+    const int batch = (int)by_batch.d;
+    const int b0 = (int)(blockIdx.z % trial_tiles) * trials, ch0 = (int)(blockIdx.z / trial_tiles) * kWave * VW;
+    const int cells = trials * kWave * VW;
+    float *acc = lds + wave * cells;
+    uint32_t *queue = reinterpret_cast<uint32_t *>(lds + kWaves * cells) + wave * kQueue;
+    const int ch = ch0 + lane * VW;
+    const bool in = ch < dim;
+    float one[VW] = {};
+    if (!kOne)
+        for (int c = lane; c < cells; c += kWave) acc[c] = 0.0f;
+    const int64_t words = (ne + 63) >> 6;
+    const int64_t w_end = min(words, (int64_t)(blockIdx.y + 1) * slice_words);
+    const uint64_t *row = bits + t * stride;
+    const T *wcol = weight + ch;
+    unsigned head = 0, tail = 0;
+
+    auto work_off = [&](int m) {
+        const uint32_t e = queue[(head + lane) & (kQueue - 1)];
+        const int i = (int)div_by(e, by_batch);
+        const int b = (int)e - i * batch - b0;
+        for (int k = 0; k < m; k += kRowLoads) {
+            float v[kRowLoads][VW];
+#pragma unroll
+            for (int u = 0; u < kRowLoads; ++u)
+                load_row<T, VW>(wcol + (int64_t)bcast_i(i, min(k + u, m - 1)) * dim, in, v[u]);
+#pragma unroll
+            for (int u = 0; u < kRowLoads; ++u) {
+                if (k + u >= m) break;
+                if (kOne) {
+#pragma unroll
+                    for (int c = 0; c < VW; ++c) one[c] += v[u][c];
+                } else {
+                    const int bb = bcast_i(b, k + u);
+                    if ((unsigned)bb < (unsigned)trials)
+#pragma unroll
+                        for (int c = 0; c < VW; ++c) lds_add(acc + (bb * VW + c) * kWave + lane, v[u][c]);
+                }
+            }
+        }
+        head += m;
+    };
+
+    for (int64_t c = (int64_t)blockIdx.y * slice_words + wave * (kWave * kWordsPerLane); c < w_end; c += kWaves * kWave * kWordsPerLane) {
+        uint64_t w[kWordsPerLane];
+#pragma unroll
+        for (int k = 0; k < kWordsPerLane; ++k) {
+            const int64_t at = c + k * kWave + lane;
+            w[k] = at < w_end ? row[at] : 0;
+            if (at == words - 1 && (ne & 63)) w[k] &= (1ull << (ne & 63)) - 1;
+        }
+#pragma unroll
+        for (int k = 0; k < kWordsPerLane; ++k) {
+            const uint32_t first = (uint32_t)((c + k * kWave + lane) << 6);
+            unsigned long long mask;
+            while ((mask = __ballot(w[k] != 0)) != 0) {
+                if (w[k] != 0) {
+                    queue[(tail + lane_prefix(mask)) & (kQueue - 1)] = first + (uint32_t)__builtin_ctzll(w[k]);
+                    w[k] &= w[k] - 1;
+                }
+                tail += (unsigned)__popcll(mask);
+                wave_order();
+                if (tail - head >= kWave) {
+                    work_off(kWave);
+                    wave_order();
+                }
+            }
+        }
+    }
+    if (tail != head) work_off((int)(tail - head));
+    if (kOne)
+#pragma unroll
+        for (int c = 0; c < VW; ++c) acc[c * kWave + lane] = one[c];
+    __syncthreads();
+    const int here = min(trials, batch - b0);
+    const int64_t out = (t * batch + b0) * (int64_t)dim + ch0;
+    const int64_t plane = (int64_t)gridDim.x * batch * dim;
+    for (int c = threadIdx.x; c < here * kWave * VW; c += kWaves * kWave) {
+        const int l = c % (kWave * VW), b = c / (kWave * VW);
+        if (ch0 + l >= dim) continue;
+        const float *a = lds + (b * VW + l % VW) * kWave + l / VW;
+        float s = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kWaves; ++k) s += a[k * cells];
+        if (part)
+            part[blockIdx.y * plane + out + (int64_t)b * dim + l] = s;
+        else
+            y[out + (int64_t)b * dim + l] = (T)s;
+    }
+}
+
+template <typename T>
+__global__ void __launch_bounds__(kBlock) spike_join_kernel(const float *__restrict__ part, int slices, int64_t plane, T *__restrict__ y)
+{
+    const int64_t c = (int64_t)blockIdx.x * kBlock + threadIdx.x;
+    if (c >= plane) return;
+    float s = 0.0f;
+    for (int k = 0; k < slices; ++k) s += part[k * plane + c];
+    y[c] = (T)s;
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Gradient by the weights: row i is the sum of dy[t, b] over the spikes of neuron i.  A wavefront owns `own` neurons and their
+// sums (in LDS), looks through their bits of all steps and reads the dy rows as the forward pass reads the weights.  Nobody else
+// adds to its sums: the order is fixed and nothing has to be joined.
+template <typename T, int VW>
+__global__ void __launch_bounds__(kWaves * kWave)
+spike_bwd_weight_kernel(const uint64_t *__restrict__ bits, int64_t stride, int64_t n_steps, int64_t n, FastDiv by_batch, int own,
+                        const T *__restrict__ dy, int dim, T *__restrict__ d_weight)
+{
+    extern __shared__ float lds[];
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
+    const int batch = (int)by_batch.d;
+    const int cells = own * kWave * VW;
+    float *acc = lds + wave * cells;
+    uint64_t *queue = reinterpret_cast<uint64_t *>(lds + kWaves * cells) + wave * kQueue;
+    const int ch0 = blockIdx.y * kWave * VW, ch = ch0 + lane * VW;
+    const bool in = ch < dim;
+    const int64_t i0 = ((int64_t)blockIdx.x * kWaves + wave) * own;
+    if (i0 >= n) return;
+    const int mine = (int)min((int64_t)own, n - i0);
+    for (int c = lane; c < cells; c += kWave) acc[c] = 0.0f;
+    wave_order();
+    // bits e0 .. e1 of a step, in words w0 .. w0 + nw
+    const int64_t e0 = i0 * batch, e1 = (i0 + mine) * batch, w0 = e0 >> 6;
+    const int nw = (int)(((e1 + 63) >> 6) - w0);
+    const uint64_t first_mask = ~0ull << (e0 & 63), last_mask = (e1 & 63) ? (1ull << (e1 & 63)) - 1 : ~0ull;
+    const T *dcol = dy + ch;
+    unsigned head = 0, tail = 0;
+
+    auto work_off = [&](int m) {
+        const uint64_t q = queue[(head + lane) & (kQueue - 1)];
+        const uint32_t e = (uint32_t)q;
+        const int i = (int)div_by(e, by_batch);
+        const int r = (int)((uint32_t)(q >> 32) * (uint32_t)batch + (e - (uint32_t)i * (uint32_t)batch));
+        for (int k = 0; k < m; k += kRowLoads) {
+            float v[kRowLoads][VW];
+#pragma unroll
+            for (int u = 0; u < kRowLoads; ++u)
+                load_row<T, VW>(dcol + (int64_t)bcast_i(r, min(k + u, m - 1)) * dim, in, v[u]);
+#pragma unroll
+            for (int u = 0; u < kRowLoads; ++u) {
+                if (k + u >= m) break;
+                const int ii = bcast_i(i, k + u);
+#pragma unroll
+                for (int c = 0; c < VW; ++c) lds_add(acc + (ii * VW + c) * kWave + lane, v[u][c]);
+            }
+        }
+        head += m;
+    };
+
+    // (step, word) pairs, the word faster: lane l begins with pair l and goes on by 64
+    int64_t t = lane / nw;
+    int w_at = lane % nw;
+    const int dt = kWave / nw, dw = kWave % nw;
+    while (__ballot(t < n_steps) != 0) {
+        uint64_t w[kWordsPerLane];
+        uint32_t at_t[kWordsPerLane], at_e[kWordsPerLane];
+#pragma unroll
+        for (int k = 0; k < kWordsPerLane; ++k) {
+            w[k] = t < n_steps ? bits[t * stride + w0 + w_at] : 0;
+            if (w_at == 0) w[k] &= first_mask;
+            if (w_at == nw - 1) w[k] &= last_mask;
+            at_t[k] = (uint32_t)t;
+            at_e[k] = (uint32_t)(((w0 + w_at) << 6) - e0);   // (of the first word perhaps below zero: its bits are set from e0 on)
+            t += dt;
+            w_at += dw;
+            if (w_at >= nw) {
+                w_at -= nw;
+                ++t;
+            }
+        }
+#pragma unroll
+        for (int k = 0; k < kWordsPerLane; ++k) {
+            unsigned long long mask;
+            while ((mask = __ballot(w[k] != 0)) != 0) {
+                if (w[k] != 0) {
+                    queue[(tail + lane_prefix(mask)) & (kQueue - 1)] = ((uint64_t)at_t[k] << 32) | (uint32_t)(at_e[k] + (uint32_t)__builtin_ctzll(w[k]));
+                    w[k] &= w[k] - 1;
+                }
+                tail += (unsigned)__popcll(mask);
+                wave_order();
+                if (tail - head >= kWave) {
+                    work_off(kWave);
+                    wave_order();
+                }
+            }
+        }
+    }
+    if (tail != head) work_off((int)(tail - head));
+    wave_order();
+    if (in)
+        for (int i = 0; i < mine; ++i) {
+            Pack<T, VW> q;
+#pragma unroll
+            for (int c = 0; c < VW; ++c) q.v[c] = (T)acc[(i * VW + c) * kWave + lane];
+            *reinterpret_cast<Pack<T, VW> *>(d_weight + (i0 + i) * dim + ch) = q;
+        }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Gradient by the spikes: dl_dz[t, i, b] = dy[t, b] . W[i], a matrix product whose result is most of its traffic.  A wavefront keeps
+// the weights of 64 neurons in registers and multiplies them with the dy rows of 32 (step, trial) pairs at a time.
+// A lane's share of a row is half of it: the order of the channels in the products is free as long as both operands have the same.
+typedef float f32x16 __attribute__((ext_vector_type(16)));
+constexpr int kDzK = 64;          // channels at a time
+constexpr int kDzNeurons = 64;    // of a wavefront
+constexpr int kDzRows = 32;       // (step, trial) pairs at a time
+
+template <typename T, int VL>
+__device__ __forceinline__ void load_half(const T *__restrict__ base, int64_t row, bool there, int dim, int k0, float (&v)[kDzK / 2])
+{
+    const T *p = base + row * dim + k0;
+#pragma unroll
+    for (int s = 0; s < kDzK / 2; s += VL) {
+        Pack<T, VL> q{};
+        if (there && k0 + s < dim) q = *reinterpret_cast<const Pack<T, VL> *>(p + s);
+#pragma unroll
+        for (int c = 0; c < VL; ++c) v[s + c] = (float)q.v[c];
+    }
+}
+
+// kAcross: neighbouring lanes hold neighbouring neurons (one trial); else neighbouring (step, trial) pairs
+template <typename T, int VL, bool kAcross>
+__global__ void __launch_bounds__(kWaves * kWave)
+spike_bwd_spikes_kernel(const T *__restrict__ weight, const T *__restrict__ dy, int64_t rows, int64_t n, FastDiv by_batch, int dim,
+                        int64_t rows_per_block, float *__restrict__ dl_dz)
+{
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
+    const int half = lane / 32, col = lane % 32;
+    const int batch = (int)by_batch.d;
+    const int64_t ne = n * batch;
+    const int64_t i0 = ((int64_t)blockIdx.x * kWaves + wave) * kDzNeurons;
+    if (i0 >= n) return;
+    const int64_t r_end = min(rows, (int64_t)(blockIdx.y + 1) * rows_per_block);
+    float a[2][kDzK / 2];
+    const bool one_pass = dim <= kDzK;
+    if (one_pass)
+#pragma unroll
+        for (int g = 0; g < 2; ++g) load_half<T, VL>(weight, i0 + g * 32 + col, i0 + g * 32 + col < n, dim, half * (kDzK / 2), a[g]);
+    for (int64_t r0 = (int64_t)blockIdx.y * rows_per_block; r0 < r_end; r0 += kDzRows) {
+        f32x16 acc[2] = {};
+        for (int k0 = 0; k0 < dim; k0 += kDzK) {
+            float b[kDzK / 2];
+            load_half<T, VL>(dy, r0 + col, r0 + col < r_end, dim, k0 + half * (kDzK / 2), b);
+            if (!one_pass)
+#pragma unroll
+                for (int g = 0; g < 2; ++g)
+                    load_half<T, VL>(weight, i0 + g * 32 + col, i0 + g * 32 + col < n, dim, k0 + half * (kDzK / 2), a[g]);
+#pragma unroll
+            for (int g = 0; g < 2; ++g)
+#pragma unroll
+                for (int s = 0; s < kDzK / 2; ++s)
+                    acc[g] = kAcross ? __builtin_amdgcn_mfma_f32_32x32x2f32(b[s], a[g][s], acc[g], 0, 0, 0)
+                                     : __builtin_amdgcn_mfma_f32_32x32x2f32(a[g][s], b[s], acc[g], 0, 0, 0);
+        }
+        // register k of a lane: column col, row 8 (k / 4) + 4 half + k % 4
+        if (kAcross) {
+#pragma unroll
+            for (int k = 0; k < 16; ++k) {
+                const int64_t r = r0 + 8 * (k / 4) + 4 * half + k % 4;
+                if (r >= r_end) continue;
+                const uint32_t t = div_by((uint32_t)r, by_batch);
+                float *p = dl_dz + t * ne + (r - (int64_t)t * batch);
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    const int64_t i = i0 + g * 32 + col;
+                    if (i < n) p[i * batch] = acc[g][k];
+                }
+            }
+        } else if (r0 + col < r_end) {
+            const uint32_t t = div_by((uint32_t)(r0 + col), by_batch);
+            float *p = dl_dz + t * ne + (r0 + col - (int64_t)t * batch);
+#pragma unroll
+            for (int g = 0; g < 2; ++g)
+#pragma unroll
+                for (int k = 0; k < 16; ++k) {
+                    const int64_t i = i0 + g * 32 + 8 * (k / 4) + 4 * half + k % 4;
+                    if (i < n) p[i * batch] = acc[g][k];
+                }
+        }
+    }
+}
+
+// channels a lane takes: as many as cover a row, of those that its alignment allows and whose sums have room
+int lane_channels(int dim, int dtype, const void *p, int rows_in_lds)
+{
+    int vw = 1;
+    while (vw < 4 && vw * kWave < dim && dim % (2 * vw) == 0 && aligned(p, 2 * vw * type_size(dtype)) && rows_in_lds * 2 * vw <= kSumRows) vw *= 2;
+    return vw;
+}
+
+// slices of a step's words: enough workgroups to fill the chip, a load of words for every wavefront at least
+int64_t fwd_slices(int64_t n_steps, int64_t words, int tiles)
+{
+    const int64_t most = div_up(words, kWaves * kWave);
+    int64_t s = 1024 / (n_steps * tiles);
+    s = s < 1 ? 1 : s;
+    return s < most ? s : most;
+}
+
+struct FwdPlan {
+    int vw, trials, trial_tiles, tiles;
+    int64_t slices, slice_words;
+};
+FwdPlan fwd_plan(int64_t n_steps, int64_t n, int batch, int dim, int dtype, const void *weight)
+{
+    FwdPlan p;
+    p.trial_tiles = (int)div_up(batch, kSumRows);
+    p.trials = (int)div_up(batch, p.trial_tiles);
+    p.vw = lane_channels(dim, dtype, weight, p.trials);
+    p.tiles = p.trial_tiles * (int)div_up(dim, kWave * p.vw);
+    const int64_t words = (n * batch + 63) / 64;
+    p.slices = fwd_slices(n_steps, words, p.tiles);
+    p.slice_words = div_up(div_up(words, p.slices), kWave) * kWave;
+    p.slices = div_up(words, p.slice_words);
+    return p;
+}
+
+int check_sizes(const char *who, int64_t n_steps, int64_t n, int32_t batch, int32_t dim, int32_t dtype)
+{
+    BMTK_REQUIRE(n_steps > 0 && n > 0 && batch > 0 && dim > 0, "%s: sizes must be positive", who);
+    BMTK_REQUIRE(dtype == BMTK_F32 || dtype == BMTK_BF16 || dtype == BMTK_F16, "%s: unknown type %d", who, dtype);
+    BMTK_REQUIRE(n < (1ll << 31) && n * (int64_t)batch < (1ll << 31) - 64, "%s: n_neurons * batch must stay below 2^31 - 64", who);
+    BMTK_REQUIRE(n_steps < (1ll << 24) && n_steps * (int64_t)batch < (1ll << 31) - 64, "%s: n_steps must stay below 2^24 and n_steps * batch below 2^31 - 64", who);
+    BMTK_REQUIRE(dim <= 65536 && batch <= 65536, "%s: batch and dim are at most 65,536", who);
+    return BMTK_OK;
+}
+
+}  // namespace
+}  // namespace bmtk
+
+using namespace bmtk;
+
+extern "C" int64_t bmtk_spike_readout_workspace_bytes(int64_t n_steps, int64_t n_neurons, int32_t batch, int32_t dim)
+{
+    if (check_sizes("spike_readout_workspace_bytes", n_steps, n_neurons, batch, dim, BMTK_F32) != BMTK_OK) return 0;
+    // (as many slices as any alignment of the weights takes: fewest tiles)
+    const int tiles = (int)(div_up(batch, kSumRows) * div_up(dim, kWave * 4));
+    const int64_t slices = fwd_slices(n_steps, (n_neurons * batch + 63) / 64, tiles);
+    return slices > 1 ? slices * n_steps * batch * dim * (int64_t)sizeof(float) : 0;
+}
+
+extern "C" int bmtk_spike_readout_fwd(const uint64_t *spike_bits, int64_t stride, int64_t n_steps, int64_t n_neurons, int32_t batch, const void *weight,
+                                      int32_t dim, int32_t dtype, void *y, float *workspace, void *stream)
+{
+    BMTK_REQUIRE(spike_bits && weight && y, "spike_readout_fwd: pointers must be non-null");
+    int rc = check_sizes("spike_readout_fwd", n_steps, n_neurons, batch, dim, dtype);
+    if (rc != BMTK_OK) return rc;
+    BMTK_REQUIRE(stride >= (n_neurons * batch + 63) / 64, "spike_readout_fwd: stride is shorter than a step's words");
+    const FwdPlan p = fwd_plan(n_steps, n_neurons, batch, dim, dtype, weight);
+    BMTK_REQUIRE(p.tiles < 65536 && p.slices < 65536, "spike_readout_fwd: too many trials and channels");
+    BMTK_REQUIRE(p.slices == 1 || workspace, "spike_readout_fwd: needs its workspace");
+    float *part = p.slices > 1 ? workspace : nullptr;
+    const int64_t plane = n_steps * batch * (int64_t)dim;
+    BMTK_REQUIRE(plane < (1ll << 31), "spike_readout_fwd: the result is too large");
+    const dim3 grid((unsigned)n_steps, (unsigned)p.slices, (unsigned)p.tiles);
+    const size_t lds = (size_t)kWaves * (p.trials * kWave * p.vw * sizeof(float) + kQueue * sizeof(uint32_t));
+    const hipStream_t st = (hipStream_t)stream;
+    const FastDiv by_batch = fast_div((uint32_t)batch);
+#define BMTK_FWD(VW, ONE)                                                                                                                      \
+    hipLaunchKernelGGL((spike_fwd_kernel<T, VW, ONE>), grid, dim3(kWaves *kWave), lds, st, spike_bits, stride, n_neurons *batch, by_batch, p.trials, \
+                       p.trial_tiles, (const T *)weight, dim, p.slice_words, (T *)y, part)
+    BMTK_BY_TYPE(dtype, T, {
+        if (batch == 1) {
+            if (p.vw == 1) BMTK_FWD(1, true);
+            else if (p.vw == 2) BMTK_FWD(2, true);
+            else BMTK_FWD(4, true);
+        } else {
+            if (p.vw == 1) BMTK_FWD(1, false);
+            else if (p.vw == 2) BMTK_FWD(2, false);
+            else BMTK_FWD(4, false);
+        }
+        if (part)
+            hipLaunchKernelGGL((spike_join_kernel<T>), dim3((unsigned)div_up(plane, kBlock)), dim3(kBlock), 0, st, part, (int)p.slices, plane, (T *)y);
+    });
+#undef BMTK_FWD
+    BMTK_CHECK_LAUNCH("spike_readout_fwd");
+    return BMTK_OK;
+}
+
+extern "C" int bmtk_spike_readout_bwd_weight(const uint64_t *spike_bits, int64_t stride, int64_t n_steps, int64_t n_neurons, int32_t batch, const void *dy,
+                                             int32_t dim, int32_t dtype, void *d_weight, void *stream)
+{
+    BMTK_REQUIRE(spike_bits && dy && d_weight, "spike_readout_bwd_weight: pointers must be non-null");
+    int rc = check_sizes("spike_readout_bwd_weight", n_steps, n_neurons, batch, dim, dtype);
+    if (rc != BMTK_OK) return rc;
+    BMTK_REQUIRE(stride >= (n_neurons * batch + 63) / 64, "spike_readout_bwd_weight: stride is shorter than a step's words");
+    // neurons of a wavefront: 256 bits of a step where there are enough of them to fill the chip
+    int64_t own = div_up(256, batch);
+    if (own > kSumRows) own = kSumRows;
+    const int64_t fill = n_neurons / 2048;
+    if (own > fill) own = fill < 1 ? 1 : fill;
+    int vw = lane_channels(dim, dtype, dy, (int)own);
+    while (vw > 1 && !aligned(d_weight, vw * type_size(dtype))) vw /= 2;
+    const dim3 grid((unsigned)div_up(n_neurons, kWaves * own), (unsigned)div_up(dim, kWave * vw));
+    const size_t lds = (size_t)kWaves * (own * kWave * vw * sizeof(float) + kQueue * sizeof(uint64_t));
+    const hipStream_t st = (hipStream_t)stream;
+    const FastDiv by_batch = fast_div((uint32_t)batch);
+#define BMTK_BWD(VW)                                                                                                                       \
+    hipLaunchKernelGGL((spike_bwd_weight_kernel<T, VW>), grid, dim3(kWaves *kWave), lds, st, spike_bits, stride, n_steps, n_neurons, by_batch, \
+                       (int)own, (const T *)dy, dim, (T *)d_weight)
+    BMTK_BY_TYPE(dtype, T, {
+        if (vw == 1) BMTK_BWD(1);
+        else if (vw == 2) BMTK_BWD(2);
+        else BMTK_BWD(4);
+    });
+#undef BMTK_BWD
+    BMTK_CHECK_LAUNCH("spike_readout_bwd_weight");
+    return BMTK_OK;
+}
+
+extern "C" int bmtk_spike_readout_bwd_spikes(const void *weight, const void *dy, int64_t n_steps, int64_t n_neurons, int32_t batch, int32_t dim, int32_t dtype,
+                                             float *dl_dz, void *stream)
+{
+    BMTK_REQUIRE(weight && dy && dl_dz, "spike_readout_bwd_spikes: pointers must be non-null");
+    int rc = check_sizes("spike_readout_bwd_spikes", n_steps, n_neurons, batch, dim, dtype);
+    if (rc != BMTK_OK) return rc;
+    const int64_t rows = n_steps * batch, across = div_up(n_neurons, kWaves * kDzNeurons);
+    int64_t blocks = div_up(4096, across);
+    const int64_t most = div_up(rows, kDzRows);
+    if (blocks > most) blocks = most;
+    if (blocks > 65535) blocks = 65535;
+    const int64_t per_block = div_up(most, blocks) * kDzRows;
+    const dim3 grid((unsigned)across, (unsigned)div_up(rows, per_block));
+    const bool wide = dim % 4 == 0 && aligned(weight, 4 * type_size(dtype)) && aligned(dy, 4 * type_size(dtype));
+    const hipStream_t st = (hipStream_t)stream;
+    const FastDiv by_batch = fast_div((uint32_t)batch);
+#define BMTK_DZ(VL, ACROSS)                                                                                                                       \
+    hipLaunchKernelGGL((spike_bwd_spikes_kernel<T, VL, ACROSS>), grid, dim3(kWaves *kWave), 0, st, (const T *)weight, (const T *)dy, rows, n_neurons, \
+                       by_batch, dim, per_block, dl_dz)
+    BMTK_BY_TYPE(dtype, T, {
+        if (wide) {
+            if (batch == 1) BMTK_DZ(4, true);
+            else BMTK_DZ(4, false);
+        } else {
+            if (batch == 1) BMTK_DZ(1, true);
+            else BMTK_DZ(1, false);
+        }
+    });
+#undef BMTK_DZ
+    BMTK_CHECK_LAUNCH("spike_readout_bwd_spikes");
+    return BMTK_OK;
+}

@@ -10,7 +10,7 @@ import ctypes as C
 import numpy as np
 import torch
 
-from . import _lib
+from . import _lib, readout
 from .layout import NASC, NREC
 from .ops import _p, _stream
 
@@ -69,6 +69,28 @@ def rate_mse(counts, n_steps, batch, pop_id, targets):
     # d loss / d z[b, i, t] = 2 err[b, p(i)] / (batch * n_pops) / (size[p(i)] * n_steps)
     g = 2.0 * err / (batch * n_pops) / (size.view(1, -1) * n_steps)
     return loss, g.t()[pop_id].contiguous().view(-1)
+
+
+def label_loss(bits, batch, weight, decay, labels, ignore=-100, state=None, top=0):
+    """Cross entropy of the labels that a trained readout should answer, and its derivatives.
+
+    bits    int64 [steps, words] spike bits of a run of ``batch`` trials (``fwd["bits"]``)
+    weight  [neurons, classes], decay float32 [classes]: the readout, y = sum of the weight rows of what fired, h[t] = decay * h[t - 1] + y[t]; the
+            classes' probabilities in every step are the softmax of h (``readout.spike_readout``, ``gated_scan``, ``token_logprobs``)
+    labels  int64 [steps, batch]: the class wanted in each step and trial, ``ignore`` where none is
+    state   float32 [batch, classes]: h before the first step (None: zero)
+    Returns (loss, dl_dz, gradients, answer): the mean of -log p(label) over the steps and trials that have one; dl_dz float32
+    [steps, neurons * batch], what ``Glif3Bptt.backward`` takes; a dict of the gradients by "weight", "decay" and "state"; and
+    the ``readout.LogProbs`` of every step and trial with its ``top`` most probable classes.  Nothing synchronises."""
+    y = readout.spike_readout(bits, weight, batch)
+    h, _, saved = readout.gated_scan(y, decay, state, save_state=True)
+    answer = readout.token_logprobs(h, labels, top=top, ignore=ignore)
+    share = 1.0 / (labels != ignore).sum().clamp_(min=1).to(torch.float32)
+    loss = -answer.logp.sum() * share
+    dh = readout.token_logprobs_bwd(h, labels, answer, d_logp=(-share).expand(labels.shape).contiguous(), ignore=ignore, out=h)
+    dy, d_decay, d_state = readout.gated_scan_bwd(y, decay, saved, dh)
+    d_weight, dl_dz = readout.spike_readout_bwd(bits, weight, dy, batch)
+    return loss, dl_dz, {"weight": d_weight, "decay": d_decay, "state": d_state}, answer
 
 
 class Glif3Bptt:

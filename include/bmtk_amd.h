@@ -49,7 +49,7 @@ extern "C" {
 
 /* Bumped whenever a struct layout or a signature below changes; bmtk_amd_abi_version() returns the value the
  * library was built with. */
-#define BMTK_AMD_ABI_VERSION 37
+#define BMTK_AMD_ABI_VERSION 38
 int bmtk_amd_abi_version(void);
 const char *bmtk_amd_last_error(void);
 /* sizeof(bmtk_glif3_sim) as the library was compiled, for bindings that mirror the struct */
@@ -696,6 +696,63 @@ int bmtk_spike_counts(const uint64_t *spike_bits, int64_t stride, int64_t n_step
  * n_pops + 1 words, zero; the last is 1 afterwards if some pop_id lies outside 0 .. n_pops - 1 (such neurons are left out). */
 int bmtk_rate_mse(const int32_t *counts, int64_t n_neurons, int32_t batch, int64_t n_steps, const int64_t *pop_id, int64_t n_pops,
                   const float *targets, int64_t *work, float *loss, float *per_spike, void *stream);
+
+/* ---------------------------------------------------------------------------
+ * A readout that is trained on what it answers: spikes -> sums of weight rows -> a memory over steps -> log probabilities, each with its
+ * gradient, down to the dl_dz of bmtk_glif3_bwd.  No counterpart in the reference (bmtk has no gradients).
+ *
+ * dtype: the type of the values that are read and written, BMTK_F32, BMTK_BF16 or BMTK_F16; all arithmetic is in 32 bits, and a value of a
+ * 16-bit type is rounded once, when it is written.  The workspaces need not be cleared, hold nothing between calls, and belong to a call
+ * until its work is done.  Sums are made in an order that only the sizes and alignments decide: the same call gives the same bits. */
+#define BMTK_F32 0
+#define BMTK_BF16 1
+#define BMTK_F16 2
+
+/* y[t][b][:] = sum of weight[i][:] over the neurons i that fired in step t of trial b.  spike_bits: n_steps rows of `stride` words (bits
+ * behind n_neurons * batch are not looked at); weight [n_neurons][dim], y [n_steps][batch][dim], contiguous.
+ * Limits: n_neurons * batch < 2^31 - 64, n_steps < 2^24, n_steps * batch < 2^31 - 64, n_steps * batch * dim < 2^31, batch and dim up to 65,536. */
+int64_t bmtk_spike_readout_workspace_bytes(int64_t n_steps, int64_t n_neurons, int32_t batch, int32_t dim);
+int bmtk_spike_readout_fwd(const uint64_t *spike_bits, int64_t stride, int64_t n_steps, int64_t n_neurons, int32_t batch, const void *weight, int32_t dim,
+                           int32_t dtype, void *y, float *workspace, void *stream);
+/* d_weight[i][:] = sum of dy[t][b][:] over the spikes of neuron i (all rows are written) */
+int bmtk_spike_readout_bwd_weight(const uint64_t *spike_bits, int64_t stride, int64_t n_steps, int64_t n_neurons, int32_t batch, const void *dy, int32_t dim,
+                                  int32_t dtype, void *d_weight, void *stream);
+/* dl_dz[t][i * batch + b] = dy[t][b][:] . weight[i][:], in 32 bits: what bmtk_glif3_bwd takes */
+int bmtk_spike_readout_bwd_spikes(const void *weight, const void *dy, int64_t n_steps, int64_t n_neurons, int32_t batch, int32_t dim, int32_t dtype,
+                                  float *dl_dz, void *stream);
+
+/* h[t][b][c] = a h[t-1][b][c] + x[t][b][c] for the steps t < lengths[b] (NULL: all n_steps), from state [batch][dim] (NULL: zero); h is 0 behind
+ * a sequence's end and nothing of x or decay is read there.  last [batch][dim]: the state behind each sequence's last step.
+ * groups: 0: one decay per channel, decay [dim]; else decays per step and sequence, [n_steps][batch][groups], each for dim / groups neighbouring
+ * channels.  gate_dtype: the decays' type, BMTK_F32 or dtype.  x_t, x_b, a_t, a_b, dh_t, dh_b: distance of steps and of sequences in x, decay
+ * and dh, in elements (a channel's neighbour is next to it); h, dx and d_decay are contiguous.  state, last, d_last, d_state, marks: 32 bits.
+ * marks (NULL: not kept): the state before every BMTK_SCAN_MARK-th step, [ceil(n_steps / BMTK_SCAN_MARK)][batch][dim], from which the backward
+ * pass computes the others again.  Decays of up to 1 in magnitude, or of which the products over a sequence stay in 32 bits.
+ * Limits: batch * dim < 2^31, n_steps < 2^31 - 4096. */
+#define BMTK_SCAN_MARK 16
+int64_t bmtk_gated_scan_workspace_bytes(int64_t n_steps, int64_t batch, int32_t dim, int32_t groups, int32_t backward);
+int bmtk_gated_scan_fwd(int64_t n_steps, int64_t batch, int32_t dim, int32_t groups, int32_t dtype, int32_t gate_dtype, const void *x, int64_t x_t,
+                        int64_t x_b, const void *decay, int64_t a_t, int64_t a_b, const float *state, const int32_t *lengths, void *h, float *last,
+                        float *marks, float *workspace, void *stream);
+/* dh, d_last (NULL: zero): gradients of h and last; dx, d_decay, d_state (NULL: not wanted): of x, decay and state */
+int bmtk_gated_scan_bwd(int64_t n_steps, int64_t batch, int32_t dim, int32_t groups, int32_t dtype, int32_t gate_dtype, const void *x, int64_t x_t,
+                        int64_t x_b, const void *decay, int64_t a_t, int64_t a_b, const float *marks, const int32_t *lengths, const void *dh, int64_t dh_t,
+                        int64_t dh_b, const float *d_last, void *dx, void *d_decay, float *d_state, float *workspace, void *stream);
+
+/* Of each of `rows` rows of logits (rows row_stride elements apart): lse = log of the sum of e^logit, logp = logit of its token - lse (0 where the
+ * token is `ignore`, NaN where it lies outside 0 .. vocab - 1), entropy = -sum p log p, and the `top` most probable alternatives, the lower
+ * index first of equal ones: top_logp, top_index [rows][top] (NULL for top 0).  Logits of -inf have no probability; of a row of nothing else
+ * lse is -inf, the entropy 0; of a row with NaN or +inf lse, logp, entropy and top_logp are NaN (NaN comes first among the alternatives).
+ * Limits: rows < 2^24, vocab < 2^30, top up to BMTK_LOGPROBS_MAX_TOP and vocab. */
+#define BMTK_LOGPROBS_MAX_TOP 64
+int64_t bmtk_token_logprobs_workspace_bytes(int64_t rows, int32_t vocab, int32_t dtype, int32_t top);
+int bmtk_token_logprobs_fwd(int64_t rows, int32_t vocab, int32_t dtype, const void *logits, int64_t row_stride, const int64_t *tokens, int64_t ignore,
+                            int32_t top, float *logp, float *entropy, float *lse, float *top_logp, int64_t *top_index, void *workspace, void *stream);
+/* d_logits = d_logp (delta - p) - d_entropy p (log p + entropy), row by row; d_logp or d_entropy may be NULL.  lse and entropy are the forward
+ * pass's.  d_logits may be the logits themselves, with the same distance of rows, or share nothing with them. */
+int bmtk_token_logprobs_bwd(int64_t rows, int32_t vocab, int32_t dtype, const void *logits, int64_t row_stride, const int64_t *tokens, int64_t ignore,
+                            const float *lse, const float *entropy, const float *d_logp, const float *d_entropy, void *d_logits, int64_t out_stride,
+                            void *stream);
 
 /* ---------------------------------------------------------------------------
  * Three measurements the kernels' design rests on, kept in the library so that they can be repeated
