@@ -5,10 +5,11 @@ namespace bmtk {
 namespace {
 
 constexpr int kWaves = 4;
-constexpr int kQueue = 128;       // spikes found and not yet added: at most 63 left over and 64 new ones
+constexpr int kFwdWaves = 8;
 constexpr int kWordsPerLane = 4;  // spike words that a lane has under way at once
-constexpr int kRowLoads = 8;      // rows under way at once
-constexpr int kSumRows = 60;      // rows of 64 sums of a wavefront, in LDS: four wavefronts' and their queues are 64 KB
+constexpr int kQueue = 512;       // spikes found and not yet added: at most 63 left over and one of each word under way
+static_assert(kQueue >= kWave * (kWordsPerLane + 1) && (kQueue & (kQueue - 1)) == 0, "room for what a round finds");
+constexpr int kSums = 32;         // sums of a lane, in registers
 
 // A wavefront's own queue is written and read by different lanes of it, in order: what the compiler must keep is that order.
 __device__ __forceinline__ void wave_order()
@@ -17,116 +18,147 @@ __device__ __forceinline__ void wave_order()
     __builtin_amdgcn_wave_barrier();
 }
 
-__device__ __forceinline__ void lds_add(float *p, float v)
-{
-    __hip_atomic_fetch_add(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_WORKGROUP);
-}
-
-template <typename T, int VW>
-__device__ __forceinline__ void load_row(const T *p, bool in, float (&v)[VW])
-{
-    Pack<T, VW> q{};
-    if (in) q = *reinterpret_cast<const Pack<T, VW> *>(p);
+// Sums of a lane, VW channels of each of N trials or neurons.  Which of them a spike adds to is the same for all lanes, so that they stay in registers and
+// are picked by number (an LDS addition of 64 floats takes 194 clocks on this chip, these seven instructions a tenth of it).
+template <int VW, int N>
+struct Accumulators {
+    typedef float Vec __attribute__((ext_vector_type(N)));
+    Vec sum[VW];
+    __device__ __forceinline__ void clear()
+    {
 #pragma unroll
-    for (int c = 0; c < VW; ++c) v[c] = (float)q.v[c];
+        for (int c = 0; c < VW; ++c) sum[c] = 0.0f;
+    }
+    __device__ __forceinline__ void add(int which, const float (&v)[VW])
+    {
+#pragma unroll
+        for (int c = 0; c < VW; ++c) sum[c][N == 1 ? 0 : which] += v[c];
+    }
+    __device__ __forceinline__ float get(int c, int which) const { return sum[c][N == 1 ? 0 : which]; }
+};
+
+// Adds the rows of m of a queue's spikes: row of lane k's spike to the sums of lane k's `which`.  Rows are asked for sixteen (of
+// four channels a lane: eight) at a time; `at` is where the lane's channels begin, within a row.
+template <typename T, int VW, int N>
+__device__ __forceinline__ void add_rows(Accumulators<VW, N> &acc, const T *__restrict__ rows, int dim, unsigned at, int row, int which, int m)
+{
+    constexpr int kLoads = VW == 4 ? 8 : 16;
+    for (int k = 0; k < m; k += kLoads) {
+        Pack<T, VW> q[kLoads];
+#pragma unroll
+        for (int u = 0; u < kLoads; ++u) {
+            const T *p = rows + (int64_t)bcast_i(row, min(k + u, m - 1)) * dim;
+            q[u] = *reinterpret_cast<const Pack<T, VW> *>(p + at);
+        }
+#pragma unroll
+        for (int u = 0; u < kLoads; ++u) {
+            if (k + u < m) {
+                float v[VW];
+#pragma unroll
+                for (int c = 0; c < VW; ++c) v[c] = (float)q[u].v[c];
+                acc.add(N == 1 ? 0 : bcast_i(which, k + u), v);
+            }
+        }
+    }
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
 // Forward.  A workgroup takes one step and a slice of its words of spike bits; a wavefront turns the set bits of 256 words at a
 // time into a queue of element numbers, works it off 64 spikes at a time (each lane divides one of them into neuron and trial),
-// and reads the weight rows, one per spike, 64 * VW channels by its 64 lanes.  The sums of a trial are the wavefront's own (in LDS, or
-// in registers for one trial), so their order is fixed; the wavefronts' sums are added in order at the end.
-template <typename T, int VW, bool kOne>
-__global__ void __launch_bounds__(kWaves * kWave)
+// and reads the weight rows, one per spike, 64 * VW channels by its 64 lanes.  The sums of a trial are the wavefront's own, so their
+// order is fixed; the wavefronts' sums are added in order at the end.
+template <typename T, int VW, int N>
+__global__ void __launch_bounds__(kFwdWaves * kWave)
 spike_fwd_kernel(const uint64_t *__restrict__ bits, int64_t stride, int64_t ne, FastDiv by_batch, int trials, int trial_tiles,
                  const T *__restrict__ weight, int dim, int64_t slice_words, T *__restrict__ y, float *__restrict__ part)
 {
     extern __shared__ float lds[];
+    __shared__ uint32_t queues[kFwdWaves][kQueue];
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
     const int64_t t = blockIdx.x;
     const int batch = (int)by_batch.d;
     const int b0 = (int)(blockIdx.z % trial_tiles) * trials, ch0 = (int)(blockIdx.z / trial_tiles) * kWave * VW;
     const int cells = trials * kWave * VW;
-    float *acc = lds + wave * cells;
-    uint32_t *queue = reinterpret_cast<uint32_t *>(lds + kWaves * cells) + wave * kQueue;
-    const int ch = ch0 + lane * VW;
-    const bool in = ch < dim;
-    float one[VW] = {};
-    if (!kOne)
-        for (int c = lane; c < cells; c += kWave) acc[c] = 0.0f;
+    uint32_t *queue = queues[wave];
+    // (a lane without channels of its own reads the first ones and writes nothing)
+    const unsigned at_ch = ch0 + lane * VW < dim ? ch0 + lane * VW : 0;
+    Accumulators<VW, N> acc;
+    acc.clear();
     const int64_t words = (ne + 63) >> 6;
-    const int64_t w_end = min(words, (int64_t)(blockIdx.y + 1) * slice_words);
-    const uint64_t *row = bits + t * stride;
-    const T *wcol = weight + ch;
+    const int64_t w_begin = (int64_t)blockIdx.y * slice_words;
+    const int w_count = (int)min(slice_words, words - w_begin);
+    const uint64_t *row = bits + t * stride + w_begin;
+    const uint64_t last_mask = (ne & 63) ? (1ull << (ne & 63)) - 1 : ~0ull;
+    const int last_word = (int)min(words - 1 - w_begin, (int64_t)INT32_MAX);
+    const uint32_t first_element = (uint32_t)(w_begin << 6);
     unsigned head = 0, tail = 0;
 
-    auto work_off = [&](int m) {
-        const uint32_t e = queue[(head + lane) & (kQueue - 1)];
-        const int i = (int)div_by(e, by_batch);
-        const int b = (int)e - i * batch - b0;
-        for (int k = 0; k < m; k += kRowLoads) {
-            float v[kRowLoads][VW];
+    auto load = [&](int c, uint64_t (&w)[kWordsPerLane]) {
 #pragma unroll
-            for (int u = 0; u < kRowLoads; ++u)
-                load_row<T, VW>(wcol + (int64_t)bcast_i(i, min(k + u, m - 1)) * dim, in, v[u]);
-#pragma unroll
-            for (int u = 0; u < kRowLoads; ++u) {
-                if (k + u >= m) break;
-                if (kOne) {
-#pragma unroll
-                    for (int c = 0; c < VW; ++c) one[c] += v[u][c];
-                } else {
-                    const int bb = bcast_i(b, k + u);
-                    if ((unsigned)bb < (unsigned)trials)
-#pragma unroll
-                        for (int c = 0; c < VW; ++c) lds_add(acc + (bb * VW + c) * kWave + lane, v[u][c]);
-                }
-            }
-        }
-        head += m;
+        for (int k = 0; k < kWordsPerLane; ++k) w[k] = row[min(c + k * kWave + lane, w_count - 1)];
     };
 
-    for (int64_t c = (int64_t)blockIdx.y * slice_words + wave * (kWave * kWordsPerLane); c < w_end; c += kWaves * kWave * kWordsPerLane) {
-        uint64_t w[kWordsPerLane];
+    constexpr int kStep = kWave * kWordsPerLane;
+    uint64_t w[kWordsPerLane] = {}, next[kWordsPerLane];
+    uint32_t first = 0;
+    int c = wave * kStep;
+    load(c, next);
+    for (;;) {
+        bool more = true;
+        while (tail - head < kWave) {
+            uint64_t any = 0;
 #pragma unroll
-        for (int k = 0; k < kWordsPerLane; ++k) {
-            const int64_t at = c + k * kWave + lane;
-            w[k] = at < w_end ? row[at] : 0;
-            if (at == words - 1 && (ne & 63)) w[k] &= (1ull << (ne & 63)) - 1;
-        }
+            for (int k = 0; k < kWordsPerLane; ++k) any |= w[k];
+            if (__ballot(any != 0) == 0) {
+                more = c < w_count;
+                if (!more) break;
 #pragma unroll
-        for (int k = 0; k < kWordsPerLane; ++k) {
-            const uint32_t first = (uint32_t)((c + k * kWave + lane) << 6);
-            unsigned long long mask;
-            while ((mask = __ballot(w[k] != 0)) != 0) {
-                if (w[k] != 0) {
-                    queue[(tail + lane_prefix(mask)) & (kQueue - 1)] = first + (uint32_t)__builtin_ctzll(w[k]);
-                    w[k] &= w[k] - 1;
+                for (int k = 0; k < kWordsPerLane; ++k) {
+                    const int at = c + k * kWave + lane;
+                    w[k] = at < w_count ? next[k] & (at == last_word ? last_mask : ~0ull) : 0;
                 }
+                first = first_element + (uint32_t)((c + lane) << 6);
+                c += kFwdWaves * kStep;
+                load(c, next);
+            }
+            // one spike of every word
+#pragma unroll
+            for (int k = 0; k < kWordsPerLane; ++k) {
+                const uint32_t e = first + (uint32_t)(k * kWave * 64) + (uint32_t)__builtin_ctzll(w[k]);
+                bool mine = w[k] != 0;
+                if (trial_tiles > 1) mine = mine && (unsigned)((int)(e - div_by(e, by_batch) * (uint32_t)batch) - b0) < (unsigned)trials;
+                w[k] &= w[k] - 1;
+                const unsigned long long mask = __ballot(mine);
+                if (mine) queue[(tail + lane_prefix(mask)) & (kQueue - 1)] = e;
                 tail += (unsigned)__popcll(mask);
-                wave_order();
-                if (tail - head >= kWave) {
-                    work_off(kWave);
-                    wave_order();
-                }
             }
         }
+        wave_order();
+        const int m = (int)min(tail - head, (unsigned)kWave);
+        if (m > 0) {
+            const uint32_t e = queue[(head + lane) & (kQueue - 1)];
+            const int i = (int)div_by(e, by_batch);
+            add_rows<T, VW, N>(acc, weight, dim, at_ch, i, (int)e - i * batch - b0, m);
+            head += m;
+        }
+        wave_order();
+        if (!more && tail == head) break;
     }
-    if (tail != head) work_off((int)(tail - head));
-    if (kOne)
+    float *mine = lds + wave * cells;
+    for (int b = 0; b < trials; ++b)
 #pragma unroll
-        for (int c = 0; c < VW; ++c) acc[c * kWave + lane] = one[c];
+        for (int c = 0; c < VW; ++c) mine[(b * VW + c) * kWave + lane] = acc.get(c, b);
     __syncthreads();
     const int here = min(trials, batch - b0);
     const int64_t out = (t * batch + b0) * (int64_t)dim + ch0;
     const int64_t plane = (int64_t)gridDim.x * batch * dim;
-    for (int c = threadIdx.x; c < here * kWave * VW; c += kWaves * kWave) {
+    for (int c = threadIdx.x; c < here * kWave * VW; c += kFwdWaves * kWave) {
         const int l = c % (kWave * VW), b = c / (kWave * VW);
         if (ch0 + l >= dim) continue;
         const float *a = lds + (b * VW + l % VW) * kWave + l / VW;
         float s = 0.0f;
 #pragma unroll
-        for (int k = 0; k < kWaves; ++k) s += a[k * cells];
+        for (int k = 0; k < kFwdWaves; ++k) s += a[k * cells];
         if (part)
             part[blockIdx.y * plane + out + (int64_t)b * dim + l] = s;
         else
@@ -146,68 +178,44 @@ __global__ void __launch_bounds__(kBlock) spike_join_kernel(const float *__restr
 
 // ---------------------------------------------------------------------------------------------------------------------
 // Gradient by the weights: row i is the sum of dy[t, b] over the spikes of neuron i.  A wavefront owns `own` neurons and their
-// sums (in LDS), looks through their bits of all steps and reads the dy rows as the forward pass reads the weights.  Nobody else
+// sums, looks through their bits of all steps and reads the dy rows as the forward pass reads the weights.  Nobody else
 // adds to its sums: the order is fixed and nothing has to be joined.
-template <typename T, int VW>
+template <typename T, int VW, int N>
 __global__ void __launch_bounds__(kWaves * kWave)
 spike_bwd_weight_kernel(const uint64_t *__restrict__ bits, int64_t stride, int64_t n_steps, int64_t n, FastDiv by_batch, int own,
                         const T *__restrict__ dy, int dim, T *__restrict__ d_weight)
 {
-    extern __shared__ float lds[];
+    __shared__ uint64_t queues[kWaves][kQueue];
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
     const int batch = (int)by_batch.d;
-    const int cells = own * kWave * VW;
-    float *acc = lds + wave * cells;
-    uint64_t *queue = reinterpret_cast<uint64_t *>(lds + kWaves * cells) + wave * kQueue;
-    const int ch0 = blockIdx.y * kWave * VW, ch = ch0 + lane * VW;
+    uint64_t *queue = queues[wave];
+    const int ch = blockIdx.y * kWave * VW + lane * VW;
     const bool in = ch < dim;
+    const unsigned at_ch = in ? ch : 0;
     const int64_t i0 = ((int64_t)blockIdx.x * kWaves + wave) * own;
     if (i0 >= n) return;
     const int mine = (int)min((int64_t)own, n - i0);
-    for (int c = lane; c < cells; c += kWave) acc[c] = 0.0f;
-    wave_order();
+    Accumulators<VW, N> acc;
+    acc.clear();
     // bits e0 .. e1 of a step, in words w0 .. w0 + nw
     const int64_t e0 = i0 * batch, e1 = (i0 + mine) * batch, w0 = e0 >> 6;
     const int nw = (int)(((e1 + 63) >> 6) - w0);
     const uint64_t first_mask = ~0ull << (e0 & 63), last_mask = (e1 & 63) ? (1ull << (e1 & 63)) - 1 : ~0ull;
-    const T *dcol = dy + ch;
+    const uint64_t *own_bits = bits + w0;
+    const uint32_t first_element = (uint32_t)((w0 << 6) - e0);   // (perhaps below zero: the first word's bits are looked at from e0 on)
     unsigned head = 0, tail = 0;
 
-    auto work_off = [&](int m) {
-        const uint64_t q = queue[(head + lane) & (kQueue - 1)];
-        const uint32_t e = (uint32_t)q;
-        const int i = (int)div_by(e, by_batch);
-        const int r = (int)((uint32_t)(q >> 32) * (uint32_t)batch + (e - (uint32_t)i * (uint32_t)batch));
-        for (int k = 0; k < m; k += kRowLoads) {
-            float v[kRowLoads][VW];
-#pragma unroll
-            for (int u = 0; u < kRowLoads; ++u)
-                load_row<T, VW>(dcol + (int64_t)bcast_i(r, min(k + u, m - 1)) * dim, in, v[u]);
-#pragma unroll
-            for (int u = 0; u < kRowLoads; ++u) {
-                if (k + u >= m) break;
-                const int ii = bcast_i(i, k + u);
-#pragma unroll
-                for (int c = 0; c < VW; ++c) lds_add(acc + (ii * VW + c) * kWave + lane, v[u][c]);
-            }
-        }
-        head += m;
-    };
-
     // (step, word) pairs, the word faster: lane l begins with pair l and goes on by 64
-    int64_t t = lane / nw;
-    int w_at = lane % nw;
-    const int dt = kWave / nw, dw = kWave % nw;
-    while (__ballot(t < n_steps) != 0) {
-        uint64_t w[kWordsPerLane];
-        uint32_t at_t[kWordsPerLane], at_e[kWordsPerLane];
+    int t = lane / nw, w_at = lane % nw;
+    const int dt = kWave / nw, dw = kWave % nw, steps = (int)n_steps;
+    uint64_t next[kWordsPerLane];
+    uint32_t next_t[kWordsPerLane], next_w[kWordsPerLane];
+    auto load = [&] {
 #pragma unroll
         for (int k = 0; k < kWordsPerLane; ++k) {
-            w[k] = t < n_steps ? bits[t * stride + w0 + w_at] : 0;
-            if (w_at == 0) w[k] &= first_mask;
-            if (w_at == nw - 1) w[k] &= last_mask;
-            at_t[k] = (uint32_t)t;
-            at_e[k] = (uint32_t)(((w0 + w_at) << 6) - e0);   // (of the first word perhaps below zero: its bits are set from e0 on)
+            next[k] = own_bits[min(t, steps - 1) * stride + w_at];
+            next_t[k] = (uint32_t)t;
+            next_w[k] = (uint32_t)w_at;
             t += dt;
             w_at += dw;
             if (w_at >= nw) {
@@ -215,30 +223,54 @@ spike_bwd_weight_kernel(const uint64_t *__restrict__ bits, int64_t stride, int64
                 ++t;
             }
         }
+    };
+    load();
+    uint64_t w[kWordsPerLane] = {};
+    uint32_t at_t[kWordsPerLane] = {}, at_e[kWordsPerLane] = {};
+    for (;;) {
+        bool more = true;
+        while (tail - head < kWave) {
+            uint64_t any = 0;
 #pragma unroll
-        for (int k = 0; k < kWordsPerLane; ++k) {
-            unsigned long long mask;
-            while ((mask = __ballot(w[k] != 0)) != 0) {
-                if (w[k] != 0) {
-                    queue[(tail + lane_prefix(mask)) & (kQueue - 1)] = ((uint64_t)at_t[k] << 32) | (uint32_t)(at_e[k] + (uint32_t)__builtin_ctzll(w[k]));
-                    w[k] &= w[k] - 1;
+            for (int k = 0; k < kWordsPerLane; ++k) any |= w[k];
+            if (__ballot(any != 0) == 0) {
+                more = __ballot((int)next_t[0] < steps) != 0;
+                if (!more) break;
+#pragma unroll
+                for (int k = 0; k < kWordsPerLane; ++k) {
+                    w[k] = (int)next_t[k] < steps ? next[k] : 0;
+                    if (next_w[k] == 0) w[k] &= first_mask;
+                    if ((int)next_w[k] == nw - 1) w[k] &= last_mask;
+                    at_t[k] = next_t[k];
+                    at_e[k] = first_element + (next_w[k] << 6);
                 }
+                load();
+            }
+#pragma unroll
+            for (int k = 0; k < kWordsPerLane; ++k) {
+                const unsigned long long mask = __ballot(w[k] != 0);
+                if (w[k] != 0) queue[(tail + lane_prefix(mask)) & (kQueue - 1)] = ((uint64_t)at_t[k] << 32) | (uint32_t)(at_e[k] + (uint32_t)__builtin_ctzll(w[k]));
+                w[k] &= w[k] - 1;
                 tail += (unsigned)__popcll(mask);
-                wave_order();
-                if (tail - head >= kWave) {
-                    work_off(kWave);
-                    wave_order();
-                }
             }
         }
+        wave_order();
+        const int m = (int)min(tail - head, (unsigned)kWave);
+        if (m > 0) {
+            const uint64_t q = queue[(head + lane) & (kQueue - 1)];
+            const uint32_t e = (uint32_t)q;
+            const int i = (int)div_by(e, by_batch);
+            add_rows<T, VW, N>(acc, dy, dim, at_ch, (int)((uint32_t)(q >> 32) * (uint32_t)batch + (e - (uint32_t)i * (uint32_t)batch)), i, m);
+            head += m;
+        }
+        wave_order();
+        if (!more && tail == head) break;
     }
-    if (tail != head) work_off((int)(tail - head));
-    wave_order();
     if (in)
         for (int i = 0; i < mine; ++i) {
             Pack<T, VW> q;
 #pragma unroll
-            for (int c = 0; c < VW; ++c) q.v[c] = (T)acc[(i * VW + c) * kWave + lane];
+            for (int c = 0; c < VW; ++c) q.v[c] = (T)acc.get(c, i);
             *reinterpret_cast<Pack<T, VW> *>(d_weight + (i0 + i) * dim + ch) = q;
         }
 }
@@ -327,19 +359,19 @@ spike_bwd_spikes_kernel(const T *__restrict__ weight, const T *__restrict__ dy, 
     }
 }
 
-// channels a lane takes: as many as cover a row, of those that its alignment allows and whose sums have room
-int lane_channels(int dim, int dtype, const void *p, int rows_in_lds)
+// channels a lane takes: as many as cover a row, of those that its alignment allows
+int lane_channels(int dim, int dtype, const void *p)
 {
     int vw = 1;
-    while (vw < 4 && vw * kWave < dim && dim % (2 * vw) == 0 && aligned(p, 2 * vw * type_size(dtype)) && rows_in_lds * 2 * vw <= kSumRows) vw *= 2;
+    while (vw < 4 && vw * kWave < dim && dim % (2 * vw) == 0 && aligned(p, 2 * vw * type_size(dtype))) vw *= 2;
     return vw;
 }
 
 // slices of a step's words: enough workgroups to fill the chip, a load of words for every wavefront at least
-int64_t fwd_slices(int64_t n_steps, int64_t words, int tiles)
+int64_t fwd_slices(int64_t n_steps, int64_t words, int64_t tiles)
 {
-    const int64_t most = div_up(words, kWaves * kWave);
-    int64_t s = 1024 / (n_steps * tiles);
+    const int64_t most = div_up(words, kFwdWaves * kWave);
+    int64_t s = 512 / (n_steps * tiles);
     s = s < 1 ? 1 : s;
     return s < most ? s : most;
 }
@@ -348,13 +380,13 @@ struct FwdPlan {
     int vw, trials, trial_tiles, tiles;
     int64_t slices, slice_words;
 };
-FwdPlan fwd_plan(int64_t n_steps, int64_t n, int batch, int dim, int dtype, const void *weight)
+FwdPlan fwd_plan(int64_t n_steps, int64_t n, int batch, int dim, int vw)
 {
     FwdPlan p;
-    p.trial_tiles = (int)div_up(batch, kSumRows);
+    p.vw = vw;
+    p.trial_tiles = (int)div_up(batch, kSums / vw);
     p.trials = (int)div_up(batch, p.trial_tiles);
-    p.vw = lane_channels(dim, dtype, weight, p.trials);
-    p.tiles = p.trial_tiles * (int)div_up(dim, kWave * p.vw);
+    p.tiles = p.trial_tiles * (int)div_up(dim, kWave * vw);
     const int64_t words = (n * batch + 63) / 64;
     p.slices = fwd_slices(n_steps, words, p.tiles);
     p.slice_words = div_up(div_up(words, p.slices), kWave) * kWave;
@@ -380,9 +412,11 @@ using namespace bmtk;
 extern "C" int64_t bmtk_spike_readout_workspace_bytes(int64_t n_steps, int64_t n_neurons, int32_t batch, int32_t dim)
 {
     if (check_sizes("spike_readout_workspace_bytes", n_steps, n_neurons, batch, dim, BMTK_F32) != BMTK_OK) return 0;
-    // (as many slices as any alignment of the weights takes: fewest tiles)
-    const int tiles = (int)(div_up(batch, kSumRows) * div_up(dim, kWave * 4));
-    const int64_t slices = fwd_slices(n_steps, (n_neurons * batch + 63) / 64, tiles);
+    int64_t slices = 1;   // (as many as any alignment of the weights takes)
+    for (int vw = 1; vw <= 4; vw *= 2) {
+        const FwdPlan p = fwd_plan(n_steps, n_neurons, batch, dim, vw);
+        slices = p.slices > slices ? p.slices : slices;
+    }
     return slices > 1 ? slices * n_steps * batch * dim * (int64_t)sizeof(float) : 0;
 }
 
@@ -393,28 +427,28 @@ extern "C" int bmtk_spike_readout_fwd(const uint64_t *spike_bits, int64_t stride
     int rc = check_sizes("spike_readout_fwd", n_steps, n_neurons, batch, dim, dtype);
     if (rc != BMTK_OK) return rc;
     BMTK_REQUIRE(stride >= (n_neurons * batch + 63) / 64, "spike_readout_fwd: stride is shorter than a step's words");
-    const FwdPlan p = fwd_plan(n_steps, n_neurons, batch, dim, dtype, weight);
+    const FwdPlan p = fwd_plan(n_steps, n_neurons, batch, dim, lane_channels(dim, dtype, weight));
     BMTK_REQUIRE(p.tiles < 65536 && p.slices < 65536, "spike_readout_fwd: too many trials and channels");
     BMTK_REQUIRE(p.slices == 1 || workspace, "spike_readout_fwd: needs its workspace");
     float *part = p.slices > 1 ? workspace : nullptr;
     const int64_t plane = n_steps * batch * (int64_t)dim;
     BMTK_REQUIRE(plane < (1ll << 31), "spike_readout_fwd: the result is too large");
     const dim3 grid((unsigned)n_steps, (unsigned)p.slices, (unsigned)p.tiles);
-    const size_t lds = (size_t)kWaves * (p.trials * kWave * p.vw * sizeof(float) + kQueue * sizeof(uint32_t));
+    const size_t lds = (size_t)kFwdWaves * p.trials * kWave * p.vw * sizeof(float);
     const hipStream_t st = (hipStream_t)stream;
     const FastDiv by_batch = fast_div((uint32_t)batch);
-#define BMTK_FWD(VW, ONE)                                                                                                                      \
-    hipLaunchKernelGGL((spike_fwd_kernel<T, VW, ONE>), grid, dim3(kWaves *kWave), lds, st, spike_bits, stride, n_neurons *batch, by_batch, p.trials, \
+#define BMTK_FWD(VW, N)                                                                                                                      \
+    hipLaunchKernelGGL((spike_fwd_kernel<T, VW, N>), grid, dim3(kFwdWaves *kWave), lds, st, spike_bits, stride, n_neurons *batch, by_batch, p.trials, \
                        p.trial_tiles, (const T *)weight, dim, p.slice_words, (T *)y, part)
     BMTK_BY_TYPE(dtype, T, {
         if (batch == 1) {
-            if (p.vw == 1) BMTK_FWD(1, true);
-            else if (p.vw == 2) BMTK_FWD(2, true);
-            else BMTK_FWD(4, true);
+            if (p.vw == 1) BMTK_FWD(1, 1);
+            else if (p.vw == 2) BMTK_FWD(2, 1);
+            else BMTK_FWD(4, 1);
         } else {
-            if (p.vw == 1) BMTK_FWD(1, false);
-            else if (p.vw == 2) BMTK_FWD(2, false);
-            else BMTK_FWD(4, false);
+            if (p.vw == 1) BMTK_FWD(1, 32);
+            else if (p.vw == 2) BMTK_FWD(2, 16);
+            else BMTK_FWD(4, 8);
         }
         if (part)
             hipLaunchKernelGGL((spike_join_kernel<T>), dim3((unsigned)div_up(plane, kBlock)), dim3(kBlock), 0, st, part, (int)p.slices, plane, (T *)y);
@@ -431,24 +465,29 @@ extern "C" int bmtk_spike_readout_bwd_weight(const uint64_t *spike_bits, int64_t
     int rc = check_sizes("spike_readout_bwd_weight", n_steps, n_neurons, batch, dim, dtype);
     if (rc != BMTK_OK) return rc;
     BMTK_REQUIRE(stride >= (n_neurons * batch + 63) / 64, "spike_readout_bwd_weight: stride is shorter than a step's words");
+    int vw = lane_channels(dim, dtype, dy);
+    while (vw > 1 && !aligned(d_weight, vw * type_size(dtype))) vw /= 2;
     // neurons of a wavefront: 256 bits of a step where there are enough of them to fill the chip
     int64_t own = div_up(256, batch);
-    if (own > kSumRows) own = kSumRows;
-    const int64_t fill = n_neurons / 2048;
-    if (own > fill) own = fill < 1 ? 1 : fill;
-    int vw = lane_channels(dim, dtype, dy, (int)own);
-    while (vw > 1 && !aligned(d_weight, vw * type_size(dtype))) vw /= 2;
+    const int64_t fill = n_neurons / 2048 < 1 ? 1 : n_neurons / 2048;
+    if (own > fill) own = fill;
+    if (own > kSums / vw) own = kSums / vw;
     const dim3 grid((unsigned)div_up(n_neurons, kWaves * own), (unsigned)div_up(dim, kWave * vw));
-    const size_t lds = (size_t)kWaves * (own * kWave * vw * sizeof(float) + kQueue * sizeof(uint64_t));
     const hipStream_t st = (hipStream_t)stream;
     const FastDiv by_batch = fast_div((uint32_t)batch);
-#define BMTK_BWD(VW)                                                                                                                       \
-    hipLaunchKernelGGL((spike_bwd_weight_kernel<T, VW>), grid, dim3(kWaves *kWave), lds, st, spike_bits, stride, n_steps, n_neurons, by_batch, \
+#define BMTK_BWD(VW, N)                                                                                                                       \
+    hipLaunchKernelGGL((spike_bwd_weight_kernel<T, VW, N>), grid, dim3(kWaves *kWave), 0, st, spike_bits, stride, n_steps, n_neurons, by_batch, \
                        (int)own, (const T *)dy, dim, (T *)d_weight)
     BMTK_BY_TYPE(dtype, T, {
-        if (vw == 1) BMTK_BWD(1);
-        else if (vw == 2) BMTK_BWD(2);
-        else BMTK_BWD(4);
+        if (own == 1) {
+            if (vw == 1) BMTK_BWD(1, 1);
+            else if (vw == 2) BMTK_BWD(2, 1);
+            else BMTK_BWD(4, 1);
+        } else {
+            if (vw == 1) BMTK_BWD(1, 32);
+            else if (vw == 2) BMTK_BWD(2, 16);
+            else BMTK_BWD(4, 8);
+        }
     });
 #undef BMTK_BWD
     BMTK_CHECK_LAUNCH("spike_readout_bwd_weight");
