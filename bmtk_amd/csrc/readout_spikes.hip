@@ -277,85 +277,215 @@ spike_bwd_weight_kernel(const uint64_t *__restrict__ bits, int64_t stride, int64
 
 // ---------------------------------------------------------------------------------------------------------------------
 // Gradient by the spikes: dl_dz[t, i, b] = dy[t, b] . W[i], a matrix product whose result is most of its traffic.  A wavefront keeps
-// the weights of 64 neurons in registers and multiplies them with the dy rows of 32 (step, trial) pairs at a time.
-// A lane's share of a row is half of it: the order of the channels in the products is free as long as both operands have the same.
+// the weights of 64 neurons in registers, 64 channels of them; the workgroup puts the dy rows of 64 (step, trial) pairs into LDS, in the order in which
+// the matrix instructions take them, while those before are multiplied.
+//
+// fp32: the matrix instructions take 16-bit operands sixteen times as fast as 32-bit ones.  Each operand is the sum of three bf16 numbers of 8 bits each
+// (what the one before leaves, rounded), exact to 2^-27 of it; of the nine products the six that are not below 2^-24 of the whole
+// are made and added up in fp32.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
+typedef f16 f16x8 __attribute__((ext_vector_type(8)));
 constexpr int kDzK = 64;          // channels at a time
 constexpr int kDzNeurons = 64;    // of a wavefront
-constexpr int kDzRows = 32;       // (step, trial) pairs at a time
+constexpr int kDzRows = 64;       // (step, trial) pairs at a time
+
+// Eight channels of a row as operands of a matrix instruction
+template <typename T>
+struct Operand;
+template <>
+struct Operand<float> {
+    static constexpr int kParts = 3;
+    typedef bf16x8 Part;
+    // whether all numbers are finite (as bf16, too): only then are they the sum of their parts
+    __device__ __forceinline__ static bool split(const float (&v)[8], Part (&part)[3])
+    {
+        float odd = 0.0f;
+#pragma unroll
+        for (int s = 0; s < 8; ++s) {
+            float left = v[s];
+#pragma unroll
+            for (int p = 0; p < 3; ++p) {
+                const bf16 b = (bf16)left;
+                part[p][s] = b;
+                if (p == 0) odd += (float)b * 0.0f;
+                left -= (float)b;
+            }
+        }
+        return odd == 0.0f;
+    }
+    __device__ __forceinline__ static f32x16 multiply(const Part &a, const Part &b, const f32x16 &acc) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, acc, 0, 0, 0); }
+};
+template <>
+struct Operand<bf16> {
+    static constexpr int kParts = 1;
+    typedef bf16x8 Part;
+    __device__ __forceinline__ static bool split(const bf16 (&v)[8], Part (&part)[1])
+    {
+#pragma unroll
+        for (int s = 0; s < 8; ++s) part[0][s] = v[s];
+        return true;
+    }
+    __device__ __forceinline__ static f32x16 multiply(const Part &a, const Part &b, const f32x16 &acc) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, acc, 0, 0, 0); }
+};
+template <>
+struct Operand<f16> {
+    static constexpr int kParts = 1;
+    typedef f16x8 Part;
+    __device__ __forceinline__ static bool split(const f16 (&v)[8], Part (&part)[1])
+    {
+#pragma unroll
+        for (int s = 0; s < 8; ++s) part[0][s] = v[s];
+        return true;
+    }
+    __device__ __forceinline__ static f32x16 multiply(const Part &a, const Part &b, const f32x16 &acc) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, acc, 0, 0, 0); }
+};
 
 template <typename T, int VL>
-__device__ __forceinline__ void load_half(const T *__restrict__ base, int64_t row, bool there, int dim, int k0, float (&v)[kDzK / 2])
+__device__ __forceinline__ void load_eight(const T *__restrict__ base, int64_t row, bool there, int dim, int k0, T (&v)[8])
 {
     const T *p = base + row * dim + k0;
 #pragma unroll
-    for (int s = 0; s < kDzK / 2; s += VL) {
+    for (int s = 0; s < 8; s += VL) {
         Pack<T, VL> q{};
         if (there && k0 + s < dim) q = *reinterpret_cast<const Pack<T, VL> *>(p + s);
 #pragma unroll
-        for (int c = 0; c < VL; ++c) v[s + c] = (float)q.v[c];
+        for (int c = 0; c < VL; ++c) v[s + c] = q.v[c];
     }
 }
 
-// kAcross: neighbouring lanes hold neighbouring neurons (one trial); else neighbouring (step, trial) pairs
-template <typename T, int VL, bool kAcross>
-__global__ void __launch_bounds__(kWaves * kWave)
+// kAcross: neighbouring lanes hold neighbouring neurons (one trial); else neighbouring (step, trial) pairs.  kOnePass: up to 64 channels
+template <typename T, int VL, bool kAcross, bool kOnePass>
+__global__ void __launch_bounds__(kWaves * kWave, 2)
 spike_bwd_spikes_kernel(const T *__restrict__ weight, const T *__restrict__ dy, int64_t rows, int64_t n, FastDiv by_batch, int dim,
                         int64_t rows_per_block, float *__restrict__ dl_dz)
 {
+    typedef Operand<T> Op;
+    typedef typename Op::Part Part;
+    constexpr int P = Op::kParts, kSub = kDzRows / 32;
+    constexpr int kChunks = kDzRows * kDzK / 8 / (kWaves * kWave);   // of eight channels, of a thread
+    // [part][eighth of the channels][row]: what a wavefront reads at once, rows of two eighths, lies together
+    __shared__ Part staged[2][P][kDzK / 8][kDzRows];
+    __shared__ int odd_stage[2];
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
     const int half = lane / 32, col = lane % 32;
     const int batch = (int)by_batch.d;
     const int64_t ne = n * batch;
     const int64_t i0 = ((int64_t)blockIdx.x * kWaves + wave) * kDzNeurons;
-    if (i0 >= n) return;
-    const int64_t r_end = min(rows, (int64_t)(blockIdx.y + 1) * rows_per_block);
-    float a[2][kDzK / 2];
-    const bool one_pass = dim <= kDzK;
-    if (one_pass)
+    const int64_t r_begin = (int64_t)blockIdx.y * rows_per_block, r_end = min(rows, r_begin + rows_per_block);
+    const int passes = kOnePass ? 1 : (dim + kDzK - 1) / kDzK;
+    const int stages = (int)((r_end - r_begin + kDzRows - 1) / kDzRows) * passes;
+    T next[kChunks][8];
+    auto load_rows = [&](int stage) {
 #pragma unroll
-        for (int g = 0; g < 2; ++g) load_half<T, VL>(weight, i0 + g * 32 + col, i0 + g * 32 + col < n, dim, half * (kDzK / 2), a[g]);
-    for (int64_t r0 = (int64_t)blockIdx.y * rows_per_block; r0 < r_end; r0 += kDzRows) {
-        f32x16 acc[2] = {};
-        for (int k0 = 0; k0 < dim; k0 += kDzK) {
-            float b[kDzK / 2];
-            load_half<T, VL>(dy, r0 + col, r0 + col < r_end, dim, k0 + half * (kDzK / 2), b);
-            if (!one_pass)
-#pragma unroll
-                for (int g = 0; g < 2; ++g)
-                    load_half<T, VL>(weight, i0 + g * 32 + col, i0 + g * 32 + col < n, dim, k0 + half * (kDzK / 2), a[g]);
-#pragma unroll
-            for (int g = 0; g < 2; ++g)
-#pragma unroll
-                for (int s = 0; s < kDzK / 2; ++s)
-                    acc[g] = kAcross ? __builtin_amdgcn_mfma_f32_32x32x2f32(b[s], a[g][s], acc[g], 0, 0, 0)
-                                     : __builtin_amdgcn_mfma_f32_32x32x2f32(a[g][s], b[s], acc[g], 0, 0, 0);
+        for (int c = 0; c < kChunks; ++c) {
+            const int id = c * kWaves * kWave + threadIdx.x;
+            const int64_t r = r_begin + (int64_t)(stage / passes) * kDzRows + id / 8;
+            load_eight<T, VL>(dy, r, r < r_end, dim, stage % passes * kDzK + id % 8 * 8, next[c]);
         }
-        // register k of a lane: column col, row 8 (k / 4) + 4 half + k % 4
-        if (kAcross) {
+    };
+    Part a[2][P][kDzK / 16];
+    bool plain_weights = true;
+    auto load_weights = [&](int pass) {
 #pragma unroll
-            for (int k = 0; k < 16; ++k) {
-                const int64_t r = r0 + 8 * (k / 4) + 4 * half + k % 4;
-                if (r >= r_end) continue;
-                const uint32_t t = div_by((uint32_t)r, by_batch);
-                float *p = dl_dz + t * ne + (r - (int64_t)t * batch);
+        for (int g = 0; g < 2; ++g)
+#pragma unroll
+            for (int q = 0; q < kDzK / 16; ++q) {
+                T v[8];
+                Part part[P];
+                load_eight<T, VL>(weight, i0 + g * 32 + col, i0 + g * 32 + col < n, dim, pass * kDzK + (2 * q + half) * 8, v);
+                plain_weights = Op::split(v, part) && plain_weights;
+#pragma unroll
+                for (int p = 0; p < P; ++p) a[g][p][q] = part[p];
+            }
+    };
+    if (threadIdx.x < 2) odd_stage[threadIdx.x] = -1;
+    __syncthreads();
+    load_rows(0);
+    load_weights(0);
+    f32x16 acc[kOnePass ? 1 : kSub][2];
+    bool plain = true;
+    for (int stage = 0; stage < stages; ++stage) {
+        const int buffer = stage & 1, pass = kOnePass ? 0 : stage % passes;
+        bool fine = true;
+#pragma unroll
+        for (int c = 0; c < kChunks; ++c) {
+            const int id = c * kWaves * kWave + threadIdx.x;
+            Part part[P];
+            fine = Op::split(next[c], part) && fine;
+#pragma unroll
+            for (int p = 0; p < P; ++p) staged[buffer][p][id % 8][id / 8] = part[p];
+        }
+        if (P > 1 && !fine) odd_stage[buffer] = stage;
+        if (stage + 1 < stages) load_rows(stage + 1);
+        // (two buffers in turn: whoever writes the one of a stage has passed the barrier behind the reads of the stage before the last)
+        __syncthreads();
+        if (i0 >= n) continue;
+        if (pass == 0) plain = plain_weights;
+        plain = plain && odd_stage[buffer] != stage;
+        const int64_t r_stage = r_begin + (int64_t)(stage / passes) * kDzRows;
+#pragma unroll
+        for (int sub = 0; sub < kSub; ++sub) {
+            f32x16(&sums)[2] = acc[kOnePass ? 0 : sub];
+            if (pass == 0) sums[0] = 0.0f, sums[1] = 0.0f;
+#pragma unroll
+            for (int q = 0; q < kDzK / 16; ++q) {
+                Part b[P];
+#pragma unroll
+                for (int p = 0; p < P; ++p) b[p] = staged[buffer][p][2 * q + half][sub * 32 + col];
+#pragma unroll
+                for (int order = P - 1; order >= 0; --order)   // the small ones first
+#pragma unroll
+                    for (int p = 0; p <= order; ++p)
+#pragma unroll
+                        for (int g = 0; g < 2; ++g)
+                            sums[g] = kAcross ? Op::multiply(b[order - p], a[g][p][q], sums[g]) : Op::multiply(a[g][p][q], b[order - p], sums[g]);
+            }
+            if (!kOnePass && pass < passes - 1) continue;
+            const int64_t r0 = r_stage + sub * 32;
+            if (P > 1 && __ballot(!plain) != 0) {
+                // an infinity or NaN among them: in fp32 throughout, as it comes
 #pragma unroll
                 for (int g = 0; g < 2; ++g) {
-                    const int64_t i = i0 + g * 32 + col;
-                    if (i < n) p[i * batch] = acc[g][k];
+                    sums[g] = 0.0f;
+                    for (int k = 0; k < dim; k += 2) {
+                        const bool in = k + half < dim;
+                        const float w = in && i0 + g * 32 + col < n ? (float)weight[(i0 + g * 32 + col) * dim + k + half] : 0.0f;
+                        const float d = in && r0 + col < r_end ? (float)dy[(r0 + col) * dim + k + half] : 0.0f;
+                        sums[g] = kAcross ? __builtin_amdgcn_mfma_f32_32x32x2f32(d, w, sums[g], 0, 0, 0) : __builtin_amdgcn_mfma_f32_32x32x2f32(w, d, sums[g], 0, 0, 0);
+                    }
                 }
             }
-        } else if (r0 + col < r_end) {
-            const uint32_t t = div_by((uint32_t)(r0 + col), by_batch);
-            float *p = dl_dz + t * ne + (r0 + col - (int64_t)t * batch);
-#pragma unroll
-            for (int g = 0; g < 2; ++g)
+            // register k of a lane: column col, row 8 (k / 4) + 4 half + k % 4.  (Pointers that move on: 32 places kept are as many registers.)
+            const bool whole = i0 + kDzNeurons <= n && r0 + 32 <= r_end;
+            if (kAcross) {
+                int64_t r = r0 + 4 * half;
 #pragma unroll
                 for (int k = 0; k < 16; ++k) {
-                    const int64_t i = i0 + g * 32 + 8 * (k / 4) + 4 * half + k % 4;
-                    if (i < n) p[i * batch] = acc[g][k];
+                    if (whole || r < r_end) {
+                        // (one trial: a pair is a step)
+                        float *p = dl_dz + r * ne + i0 + col;
+                        if (whole || i0 + col < n) p[0] = sums[0][k];
+                        if (whole || i0 + 32 + col < n) p[32] = sums[1][k];
+                    }
+                    r += k % 4 == 3 ? 5 : 1;
                 }
+            } else {
+                const uint32_t t = div_by((uint32_t)min(r0 + col, r_end - 1), by_batch);
+                int64_t i = i0 + 4 * half;
+                float *p = dl_dz + t * ne + (r0 + col - (int64_t)t * batch) + i * batch;
+#pragma unroll
+                for (int g = 0; g < 2; ++g)
+#pragma unroll
+                    for (int k = 0; k < 16; ++k) {
+                        if (whole || (i < n && r0 + col < r_end)) *p = sums[g][k];
+                        const int on = k % 4 == 3 ? 5 : 1;
+                        p += (int64_t)on * batch;
+                        i += on;
+                    }
+            }
         }
+        if (!kOnePass) load_weights(pass < passes - 1 ? pass + 1 : 0);
     }
 }
 
@@ -507,21 +637,25 @@ extern "C" int bmtk_spike_readout_bwd_spikes(const void *weight, const void *dy,
     if (blocks > 65535) blocks = 65535;
     const int64_t per_block = div_up(most, blocks) * kDzRows;
     const dim3 grid((unsigned)across, (unsigned)div_up(rows, per_block));
-    const bool wide = dim % 4 == 0 && aligned(weight, 4 * type_size(dtype)) && aligned(dy, 4 * type_size(dtype));
+    const int vl = 16 / (int)type_size(dtype);   // 16 bytes a load
+    const bool wide = dim % vl == 0 && aligned(weight, 16) && aligned(dy, 16);
     const hipStream_t st = (hipStream_t)stream;
     const FastDiv by_batch = fast_div((uint32_t)batch);
-#define BMTK_DZ(VL, ACROSS)                                                                                                                       \
-    hipLaunchKernelGGL((spike_bwd_spikes_kernel<T, VL, ACROSS>), grid, dim3(kWaves *kWave), 0, st, (const T *)weight, (const T *)dy, rows, n_neurons, \
+#define BMTK_DZ(VL, ACROSS, ONE)                                                                                                                       \
+    hipLaunchKernelGGL((spike_bwd_spikes_kernel<T, VL, ACROSS, ONE>), grid, dim3(kWaves *kWave), 0, st, (const T *)weight, (const T *)dy, rows, n_neurons, \
                        by_batch, dim, per_block, dl_dz)
+#define BMTK_DZ_BY(VL)                                      \
+    do {                                                    \
+        if (batch == 1 && dim <= kDzK) BMTK_DZ(VL, true, true);   \
+        else if (batch == 1) BMTK_DZ(VL, true, false);      \
+        else if (dim <= kDzK) BMTK_DZ(VL, false, true);     \
+        else BMTK_DZ(VL, false, false);                     \
+    } while (0)
     BMTK_BY_TYPE(dtype, T, {
-        if (wide) {
-            if (batch == 1) BMTK_DZ(4, true);
-            else BMTK_DZ(4, false);
-        } else {
-            if (batch == 1) BMTK_DZ(1, true);
-            else BMTK_DZ(1, false);
-        }
+        if (wide) BMTK_DZ_BY(16 / sizeof(T));
+        else BMTK_DZ_BY(1);
     });
+#undef BMTK_DZ_BY
 #undef BMTK_DZ
     BMTK_CHECK_LAUNCH("spike_readout_bwd_spikes");
     return BMTK_OK;
