@@ -129,10 +129,10 @@ SIGNATURES = {
     "bmtk_microbench_atomics": (c_int32, [c_void_p, c_int64, c_int32, c_int32, c_int32, c_void_p]),
     "bmtk_microbench_hop": (c_int32, [c_void_p, c_void_p, c_int32, c_int32, c_int32, C.c_uint32, c_void_p]),
     "bmtk_spike_counts": (c_int32, [c_void_p, c_int64, c_int64, c_int64, c_void_p, c_void_p]),
-    "bmtk_spike_readout_workspace_bytes": (c_int64, [c_int64, c_int64, c_int32, c_int32]),
+    "bmtk_spike_readout_workspace_bytes": (c_int64, [c_int64, c_int64, c_int32, c_int32, c_int32]),
     "bmtk_spike_readout_fwd": (c_int32, [c_void_p, c_int64, c_int64, c_int64, c_int32, c_void_p, c_int32, c_int32, c_void_p, c_void_p, c_void_p]),
     "bmtk_spike_readout_bwd_weight": (c_int32, [c_void_p, c_int64, c_int64, c_int64, c_int32, c_void_p, c_int32, c_int32, c_void_p, c_void_p]),
-    "bmtk_spike_readout_bwd_spikes": (c_int32, [c_void_p, c_void_p, c_int64, c_int64, c_int32, c_int32, c_int32, c_void_p, c_void_p]),
+    "bmtk_spike_readout_bwd_spikes": (c_int32, [c_void_p, c_void_p, c_int64, c_int64, c_int32, c_int32, c_int32, c_void_p, c_void_p, c_void_p]),
     "bmtk_gated_scan_workspace_bytes": (c_int64, [c_int64, c_int64, c_int32, c_int32, c_int32]),
     "bmtk_gated_scan_fwd": (c_int32, [c_int64, c_int64] + [c_int32] * 4 + [c_void_p, c_int64, c_int64] * 2 + [c_void_p] * 7),
     "bmtk_gated_scan_bwd": (c_int32, [c_int64, c_int64] + [c_int32] * 4 + [c_void_p, c_int64, c_int64] * 2 + [c_void_p] * 2 +

@@ -1,4 +1,6 @@
 // Readout of spikes: y[t, b] = sum of the weight rows of the neurons that fired in step t of trial b, and its gradients.
+#include <type_traits>
+
 #include "readout.hpp"
 
 namespace bmtk {
@@ -277,18 +279,21 @@ spike_bwd_weight_kernel(const uint64_t *__restrict__ bits, int64_t stride, int64
 
 // ---------------------------------------------------------------------------------------------------------------------
 // Gradient by the spikes: dl_dz[t, i, b] = dy[t, b] . W[i], a matrix product whose result is most of its traffic.  A wavefront keeps
-// the weights of 64 neurons in registers, 64 channels of them; the workgroup puts the dy rows of 64 (step, trial) pairs into LDS, in the order in which
+// the weights of 64 neurons in registers, 64 channels of them; the workgroup puts the dy rows of 32 (step, trial) pairs into LDS, in the order in which
 // the matrix instructions take them, while those before are multiplied.
 //
 // fp32: the matrix instructions take 16-bit operands sixteen times as fast as 32-bit ones.  Each operand is the sum of three bf16 numbers of 8 bits each
 // (what the one before leaves, rounded), exact to 2^-27 of it; of the nine products the six that are not below 2^-24 of the whole
 // are made and added up in fp32.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
+typedef float f32x4 __attribute__((ext_vector_type(4)));
 typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef f16 f16x8 __attribute__((ext_vector_type(8)));
 constexpr int kDzK = 64;          // channels at a time
-constexpr int kDzNeurons = 64;    // of a wavefront
-constexpr int kDzRows = 64;       // (step, trial) pairs at a time
+constexpr int kDzWaves = 4;
+constexpr int kDzGroups = 2;      // of 32 neurons, of a wavefront
+constexpr int kDzNeurons = 32 * kDzGroups;
+constexpr int kDzRows = 32;       // (step, trial) pairs at a time
 
 // Eight channels of a row as operands of a matrix instruction
 template <typename T>
@@ -341,151 +346,192 @@ struct Operand<f16> {
     __device__ __forceinline__ static f32x16 multiply(const Part &a, const Part &b, const f32x16 &acc) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, acc, 0, 0, 0); }
 };
 
+// Eight channels of row `row` of those that begin at `base`, of which there are `rows` (at least one) left; zero where there is no such row or channel.
+// (No branches: what lies outside is read from elsewhere in the last row, and its bits are cleared.  Offsets of 32 bits from a place that is the
+// same for all lanes.)
 template <typename T, int VL>
-__device__ __forceinline__ void load_eight(const T *__restrict__ base, int64_t row, bool there, int dim, int k0, T (&v)[8])
+__device__ __forceinline__ void load_eight(const T *__restrict__ base, int row, int rows, int dim, int k0, T (&v)[8])
 {
-    const T *p = base + row * dim + k0;
+    constexpr int kBytes = VL * sizeof(T);
+    typedef typename std::conditional<kBytes % 4 == 0, uint32_t, uint16_t>::type Word;
+    const unsigned at = (unsigned)min(row, rows - 1) * (unsigned)dim;
 #pragma unroll
     for (int s = 0; s < 8; s += VL) {
-        Pack<T, VL> q{};
-        if (there && k0 + s < dim) q = *reinterpret_cast<const Pack<T, VL> *>(p + s);
+        Pack<T, VL> q = *reinterpret_cast<const Pack<T, VL> *>(base + (at + (unsigned)min(k0 + s, dim - VL)));
+        Word w[kBytes / sizeof(Word)];
+        __builtin_memcpy(w, &q, kBytes);
+        const Word keep = (Word)-(int)(row < rows && k0 + s < dim);
+#pragma unroll
+        for (unsigned c = 0; c < kBytes / sizeof(Word); ++c) w[c] &= keep;
+        __builtin_memcpy(&q, w, kBytes);
 #pragma unroll
         for (int c = 0; c < VL; ++c) v[s + c] = q.v[c];
     }
 }
 
-// kAcross: neighbouring lanes hold neighbouring neurons (one trial); else neighbouring (step, trial) pairs.  kOnePass: up to 64 channels
-template <typename T, int VL, bool kAcross, bool kOnePass>
-__global__ void __launch_bounds__(kWaves * kWave, 2)
+// How the products reach memory.  kPairs: neighbouring lanes hold neighbouring (step, trial) pairs.  kAcross (one trial): neighbouring
+// neurons.  kTurned + s (4, 8, 16 or a multiple of 32 trials, 2^s fours of them in a tile, and rows that begin on 128 bytes): through LDS into the
+// order of memory, 16 bytes a lane, whole lines past the caches.  (Parts of lines written past the caches take five times as long.)
+enum { kPairs = 0, kAcross = 1, kTurned = 2 };
+
+// kOnePass: up to 64 channels
+template <typename T, int VL, int kOut, bool kOnePass>
+__global__ void __launch_bounds__(kDzWaves * kWave, (kOnePass && kOut >= kTurned) || sizeof(T) == 2 ? 3 : 2)
 spike_bwd_spikes_kernel(const T *__restrict__ weight, const T *__restrict__ dy, int64_t rows, int64_t n, FastDiv by_batch, int dim,
-                        int64_t rows_per_block, float *__restrict__ dl_dz)
+                        int64_t rows_per_block, int32_t *__restrict__ not_finite, float *__restrict__ dl_dz)
 {
     typedef Operand<T> Op;
     typedef typename Op::Part Part;
-    constexpr int P = Op::kParts, kSub = kDzRows / 32;
-    constexpr int kChunks = kDzRows * kDzK / 8 / (kWaves * kWave);   // of eight channels, of a thread
+    constexpr int P = Op::kParts;
+    static_assert(kDzRows * kDzK / 8 == kDzWaves * kWave, "eight channels of a row for every thread");
     // [part][eighth of the channels][row]: what a wavefront reads at once, rows of two eighths, lies together
     __shared__ Part staged[2][P][kDzK / 8][kDzRows];
-    __shared__ int odd_stage[2];
+    __shared__ f32x4 turn[kOut >= kTurned ? kDzWaves : 1][32 * 8];
+    __shared__ int odd;   // some number is not finite
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
     const int half = lane / 32, col = lane % 32;
     const int batch = (int)by_batch.d;
     const int64_t ne = n * batch;
-    const int64_t i0 = ((int64_t)blockIdx.x * kWaves + wave) * kDzNeurons;
+    const int64_t i0 = ((int64_t)blockIdx.x * kDzWaves + wave) * kDzNeurons;
     const int64_t r_begin = (int64_t)blockIdx.y * rows_per_block, r_end = min(rows, r_begin + rows_per_block);
     const int passes = kOnePass ? 1 : (dim + kDzK - 1) / kDzK;
     const int stages = (int)((r_end - r_begin + kDzRows - 1) / kDzRows) * passes;
-    T next[kChunks][8];
+    T next[8];
     auto load_rows = [&](int stage) {
-#pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-            const int id = c * kWaves * kWave + threadIdx.x;
-            const int64_t r = r_begin + (int64_t)(stage / passes) * kDzRows + id / 8;
-            load_eight<T, VL>(dy, r, r < r_end, dim, stage % passes * kDzK + id % 8 * 8, next[c]);
-        }
+        const int at = min(stage, stages - 1);   // (behind the last one: it again, which nobody looks at)
+        const int64_t r = r_begin + (int64_t)(at / passes) * kDzRows;
+        load_eight<T, VL>(dy + r * dim, threadIdx.x / 8, (int)min(r_end - r, (int64_t)kDzRows), dim, at % passes * kDzK + threadIdx.x % 8 * 8, next);
     };
-    Part a[2][P][kDzK / 16];
-    bool plain_weights = true;
+    Part a[kDzGroups][P][kDzK / 16];
     auto load_weights = [&](int pass) {
+        bool fine = true;
 #pragma unroll
-        for (int g = 0; g < 2; ++g)
+        for (int g = 0; g < kDzGroups; ++g)
 #pragma unroll
             for (int q = 0; q < kDzK / 16; ++q) {
                 T v[8];
                 Part part[P];
-                load_eight<T, VL>(weight, i0 + g * 32 + col, i0 + g * 32 + col < n, dim, pass * kDzK + (2 * q + half) * 8, v);
-                plain_weights = Op::split(v, part) && plain_weights;
+                if (pass * kDzK + q * 16 >= dim) break;
+                // (a wavefront behind the last neuron multiplies the last one's weights, and writes nothing)
+                const int64_t first = min(i0, n - 1);
+                load_eight<T, VL>(weight + first * dim, g * 32 + col, (int)min(n - first, (int64_t)kDzNeurons), dim, pass * kDzK + (2 * q + half) * 8, v);
+                fine = Op::split(v, part) && fine;
 #pragma unroll
                 for (int p = 0; p < P; ++p) a[g][p][q] = part[p];
             }
+        return fine;
     };
-    if (threadIdx.x < 2) odd_stage[threadIdx.x] = -1;
-    __syncthreads();
-    load_rows(0);
-    load_weights(0);
-    f32x16 acc[kOnePass ? 1 : kSub][2];
-    bool plain = true;
-    for (int stage = 0; stage < stages; ++stage) {
-        const int buffer = stage & 1, pass = kOnePass ? 0 : stage % passes;
-        bool fine = true;
+    f32x16 sums[kDzGroups];
+    // register k of a lane: column col, row 8 (k / 4) + 4 half + k % 4.  (Pointers that move on: places kept are as many registers.)
+    auto put = [&](int64_t r0) {
+        const bool whole = i0 + kDzNeurons <= n && r0 + kDzRows <= r_end;
 #pragma unroll
-        for (int c = 0; c < kChunks; ++c) {
-            const int id = c * kWaves * kWave + threadIdx.x;
-            Part part[P];
-            fine = Op::split(next[c], part) && fine;
+        for (int g = 0; g < kDzGroups; ++g) {
+            const int64_t ig = i0 + g * 32;
+            if (kOut >= kTurned) {
+                // [neuron][pairs by four], turned by the neuron so that neither side meets itself in a bank
 #pragma unroll
-            for (int p = 0; p < P; ++p) staged[buffer][p][id % 8][id / 8] = part[p];
-        }
-        if (P > 1 && !fine) odd_stage[buffer] = stage;
-        if (stage + 1 < stages) load_rows(stage + 1);
-        // (two buffers in turn: whoever writes the one of a stage has passed the barrier behind the reads of the stage before the last)
-        __syncthreads();
-        if (i0 >= n) continue;
-        if (pass == 0) plain = plain_weights;
-        plain = plain && odd_stage[buffer] != stage;
-        const int64_t r_stage = r_begin + (int64_t)(stage / passes) * kDzRows;
+                for (int q = 0; q < 4; ++q)
+                    turn[wave][col * 8 + ((2 * q + half) ^ (col & 7))] = f32x4{sums[g][4 * q], sums[g][4 * q + 1], sums[g][4 * q + 2], sums[g][4 * q + 3]};
+                wave_order();
+                // A neuron has 2^kShift fours of trials in a step; up to 32 trials the tile begins with a step, of more it is a part of one.  Four `at`
+                // of the tile, in the order of memory: step at >> (kShift + 5), neuron (at >> kShift) & 31; of 64 k + lane the sum of both parts'.
+                constexpr int kShift = kOut - kTurned;
+                const int64_t t0 = kShift < 3 ? r0 >> (kShift + 2) : (int64_t)div_by((uint32_t)r0, by_batch);
+                const int c = lane & ((1 << kShift) - 1), i_lane = (lane >> kShift) & 31, step_lane = lane >> (kShift + 5);
+                float *to = dl_dz + (t0 + step_lane) * ne + (ig + i_lane) * batch + (r0 - t0 * batch) + 4 * c;
 #pragma unroll
-        for (int sub = 0; sub < kSub; ++sub) {
-            f32x16(&sums)[2] = acc[kOnePass ? 0 : sub];
-            if (pass == 0) sums[0] = 0.0f, sums[1] = 0.0f;
-#pragma unroll
-            for (int q = 0; q < kDzK / 16; ++q) {
-                Part b[P];
-#pragma unroll
-                for (int p = 0; p < P; ++p) b[p] = staged[buffer][p][2 * q + half][sub * 32 + col];
-#pragma unroll
-                for (int order = P - 1; order >= 0; --order)   // the small ones first
-#pragma unroll
-                    for (int p = 0; p <= order; ++p)
-#pragma unroll
-                        for (int g = 0; g < 2; ++g)
-                            sums[g] = kAcross ? Op::multiply(b[order - p], a[g][p][q], sums[g]) : Op::multiply(a[g][p][q], b[order - p], sums[g]);
-            }
-            if (!kOnePass && pass < passes - 1) continue;
-            const int64_t r0 = r_stage + sub * 32;
-            if (P > 1 && __ballot(!plain) != 0) {
-                // an infinity or NaN among them: in fp32 throughout, as it comes
-#pragma unroll
-                for (int g = 0; g < 2; ++g) {
-                    sums[g] = 0.0f;
-                    for (int k = 0; k < dim; k += 2) {
-                        const bool in = k + half < dim;
-                        const float w = in && i0 + g * 32 + col < n ? (float)weight[(i0 + g * 32 + col) * dim + k + half] : 0.0f;
-                        const float d = in && r0 + col < r_end ? (float)dy[(r0 + col) * dim + k + half] : 0.0f;
-                        sums[g] = kAcross ? __builtin_amdgcn_mfma_f32_32x32x2f32(d, w, sums[g], 0, 0, 0) : __builtin_amdgcn_mfma_f32_32x32x2f32(w, d, sums[g], 0, 0, 0);
-                    }
+                for (int k = 0; k < 4; ++k) {
+                    const int i_k = ((k * kWave) >> kShift) & 31, step_k = (k * kWave) >> (kShift + 5);
+                    const int i = i_lane + i_k, c4 = ((step_lane + step_k) << kShift) + c;
+                    const f32x4 v = turn[wave][i * 8 + (c4 ^ (i & 7))];
+                    if (whole || (ig + i < n && r0 + 4 * c4 < r_end)) __builtin_nontemporal_store(v, reinterpret_cast<f32x4 *>(to + (step_k * ne + i_k * batch)));
                 }
-            }
-            // register k of a lane: column col, row 8 (k / 4) + 4 half + k % 4.  (Pointers that move on: 32 places kept are as many registers.)
-            const bool whole = i0 + kDzNeurons <= n && r0 + 32 <= r_end;
-            if (kAcross) {
+                wave_order();
+            } else if (kOut == kAcross) {
                 int64_t r = r0 + 4 * half;
 #pragma unroll
                 for (int k = 0; k < 16; ++k) {
-                    if (whole || r < r_end) {
-                        // (one trial: a pair is a step)
-                        float *p = dl_dz + r * ne + i0 + col;
-                        if (whole || i0 + col < n) p[0] = sums[0][k];
-                        if (whole || i0 + 32 + col < n) p[32] = sums[1][k];
-                    }
+                    // (one trial: a pair is a step)
+                    if (whole || (r < r_end && ig + col < n)) dl_dz[r * ne + ig + col] = sums[g][k];
                     r += k % 4 == 3 ? 5 : 1;
                 }
             } else {
                 const uint32_t t = div_by((uint32_t)min(r0 + col, r_end - 1), by_batch);
-                int64_t i = i0 + 4 * half;
+                int64_t i = ig + 4 * half;
                 float *p = dl_dz + t * ne + (r0 + col - (int64_t)t * batch) + i * batch;
 #pragma unroll
-                for (int g = 0; g < 2; ++g)
-#pragma unroll
-                    for (int k = 0; k < 16; ++k) {
-                        if (whole || (i < n && r0 + col < r_end)) *p = sums[g][k];
-                        const int on = k % 4 == 3 ? 5 : 1;
-                        p += (int64_t)on * batch;
-                        i += on;
-                    }
+                for (int k = 0; k < 16; ++k) {
+                    if (whole || (i < n && r0 + col < r_end)) *p = sums[g][k];
+                    const int on = k % 4 == 3 ? 5 : 1;
+                    p += (int64_t)on * batch;
+                    i += on;
+                }
             }
         }
-        if (!kOnePass) load_weights(pass < passes - 1 ? pass + 1 : 0);
+    };
+
+    if (threadIdx.x == 0) odd = 0;
+    __syncthreads();
+    load_rows(0);
+    if (!load_weights(0)) odd = 1;
+    for (int stage = 0; stage < stages; ++stage) {
+        const int buffer = stage & 1, pass = kOnePass ? 0 : stage % passes;
+        {
+            Part part[P];
+            if (!Op::split(next, part)) odd = 1;
+#pragma unroll
+            for (int p = 0; p < P; ++p) staged[buffer][p][threadIdx.x % 8][threadIdx.x / 8] = part[p];
+        }
+        load_rows(stage + 1);
+        // (two buffers in turn: whoever writes the one of a stage has passed the barrier behind the reads of the stage before the last)
+        __syncthreads();
+        if (pass == 0)
+#pragma unroll
+            for (int g = 0; g < kDzGroups; ++g) sums[g] = 0.0f;
+#pragma unroll
+        for (int q = 0; q < kDzK / 16; ++q) {
+            if (pass * kDzK + q * 16 >= dim) break;
+            Part b[P];
+#pragma unroll
+            for (int p = 0; p < P; ++p) b[p] = staged[buffer][p][2 * q + half][col];
+#pragma unroll
+            for (int order = P - 1; order >= 0; --order)   // the small ones first
+#pragma unroll
+                for (int p = 0; p <= order; ++p)
+#pragma unroll
+                    for (int g = 0; g < kDzGroups; ++g)
+                        sums[g] = kOut == kPairs ? Op::multiply(a[g][p][q], b[order - p], sums[g]) : Op::multiply(b[order - p], a[g][p][q], sums[g]);
+        }
+        if (!kOnePass && !load_weights(pass < passes - 1 ? pass + 1 : 0)) odd = 1;
+        if (kOnePass || pass == passes - 1) put(r_begin + (int64_t)(stage / passes) * kDzRows);
+    }
+    if (P > 1) {
+        __syncthreads();
+        if (threadIdx.x == 0) not_finite[blockIdx.y * gridDim.x + blockIdx.x] = odd;
+    }
+}
+
+// The parts of the result with an infinity or NaN among their operands (which their parts do not add up to) once more, product by product in fp32, as
+// it comes.  A workgroup looks at 256 parts.
+__global__ void __launch_bounds__(kBlock)
+spike_bwd_spikes_again_kernel(const float *__restrict__ weight, const float *__restrict__ dy, int64_t rows, int64_t n, FastDiv by_batch, int dim,
+                              int64_t rows_per_block, int parts_across, int parts, const int32_t *__restrict__ not_finite, float *__restrict__ dl_dz)
+{
+    const int first = blockIdx.x * kBlock;
+    if (!__syncthreads_or(first + (int)threadIdx.x < parts && not_finite[first + threadIdx.x] != 0)) return;
+    for (int part = first; part < min(parts, first + kBlock); ++part) {
+        if (not_finite[part] == 0) continue;
+        const int64_t r_begin = (int64_t)(part / parts_across) * rows_per_block, r_end = min(rows, r_begin + rows_per_block);
+        const int64_t i_begin = (int64_t)(part % parts_across) * kDzWaves * kDzNeurons, i_end = min(n, i_begin + kDzWaves * kDzNeurons);
+        for (int64_t r = r_begin; r < r_end; ++r) {
+            const uint32_t t = div_by((uint32_t)r, by_batch);
+            for (int64_t i = i_begin + threadIdx.x; i < i_end; i += kBlock) {
+                float s = 0.0f;
+                for (int c = 0; c < dim; ++c) s += weight[i * dim + c] * dy[r * dim + c];
+                dl_dz[(t * n + i) * by_batch.d + (r - (int64_t)t * by_batch.d)] = s;
+            }
+        }
     }
 }
 
@@ -524,6 +570,22 @@ FwdPlan fwd_plan(int64_t n_steps, int64_t n, int batch, int dim, int vw)
     return p;
 }
 
+struct DzPlan {
+    int64_t across, per_block, down, parts;
+};
+DzPlan dz_plan(int64_t n_steps, int64_t n, int batch)
+{
+    DzPlan p;
+    p.across = div_up(n, kDzWaves * kDzNeurons);
+    const int64_t rows = n_steps * batch, most = div_up(rows, kDzRows);
+    int64_t blocks = div_up(4096, p.across);
+    if (blocks > most) blocks = most;
+    p.per_block = div_up(most, blocks) * kDzRows;
+    p.down = div_up(rows, p.per_block);
+    p.parts = p.across * p.down;
+    return p;
+}
+
 int check_sizes(const char *who, int64_t n_steps, int64_t n, int32_t batch, int32_t dim, int32_t dtype)
 {
     BMTK_REQUIRE(n_steps > 0 && n > 0 && batch > 0 && dim > 0, "%s: sizes must be positive", who);
@@ -539,9 +601,10 @@ int check_sizes(const char *who, int64_t n_steps, int64_t n, int32_t batch, int3
 
 using namespace bmtk;
 
-extern "C" int64_t bmtk_spike_readout_workspace_bytes(int64_t n_steps, int64_t n_neurons, int32_t batch, int32_t dim)
+extern "C" int64_t bmtk_spike_readout_workspace_bytes(int64_t n_steps, int64_t n_neurons, int32_t batch, int32_t dim, int32_t backward)
 {
     if (check_sizes("spike_readout_workspace_bytes", n_steps, n_neurons, batch, dim, BMTK_F32) != BMTK_OK) return 0;
+    if (backward) return dz_plan(n_steps, n_neurons, batch).parts * (int64_t)sizeof(int32_t);
     int64_t slices = 1;   // (as many as any alignment of the weights takes)
     for (int vw = 1; vw <= 4; vw *= 2) {
         const FwdPlan p = fwd_plan(n_steps, n_neurons, batch, dim, vw);
@@ -625,37 +688,47 @@ extern "C" int bmtk_spike_readout_bwd_weight(const uint64_t *spike_bits, int64_t
 }
 
 extern "C" int bmtk_spike_readout_bwd_spikes(const void *weight, const void *dy, int64_t n_steps, int64_t n_neurons, int32_t batch, int32_t dim, int32_t dtype,
-                                             float *dl_dz, void *stream)
+                                             float *dl_dz, int32_t *workspace, void *stream)
 {
     BMTK_REQUIRE(weight && dy && dl_dz, "spike_readout_bwd_spikes: pointers must be non-null");
     int rc = check_sizes("spike_readout_bwd_spikes", n_steps, n_neurons, batch, dim, dtype);
     if (rc != BMTK_OK) return rc;
-    const int64_t rows = n_steps * batch, across = div_up(n_neurons, kWaves * kDzNeurons);
-    int64_t blocks = div_up(4096, across);
-    const int64_t most = div_up(rows, kDzRows);
-    if (blocks > most) blocks = most;
-    if (blocks > 65535) blocks = 65535;
-    const int64_t per_block = div_up(most, blocks) * kDzRows;
-    const dim3 grid((unsigned)across, (unsigned)div_up(rows, per_block));
+    BMTK_REQUIRE(dtype != BMTK_F32 || workspace, "spike_readout_bwd_spikes: needs its workspace");
+    const DzPlan p = dz_plan(n_steps, n_neurons, batch);
+    const int64_t rows = n_steps * batch;
+    const dim3 grid((unsigned)p.across, (unsigned)p.down);
     const int vl = 16 / (int)type_size(dtype);   // 16 bytes a load
     const bool wide = dim % vl == 0 && aligned(weight, 16) && aligned(dy, 16);
     const hipStream_t st = (hipStream_t)stream;
     const FastDiv by_batch = fast_div((uint32_t)batch);
-#define BMTK_DZ(VL, ACROSS, ONE)                                                                                                                       \
-    hipLaunchKernelGGL((spike_bwd_spikes_kernel<T, VL, ACROSS, ONE>), grid, dim3(kWaves *kWave), 0, st, (const T *)weight, (const T *)dy, rows, n_neurons, \
-                       by_batch, dim, per_block, dl_dz)
-#define BMTK_DZ_BY(VL)                                      \
-    do {                                                    \
-        if (batch == 1 && dim <= kDzK) BMTK_DZ(VL, true, true);   \
-        else if (batch == 1) BMTK_DZ(VL, true, false);      \
-        else if (dim <= kDzK) BMTK_DZ(VL, false, true);     \
-        else BMTK_DZ(VL, false, false);                     \
+    // (a tile's pairs are whole steps, or 32 trials of one)
+    const bool turned = (batch % 32 == 0 || batch == 4 || batch == 8 || batch == 16) && aligned(dl_dz, 128) && n_neurons * batch % 32 == 0;
+#define BMTK_DZ(VL, OUT, ONE)                                                                                                                       \
+    hipLaunchKernelGGL((spike_bwd_spikes_kernel<T, VL, OUT, ONE>), grid, dim3(kDzWaves *kWave), 0, st, (const T *)weight, (const T *)dy, rows, n_neurons, \
+                       by_batch, dim, p.per_block, workspace, dl_dz)
+#define BMTK_DZ_OUT(VL, ONE)                                 \
+    do {                                                     \
+        if (batch == 1) BMTK_DZ(VL, kAcross, ONE);           \
+        else if (!turned) BMTK_DZ(VL, kPairs, ONE);          \
+        else if (batch == 4) BMTK_DZ(VL, kTurned, ONE);      \
+        else if (batch == 8) BMTK_DZ(VL, kTurned + 1, ONE);  \
+        else if (batch == 16) BMTK_DZ(VL, kTurned + 2, ONE); \
+        else BMTK_DZ(VL, kTurned + 3, ONE);                  \
+    } while (0)
+#define BMTK_DZ_BY(VL)                            \
+    do {                                          \
+        if (dim <= kDzK) BMTK_DZ_OUT(VL, true);   \
+        else BMTK_DZ_OUT(VL, false);              \
     } while (0)
     BMTK_BY_TYPE(dtype, T, {
         if (wide) BMTK_DZ_BY(16 / sizeof(T));
         else BMTK_DZ_BY(1);
     });
+    if (dtype == BMTK_F32)
+        hipLaunchKernelGGL(spike_bwd_spikes_again_kernel, dim3((unsigned)div_up(p.parts, kBlock)), dim3(kBlock), 0, st, (const float *)weight, (const float *)dy, rows,
+                           n_neurons, by_batch, dim, p.per_block, (int)p.across, (int)p.parts, workspace, dl_dz);
 #undef BMTK_DZ_BY
+#undef BMTK_DZ_OUT
 #undef BMTK_DZ
     BMTK_CHECK_LAUNCH("spike_readout_bwd_spikes");
     return BMTK_OK;

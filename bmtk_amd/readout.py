@@ -75,7 +75,7 @@ def spike_readout(bits, weight, batch=1):
     y = torch.empty(steps, batch, dim, dtype=weight.dtype, device=weight.device)
     if steps:
         lib = _lib.load()
-        ws = _workspace(lib.bmtk_spike_readout_workspace_bytes(steps, n, batch, dim), weight.device)
+        ws = _workspace(lib.bmtk_spike_readout_workspace_bytes(steps, n, batch, dim, 0), weight.device)
         _lib.check(lib.bmtk_spike_readout_fwd(bits.data_ptr(), stride, steps, n, batch, weight.data_ptr(), dim, _CODE[weight.dtype], y.data_ptr(), ws, _stream()))
     return y
 
@@ -94,7 +94,8 @@ def spike_readout_bwd(bits, weight, dy, batch=1, spikes=True):
         lib, code = _lib.load(), _CODE[weight.dtype]
         _lib.check(lib.bmtk_spike_readout_bwd_weight(bits.data_ptr(), stride, steps, n, batch, dy.data_ptr(), dim, code, d_weight.data_ptr(), _stream()))
         if spikes:
-            _lib.check(lib.bmtk_spike_readout_bwd_spikes(weight.data_ptr(), dy.data_ptr(), steps, n, batch, dim, code, dl_dz.data_ptr(), _stream()))
+            ws = _workspace(lib.bmtk_spike_readout_workspace_bytes(steps, n, batch, dim, 1) if code == 0 else 0, dev)
+            _lib.check(lib.bmtk_spike_readout_bwd_spikes(weight.data_ptr(), dy.data_ptr(), steps, n, batch, dim, code, dl_dz.data_ptr(), ws, _stream()))
     return d_weight, dl_dz
 
 

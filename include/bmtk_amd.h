@@ -711,15 +711,15 @@ int bmtk_rate_mse(const int32_t *counts, int64_t n_neurons, int32_t batch, int64
 /* y[t][b][:] = sum of weight[i][:] over the neurons i that fired in step t of trial b.  spike_bits: n_steps rows of `stride` words (bits
  * behind n_neurons * batch are not looked at); weight [n_neurons][dim], y [n_steps][batch][dim], contiguous.
  * Limits: n_neurons * batch < 2^31 - 64, n_steps < 2^24, n_steps * batch < 2^31 - 64, n_steps * batch * dim < 2^31, batch and dim up to 65,536. */
-int64_t bmtk_spike_readout_workspace_bytes(int64_t n_steps, int64_t n_neurons, int32_t batch, int32_t dim);
+int64_t bmtk_spike_readout_workspace_bytes(int64_t n_steps, int64_t n_neurons, int32_t batch, int32_t dim, int32_t backward);
 int bmtk_spike_readout_fwd(const uint64_t *spike_bits, int64_t stride, int64_t n_steps, int64_t n_neurons, int32_t batch, const void *weight, int32_t dim,
                            int32_t dtype, void *y, float *workspace, void *stream);
 /* d_weight[i][:] = sum of dy[t][b][:] over the spikes of neuron i (all rows are written) */
 int bmtk_spike_readout_bwd_weight(const uint64_t *spike_bits, int64_t stride, int64_t n_steps, int64_t n_neurons, int32_t batch, const void *dy, int32_t dim,
                                   int32_t dtype, void *d_weight, void *stream);
-/* dl_dz[t][i * batch + b] = dy[t][b][:] . weight[i][:], in 32 bits: what bmtk_glif3_bwd takes */
+/* dl_dz[t][i * batch + b] = dy[t][b][:] . weight[i][:], in 32 bits: what bmtk_glif3_bwd takes.  workspace: only for BMTK_F32 */
 int bmtk_spike_readout_bwd_spikes(const void *weight, const void *dy, int64_t n_steps, int64_t n_neurons, int32_t batch, int32_t dim, int32_t dtype,
-                                  float *dl_dz, void *stream);
+                                  float *dl_dz, int32_t *workspace, void *stream);
 
 /* h[t][b][c] = a h[t-1][b][c] + x[t][b][c] for the steps t < lengths[b] (NULL: all n_steps), from state [batch][dim] (NULL: zero); h is 0 behind
  * a sequence's end and nothing of x or decay is read there.  last [batch][dim]: the state behind each sequence's last step.
