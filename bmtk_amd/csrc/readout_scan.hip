@@ -48,19 +48,34 @@ __device__ __forceinline__ void store_v(T *p, const float (&v)[V])
     *reinterpret_cast<Pack<T, V> *>(p) = q;
 }
 
-// Gates: one per channel for all steps, one per channel and step, or one per step for several neighbouring channels
+// Gates: one per channel for all steps, one per channel and step, or one per step for several neighbouring channels (a lane's are of one gate)
 enum { kConst = 0, kEach = 1, kShared = 2 };
 
-template <typename TA, int V, int G>
-__device__ __forceinline__ void load_gate(const TA *p, const int (&off)[V], bool there, float (&v)[V])
-{
-    if (G == kEach) {
-        load_v<TA, V>(p + off[0], there, 1.0f, v);
-    } else {
+// A lane's part of a block of steps as it lies in memory
+template <typename T, int V>
+struct Block {
+    Pack<T, V> v[kSteps];
+    // (behind `end` the last step again: nothing outside is read, and nothing depends on a lane)
+    __device__ __forceinline__ void load(const T *p, int64_t stride, int64_t t0, int64_t end)
+    {
+        if (t0 + kSteps <= end) {
 #pragma unroll
-        for (int c = 0; c < V; ++c) v[c] = there ? (float)p[off[c]] : 1.0f;
+            for (int k = 0; k < kSteps; ++k) v[k] = *reinterpret_cast<const Pack<T, V> *>(p + (t0 + k) * stride);
+        } else {
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) v[k] = *reinterpret_cast<const Pack<T, V> *>(p + min(t0 + k, end - 1) * stride);
+        }
     }
-}
+    // steps from `there` on are as if they were `other`
+    __device__ __forceinline__ void cut(int there, float other)
+    {
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k)
+#pragma unroll
+            for (int c = 0; c < V; ++c) v[k].v[c] = k < there ? v[k].v[c] : (T)other;
+    }
+    __device__ __forceinline__ float get(int k, int c) const { return (float)v[k].v[V == 1 ? 0 : c]; }
+};
 
 // What a lane knows of its columns
 template <int V>
@@ -68,7 +83,7 @@ struct Lane {
     int64_t col;
     bool in;
     int32_t b, ch, len;
-    int gate[V];
+    int gate;
 };
 template <int V, int G>
 __device__ __forceinline__ Lane<V> lane_of(const ScanArgs &s)
@@ -76,12 +91,11 @@ __device__ __forceinline__ Lane<V> lane_of(const ScanArgs &s)
     Lane<V> l;
     l.col = ((int64_t)blockIdx.x * kWave + lane_id()) * V;
     l.in = l.col < s.columns;
-    const int64_t q = l.in ? l.col : 0;
+    const int64_t q = l.in ? l.col : 0;   // (a lane without columns reads those of the first one and writes nothing)
     l.b = (int32_t)(q / s.dim);
     l.ch = (int32_t)(q - (int64_t)l.b * s.dim);
-    l.len = !l.in ? 0 : s.lengths ? min(max(s.lengths[l.b], 0), (int32_t)s.n_steps) : (int32_t)s.n_steps;
-#pragma unroll
-    for (int c = 0; c < V; ++c) l.gate[c] = G == kShared ? (l.ch + c) / s.channels : l.ch + c;
+    l.len = s.lengths ? min(max(s.lengths[l.b], 0), (int32_t)s.n_steps) : (int32_t)s.n_steps;
+    l.gate = G == kShared ? l.ch / s.channels : l.ch;
     return l;
 }
 
@@ -104,155 +118,279 @@ __device__ __forceinline__ void fold(const float *sums, int64_t columns, const L
 
 // One pass over the steps of a stretch in rounds: each wavefront takes kSteps steps into registers, finds what they do to a state
 // that enters them, (product of the gates, end from zero), the wavefronts tell each other, and each then computes its steps from the
-// state that really enters.  Everything is read once.  kBack: in descending order of time, the state being c[t] = a[t] (dh[t] + c[t + 1]),
-// what a gradient that enters behind step t becomes before it.  kSumsOnly: only what the whole stretch does, for the stretches behind it.
-template <typename TX, typename TA, int V, int G, bool kBack, bool kSumsOnly>
-__global__ void __launch_bounds__(kMaxWaves * kWave) scan_kernel(const ScanArgs s)
+// state that really enters.  Everything is read once, a round ahead.
+template <int V>
+struct Tell {
+    float v[2][kMaxWaves][2][V][kWave];   // [round in turn][wavefront][product, end]
+};
+
+// A round's exchange: `enter` is the state before the round and becomes the one behind it; returns in `mine` the one before the wavefront's block
+template <int V>
+__device__ __forceinline__ void exchange(Tell<V> &tell, int turn, int wave, int waves, const float (&p)[V], const float (&e)[V], float (&enter)[V], float (&mine)[V])
 {
-    __shared__ float tell[2][kMaxWaves][2][V][kWave];
+    const int lane = lane_id();
+#pragma unroll
+    for (int c = 0; c < V; ++c) {
+        tell.v[turn][wave][0][c][lane] = p[c];
+        tell.v[turn][wave][1][c][lane] = e[c];
+    }
+    // (two sets of places in turn: whoever writes the one of a round has passed the barrier behind the round before)
+    __syncthreads();
+    for (int w = 0; w < waves; ++w) {
+        if (w == wave)
+#pragma unroll
+            for (int c = 0; c < V; ++c) mine[c] = enter[c];
+#pragma unroll
+        for (int c = 0; c < V; ++c) enter[c] = passed(tell.v[turn][w][0][c][lane], enter[c]) + tell.v[turn][w][1][c][lane];
+    }
+}
+
+template <typename TX, typename TA, int V, int G>
+__global__ void __launch_bounds__(kMaxWaves * kWave) scan_fwd_kernel(const ScanArgs s)
+{
+    constexpr int VA = G == kEach ? V : 1;
+    __shared__ Tell<V> tell;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), waves = blockDim.x / kWave;
+    const Lane<V> l = lane_of<V, G>(s);
+    const int64_t t_lo = (int64_t)blockIdx.y * s.split_steps, t_hi = min(s.n_steps, t_lo + s.split_steps);
+    const TX *x = static_cast<const TX *>(s.x) + (int64_t)l.b * s.x_b + l.ch;
+    const TA *a = static_cast<const TA *>(s.a) + (G == kConst ? 0 : (int64_t)l.b * s.a_b) + l.gate;
+    TX *h = static_cast<TX *>(s.h) + l.col;
+    float a_const[V];
+    if (G == kConst) load_v<TA, V>(a, true, 0.0f, a_const);
+    float enter[V];
+#pragma unroll
+    for (int c = 0; c < V; ++c) enter[c] = 0.0f;
+    if (s.state && l.in) load_v<float, V>(s.state + l.col, true, 0.0f, enter);
+    fold<V>(s.sums, s.columns, l, 0, blockIdx.y, 1, enter);
+
+    const int64_t round_steps = (int64_t)waves * kSteps;
+    Block<TX, V> xb[2];
+    Block<TA, VA> ab[2];
+    auto load = [&](int i, int64_t t0) {
+        xb[i].load(x, s.x_t, t0, t_hi);
+        if (G != kConst) ab[i].load(a, s.a_t, t0, t_hi);
+    };
+    auto round = [&](int i, int64_t t0) {
+        const int there = (int)min(max(min((int64_t)l.len, t_hi) - t0, (int64_t)0), (int64_t)kSteps);
+        const bool all = __ballot(there < kSteps) == 0;
+        if (!all) {
+            xb[i].cut(there, 0.0f);
+            if (G != kConst) ab[i].cut(there, 1.0f);
+        }
+        auto gate = [&](int k, int c) { return G == kConst ? (k < there ? a_const[c] : 1.0f) : ab[i].get(k, c); };
+        float p[V], e[V], mine[V];
+#pragma unroll
+        for (int c = 0; c < V; ++c) {
+            p[c] = 1.0f, e[c] = 0.0f;
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) e[c] = __builtin_fmaf(gate(k, c), e[c], xb[i].get(k, c)), p[c] *= gate(k, c);
+        }
+        exchange<V>(tell, i, wave, waves, p, e, enter, mine);
+        if (t0 >= t_hi) return;
+        if (s.marks && l.in) store_v<float, V>(s.marks + t0 / kSteps * s.columns + l.col, mine);
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) {
+            float out[V];
+#pragma unroll
+            for (int c = 0; c < V; ++c) {
+                mine[c] = __builtin_fmaf(gate(k, c), mine[c], xb[i].get(k, c));
+                out[c] = k < there ? mine[c] : 0.0f;
+            }
+            if (t0 + k < t_hi && l.in) store_v<TX, V>(h + (t0 + k) * s.columns, out);
+        }
+    };
+    int64_t t0 = t_lo + wave * kSteps;
+    load(0, t0);
+    for (int64_t done = t_lo; done < t_hi; done += 2 * round_steps, t0 += 2 * round_steps) {
+        load(1, t0 + round_steps);
+        round(0, t0);
+        if (done + round_steps >= t_hi) break;
+        load(0, t0 + 2 * round_steps);
+        round(1, t0 + round_steps);
+    }
+    if (wave == 0 && blockIdx.y == gridDim.y - 1 && l.in) store_v<float, V>(s.last + l.col, enter);
+}
+
+// On the way back the state is c[t] = a[t] (dh[t] + c[t + 1]), what a gradient that enters behind step t becomes before it.
+template <typename TX, typename TA, int V, int G>
+__global__ void __launch_bounds__(kMaxWaves * kWave) scan_bwd_kernel(const ScanArgs s)
+{
+    constexpr int VA = G == kEach ? V : 1;
+    __shared__ Tell<V> tell;
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), waves = blockDim.x / kWave;
     const Lane<V> l = lane_of<V, G>(s);
     const int64_t t_lo = (int64_t)blockIdx.y * s.split_steps, t_hi = min(s.n_steps, t_lo + s.split_steps);
     const TX *x = static_cast<const TX *>(s.x) + (int64_t)l.b * s.x_b + l.ch;
-    const TA *a = static_cast<const TA *>(s.a) + (G == kConst ? 0 : (int64_t)l.b * s.a_b);
-    const TX *dh = static_cast<const TX *>(s.dh) + (kBack ? (int64_t)l.b * s.dh_b + l.ch : 0);
-    float a_const[V], d_const[V] = {};
-    if (G == kConst) load_gate<TA, V, kEach>(a, l.gate, l.in, a_const);
+    const TA *a = static_cast<const TA *>(s.a) + (G == kConst ? 0 : (int64_t)l.b * s.a_b) + l.gate;
+    const TX *dh = static_cast<const TX *>(s.dh) + (int64_t)l.b * s.dh_b + l.ch;
+    TX *dx = static_cast<TX *>(s.dx) + l.col;
+    TA *da = static_cast<TA *>(s.da);
+    float a_const[V], d_const[V];
+    if (G == kConst) load_v<TA, V>(a, true, 0.0f, a_const);
+    float enter[V];
+#pragma unroll
+    for (int c = 0; c < V; ++c) enter[c] = d_const[c] = 0.0f;
+    if (s.d_last && l.in) load_v<float, V>(s.d_last + l.col, true, 0.0f, enter);
+    fold<V>(s.sums, s.columns, l, gridDim.y - 1, blockIdx.y, -1, enter);
 
-    float enter[V], whole[V];   // the state that enters a round; kSumsOnly: product of the gates so far, too
-#pragma unroll
-    for (int c = 0; c < V; ++c) enter[c] = 0.0f, whole[c] = 1.0f;
-    if (!kSumsOnly) {
-        if (kBack) {
-            if (s.d_last && l.in) load_v<float, V>(s.d_last + l.col, true, 0.0f, enter);
-            fold<V>(s.sums, s.columns, l, gridDim.y - 1, blockIdx.y, -1, enter);
-        } else {
-            if (s.state && l.in) load_v<float, V>(s.state + l.col, true, 0.0f, enter);
-            fold<V>(s.sums, s.columns, l, 0, blockIdx.y, 1, enter);
-        }
-    }
-    const int64_t rounds = (t_hi - t_lo + (int64_t)waves * kSteps - 1) / ((int64_t)waves * kSteps);
+    const int64_t round_steps = (int64_t)waves * kSteps;
+    const int64_t rounds = (t_hi - t_lo + round_steps - 1) / round_steps;
+    Block<TX, V> xb, gb;
+    Block<TA, VA> ab;
+    float before[kSteps][V];
     for (int64_t round = 0; round < rounds; ++round) {
-        // a wavefront's block in the order in which the state passes: the last block first on the way back
-        const int64_t block = kBack ? rounds * waves - 1 - (round * waves + wave) : round * waves + wave;
-        const int64_t t0 = t_lo + block * kSteps;
-        float xv[kSteps][V], av[kSteps][V], gv[kBack ? kSteps : 1][V];
-#pragma unroll
-        for (int k = 0; k < kSteps; ++k) {
-            const int64_t t = t0 + k;
-            const bool there = t < t_hi && t < l.len;
-            if (!(kBack && kSumsOnly)) load_v<TX, V>(x + t * s.x_t, there, 0.0f, xv[k]);
-            if (kBack) load_v<TX, V>(dh + t * s.dh_t, there, 0.0f, gv[k]);
-            if (G == kConst) {
-#pragma unroll
-                for (int c = 0; c < V; ++c) av[k][c] = there ? a_const[c] : 1.0f;
-            } else {
-                load_gate<TA, V, G>(a + t * s.a_t, l.gate, there, av[k]);
-            }
+        // the last block first
+        const int64_t t0 = t_lo + (rounds * waves - 1 - (round * waves + wave)) * kSteps;
+        gb.load(dh, s.dh_t, t0, t_hi);
+        if (G != kConst) ab.load(a, s.a_t, t0, t_hi);
+        xb.load(x, s.x_t, t0, t_hi);
+        // (columns that are not there: as behind their end)
+        const int there = l.in ? (int)min(max(min((int64_t)l.len, t_hi) - t0, (int64_t)0), (int64_t)kSteps) : 0;
+        if (__ballot(there < kSteps) != 0) {
+            gb.cut(there, 0.0f);
+            xb.cut(there, 0.0f);
+            if (G != kConst) ab.cut(there, 1.0f);
         }
-        float p[V], e[V];
+        auto gate = [&](int k, int c) { return G == kConst ? (k < there ? a_const[c] : 1.0f) : ab.get(k, c); };
+        if (l.in && t0 < t_hi) load_v<float, V>(s.marks + t0 / kSteps * s.columns + l.col, true, 0.0f, before[0]);
+        else
+#pragma unroll
+            for (int c = 0; c < V; ++c) before[0][c] = 0.0f;
+        float p[V], e[V], mine[V];
 #pragma unroll
         for (int c = 0; c < V; ++c) {
             p[c] = 1.0f, e[c] = 0.0f;
-            if (kBack) {
 #pragma unroll
-                for (int k = kSteps - 1; k >= 0; --k) e[c] = av[k][c] * (gv[k][c] + e[c]), p[c] *= av[k][c];
-            } else {
-#pragma unroll
-                for (int k = 0; k < kSteps; ++k) e[c] = av[k][c] * e[c] + xv[k][c], p[c] *= av[k][c];
-            }
-            tell[round & 1][wave][0][c][lane] = p[c];
-            tell[round & 1][wave][1][c][lane] = e[c];
+            for (int k = kSteps - 1; k >= 0; --k) e[c] = gate(k, c) * (gb.get(k, c) + e[c]), p[c] *= gate(k, c);
         }
-        // (two sets of places in turn: whoever writes the one of a round has passed the barrier behind the round before)
-        __syncthreads();
-        float mine[V];
-        for (int w = 0; w < waves; ++w) {
-            if (w == wave)
+        // the states before each step, again from the kept one
 #pragma unroll
-                for (int c = 0; c < V; ++c) mine[c] = enter[c];
+        for (int k = 1; k < kSteps; ++k)
+#pragma unroll
+            for (int c = 0; c < V; ++c) before[k][c] = __builtin_fmaf(gate(k - 1, c), before[k - 1][c], xb.get(k - 1, c));
+        exchange<V>(tell, (int)(round & 1), wave, waves, p, e, enter, mine);
+        if (t0 >= t_hi) continue;
+#pragma unroll
+        for (int k = kSteps - 1; k >= 0; --k) {
+            const int64_t t = t0 + k;
+            float g[V], d[V];
 #pragma unroll
             for (int c = 0; c < V; ++c) {
-                const float pw = tell[round & 1][w][0][c][lane];
-                enter[c] = passed(pw, enter[c]) + tell[round & 1][w][1][c][lane];
-                if (kSumsOnly) whole[c] *= pw;
+                const float all = gb.get(k, c) + mine[c];
+                g[c] = k < there ? all : 0.0f;   // (behind a sequence's end the gradient of its last state passes through)
+                d[c] = k < there ? all * before[k][c] : 0.0f;
+                mine[c] = gate(k, c) * all;
+                if (G == kConst) d_const[c] += d[c];
             }
-        }
-        if (kSumsOnly || t0 >= t_hi) continue;
-        if (!kBack) {
-            TX *h = static_cast<TX *>(s.h);
-            if (s.marks && l.in) store_v<float, V>(s.marks + t0 / kSteps * s.columns + l.col, mine);
-#pragma unroll
-            for (int k = 0; k < kSteps; ++k) {
-                float out[V];
-#pragma unroll
-                for (int c = 0; c < V; ++c) {
-                    mine[c] = av[k][c] * mine[c] + xv[k][c];
-                    out[c] = t0 + k < l.len ? mine[c] : 0.0f;
-                }
-                if (t0 + k < t_hi && l.in) store_v<TX, V>(h + (t0 + k) * s.columns + l.col, out);
-            }
-        } else {
-            // the states before each step, again from the kept one
-            float before[kSteps][V];
-            if (l.in) load_v<float, V>(s.marks + t0 / kSteps * s.columns + l.col, true, 0.0f, before[0]);
-            else
-#pragma unroll
-                for (int c = 0; c < V; ++c) before[0][c] = 0.0f;
-#pragma unroll
-            for (int k = 1; k < kSteps; ++k)
-#pragma unroll
-                for (int c = 0; c < V; ++c) before[k][c] = av[k - 1][c] * before[k - 1][c] + xv[k - 1][c];
-            TX *dx = static_cast<TX *>(s.dx);
-            TA *da = static_cast<TA *>(s.da);
-#pragma unroll
-            for (int k = kSteps - 1; k >= 0; --k) {
-                const int64_t t = t0 + k;
-                float g[V], d[V];
-#pragma unroll
-                for (int c = 0; c < V; ++c) {
-                    const float all = gv[k][c] + mine[c];
-                    g[c] = t < l.len ? all : 0.0f;   // (behind a sequence's end the gradient of its last state passes through)
-                    d[c] = t < l.len ? all * before[k][c] : 0.0f;
-                    mine[c] = av[k][c] * all;
-                    if (G == kConst) d_const[c] += d[c];
-                }
-                const bool write = t < t_hi && l.in;
-                if (write) store_v<TX, V>(dx + t * s.columns + l.col, g);
-                if (G == kEach && write) store_v<TA, V>(da + t * s.columns + l.col, d);
-                if (G == kShared) {
-                    float sum = d[0];
-                    if (V == 2 && s.seg_lanes) sum += d[1];
-                    for (int m = 1; m < s.seg_lanes; m *= 2) sum += __shfl_xor(sum, m);
-                    if (write) {
-                        // a gate's channels within the lanes: its gradient; else parts of it, to be joined
-                        const int64_t at = (t * (s.columns / s.dim) + l.b) * (int64_t)s.parts;
-                        if (s.da_part == nullptr) {
-                            if (lane % s.seg_lanes == 0) da[at + l.gate[0]] = (TA)sum;
-                        } else if (s.seg_lanes) {
-                            if (lane % s.seg_lanes == 0) s.da_part[at + l.ch / (V * s.seg_lanes)] = sum;
-                        } else {
-                            store_v<float, V>(s.da_part + at + l.ch, d);
-                        }
+            const bool write = t < t_hi && l.in;
+            if (write) store_v<TX, V>(dx + t * s.columns, g);
+            if (G == kEach && write) store_v<TA, V>(da + t * s.columns + l.col, d);
+            if (G == kShared) {
+                float sum = d[0];
+                if (V == 2 && s.seg_lanes) sum += d[1];
+                for (int m = 1; m < s.seg_lanes; m *= 2) sum += __shfl_xor(sum, m);
+                if (write) {
+                    // a gate's channels within the lanes: its gradient; else parts of it, to be joined
+                    const int64_t at = (t * (s.columns / s.dim) + l.b) * (int64_t)s.parts;
+                    if (s.da_part == nullptr) {
+                        if (lane % s.seg_lanes == 0) da[at + l.gate] = (TA)sum;
+                    } else if (s.seg_lanes) {
+                        if (lane % s.seg_lanes == 0) s.da_part[at + l.ch / (V * s.seg_lanes)] = sum;
+                    } else {
+                        store_v<float, V>(s.da_part + at + l.ch, d);
                     }
                 }
             }
         }
     }
     if (!l.in) return;
-    if (kSumsOnly) {
-        if (wave == 0) {
-            store_v<float, V>(s.sums + (int64_t)(2 * blockIdx.y) * s.columns + l.col, whole);
-            store_v<float, V>(s.sums + (int64_t)(2 * blockIdx.y + 1) * s.columns + l.col, enter);
-        }
-        return;
-    }
-    if (!kBack) {
-        if (wave == 0 && blockIdx.y == gridDim.y - 1) store_v<float, V>(s.last + l.col, enter);
-        return;
-    }
     if (wave == 0 && blockIdx.y == 0 && s.d_state) store_v<float, V>(s.d_state + l.col, enter);
     if (G == kConst) store_v<float, V>(s.da_part + ((int64_t)blockIdx.y * waves + wave) * s.columns + l.col, d_const);
+}
+
+// What a whole stretch does, for the stretches that are computed from it: the product of its gates and its end from zero, forwards or backwards.  Each
+// wavefront takes every waves-th block, from the stretch's other end to where the pass proper begins, so that what that pass reads first was
+// read last; the wavefronts' blocks of a round are joined as they come, in the order of time.
+template <typename TX, typename TA, int V, int G, bool kBack>
+__global__ void __launch_bounds__(kMaxWaves * kWave) scan_sums_kernel(const ScanArgs s)
+{
+    constexpr int VA = G == kEach ? V : 1;
+    __shared__ Tell<V> tell;
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), waves = blockDim.x / kWave;
+    const Lane<V> l = lane_of<V, G>(s);
+    const int64_t t_lo = (int64_t)blockIdx.y * s.split_steps, t_hi = min(s.n_steps, t_lo + s.split_steps);
+    const TX *x = kBack ? static_cast<const TX *>(s.dh) + (int64_t)l.b * s.dh_b + l.ch : static_cast<const TX *>(s.x) + (int64_t)l.b * s.x_b + l.ch;
+    const int64_t x_t = kBack ? s.dh_t : s.x_t;
+    const TA *a = static_cast<const TA *>(s.a) + (G == kConst ? 0 : (int64_t)l.b * s.a_b) + l.gate;
+    float a_const[V];
+    if (G == kConst) load_v<TA, V>(a, true, 0.0f, a_const);
+    const int64_t round_steps = (int64_t)waves * kSteps;
+    const int64_t rounds = (t_hi - t_lo + round_steps - 1) / round_steps;
+    float product[V], end[V];
+#pragma unroll
+    for (int c = 0; c < V; ++c) product[c] = 1.0f, end[c] = 0.0f;
+    Block<TX, V> xb[2];
+    Block<TA, VA> ab[2];
+    auto block_of = [&](int64_t round) { return t_lo + (kBack ? round : rounds - 1 - round) * round_steps + wave * kSteps; };
+    auto load = [&](int i, int64_t round) {
+        const int64_t t0 = block_of(round < rounds ? round : rounds - 1);
+        xb[i].load(x, x_t, t0, t_hi);
+        if (G != kConst) ab[i].load(a, s.a_t, t0, t_hi);
+    };
+    auto take = [&](int i, int64_t round) {
+        const int64_t t0 = block_of(round);
+        const int there = (int)min(max(min((int64_t)l.len, t_hi) - t0, (int64_t)0), (int64_t)kSteps);
+        if (__ballot(there < kSteps) != 0) {
+            xb[i].cut(there, 0.0f);
+            if (G != kConst) ab[i].cut(there, 1.0f);
+        }
+        auto gate = [&](int k, int c) { return G == kConst ? (k < there ? a_const[c] : 1.0f) : ab[i].get(k, c); };
+#pragma unroll
+        for (int c = 0; c < V; ++c) {
+            float p = 1.0f, e = 0.0f;
+#pragma unroll
+            for (int j = 0; j < kSteps; ++j) {
+                const int k = kBack ? kSteps - 1 - j : j;
+                e = kBack ? gate(k, c) * (xb[i].get(k, c) + e) : __builtin_fmaf(gate(k, c), e, xb[i].get(k, c));
+                p *= gate(k, c);
+            }
+            tell.v[i][wave][0][c][lane] = p;
+            tell.v[i][wave][1][c][lane] = e;
+        }
+        __syncthreads();
+        if (wave != 0) return;
+        // the round's blocks, then what was found before, which the state passes afterwards
+        float rp[V], re[V];
+#pragma unroll
+        for (int c = 0; c < V; ++c) rp[c] = 1.0f, re[c] = 0.0f;
+        for (int j = 0; j < waves; ++j) {
+            const int w = kBack ? waves - 1 - j : j;
+#pragma unroll
+            for (int c = 0; c < V; ++c) {
+                const float pw = tell.v[i][w][0][c][lane];
+                re[c] = passed(pw, re[c]) + tell.v[i][w][1][c][lane];
+                rp[c] *= pw;
+            }
+        }
+#pragma unroll
+        for (int c = 0; c < V; ++c) {
+            end[c] = passed(product[c], re[c]) + end[c];
+            product[c] *= rp[c];
+        }
+    };
+    load(0, 0);
+    for (int64_t round = 0; round < rounds; round += 2) {
+        load(1, round + 1);
+        take(0, round);
+        if (round + 1 >= rounds) break;
+        load(0, round + 2);
+        take(1, round + 1);
+    }
+    if (wave == 0 && l.in) {
+        store_v<float, V>(s.sums + (int64_t)(2 * blockIdx.y) * s.columns + l.col, product);
+        store_v<float, V>(s.sums + (int64_t)(2 * blockIdx.y + 1) * s.columns + l.col, end);
+    }
 }
 
 // One step: nothing to join
@@ -264,17 +402,24 @@ __global__ void __launch_bounds__(kBlock) scan_one_kernel(const ScanArgs s)
     if (l.col >= s.columns) return;
     l.b = (int32_t)(l.col / s.dim);
     l.ch = (int32_t)(l.col - (int64_t)l.b * s.dim);
-#pragma unroll
-    for (int c = 0; c < V; ++c) l.gate[c] = G == kShared ? (l.ch + c) / s.channels : l.ch + c;
+    l.gate = G == kShared ? l.ch / s.channels : l.ch;
     const bool there = !s.lengths || s.lengths[l.b] > 0;
     float x[V], a[V], h[V], out[V];
     load_v<TX, V>(static_cast<const TX *>(s.x) + (int64_t)l.b * s.x_b + l.ch, there, 0.0f, x);
-    load_gate<TA, V, G == kShared ? kShared : kEach>(static_cast<const TA *>(s.a) + (G == kConst ? 0 : (int64_t)l.b * s.a_b), l.gate, there, a);
+    const TA *gate = static_cast<const TA *>(s.a) + (G == kConst ? 0 : (int64_t)l.b * s.a_b) + l.gate;
+    if (G == kShared) {
+        float one[1];
+        load_v<TA, 1>(gate, there, 1.0f, one);
+#pragma unroll
+        for (int c = 0; c < V; ++c) a[c] = one[0];
+    } else {
+        load_v<TA, V>(gate, there, 1.0f, a);
+    }
     load_v<float, V>(s.state + l.col, s.state != nullptr, 0.0f, h);
     if (s.marks) store_v<float, V>(s.marks + l.col, h);
 #pragma unroll
     for (int c = 0; c < V; ++c) {
-        h[c] = a[c] * h[c] + x[c];
+        h[c] = __builtin_fmaf(a[c], h[c], x[c]);
         out[c] = there ? h[c] : 0.0f;
     }
     store_v<TX, V>(static_cast<TX *>(s.h) + l.col, out);
@@ -321,7 +466,8 @@ struct Plan {
 Plan plan_of(int64_t n_steps, int64_t batch, int32_t dim, int32_t groups, int32_t dtype, bool pairs)
 {
     Plan p;
-    p.v = dtype != BMTK_F32 && dim % 2 == 0 && pairs ? 2 : 1;
+    const int channels = groups > 0 ? dim / groups : 1;
+    p.v = dtype != BMTK_F32 && dim % 2 == 0 && pairs && (groups == 0 || groups == dim || channels % 2 == 0) ? 2 : 1;
     p.tiles = div_up(batch * dim, kWave * p.v);
     int64_t w = div_up(n_steps, kSteps);
     p.waves = (int)(w < kMaxWaves ? w : kMaxWaves);
@@ -334,7 +480,7 @@ Plan plan_of(int64_t n_steps, int64_t batch, int32_t dim, int32_t groups, int32_
     p.splits = div_up(n_steps, p.split_steps);
     p.seg_lanes = p.parts = 0;
     if (groups > 0 && groups != dim) {
-        const int channels = dim / groups, seg = gcd(channels, kWave * p.v);
+        const int seg = gcd(channels, kWave * p.v);
         p.seg_lanes = seg >= p.v ? seg / p.v : 0;
         p.parts = p.seg_lanes ? dim / seg : dim;
     }
@@ -370,12 +516,13 @@ extern "C" int64_t bmtk_gated_scan_workspace_bytes(int64_t n_steps, int64_t batc
     return most * (int64_t)sizeof(float);
 }
 
-#define BMTK_SCAN_LAUNCH(BACK, SUMS)                                                                                                      \
-    do {                                                                                                                                  \
-        if (groups == 0) hipLaunchKernelGGL((scan_kernel<TX, TA, V, kConst, BACK, SUMS>), grid, dim3(p.waves *kWave), 0, st, s);           \
-        else if (groups == dim) hipLaunchKernelGGL((scan_kernel<TX, TA, V, kEach, BACK, SUMS>), grid, dim3(p.waves *kWave), 0, st, s);     \
-        else hipLaunchKernelGGL((scan_kernel<TX, TA, V, kShared, BACK, SUMS>), grid, dim3(p.waves *kWave), 0, st, s);                      \
+#define BMTK_SCAN_LAUNCH(KERNEL, ...)                                                                                                         \
+    do {                                                                                                                                      \
+        if (groups == 0) hipLaunchKernelGGL((KERNEL<TX, TA, V, kConst __VA_ARGS__>), grid, dim3(p.waves *kWave), 0, st, s);                    \
+        else if (groups == dim) hipLaunchKernelGGL((KERNEL<TX, TA, V, kEach __VA_ARGS__>), grid, dim3(p.waves *kWave), 0, st, s);              \
+        else hipLaunchKernelGGL((KERNEL<TX, TA, V, kShared __VA_ARGS__>), grid, dim3(p.waves *kWave), 0, st, s);                               \
     } while (0)
+#define BMTK_COMMA ,
 
 namespace {
 
@@ -391,8 +538,8 @@ void launch_fwd(const ScanArgs &s, const Plan &p, int groups, hipStream_t st)
         return;
     }
     dim3 grid((unsigned)p.tiles, (unsigned)p.splits);
-    if (p.splits > 1) BMTK_SCAN_LAUNCH(false, true);
-    BMTK_SCAN_LAUNCH(false, false);
+    if (p.splits > 1) BMTK_SCAN_LAUNCH(scan_sums_kernel, BMTK_COMMA false);
+    BMTK_SCAN_LAUNCH(scan_fwd_kernel, );
 }
 
 template <typename TX, typename TA, int V>
@@ -401,8 +548,8 @@ void launch_bwd(ScanArgs s, const Plan &p, int groups, hipStream_t st)
     const int dim = s.dim;
     const int64_t batch = s.columns / dim;
     dim3 grid((unsigned)p.tiles, (unsigned)p.splits);
-    if (p.splits > 1) BMTK_SCAN_LAUNCH(true, true);
-    BMTK_SCAN_LAUNCH(true, false);
+    if (p.splits > 1) BMTK_SCAN_LAUNCH(scan_sums_kernel, BMTK_COMMA true);
+    BMTK_SCAN_LAUNCH(scan_bwd_kernel, );
     if (groups == 0)
         hipLaunchKernelGGL((scan_join_const_kernel<TA>), dim3((unsigned)div_up(dim, kWave)), dim3(kBlock), 0, st, s.da_part, p.splits * p.waves * batch, dim,
                            (TA *)s.da);
