@@ -22,8 +22,9 @@ struct ScanArgs {
     int64_t n_steps, columns, split_steps;
     int64_t x_t, x_b, a_t, a_b, dh_t, dh_b;   // strides of what is read, in elements; what is written is contiguous
     int32_t dim, channels;      // channels of a gate
-    int32_t seg_lanes;          // lanes whose part of a gate's gradient is summed at once (0: nothing is summed)
-    int32_t groups, parts;      // gates of a step and sequence; entries of da_part of a step and sequence
+    int32_t seg_lanes;          // lanes whose part of a gate's gradient is summed at once
+    int32_t parts;              // such sums of a step and sequence
+    int64_t sequences;
 };
 
 template <typename T, int V>
@@ -55,15 +56,17 @@ enum { kConst = 0, kEach = 1, kShared = 2 };
 template <typename T, int V>
 struct Block {
     Pack<T, V> v[kSteps];
-    // (behind `end` the last step again: nothing outside is read, and nothing depends on a lane)
-    __device__ __forceinline__ void load(const T *p, int64_t stride, int64_t t0, int64_t end)
+    // `last`: the last step that one of the wavefront's sequences has (or step 0); behind it that one again: nothing outside is read, there are no
+    // branches, and those steps are cut
+    __device__ __forceinline__ void load(const T *p, int64_t stride, int64_t t0, int64_t last)
     {
-        if (t0 + kSteps <= end) {
+        int64_t at = min(t0, last);
+        const T *row = p + at * stride;
 #pragma unroll
-            for (int k = 0; k < kSteps; ++k) v[k] = *reinterpret_cast<const Pack<T, V> *>(p + (t0 + k) * stride);
-        } else {
-#pragma unroll
-            for (int k = 0; k < kSteps; ++k) v[k] = *reinterpret_cast<const Pack<T, V> *>(p + min(t0 + k, end - 1) * stride);
+        for (int k = 0; k < kSteps; ++k) {
+            v[k] = *reinterpret_cast<const Pack<T, V> *>(row);
+            row += at < last ? stride : 0;
+            ++at;
         }
     }
     // steps from `there` on are as if they were `other`
@@ -82,7 +85,7 @@ template <int V>
 struct Lane {
     int64_t col;
     bool in;
-    int32_t b, ch, len;
+    int32_t b, ch, len, longest;   // longest: of the wavefront's sequences
     int gate;
 };
 template <int V, int G>
@@ -95,6 +98,12 @@ __device__ __forceinline__ Lane<V> lane_of(const ScanArgs &s)
     l.b = (int32_t)(q / s.dim);
     l.ch = (int32_t)(q - (int64_t)l.b * s.dim);
     l.len = s.lengths ? min(max(s.lengths[l.b], 0), (int32_t)s.n_steps) : (int32_t)s.n_steps;
+    l.longest = l.len;
+    if (s.lengths) {
+#pragma unroll
+        for (int m = kWave / 2; m > 0; m /= 2) l.longest = max(l.longest, __shfl_xor(l.longest, m));
+    }
+    l.longest = __builtin_amdgcn_readfirstlane(l.longest);
     l.gate = G == kShared ? l.ch / s.channels : l.ch;
     return l;
 }
@@ -167,9 +176,10 @@ __global__ void __launch_bounds__(kMaxWaves * kWave) scan_fwd_kernel(const ScanA
     const int64_t round_steps = (int64_t)waves * kSteps;
     Block<TX, V> xb[2];
     Block<TA, VA> ab[2];
+    const int64_t last = max(min(t_hi, (int64_t)l.longest) - 1, (int64_t)0);
     auto load = [&](int i, int64_t t0) {
-        xb[i].load(x, s.x_t, t0, t_hi);
-        if (G != kConst) ab[i].load(a, s.a_t, t0, t_hi);
+        xb[i].load(x, s.x_t, t0, last);
+        if (G != kConst) ab[i].load(a, s.a_t, t0, last);
     };
     auto round = [&](int i, int64_t t0) {
         const int there = (int)min(max(min((int64_t)l.len, t_hi) - t0, (int64_t)0), (int64_t)kSteps);
@@ -212,9 +222,33 @@ __global__ void __launch_bounds__(kMaxWaves * kWave) scan_fwd_kernel(const ScanA
     if (wave == 0 && blockIdx.y == gridDim.y - 1 && l.in) store_v<float, V>(s.last + l.col, enter);
 }
 
+// Sum over `lanes` neighbouring lanes (a power of two, the same for all), in each of them.  Moves within the vector unit: a sum over 32 lanes by
+// moves through LDS (__shfl_xor) takes 35 of a backward pass's 130 us (4,096 x 8 x 2,048, a gate per 64 channels).
+template <int kCtrl>
+__device__ __forceinline__ float plus_moved(float v)
+{
+    return v + __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), kCtrl, 0xF, 0xF, true));
+}
+__device__ __forceinline__ float sum_lanes(float v, int lanes)
+{
+    if (lanes > 1) v = plus_moved<0xB1>(v);    // neighbours of two: quad_perm 1, 0, 3, 2
+    if (lanes > 2) v = plus_moved<0x4E>(v);    // pairs of four: quad_perm 2, 3, 0, 1
+    if (lanes > 4) v = plus_moved<0x141>(v);   // fours of eight (each holds one value): row_half_mirror
+    if (lanes > 8) v = plus_moved<0x140>(v);   // eights of sixteen: row_mirror
+    if (lanes > 16) {
+        const auto r = __builtin_amdgcn_permlane16_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    if (lanes > 32) {
+        const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+        v = __uint_as_float(r[0]) + __uint_as_float(r[1]);
+    }
+    return v;
+}
+
 // On the way back the state is c[t] = a[t] (dh[t] + c[t + 1]), what a gradient that enters behind step t becomes before it.
 template <typename TX, typename TA, int V, int G>
-__global__ void __launch_bounds__(kMaxWaves * kWave) scan_bwd_kernel(const ScanArgs s)
+__global__ void __launch_bounds__(kMaxWaves * kWave, 4) scan_bwd_kernel(const ScanArgs s)
 {
     constexpr int VA = G == kEach ? V : 1;
     __shared__ Tell<V> tell;
@@ -235,16 +269,16 @@ __global__ void __launch_bounds__(kMaxWaves * kWave) scan_bwd_kernel(const ScanA
     fold<V>(s.sums, s.columns, l, gridDim.y - 1, blockIdx.y, -1, enter);
 
     const int64_t round_steps = (int64_t)waves * kSteps;
-    const int64_t rounds = (t_hi - t_lo + round_steps - 1) / round_steps;
+    const int64_t rounds = (t_hi - t_lo + round_steps - 1) / round_steps, last = max(min(t_hi, (int64_t)l.longest) - 1, (int64_t)0);
     Block<TX, V> xb, gb;
     Block<TA, VA> ab;
     float before[kSteps][V];
     for (int64_t round = 0; round < rounds; ++round) {
         // the last block first
         const int64_t t0 = t_lo + (rounds * waves - 1 - (round * waves + wave)) * kSteps;
-        gb.load(dh, s.dh_t, t0, t_hi);
-        if (G != kConst) ab.load(a, s.a_t, t0, t_hi);
-        xb.load(x, s.x_t, t0, t_hi);
+        gb.load(dh, s.dh_t, t0, last);
+        if (G != kConst) ab.load(a, s.a_t, t0, last);
+        xb.load(x, s.x_t, t0, last);
         // (columns that are not there: as behind their end)
         const int there = l.in ? (int)min(max(min((int64_t)l.len, t_hi) - t0, (int64_t)0), (int64_t)kSteps) : 0;
         if (__ballot(there < kSteps) != 0) {
@@ -287,26 +321,29 @@ __global__ void __launch_bounds__(kMaxWaves * kWave) scan_bwd_kernel(const ScanA
             if (write) store_v<TX, V>(dx + t * s.columns, g);
             if (G == kEach && write) store_v<TA, V>(da + t * s.columns + l.col, d);
             if (G == kShared) {
-                float sum = d[0];
-                if (V == 2 && s.seg_lanes) sum += d[1];
-                for (int m = 1; m < s.seg_lanes; m *= 2) sum += __shfl_xor(sum, m);
-                if (write) {
+                const float sum = sum_lanes(V == 2 ? d[0] + d[V - 1] : d[0], s.seg_lanes);
+                if (write && (lane & (s.seg_lanes - 1)) == 0) {
                     // a gate's channels within the lanes: its gradient; else parts of it, to be joined
-                    const int64_t at = (t * (s.columns / s.dim) + l.b) * (int64_t)s.parts;
-                    if (s.da_part == nullptr) {
-                        if (lane % s.seg_lanes == 0) da[at + l.gate] = (TA)sum;
-                    } else if (s.seg_lanes) {
-                        if (lane % s.seg_lanes == 0) s.da_part[at + l.ch / (V * s.seg_lanes)] = sum;
-                    } else {
-                        store_v<float, V>(s.da_part + at + l.ch, d);
-                    }
+                    const int64_t at = (t * s.sequences + l.b) * s.parts;
+                    if (s.da_part) s.da_part[at + l.ch / (V * s.seg_lanes)] = sum;
+                    else da[at + l.gate] = (TA)sum;
                 }
             }
         }
     }
-    if (!l.in) return;
-    if (wave == 0 && blockIdx.y == 0 && s.d_state) store_v<float, V>(s.d_state + l.col, enter);
-    if (G == kConst) store_v<float, V>(s.da_part + ((int64_t)blockIdx.y * waves + wave) * s.columns + l.col, d_const);
+    if (l.in && wave == 0 && blockIdx.y == 0 && s.d_state) store_v<float, V>(s.d_state + l.col, enter);
+    if (G == kConst) {
+        // the wavefronts' sums together, in order
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < V; ++c) tell.v[0][wave][0][c][lane] = d_const[c];
+        __syncthreads();
+        if (wave != 0 || !l.in) return;
+        for (int w = 1; w < waves; ++w)
+#pragma unroll
+            for (int c = 0; c < V; ++c) d_const[c] += tell.v[0][w][0][c][lane];
+        store_v<float, V>(s.da_part + (int64_t)blockIdx.y * s.columns + l.col, d_const);
+    }
 }
 
 // What a whole stretch does, for the stretches that are computed from it: the product of its gates and its end from zero, forwards or backwards.  Each
@@ -319,7 +356,9 @@ __global__ void __launch_bounds__(kMaxWaves * kWave) scan_sums_kernel(const Scan
     __shared__ Tell<V> tell;
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), waves = blockDim.x / kWave;
     const Lane<V> l = lane_of<V, G>(s);
-    const int64_t t_lo = (int64_t)blockIdx.y * s.split_steps, t_hi = min(s.n_steps, t_lo + s.split_steps);
+    // (stretch blockIdx.y, on the way back + 1: what the last one to be passed does, nobody asks)
+    const int stretch = blockIdx.y + (kBack ? 1 : 0);
+    const int64_t t_lo = (int64_t)stretch * s.split_steps, t_hi = min(s.n_steps, t_lo + s.split_steps);
     const TX *x = kBack ? static_cast<const TX *>(s.dh) + (int64_t)l.b * s.dh_b + l.ch : static_cast<const TX *>(s.x) + (int64_t)l.b * s.x_b + l.ch;
     const int64_t x_t = kBack ? s.dh_t : s.x_t;
     const TA *a = static_cast<const TA *>(s.a) + (G == kConst ? 0 : (int64_t)l.b * s.a_b) + l.gate;
@@ -327,6 +366,7 @@ __global__ void __launch_bounds__(kMaxWaves * kWave) scan_sums_kernel(const Scan
     if (G == kConst) load_v<TA, V>(a, true, 0.0f, a_const);
     const int64_t round_steps = (int64_t)waves * kSteps;
     const int64_t rounds = (t_hi - t_lo + round_steps - 1) / round_steps;
+    const int64_t last = max(min(t_hi, (int64_t)l.longest) - 1, (int64_t)0);
     float product[V], end[V];
 #pragma unroll
     for (int c = 0; c < V; ++c) product[c] = 1.0f, end[c] = 0.0f;
@@ -335,8 +375,8 @@ __global__ void __launch_bounds__(kMaxWaves * kWave) scan_sums_kernel(const Scan
     auto block_of = [&](int64_t round) { return t_lo + (kBack ? round : rounds - 1 - round) * round_steps + wave * kSteps; };
     auto load = [&](int i, int64_t round) {
         const int64_t t0 = block_of(round < rounds ? round : rounds - 1);
-        xb[i].load(x, x_t, t0, t_hi);
-        if (G != kConst) ab[i].load(a, s.a_t, t0, t_hi);
+        xb[i].load(x, x_t, t0, last);
+        if (G != kConst) ab[i].load(a, s.a_t, t0, last);
     };
     auto take = [&](int i, int64_t round) {
         const int64_t t0 = block_of(round);
@@ -388,8 +428,8 @@ __global__ void __launch_bounds__(kMaxWaves * kWave) scan_sums_kernel(const Scan
         take(1, round + 1);
     }
     if (wave == 0 && l.in) {
-        store_v<float, V>(s.sums + (int64_t)(2 * blockIdx.y) * s.columns + l.col, product);
-        store_v<float, V>(s.sums + (int64_t)(2 * blockIdx.y + 1) * s.columns + l.col, end);
+        store_v<float, V>(s.sums + (int64_t)(2 * stretch) * s.columns + l.col, product);
+        store_v<float, V>(s.sums + (int64_t)(2 * stretch + 1) * s.columns + l.col, end);
     }
 }
 
@@ -426,20 +466,28 @@ __global__ void __launch_bounds__(kBlock) scan_one_kernel(const ScanArgs s)
     store_v<float, V>(s.last + l.col, h);
 }
 
-// Gradient of one decay per channel: its parts by stretch, wavefront and sequence, in order
+// Gradient of one decay per channel: its parts by stretch and sequence, every sixteenth by one wavefront, in order
+constexpr int kJoinWaves = 16;
 template <typename TA>
-__global__ void __launch_bounds__(kBlock) scan_join_const_kernel(const float *__restrict__ part, int64_t parts, int dim, TA *__restrict__ da)
+__global__ void __launch_bounds__(kJoinWaves * kWave) scan_join_const_kernel(const float *__restrict__ part, int64_t parts, int dim, TA *__restrict__ da)
 {
-    __shared__ float sum[kBlock];
+    __shared__ float sum[kJoinWaves][kWave];
     const int lane = lane_id(), wave = threadIdx.x / kWave;
     const int ch = blockIdx.x * kWave + lane;
+    const float *p = part + (ch < dim ? ch : 0);
     float v = 0.0f;
-    if (ch < dim)
-        for (int64_t k = wave; k < parts; k += kBlock / kWave) v += part[k * dim + ch];
-    sum[threadIdx.x] = v;
+    int64_t k = wave;
+    for (; k + 3 * kJoinWaves < parts; k += 4 * kJoinWaves) {
+        float w[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) w[u] = p[(k + u * kJoinWaves) * dim];
+        v += (w[0] + w[1]) + (w[2] + w[3]);
+    }
+    for (; k < parts; k += kJoinWaves) v += p[k * dim];
+    sum[wave][lane] = v;
     __syncthreads();
     if (wave == 0 && ch < dim) {
-        for (int w = 1; w < kBlock / kWave; ++w) v += sum[w * kWave + lane];
+        for (int w = 1; w < kJoinWaves; ++w) v += sum[w][lane];
         da[ch] = (TA)v;
     }
 }
@@ -457,6 +505,7 @@ __global__ void __launch_bounds__(kBlock) scan_join_shared_kernel(const float *_
 
 int gcd(int a, int b) { return b ? gcd(b, a % b) : a; }
 
+constexpr int kFillBlocks = 512;   // workgroups that fill the chip
 // How a call is laid out.  A lane takes two channels of a 16-bit type where rows and strides allow it (four bytes a lane and load).
 struct Plan {
     int v, waves, seg_lanes, parts;
@@ -472,7 +521,7 @@ Plan plan_of(int64_t n_steps, int64_t batch, int32_t dim, int32_t groups, int32_
     int64_t w = div_up(n_steps, kSteps);
     p.waves = (int)(w < kMaxWaves ? w : kMaxWaves);
     // stretches of time: as many as fill the chip, of two rounds at least
-    int64_t s = 1024 / p.tiles, most = n_steps / (2 * kMaxWaves * kSteps);
+    int64_t s = kFillBlocks / p.tiles, most = n_steps / (2 * kMaxWaves * kSteps);
     if (s > most) s = most;
     if (s > 64) s = 64;
     if (s < 1) s = 1;
@@ -481,8 +530,8 @@ Plan plan_of(int64_t n_steps, int64_t batch, int32_t dim, int32_t groups, int32_
     p.seg_lanes = p.parts = 0;
     if (groups > 0 && groups != dim) {
         const int seg = gcd(channels, kWave * p.v);
-        p.seg_lanes = seg >= p.v ? seg / p.v : 0;
-        p.parts = p.seg_lanes ? dim / seg : dim;
+        p.seg_lanes = seg / p.v;   // (two channels a lane only where a gate has an even number of them)
+        p.parts = dim / seg;
     }
     return p;
 }
@@ -509,7 +558,7 @@ extern "C" int64_t bmtk_gated_scan_workspace_bytes(int64_t n_steps, int64_t batc
     for (int pairs = 0; pairs < 2; ++pairs) {
         const Plan p = plan_of(n_steps, batch, dim, groups, BMTK_BF16, pairs != 0);
         int64_t floats = p.splits > 1 ? 2 * p.splits * batch * dim : 0;
-        if (backward && groups == 0) floats += p.splits * p.waves * batch * dim;
+        if (backward && groups == 0) floats += p.splits * batch * dim;
         if (backward && groups > 0 && groups != dim && p.parts != groups) floats += n_steps * batch * p.parts;
         most = floats > most ? floats : most;
     }
@@ -538,7 +587,11 @@ void launch_fwd(const ScanArgs &s, const Plan &p, int groups, hipStream_t st)
         return;
     }
     dim3 grid((unsigned)p.tiles, (unsigned)p.splits);
-    if (p.splits > 1) BMTK_SCAN_LAUNCH(scan_sums_kernel, BMTK_COMMA false);
+    if (p.splits > 1) {
+        grid.y = (unsigned)p.splits - 1;
+        BMTK_SCAN_LAUNCH(scan_sums_kernel, BMTK_COMMA false);
+        grid.y = (unsigned)p.splits;
+    }
     BMTK_SCAN_LAUNCH(scan_fwd_kernel, );
 }
 
@@ -548,10 +601,14 @@ void launch_bwd(ScanArgs s, const Plan &p, int groups, hipStream_t st)
     const int dim = s.dim;
     const int64_t batch = s.columns / dim;
     dim3 grid((unsigned)p.tiles, (unsigned)p.splits);
-    if (p.splits > 1) BMTK_SCAN_LAUNCH(scan_sums_kernel, BMTK_COMMA true);
+    if (p.splits > 1) {
+        grid.y = (unsigned)p.splits - 1;
+        BMTK_SCAN_LAUNCH(scan_sums_kernel, BMTK_COMMA true);
+        grid.y = (unsigned)p.splits;
+    }
     BMTK_SCAN_LAUNCH(scan_bwd_kernel, );
     if (groups == 0)
-        hipLaunchKernelGGL((scan_join_const_kernel<TA>), dim3((unsigned)div_up(dim, kWave)), dim3(kBlock), 0, st, s.da_part, p.splits * p.waves * batch, dim,
+        hipLaunchKernelGGL((scan_join_const_kernel<TA>), dim3((unsigned)div_up(dim, kWave)), dim3(kJoinWaves * kWave), 0, st, s.da_part, p.splits * batch, dim,
                            (TA *)s.da);
     else if (s.da_part)
         hipLaunchKernelGGL((scan_join_shared_kernel<TA>), dim3((unsigned)div_up(s.n_steps * batch * groups, kBlock)), dim3(kBlock), 0, st, s.da_part,
@@ -604,7 +661,7 @@ extern "C" int bmtk_gated_scan_fwd(int64_t n_steps, int64_t batch, int32_t dim, 
     s.x = x, s.a = decay, s.state = state, s.lengths = lengths, s.h = h, s.last = last, s.marks = marks, s.sums = workspace;
     s.n_steps = n_steps, s.columns = batch * dim, s.split_steps = p.split_steps;
     s.x_t = x_t, s.x_b = x_b, s.a_t = a_t, s.a_b = a_b;
-    s.dim = dim, s.channels = groups > 0 ? dim / groups : 1, s.groups = groups;
+    s.dim = dim, s.channels = groups > 0 ? dim / groups : 1, s.sequences = batch;
     const hipStream_t st = (hipStream_t)stream;
 #define BMTK_DO(TX, TA, V) launch_fwd<TX, TA, V>(s, p, groups, st)
     BMTK_SCAN_TYPES(BMTK_DO);
@@ -632,7 +689,7 @@ extern "C" int bmtk_gated_scan_bwd(int64_t n_steps, int64_t batch, int32_t dim, 
     if (joined) s.da_part = workspace + (p.splits > 1 ? 2 * p.splits * batch * dim : 0);
     s.n_steps = n_steps, s.columns = batch * dim, s.split_steps = p.split_steps;
     s.x_t = x_t, s.x_b = x_b, s.a_t = a_t, s.a_b = a_b, s.dh_t = dh_t, s.dh_b = dh_b;
-    s.dim = dim, s.channels = groups > 0 ? dim / groups : 1, s.groups = groups, s.seg_lanes = p.seg_lanes, s.parts = p.parts;
+    s.dim = dim, s.channels = groups > 0 ? dim / groups : 1, s.sequences = batch, s.seg_lanes = p.seg_lanes, s.parts = p.parts;
     const hipStream_t st = (hipStream_t)stream;
 #define BMTK_DO(TX, TA, V) launch_bwd<TX, TA, V>(s, p, groups, st)
     BMTK_SCAN_TYPES(BMTK_DO);
