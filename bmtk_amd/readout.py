@@ -10,6 +10,7 @@ them (arguments that require gradients are refused while it records).  Tensors a
 nothing synchronises, so all of it can be captured.  float32, bfloat16 and float16; arithmetic in 32 bits, what is returned in 16 bits is rounded
 once.  The same call gives the same bits.  The reference has no counterpart (bmtk has no gradients).
 """
+import ctypes as C
 from typing import NamedTuple, Optional
 
 import torch
@@ -18,6 +19,37 @@ from . import _lib
 from .ops import _stream
 
 _CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
+
+
+class _Native:
+    """The same calls in native code for arguments that are as they should be, where that has been built for this torch; None for all others."""
+    NAMES = ("spike_readout", "spike_readout_bwd", "gated_scan", "gated_scan_bwd", "token_logprobs", "token_logprobs_bwd")
+    LIBRARY = ("spike_readout_workspace_bytes", "spike_readout_fwd", "spike_readout_bwd_weight", "spike_readout_bwd_spikes", "gated_scan_workspace_bytes",
+               "gated_scan_fwd", "gated_scan_bwd", "token_logprobs_workspace_bytes", "token_logprobs_fwd", "token_logprobs_bwd")
+
+    def __init__(self):
+        for name in self.NAMES:
+            setattr(self, name, self.first)
+
+    def first(self, *_):
+        """Looks for the module, once, when the library is needed on a GPU."""
+        if not torch.cuda.is_initialized():
+            return None
+        lib = _lib.load()
+        try:
+            from . import _readout
+        except ImportError:
+            _readout = None
+        if getattr(_readout, "built_for", None) != str(torch.__version__):
+            _readout = None
+        if _readout is not None:
+            _readout.set_library(tuple(C.cast(getattr(lib, "bmtk_" + name), C.c_void_p).value for name in self.LIBRARY), torch._C._cuda_getCurrentRawStream)
+        for name in self.NAMES:
+            setattr(self, name, getattr(_readout, name, lambda *_: None))
+        return None
+
+
+_native = _Native()
 
 
 def _given(t, name, dtype=None, shape=None):
@@ -71,6 +103,9 @@ def spike_readout(bits, weight, batch=1):
 
     bits: int64 [steps, words] spike bits as ``Glif3Simulator.run`` returns them (bit e = neuron * batch + trial; what lies behind the last element
     is not looked at; rows may be further apart than they are long).  y has the type of ``weight``; the sums are in 32 bits."""
+    y = _native.spike_readout(bits, weight, batch)
+    if y is not None:
+        return y
     steps, n, dim, stride = _spikes(bits, weight, batch)
     y = torch.empty(steps, batch, dim, dtype=weight.dtype, device=weight.device)
     if steps:
@@ -85,6 +120,9 @@ def spike_readout_bwd(bits, weight, dy, batch=1, spikes=True):
 
     d_weight: as ``weight``.  dl_dz: float32 [steps, neurons * batch], the gradient by every spike, as ``Glif3Bptt.backward`` takes it;
     None with ``spikes=False`` (a network that is not trained itself)."""
+    r = _native.spike_readout_bwd(bits, weight, dy, batch, spikes)
+    if r is not None:
+        return r
     steps, n, dim, stride = _spikes(bits, weight, batch)
     _contiguous(dy, "dy", weight.dtype, (steps, batch, dim))
     dev = weight.device
@@ -140,6 +178,9 @@ def gated_scan(x, decay, state=None, lengths=None, save_state=False):
             outside 0..steps count as the nearer of the two
     h has the type and shape of ``x``, last is float32 [sequences, channels], the state behind each sequence's last step: the ``state``
     of the next call.  saved: what ``gated_scan_bwd`` takes, float32, a sixteenth of h's entries."""
+    r = _native.gated_scan(x, decay, state, lengths, save_state)
+    if r is not None:
+        return r
     steps, batch, dim, groups, args = _scan(x, decay, lengths)
     if state is not None:
         _contiguous(state, "state", torch.float32, (batch, dim))
@@ -166,6 +207,9 @@ def gated_scan_bwd(x, decay, saved, dh, d_last=None, lengths=None):
 
     dx: as ``x``, 0 behind a sequence's end.  d_decay: as ``decay``, summed over the channels of a gate, and over all steps and
     sequences where there is one decay for them.  d_state: float32 [sequences, channels]."""
+    r = _native.gated_scan_bwd(x, decay, saved, dh, d_last, lengths)
+    if r is not None:
+        return r
     steps, batch, dim, groups, args = _scan(x, decay, lengths)
     if _given(dh, "dh", x.dtype).shape != x.shape:
         raise ValueError("dh must be {}, got {}".format(tuple(x.shape), tuple(dh.shape)))
@@ -220,6 +264,9 @@ def token_logprobs(logits, tokens, top=0, ignore=-100):
     tokens  int64 [...]; ``ignore`` where a row has none (padding): its logp is 0.  A token outside the vocabulary has logp NaN
     Returns ``LogProbs``: logp, entropy, lse (log of the sum of e^logit), top_logp and top_index: of equal logits the one with the
     lower index comes first.  A row of nothing but -inf: lse and logp -inf, entropy 0; one with NaN or +inf: NaN."""
+    r = _native.token_logprobs(logits, tokens, top, ignore)
+    if r is not None:
+        return LogProbs(*r)
     _given(tokens, "tokens", torch.int64)
     rows, n, vocab, stride = _logits(logits, tokens)
     if type(top) is not int or not 0 <= top <= min(_lib.LOGPROBS_MAX_TOP, vocab):
@@ -243,6 +290,10 @@ def token_logprobs_bwd(logits, tokens, fwd, d_logp=None, d_entropy=None, ignore=
     logits, tokens, ignore: as they were; fwd: what ``token_logprobs`` returned.  The alternatives are not differentiated.  Rows without a token get
     their entropy's gradient only, rows of nothing but -inf none.  out: where to write it; ``logits`` itself is allowed, which then
     are gone."""
+    if out is None:
+        r = _native.token_logprobs_bwd(logits, tokens, fwd.lse, fwd.entropy, d_logp, d_entropy, ignore)
+        if r is not None:
+            return r
     _given(tokens, "tokens", torch.int64)
     rows, n, vocab, stride = _logits(logits, tokens)
     if d_logp is None and d_entropy is None:
