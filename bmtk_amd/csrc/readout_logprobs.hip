@@ -8,23 +8,25 @@ namespace {
 
 constexpr float kLog2e = 1.44269504088896340736f;
 
-// Sums over a part of a row: maximum m, s = sum of e^(x - m), u = sum of (x - m) e^(x - m).  Then the logarithm of the whole sum is
-// m + log s and the entropy log s - u / s: no term of it is below zero, so nothing cancels.
+// Sums over a part of a row: maximum m (NaN where there is one), s = sum of e^(x - m), u = sum of (x - m) e^(x - m).  Then the logarithm of the
+// whole sum is m + log s and the entropy log s - u / s: no term of it is below zero, so nothing cancels.
 struct Sums {
     float m, s, u;
 };
 
-// e^(x - m); the difference first, so that logits at the end of the type's range stay in it
-__device__ __forceinline__ float exp_diff(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
+// maximum with NaN as the largest value
+__device__ __forceinline__ float max_nan(float a, float b) { return __builtin_elementwise_maximum(a, b); }
 
-// maximum with NaN as the largest value: a row with one shows it
-__device__ __forceinline__ float max_nan(float a, float b) { return a >= b || a != a ? a : b; }
+// x - m, at least -200: e^-200 is 0 in fp32 and a product with it too, also where the difference is -inf, or none (-inf less -inf, or anything less NaN).
+// The difference first, then the factor of the exponent, so that logits at the end of the type's range stay in it.
+__device__ __forceinline__ float below(float x, float m) { return __builtin_fmaxf(x - m, -200.0f); }
+__device__ __forceinline__ float exp_of(float d) { return __builtin_amdgcn_exp2f(d * kLog2e); }
 
-// a part's sums under the maximum m of several (one whose logits are all -inf, or too far below to count, adds nothing)
+// a part's sums under the maximum m of several
 __device__ __forceinline__ void raise_to(Sums &q, float m)
 {
-    const float d = q.m - m, e = q.m == -INFINITY ? 0.0f : exp_diff(d);
-    q.u = e == 0.0f ? 0.0f : (q.u + d * q.s) * e;
+    const float d = below(q.m, m), e = exp_of(d);
+    q.u = __builtin_fmaf(d, q.s, q.u) * e;
     q.s *= e;
     q.m = m;
 }
@@ -36,8 +38,12 @@ __device__ __forceinline__ Sums join(Sums a, Sums b)
     raise_to(b, m);
     return Sums{m, a.s + b.s, a.u + b.u};
 }
-// log probability of a logit.  (Sums of a row with NaN or +inf are NaN.)
-__device__ __forceinline__ float logp_of(const Sums &q, float x) { return x == -INFINITY && q.s == q.s ? -INFINITY : (x - q.m) - logf(q.s); }
+// log probability of a logit.  (A row with NaN or +inf has none.)
+__device__ __forceinline__ float logp_of(const Sums &q, float x)
+{
+    if (!(q.m < INFINITY)) return NAN;
+    return x == -INFINITY ? -INFINITY : (x - q.m) - logf(q.s);
+}
 
 // Order of the alternatives: the larger logit first (NaN before all), of equal ones the lower index.  One whole number for both;
 // 0 is below every real one.
@@ -55,49 +61,82 @@ __device__ __forceinline__ float logit_of(uint64_t rank)
     return __uint_as_float((int32_t)b < 0 ? b & 0x7fffffffu : ~b);
 }
 
-__device__ __forceinline__ uint64_t lane_xor(uint64_t v, int m)
+// The value of lane (lane ^ M), by moves within the vector unit: through LDS a sort of 64 lanes waits for 21 round trips (2.5 against 0.5 us).
+// All lanes have to be active.
+template <int M>
+__device__ __forceinline__ uint32_t lane_xor(uint32_t v)
 {
-    return ((uint64_t)(uint32_t)__shfl_xor((int)(v >> 32), m) << 32) | (uint32_t)__shfl_xor((int)(uint32_t)v, m);
+#define BMTK_MOVED(x, ctrl) ((uint32_t)__builtin_amdgcn_update_dpp(0, (int)(x), (ctrl), 0xF, 0xF, true))
+    if (M == 1) return BMTK_MOVED(v, 0xB1);                       // quad_perm 1, 0, 3, 2
+    if (M == 2) return BMTK_MOVED(v, 0x4E);                       // quad_perm 2, 3, 0, 1
+    if (M == 4) return BMTK_MOVED(BMTK_MOVED(v, 0x141), 0x1B);    // row_half_mirror (^ 7), then quad_perm 3, 2, 1, 0 (^ 3)
+    if (M == 8) return BMTK_MOVED(v, 0x128);                      // row_ror 8
+    if (M == 15) return BMTK_MOVED(v, 0x140);                     // row_mirror
+    const auto r = M == 16 ? __builtin_amdgcn_permlane16_swap(v, v, false, false) : __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return (lane_id() & M) ? r[0] : r[1];
+#undef BMTK_MOVED
 }
-__device__ __forceinline__ uint64_t lane_get(uint64_t v, int src)
+template <int M>
+__device__ __forceinline__ uint64_t lane_xor(uint64_t v)
 {
-    return ((uint64_t)(uint32_t)__shfl((int)(v >> 32), src) << 32) | (uint32_t)__shfl((int)(uint32_t)v, src);
+    return ((uint64_t)lane_xor<M>((uint32_t)(v >> 32)) << 32) | lane_xor<M>((uint32_t)v);
+}
+template <int M>
+__device__ __forceinline__ float lane_xor(float v)
+{
+    return __uint_as_float(lane_xor<M>(__float_as_uint(v)));
 }
 
 // one comparison of a sorting network over lanes: the lane keeps the larger of its own and its partner's, or the smaller
-__device__ __forceinline__ uint64_t exchange(uint64_t v, int m, bool larger)
+template <int M>
+__device__ __forceinline__ uint64_t exchange(uint64_t v, bool larger)
 {
-    const uint64_t o = lane_xor(v, m);
+    const uint64_t o = lane_xor<M>(v);
     return (o > v) == larger ? o : v;
 }
-// lanes of each group of W, the largest first (bitonic)
-template <int W>
+// lanes of each group of 2 M, bitonic, the largest first where `falling`
+template <int M>
+__device__ __forceinline__ uint64_t settle(uint64_t v, bool falling)
+{
+    v = exchange<M>(v, ((lane_id() & M) == 0) == falling);
+    if constexpr (M > 1) v = settle<M / 2>(v, falling);
+    return v;
+}
+// lanes of each group of W sorted, the largest first
+template <int W, int K = 2>
 __device__ __forceinline__ uint64_t sort_lanes(uint64_t v)
 {
-    const int l = lane_id() & (W - 1);
-#pragma unroll
-    for (int k = 2; k <= W; k *= 2)
-#pragma unroll
-        for (int m = k / 2; m > 0; m /= 2) v = exchange(v, m, ((l & m) == 0) == ((l & k) == 0 || k == W));
+    v = settle<K / 2>(v, K == W || (lane_id() & K) == 0);
+    if constexpr (K < W) v = sort_lanes<W, K * 2>(v);
     return v;
 }
 // the 64 largest of two sorted lists, sorted: the larger of each pair (l, 63 - l) are those, and are bitonic
 __device__ __forceinline__ uint64_t merge_lanes(uint64_t a, uint64_t b)
 {
-    const int l = lane_id();
-    const uint64_t o = lane_get(b, kWave - 1 - l);
-    uint64_t v = a > o ? a : o;
-#pragma unroll
-    for (int m = kWave / 2; m > 0; m /= 2) v = exchange(v, m, (l & m) == 0);
-    return v;
+    const uint64_t o = lane_xor<32>(lane_xor<16>(lane_xor<15>(b)));
+    return settle<kWave / 2>(a > o ? a : o, true);
 }
 
+template <int M>
+__device__ __forceinline__ float max_lanes(float v)
+{
+    v = max_nan(v, lane_xor<M>(v));
+    if constexpr (M > 1) v = max_lanes<M / 2>(v);
+    return v;
+}
+template <int M>
+__device__ __forceinline__ float sum_lanes(float v)
+{
+    v += lane_xor<M>(v);
+    if constexpr (M > 1) v = sum_lanes<M / 2>(v);
+    return v;
+}
+// the lanes of each group of W together
 template <int W>
 __device__ __forceinline__ Sums join_lanes(Sums a)
 {
-#pragma unroll
-    for (int m = W / 2; m > 0; m /= 2) a = join(a, Sums{__shfl_xor(a.m, m), __shfl_xor(a.s, m), __shfl_xor(a.u, m)});
-    return a;
+    raise_to(a, max_lanes<W / 2>(a.m));
+    return Sums{a.m, sum_lanes<W / 2>(a.s), sum_lanes<W / 2>(a.u)};
 }
 
 struct Row {
@@ -121,8 +160,9 @@ __device__ __forceinline__ void write_row(const Row &a, int64_t r, const Sums &q
         if (token >= 0 && token < a.vocab) lp = logp_of(q, (float)static_cast<const T *>(a.logits)[r * a.row_stride + token]);
     }
     a.logp[r] = lp;
-    a.lse[r] = q.m == -INFINITY ? -INFINITY : q.m + logf(q.s);
-    a.entropy[r] = q.m == -INFINITY ? 0.0f : logf(q.s) - q.u / q.s;
+    const bool none = q.m == -INFINITY, odd = !(q.m < INFINITY);
+    a.lse[r] = odd ? NAN : none ? -INFINITY : q.m + logf(q.s);
+    a.entropy[r] = odd ? NAN : none ? 0.0f : logf(q.s) - q.u / q.s;
 }
 
 __device__ __forceinline__ void write_top(const Row &a, int64_t r, const Sums &q, int k, uint64_t rank)
@@ -140,7 +180,7 @@ __global__ void __launch_bounds__(kBlock) logprobs_short_kernel(const Row a)
     const int64_t r = (int64_t)blockIdx.x * (kBlock / W) + threadIdx.x / W;
     const bool in = r < a.rows && l < a.vocab;
     const float x = in ? (float)static_cast<const T *>(a.logits)[r * a.row_stride + l] : -INFINITY;
-    Sums q{x, x == -INFINITY ? 0.0f : 1.0f, 0.0f};
+    Sums q{x, x == -INFINITY ? 0.0f : 1.0f, 0.0f};   // (a row with NaN or +inf: by its maximum)
     q = join_lanes<W>(q);
     if (r < a.rows && l == 0) write_row<T>(a, r, q);
     if (a.top > 0) {
@@ -189,26 +229,21 @@ struct Alternatives {
     }
 };
 
-// one logit into a lane's sums; m is the maximum already
-__device__ __forceinline__ void add_logit(Sums &q, float x)
-{
-    const float d = x - q.m, e = exp_diff(d);
-    q.s += e;
-    q.u += e == 0.0f ? 0.0f : d * e;
-}
-template <typename T, int N, bool kTop>
+template <int N, bool kTop>
 __device__ __forceinline__ void take_logits(Sums &q, Alternatives &alt, const float (&x)[N], uint32_t index, bool in, int top)
 {
     float m = x[0];
 #pragma unroll
     for (int k = 1; k < N; ++k) m = max_nan(m, x[k]);
-    if (in && m != -INFINITY) {
-        if (!(m <= q.m)) raise_to(q, m);
+    if (!(m <= q.m)) raise_to(q, max_nan(q.m, m));
 #pragma unroll
-        for (int k = 0; k < N; ++k) add_logit(q, x[k]);
+    for (int k = 0; k < N; ++k) {
+        const float d = below(x[k], q.m), e = exp_of(d);
+        q.s += e;
+        q.u = __builtin_fmaf(d, e, q.u);
     }
     // (equal ones are looked at, and a NaN, which comes before all)
-    if (kTop && __ballot(in && !(m < alt.least)) != 0)
+    if (kTop && __ballot(!(m < alt.least)) != 0)
 #pragma unroll
         for (int k = 0; k < N; ++k) alt.look(x[k], index + k, in, top);
 }
@@ -238,20 +273,23 @@ __global__ void __launch_bounds__(kWaves * kWave) logprobs_kernel(const Row a, c
     const int odd = (int)((reinterpret_cast<uintptr_t>(row + begin) & 15) / sizeof(T));
     const int body = min(end, begin + (odd ? N - odd : 0));
     const int packs = (end - body) / N, tail = body + packs * N;
+    // (lanes beyond take -inf, which adds nothing)
     if (wave == 0) {
         const int at = lane < body - begin ? begin + lane : tail + lane - (body - begin);
         const bool in = at < end;
         const float x[1] = {in ? (float)row[at] : -INFINITY};
-        take_logits<T, 1, kTop>(q, alt, x, (uint32_t)at, in, a.top);
+        take_logits<1, kTop>(q, alt, x, (uint32_t)at, in, a.top);
     }
     for (int p = wave * kWave; p < packs; p += kWaves * kWave) {
         const bool in = p + lane < packs;
-        Pack<T, N> v{};
-        if (in) v = *reinterpret_cast<const Pack<T, N> *>(row + body + (p + lane) * N);
+        const Pack<T, N> v = *reinterpret_cast<const Pack<T, N> *>(row + body + min(p + lane, packs - 1) * N);
         float x[N];
 #pragma unroll
         for (int k = 0; k < N; ++k) x[k] = (float)v.v[k];
-        take_logits<T, N, kTop>(q, alt, x, (uint32_t)(body + (p + lane) * N), in, a.top);
+        if (p + kWave > packs)
+#pragma unroll
+            for (int k = 0; k < N; ++k) x[k] = in ? x[k] : -INFINITY;
+        take_logits<N, kTop>(q, alt, x, (uint32_t)(body + (p + lane) * N), in, a.top);
     }
     if (kTop)
         while (alt.waiting) alt.take(a.top);
@@ -276,24 +314,30 @@ __global__ void __launch_bounds__(kWaves * kWave) logprobs_kernel(const Row a, c
     if (kTop && lane < a.top) write_top(a, r, q, lane, alt.best);
 }
 
-// the slices of a row together
+// The slices of a row together: a wavefront takes every sixteenth, the sixteen lists are merged pair by pair
+constexpr int kJoinWaves = 16;
 template <typename T, bool kTop>
-__global__ void __launch_bounds__(kWave) logprobs_join_kernel(const Row a, const Slices sl)
+__global__ void __launch_bounds__(kJoinWaves * kWave) logprobs_join_kernel(const Row a, const Slices sl)
 {
-    const int lane = lane_id();
+    __shared__ uint64_t lists[kTop ? kJoinWaves : 1][kWave];
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), waves = blockDim.x / kWave;
     const int64_t r = blockIdx.x;
-    Sums q{-INFINITY, 0.0f, 0.0f};
     uint64_t best = 0;
+    if (kTop) {
+        for (int k = wave; k < sl.count; k += waves) best = merge_lanes(best, lane < a.top ? sl.best[(r * sl.count + k) * a.top + lane] : 0);
+        for (int half = waves / 2; half > 0; half /= 2) {
+            if (wave >= half && wave < 2 * half) lists[wave][lane] = best;
+            __syncthreads();
+            if (wave < half) best = merge_lanes(best, lists[wave + half][lane]);
+        }
+    }
+    if (wave != 0) return;
+    Sums q{-INFINITY, 0.0f, 0.0f};
     for (int k = lane; k < sl.count; k += kWave) {
         const float *p = sl.sums + (r * sl.count + k) * 3;
         q = join(q, Sums{p[0], p[1], p[2]});
     }
     q = join_lanes<kWave>(q);
-    if (kTop)
-        for (int k = 0; k < sl.count; ++k) {
-            const uint64_t v = lane < a.top ? sl.best[(r * sl.count + k) * a.top + lane] : 0;
-            best = merge_lanes(best, v);
-        }
     if (lane == 0) write_row<T>(a, r, q);
     if (kTop && lane < a.top) write_top(a, r, q, lane, best);
 }
@@ -328,7 +372,7 @@ __device__ __forceinline__ Factors factors_of(const RowBwd &a, int64_t r)
 }
 __device__ __forceinline__ float gradient(const Factors &f, float x, int j)
 {
-    const float l = x - f.lse, p = exp_diff(l);
+    const float l = x - f.lse, p = __builtin_amdgcn_exp2f(l * kLog2e);
     float d = -(p * f.by_logp);
     if (p != 0.0f) d -= p * f.by_entropy * (l + f.entropy);   // (of a logit of -inf there is nothing)
     return j == f.token ? d + f.by_logp : d;
@@ -363,7 +407,8 @@ __global__ void __launch_bounds__(kBlock) logprobs_bwd_kernel(const RowBwd a, in
 template <typename T>
 __global__ void __launch_bounds__(kBlock) logprobs_bwd_short_kernel(const RowBwd a, FastDiv by_vocab)
 {
-    const int64_t block_rows = kBlock;   // a workgroup takes this many rows, so that numbers within it are small
+    // a workgroup takes as many rows as it has threads for, or one
+    const int64_t block_rows = kBlock > a.vocab ? kBlock / a.vocab : 1;
     const int64_t r0 = (int64_t)blockIdx.x * block_rows;
     const int here = (int)min(block_rows, a.rows - r0);
     for (int c = threadIdx.x; c < here * a.vocab; c += kBlock) {
@@ -448,7 +493,10 @@ extern "C" int bmtk_token_logprobs_fwd(int64_t rows, int32_t vocab, int32_t dtyp
             else BMTK_ROWS(4, false);
         }
         if (sl.count > 1) {
-            if (top) hipLaunchKernelGGL((logprobs_join_kernel<T, true>), dim3((unsigned)rows), dim3(kWave), 0, st, a, sl);
+            // (a power of two of wavefronts, one for each slice as far as they go)
+            int waves = 1;
+            while (waves < kJoinWaves && waves < sl.count) waves *= 2;
+            if (top) hipLaunchKernelGGL((logprobs_join_kernel<T, true>), dim3((unsigned)rows), dim3(waves * kWave), 0, st, a, sl);
             else hipLaunchKernelGGL((logprobs_join_kernel<T, false>), dim3((unsigned)rows), dim3(kWave), 0, st, a, sl);
         }
     });
@@ -472,7 +520,7 @@ extern "C" int bmtk_token_logprobs_bwd(int64_t rows, int32_t vocab, int32_t dtyp
     const bool together = ((reinterpret_cast<uintptr_t>(logits) ^ reinterpret_cast<uintptr_t>(d_logits)) & 15) == 0 && (((row_stride - out_stride) * (int64_t)size) & 15) == 0;
     if (vocab < 512) {
         const FastDiv by_vocab = fast_div((uint32_t)vocab);
-        BMTK_BY_TYPE(dtype, T, hipLaunchKernelGGL((logprobs_bwd_short_kernel<T>), dim3((unsigned)div_up(rows, kBlock)), dim3(kBlock), 0, st, a, by_vocab));
+        BMTK_BY_TYPE(dtype, T, hipLaunchKernelGGL((logprobs_bwd_short_kernel<T>), dim3((unsigned)div_up(rows, vocab < kBlock ? kBlock / vocab : 1)), dim3(kBlock), 0, st, a, by_vocab));
     } else {
         Slices sl{};
         slices_of(rows, vocab, dtype, sl);
