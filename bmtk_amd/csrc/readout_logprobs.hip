@@ -202,6 +202,21 @@ struct Alternatives {
     uint64_t *queue;     // 128 places in LDS
 
     __device__ __forceinline__ void start(uint64_t *q) { best = last = 0, least = -INFINITY, waiting = 0, queue = q; }
+    // What the first N logits of every lane say before any is looked at: the best of each lane are 64 logits, so none below the last that counts of
+    // those does.  (Looked at one by one they are all taken, four sorts instead of one.)
+    template <int N>
+    __device__ __forceinline__ void prime(const float (&x)[N], uint32_t index, int top)
+    {
+        uint64_t rank = rank_of(x[0], index);
+#pragma unroll
+        for (int k = 1; k < N; ++k) {
+            const uint64_t r = rank_of(x[k], index + k);
+            rank = r > rank ? r : rank;
+        }
+        rank = bcast_u64(sort_lanes<kWave>(rank), top - 1);
+        last = rank - 1;   // (which it passes itself)
+        least = logit_of(rank);
+    }
     __device__ __forceinline__ void take(int top)
     {
         const int l = lane_id();
@@ -211,8 +226,8 @@ struct Alternatives {
         const uint64_t v = (unsigned)l < n ? queue[waiting - n + l] : 0;
         waiting -= n;
         best = merge_lanes(best, sort_lanes<kWave>(v));
-        last = bcast_u64(best, top - 1);
-        if (last != 0) least = logit_of(last);
+        const uint64_t now = bcast_u64(best, top - 1);
+        if (now > last) last = now, least = logit_of(now);
         __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
         __builtin_amdgcn_wave_barrier();
     }
@@ -280,16 +295,48 @@ __global__ void __launch_bounds__(kWaves * kWave) logprobs_kernel(const Row a, c
         const float x[1] = {in ? (float)row[at] : -INFINITY};
         take_logits<1, kTop>(q, alt, x, (uint32_t)at, in, a.top);
     }
-    for (int p = wave * kWave; p < packs; p += kWaves * kWave) {
-        const bool in = p + lane < packs;
-        const Pack<T, N> v = *reinterpret_cast<const Pack<T, N> *>(row + body + min(p + lane, packs - 1) * N);
+    // whole loads of the wavefront, the next two on their way while two are worked on; then what is left
+    const T *mine = row + body + lane * N;
+    auto take = [&](const Pack<T, N> &v, int p, bool in, bool all) {
         float x[N];
 #pragma unroll
         for (int k = 0; k < N; ++k) x[k] = (float)v.v[k];
-        if (p + kWave > packs)
+        if (!all)
 #pragma unroll
             for (int k = 0; k < N; ++k) x[k] = in ? x[k] : -INFINITY;
         take_logits<N, kTop>(q, alt, x, (uint32_t)(body + (p + lane) * N), in, a.top);
+    };
+    constexpr int kStep = kWaves * kWave;
+    int p = wave * kWave;
+    if (p + kStep + kWave <= packs) {
+        Pack<T, N> v[2], w[2];
+        auto load = [&](Pack<T, N>(&u)[2], int at) {
+#pragma unroll
+            for (int k = 0; k < 2; ++k) u[k] = *reinterpret_cast<const Pack<T, N> *>(mine + min(at + k * kStep, packs - kWave) * N);
+        };
+        load(v, p);
+        if (kTop) {
+            float x[N];
+#pragma unroll
+            for (int k = 0; k < N; ++k) x[k] = (float)v[0].v[k];
+            alt.prime(x, (uint32_t)(body + (p + lane) * N), a.top);
+        }
+        for (;;) {
+            load(w, p + 2 * kStep);
+            take(v[0], p, true, true);
+            take(v[1], p + kStep, true, true);
+            p += 2 * kStep;
+            if (p + kStep + kWave > packs) break;
+            load(v, p + 2 * kStep);
+            take(w[0], p, true, true);
+            take(w[1], p + kStep, true, true);
+            p += 2 * kStep;
+            if (p + kStep + kWave > packs) break;
+        }
+    }
+    for (; p < packs; p += kStep) {
+        const bool in = p + lane < packs;
+        take(*reinterpret_cast<const Pack<T, N> *>(row + body + min(p + lane, packs - 1) * N), p, in, false);
     }
     if (kTop)
         while (alt.waiting) alt.take(a.top);
