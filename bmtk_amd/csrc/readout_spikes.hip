@@ -7,7 +7,7 @@ namespace bmtk {
 namespace {
 
 constexpr int kWaves = 4;
-constexpr int kFwdWaves = 8;
+constexpr int kManyWaves = 8, kOneBlockWaves = 16;   // of a workgroup of the forward pass
 constexpr int kWordsPerLane = 4;  // spike words that a lane has under way at once
 constexpr int kQueue = 512;       // spikes found and not yet added: at most 63 left over and one of each word under way
 static_assert(kQueue >= kWave * (kWordsPerLane + 1) && (kQueue & (kQueue - 1)) == 0, "room for what a round finds");
@@ -39,37 +39,49 @@ struct Accumulators {
     __device__ __forceinline__ float get(int c, int which) const { return sum[c][N == 1 ? 0 : which]; }
 };
 
-// Adds the rows of m of a queue's spikes: row of lane k's spike to the sums of lane k's `which`.  Rows are asked for sixteen (of
+// Adds the rows of m of a queue's spikes: that of lane k's spike, `row`, to the sums of lane k's `which`.  Rows are asked for sixteen (of
 // four channels a lane: eight) at a time; `at` is where the lane's channels begin, within a row.
 template <typename T, int VW, int N>
 __device__ __forceinline__ void add_rows(Accumulators<VW, N> &acc, const T *__restrict__ rows, int dim, unsigned at, int row, int which, int m)
 {
     constexpr int kLoads = VW == 4 ? 8 : 16;
-    for (int k = 0; k < m; k += kLoads) {
-        Pack<T, VW> q[kLoads];
+    // (a lane works out its own row's distance, once for all)
+    const uint64_t distance = (uint64_t)(uint32_t)row * (uint64_t)((uint32_t)dim * (uint32_t)sizeof(T));
+    auto load = [&](Pack<T, VW>(&q)[kLoads], int k, int last) {
 #pragma unroll
         for (int u = 0; u < kLoads; ++u) {
-            const T *p = rows + (int64_t)bcast_i(row, min(k + u, m - 1)) * dim;
+            const T *p = reinterpret_cast<const T *>(reinterpret_cast<const char *>(rows) + bcast_u64(distance, min(k + u, last)));
             q[u] = *reinterpret_cast<const Pack<T, VW> *>(p + at);
         }
+    };
+    auto add = [&](const Pack<T, VW> &q, int lane) {
+        float v[VW];
 #pragma unroll
-        for (int u = 0; u < kLoads; ++u) {
-            if (k + u < m) {
-                float v[VW];
+        for (int c = 0; c < VW; ++c) v[c] = (float)q.v[c];
+        acc.add(N == 1 ? 0 : bcast_i(which, lane), v);
+    };
+    int k = 0;
+    for (; k + kLoads <= m; k += kLoads) {
+        Pack<T, VW> q[kLoads];
+        load(q, k, kWave - 1);
 #pragma unroll
-                for (int c = 0; c < VW; ++c) v[c] = (float)q[u].v[c];
-                acc.add(N == 1 ? 0 : bcast_i(which, k + u), v);
-            }
-        }
+        for (int u = 0; u < kLoads; ++u) add(q[u], k + u);
+    }
+    if (k < m) {
+        Pack<T, VW> q[kLoads];
+        load(q, k, m - 1);
+#pragma unroll
+        for (int u = 0; u < kLoads; ++u)
+            if (k + u < m) add(q[u], k + u);
     }
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// Forward.  A workgroup takes one step and a slice of its words of spike bits; a wavefront turns the set bits of 256 words at a
+// Forward.  A workgroup takes one step and a slice of its words of spike bits; a wavefront turns the set bits of 64 kWords words at a
 // time into a queue of element numbers, works it off 64 spikes at a time (each lane divides one of them into neuron and trial),
 // and reads the weight rows, one per spike, 64 * VW channels by its 64 lanes.  The sums of a trial are the wavefront's own, so their
 // order is fixed; the wavefronts' sums are added in order at the end.
-template <typename T, int VW, int N>
+template <typename T, int VW, int N, int kFwdWaves, int kWords>
 __global__ void __launch_bounds__(kFwdWaves * kWave)
 spike_fwd_kernel(const uint64_t *__restrict__ bits, int64_t stride, int64_t ne, FastDiv by_batch, int trials, int trial_tiles,
                  const T *__restrict__ weight, int dim, int64_t slice_words, T *__restrict__ y, float *__restrict__ part)
@@ -95,13 +107,13 @@ spike_fwd_kernel(const uint64_t *__restrict__ bits, int64_t stride, int64_t ne, 
     const uint32_t first_element = (uint32_t)(w_begin << 6);
     unsigned head = 0, tail = 0;
 
-    auto load = [&](int c, uint64_t (&w)[kWordsPerLane]) {
+    auto load = [&](int c, uint64_t (&w)[kWords]) {
 #pragma unroll
-        for (int k = 0; k < kWordsPerLane; ++k) w[k] = row[min(c + k * kWave + lane, w_count - 1)];
+        for (int k = 0; k < kWords; ++k) w[k] = row[min(c + k * kWave + lane, w_count - 1)];
     };
 
-    constexpr int kStep = kWave * kWordsPerLane;
-    uint64_t w[kWordsPerLane] = {}, next[kWordsPerLane];
+    constexpr int kStep = kWave * kWords;
+    uint64_t w[kWords] = {}, next[kWords];
     uint32_t first = 0;
     int c = wave * kStep;
     load(c, next);
@@ -110,12 +122,12 @@ spike_fwd_kernel(const uint64_t *__restrict__ bits, int64_t stride, int64_t ne, 
         while (tail - head < kWave) {
             uint64_t any = 0;
 #pragma unroll
-            for (int k = 0; k < kWordsPerLane; ++k) any |= w[k];
+            for (int k = 0; k < kWords; ++k) any |= w[k];
             if (__ballot(any != 0) == 0) {
                 more = c < w_count;
                 if (!more) break;
 #pragma unroll
-                for (int k = 0; k < kWordsPerLane; ++k) {
+                for (int k = 0; k < kWords; ++k) {
                     const int at = c + k * kWave + lane;
                     w[k] = at < w_count ? next[k] & (at == last_word ? last_mask : ~0ull) : 0;
                 }
@@ -125,7 +137,7 @@ spike_fwd_kernel(const uint64_t *__restrict__ bits, int64_t stride, int64_t ne, 
             }
             // one spike of every word
 #pragma unroll
-            for (int k = 0; k < kWordsPerLane; ++k) {
+            for (int k = 0; k < kWords; ++k) {
                 const uint32_t e = first + (uint32_t)(k * kWave * 64) + (uint32_t)__builtin_ctzll(w[k]);
                 bool mine = w[k] != 0;
                 if (trial_tiles > 1) mine = mine && (unsigned)((int)(e - div_by(e, by_batch) * (uint32_t)batch) - b0) < (unsigned)trials;
@@ -287,6 +299,7 @@ spike_bwd_weight_kernel(const uint64_t *__restrict__ bits, int64_t stride, int64
 // are made and added up in fp32.
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x8 __attribute__((ext_vector_type(8)));
 typedef bf16 bf16x8 __attribute__((ext_vector_type(8)));
 typedef f16 f16x8 __attribute__((ext_vector_type(8)));
 constexpr int kDzK = 64;          // channels at a time
@@ -320,6 +333,25 @@ struct Operand<float> {
         return odd == 0.0f;
     }
     __device__ __forceinline__ static f32x16 multiply(const Part &a, const Part &b, const f32x16 &acc) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, acc, 0, 0, 0); }
+};
+// fp32 as it is: for small products, whose time is not the matrix instructions'
+struct Whole {};
+template <>
+struct Operand<Whole> {
+    static constexpr int kParts = 1;
+    typedef f32x8 Part;
+    __device__ __forceinline__ static bool split(const float (&v)[8], Part (&part)[1])
+    {
+#pragma unroll
+        for (int s = 0; s < 8; ++s) part[0][s] = v[s];
+        return true;
+    }
+    __device__ __forceinline__ static f32x16 multiply(const Part &a, const Part &b, f32x16 acc)
+    {
+#pragma unroll
+        for (int s = 0; s < 8; ++s) acc = __builtin_amdgcn_mfma_f32_32x32x2f32(a[s], b[s], acc, 0, 0, 0);
+        return acc;
+    }
 };
 template <>
 struct Operand<bf16> {
@@ -375,12 +407,12 @@ __device__ __forceinline__ void load_eight(const T *__restrict__ base, int row, 
 enum { kPairs = 0, kAcross = 1, kTurned = 2 };
 
 // kOnePass: up to 64 channels
-template <typename T, int VL, int kOut, bool kOnePass>
+template <typename T, typename O, int VL, int kOut, bool kOnePass>
 __global__ void __launch_bounds__(kDzWaves * kWave, (kOnePass && kOut >= kTurned) || sizeof(T) == 2 ? 3 : 2)
 spike_bwd_spikes_kernel(const T *__restrict__ weight, const T *__restrict__ dy, int64_t rows, int64_t n, FastDiv by_batch, int dim,
                         int64_t rows_per_block, int32_t *__restrict__ not_finite, float *__restrict__ dl_dz)
 {
-    typedef Operand<T> Op;
+    typedef Operand<O> Op;
     typedef typename Op::Part Part;
     constexpr int P = Op::kParts;
     static_assert(kDzRows * kDzK / 8 == kDzWaves * kWave, "eight channels of a row for every thread");
@@ -546,14 +578,14 @@ int lane_channels(int dim, int dtype, const void *p)
 // slices of a step's words: enough workgroups to fill the chip, a load of words for every wavefront at least
 int64_t fwd_slices(int64_t n_steps, int64_t words, int64_t tiles)
 {
-    const int64_t most = div_up(words, kFwdWaves * kWave);
+    const int64_t most = div_up(words, kManyWaves * kWave);
     int64_t s = 512 / (n_steps * tiles);
     s = s < 1 ? 1 : s;
     return s < most ? s : most;
 }
 
 struct FwdPlan {
-    int vw, trials, trial_tiles, tiles;
+    int vw, trials, trial_tiles, tiles, waves, words_per_lane;
     int64_t slices, slice_words;
 };
 FwdPlan fwd_plan(int64_t n_steps, int64_t n, int batch, int dim, int vw)
@@ -565,17 +597,26 @@ FwdPlan fwd_plan(int64_t n_steps, int64_t n, int batch, int dim, int vw)
     p.tiles = p.trial_tiles * (int)div_up(dim, kWave * vw);
     const int64_t words = (n * batch + 63) / 64;
     p.slices = fwd_slices(n_steps, words, p.tiles);
+    p.waves = kManyWaves;
+    // one step of one trial whose words one workgroup has on their way at once: no slices to join (230,924 neurons, 64 channels: 9.3 us in 8 slices
+    // and their sum, 8.3 in one launch)
+    if (batch == 1 && p.slices > 1 && words <= kOneBlockWaves * kWave * kWordsPerLane) p.slices = 1, p.waves = kOneBlockWaves;
     p.slice_words = div_up(div_up(words, p.slices), kWave) * kWave;
     p.slices = div_up(words, p.slice_words);
+    // (one where four would leave wavefronts without any)
+    p.words_per_lane = p.slice_words < p.waves * kWave * kWordsPerLane ? 1 : kWordsPerLane;
     return p;
 }
 
 struct DzPlan {
     int64_t across, per_block, down, parts;
+    bool whole;   // fp32: in fp32 instructions.  Up to this many products they take some us at most, less than the launch that looks for infinities
 };
-DzPlan dz_plan(int64_t n_steps, int64_t n, int batch)
+constexpr double kWholeProducts = 3e8;
+DzPlan dz_plan(int64_t n_steps, int64_t n, int batch, int dim)
 {
     DzPlan p;
+    p.whole = (double)n_steps * batch * n * dim < kWholeProducts;
     p.across = div_up(n, kDzWaves * kDzNeurons);
     const int64_t rows = n_steps * batch, most = div_up(rows, kDzRows);
     int64_t blocks = div_up(4096, p.across);
@@ -604,7 +645,10 @@ using namespace bmtk;
 extern "C" int64_t bmtk_spike_readout_workspace_bytes(int64_t n_steps, int64_t n_neurons, int32_t batch, int32_t dim, int32_t backward)
 {
     if (check_sizes("spike_readout_workspace_bytes", n_steps, n_neurons, batch, dim, BMTK_F32) != BMTK_OK) return 0;
-    if (backward) return dz_plan(n_steps, n_neurons, batch).parts * (int64_t)sizeof(int32_t);
+    if (backward) {
+        const DzPlan p = dz_plan(n_steps, n_neurons, batch, dim);
+        return p.whole ? 0 : p.parts * (int64_t)sizeof(int32_t);
+    }
     int64_t slices = 1;   // (as many as any alignment of the weights takes)
     for (int vw = 1; vw <= 4; vw *= 2) {
         const FwdPlan p = fwd_plan(n_steps, n_neurons, batch, dim, vw);
@@ -627,26 +671,36 @@ extern "C" int bmtk_spike_readout_fwd(const uint64_t *spike_bits, int64_t stride
     const int64_t plane = n_steps * batch * (int64_t)dim;
     BMTK_REQUIRE(plane < (1ll << 31), "spike_readout_fwd: the result is too large");
     const dim3 grid((unsigned)n_steps, (unsigned)p.slices, (unsigned)p.tiles);
-    const size_t lds = (size_t)kFwdWaves * p.trials * kWave * p.vw * sizeof(float);
+    const size_t lds = (size_t)p.waves * p.trials * kWave * p.vw * sizeof(float);
     const hipStream_t st = (hipStream_t)stream;
     const FastDiv by_batch = fast_div((uint32_t)batch);
-#define BMTK_FWD(VW, N)                                                                                                                      \
-    hipLaunchKernelGGL((spike_fwd_kernel<T, VW, N>), grid, dim3(kFwdWaves *kWave), lds, st, spike_bits, stride, n_neurons *batch, by_batch, p.trials, \
+#define BMTK_FWD_W(VW, N, WAVES, WORDS)                                                                                                                      \
+    hipLaunchKernelGGL((spike_fwd_kernel<T, VW, N, WAVES, WORDS>), grid, dim3(WAVES *kWave), lds, st, spike_bits, stride, n_neurons *batch, by_batch, p.trials, \
                        p.trial_tiles, (const T *)weight, dim, p.slice_words, (T *)y, part)
+#define BMTK_FWD(VW, N, WAVES)                                                   \
+    do {                                                                         \
+        if (p.words_per_lane == 1) BMTK_FWD_W(VW, N, WAVES, 1);                  \
+        else BMTK_FWD_W(VW, N, WAVES, kWordsPerLane);                            \
+    } while (0)
     BMTK_BY_TYPE(dtype, T, {
-        if (batch == 1) {
-            if (p.vw == 1) BMTK_FWD(1, 1);
-            else if (p.vw == 2) BMTK_FWD(2, 1);
-            else BMTK_FWD(4, 1);
+        if (p.waves == kOneBlockWaves) {
+            if (p.vw == 1) BMTK_FWD(1, 1, kOneBlockWaves);
+            else if (p.vw == 2) BMTK_FWD(2, 1, kOneBlockWaves);
+            else BMTK_FWD(4, 1, kOneBlockWaves);
+        } else if (batch == 1) {
+            if (p.vw == 1) BMTK_FWD(1, 1, kManyWaves);
+            else if (p.vw == 2) BMTK_FWD(2, 1, kManyWaves);
+            else BMTK_FWD(4, 1, kManyWaves);
         } else {
-            if (p.vw == 1) BMTK_FWD(1, 32);
-            else if (p.vw == 2) BMTK_FWD(2, 16);
-            else BMTK_FWD(4, 8);
+            if (p.vw == 1) BMTK_FWD(1, 32, kManyWaves);
+            else if (p.vw == 2) BMTK_FWD(2, 16, kManyWaves);
+            else BMTK_FWD(4, 8, kManyWaves);
         }
         if (part)
             hipLaunchKernelGGL((spike_join_kernel<T>), dim3((unsigned)div_up(plane, kBlock)), dim3(kBlock), 0, st, part, (int)p.slices, plane, (T *)y);
     });
 #undef BMTK_FWD
+#undef BMTK_FWD_W
     BMTK_CHECK_LAUNCH("spike_readout_fwd");
     return BMTK_OK;
 }
@@ -693,8 +747,8 @@ extern "C" int bmtk_spike_readout_bwd_spikes(const void *weight, const void *dy,
     BMTK_REQUIRE(weight && dy && dl_dz, "spike_readout_bwd_spikes: pointers must be non-null");
     int rc = check_sizes("spike_readout_bwd_spikes", n_steps, n_neurons, batch, dim, dtype);
     if (rc != BMTK_OK) return rc;
-    BMTK_REQUIRE(dtype != BMTK_F32 || workspace, "spike_readout_bwd_spikes: needs its workspace");
-    const DzPlan p = dz_plan(n_steps, n_neurons, batch);
+    const DzPlan p = dz_plan(n_steps, n_neurons, batch, dim);
+    BMTK_REQUIRE(dtype != BMTK_F32 || p.whole || workspace, "spike_readout_bwd_spikes: needs its workspace");
     const int64_t rows = n_steps * batch;
     const dim3 grid((unsigned)p.across, (unsigned)p.down);
     const int vl = 16 / (int)type_size(dtype);   // 16 bytes a load
@@ -703,28 +757,34 @@ extern "C" int bmtk_spike_readout_bwd_spikes(const void *weight, const void *dy,
     const FastDiv by_batch = fast_div((uint32_t)batch);
     // (a tile's pairs are whole steps, or 32 trials of one)
     const bool turned = (batch % 32 == 0 || batch == 4 || batch == 8 || batch == 16) && aligned(dl_dz, 128) && n_neurons * batch % 32 == 0;
-#define BMTK_DZ(VL, OUT, ONE)                                                                                                                       \
-    hipLaunchKernelGGL((spike_bwd_spikes_kernel<T, VL, OUT, ONE>), grid, dim3(kDzWaves *kWave), 0, st, (const T *)weight, (const T *)dy, rows, n_neurons, \
+#define BMTK_DZ(O, VL, OUT, ONE)                                                                                                                       \
+    hipLaunchKernelGGL((spike_bwd_spikes_kernel<T, O, VL, OUT, ONE>), grid, dim3(kDzWaves *kWave), 0, st, (const T *)weight, (const T *)dy, rows, n_neurons, \
                        by_batch, dim, p.per_block, workspace, dl_dz)
-#define BMTK_DZ_OUT(VL, ONE)                                 \
+#define BMTK_DZ_OUT(O, VL, ONE)                                 \
     do {                                                     \
-        if (batch == 1) BMTK_DZ(VL, kAcross, ONE);           \
-        else if (!turned) BMTK_DZ(VL, kPairs, ONE);          \
-        else if (batch == 4) BMTK_DZ(VL, kTurned, ONE);      \
-        else if (batch == 8) BMTK_DZ(VL, kTurned + 1, ONE);  \
-        else if (batch == 16) BMTK_DZ(VL, kTurned + 2, ONE); \
-        else BMTK_DZ(VL, kTurned + 3, ONE);                  \
+        if (batch == 1) BMTK_DZ(O, VL, kAcross, ONE);           \
+        else if (!turned) BMTK_DZ(O, VL, kPairs, ONE);          \
+        else if (batch == 4) BMTK_DZ(O, VL, kTurned, ONE);      \
+        else if (batch == 8) BMTK_DZ(O, VL, kTurned + 1, ONE);  \
+        else if (batch == 16) BMTK_DZ(O, VL, kTurned + 2, ONE); \
+        else BMTK_DZ(O, VL, kTurned + 3, ONE);                  \
     } while (0)
-#define BMTK_DZ_BY(VL)                            \
+#define BMTK_DZ_BY(O, VL)                            \
     do {                                          \
-        if (dim <= kDzK) BMTK_DZ_OUT(VL, true);   \
-        else BMTK_DZ_OUT(VL, false);              \
+        if (dim <= kDzK) BMTK_DZ_OUT(O, VL, true);   \
+        else BMTK_DZ_OUT(O, VL, false);              \
     } while (0)
-    BMTK_BY_TYPE(dtype, T, {
-        if (wide) BMTK_DZ_BY(16 / sizeof(T));
-        else BMTK_DZ_BY(1);
-    });
-    if (dtype == BMTK_F32)
+    if (dtype == BMTK_F32 && p.whole) {
+        typedef float T;
+        if (wide) BMTK_DZ_BY(Whole, 4);
+        else BMTK_DZ_BY(Whole, 1);
+    } else {
+        BMTK_BY_TYPE(dtype, T, {
+            if (wide) BMTK_DZ_BY(T, 16 / sizeof(T));
+            else BMTK_DZ_BY(T, 1);
+        });
+    }
+    if (dtype == BMTK_F32 && !p.whole)
         hipLaunchKernelGGL(spike_bwd_spikes_again_kernel, dim3((unsigned)div_up(p.parts, kBlock)), dim3(kBlock), 0, st, (const float *)weight, (const float *)dy, rows,
                            n_neurons, by_batch, dim, p.per_block, (int)p.across, (int)p.parts, workspace, dl_dz);
 #undef BMTK_DZ_BY

@@ -717,7 +717,8 @@ int bmtk_spike_readout_fwd(const uint64_t *spike_bits, int64_t stride, int64_t n
 /* d_weight[i][:] = sum of dy[t][b][:] over the spikes of neuron i (all rows are written) */
 int bmtk_spike_readout_bwd_weight(const uint64_t *spike_bits, int64_t stride, int64_t n_steps, int64_t n_neurons, int32_t batch, const void *dy, int32_t dim,
                                   int32_t dtype, void *d_weight, void *stream);
-/* dl_dz[t][i * batch + b] = dy[t][b][:] . weight[i][:], in 32 bits: what bmtk_glif3_bwd takes.  workspace: only for BMTK_F32 */
+/* dl_dz[t][i * batch + b] = dy[t][b][:] . weight[i][:], in 32 bits: what bmtk_glif3_bwd takes.  workspace: where
+ * bmtk_spike_readout_workspace_bytes says so, for BMTK_F32 only */
 int bmtk_spike_readout_bwd_spikes(const void *weight, const void *dy, int64_t n_steps, int64_t n_neurons, int32_t batch, int32_t dim, int32_t dtype,
                                   float *dl_dz, int32_t *workspace, void *stream);
 

@@ -137,6 +137,34 @@ def test_infinite_gradients_reach_their_spikes_only():
     assert torch.isfinite(dl_dz).all()
 
 
+@pytest.mark.parametrize("steps,n,batch,dim", [(20, 9001, 32, 64), (40, 8111, 12, 100), (701, 5003, 1, 128), (30, 10016, 4, 300), (60, 9000, 8, 96), (31, 10000, 16, 65),
+                                               (9, 9000, 64, 61), (7, 5003, 45, 260)])
+def test_products_in_parts(steps, n, batch, dim):
+    """fp32 of more products than are made in fp32 instructions (3e8): every way in which the result reaches memory, one pass over the channels and more,
+    partial tiles; then with an infinity in a weight, an infinity and a NaN in a gradient: those reach what they take part in and nothing else."""
+    g = gen(steps)
+    w, dy = torch.randn(n, dim, generator=g), torch.randn(steps, batch, dim, generator=g)
+    bits = torch.zeros(steps, (n * batch + 63) // 64, dtype=torch.int64, device="cuda")
+
+    def dl_dz():
+        return readout.spike_readout_bwd(bits, w.cuda(), dy.cuda(), batch)[1].view(steps, n, batch)
+
+    def products(a, b):
+        return (b.double().view(steps * batch, dim) @ a.double().t()).view(steps, batch, n).transpose(1, 2)
+    first = dl_dz()
+    close(first, products(w, dy), (dim + 8) * 2 * U * products(w.abs(), dy.abs()), "dl_dz")
+    w[5, dim - 1], dy[steps - 1, batch - 1, 0], dy[0, 0, dim // 2] = math.inf, -math.inf, math.nan
+    w[5, 0] = 2.0
+    got, want = dl_dz().cpu(), products(w, dy)
+    reached = torch.zeros(steps, n, batch, dtype=torch.bool)
+    reached[:, 5], reached[steps - 1, :, batch - 1], reached[0, :, 0] = True, True, True
+    assert torch.isfinite(got[~reached]).all()
+    assert torch.equal(got[reached].isnan(), want[reached].isnan())
+    inf = reached & want.isinf()
+    assert inf.any() and torch.equal(got[inf].double(), want[inf])
+    close(got[~reached], want[~reached], (dim + 8) * 2 * U * products(w.nan_to_num(0, 0, 0).abs(), dy.nan_to_num(0, 0, 0).abs())[~reached], "the rest")
+
+
 def test_no_steps():
     bits, w = torch.zeros(0, 5, dtype=torch.int64, device="cuda"), torch.ones(20, 3, device="cuda")
     assert readout.spike_readout(bits, w, 4).shape == (0, 4, 3)
@@ -621,6 +649,14 @@ def test_two_streams_at_once():
     for k in (0, 1):
         for out in got[k]:
             assert all(torch.equal(p, q) for p, q in zip(out, want[k]))
+
+
+def test_calls_in_native_code_and_in_python_are_the_same(monkeypatch):
+    case = chain_case(6)
+    native = everything(case)
+    assert readout._native.gated_scan.__name__ == "gated_scan" and readout._native.gated_scan(None, None, None, None, False) is None
+    monkeypatch.setattr(readout, "_native", type("Nothing", (), {name: staticmethod(lambda *_: None) for name in readout._Native.NAMES}))
+    assert all(torch.equal(p, q) and p.dtype == q.dtype and p.shape == q.shape for p, q in zip(everything(case), native))
 
 
 def test_label_loss_trains_a_network_down_to_its_spikes():

@@ -48,7 +48,7 @@ def test_spike_readout_bwd():
     refused(lib.bmtk_spike_readout_bwd_weight(P, 1, 3, 10, 4, P, 8, 7, P, None), "type")
     refused(lib.bmtk_spike_readout_bwd_spikes(P, P, 3, 10, 4, 8, 0, None, P, None), "null")
     refused(lib.bmtk_spike_readout_bwd_spikes(P, P, 3, 1 << 30, 4, 8, 0, P, P, None), "2^31")
-    refused(lib.bmtk_spike_readout_bwd_spikes(P, P, 3, 10, 4, 8, 0, P, None, None), "workspace")
+    refused(lib.bmtk_spike_readout_bwd_spikes(P, P, 300, 10000, 32, 8, 0, P, None, None), "workspace")
     assert lib.bmtk_spike_readout_workspace_bytes(0, 10, 4, 8, 0) == 0
     assert lib.bmtk_spike_readout_workspace_bytes(1000, 10000, 1, 8, 0) == 0            # steps enough
     assert lib.bmtk_spike_readout_workspace_bytes(1, 1 << 20, 1, 8, 0) % (8 * 4) == 0 < lib.bmtk_spike_readout_workspace_bytes(1, 1 << 20, 1, 8, 0)
