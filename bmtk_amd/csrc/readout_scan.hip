@@ -520,12 +520,13 @@ Plan plan_of(int64_t n_steps, int64_t batch, int32_t dim, int32_t groups, int32_
     p.tiles = div_up(batch * dim, kWave * p.v);
     int64_t w = div_up(n_steps, kSteps);
     p.waves = (int)(w < kMaxWaves ? w : kMaxWaves);
-    // stretches of time: as many as fill the chip, of two rounds at least
-    int64_t s = kFillBlocks / p.tiles, most = n_steps / (2 * kMaxWaves * kSteps);
+    // stretches of time, of whole rounds: as many as fill the chip
+    const int64_t round = (int64_t)p.waves * kSteps;
+    int64_t s = kFillBlocks / p.tiles, most = div_up(n_steps, round);
     if (s > most) s = most;
     if (s > 64) s = 64;
     if (s < 1) s = 1;
-    p.split_steps = div_up(div_up(n_steps, s), kSteps) * kSteps;
+    p.split_steps = div_up(div_up(n_steps, s), round) * round;
     p.splits = div_up(n_steps, p.split_steps);
     p.seg_lanes = p.parts = 0;
     if (groups > 0 && groups != dim) {
