@@ -1,4 +1,6 @@
 // Gated linear recurrence over the steps of many sequences, h[t] = a[t] h[t - 1] + x[t], and its backward pass.
+#include <type_traits>
+
 #include "readout.hpp"
 
 namespace bmtk {
@@ -52,10 +54,11 @@ __device__ __forceinline__ void store_v(T *p, const float (&v)[V])
 // Gates: one per channel for all steps, one per channel and step, or one per step for several neighbouring channels (a lane's are of one gate)
 enum { kConst = 0, kEach = 1, kShared = 2 };
 
-// A lane's part of a block of steps as it lies in memory
+// A lane's part of a block of steps as it lies in memory, in whole registers: two 16-bit numbers stay in one until they are computed with
 template <typename T, int V>
 struct Block {
-    Pack<T, V> v[kSteps];
+    static constexpr int kBytes = V * (int)sizeof(T), kRegs = (kBytes + 3) / 4;
+    uint32_t w[kSteps][kRegs];
     // `last`: the last step that one of the wavefront's sequences has (or step 0); behind it that one again: nothing outside is read, there are no
     // branches, and those steps are cut
     __device__ __forceinline__ void load(const T *p, int64_t stride, int64_t t0, int64_t last)
@@ -64,7 +67,13 @@ struct Block {
         const T *row = p + at * stride;
 #pragma unroll
         for (int k = 0; k < kSteps; ++k) {
-            v[k] = *reinterpret_cast<const Pack<T, V> *>(row);
+            if constexpr (kBytes == 2) {
+                w[k][0] = *reinterpret_cast<const uint16_t *>(row);
+            } else {
+                const Pack<uint32_t, kRegs> q = *reinterpret_cast<const Pack<uint32_t, kRegs> *>(row);
+#pragma unroll
+                for (int r = 0; r < kRegs; ++r) w[k][r] = q.v[r];
+            }
             row += at < last ? stride : 0;
             ++at;
         }
@@ -72,12 +81,41 @@ struct Block {
     // steps from `there` on are as if they were `other`
     __device__ __forceinline__ void cut(int there, float other)
     {
+        uint32_t o;
+        if constexpr (sizeof(T) == 4) {
+            o = __float_as_uint(other);
+        } else {
+            const T h = (T)other;
+            uint16_t bits;
+            __builtin_memcpy(&bits, &h, 2);
+            o = bits * 0x10001u;
+        }
 #pragma unroll
         for (int k = 0; k < kSteps; ++k)
 #pragma unroll
-            for (int c = 0; c < V; ++c) v[k].v[c] = k < there ? v[k].v[c] : (T)other;
+            for (int r = 0; r < kRegs; ++r) w[k][r] = k < there ? w[k][r] : o;
     }
-    __device__ __forceinline__ float get(int k, int c) const { return (float)v[k].v[V == 1 ? 0 : c]; }
+    // (of a single number, that one whatever c is)
+    __device__ __forceinline__ float get(int k, int c) const
+    {
+        if constexpr (sizeof(T) == 4) {
+            return __uint_as_float(w[k][V == 1 ? 0 : c]);
+        } else if constexpr (std::is_same<T, bf16>::value) {
+            return __uint_as_float(V == 1 || c == 0 ? w[k][0] << 16 : w[k][0] & 0xffff0000u);
+        } else {
+            const uint16_t bits = (uint16_t)(V == 1 || c == 0 ? w[k][0] : w[k][0] >> 16);
+            f16 h;
+            __builtin_memcpy(&h, &bits, 2);
+            return (float)h;
+        }
+    }
+    // What follows makes its 32-bit numbers of the block again: kept from before they would be twice the registers.
+    __device__ __forceinline__ void again()
+    {
+        if (sizeof(T) == 4) return;
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) asm volatile("" : "+v"(w[k][0]));
+    }
 };
 
 // What a lane knows of its columns
@@ -89,10 +127,10 @@ struct Lane {
     int gate;
 };
 template <int V, int G>
-__device__ __forceinline__ Lane<V> lane_of(const ScanArgs &s)
+__device__ __forceinline__ Lane<V> lane_of(const ScanArgs &s, int64_t tile)
 {
     Lane<V> l;
-    l.col = ((int64_t)blockIdx.x * kWave + lane_id()) * V;
+    l.col = (tile * kWave + lane_id()) * V;
     l.in = l.col < s.columns;
     const int64_t q = l.in ? l.col : 0;   // (a lane without columns reads those of the first one and writes nothing)
     l.b = (int32_t)(q / s.dim);
@@ -160,7 +198,7 @@ __global__ void __launch_bounds__(kMaxWaves * kWave) scan_fwd_kernel(const ScanA
     constexpr int VA = G == kEach ? V : 1;
     __shared__ Tell<V> tell;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), waves = blockDim.x / kWave;
-    const Lane<V> l = lane_of<V, G>(s);
+    const Lane<V> l = lane_of<V, G>(s, blockIdx.x);
     const int64_t t_lo = (int64_t)blockIdx.y * s.split_steps, t_hi = min(s.n_steps, t_lo + s.split_steps);
     const TX *x = static_cast<const TX *>(s.x) + (int64_t)l.b * s.x_b + l.ch;
     const TA *a = static_cast<const TA *>(s.a) + (G == kConst ? 0 : (int64_t)l.b * s.a_b) + l.gate;
@@ -198,6 +236,8 @@ __global__ void __launch_bounds__(kMaxWaves * kWave) scan_fwd_kernel(const ScanA
         }
         exchange<V>(tell, i, wave, waves, p, e, enter, mine);
         if (t0 >= t_hi) return;
+        xb[i].again();
+        if (G != kConst) ab[i].again();
         if (s.marks && l.in) store_v<float, V>(s.marks + t0 / kSteps * s.columns + l.col, mine);
 #pragma unroll
         for (int k = 0; k < kSteps; ++k) {
@@ -246,6 +286,41 @@ __device__ __forceinline__ float sum_lanes(float v, int lanes)
     return v;
 }
 
+// The last part of a block on the way back, from the gradient `mine` that enters behind its last step
+template <typename TX, typename TA, int V, int G, int VA>
+__device__ __forceinline__ void backward_block(const ScanArgs &s, const Lane<V> &l, const Block<TX, V> &gb, const Block<TA, VA> &ab, const float (&a_const)[V],
+                                               const float (&before)[kSteps][V], int there, int64_t t0, int64_t t_hi, float (&mine)[V], float (&d_const)[V])
+{
+    const int lane = lane_id();
+    TX *dx = static_cast<TX *>(s.dx) + l.col;
+    TA *da = static_cast<TA *>(s.da);
+#pragma unroll
+    for (int k = kSteps - 1; k >= 0; --k) {
+        const int64_t t = t0 + k;
+        float g[V], d[V];
+#pragma unroll
+        for (int c = 0; c < V; ++c) {
+            const float all = gb.get(k, c) + mine[c];
+            g[c] = k < there ? all : 0.0f;   // (behind a sequence's end the gradient of its last state passes through)
+            d[c] = k < there ? all * before[k][c] : 0.0f;
+            mine[c] = (G == kConst ? (k < there ? a_const[c] : 1.0f) : ab.get(k, c)) * all;
+            if (G == kConst) d_const[c] += d[c];
+        }
+        const bool write = t < t_hi && l.in;
+        if (write) store_v<TX, V>(dx + t * s.columns, g);
+        if (G == kEach && write) store_v<TA, V>(da + t * s.columns + l.col, d);
+        if (G == kShared) {
+            const float sum = sum_lanes(V == 2 ? d[0] + d[V - 1] : d[0], s.seg_lanes);
+            if (write && (lane & (s.seg_lanes - 1)) == 0) {
+                // a gate's channels within the lanes: its gradient; else parts of it, to be joined
+                const int64_t at = (t * s.sequences + l.b) * s.parts;
+                if (s.da_part) s.da_part[at + l.ch / (V * s.seg_lanes)] = sum;
+                else da[at + l.gate] = (TA)sum;
+            }
+        }
+    }
+}
+
 // On the way back the state is c[t] = a[t] (dh[t] + c[t + 1]), what a gradient that enters behind step t becomes before it.
 template <typename TX, typename TA, int V, int G>
 __global__ void __launch_bounds__(kMaxWaves * kWave, 4) scan_bwd_kernel(const ScanArgs s)
@@ -253,13 +328,11 @@ __global__ void __launch_bounds__(kMaxWaves * kWave, 4) scan_bwd_kernel(const Sc
     constexpr int VA = G == kEach ? V : 1;
     __shared__ Tell<V> tell;
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), waves = blockDim.x / kWave;
-    const Lane<V> l = lane_of<V, G>(s);
+    const Lane<V> l = lane_of<V, G>(s, blockIdx.x);
     const int64_t t_lo = (int64_t)blockIdx.y * s.split_steps, t_hi = min(s.n_steps, t_lo + s.split_steps);
     const TX *x = static_cast<const TX *>(s.x) + (int64_t)l.b * s.x_b + l.ch;
     const TA *a = static_cast<const TA *>(s.a) + (G == kConst ? 0 : (int64_t)l.b * s.a_b) + l.gate;
     const TX *dh = static_cast<const TX *>(s.dh) + (int64_t)l.b * s.dh_b + l.ch;
-    TX *dx = static_cast<TX *>(s.dx) + l.col;
-    TA *da = static_cast<TA *>(s.da);
     float a_const[V], d_const[V];
     if (G == kConst) load_v<TA, V>(a, true, 0.0f, a_const);
     float enter[V];
@@ -304,32 +377,9 @@ __global__ void __launch_bounds__(kMaxWaves * kWave, 4) scan_bwd_kernel(const Sc
 #pragma unroll
             for (int c = 0; c < V; ++c) before[k][c] = __builtin_fmaf(gate(k - 1, c), before[k - 1][c], xb.get(k - 1, c));
         exchange<V>(tell, (int)(round & 1), wave, waves, p, e, enter, mine);
-        if (t0 >= t_hi) continue;
-#pragma unroll
-        for (int k = kSteps - 1; k >= 0; --k) {
-            const int64_t t = t0 + k;
-            float g[V], d[V];
-#pragma unroll
-            for (int c = 0; c < V; ++c) {
-                const float all = gb.get(k, c) + mine[c];
-                g[c] = k < there ? all : 0.0f;   // (behind a sequence's end the gradient of its last state passes through)
-                d[c] = k < there ? all * before[k][c] : 0.0f;
-                mine[c] = gate(k, c) * all;
-                if (G == kConst) d_const[c] += d[c];
-            }
-            const bool write = t < t_hi && l.in;
-            if (write) store_v<TX, V>(dx + t * s.columns, g);
-            if (G == kEach && write) store_v<TA, V>(da + t * s.columns + l.col, d);
-            if (G == kShared) {
-                const float sum = sum_lanes(V == 2 ? d[0] + d[V - 1] : d[0], s.seg_lanes);
-                if (write && (lane & (s.seg_lanes - 1)) == 0) {
-                    // a gate's channels within the lanes: its gradient; else parts of it, to be joined
-                    const int64_t at = (t * s.sequences + l.b) * s.parts;
-                    if (s.da_part) s.da_part[at + l.ch / (V * s.seg_lanes)] = sum;
-                    else da[at + l.gate] = (TA)sum;
-                }
-            }
-        }
+        gb.again();
+        if (G != kConst) ab.again();
+        if (t0 < t_hi) backward_block<TX, TA, V, G>(s, l, gb, ab, a_const, before, there, t0, t_hi, mine, d_const);
     }
     if (l.in && wave == 0 && blockIdx.y == 0 && s.d_state) store_v<float, V>(s.d_state + l.col, enter);
     if (G == kConst) {
@@ -355,7 +405,7 @@ __global__ void __launch_bounds__(kMaxWaves * kWave) scan_sums_kernel(const Scan
     constexpr int VA = G == kEach ? V : 1;
     __shared__ Tell<V> tell;
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), waves = blockDim.x / kWave;
-    const Lane<V> l = lane_of<V, G>(s);
+    const Lane<V> l = lane_of<V, G>(s, blockIdx.x);
     // (stretch blockIdx.y, on the way back + 1: what the last one to be passed does, nobody asks)
     const int stretch = blockIdx.y + (kBack ? 1 : 0);
     const int64_t t_lo = (int64_t)stretch * s.split_steps, t_hi = min(s.n_steps, t_lo + s.split_steps);
@@ -430,6 +480,280 @@ __global__ void __launch_bounds__(kMaxWaves * kWave) scan_sums_kernel(const Scan
     if (wave == 0 && l.in) {
         store_v<float, V>(s.sums + (int64_t)(2 * stretch) * s.columns + l.col, product);
         store_v<float, V>(s.sums + (int64_t)(2 * stretch + 1) * s.columns + l.col, end);
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// Long sequences of few columns in one pass over the data.  A workgroup holds a stretch, one block a wavefront, in registers, and tells
+// what it does to a state (product, end from zero) as soon as it knows; what enters it follows from the stretches of its group of kGroup before it and from
+// the state that entered the group, which the last workgroup of the group before tells.  So every sum is made in an order that is
+// fixed, and the way from one group to the next is all that happens one after the other.
+//
+// Workgroups take their stretches by a counter, in the order in which the state passes: what one waits for comes from workgroups that have begun before
+// it and wait for earlier ones only, so every wait ends, however few run at once.  Values are told as 64 bits at a time, all ones being none yet.
+constexpr int kChainWaves = 8, kGroup = 16, kChainLeast = 6;
+constexpr uint64_t kNone = ~0ull;
+
+struct Chain {
+    uint64_t *stretch;   // [stretches][columns]: product and end
+    uint64_t *group;     // [groups + 1][columns]: the state that enters
+    uint32_t *counter;
+    int64_t tiles, stretches;
+};
+
+constexpr int kClear = 4;   // values of a thread
+__global__ void __launch_bounds__(kBlock) chain_clear_kernel(uint64_t *p, int64_t n, uint32_t *counter)
+{
+    const int64_t first = (int64_t)blockIdx.x * kBlock * kClear + threadIdx.x;
+#pragma unroll
+    for (int k = 0; k < kClear; ++k)
+        if (first + k * kBlock < n) p[first + k * kBlock] = kNone;
+    if (first == 0) *counter = 0;
+}
+
+template <int V>
+__device__ __forceinline__ void say(uint64_t *p, const float (&hi)[V], const float (&lo)[V])
+{
+#pragma unroll
+    for (int c = 0; c < V; ++c) {
+        // (a NaN of all ones in both would be taken for none)
+        const uint32_t h = hi[c] != hi[c] ? 0x7fc00000u : __float_as_uint(hi[c]);
+        __hip_atomic_store(p + c, ((uint64_t)h << 32) | __float_as_uint(lo[c]), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    }
+}
+// K values as they are told; the loop's bound is never met (see above), and would show as NaN
+template <int V, int K>
+__device__ __forceinline__ void hear(const uint64_t *const (&p)[K], const bool (&asked)[K], uint64_t (&v)[K][V])
+{
+#pragma unroll
+    for (int k = 0; k < K; ++k)
+#pragma unroll
+        for (int c = 0; c < V; ++c) v[k][c] = 0;
+    for (int tries = 0; tries < (1 << 22); ++tries) {
+        bool some = false;
+#pragma unroll
+        for (int k = 0; k < K; ++k)
+            if (asked[k])
+#pragma unroll
+                for (int c = 0; c < V; ++c) {
+                    v[k][c] = __hip_atomic_load(p[k] + c, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+                    some = some || v[k][c] == kNone;
+                }
+        if (__ballot(some) == 0) return;
+        __builtin_amdgcn_s_sleep(2);
+    }
+}
+
+// What a stretch's wavefronts know of one another
+template <int V>
+struct ChainShared {
+    float block[kChainWaves][2][V][kWave];    // of the stretch: product, end
+    float before[kChainWaves][2][V][kWave];   // of the stretches before it in its group, a part of them each
+    float group[V][kWave];                    // the state that entered the group
+    uint32_t ticket;
+};
+
+// The state that enters this wavefront's block: `mine`.  order: how many stretches come before.  `given`: what enters the first one.  Whoever is last of all
+// leaves the end state in `last`.
+template <int V>
+__device__ __forceinline__ void chain(ChainShared<V> &sh, const Chain &ch, const Lane<V> &l, int64_t columns, int64_t order, int wave, const float (&p)[V],
+                                      const float (&e)[V], const float *given, float *last, float (&mine)[V])
+{
+    const int lane = lane_id();
+#pragma unroll
+    for (int c = 0; c < V; ++c) sh.block[wave][0][c][lane] = p[c], sh.block[wave][1][c][lane] = e[c];
+    __syncthreads();
+    // the blocks before this one, and the whole stretch
+    float pp[V], pe[V], wp[V], we[V];
+#pragma unroll
+    for (int c = 0; c < V; ++c) wp[c] = 1.0f, we[c] = 0.0f;
+#pragma unroll
+    for (int w = 0; w < kChainWaves; ++w) {
+        if (w == wave)
+#pragma unroll
+            for (int c = 0; c < V; ++c) pp[c] = wp[c], pe[c] = we[c];
+#pragma unroll
+        for (int c = 0; c < V; ++c) {
+            const float bp = sh.block[w][0][c][lane];
+            we[c] = passed(bp, we[c]) + sh.block[w][1][c][lane];
+            wp[c] *= bp;
+        }
+    }
+    if (wave == 0 && l.in) say<V>(ch.stretch + order * columns + l.col, wp, we);
+    // a part of the group's stretches before
+    constexpr int kPart = kGroup / kChainWaves;
+    const int64_t group = order / kGroup, first = group * kGroup + wave * kPart;
+    {
+        const uint64_t *from[kPart];
+        bool asked[kPart];
+        uint64_t v[kPart][V];
+#pragma unroll
+        for (int k = 0; k < kPart; ++k) {
+            asked[k] = l.in && first + k < order;
+            from[k] = ch.stretch + (asked[k] ? (first + k) * columns + l.col : 0);
+        }
+        hear<V, kPart>(from, asked, v);
+        float fp[V], fe[V];
+#pragma unroll
+        for (int c = 0; c < V; ++c) fp[c] = 1.0f, fe[c] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kPart; ++k)
+            if (asked[k])
+#pragma unroll
+                for (int c = 0; c < V; ++c) {
+                    const float sp = __uint_as_float((uint32_t)(v[k][c] >> 32));
+                    fe[c] = passed(sp, fe[c]) + __uint_as_float((uint32_t)v[k][c]);
+                    fp[c] *= sp;
+                }
+#pragma unroll
+        for (int c = 0; c < V; ++c) sh.before[wave][0][c][lane] = fp[c], sh.before[wave][1][c][lane] = fe[c];
+    }
+    if (wave == kChainWaves - 1) {
+        float h[V];
+#pragma unroll
+        for (int c = 0; c < V; ++c) h[c] = 0.0f;
+        if (group == 0) {
+            if (given && l.in) load_v<float, V>(given + l.col, true, 0.0f, h);
+        } else {
+            const uint64_t *from[1] = {ch.group + (l.in ? group * columns + l.col : 0)};
+            const bool asked[1] = {l.in};
+            uint64_t v[1][V];
+            hear<V, 1>(from, asked, v);
+#pragma unroll
+            for (int c = 0; c < V; ++c) h[c] = __uint_as_float((uint32_t)v[0][c]);
+        }
+#pragma unroll
+        for (int c = 0; c < V; ++c) sh.group[c][lane] = h[c];
+    }
+    __syncthreads();
+    float h[V];
+#pragma unroll
+    for (int c = 0; c < V; ++c) {
+        h[c] = sh.group[c][lane];
+#pragma unroll
+        for (int w = 0; w < kChainWaves; ++w) h[c] = passed(sh.before[w][0][c][lane], h[c]) + sh.before[w][1][c][lane];
+        mine[c] = passed(pp[c], h[c]) + pe[c];
+    }
+    const bool ends = order == ch.stretches - 1;
+    if (wave == 0 && l.in && (ends || order % kGroup == kGroup - 1)) {
+        float out[V], zero[V];
+#pragma unroll
+        for (int c = 0; c < V; ++c) out[c] = passed(wp[c], h[c]) + we[c], zero[c] = 0.0f;
+        if (!ends) say<V>(ch.group + (group + 1) * columns + l.col, zero, out);
+        else if (last) store_v<float, V>(last + l.col, out);
+    }
+}
+
+template <typename TX, typename TA, int V, int G>
+__global__ void __launch_bounds__(kChainWaves * kWave, 4) scan_fwd_chain_kernel(const ScanArgs s, const Chain ch)
+{
+    constexpr int VA = G == kEach ? V : 1;
+    __shared__ ChainShared<V> sh;
+    const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
+    if (threadIdx.x == 0) sh.ticket = __hip_atomic_fetch_add(ch.counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    const int64_t ticket = __builtin_amdgcn_readfirstlane((int)sh.ticket), order = ticket / ch.tiles;
+    const Lane<V> l = lane_of<V, G>(s, ticket - order * ch.tiles);
+    const int64_t t0 = (order * kChainWaves + wave) * kSteps, t_hi = s.n_steps;
+    const TA *a = static_cast<const TA *>(s.a) + (G == kConst ? 0 : (int64_t)l.b * s.a_b) + l.gate;
+    Block<TX, V> xb;
+    Block<TA, VA> ab;
+    const int64_t last = max(min(t_hi, (int64_t)l.longest) - 1, (int64_t)0);
+    xb.load(static_cast<const TX *>(s.x) + (int64_t)l.b * s.x_b + l.ch, s.x_t, t0, last);
+    if (G != kConst) ab.load(a, s.a_t, t0, last);
+    float a_const[V];
+    if (G == kConst) load_v<TA, V>(a, true, 0.0f, a_const);
+    const int there = (int)min(max(min((int64_t)l.len, t_hi) - t0, (int64_t)0), (int64_t)kSteps);
+    if (__ballot(there < kSteps) != 0) {
+        xb.cut(there, 0.0f);
+        if (G != kConst) ab.cut(there, 1.0f);
+    }
+    auto gate = [&](int k, int c) { return G == kConst ? (k < there ? a_const[c] : 1.0f) : ab.get(k, c); };
+    float p[V], e[V], mine[V];
+#pragma unroll
+    for (int c = 0; c < V; ++c) {
+        p[c] = 1.0f, e[c] = 0.0f;
+#pragma unroll
+        for (int k = 0; k < kSteps; ++k) e[c] = __builtin_fmaf(gate(k, c), e[c], xb.get(k, c)), p[c] *= gate(k, c);
+    }
+    chain<V>(sh, ch, l, s.columns, order, wave, p, e, s.state, s.last, mine);
+    if (t0 >= t_hi || !l.in) return;
+    xb.again();
+    if (G != kConst) ab.again();
+    if (s.marks) store_v<float, V>(s.marks + t0 / kSteps * s.columns + l.col, mine);
+    TX *h = static_cast<TX *>(s.h) + l.col;
+#pragma unroll
+    for (int k = 0; k < kSteps; ++k) {
+        float out[V];
+#pragma unroll
+        for (int c = 0; c < V; ++c) {
+            mine[c] = __builtin_fmaf(gate(k, c), mine[c], xb.get(k, c));
+            out[c] = k < there ? mine[c] : 0.0f;
+        }
+        if (t0 + k < t_hi) store_v<TX, V>(h + (t0 + k) * s.columns, out);
+    }
+}
+
+template <typename TX, typename TA, int V, int G>
+__global__ void __launch_bounds__(kChainWaves * kWave, 4) scan_bwd_chain_kernel(const ScanArgs s, const Chain ch)
+{
+    constexpr int VA = G == kEach ? V : 1;
+    __shared__ ChainShared<V> sh;
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
+    if (threadIdx.x == 0) sh.ticket = __hip_atomic_fetch_add(ch.counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+    __syncthreads();
+    const int64_t ticket = __builtin_amdgcn_readfirstlane((int)sh.ticket), order = ticket / ch.tiles;
+    const Lane<V> l = lane_of<V, G>(s, ticket - order * ch.tiles);
+    // from the last block on
+    const int64_t stretch = ch.stretches - 1 - order, t0 = (stretch * kChainWaves + kChainWaves - 1 - wave) * kSteps, t_hi = s.n_steps;
+    const TA *a = static_cast<const TA *>(s.a) + (G == kConst ? 0 : (int64_t)l.b * s.a_b) + l.gate;
+    Block<TX, V> xb, gb;
+    Block<TA, VA> ab;
+    const int64_t last = max(min(t_hi, (int64_t)l.longest) - 1, (int64_t)0);
+    gb.load(static_cast<const TX *>(s.dh) + (int64_t)l.b * s.dh_b + l.ch, s.dh_t, t0, last);
+    if (G != kConst) ab.load(a, s.a_t, t0, last);
+    xb.load(static_cast<const TX *>(s.x) + (int64_t)l.b * s.x_b + l.ch, s.x_t, t0, last);
+    float a_const[V], d_const[V];
+    if (G == kConst) load_v<TA, V>(a, true, 0.0f, a_const);
+    const int there = l.in ? (int)min(max(min((int64_t)l.len, t_hi) - t0, (int64_t)0), (int64_t)kSteps) : 0;
+    if (__ballot(there < kSteps) != 0) {
+        gb.cut(there, 0.0f);
+        xb.cut(there, 0.0f);
+        if (G != kConst) ab.cut(there, 1.0f);
+    }
+    auto gate = [&](int k, int c) { return G == kConst ? (k < there ? a_const[c] : 1.0f) : ab.get(k, c); };
+    float p[V], e[V], mine[V], before[kSteps][V];
+    if (l.in && t0 < t_hi) load_v<float, V>(s.marks + t0 / kSteps * s.columns + l.col, true, 0.0f, before[0]);
+    else
+#pragma unroll
+        for (int c = 0; c < V; ++c) before[0][c] = 0.0f;
+#pragma unroll
+    for (int c = 0; c < V; ++c) {
+        d_const[c] = 0.0f;
+        p[c] = 1.0f, e[c] = 0.0f;
+#pragma unroll
+        for (int k = kSteps - 1; k >= 0; --k) e[c] = gate(k, c) * (gb.get(k, c) + e[c]), p[c] *= gate(k, c);
+    }
+    chain<V>(sh, ch, l, s.columns, order, wave, p, e, s.d_last, s.d_state, mine);
+    gb.again();
+    if (G != kConst) ab.again();
+    // the states before each step, again from the kept one
+#pragma unroll
+    for (int k = 1; k < kSteps; ++k)
+#pragma unroll
+        for (int c = 0; c < V; ++c) before[k][c] = __builtin_fmaf(gate(k - 1, c), before[k - 1][c], xb.get(k - 1, c));
+    if (t0 < t_hi) backward_block<TX, TA, V, G>(s, l, gb, ab, a_const, before, there, t0, t_hi, mine, d_const);
+    if (G == kConst) {
+        // the wavefronts' sums together, in order
+        __syncthreads();
+#pragma unroll
+        for (int c = 0; c < V; ++c) sh.block[wave][0][c][lane] = d_const[c];
+        __syncthreads();
+        if (wave != 0 || !l.in) return;
+        for (int w = 1; w < kChainWaves; ++w)
+#pragma unroll
+            for (int c = 0; c < V; ++c) d_const[c] += sh.block[w][0][c][lane];
+        store_v<float, V>(s.da_part + order * s.columns + l.col, d_const);
     }
 }
 
@@ -510,6 +834,12 @@ constexpr int kFillBlocks = 512;   // workgroups that fill the chip
 struct Plan {
     int v, waves, seg_lanes, parts;
     int64_t tiles, splits, split_steps;
+    int64_t chained;   // stretches of a chain; 0: two passes where there are stretches
+    int64_t parts_const() const { return chained ? chained : splits; }
+    int64_t sums_floats(int64_t columns) const
+    {
+        return chained ? 2 * (columns * (chained + chained / kGroup + 1) + 1) : splits > 1 ? 2 * splits * columns : 0;
+    }
 };
 
 Plan plan_of(int64_t n_steps, int64_t batch, int32_t dim, int32_t groups, int32_t dtype, bool pairs)
@@ -528,6 +858,11 @@ Plan plan_of(int64_t n_steps, int64_t batch, int32_t dim, int32_t groups, int32_
     if (s < 1) s = 1;
     p.split_steps = div_up(div_up(n_steps, s), round) * round;
     p.splits = div_up(n_steps, p.split_steps);
+    // A chain reads everything once, and has its clearing and its waits: for sequences of some stretches.  Forward, chain / two passes, us: 300 x 64 x 256 bf16
+    // (3 stretches) 15.1 / 13.9; 600 x 32 x 64 fp32 9.4 / 9.4; 1,024 x 4 x 512 bf16 10.5 / 11.6; 4,096 x 256 10.5 / 16.9; 65,536 x 1,000 115 / 156
+    p.chained = div_up(n_steps, kChainWaves * kSteps);
+    if (p.splits > 1 && p.chained >= kChainLeast) p.splits = 1;
+    else p.chained = 0;
     p.seg_lanes = p.parts = 0;
     if (groups > 0 && groups != dim) {
         const int seg = gcd(channels, kWave * p.v);
@@ -558,8 +893,8 @@ extern "C" int64_t bmtk_gated_scan_workspace_bytes(int64_t n_steps, int64_t batc
     int64_t most = 0;
     for (int pairs = 0; pairs < 2; ++pairs) {
         const Plan p = plan_of(n_steps, batch, dim, groups, BMTK_BF16, pairs != 0);
-        int64_t floats = p.splits > 1 ? 2 * p.splits * batch * dim : 0;
-        if (backward && groups == 0) floats += p.splits * batch * dim;
+        int64_t floats = p.sums_floats(batch * dim);
+        if (backward && groups == 0) floats += p.parts_const() * batch * dim;
         if (backward && groups > 0 && groups != dim && p.parts != groups) floats += n_steps * batch * p.parts;
         most = floats > most ? floats : most;
     }
@@ -573,8 +908,28 @@ extern "C" int64_t bmtk_gated_scan_workspace_bytes(int64_t n_steps, int64_t batc
         else hipLaunchKernelGGL((KERNEL<TX, TA, V, kShared __VA_ARGS__>), grid, dim3(p.waves *kWave), 0, st, s);                               \
     } while (0)
 #define BMTK_COMMA ,
+#define BMTK_CHAIN_LAUNCH(KERNEL)                                                                                             \
+    do {                                                                                                                      \
+        const dim3 grid((unsigned)(p.tiles * p.chained)), block(kChainWaves *kWave);                                          \
+        if (groups == 0) hipLaunchKernelGGL((KERNEL<TX, TA, V, kConst>), grid, block, 0, st, s, ch);                          \
+        else if (groups == dim) hipLaunchKernelGGL((KERNEL<TX, TA, V, kEach>), grid, block, 0, st, s, ch);                    \
+        else hipLaunchKernelGGL((KERNEL<TX, TA, V, kShared>), grid, block, 0, st, s, ch);                                     \
+    } while (0)
 
 namespace {
+
+// (`sums` is the chain's: its values, and the counter behind them)
+Chain chain_of(const ScanArgs &s, const Plan &p, hipStream_t st)
+{
+    Chain ch;
+    ch.tiles = p.tiles, ch.stretches = p.chained;
+    ch.stretch = reinterpret_cast<uint64_t *>(s.sums);
+    ch.group = ch.stretch + p.chained * s.columns;
+    const int64_t values = (p.chained + p.chained / kGroup + 1) * s.columns;
+    ch.counter = reinterpret_cast<uint32_t *>(ch.stretch + values);
+    hipLaunchKernelGGL(chain_clear_kernel, dim3((unsigned)div_up(values, kBlock * kClear)), dim3(kBlock), 0, st, ch.stretch, values, ch.counter);
+    return ch;
+}
 
 template <typename TX, typename TA, int V>
 void launch_fwd(const ScanArgs &s, const Plan &p, int groups, hipStream_t st)
@@ -585,6 +940,11 @@ void launch_fwd(const ScanArgs &s, const Plan &p, int groups, hipStream_t st)
         if (groups == 0) hipLaunchKernelGGL((scan_one_kernel<TX, TA, V, kConst>), one, dim3(kBlock), 0, st, s);
         else if (groups == dim) hipLaunchKernelGGL((scan_one_kernel<TX, TA, V, kEach>), one, dim3(kBlock), 0, st, s);
         else hipLaunchKernelGGL((scan_one_kernel<TX, TA, V, kShared>), one, dim3(kBlock), 0, st, s);
+        return;
+    }
+    if (p.chained) {
+        const Chain ch = chain_of(s, p, st);
+        BMTK_CHAIN_LAUNCH(scan_fwd_chain_kernel);
         return;
     }
     dim3 grid((unsigned)p.tiles, (unsigned)p.splits);
@@ -601,15 +961,20 @@ void launch_bwd(ScanArgs s, const Plan &p, int groups, hipStream_t st)
 {
     const int dim = s.dim;
     const int64_t batch = s.columns / dim;
-    dim3 grid((unsigned)p.tiles, (unsigned)p.splits);
-    if (p.splits > 1) {
-        grid.y = (unsigned)p.splits - 1;
-        BMTK_SCAN_LAUNCH(scan_sums_kernel, BMTK_COMMA true);
-        grid.y = (unsigned)p.splits;
+    if (p.chained) {
+        const Chain ch = chain_of(s, p, st);
+        BMTK_CHAIN_LAUNCH(scan_bwd_chain_kernel);
+    } else {
+        dim3 grid((unsigned)p.tiles, (unsigned)p.splits);
+        if (p.splits > 1) {
+            grid.y = (unsigned)p.splits - 1;
+            BMTK_SCAN_LAUNCH(scan_sums_kernel, BMTK_COMMA true);
+            grid.y = (unsigned)p.splits;
+        }
+        BMTK_SCAN_LAUNCH(scan_bwd_kernel, );
     }
-    BMTK_SCAN_LAUNCH(scan_bwd_kernel, );
     if (groups == 0)
-        hipLaunchKernelGGL((scan_join_const_kernel<TA>), dim3((unsigned)div_up(dim, kWave)), dim3(kJoinWaves * kWave), 0, st, s.da_part, p.splits * batch, dim,
+        hipLaunchKernelGGL((scan_join_const_kernel<TA>), dim3((unsigned)div_up(dim, kWave)), dim3(kJoinWaves * kWave), 0, st, s.da_part, p.parts_const() * batch, dim,
                            (TA *)s.da);
     else if (s.da_part)
         hipLaunchKernelGGL((scan_join_shared_kernel<TA>), dim3((unsigned)div_up(s.n_steps * batch * groups, kBlock)), dim3(kBlock), 0, st, s.da_part,
@@ -657,7 +1022,8 @@ extern "C" int bmtk_gated_scan_fwd(int64_t n_steps, int64_t batch, int32_t dim, 
     bool pairs = in_pairs(x, dtype, x_t, x_b) && in_pairs(h, dtype, 0, 0) && aligned(state, 8) && aligned(last, 8) && aligned(marks, 8);
     if (groups == dim || groups == 0) pairs = pairs && in_pairs(decay, gate_dtype, a_t, a_b);
     const Plan p = plan_of(n_steps, batch, dim, groups, dtype, pairs);
-    BMTK_REQUIRE(p.splits == 1 || n_steps == 1 || workspace, "gated_scan_fwd: needs its workspace");
+    BMTK_REQUIRE(p.sums_floats(batch * dim) == 0 || n_steps == 1 || (workspace && aligned(workspace, 8)), "gated_scan_fwd: needs its workspace");
+    BMTK_REQUIRE(p.tiles * p.chained < (1 << 22), "gated_scan_fwd: too many steps and columns");
     ScanArgs s{};
     s.x = x, s.a = decay, s.state = state, s.lengths = lengths, s.h = h, s.last = last, s.marks = marks, s.sums = workspace;
     s.n_steps = n_steps, s.columns = batch * dim, s.split_steps = p.split_steps;
@@ -683,11 +1049,12 @@ extern "C" int bmtk_gated_scan_bwd(int64_t n_steps, int64_t batch, int32_t dim, 
     if (groups == dim || groups == 0) pairs = pairs && in_pairs(decay, gate_dtype, a_t, a_b) && in_pairs(d_decay, gate_dtype, 0, 0);
     const Plan p = plan_of(n_steps, batch, dim, groups, dtype, pairs);
     const bool joined = groups == 0 || (groups != dim && p.parts != groups);
-    BMTK_REQUIRE((p.splits == 1 && !joined) || workspace, "gated_scan_bwd: needs its workspace");
+    BMTK_REQUIRE((p.sums_floats(batch * dim) == 0 && !joined) || (workspace && aligned(workspace, 8)), "gated_scan_bwd: needs its workspace");
+    BMTK_REQUIRE(p.tiles * p.chained < (1 << 22), "gated_scan_bwd: too many steps and columns");
     ScanArgs s{};
     s.x = x, s.a = decay, s.lengths = lengths, s.marks = const_cast<float *>(marks), s.dh = dh, s.d_last = d_last;
     s.dx = dx, s.da = d_decay, s.d_state = d_state, s.sums = workspace;
-    if (joined) s.da_part = workspace + (p.splits > 1 ? 2 * p.splits * batch * dim : 0);
+    if (joined) s.da_part = workspace + p.sums_floats(batch * dim);
     s.n_steps = n_steps, s.columns = batch * dim, s.split_steps = p.split_steps;
     s.x_t = x_t, s.x_b = x_b, s.a_t = a_t, s.a_b = a_b, s.dh_t = dh_t, s.dh_b = dh_b;
     s.dim = dim, s.channels = groups > 0 ? dim / groups : 1, s.sequences = batch, s.seg_lanes = p.seg_lanes, s.parts = p.parts;

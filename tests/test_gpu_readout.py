@@ -289,6 +289,20 @@ def test_long_sequences_in_stretches(batch, dim, groups, dtype):
     scan_check(*scan_case(6007, batch, dim, groups, dtype, torch.float32, lengths=[6007, 3111]))
 
 
+@pytest.mark.parametrize("dtype,gates,batch,dim,groups,lengths", [
+    (torch.bfloat16, torch.bfloat16, 2, 260, 260, None), (torch.float32, torch.float32, 2, 260, 0, [8200, 5001]), (torch.bfloat16, torch.float32, 1, 520, 8, [8200]),
+    (torch.float16, torch.float16, 2, 260, 26, [4099, 8200]), (torch.bfloat16, torch.bfloat16, 2, 261, 9, [8199, 0])])
+def test_long_sequences_in_one_pass(dtype, gates, batch, dim, groups, lengths):
+    """65 stretches of a chain in five groups, the last one not whole."""
+    scan_check(*scan_case(8200, batch, dim, groups, dtype, gates, lengths=lengths))
+
+
+@pytest.mark.parametrize("dtype,dim,groups", [(torch.float32, 128, 128), (torch.bfloat16, 256, 0), (torch.bfloat16, 256, 4), (torch.float16, 129, 43)])
+def test_stretches_of_several_rounds(dtype, dim, groups):
+    """Many columns: two or three stretches of two rounds and more."""
+    scan_check(*scan_case(700, 64, dim, groups, dtype, dtype, lengths=[700, 300, 0, 511]))
+
+
 @pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
 def test_strides(dtype):
     """[sequences, steps, channels] transposed, parts of wider rows, rows on odd addresses, gates that sequences share, no state."""
