@@ -861,7 +861,7 @@ Plan plan_of(int64_t n_steps, int64_t batch, int32_t dim, int32_t groups, int32_
     // A chain reads everything once, and has its clearing and its waits: for sequences of some stretches.  Forward, chain / two passes, us: 300 x 64 x 256 bf16
     // (3 stretches) 15.1 / 13.9; 600 x 32 x 64 fp32 9.4 / 9.4; 1,024 x 4 x 512 bf16 10.5 / 11.6; 4,096 x 256 10.5 / 16.9; 65,536 x 1,000 115 / 156
     p.chained = div_up(n_steps, kChainWaves * kSteps);
-    if (p.splits > 1 && p.chained >= kChainLeast) p.splits = 1;
+    if (p.splits > 1 && p.chained >= kChainLeast && p.tiles * p.chained < (1 << 22)) p.splits = 1;
     else p.chained = 0;
     p.seg_lanes = p.parts = 0;
     if (groups > 0 && groups != dim) {
@@ -1023,7 +1023,7 @@ extern "C" int bmtk_gated_scan_fwd(int64_t n_steps, int64_t batch, int32_t dim, 
     if (groups == dim || groups == 0) pairs = pairs && in_pairs(decay, gate_dtype, a_t, a_b);
     const Plan p = plan_of(n_steps, batch, dim, groups, dtype, pairs);
     BMTK_REQUIRE(p.sums_floats(batch * dim) == 0 || n_steps == 1 || (workspace && aligned(workspace, 8)), "gated_scan_fwd: needs its workspace");
-    BMTK_REQUIRE(p.tiles * p.chained < (1 << 22), "gated_scan_fwd: too many steps and columns");
+    BMTK_REQUIRE(p.tiles * p.waves * kWave < (1ll << 32), "gated_scan_fwd: too many columns");
     ScanArgs s{};
     s.x = x, s.a = decay, s.state = state, s.lengths = lengths, s.h = h, s.last = last, s.marks = marks, s.sums = workspace;
     s.n_steps = n_steps, s.columns = batch * dim, s.split_steps = p.split_steps;
@@ -1050,7 +1050,7 @@ extern "C" int bmtk_gated_scan_bwd(int64_t n_steps, int64_t batch, int32_t dim, 
     const Plan p = plan_of(n_steps, batch, dim, groups, dtype, pairs);
     const bool joined = groups == 0 || (groups != dim && p.parts != groups);
     BMTK_REQUIRE((p.sums_floats(batch * dim) == 0 && !joined) || (workspace && aligned(workspace, 8)), "gated_scan_bwd: needs its workspace");
-    BMTK_REQUIRE(p.tiles * p.chained < (1 << 22), "gated_scan_bwd: too many steps and columns");
+    BMTK_REQUIRE(p.tiles * p.waves * kWave < (1ll << 32), "gated_scan_bwd: too many columns");
     ScanArgs s{};
     s.x = x, s.a = decay, s.lengths = lengths, s.marks = const_cast<float *>(marks), s.dh = dh, s.d_last = d_last;
     s.dx = dx, s.da = d_decay, s.d_state = d_state, s.sums = workspace;

@@ -80,20 +80,18 @@ __device__ __forceinline__ void add_rows(Accumulators<VW, N> &acc, const T *__re
 // Forward.  A workgroup takes one step and a slice of its words of spike bits; a wavefront turns the set bits of 64 kWords words at a
 // time into a queue of element numbers, works it off 64 spikes at a time (each lane divides one of them into neuron and trial),
 // and reads the weight rows, one per spike, 64 * VW channels by its 64 lanes.  The sums of a trial are the wavefront's own, so their
-// order is fixed; the wavefronts' sums are added in order at the end.
+// order is fixed; the wavefronts' sums are added in order at the end, in the LDS that held the queues.
 template <typename T, int VW, int N, int kFwdWaves, int kWords>
 __global__ void __launch_bounds__(kFwdWaves * kWave)
 spike_fwd_kernel(const uint64_t *__restrict__ bits, int64_t stride, int64_t ne, FastDiv by_batch, int trials, int trial_tiles,
                  const T *__restrict__ weight, int dim, int64_t slice_words, T *__restrict__ y, float *__restrict__ part)
 {
-    extern __shared__ float lds[];
-    __shared__ uint32_t queues[kFwdWaves][kQueue];
+    extern __shared__ float lds[];   // the queues, then half of the wavefronts' sums
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave);
     const int64_t t = blockIdx.x;
     const int batch = (int)by_batch.d;
     const int b0 = (int)(blockIdx.z % trial_tiles) * trials, ch0 = (int)(blockIdx.z / trial_tiles) * kWave * VW;
-    const int cells = trials * kWave * VW;
-    uint32_t *queue = queues[wave];
+    uint32_t *queue = reinterpret_cast<uint32_t *>(lds) + wave * kQueue;
     // (a lane without channels of its own reads the first ones and writes nothing)
     const unsigned at_ch = ch0 + lane * VW < dim ? ch0 + lane * VW : 0;
     Accumulators<VW, N> acc;
@@ -131,7 +129,7 @@ spike_fwd_kernel(const uint64_t *__restrict__ bits, int64_t stride, int64_t ne, 
                     const int at = c + k * kWave + lane;
                     w[k] = at < w_count ? next[k] & (at == last_word ? last_mask : ~0ull) : 0;
                 }
-                first = first_element + (uint32_t)((c + lane) << 6);
+                first = first_element + ((uint32_t)(c + lane) << 6);
                 c += kFwdWaves * kStep;
                 load(c, next);
             }
@@ -158,10 +156,27 @@ spike_fwd_kernel(const uint64_t *__restrict__ bits, int64_t stride, int64_t ne, 
         wave_order();
         if (!more && tail == head) break;
     }
-    float *mine = lds + wave * cells;
-    for (int b = 0; b < trials; ++b)
+    // the upper half of the wavefronts' sums to the lower half's, then those together
+    constexpr int kHalf = kFwdWaves / 2;
+    const int cells = trials * kWave * VW;
+    float *slot = lds + (wave % kHalf) * cells;
+    auto put = [&] {
+        for (int b = 0; b < trials; ++b)
 #pragma unroll
-        for (int c = 0; c < VW; ++c) mine[(b * VW + c) * kWave + lane] = acc.get(c, b);
+            for (int c = 0; c < VW; ++c) slot[(b * VW + c) * kWave + lane] = acc.get(c, b);
+    };
+    __syncthreads();
+    if (wave >= kHalf) put();
+    __syncthreads();
+    if (wave < kHalf) {
+        for (int b = 0; b < trials; ++b) {
+            float v[VW];
+#pragma unroll
+            for (int c = 0; c < VW; ++c) v[c] = slot[(b * VW + c) * kWave + lane];
+            acc.add(b, v);
+        }
+        put();   // (its own places)
+    }
     __syncthreads();
     const int here = min(trials, batch - b0);
     const int64_t out = (t * batch + b0) * (int64_t)dim + ch0;
@@ -172,7 +187,7 @@ spike_fwd_kernel(const uint64_t *__restrict__ bits, int64_t stride, int64_t ne, 
         const float *a = lds + (b * VW + l % VW) * kWave + l / VW;
         float s = 0.0f;
 #pragma unroll
-        for (int k = 0; k < kFwdWaves; ++k) s += a[k * cells];
+        for (int k = 0; k < kHalf; ++k) s += a[k * cells];
         if (part)
             part[blockIdx.y * plane + out + (int64_t)b * dim + l] = s;
         else
@@ -671,7 +686,8 @@ extern "C" int bmtk_spike_readout_fwd(const uint64_t *spike_bits, int64_t stride
     const int64_t plane = n_steps * batch * (int64_t)dim;
     BMTK_REQUIRE(plane < (1ll << 31), "spike_readout_fwd: the result is too large");
     const dim3 grid((unsigned)n_steps, (unsigned)p.slices, (unsigned)p.tiles);
-    const size_t lds = (size_t)p.waves * p.trials * kWave * p.vw * sizeof(float);
+    const size_t queues = (size_t)p.waves * kQueue * sizeof(uint32_t), sums = (size_t)p.waves / 2 * p.trials * kWave * p.vw * sizeof(float);
+    const size_t lds = queues > sums ? queues : sums;   // (at most 32 KB)
     const hipStream_t st = (hipStream_t)stream;
     const FastDiv by_batch = fast_div((uint32_t)batch);
 #define BMTK_FWD_W(VW, N, WAVES, WORDS)                                                                                                                      \
