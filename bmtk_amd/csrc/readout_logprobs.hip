@@ -404,6 +404,7 @@ struct RowBwd {
 struct Factors {
     float lse, by_logp, by_entropy, entropy;
     int64_t token;
+    bool none;   // a row without a token whose entropy nobody asks about: nothing, whatever its logits are
 };
 __device__ __forceinline__ Factors factors_of(const RowBwd &a, int64_t r)
 {
@@ -414,6 +415,7 @@ __device__ __forceinline__ Factors factors_of(const RowBwd &a, int64_t r)
     f.by_logp = f.token == a.ignore ? 0.0f : a.d_logp ? a.d_logp[r] : 0.0f;
     f.by_entropy = a.d_entropy ? a.d_entropy[r] : 0.0f;
     if (f.token != a.ignore && (f.token < 0 || f.token >= a.vocab)) f.by_logp = NAN;   // as its log probability is
+    f.none = f.token == a.ignore && f.by_entropy == 0.0f;
     if (f.lse == -INFINITY) f.lse = f.by_logp = f.by_entropy = 0.0f;                      // a row of nothing but -inf: nothing moves it
     return f;
 }
@@ -422,6 +424,7 @@ __device__ __forceinline__ float gradient(const Factors &f, float x, int j)
     const float l = x - f.lse, p = __builtin_amdgcn_exp2f(l * kLog2e);
     float d = -(p * f.by_logp);
     if (p != 0.0f) d -= p * f.by_entropy * (l + f.entropy);   // (of a logit of -inf there is nothing)
+    if (f.none) return 0.0f;
     return j == f.token ? d + f.by_logp : d;
 }
 

@@ -649,7 +649,7 @@ int check_sizes(const char *who, int64_t n_steps, int64_t n, int32_t batch, int3
     BMTK_REQUIRE(n_steps > 0 && n > 0 && batch > 0 && dim > 0, "%s: sizes must be positive", who);
     BMTK_REQUIRE(dtype == BMTK_F32 || dtype == BMTK_BF16 || dtype == BMTK_F16, "%s: unknown type %d", who, dtype);
     BMTK_REQUIRE(n < (1ll << 31) && n * (int64_t)batch < (1ll << 31) - 64, "%s: n_neurons * batch must stay below 2^31 - 64", who);
-    BMTK_REQUIRE(n_steps < (1ll << 24) && n_steps * (int64_t)batch < (1ll << 31) - 64, "%s: n_steps must stay below 2^24 and n_steps * batch below 2^31 - 64", who);
+    BMTK_REQUIRE(n_steps < (1ll << 23) && n_steps * (int64_t)batch < (1ll << 31) - 64, "%s: n_steps must stay below 2^23 and n_steps * batch below 2^31 - 64", who);
     BMTK_REQUIRE(dim <= 65536 && batch <= 65536, "%s: batch and dim are at most 65,536", who);
     return BMTK_OK;
 }

@@ -76,8 +76,12 @@ def _contiguous(t, name, dtype=None, shape=None):
     return t
 
 
-def _workspace(n_bytes, device):
-    return torch.empty(n_bytes, dtype=torch.uint8, device=device).data_ptr() if n_bytes else None
+class _Workspace:
+    """Device memory of a call.  (Held until its kernels are enqueued: before that, another call of this stream could be given it.)"""
+
+    def __init__(self, n_bytes, device):
+        self.memory = torch.empty(n_bytes, dtype=torch.uint8, device=device) if n_bytes else None
+        self.ptr = self.memory.data_ptr() if n_bytes else None
 
 
 # ---------------------------------------------------------------------------------------------------------------------
@@ -110,8 +114,8 @@ def spike_readout(bits, weight, batch=1):
     y = torch.empty(steps, batch, dim, dtype=weight.dtype, device=weight.device)
     if steps:
         lib = _lib.load()
-        ws = _workspace(lib.bmtk_spike_readout_workspace_bytes(steps, n, batch, dim, 0), weight.device)
-        _lib.check(lib.bmtk_spike_readout_fwd(bits.data_ptr(), stride, steps, n, batch, weight.data_ptr(), dim, _CODE[weight.dtype], y.data_ptr(), ws, _stream()))
+        ws = _Workspace(lib.bmtk_spike_readout_workspace_bytes(steps, n, batch, dim, 0), weight.device)
+        _lib.check(lib.bmtk_spike_readout_fwd(bits.data_ptr(), stride, steps, n, batch, weight.data_ptr(), dim, _CODE[weight.dtype], y.data_ptr(), ws.ptr, _stream()))
     return y
 
 
@@ -132,8 +136,8 @@ def spike_readout_bwd(bits, weight, dy, batch=1, spikes=True):
         lib, code = _lib.load(), _CODE[weight.dtype]
         _lib.check(lib.bmtk_spike_readout_bwd_weight(bits.data_ptr(), stride, steps, n, batch, dy.data_ptr(), dim, code, d_weight.data_ptr(), _stream()))
         if spikes:
-            ws = _workspace(lib.bmtk_spike_readout_workspace_bytes(steps, n, batch, dim, 1) if code == 0 else 0, dev)
-            _lib.check(lib.bmtk_spike_readout_bwd_spikes(weight.data_ptr(), dy.data_ptr(), steps, n, batch, dim, code, dl_dz.data_ptr(), ws, _stream()))
+            ws = _Workspace(lib.bmtk_spike_readout_workspace_bytes(steps, n, batch, dim, 1) if code == 0 else 0, dev)
+            _lib.check(lib.bmtk_spike_readout_bwd_spikes(weight.data_ptr(), dy.data_ptr(), steps, n, batch, dim, code, dl_dz.data_ptr(), ws.ptr, _stream()))
     return d_weight, dl_dz
 
 
@@ -146,7 +150,7 @@ def _rows(t, name):
 
 
 def _scan(x, decay, lengths):
-    """(steps, sequences, channels, gates, arguments that both directions share)"""
+    """(steps, sequences, channels, gates, arguments that both directions share, the decays that those point to)"""
     _given(x, "x")
     _given(decay, "decay")
     if x.dim() != 3 or x.shape[1] == 0 or x.shape[2] == 0:
@@ -155,7 +159,8 @@ def _scan(x, decay, lengths):
     if decay.dtype != torch.float32 and decay.dtype != x.dtype:
         raise TypeError("decay must be float32 or of the type of x, {}, got {}".format(x.dtype, decay.dtype))
     if decay.dim() == 1 and decay.shape[0] == dim:
-        groups, a = 0, (decay.contiguous().data_ptr(), 0, 0)
+        decay = decay.contiguous()
+        groups, a = 0, (decay.data_ptr(), 0, 0)
     elif decay.dim() == 3 and decay.shape[0] == steps and decay.shape[1] == batch and decay.shape[2] and dim % decay.shape[2] == 0:
         groups, a = decay.shape[2], _rows(decay, "decay")
     else:
@@ -163,7 +168,7 @@ def _scan(x, decay, lengths):
             tuple(decay.shape), tuple(x.shape)))
     if lengths is not None:
         _contiguous(lengths, "lengths", torch.int32, (batch,))
-    return steps, batch, dim, groups, (steps, batch, dim, groups, _CODE[x.dtype], _CODE[decay.dtype]) + _rows(x, "x") + a
+    return steps, batch, dim, groups, (steps, batch, dim, groups, _CODE[x.dtype], _CODE[decay.dtype]) + _rows(x, "x") + a, decay
 
 
 def gated_scan(x, decay, state=None, lengths=None, save_state=False):
@@ -174,14 +179,14 @@ def gated_scan(x, decay, state=None, lengths=None, save_state=False):
     decay   [channels]: one per channel for all steps (a leaky integrator), or [steps, sequences, gates]: the gates of each step, each
             for channels / gates neighbouring channels; of the type of ``x`` or float32.  Of magnitude up to 1
     state   float32 [sequences, channels]: the state before the first step (None: zero)
-    lengths int32 [sequences]: steps of each sequence (None: all).  h is 0 behind them, and nothing of x and decay is read there; values
+    lengths int32 [sequences]: steps of each sequence (None: all).  h is 0 behind them, and nothing of x and decay counts there; values
             outside 0..steps count as the nearer of the two
     h has the type and shape of ``x``, last is float32 [sequences, channels], the state behind each sequence's last step: the ``state``
     of the next call.  saved: what ``gated_scan_bwd`` takes, float32, a sixteenth of h's entries."""
     r = _native.gated_scan(x, decay, state, lengths, save_state)
     if r is not None:
         return r
-    steps, batch, dim, groups, args = _scan(x, decay, lengths)
+    steps, batch, dim, groups, args, decay = _scan(x, decay, lengths)
     if state is not None:
         _contiguous(state, "state", torch.float32, (batch, dim))
     dev = x.device
@@ -190,9 +195,9 @@ def gated_scan(x, decay, state=None, lengths=None, save_state=False):
     saved = torch.empty(-(-steps // _lib.SCAN_MARK), batch, dim, dtype=torch.float32, device=dev) if save_state else None
     if steps:
         lib = _lib.load()
-        ws = _workspace(lib.bmtk_gated_scan_workspace_bytes(steps, batch, dim, groups, 0), dev)
+        ws = _Workspace(lib.bmtk_gated_scan_workspace_bytes(steps, batch, dim, groups, 0), dev)
         _lib.check(lib.bmtk_gated_scan_fwd(*args, state.data_ptr() if state is not None else None, lengths.data_ptr() if lengths is not None else None,
-                                           h.data_ptr(), last.data_ptr(), saved.data_ptr() if save_state else None, ws, _stream()))
+                                           h.data_ptr(), last.data_ptr(), saved.data_ptr() if save_state else None, ws.ptr, _stream()))
     elif state is not None:
         last.copy_(state)
     else:
@@ -210,7 +215,7 @@ def gated_scan_bwd(x, decay, saved, dh, d_last=None, lengths=None):
     r = _native.gated_scan_bwd(x, decay, saved, dh, d_last, lengths)
     if r is not None:
         return r
-    steps, batch, dim, groups, args = _scan(x, decay, lengths)
+    steps, batch, dim, groups, args, decay = _scan(x, decay, lengths)
     if _given(dh, "dh", x.dtype).shape != x.shape:
         raise ValueError("dh must be {}, got {}".format(tuple(x.shape), tuple(dh.shape)))
     _contiguous(saved, "saved", torch.float32, (-(-steps // _lib.SCAN_MARK), batch, dim))
@@ -222,9 +227,9 @@ def gated_scan_bwd(x, decay, saved, dh, d_last=None, lengths=None):
     d_state = torch.empty(batch, dim, dtype=torch.float32, device=dev)
     if steps:
         lib = _lib.load()
-        ws = _workspace(lib.bmtk_gated_scan_workspace_bytes(steps, batch, dim, groups, 1), dev)
+        ws = _Workspace(lib.bmtk_gated_scan_workspace_bytes(steps, batch, dim, groups, 1), dev)
         _lib.check(lib.bmtk_gated_scan_bwd(*args, saved.data_ptr(), lengths.data_ptr() if lengths is not None else None, *_rows(dh, "dh"),
-                                           d_last.data_ptr() if d_last is not None else None, dx.data_ptr(), d_decay.data_ptr(), d_state.data_ptr(), ws, _stream()))
+                                           d_last.data_ptr() if d_last is not None else None, dx.data_ptr(), d_decay.data_ptr(), d_state.data_ptr(), ws.ptr, _stream()))
     elif d_last is not None:
         d_state.copy_(d_last)
     else:
@@ -278,9 +283,9 @@ def token_logprobs(logits, tokens, top=0, ignore=-100):
     if n:
         lib, code = _lib.load(), _CODE[logits.dtype]
         tokens = tokens.contiguous()
-        ws = _workspace(lib.bmtk_token_logprobs_workspace_bytes(n, vocab, code, top), dev)
+        ws = _Workspace(lib.bmtk_token_logprobs_workspace_bytes(n, vocab, code, top), dev)
         _lib.check(lib.bmtk_token_logprobs_fwd(n, vocab, code, rows.data_ptr(), stride, tokens.data_ptr(), ignore, top, r.logp.data_ptr(), r.entropy.data_ptr(),
-                                               r.lse.data_ptr(), r.top_logp.data_ptr() if top else None, r.top_index.data_ptr() if top else None, ws, _stream()))
+                                               r.lse.data_ptr(), r.top_logp.data_ptr() if top else None, r.top_index.data_ptr() if top else None, ws.ptr, _stream()))
     return r
 
 
@@ -288,8 +293,8 @@ def token_logprobs_bwd(logits, tokens, fwd, d_logp=None, d_entropy=None, ignore=
     """Gradient by the logits, of their type and shape, from those of logp and entropy (float32, of the shape of the tokens; one may be None).
 
     logits, tokens, ignore: as they were; fwd: what ``token_logprobs`` returned.  The alternatives are not differentiated.  Rows without a token get
-    their entropy's gradient only, rows of nothing but -inf none.  out: where to write it; ``logits`` itself is allowed, which then
-    are gone."""
+    their entropy's gradient only (0, whatever their logits, where there is none), rows of nothing but -inf none.  out: where to write
+    it; ``logits`` itself is allowed, which then are gone."""
     if out is None:
         r = _native.token_logprobs_bwd(logits, tokens, fwd.lse, fwd.entropy, d_logp, d_entropy, ignore)
         if r is not None:

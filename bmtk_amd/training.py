@@ -71,6 +71,14 @@ def rate_mse(counts, n_steps, batch, pop_id, targets):
     return loss, g.t()[pop_id].contiguous().view(-1)
 
 
+def _total(t):
+    """Sum of all entries, 1,024 at a time.  (One call for more of them clears memory by an operation that replays of a captured graph do not repeat.)"""
+    t = t.reshape(-1)
+    while t.numel() > 1024:
+        t = torch.nn.functional.pad(t, (0, -t.numel() % 1024)).view(-1, 1024).sum(1)
+    return t.sum()
+
+
 def label_loss(bits, batch, weight, decay, labels, ignore=-100, state=None, top=0):
     """Cross entropy of the labels that a trained readout should answer, and its derivatives.
 
@@ -85,8 +93,8 @@ def label_loss(bits, batch, weight, decay, labels, ignore=-100, state=None, top=
     y = readout.spike_readout(bits, weight, batch)
     h, _, saved = readout.gated_scan(y, decay, state, save_state=True)
     answer = readout.token_logprobs(h, labels, top=top, ignore=ignore)
-    share = 1.0 / (labels != ignore).sum().clamp_(min=1).to(torch.float32)
-    loss = -answer.logp.sum() * share
+    share = 1.0 / _total(labels != ignore).clamp_(min=1).to(torch.float32)
+    loss = -_total(answer.logp) * share
     dh = readout.token_logprobs_bwd(h, labels, answer, d_logp=(-share).expand(labels.shape).contiguous(), ignore=ignore, out=h)
     dy, d_decay, d_state = readout.gated_scan_bwd(y, decay, saved, dh)
     d_weight, dl_dz = readout.spike_readout_bwd(bits, weight, dy, batch)

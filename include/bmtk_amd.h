@@ -710,7 +710,7 @@ int bmtk_rate_mse(const int32_t *counts, int64_t n_neurons, int32_t batch, int64
 
 /* y[t][b][:] = sum of weight[i][:] over the neurons i that fired in step t of trial b.  spike_bits: n_steps rows of `stride` words (bits
  * behind n_neurons * batch are not looked at); weight [n_neurons][dim], y [n_steps][batch][dim], contiguous.
- * Limits: n_neurons * batch < 2^31 - 64, n_steps < 2^24, n_steps * batch < 2^31 - 64, n_steps * batch * dim < 2^31, batch and dim up to 65,536. */
+ * Limits: n_neurons * batch < 2^31 - 64, n_steps < 2^23, n_steps * batch < 2^31 - 64, n_steps * batch * dim < 2^31, batch and dim up to 65,536. */
 int64_t bmtk_spike_readout_workspace_bytes(int64_t n_steps, int64_t n_neurons, int32_t batch, int32_t dim, int32_t backward);
 int bmtk_spike_readout_fwd(const uint64_t *spike_bits, int64_t stride, int64_t n_steps, int64_t n_neurons, int32_t batch, const void *weight, int32_t dim,
                            int32_t dtype, void *y, float *workspace, void *stream);
@@ -723,12 +723,12 @@ int bmtk_spike_readout_bwd_spikes(const void *weight, const void *dy, int64_t n_
                                   float *dl_dz, int32_t *workspace, void *stream);
 
 /* h[t][b][c] = a h[t-1][b][c] + x[t][b][c] for the steps t < lengths[b] (NULL: all n_steps), from state [batch][dim] (NULL: zero); h is 0 behind
- * a sequence's end and nothing of x or decay is read there.  last [batch][dim]: the state behind each sequence's last step.
+ * a sequence's end and nothing of x or decay counts there.  last [batch][dim]: the state behind each sequence's last step.
  * groups: 0: one decay per channel, decay [dim]; else decays per step and sequence, [n_steps][batch][groups], each for dim / groups neighbouring
  * channels.  gate_dtype: the decays' type, BMTK_F32 or dtype.  x_t, x_b, a_t, a_b, dh_t, dh_b: distance of steps and of sequences in x, decay
  * and dh, in elements (a channel's neighbour is next to it); h, dx and d_decay are contiguous.  state, last, d_last, d_state, marks: 32 bits.
  * marks (NULL: not kept): the state before every BMTK_SCAN_MARK-th step, [ceil(n_steps / BMTK_SCAN_MARK)][batch][dim], from which the backward
- * pass computes the others again.  Decays of up to 1 in magnitude, or of which the products over a sequence stay in 32 bits.
+ * pass computes the others again.  Decays of up to 1 in magnitude, or of which the products over any steps in a row stay in 32 bits.
  * Limits: batch * dim < 2^31, n_steps < 2^31 - 4096. */
 #define BMTK_SCAN_MARK 16
 int64_t bmtk_gated_scan_workspace_bytes(int64_t n_steps, int64_t batch, int32_t dim, int32_t groups, int32_t backward);

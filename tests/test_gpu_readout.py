@@ -509,6 +509,23 @@ def test_tokens_that_are_ignored_or_outside(dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("vocab", [10, 300, 3001])
+def test_padding_of_any_content(dtype, vocab):
+    """Rows without a token that hold NaN and infinities: what nobody asks about has no gradient."""
+    x, tokens, dl, de = logits_case(6, vocab, dtype, ignored=0.0)
+    x[1], x[2, 3], x[4, 0] = math.nan, math.inf, math.nan
+    tokens[1:3] = -100
+    r = readout.token_logprobs(x, tokens)
+    de[1:3] = 0.0
+    for d_entropy in (None, de):
+        d = readout.token_logprobs_bwd(x, tokens, r, dl, d_entropy)
+        assert (d[1:3] == 0).all() and d[4].isnan().all()
+        kept = torch.tensor([0, 3, 5])
+        part = readout.LogProbs(*(None if t is None else t[kept] for t in r))
+        assert torch.equal(d[kept], readout.token_logprobs_bwd(x[kept], tokens[kept], part, dl[kept], None if d_entropy is None else de[kept]))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("vocab", [30, 333, 3000, 20000])
 def test_rows_of_any_distance_and_address(vocab, dtype):
     x, tokens, dl, de = logits_case(6, vocab, dtype)
@@ -598,6 +615,22 @@ def _shifted(r, tokens, one):
     return readout.token_logprobs_bwd(both[:3], tokens, r, one, out=both[1:])
 
 
+def test_decays_further_apart():
+    """One decay per channel, every other entry of a tensor: what is computed from must outlive the call's results being made."""
+    dim = 1 << 20
+    g = gen(11)
+    x = torch.randn(2, 1, dim, generator=g).bfloat16().cuda()
+    decay = torch.rand(2 * dim, generator=g).cuda()[::2]
+    for _ in range(3):
+        h, last, saved = readout.gated_scan(x, decay, save_state=True)
+        got = readout.gated_scan_bwd(x, decay, saved, x)
+        want_h, want_last, want_saved = readout.gated_scan(x, decay.clone(), save_state=True)
+        want = readout.gated_scan_bwd(x, decay.clone(), want_saved, x)
+        for p, q in zip((h, last, saved, *got), (want_h, want_last, want_saved, *want)):
+            assert torch.equal(p, q)
+        del h, last, saved, got, want_h, want_last, want_saved, want, p, q
+
+
 def everything(s):
     """One pass of all operations, as a training step makes them; what it returns."""
     y = readout.spike_readout(s["bits"], s["w"], s["batch"])
@@ -647,6 +680,37 @@ def test_captured_and_replayed():
         torch.cuda.synchronize()
         for k, (_, _, out) in enumerate(graphs):
             assert all(torch.equal(p, q) for p, q in zip(out, want[(turn + k) % 3]))
+
+
+def test_label_loss_captured_and_replayed():
+    """Of more labels than one launch sums up."""
+    cases = [chain_case(s, steps=2000, batch=16, n=24) for s in (0, 1)]
+    for c in cases:
+        c["labels"][::3] = -100
+
+    def run(c):
+        loss, dl_dz, grads, answer = training.label_loss(c["bits"], c["batch"], c["w"], c["decay"], c["labels"], state=c["state"], top=1)
+        return [loss, dl_dz, *grads.values(), *answer]
+    want = [[t.clone() for t in run(c)] for c in cases]
+    mean = -(want[0][5].double().sum() / (cases[0]["labels"] != -100).sum()).cpu()
+    close(want[0][0], mean, 20 * U * mean.abs())   # (sums of 1,024, of those and their share: at most 10 + 5 + 3 half steps each way)
+    held = {name: t.clone() if torch.is_tensor(t) else t for name, t in cases[0].items()}
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        run(held)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = run(held)
+    for turn in range(5):
+        for name, t in cases[turn % 2].items():
+            if torch.is_tensor(t):
+                held[name].copy_(t)
+        graph.replay()
+        run(cases[0])
+        torch.cuda.synchronize()
+        assert all(torch.equal(p, q) for p, q in zip(out, want[turn % 2]))
 
 
 def test_two_streams_at_once():

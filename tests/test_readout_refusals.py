@@ -35,7 +35,7 @@ def spikes_fwd(bits=P, stride=100, steps=3, n=10, batch=4, weight=P, dim=8, dtyp
 @pytest.mark.parametrize("change,word", [
     (dict(bits=None), "null"), (dict(weight=None), "null"), (dict(y=None), "null"), (dict(steps=0), "positive"), (dict(n=0), "positive"), (dict(batch=0), "positive"),
     (dict(dim=0), "positive"), (dict(dim=-1), "positive"), (dict(dtype=3), "type"), (dict(dtype=-1), "type"), (dict(stride=0), "stride"), (dict(n=1 << 31), "2^31"),
-    (dict(n=1 << 29, batch=4), "2^31"), (dict(steps=1 << 24), "2^24"), (dict(steps=1 << 23, batch=1 << 9), "2^31"), (dict(dim=65537), "65,536"), (dict(batch=65537), "65,536"),
+    (dict(n=1 << 29, batch=4), "2^31"), (dict(steps=1 << 23), "2^23"), (dict(steps=1 << 22, batch=1 << 9), "2^31"), (dict(dim=65537), "65,536"), (dict(batch=65537), "65,536"),
     (dict(steps=1 << 20, batch=1, n=10, dim=4096), "too large"), (dict(n=1 << 20, batch=1, steps=1, stride=1 << 20, ws=None), "workspace")])
 def test_spike_readout_fwd(change, word):
     refused(spikes_fwd(**change), "spike_readout_fwd", word)
