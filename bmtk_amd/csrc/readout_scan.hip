@@ -7,7 +7,7 @@ namespace bmtk {
 namespace {
 
 constexpr int kSteps = BMTK_SCAN_MARK;  // steps that a wavefront holds in registers; the state before each such block is kept
-constexpr int kMaxWaves = 8;
+constexpr int kMaxWaves = 8, kRoundWaves = 16;   // of a workgroup that takes rounds; of one that takes a single one
 
 // One column is one channel of one sequence: column q = sequence q / dim, channel q % dim.  A lane takes V neighbouring columns.
 struct ScanArgs {
@@ -166,14 +166,14 @@ __device__ __forceinline__ void fold(const float *sums, int64_t columns, const L
 // One pass over the steps of a stretch in rounds: each wavefront takes kSteps steps into registers, finds what they do to a state
 // that enters them, (product of the gates, end from zero), the wavefronts tell each other, and each then computes its steps from the
 // state that really enters.  Everything is read once, a round ahead.
-template <int V>
+template <int V, int kWaves>
 struct Tell {
-    float v[2][kMaxWaves][2][V][kWave];   // [round in turn][wavefront][product, end]
+    float v[2][kWaves][2][V][kWave];   // [round in turn][wavefront][product, end]
 };
 
 // A round's exchange: `enter` is the state before the round and becomes the one behind it; returns in `mine` the one before the wavefront's block
-template <int V>
-__device__ __forceinline__ void exchange(Tell<V> &tell, int turn, int wave, int waves, const float (&p)[V], const float (&e)[V], float (&enter)[V], float (&mine)[V])
+template <int V, int kWaves>
+__device__ __forceinline__ void exchange(Tell<V, kWaves> &tell, int turn, int wave, int waves, const float (&p)[V], const float (&e)[V], float (&enter)[V], float (&mine)[V])
 {
     const int lane = lane_id();
 #pragma unroll
@@ -192,11 +192,14 @@ __device__ __forceinline__ void exchange(Tell<V> &tell, int turn, int wave, int 
     }
 }
 
-template <typename TX, typename TA, int V, int G>
-__global__ void __launch_bounds__(kMaxWaves * kWave) scan_fwd_kernel(const ScanArgs s)
+// (kOne: a single round, of which none has to be read ahead: stretches of 128 steps, 600 x 32 x 64 fp32, 8.3 us
+// against 9.3)
+template <typename TX, typename TA, int V, int G, bool kOne>
+__global__ void __launch_bounds__((kOne ? kRoundWaves : kMaxWaves) * kWave) scan_fwd_kernel(const ScanArgs s)
 {
+    constexpr int kWaves = kOne ? kRoundWaves : kMaxWaves;
     constexpr int VA = G == kEach ? V : 1;
-    __shared__ Tell<V> tell;
+    __shared__ Tell<V, kWaves> tell;
     const int wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), waves = blockDim.x / kWave;
     const Lane<V> l = lane_of<V, G>(s, blockIdx.x);
     const int64_t t_lo = (int64_t)blockIdx.y * s.split_steps, t_hi = min(s.n_steps, t_lo + s.split_steps);
@@ -234,7 +237,7 @@ __global__ void __launch_bounds__(kMaxWaves * kWave) scan_fwd_kernel(const ScanA
 #pragma unroll
             for (int k = 0; k < kSteps; ++k) e[c] = __builtin_fmaf(gate(k, c), e[c], xb[i].get(k, c)), p[c] *= gate(k, c);
         }
-        exchange<V>(tell, i, wave, waves, p, e, enter, mine);
+        exchange(tell, i, wave, waves, p, e, enter, mine);
         if (t0 >= t_hi) return;
         xb[i].again();
         if (G != kConst) ab[i].again();
@@ -253,9 +256,9 @@ __global__ void __launch_bounds__(kMaxWaves * kWave) scan_fwd_kernel(const ScanA
     int64_t t0 = t_lo + wave * kSteps;
     load(0, t0);
     for (int64_t done = t_lo; done < t_hi; done += 2 * round_steps, t0 += 2 * round_steps) {
-        load(1, t0 + round_steps);
+        if (!kOne) load(1, t0 + round_steps);
         round(0, t0);
-        if (done + round_steps >= t_hi) break;
+        if (kOne || done + round_steps >= t_hi) break;
         load(0, t0 + 2 * round_steps);
         round(1, t0 + round_steps);
     }
@@ -323,10 +326,10 @@ __device__ __forceinline__ void backward_block(const ScanArgs &s, const Lane<V> 
 
 // On the way back the state is c[t] = a[t] (dh[t] + c[t + 1]), what a gradient that enters behind step t becomes before it.
 template <typename TX, typename TA, int V, int G>
-__global__ void __launch_bounds__(kMaxWaves * kWave, 4) scan_bwd_kernel(const ScanArgs s)
+__global__ void __launch_bounds__(kRoundWaves * kWave) scan_bwd_kernel(const ScanArgs s)
 {
     constexpr int VA = G == kEach ? V : 1;
-    __shared__ Tell<V> tell;
+    __shared__ Tell<V, kRoundWaves> tell;
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), waves = blockDim.x / kWave;
     const Lane<V> l = lane_of<V, G>(s, blockIdx.x);
     const int64_t t_lo = (int64_t)blockIdx.y * s.split_steps, t_hi = min(s.n_steps, t_lo + s.split_steps);
@@ -376,7 +379,7 @@ __global__ void __launch_bounds__(kMaxWaves * kWave, 4) scan_bwd_kernel(const Sc
         for (int k = 1; k < kSteps; ++k)
 #pragma unroll
             for (int c = 0; c < V; ++c) before[k][c] = __builtin_fmaf(gate(k - 1, c), before[k - 1][c], xb.get(k - 1, c));
-        exchange<V>(tell, (int)(round & 1), wave, waves, p, e, enter, mine);
+        exchange(tell, (int)(round & 1), wave, waves, p, e, enter, mine);
         gb.again();
         if (G != kConst) ab.again();
         if (t0 < t_hi) backward_block<TX, TA, V, G>(s, l, gb, ab, a_const, before, there, t0, t_hi, mine, d_const);
@@ -399,11 +402,11 @@ __global__ void __launch_bounds__(kMaxWaves * kWave, 4) scan_bwd_kernel(const Sc
 // What a whole stretch does, for the stretches that are computed from it: the product of its gates and its end from zero, forwards or backwards.  Each
 // wavefront takes every waves-th block, from the stretch's other end to where the pass proper begins, so that what that pass reads first was
 // read last; the wavefronts' blocks of a round are joined as they come, in the order of time.
-template <typename TX, typename TA, int V, int G, bool kBack>
+template <typename TX, typename TA, int V, int G, bool kBack, bool kOne>
 __global__ void __launch_bounds__(kMaxWaves * kWave) scan_sums_kernel(const ScanArgs s)
 {
     constexpr int VA = G == kEach ? V : 1;
-    __shared__ Tell<V> tell;
+    __shared__ Tell<V, kMaxWaves> tell;
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane((int)threadIdx.x / kWave), waves = blockDim.x / kWave;
     const Lane<V> l = lane_of<V, G>(s, blockIdx.x);
     // (stretch blockIdx.y, on the way back + 1: what the last one to be passed does, nobody asks)
@@ -471,9 +474,9 @@ __global__ void __launch_bounds__(kMaxWaves * kWave) scan_sums_kernel(const Scan
     };
     load(0, 0);
     for (int64_t round = 0; round < rounds; round += 2) {
-        load(1, round + 1);
+        if (!kOne) load(1, round + 1);
         take(0, round);
-        if (round + 1 >= rounds) break;
+        if (kOne || round + 1 >= rounds) break;
         load(0, round + 2);
         take(1, round + 1);
     }
@@ -491,7 +494,7 @@ __global__ void __launch_bounds__(kMaxWaves * kWave) scan_sums_kernel(const Scan
 //
 // Workgroups take their stretches by a counter, in the order in which the state passes: what one waits for comes from workgroups that have begun before
 // it and wait for earlier ones only, so every wait ends, however few run at once.  Values are told as 64 bits at a time, all ones being none yet.
-constexpr int kChainWaves = 8, kGroup = 16, kChainLeast = 6;
+constexpr int kChainWaves = 8, kGroup = 16, kChainLeast = 20, kChainFew = 8;
 constexpr uint64_t kNone = ~0ull;
 
 struct Chain {
@@ -835,6 +838,7 @@ struct Plan {
     int v, waves, seg_lanes, parts;
     int64_t tiles, splits, split_steps;
     int64_t chained;   // stretches of a chain; 0: two passes where there are stretches
+    bool one_round() const { return split_steps <= (int64_t)waves * kSteps; }   // of a stretch
     int64_t parts_const() const { return chained ? chained : splits; }
     int64_t sums_floats(int64_t columns) const
     {
@@ -858,11 +862,15 @@ Plan plan_of(int64_t n_steps, int64_t batch, int32_t dim, int32_t groups, int32_
     if (s < 1) s = 1;
     p.split_steps = div_up(div_up(n_steps, s), round) * round;
     p.splits = div_up(n_steps, p.split_steps);
-    // A chain reads everything once, and has its clearing and its waits: for sequences of some stretches.  Forward, chain / two passes, us: 300 x 64 x 256 bf16
-    // (3 stretches) 15.1 / 13.9; 600 x 32 x 64 fp32 9.4 / 9.4; 1,024 x 4 x 512 bf16 10.5 / 11.6; 4,096 x 256 10.5 / 16.9; 65,536 x 1,000 115 / 156
+    // A chain reads everything once, and has its clearing and its waits: for many stretches, or few columns.  Chain / two passes, us, forward and back:
+    // 300 x 12 x 17 fp32 7.0 / 7.7, 9.9 / 10.7; 700 x 4 x 64 bf16 8.4 / 9.3, 9.7 / 11.1; 700 x 32 x 64 fp32 9.6 / 8.4, 13.7 / 12.0;
+    // 2,000 x 32 x 64 fp32 18.1 / 16.3, 20.4 / 19.8; 4,096 x 256 bf16 10.5 / 16.9 and 65,536 x 1,000 bf16 112 / 156 forward
     p.chained = div_up(n_steps, kChainWaves * kSteps);
-    if (p.splits > 1 && p.chained >= kChainLeast && p.tiles * p.chained < (1 << 22)) p.splits = 1;
+    if (p.splits > 1 && (p.chained >= kChainLeast || (w > kRoundWaves && p.tiles <= kChainFew)) && p.tiles * p.chained < (1 << 22)) p.splits = 1;
     else p.chained = 0;
+    // One round of more wavefronts in the place of stretches: 150 x 32 x 64 fp32 4.9 / 8.3 us forward, 7.8 / 10.7 back; two such rounds would take 10.1 / 8.0
+    // and 13.4 / 11.2 (500 x 32 x 64)
+    if (p.splits > 1 && w <= kRoundWaves) p.splits = 1, p.waves = (int)w, p.split_steps = w * kSteps;
     p.seg_lanes = p.parts = 0;
     if (groups > 0 && groups != dim) {
         const int seg = gcd(channels, kWave * p.v);
@@ -950,10 +958,12 @@ void launch_fwd(const ScanArgs &s, const Plan &p, int groups, hipStream_t st)
     dim3 grid((unsigned)p.tiles, (unsigned)p.splits);
     if (p.splits > 1) {
         grid.y = (unsigned)p.splits - 1;
-        BMTK_SCAN_LAUNCH(scan_sums_kernel, BMTK_COMMA false);
+        if (p.one_round()) BMTK_SCAN_LAUNCH(scan_sums_kernel, BMTK_COMMA false BMTK_COMMA true);
+        else BMTK_SCAN_LAUNCH(scan_sums_kernel, BMTK_COMMA false BMTK_COMMA false);
         grid.y = (unsigned)p.splits;
     }
-    BMTK_SCAN_LAUNCH(scan_fwd_kernel, );
+    if (p.one_round()) BMTK_SCAN_LAUNCH(scan_fwd_kernel, BMTK_COMMA true);
+    else BMTK_SCAN_LAUNCH(scan_fwd_kernel, BMTK_COMMA false);
 }
 
 template <typename TX, typename TA, int V>
@@ -968,7 +978,8 @@ void launch_bwd(ScanArgs s, const Plan &p, int groups, hipStream_t st)
         dim3 grid((unsigned)p.tiles, (unsigned)p.splits);
         if (p.splits > 1) {
             grid.y = (unsigned)p.splits - 1;
-            BMTK_SCAN_LAUNCH(scan_sums_kernel, BMTK_COMMA true);
+            if (p.one_round()) BMTK_SCAN_LAUNCH(scan_sums_kernel, BMTK_COMMA true BMTK_COMMA true);
+            else BMTK_SCAN_LAUNCH(scan_sums_kernel, BMTK_COMMA true BMTK_COMMA false);
             grid.y = (unsigned)p.splits;
         }
         BMTK_SCAN_LAUNCH(scan_bwd_kernel, );

@@ -297,6 +297,21 @@ def test_long_sequences_in_one_pass(dtype, gates, batch, dim, groups, lengths):
     scan_check(*scan_case(8200, batch, dim, groups, dtype, gates, lengths=lengths))
 
 
+@pytest.mark.parametrize("dtype,batch,dim,groups", [(torch.float32, 4, 100, 0), (torch.bfloat16, 20, 64, 64), (torch.float16, 7, 60, 5), (torch.float32, 33, 30, 30)])
+@pytest.mark.parametrize("steps", [300, 2433, 2432])
+def test_between_stretches_and_one_pass(steps, batch, dim, groups, dtype):
+    """Three stretches of few and of many columns; 19 and 20 of them."""
+    scan_check(*scan_case(steps, batch, dim, groups, dtype, dtype, lengths=[steps, 0, 257, steps - 1, 129]))
+
+
+@pytest.mark.parametrize("steps", [128, 129, 144, 200, 256, 257])
+@pytest.mark.parametrize("dtype,gates,dim,groups", [(torch.float32, torch.float32, 33, 0), (torch.bfloat16, torch.float32, 64, 64), (torch.bfloat16, torch.bfloat16, 96, 6),
+                                                    (torch.float16, torch.float16, 31, 31)])
+def test_one_round_of_many_wavefronts(steps, dtype, gates, dim, groups):
+    """And what is just too short or too long for it."""
+    scan_check(*scan_case(steps, 5, dim, groups, dtype, gates, lengths=[steps, 0, 1, 127, steps - 1]))
+
+
 @pytest.mark.parametrize("dtype,dim,groups", [(torch.float32, 128, 128), (torch.bfloat16, 256, 0), (torch.bfloat16, 256, 4), (torch.float16, 129, 43)])
 def test_stretches_of_several_rounds(dtype, dim, groups):
     """Many columns: two or three stretches of two rounds and more."""
