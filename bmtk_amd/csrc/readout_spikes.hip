@@ -416,6 +416,41 @@ __device__ __forceinline__ void load_eight(const T *__restrict__ base, int row, 
     }
 }
 
+// The same of rows at any distance, for kAny: 16 bytes a load all the same, which need no other alignment than their numbers'.  What would reach behind a row
+// is read from further left and moved there.  (At least 16 bytes a row.)
+constexpr int kAny = 0;
+template <typename T>
+__device__ __forceinline__ void load_eight_any(const T *__restrict__ base, int row, int rows, int dim, int k0, T (&v)[8])
+{
+    constexpr int N = 16 / sizeof(T);
+    struct __attribute__((packed, aligned(sizeof(T)))) Loose {
+        uint32_t w[4];
+    };
+    const unsigned at = (unsigned)min(row, rows - 1) * (unsigned)dim;
+#pragma unroll
+    for (int s = 0; s < 8; s += N) {
+        const int from = min(k0 + s, dim - N), shift = row < rows ? k0 + s - from : N;
+        const Loose q = *reinterpret_cast<const Loose *>(base + (at + (unsigned)from));
+        uint32_t w0 = q.w[0], w1 = q.w[1], w2 = q.w[2], w3 = q.w[3];
+        if constexpr (sizeof(T) == 2) {
+            const bool half = shift & 1;
+            w0 = half ? (w0 >> 16) | (w1 << 16) : w0, w1 = half ? (w1 >> 16) | (w2 << 16) : w1, w2 = half ? (w2 >> 16) | (w3 << 16) : w2, w3 = half ? w3 >> 16 : w3;
+        }
+        const int words = shift * (int)sizeof(T) / 4;
+        const bool one = words & 1, two = words & 2, none = shift >= N;
+        w0 = one ? w1 : w0, w1 = one ? w2 : w1, w2 = one ? w3 : w2, w3 = one ? 0 : w3;
+        w0 = two ? w2 : w0, w1 = two ? w3 : w1, w2 = two ? 0 : w2, w3 = two ? 0 : w3;
+        const uint32_t w[4] = {none ? 0 : w0, none ? 0 : w1, none ? 0 : w2, none ? 0 : w3};
+        __builtin_memcpy(v + s, w, 16);
+    }
+}
+template <typename T, int VL>
+__device__ __forceinline__ void load_eight_of(const T *__restrict__ base, int row, int rows, int dim, int k0, T (&v)[8])
+{
+    if constexpr (VL == kAny) load_eight_any<T>(base, row, rows, dim, k0, v);
+    else load_eight<T, VL>(base, row, rows, dim, k0, v);
+}
+
 // How the products reach memory.  kPairs: neighbouring lanes hold neighbouring (step, trial) pairs.  kAcross (one trial): neighbouring
 // neurons.  kTurned + s (4, 8, 16 or a multiple of 32 trials, 2^s fours of them in a tile, and rows that begin on 128 bytes): through LDS into the
 // order of memory, 16 bytes a lane, whole lines past the caches.  (Parts of lines written past the caches take five times as long.)
@@ -447,7 +482,7 @@ spike_bwd_spikes_kernel(const T *__restrict__ weight, const T *__restrict__ dy, 
     auto load_rows = [&](int stage) {
         const int at = min(stage, stages - 1);   // (behind the last one: it again, which nobody looks at)
         const int64_t r = r_begin + (int64_t)(at / passes) * kDzRows;
-        load_eight<T, VL>(dy + r * dim, threadIdx.x / 8, (int)min(r_end - r, (int64_t)kDzRows), dim, at % passes * kDzK + threadIdx.x % 8 * 8, next);
+        load_eight_of<T, VL>(dy + r * dim, threadIdx.x / 8, (int)min(r_end - r, (int64_t)kDzRows), dim, at % passes * kDzK + threadIdx.x % 8 * 8, next);
     };
     Part a[kDzGroups][P][kDzK / 16];
     auto load_weights = [&](int pass) {
@@ -461,7 +496,7 @@ spike_bwd_spikes_kernel(const T *__restrict__ weight, const T *__restrict__ dy, 
                 if (pass * kDzK + q * 16 >= dim) break;
                 // (a wavefront behind the last neuron multiplies the last one's weights, and writes nothing)
                 const int64_t first = min(i0, n - 1);
-                load_eight<T, VL>(weight + first * dim, g * 32 + col, (int)min(n - first, (int64_t)kDzNeurons), dim, pass * kDzK + (2 * q + half) * 8, v);
+                load_eight_of<T, VL>(weight + first * dim, g * 32 + col, (int)min(n - first, (int64_t)kDzNeurons), dim, pass * kDzK + (2 * q + half) * 8, v);
                 fine = Op::split(v, part) && fine;
 #pragma unroll
                 for (int p = 0; p < P; ++p) a[g][p][q] = part[p];
@@ -770,7 +805,7 @@ extern "C" int bmtk_spike_readout_bwd_spikes(const void *weight, const void *dy,
     const int64_t rows = n_steps * batch;
     const dim3 grid((unsigned)p.across, (unsigned)p.down);
     const int vl = 16 / (int)type_size(dtype);   // 16 bytes a load
-    const bool wide = dim % vl == 0 && aligned(weight, 16) && aligned(dy, 16);
+    const bool wide = dim % vl == 0 && aligned(weight, 16) && aligned(dy, 16), any = dim >= vl;
     const hipStream_t st = (hipStream_t)stream;
     const FastDiv by_batch = fast_div((uint32_t)batch);
     // (a tile's pairs are whole steps, or 32 trials of one)
@@ -795,10 +830,12 @@ extern "C" int bmtk_spike_readout_bwd_spikes(const void *weight, const void *dy,
     if (dtype == BMTK_F32 && p.whole) {
         typedef float T;
         if (wide) BMTK_DZ_BY(Whole, 4);
+        else if (any) BMTK_DZ_BY(Whole, kAny);
         else BMTK_DZ_BY(Whole, 1);
     } else {
         BMTK_BY_TYPE(dtype, T, {
             if (wide) BMTK_DZ_BY(T, 16 / sizeof(T));
+            else if (any) BMTK_DZ_BY(T, kAny);
             else BMTK_DZ_BY(T, 1);
         });
     }
