@@ -166,6 +166,8 @@ __device__ __forceinline__ void fold(const float *sums, int64_t columns, const L
 // One pass over the steps of a stretch in rounds: each wavefront takes kSteps steps into registers, finds what they do to a state
 // that enters them, (product of the gates, end from zero), the wavefronts tell each other, and each then computes its steps from the
 // state that really enters.  Everything is read once, a round ahead.
+// Short sequences are bound by the launches and by a round's way from load over exchange to store: 600 x 32 x 64 fp32 (4.9 MB each way) 8.3 us forward in
+// two launches, 11.9 back in three.
 template <int V, int kWaves>
 struct Tell {
     float v[2][kWaves][2][V][kWave];   // [round in turn][wavefront][product, end]
@@ -491,6 +493,9 @@ __global__ void __launch_bounds__(kMaxWaves * kWave) scan_sums_kernel(const Scan
 // what it does to a state (product, end from zero) as soon as it knows; what enters it follows from the stretches of its group of kGroup before it and from
 // the state that entered the group, which the last workgroup of the group before tells.  So every sum is made in an order that is
 // fixed, and the way from one group to the next is all that happens one after the other.
+//
+// 65,536 x 1,000 bf16, a gate per channel: 112 us forward (393 MB, 3.5 TB/s; two passes 156).  4,096 x 8 x 2,048 bf16, a gate per 64 channels, ragged: 77 us
+// forward and 111 back.  Three workgroups on a compute unit in the place of two change nothing: what is left is memory that is read and written by turns.
 //
 // Workgroups take their stretches by a counter, in the order in which the state passes: what one waits for comes from workgroups that have begun before
 // it and wait for earlier ones only, so every wait ends, however few run at once.  Values are told as 64 bits at a time, all ones being none yet.
