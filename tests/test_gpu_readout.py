@@ -93,6 +93,13 @@ def test_spikes_against_64_bits(steps, n, batch, dim, p, dtype):
     spikes_check(*spike_case(steps, n, batch, dim, dtype, p), batch)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("steps,n,batch,dim,p", [(2, 5003, 32, 33, 0.003), (1, 270011, 1, 20, 0.002), (3, 4001, 45, 9, 0.01), (64, 5003, 32, 33, 0.002)])
+def test_spikes_of_steps_in_slices(steps, n, batch, dim, p, dtype):
+    """And, the last one, a large product of rows that no load of 16 bytes divides."""
+    spikes_check(*spike_case(steps, n, batch, dim, dtype, p), batch)
+
+
 @pytest.mark.parametrize("p", [0.0, 1.0])
 @pytest.mark.parametrize("batch,n", [(1, 200), (12, 37), (64, 11), (130, 3)])
 def test_nothing_fired_and_everything_fired(batch, n, p):
