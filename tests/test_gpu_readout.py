@@ -100,6 +100,22 @@ def test_spikes_of_steps_in_slices(steps, n, batch, dim, p, dtype):
     spikes_check(*spike_case(steps, n, batch, dim, dtype, p), batch)
 
 
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("steps,n,batch,dim", [(250, 20011, 32, 70), (670, 20011, 12, 128), (8003, 20011, 1, 257), (250, 20016, 32, 20)])
+def test_large_products(steps, n, batch, dim, dtype):
+    """Several tiles of rows to a workgroup, not a whole number of what it takes at once; the product in 64 bits on the device, step by step."""
+    g = gen(steps)
+    w, dy = torch.randn(n, dim, generator=g).to(dtype).cuda(), torch.randn(steps, batch, dim, generator=g).to(dtype).cuda()
+    bits = torch.zeros(steps, (n * batch + 63) // 64, dtype=torch.int64, device="cuda")
+    dl_dz = readout.spike_readout_bwd(bits, w, dy, batch)[1].view(steps, n, batch)
+    wd = w.double()
+    for t in range(0, steps, 40):
+        d = dy[t:t + 40].double().reshape(-1, dim).t().contiguous()
+        want, mag = (a.view(n, -1, batch).transpose(0, 1) for a in (wd @ d, wd.abs() @ d.abs()))
+        # (products and additions of a row's channels, twice: see spikes_check)
+        assert ((dl_dz[t:t + 40].double() - want).abs() <= (dim + 8) * 2 * U * mag).all()
+
+
 @pytest.mark.parametrize("p", [0.0, 1.0])
 @pytest.mark.parametrize("batch,n", [(1, 200), (12, 37), (64, 11), (130, 3)])
 def test_nothing_fired_and_everything_fired(batch, n, p):
