@@ -461,7 +461,10 @@ __device__ __forceinline__ void load_eight_of(const T *__restrict__ base, int ro
 // How the products reach memory.  kPairs: neighbouring lanes hold neighbouring (step, trial) pairs.  kAcross (one trial): neighbouring
 // neurons.  kTurned + s (4, 8, 16 or a multiple of 32 trials, 2^s fours of them in a tile, and rows that begin on 128 bytes): through LDS into the
 // order of memory, 16 bytes a lane, whole lines past the caches.  (Parts of lines written past the caches take five times as long.)
-enum { kPairs = 0, kAcross = 1, kTurned = 2 };
+// kSteps1, kSteps4 (2 to 31 trials, up to 64 channels, no small product): a tile is whole steps, 24 pairs at least, and goes through LDS into the order of
+// memory too, 4 or (where that divides the trials) 16 bytes a lane.  600 steps of 20,000, against kPairs: 24 trials, 64 channels bf16 244 / 480 us; 12, 64 fp32
+// 242 / 266; 10, 33 bf16 139 / 161.  (More channels: the smaller tiles read the weights more often, 12 trials, 300 fp16 269 / 231.)
+enum { kPairs = 0, kAcross = 1, kTurned = 2, kSteps1 = 6, kSteps4 = 7 };
 
 // kOnePass: up to 64 channels.  More: passes over 64 of them at a time, each for kTiles tiles of rows, whose sums wait in registers meanwhile (weights that
 // are read again for every tile take 710 us where these take 522, 415 where these take 229: 300 steps of 20,000 x 32, 128 channels fp32, and x 12, 300 fp16).
@@ -486,12 +489,13 @@ spike_bwd_spikes_kernel(const T *__restrict__ weight, const T *__restrict__ dy, 
     const int64_t r_begin = (int64_t)blockIdx.y * rows_per_block, r_end = min(rows, r_begin + rows_per_block);
     const int passes = kOnePass ? 1 : (dim + kDzK - 1) / kDzK;
     // a stage: a tile of rows and a pass; the tiles of a pass one after the other, then the next pass
-    const int all_tiles = (int)((r_end - r_begin + kDzRows - 1) / kDzRows), tiles = kOnePass ? 1 : min(kTiles, all_tiles);
+    const int tile_rows = kOut >= kSteps1 ? kDzRows / batch * batch : kDzRows;
+    const int all_tiles = (int)((r_end - r_begin + tile_rows - 1) / tile_rows), tiles = kOnePass ? 1 : min(kTiles, all_tiles);
     const int stages = (all_tiles + tiles - 1) / tiles * passes * tiles;
     T next[8];
     auto load_rows = [&](int stage) {
         const int at = min(stage, stages - 1);   // (behind the last one: it again, which nobody looks at)
-        const int64_t r = min(r_begin + ((int64_t)(at / tiles / passes) * tiles + at % tiles) * kDzRows, r_end - 1);
+        const int64_t r = min(r_begin + ((int64_t)(at / tiles / passes) * tiles + at % tiles) * tile_rows, r_end - 1);
         load_eight_of<T, VL>(dy + r * dim, threadIdx.x / 8, (int)min(r_end - r, (int64_t)kDzRows), dim, at / tiles % passes * kDzK + threadIdx.x % 8 * 8, next);
     };
     Part a[kDzGroups][P][kDzK / 16];
@@ -526,6 +530,28 @@ spike_bwd_spikes_kernel(const T *__restrict__ weight, const T *__restrict__ dy, 
                 for (int q = 0; q < 4; ++q)
                     turn[wave][col * 8 + ((2 * q + half) ^ (col & 7))] = f32x4{sums[g][4 * q], sums[g][4 * q + 1], sums[g][4 * q + 2], sums[g][4 * q + 3]};
                 wave_order();
+                if constexpr (kOut >= kSteps1) {
+                    // 32 neurons' trials of a step lie together
+                    const int rows_here = (int)min((int64_t)tile_rows, r_end - r0), left = (int)min((int64_t)32, n - ig);
+                    float *to = dl_dz + (int64_t)div_by((uint32_t)r0, by_batch) * ne + ig * batch;
+                    if constexpr (kOut == kSteps4) {
+                        // (four trials a lane, of all steps of the tile in turn)
+#pragma unroll 1
+                        for (int at = 4 * lane; at < rows_here * 32; at += 4 * kWave) {
+                            const int all_i = (int)div_by((uint32_t)at, by_batch), i = all_i & 31, step = all_i >> 5, b = at - all_i * batch;
+                            if (i < left) *reinterpret_cast<f32x4 *>(to + (step * ne + i * batch + b)) = turn[wave][i * 8 + (((step * batch + b) >> 2) ^ (i & 7))];
+                        }
+                    } else {
+                        const float *from = reinterpret_cast<const float *>(turn[wave]);
+                        for (int pair = 0; pair < rows_here; pair += batch, to += ne)
+                            for (int at = lane; at < left * batch; at += kWave) {
+                                const int i = (int)div_by((uint32_t)at, by_batch), q = pair + at - i * batch;
+                                to[at] = from[(i * 8 + ((q >> 2) ^ (i & 7))) * 4 + (q & 3)];
+                            }
+                    }
+                    wave_order();
+                    continue;
+                }
                 // A neuron has 2^kShift fours of trials in a step; up to 32 trials the tile begins with a step, of more it is a part of one.  Four `at`
                 // of the tile, in the order of memory: step at >> (kShift + 5), neuron (at >> kShift) & 31; of 64 k + lane the sum of both parts'.
                 constexpr int kShift = kOut - kTurned;
@@ -604,7 +630,7 @@ spike_bwd_spikes_kernel(const T *__restrict__ weight, const T *__restrict__ dy, 
         if (kOnePass || pass == passes - 1)
 #pragma unroll
             for (int j = 0; j < kTiles; ++j) {
-                const int64_t r0 = r_begin + ((int64_t)(first / tiles / passes) * tiles + j) * kDzRows;
+                const int64_t r0 = r_begin + ((int64_t)(first / tiles / passes) * tiles + j) * tile_rows;
                 if (j == 0 || (j < tiles && r0 < r_end)) put(r0, sums[j]);
             }
     }
@@ -683,6 +709,7 @@ FwdPlan fwd_plan(int64_t n_steps, int64_t n, int batch, int dim, int vw)
 
 struct DzPlan {
     int64_t across, per_block, down, parts;
+    int tile_rows;   // (step, trial) pairs of a tile
     bool whole;   // fp32: in fp32 instructions.  Up to this many products they take some us at most, less than the launch that looks for infinities
 };
 constexpr double kWholeProducts = 3e8;
@@ -691,10 +718,12 @@ DzPlan dz_plan(int64_t n_steps, int64_t n, int batch, int dim)
     DzPlan p;
     p.whole = (double)n_steps * batch * n * dim < kWholeProducts;
     p.across = div_up(n, kDzWaves * kDzNeurons);
-    const int64_t rows = n_steps * batch, most = div_up(rows, kDzRows);
+    p.tile_rows = batch > 1 && batch < kDzRows ? kDzRows / batch * batch : kDzRows;
+    if (p.whole || dim > kDzK || 4 * p.tile_rows < 3 * kDzRows) p.tile_rows = kDzRows;
+    const int64_t rows = n_steps * batch, most = div_up(rows, p.tile_rows);
     int64_t blocks = div_up(4096, p.across);
     if (blocks > most) blocks = most;
-    p.per_block = div_up(most, blocks) * kDzRows;
+    p.per_block = div_up(most, blocks) * p.tile_rows;
     p.down = div_up(rows, p.per_block);
     p.parts = p.across * p.down;
     return p;
@@ -831,6 +860,7 @@ extern "C" int bmtk_spike_readout_bwd_spikes(const void *weight, const void *dy,
     const FastDiv by_batch = fast_div((uint32_t)batch);
     // (a tile's pairs are whole steps, or 32 trials of one)
     const bool turned = (batch % 32 == 0 || batch == 4 || batch == 8 || batch == 16) && aligned(dl_dz, 128) && n_neurons * batch % 32 == 0;
+    const bool steps = batch < kDzRows && !p.whole && dim <= kDzK && p.tile_rows % batch == 0, four = batch % 4 == 0 && aligned(dl_dz, 16);
 #define BMTK_DZ(O, VL, OUT, ONE)                                                                                                                       \
     hipLaunchKernelGGL((spike_bwd_spikes_kernel<T, O, VL, OUT, ONE>), grid, dim3(kDzWaves *kWave), 0, st, (const T *)weight, (const T *)dy, rows, n_neurons, \
                        by_batch, dim, p.per_block, workspace, dl_dz)
@@ -844,9 +874,15 @@ extern "C" int bmtk_spike_readout_bwd_spikes(const void *weight, const void *dy,
         else BMTK_DZ(O, VL, kTurned + 3, ONE);                  \
     } while (0)
 #define BMTK_DZ_BY(O, VL)                            \
-    do {                                          \
+    do {                                             \
         if (dim <= kDzK) BMTK_DZ_OUT(O, VL, true);   \
         else BMTK_DZ_OUT(O, VL, false);              \
+    } while (0)
+#define BMTK_DZ_STEPS(O, VL)                                          \
+    do {                                                              \
+        if (turned || !steps || batch == 1) BMTK_DZ_BY(O, VL);        \
+        else if (four) BMTK_DZ(O, VL, kSteps4, true);                 \
+        else BMTK_DZ(O, VL, kSteps1, true);                           \
     } while (0)
     if (dtype == BMTK_F32 && p.whole) {
         typedef float T;
@@ -855,14 +891,15 @@ extern "C" int bmtk_spike_readout_bwd_spikes(const void *weight, const void *dy,
         else BMTK_DZ_BY(Whole, 1);
     } else {
         BMTK_BY_TYPE(dtype, T, {
-            if (wide) BMTK_DZ_BY(T, 16 / sizeof(T));
-            else if (any) BMTK_DZ_BY(T, kAny);
-            else BMTK_DZ_BY(T, 1);
+            if (wide) BMTK_DZ_STEPS(T, 16 / sizeof(T));
+            else if (any) BMTK_DZ_STEPS(T, kAny);
+            else BMTK_DZ_STEPS(T, 1);
         });
     }
     if (dtype == BMTK_F32 && !p.whole)
         hipLaunchKernelGGL(spike_bwd_spikes_again_kernel, dim3((unsigned)div_up(p.parts, kBlock)), dim3(kBlock), 0, st, (const float *)weight, (const float *)dy, rows,
                            n_neurons, by_batch, dim, p.per_block, (int)p.across, (int)p.parts, workspace, dl_dz);
+#undef BMTK_DZ_STEPS
 #undef BMTK_DZ_BY
 #undef BMTK_DZ_OUT
 #undef BMTK_DZ

@@ -101,7 +101,8 @@ def test_spikes_of_steps_in_slices(steps, n, batch, dim, p, dtype):
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
-@pytest.mark.parametrize("steps,n,batch,dim", [(250, 20011, 32, 70), (670, 20011, 12, 128), (8003, 20011, 1, 257), (250, 20016, 32, 20)])
+@pytest.mark.parametrize("steps,n,batch,dim", [(250, 20011, 32, 70), (670, 20011, 12, 128), (8003, 20011, 1, 257), (250, 20016, 32, 20), (671, 20011, 12, 31), (900, 20011, 9, 64), (2801, 20011, 3, 50),
+                                                 (331, 20011, 24, 17), (399, 20011, 20, 33), (999, 20011, 8, 64)])
 def test_large_products(steps, n, batch, dim, dtype):
     """Several tiles of rows to a workgroup, not a whole number of what it takes at once; the product in 64 bits on the device, step by step."""
     g = gen(steps)
