@@ -82,7 +82,7 @@ __device__ __forceinline__ void add_rows(Accumulators<VW, N> &acc, const T *__re
 // and reads the weight rows, one per spike, 64 * VW channels by its 64 lanes.  The sums of a trial are the wavefront's own, so their
 // order is fixed; the wavefronts' sums are added in order at the end, in the LDS that held the queues.
 //
-// What bounds it is reading rows at random from the caches behind the L1: at 0.3 % of the neurons a step, 1,000 steps of 230,924 x 256 bf16 take 55 us
+// What bounds it is reading rows at random from the L2s and from behind them: at 0.3 % of the neurons a step, 1,000 steps of 230,924 x 256 bf16 take 55 us
 // (355 MB of rows, 6.4 TB/s), 600 steps of 51,978 x 32 x 64 fp32 127 us (766 MB, 6.0 TB/s); one step of the former with 64 channels fp32 6.9 us, most of
 // it the launch and three dependent reads.
 template <typename T, int VW, int N, int kFwdWaves, int kWords>
@@ -212,7 +212,8 @@ __global__ void __launch_bounds__(kBlock) spike_join_kernel(const float *__restr
 // ---------------------------------------------------------------------------------------------------------------------
 // Gradient by the weights: row i is the sum of dy[t, b] over the spikes of neuron i.  A wavefront owns `own` neurons and their
 // sums, looks through their bits of all steps and reads the dy rows as the forward pass reads the weights.  Nobody else
-// adds to its sums: the order is fixed and nothing has to be joined.  600 steps of 51,978 x 32 x 64 fp32: 147 us (766 MB of dy rows, 5.2 TB/s; they stay in the L2s).
+// adds to its sums: the order is fixed and nothing has to be joined.  600 steps of 51,978 x 32 x 64 fp32: 147 us (766 MB of dy rows, 5.2 TB/s, more
+// than half of them out of the L2s).
 template <typename T, int VW, int N>
 __global__ void __launch_bounds__(kWaves * kWave)
 spike_bwd_weight_kernel(const uint64_t *__restrict__ bits, int64_t stride, int64_t n_steps, int64_t n, FastDiv by_batch, int own,
