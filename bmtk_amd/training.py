@@ -84,12 +84,20 @@ def label_loss(bits, batch, weight, decay, labels, ignore=-100, state=None, top=
 
     bits    int64 [steps, words] spike bits of a run of ``batch`` trials (``fwd["bits"]``)
     weight  [neurons, classes], decay float32 [classes]: the readout, y = sum of the weight rows of what fired, h[t] = decay * h[t - 1] + y[t]; the
-            classes' probabilities in every step are the softmax of h (``readout.spike_readout``, ``gated_scan``, ``token_logprobs``)
+            classes' probabilities in every step are the softmax of h (``readout.spike_readout``, ``gated_scan``, ``token_logprobs``).  y, h and
+            their gradients have the type of ``weight``, rounded once each; of float16 weights they are float32: a mean over many labels leaves
+            each a gradient below what float16 holds
     labels  int64 [steps, batch]: the class wanted in each step and trial, ``ignore`` where none is
     state   float32 [batch, classes]: h before the first step (None: zero)
     Returns (loss, dl_dz, gradients, answer): the mean of -log p(label) over the steps and trials that have one; dl_dz float32
     [steps, neurons * batch], what ``Glif3Bptt.backward`` takes; a dict of the gradients by "weight", "decay" and "state"; and
     the ``readout.LogProbs`` of every step and trial with its ``top`` most probable classes.  Nothing synchronises."""
+    given = weight, decay
+    if isinstance(weight, torch.Tensor) and weight.dtype == torch.float16:
+        # (3,000 steps x 100 trials, 100 classes: in float16 92 % of the gradients by h are 0, dl_dz is off by 0.9 %, and the call takes 1.7 ms; 1.6 like this)
+        weight = weight.float()
+        if isinstance(decay, torch.Tensor) and decay.dtype == torch.float16:
+            decay = decay.float()
     y = readout.spike_readout(bits, weight, batch)
     h, _, saved = readout.gated_scan(y, decay, state, save_state=True)
     answer = readout.token_logprobs(h, labels, top=top, ignore=ignore)
@@ -98,7 +106,7 @@ def label_loss(bits, batch, weight, decay, labels, ignore=-100, state=None, top=
     dh = readout.token_logprobs_bwd(h, labels, answer, d_logp=(-share).expand(labels.shape).contiguous(), ignore=ignore, out=h)
     dy, d_decay, d_state = readout.gated_scan_bwd(y, decay, saved, dh)
     d_weight, dl_dz = readout.spike_readout_bwd(bits, weight, dy, batch)
-    return loss, dl_dz, {"weight": d_weight, "decay": d_decay, "state": d_state}, answer
+    return loss, dl_dz, {"weight": d_weight.to(given[0].dtype), "decay": d_decay.to(given[1].dtype), "state": d_state}, answer
 
 
 class Glif3Bptt:

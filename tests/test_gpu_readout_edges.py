@@ -1,0 +1,101 @@
+"""The readout operations where numbers leave the ordinary range.  Tolerances as in test_gpu_readout: bounds, made from half steps."""
+import pytest
+import torch
+
+from bmtk_amd import training
+from test_gpu_readout import DTYPES, TINY, U, close, gen, pack, raster
+
+pytestmark = pytest.mark.gpu
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# the loss on labels
+
+def label_loss_reference(z, w, decay, labels, inner):
+    """What training.label_loss returns, in 64 bits, and bounds of the errors of one that keeps sums, memory and their gradients in `inner`, rounded
+    once each, with arithmetic in fp32.  Every bound follows its value: e_ of a value is what it is off by at most."""
+    steps, batch = labels.shape
+    n, classes = w.shape
+    u, tiny = torch.finfo(inner).eps / 2, TINY[inner]
+    zero = torch.zeros(batch, classes, dtype=torch.float64, device="cuda")
+    zt = z.transpose(1, 2).reshape(steps * batch, n).double().cuda()
+    w, a = w.double().cuda(), decay.double().cuda()
+
+    def rounded(v, e):
+        return e + u * (v.abs() + e) + tiny
+    y = zt @ w
+    e_y = rounded(y, (zt.sum(1, keepdim=True) + 64) * U * (zt @ w.abs()))
+    y, e_y = y.view(steps, batch, classes), e_y.view(steps, batch, classes)
+    # S: the sum of the terms' magnitudes; a term passes two roundings a step, two more for every 16 steps, and a few at its ends; P: what the terms are off by
+    h, e_h, before, e_before = (torch.empty_like(y) for _ in range(4))
+    s, S, G, P = zero, zero, zero, zero
+    for t in range(steps):
+        before[t], e_before[t] = s, U * G + P
+        x = y[t].abs() + e_y[t]
+        s, S = a * s + y[t], a * S + x
+        G, P = a * (G + 2.2 * S) + 12 * x, a * P + e_y[t]
+        h[t], e_h[t] = s, U * G + P
+    e_h = rounded(h, e_h)
+    lse = torch.logsumexp(h, 2, keepdim=True)
+    lp = h - lse
+    # a log probability is off by its logit, by the largest of the row (through lse), and by the arithmetic: sums of positive terms, each off by 3 roundings
+    # and that of its exponent (up to 40), added in classes / 64 + 64 additions; lse and the logits round at their own size
+    e_lp = e_h + e_h.amax(2, keepdim=True) + (classes / 64 + 64 + 3 + 80 + 2 * (lp.abs() + 40)) * U + 4 * U * (lse.abs() + h.abs().amax(2, keepdim=True))
+    labels = labels.cuda()
+    given = (labels >= 0).unsqueeze(2)
+    at = labels.clamp(min=0).unsqueeze(2)
+    share = 1.0 / given.sum()
+    logp, e_logp = (torch.where(given, v.gather(2, at), 0.0) for v in (lp, e_lp))
+    out = dict(loss=-logp.sum() * share, e_loss=(e_logp.sum() + 40 * U * logp.abs().sum()) * share, logp=logp.squeeze(2), e_logp=e_logp.squeeze(2))
+    p = torch.exp(lp)
+    dh = torch.where(given, p.scatter_add(2, at, torch.full_like(lse, -1.0)), 0.0) * share
+    e_dh = torch.where(given, p * torch.expm1(e_lp) + 6 * U * (p + dh.abs() / share), 0.0) * share
+    e_dh = rounded(dh, e_dh)
+    c, S, G, P = zero, zero, zero, zero
+    dy, e_dy = torch.empty_like(y), torch.empty_like(y)
+    d_decay, e_decay, mag = (torch.zeros(classes, dtype=torch.float64, device="cuda") for _ in range(3))
+    for t in range(steps - 1, -1, -1):
+        x = dh[t].abs() + e_dh[t]
+        g, S, G, P = c + dh[t], S + x, G + 12 * x, P + e_dh[t]
+        e = U * G + P
+        dy[t], e_dy[t] = g, e
+        da = g * before[t]
+        d_decay, mag = d_decay + da.sum(0), mag + da.abs().sum(0)
+        e_decay = e_decay + (e * before[t].abs() + (g.abs() + e) * (e_before[t] + 2 * U * before[t].abs())).sum(0)
+        c, S, G, P = a * g, a * S, a * (G + 2.2 * S), a * P
+    e_dy = rounded(dy, e_dy)
+    out.update(decay=d_decay, e_decay=e_decay + min(steps * batch, 4000) * U * mag, state=c, e_state=U * (G + S) + P)
+    dy, e_dy = dy.view(-1, classes), e_dy.view(-1, classes)
+    ztt = zt.t().contiguous()
+    out.update(weight=ztt @ dy, e_weight=ztt @ e_dy + (zt.sum(0).unsqueeze(1) + 64) * U * (ztt @ (dy.abs() + e_dy)))
+    wt = w.t().contiguous()
+    order = lambda v: v.view(steps, batch, n).transpose(1, 2).reshape(steps, n * batch)  # noqa: E731
+    out.update(dl_dz=order(dy @ wt), e_dl_dz=order(e_dy @ wt.abs() + (classes + 8) * 2 * U * ((dy.abs() + e_dy) @ wt.abs())))
+    return out
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("steps,batch,classes", [(300, 8, 10), (3000, 100, 100)])
+def test_label_loss_of_every_type(steps, batch, classes, dtype):
+    """Up to 300,000 labels, whose mean gives each a gradient that fp16 does not hold: sums, memory and their gradients are in fp32 there."""
+    n = 24
+    z = raster(steps, n, batch, 0.05, 1)
+    g = gen(2)
+    weight = torch.randn(n, classes, generator=g).to(dtype)
+    decay = 0.5 + 0.45 * torch.rand(classes, generator=g)
+    labels = torch.randint(0, classes, (steps, batch), generator=g)
+    labels[torch.rand(steps, batch, generator=g) < 0.1] = -100
+    want = label_loss_reference(z, weight, decay, labels, torch.bfloat16 if dtype == torch.bfloat16 else torch.float32)
+    loss, dl_dz, grads, answer = training.label_loss(pack(z), batch, weight.cuda(), decay.cuda(), labels.cuda())
+    assert loss.dtype == dl_dz.dtype == grads["decay"].dtype == grads["state"].dtype == torch.float32 and grads["weight"].dtype == dtype
+    for name, got in dict(loss=loss, logp=answer.logp, dl_dz=dl_dz, **grads).items():
+        close(got, want[name], want["e_" + name], name)
+
+
+def test_label_loss_takes_decays_of_the_weights_type():
+    z = raster(40, 24, 4, 0.1, 3)
+    weight, decay = torch.randn(24, 6, generator=gen(4)).half().cuda(), torch.full((6,), 0.75).cuda()
+    labels = torch.randint(0, 6, (40, 4), generator=gen(5)).cuda()
+    one, other = (training.label_loss(pack(z), 4, weight, d, labels) for d in (decay, decay.half()))
+    assert torch.equal(one[0], other[0]) and torch.equal(one[1], other[1])
+    assert other[2]["decay"].dtype == torch.float16 and torch.equal(one[2]["decay"].half(), other[2]["decay"])
