@@ -2,7 +2,7 @@
 import pytest
 import torch
 
-from bmtk_amd import training
+from bmtk_amd import readout, training
 from test_gpu_readout import DTYPES, TINY, U, close, gen, pack, raster
 
 pytestmark = pytest.mark.gpu
@@ -99,3 +99,55 @@ def test_label_loss_takes_decays_of_the_weights_type():
     one, other = (training.label_loss(pack(z), 4, weight, d, labels) for d in (decay, decay.half()))
     assert torch.equal(one[0], other[0]) and torch.equal(one[1], other[1])
     assert other[2]["decay"].dtype == torch.float16 and torch.equal(one[2]["decay"].half(), other[2]["decay"])
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# log probabilities
+
+def gradient_reference(x, tokens, dl, de):
+    """In 64 bits; and bounds: p is off by the roundings of its exponent and those of the row's sum, wherever the logits lie."""
+    x = x.double().cpu()
+    vocab = x.shape[1]
+    lp = torch.log_softmax(x, 1)
+    p = torch.exp(lp)
+    lq = torch.where(p > 0, lp, 0.0)
+    H = -(p * lq).sum(1, keepdim=True)
+    dl, de, tokens = dl.double().cpu().unsqueeze(1), de.double().cpu().unsqueeze(1), tokens.cpu()
+    d = -p * dl - de * p * (lq + H)
+    d[torch.arange(len(d)), tokens] += dl.squeeze(1)
+    n = (vocab / 64 + 64 + 3 + 2 * 40) * U
+    # (a log sum of up to 64 rounds by 2^-18, 64 of these half steps)
+    per = (lq.abs() + 40) * 2 * U + 2 * n + 66 * U
+    spread = (p * lq.abs()).sum(1, keepdim=True) + 1
+    err = p * per * (dl.abs() + de.abs() * (lq.abs() + H + 1)) + p * de.abs() * (4 * n * spread + per) + 4 * U * dl.abs() * p
+    err[torch.arange(len(d)), tokens] += 2 * U * dl.squeeze(1).abs()
+    return d, err
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocab", [(5, 1), (40, 10), (7, 100), (6, 300), (9, 511), (5, 700), (4, 5003), (3, 70001), (500, 2100)])
+def test_gradient_of_logits_far_from_zero(rows, vocab, dtype):
+    """All of the type's lowest or highest value (a mask that leaves nothing), of some hundreds, thousands and ten thousands; rows of small ones among them.
+    Written to new memory and in place, with even and odd distances of rows."""
+    g = gen(vocab)
+    x = torch.randn(rows, vocab, generator=g)
+    info = torch.finfo(dtype)
+    far = [None, info.min, info.max, 150.0, -9000.0, 60000.0, -63.0]
+    for r in range(rows):
+        f = far[r % 7]
+        if f is not None:
+            x[r] = f if abs(f) > 6e4 else f + x[r]
+    if vocab > 4:
+        x[1::7, 3] = 0.0 if rows > 8 else x[1::7, 3]   # (one that the mask leaves)
+    x = x.to(dtype).cuda()
+    tokens = torch.randint(0, vocab, (rows,), generator=g).cuda()
+    dl, de = torch.randn(rows, generator=g).cuda(), torch.randn(rows, generator=g).cuda()
+    want, err = gradient_reference(x, tokens, dl, de)
+    for wide in (0, 1, 8):
+        part = torch.empty(rows, vocab + wide, dtype=dtype, device="cuda")[:, :vocab]
+        part.copy_(x)
+        r = readout.token_logprobs(part, tokens)
+        d = readout.token_logprobs_bwd(part, tokens, r, dl, de)
+        close(d, want, err, "d_logits")
+        assert readout.token_logprobs_bwd(part, tokens, r, dl, de, out=part) is part
+        assert torch.equal(part, d)
