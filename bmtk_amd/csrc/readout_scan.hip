@@ -149,6 +149,26 @@ __device__ __forceinline__ Lane<V> lane_of(const ScanArgs &s, int64_t tile)
 // What is left of a state behind several steps.  (Decays above 1 may have a product that 32 bits do not hold: it leaves nothing nothing.)
 __device__ __forceinline__ float passed(float product, float state) { return state == 0.0f ? 0.0f : product * state; }
 
+// A product of decays that 32 bits do not hold, though none of them is 0 (0.4 over 128 steps), is their smallest number: an infinite state stays infinite behind
+// it, as it does step by step, and of any other there is 2^-149 left at most.
+__device__ __forceinline__ float times(float p, float q)
+{
+    const float r = p * q;
+    return r == 0.0f && p != 0.0f && q != 0.0f ? __builtin_copysignf(0x1p-149f, r) : r;
+}
+// The same of a block's decays, `p` being their plain product: looked at again only where that is 0
+template <int V, typename Gate>
+__device__ __forceinline__ void keep_products(float (&p)[V], const Gate &gate)
+{
+#pragma unroll
+    for (int c = 0; c < V; ++c)
+        if (p[c] == 0.0f) {
+            p[c] = 1.0f;
+#pragma unroll
+            for (int k = 0; k < kSteps; ++k) p[c] = times(p[c], gate(k, c));
+        }
+}
+
 // State that a stretch begins with: the stretches before it, in order.  sums[k][0]: product of the gates of stretch k, [1]: where it ends from zero.
 template <int V>
 __device__ __forceinline__ void fold(const float *sums, int64_t columns, const Lane<V> &l, int first, int last, int by, float (&h)[V])
@@ -239,6 +259,7 @@ __global__ void __launch_bounds__((kOne ? kRoundWaves : kMaxWaves) * kWave) scan
 #pragma unroll
             for (int k = 0; k < kSteps; ++k) e[c] = __builtin_fmaf(gate(k, c), e[c], xb[i].get(k, c)), p[c] *= gate(k, c);
         }
+        keep_products<V>(p, gate);
         exchange(tell, i, wave, waves, p, e, enter, mine);
         if (t0 >= t_hi) return;
         xb[i].again();
@@ -376,6 +397,7 @@ __global__ void __launch_bounds__(kRoundWaves * kWave) scan_bwd_kernel(const Sca
 #pragma unroll
             for (int k = kSteps - 1; k >= 0; --k) e[c] = gate(k, c) * (gb.get(k, c) + e[c]), p[c] *= gate(k, c);
         }
+        keep_products<V>(p, gate);
         // the states before each step, again from the kept one
 #pragma unroll
         for (int k = 1; k < kSteps; ++k)
@@ -441,17 +463,22 @@ __global__ void __launch_bounds__(kMaxWaves * kWave) scan_sums_kernel(const Scan
             if (G != kConst) ab[i].cut(there, 1.0f);
         }
         auto gate = [&](int k, int c) { return G == kConst ? (k < there ? a_const[c] : 1.0f) : ab[i].get(k, c); };
+        float p[V], e[V];
 #pragma unroll
         for (int c = 0; c < V; ++c) {
-            float p = 1.0f, e = 0.0f;
+            p[c] = 1.0f, e[c] = 0.0f;
 #pragma unroll
             for (int j = 0; j < kSteps; ++j) {
                 const int k = kBack ? kSteps - 1 - j : j;
-                e = kBack ? gate(k, c) * (xb[i].get(k, c) + e) : __builtin_fmaf(gate(k, c), e, xb[i].get(k, c));
-                p *= gate(k, c);
+                e[c] = kBack ? gate(k, c) * (xb[i].get(k, c) + e[c]) : __builtin_fmaf(gate(k, c), e[c], xb[i].get(k, c));
+                p[c] *= gate(k, c);
             }
-            tell.v[i][wave][0][c][lane] = p;
-            tell.v[i][wave][1][c][lane] = e;
+        }
+        keep_products<V>(p, gate);
+#pragma unroll
+        for (int c = 0; c < V; ++c) {
+            tell.v[i][wave][0][c][lane] = p[c];
+            tell.v[i][wave][1][c][lane] = e[c];
         }
         __syncthreads();
         if (wave != 0) return;
@@ -465,13 +492,13 @@ __global__ void __launch_bounds__(kMaxWaves * kWave) scan_sums_kernel(const Scan
             for (int c = 0; c < V; ++c) {
                 const float pw = tell.v[i][w][0][c][lane];
                 re[c] = passed(pw, re[c]) + tell.v[i][w][1][c][lane];
-                rp[c] *= pw;
+                rp[c] = times(rp[c], pw);
             }
         }
 #pragma unroll
         for (int c = 0; c < V; ++c) {
             end[c] = passed(product[c], re[c]) + end[c];
-            product[c] *= rp[c];
+            product[c] = times(product[c], rp[c]);
         }
     };
     load(0, 0);
@@ -584,7 +611,7 @@ __device__ __forceinline__ void chain(ChainShared<V> &sh, const Chain &ch, const
         for (int c = 0; c < V; ++c) {
             const float bp = sh.block[w][0][c][lane];
             we[c] = passed(bp, we[c]) + sh.block[w][1][c][lane];
-            wp[c] *= bp;
+            wp[c] = times(wp[c], bp);
         }
     }
     if (wave == 0 && l.in) say<V>(ch.stretch + order * columns + l.col, wp, we);
@@ -611,7 +638,7 @@ __device__ __forceinline__ void chain(ChainShared<V> &sh, const Chain &ch, const
                 for (int c = 0; c < V; ++c) {
                     const float sp = __uint_as_float((uint32_t)(v[k][c] >> 32));
                     fe[c] = passed(sp, fe[c]) + __uint_as_float((uint32_t)v[k][c]);
-                    fp[c] *= sp;
+                    fp[c] = times(fp[c], sp);
                 }
 #pragma unroll
         for (int c = 0; c < V; ++c) sh.before[wave][0][c][lane] = fp[c], sh.before[wave][1][c][lane] = fe[c];
@@ -684,6 +711,7 @@ __global__ void __launch_bounds__(kChainWaves * kWave, 4) scan_fwd_chain_kernel(
 #pragma unroll
         for (int k = 0; k < kSteps; ++k) e[c] = __builtin_fmaf(gate(k, c), e[c], xb.get(k, c)), p[c] *= gate(k, c);
     }
+    keep_products<V>(p, gate);
     chain<V>(sh, ch, l, s.columns, order, wave, p, e, s.state, s.last, mine);
     if (t0 >= t_hi || !l.in) return;
     xb.again();
@@ -742,6 +770,7 @@ __global__ void __launch_bounds__(kChainWaves * kWave, 4) scan_bwd_chain_kernel(
 #pragma unroll
         for (int k = kSteps - 1; k >= 0; --k) e[c] = gate(k, c) * (gb.get(k, c) + e[c]), p[c] *= gate(k, c);
     }
+    keep_products<V>(p, gate);
     chain<V>(sh, ch, l, s.columns, order, wave, p, e, s.d_last, s.d_state, mine);
     gb.again();
     if (G != kConst) ab.again();

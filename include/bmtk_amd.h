@@ -699,7 +699,7 @@ int bmtk_rate_mse(const int32_t *counts, int64_t n_neurons, int32_t batch, int64
 
 /* ---------------------------------------------------------------------------
  * A readout that is trained on what it answers: spikes -> sums of weight rows -> a memory over steps -> log probabilities, each with its
- * gradient, down to the dl_dz of bmtk_glif3_bwd.  No counterpart in the reference (bmtk has no gradients).
+ * gradient, down to the dl_dz of bmtk_glif3_simulate_bwd.  No counterpart in the reference (bmtk has no gradients).
  *
  * dtype: the type of the values that are read and written, BMTK_F32, BMTK_BF16 or BMTK_F16; all arithmetic is in 32 bits, and a value of a
  * 16-bit type is rounded once, when it is written.  The workspaces need not be cleared, hold nothing between calls, and belong to a call
@@ -717,7 +717,7 @@ int bmtk_spike_readout_fwd(const uint64_t *spike_bits, int64_t stride, int64_t n
 /* d_weight[i][:] = sum of dy[t][b][:] over the spikes of neuron i (all rows are written) */
 int bmtk_spike_readout_bwd_weight(const uint64_t *spike_bits, int64_t stride, int64_t n_steps, int64_t n_neurons, int32_t batch, const void *dy, int32_t dim,
                                   int32_t dtype, void *d_weight, void *stream);
-/* dl_dz[t][i * batch + b] = dy[t][b][:] . weight[i][:], in 32 bits: what bmtk_glif3_bwd takes.  workspace: where
+/* dl_dz[t][i * batch + b] = dy[t][b][:] . weight[i][:], in 32 bits: what bmtk_glif3_simulate_bwd takes.  workspace: where
  * bmtk_spike_readout_workspace_bytes says so, for BMTK_F32 only */
 int bmtk_spike_readout_bwd_spikes(const void *weight, const void *dy, int64_t n_steps, int64_t n_neurons, int32_t batch, int32_t dim, int32_t dtype,
                                   float *dl_dz, int32_t *workspace, void *stream);
@@ -729,6 +729,7 @@ int bmtk_spike_readout_bwd_spikes(const void *weight, const void *dy, int64_t n_
  * and dh, in elements (a channel's neighbour is next to it); h, dx and d_decay are contiguous.  state, last, d_last, d_state, marks: 32 bits.
  * marks (NULL: not kept): the state before every BMTK_SCAN_MARK-th step, [ceil(n_steps / BMTK_SCAN_MARK)][batch][dim], from which the backward
  * pass computes the others again.  Decays of up to 1 in magnitude, or of which the products over any steps in a row stay in 32 bits.
+ * Infinities and NaN go on as they do step by step; of a state that decays to less, up to 2^-149 of what it was may be left.
  * Limits: batch * dim < 2^31, n_steps < 2^31 - 4096. */
 #define BMTK_SCAN_MARK 16
 int64_t bmtk_gated_scan_workspace_bytes(int64_t n_steps, int64_t batch, int32_t dim, int32_t groups, int32_t backward);

@@ -1,9 +1,11 @@
 """The readout operations where numbers leave the ordinary range.  Tolerances as in test_gpu_readout: bounds, made from half steps."""
+import math
+
 import pytest
 import torch
 
 from bmtk_amd import readout, training
-from test_gpu_readout import DTYPES, TINY, U, close, gen, pack, raster
+from test_gpu_readout import DTYPES, TINY, U, close, gen, pack, raster, scan_case, scan_reference
 
 pytestmark = pytest.mark.gpu
 
@@ -99,6 +101,66 @@ def test_label_loss_takes_decays_of_the_weights_type():
     one, other = (training.label_loss(pack(z), 4, weight, d, labels) for d in (decay, decay.half()))
     assert torch.equal(one[0], other[0]) and torch.equal(one[1], other[1])
     assert other[2]["decay"].dtype == torch.float16 and torch.equal(one[2]["decay"].half(), other[2]["decay"])
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# recurrence
+
+def scan_check_of_any_numbers(x, a, state, dh, d_last):
+    """scan_check for results with NaN among them, which are equal to nothing."""
+    want = scan_reference(x, a, state, None, dh, d_last)
+    runs = []
+    for _ in range(2):
+        h, last, saved = readout.gated_scan(x, a, state, save_state=True)
+        runs.append(dict(zip(("h", "last", "dx", "d_decay", "d_state"), (h, last, *readout.gated_scan_bwd(x, a, saved, dh, d_last)))))
+    for name, got in runs[0].items():
+        close(got, want[name], want[name + "_err"], name)
+        assert torch.equal(torch.nan_to_num(got), torch.nan_to_num(runs[1][name]))
+
+
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("steps,batch,dim,groups", [
+    (1, 2, 6, 6), (17, 2, 6, 6), (200, 2, 40, 0), (200, 3, 40, 8), (600, 32, 64, 0), (600, 32, 64, 64), (600, 32, 64, 4), (700, 64, 128, 128), (700, 64, 128, 0),
+    (700, 4, 64, 64), (6007, 1, 64, 0), (6007, 2, 64, 16), (3000, 1, 33, 33)])
+def test_infinities_stay_infinite(steps, batch, dim, groups, dtype):
+    """Decays around 0.4 of both signs, whose products over some hundred steps leave fp32; an input and a state that are infinite.  What they are by the
+    definition, step by step, they are however the steps are split up."""
+    for back in (False, True):
+        x, a, state, _, dh, d_last = scan_case(steps, batch, dim, groups, dtype, dtype)
+        a = torch.copysign(0.3 + 0.2 * a.abs(), a).to(a.dtype)
+        if back:
+            d_last[0, 0], d_last[-1, dim - 1] = math.inf, -math.inf
+            dh[steps // 2, 0, 1] = math.inf
+            dh[steps - 1, -1, 2] = math.nan
+        else:
+            state[0, 0], state[-1, dim - 1] = math.inf, -math.inf
+            x[steps // 2, 0, 1] = math.inf
+            x[0, -1, 2] = math.nan
+        scan_check_of_any_numbers(x, a, state, dh, d_last)
+        # a decay of nothing ends an infinite state: as 0 times infinity
+        if groups:
+            a[steps // 3, :, 0] = 0.0
+            scan_check_of_any_numbers(x, a, state, dh, d_last)
+
+
+@pytest.mark.parametrize("steps,batch,dim,groups", [(200, 2, 40, 0), (600, 32, 64, 64), (700, 64, 128, 0), (6007, 1, 64, 64)])
+def test_states_decay_to_nothing(steps, batch, dim, groups):
+    """Large states of which small decays leave nothing.
+
+    A product of decays is kept in fp32, whose numbers are 2^-149 apart below 2^-126.  Below them it stays at 2^-149 where its true value goes on falling, and
+    from 2^-126 down to there each multiplication rounds by 2^-150, of which a decay of 0.1 leaves a tenth at the next: 2^-149 of the state that passes it
+    in one join, and so at most in each of the three (blocks, stretches, groups) on its way.  Four here; gradients of the decays need none, since g is 0
+    wherever that state is not."""
+    x, a, state, _, dh, d_last = scan_case(steps, batch, dim, groups, torch.float32, torch.float32)
+    a = torch.copysign(torch.full_like(a, 0.1), a)
+    state, d_last = state.clamp(-3, 3) * 1e38, d_last.clamp(-3, 3) * 1e38
+    x, dh = torch.zeros_like(x), torch.zeros_like(dh)
+    want = scan_reference(x, a, state, None, dh, d_last)
+    h, last, saved = readout.gated_scan(x, a, state, save_state=True)
+    dx, d_decay, d_state = readout.gated_scan_bwd(x, a, saved, dh, d_last)
+    left, left_back = (4 * 2.0 ** -149 * s.abs().max().item() for s in (state, d_last))
+    for got, name, more in ((h, "h", left), (last, "last", left), (dx, "dx", left_back), (d_decay, "d_decay", 0.0), (d_state, "d_state", left_back)):
+        close(got, want[name], want[name + "_err"] + more, name)
 
 
 # ---------------------------------------------------------------------------------------------------------------------
