@@ -104,6 +104,54 @@ def test_label_loss_takes_decays_of_the_weights_type():
 
 
 # ---------------------------------------------------------------------------------------------------------------------
+# gradient by the spikes
+
+@pytest.mark.parametrize("steps,n,batch,dim", [(20, 9001, 32, 64), (40, 8111, 12, 100), (701, 5003, 1, 128), (60, 9000, 8, 96), (2000, 20011, 4, 20)])
+def test_what_is_not_finite_leaves_the_rest_as_it_is(steps, n, batch, dim):
+    """Large fp32 products: infinities, NaN and numbers that are infinite as bf16, in rows of dy, of the weights and everywhere.  All other results keep
+    their bits."""
+    g = gen(steps)
+    w, dy = torch.randn(n, dim, generator=g).cuda(), torch.randn(steps, batch, dim, generator=g).cuda()
+    bits = torch.zeros(steps, (n * batch + 63) // 64, dtype=torch.int64, device="cuda")
+
+    def dl_dz(w, dy):
+        return readout.spike_readout_bwd(bits, w, dy, batch)[1].view(steps, n, batch)
+
+    def column(w, dy, t, b):
+        return w.double() @ dy[t, b].double()
+    rest = torch.ones(steps, n, batch, dtype=torch.bool, device="cuda")
+    odd, oddw = dy.clone(), w.clone()
+    large = 3.4e38   # (bf16 ends at 3.3895e38; half a step further it is infinity)
+    odd[0, 0, dim - 1], odd[steps // 2, batch - 1, 3], odd[steps - 1, 0, 0] = math.nan, -math.inf, large
+    oddw[:, 0] *= 1e-3   # (so that this one's products stay in fp32)
+    w[:, 0] *= 1e-3
+    clean = dl_dz(w, dy)
+    oddw[7, 5], oddw[n - 1, dim // 2], oddw[n // 2, 1] = math.inf, math.nan, -large
+    for t, b in ((0, 0), (steps // 2, batch - 1), (steps - 1, 0)):
+        rest[t, :, b] = False
+    for i in (7, n - 1, n // 2):
+        rest[:, i] = False
+    got = dl_dz(oddw, odd)
+    assert torch.equal(got[rest], clean[rest])
+    assert got[0, :, 0].isnan().all() and got[:, n - 1].isnan().all()
+    fine = torch.ones(n, dtype=torch.bool, device="cuda")
+    fine[[7, n // 2, n - 1]] = False
+    want = column(oddw, odd, steps // 2, batch - 1)
+    assert want[fine].isinf().all() and torch.equal(got[steps // 2, :, batch - 1][fine].double(), want[fine])
+    want, mag = column(oddw, odd, steps - 1, 0), column(oddw.abs(), odd.abs(), steps - 1, 0)
+    close(got[steps - 1, :, 0][fine], want[fine], (dim + 8) * 2 * U * mag[fine], "a large number")
+    # an infinite weight: infinities, but where the step's dy is not finite itself
+    want = odd.double().view(-1, dim) @ oddw[7].double()
+    reached = got[:, 7].reshape(-1)
+    assert torch.equal(reached.isnan(), want.isnan()) and torch.equal(reached[want.isinf()].double(), want[want.isinf()]) and want.isinf().any()
+    # a run that has diverged
+    assert dl_dz(w, torch.full_like(dy, math.nan)).isnan().all() and dl_dz(torch.full_like(w, math.nan), dy).isnan().all()
+    got = dl_dz(w, torch.where(dy > 0, math.inf, dy))
+    want = torch.where(dy > 0, math.inf, dy)[steps - 1].double() @ w.double().t().contiguous()
+    assert torch.equal(got[steps - 1].t().isnan(), want.isnan()) and torch.equal(got[steps - 1].t().isinf(), want.isinf())
+
+
+# ---------------------------------------------------------------------------------------------------------------------
 # recurrence
 
 def scan_check_of_any_numbers(x, a, state, dh, d_last):
