@@ -52,7 +52,7 @@ struct Call {
                                           c10::DispatchKey::FuncTorchGradWrapper, c10::DispatchKey::Functionalize, c10::DispatchKey::ZeroTensor,
                                           c10::DispatchKey::Conjugate, c10::DispatchKey::Negative});
         fine = t.layout() == at::kStrided && t.has_storage() && !t.key_set().has_any(others) && t.get_device() == device &&
-               !(t.requires_grad() && c10::GradMode::is_enabled());
+               !(t.requires_grad() && c10::GradMode::is_enabled()) && !t._fw_grad(0).defined();
         return &t;
     }
     const at::Tensor *tensor(PyObject *obj, at::ScalarType type, c10::IntArrayRef shape)

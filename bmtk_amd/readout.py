@@ -6,7 +6,7 @@ on labels, and their gradients down to the ``dl_dz`` that ``training.Glif3Bptt.b
 ``token_logprobs``   logits -> log probability of each row's token (label), entropy, most probable alternatives
 
 Each has its backward pass under its name with ``_bwd``, called by the caller as ``Glif3Bptt`` is: autograd does not follow any of
-them (arguments that require gradients are refused while it records).  Tensors are on the current device, work is enqueued on the current stream;
+them (arguments that require gradients are refused while it records, those with a forward-mode tangent always).  Tensors are on the current device, work is enqueued on the current stream;
 nothing synchronises, so all of it can be captured.  float32, bfloat16 and float16; arithmetic in 32 bits, what is returned in 16 bits is rounded
 once.  The same call gives the same bits.  The reference has no counterpart (bmtk has no gradients).
 """
@@ -14,6 +14,7 @@ import ctypes as C
 from typing import NamedTuple, Optional
 
 import torch
+from torch.autograd import forward_ad
 
 from . import _lib
 from .ops import _stream
@@ -56,6 +57,8 @@ def _given(t, name, dtype=None, shape=None):
     """``t`` after the checks that every argument gets."""
     if not isinstance(t, torch.Tensor):
         raise TypeError("{} must be a tensor".format(name))
+    if forward_ad.unpack_dual(t).tangent is not None:
+        raise ValueError("{} carries a tangent, which forward-mode differentiation cannot take through this operation".format(name))
     if not t.is_cuda or t.get_device() != torch.cuda.current_device():
         raise ValueError("{} must be on the current device".format(name))
     if t.requires_grad and torch.is_grad_enabled():

@@ -3,6 +3,7 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
 from bmtk_amd import readout, training
 from test_gpu_readout import DTYPES, TINY, U, close, gen, pack, raster, scan_case, scan_reference
@@ -261,3 +262,35 @@ def test_gradient_of_logits_far_from_zero(rows, vocab, dtype):
         close(d, want, err, "d_logits")
         assert readout.token_logprobs_bwd(part, tokens, r, dl, de, out=part) is part
         assert torch.equal(part, d)
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# tensors that are not what they look like
+
+def calls(x):
+    """Every operation with `x` [3, 4, 5] among its arguments, in every place where it can be."""
+    weight, bits, dy = torch.ones(9, 5, device="cuda"), torch.zeros(3, 1, dtype=torch.int64, device="cuda"), torch.ones(3, 4, 5, device="cuda")
+    decay, one, tokens = torch.ones(5, device="cuda"), torch.ones(3, 4, device="cuda"), torch.zeros(3, 4, dtype=torch.int64, device="cuda")
+    saved, logits = torch.zeros(1, 4, 5, device="cuda"), torch.ones(3, 4, 5, device="cuda")
+    r = readout.token_logprobs(logits, tokens)
+    flat = readout.token_logprobs(logits[0], tokens[0])
+    return [
+        lambda: readout.spike_readout(bits, x.view(12, 5), 4), lambda: readout.spike_readout_bwd(bits, x.view(12, 5), dy, 4),
+        lambda: readout.spike_readout_bwd(bits, weight, x, 4), lambda: readout.gated_scan(x, decay), lambda: readout.gated_scan(dy, x[0, 0]), lambda: readout.gated_scan(dy, x),
+        lambda: readout.gated_scan(dy, decay, x[0]), lambda: readout.gated_scan_bwd(x, decay, saved, dy), lambda: readout.gated_scan_bwd(dy, x, saved, dy),
+        lambda: readout.gated_scan_bwd(dy, decay, x[:1], dy), lambda: readout.gated_scan_bwd(dy, decay, saved, x), lambda: readout.gated_scan_bwd(dy, decay, saved, dy, x[0]),
+        lambda: readout.token_logprobs(x, tokens), lambda: readout.token_logprobs(x[0], tokens[0]), lambda: readout.token_logprobs_bwd(x, tokens, r, one),
+        lambda: readout.token_logprobs_bwd(x[0], tokens[0], flat, one[0]), lambda: readout.token_logprobs_bwd(logits, tokens, r, x[..., 0].contiguous()),
+        lambda: readout.token_logprobs_bwd(logits, tokens, r, None, x[..., 0].contiguous()), lambda: readout.token_logprobs_bwd(logits, tokens, r, one, out=x),
+        lambda: training.label_loss(bits, 4, x.view(12, 5), decay, tokens), lambda: training.label_loss(bits, 4, x.view(12, 5).half(), decay, tokens)]
+
+
+@pytest.mark.parametrize("no_grad", [False, True])
+def test_tensors_with_a_tangent_are_refused(no_grad):
+    with forward_ad.dual_level():
+        x = torch.full((3, 4, 5), 0.5, device="cuda")
+        plain, dual = calls(x), calls(forward_ad.make_dual(x, torch.ones_like(x)))
+        for p, d in zip(plain, dual):
+            p()
+            with torch.set_grad_enabled(not no_grad), pytest.raises(ValueError, match="tangent"):
+                d()
