@@ -59,6 +59,8 @@ def _given(t, name, dtype=None, shape=None):
         raise TypeError("{} must be a tensor".format(name))
     if forward_ad.unpack_dual(t).tangent is not None:
         raise ValueError("{} carries a tangent, which forward-mode differentiation cannot take through this operation".format(name))
+    if t.is_neg():
+        raise ValueError("{} is a view of numbers with the other sign: call resolve_neg() on it".format(name))
     if not t.is_cuda or t.get_device() != torch.cuda.current_device():
         raise ValueError("{} must be on the current device".format(name))
     if t.requires_grad and torch.is_grad_enabled():

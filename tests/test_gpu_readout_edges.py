@@ -294,3 +294,15 @@ def test_tensors_with_a_tangent_are_refused(no_grad):
             p()
             with torch.set_grad_enabled(not no_grad), pytest.raises(ValueError, match="tangent"):
                 d()
+
+
+def test_negated_views_are_refused():
+    """The imaginary part of a conjugate is a view whose numbers have the other sign in memory."""
+    z = torch.complex(torch.ones(3, 4, 1, device="cuda"), torch.full((3, 4, 1), 0.5, device="cuda"))
+    x = z.conj().imag
+    assert x.is_neg() and x.stride(0) == 8
+    decay, tokens = torch.ones(1, device="cuda"), torch.zeros(3, 4, dtype=torch.int64, device="cuda")
+    for call in (lambda x: readout.gated_scan(x, decay)[0], lambda x: readout.gated_scan(x.resolve_neg(), x)[0], lambda x: readout.token_logprobs(x[:, 0], tokens[:, 0])[2]):
+        with pytest.raises(ValueError, match="resolve_neg"):
+            call(x)
+        call(x.resolve_neg())

@@ -15,3 +15,12 @@ def test_tangents():
             for recording in (True, False):
                 with torch.set_grad_enabled(recording), pytest.raises(ValueError, match="tangent"):
                     call()
+
+
+def test_negated_views():
+    x = torch.complex(torch.ones(3, 2, 1), torch.ones(3, 2, 1)).conj().imag
+    assert x.is_neg()
+    with pytest.raises(ValueError, match="resolve_neg"):
+        readout.gated_scan(x, torch.ones(1))
+    with pytest.raises(ValueError, match="current device"):
+        readout.gated_scan(x.resolve_neg(), torch.ones(1))
