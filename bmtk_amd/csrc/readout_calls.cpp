@@ -1,7 +1,7 @@
 // The calls of bmtk_amd/readout.py for arguments that are what they should be: checked, results allocated and the C ABI called without the steps in
 // between that a Python function takes for each of its arguments (gated_scan of one step: 12.4 us in Python).  Every function
-// returns None for what it does not take, errors included: the Python function then goes through it argument by argument.  built_for: the torch
-// whose headers it was compiled with.
+// returns None for what it does not take, errors included: the Python function then goes through it argument by argument.  built_for and
+// abi_version: the torch and the library whose headers it was compiled with.
 #define PY_SSIZE_T_CLEAN
 #include <Python.h>
 
@@ -364,7 +364,7 @@ PyModuleDef module = {PyModuleDef_HEAD_INIT, "_readout", nullptr, -1, methods, n
 PyMODINIT_FUNC PyInit__readout()
 {
     PyObject *m = PyModule_Create(&module);
-    if (m != nullptr && PyModule_AddStringConstant(m, "built_for", BMTK_AMD_TORCH) != 0) {
+    if (m != nullptr && (PyModule_AddStringConstant(m, "built_for", BMTK_AMD_TORCH) != 0 || PyModule_AddIntConstant(m, "abi_version", BMTK_AMD_ABI_VERSION) != 0)) {
         Py_DECREF(m);
         return nullptr;
     }

@@ -23,7 +23,7 @@ _CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 
 class _Native:
-    """The same calls in native code for arguments that are as they should be, where that has been built for this torch; None for all others."""
+    """The same calls in native code for arguments that are as they should be, where that has been built for this torch and library; None for all others."""
     NAMES = ("spike_readout", "spike_readout_bwd", "gated_scan", "gated_scan_bwd", "token_logprobs", "token_logprobs_bwd")
     LIBRARY = ("spike_readout_workspace_bytes", "spike_readout_fwd", "spike_readout_bwd_weight", "spike_readout_bwd_spikes", "gated_scan_workspace_bytes",
                "gated_scan_fwd", "gated_scan_bwd", "token_logprobs_workspace_bytes", "token_logprobs_fwd", "token_logprobs_bwd")
@@ -41,7 +41,8 @@ class _Native:
             from . import _readout
         except ImportError:
             _readout = None
-        if getattr(_readout, "built_for", None) != str(torch.__version__):
+        # (it calls the library by the signatures and sizes of the header that it was built with)
+        if (getattr(_readout, "built_for", None), getattr(_readout, "abi_version", None)) != (str(torch.__version__), _lib.ABI_VERSION):
             _readout = None
         if _readout is not None:
             _readout.set_library(tuple(C.cast(getattr(lib, "bmtk_" + name), C.c_void_p).value for name in self.LIBRARY), torch._C._cuda_getCurrentRawStream)

@@ -1,9 +1,13 @@
-"""Arguments of the readout operations that are not what they look like, refused before anything is asked of a device."""
+"""What the readout operations do not take for what it looks like: arguments, refused before anything is asked of a device, and calls in native code."""
+import sys
+import types
+
 import pytest
 import torch
 import torch.autograd.forward_ad as forward_ad
 
-from bmtk_amd import readout
+import bmtk_amd
+from bmtk_amd import _lib, readout
 
 
 def test_tangents():
@@ -24,3 +28,27 @@ def test_negated_views():
         readout.gated_scan(x, torch.ones(1))
     with pytest.raises(ValueError, match="current device"):
         readout.gated_scan(x.resolve_neg(), torch.ones(1))
+
+
+@pytest.mark.parametrize("torch_version,abi,taken", [(torch.__version__, _lib.ABI_VERSION, True), (torch.__version__, _lib.ABI_VERSION - 1, False), (torch.__version__, None, False),
+                                                     ("1.0", _lib.ABI_VERSION, False)])
+def test_calls_in_native_code_of_another_header(monkeypatch, torch_version, abi, taken):
+    """Compiled with another bmtk_amd.h than the library, they would call its functions by other signatures: the Python functions are used then."""
+    handed = []
+    module = types.ModuleType("bmtk_amd._readout")
+    module.built_for, module.set_library = str(torch_version), lambda *a: handed.append(a)
+    if abi is not None:
+        module.abi_version = abi
+    for name in readout._Native.NAMES:
+        setattr(module, name, lambda *_: "native")
+    monkeypatch.setitem(sys.modules, "bmtk_amd._readout", module)
+    monkeypatch.setattr(bmtk_amd, "_readout", module, raising=False)
+    monkeypatch.setattr(torch.cuda, "is_initialized", lambda: True)
+    native = readout._Native()
+    assert native.spike_readout() is None
+    assert len(handed) == taken and native.gated_scan() == ("native" if taken else None)
+
+
+def test_native_code_that_is_built_names_its_header():
+    native = pytest.importorskip("bmtk_amd._readout")
+    assert native.abi_version == _lib.ABI_VERSION and native.built_for == str(torch.__version__)
