@@ -1094,6 +1094,7 @@ extern "C" int bmtk_gated_scan_bwd(int64_t n_steps, int64_t batch, int32_t dim, 
     if (groups == dim || groups == 0) pairs = pairs && in_pairs(decay, gate_dtype, a_t, a_b) && in_pairs(d_decay, gate_dtype, 0, 0);
     const Plan p = plan_of(n_steps, batch, dim, groups, dtype, pairs);
     const bool joined = groups == 0 || (groups != dim && p.parts != groups);
+    BMTK_REQUIRE(groups == 0 || !joined || div_up(n_steps * batch * groups, kBlock) * kBlock < (1ll << 32), "gated_scan_bwd: too many gates, n_steps * batch * groups must stay below 2^32");
     BMTK_REQUIRE((p.sums_floats(batch * dim) == 0 && !joined) || (workspace && aligned(workspace, 8)), "gated_scan_bwd: needs its workspace");
     BMTK_REQUIRE(p.tiles * p.waves * kWave < (1ll << 32), "gated_scan_bwd: too many columns");
     ScanArgs s{};

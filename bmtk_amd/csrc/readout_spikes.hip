@@ -843,6 +843,7 @@ extern "C" int bmtk_spike_readout_bwd_weight(const uint64_t *spike_bits, int64_t
     const int64_t fill = n_neurons / 2048 < 1 ? 1 : n_neurons / 2048;
     if (own > fill) own = fill;
     if (own > kSums / vw) own = kSums / vw;
+    BMTK_REQUIRE(div_up(n_neurons, kWaves * own) * kWaves * kWave < (1ll << 32), "spike_readout_bwd_weight: too many neurons");
     const dim3 grid((unsigned)div_up(n_neurons, kWaves * own), (unsigned)div_up(dim, kWave * vw));
     const hipStream_t st = (hipStream_t)stream;
     const FastDiv by_batch = fast_div((uint32_t)batch);

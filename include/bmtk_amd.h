@@ -730,7 +730,7 @@ int bmtk_spike_readout_bwd_spikes(const void *weight, const void *dy, int64_t n_
  * marks (NULL: not kept): the state before every BMTK_SCAN_MARK-th step, [ceil(n_steps / BMTK_SCAN_MARK)][batch][dim], from which the backward
  * pass computes the others again.  Decays of up to 1 in magnitude, or of which the products over any steps in a row stay in 32 bits.
  * Infinities and NaN go on as they do step by step; of a state that decays to less, up to 2^-149 of what it was may be left.
- * Limits: batch * dim < 2^31, n_steps < 2^31 - 4096. */
+ * Limits: batch * dim < 2^31, n_steps < 2^31 - 4096; backward, with gates for several channels, n_steps * batch * groups < 2^32. */
 #define BMTK_SCAN_MARK 16
 int64_t bmtk_gated_scan_workspace_bytes(int64_t n_steps, int64_t batch, int32_t dim, int32_t groups, int32_t backward);
 int bmtk_gated_scan_fwd(int64_t n_steps, int64_t batch, int32_t dim, int32_t groups, int32_t dtype, int32_t gate_dtype, const void *x, int64_t x_t,

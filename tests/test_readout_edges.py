@@ -1,4 +1,5 @@
 """What the readout operations do not take for what it looks like: arguments, refused before anything is asked of a device, and calls in native code."""
+import ctypes as C
 import sys
 import types
 
@@ -52,3 +53,18 @@ def test_calls_in_native_code_of_another_header(monkeypatch, torch_version, abi,
 def test_native_code_that_is_built_names_its_header():
     native = pytest.importorskip("bmtk_amd._readout")
     assert native.abi_version == _lib.ABI_VERSION and native.built_for == str(torch.__version__)
+
+
+def test_launches_of_too_many_threads():
+    """2^32 threads are more than a launch takes: refused before anything of the call is enqueued."""
+    lib, buf = _lib.load(), C.create_string_buffer(256)
+    p = C.addressof(buf)
+
+    def refused(code, *words):
+        message = lib.bmtk_amd_last_error().decode()
+        assert code == -1 and all(w in message for w in words), (code, message)
+    # gates of three channels each, whose parts of the gradient are joined
+    refused(lib.bmtk_gated_scan_bwd(1 << 22, 32, 96, 32, 1, 1, p, 32 * 96, 96, p, 32 * 32, 32, p, None, p, 32 * 96, 96, None, p, p, None, p, None), "gated_scan_bwd", "too many gates")
+    # single trials, 128 neurons a workgroup
+    n = (1 << 31) - 65
+    refused(lib.bmtk_spike_readout_bwd_weight(p, (n + 63) // 64, 1, n, 1, p, 1, 0, p, None), "spike_readout_bwd_weight", "too many neurons")
