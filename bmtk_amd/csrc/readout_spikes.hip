@@ -141,7 +141,8 @@ spike_fwd_kernel(const uint64_t *__restrict__ bits, int64_t stride, int64_t ne, 
             // one spike of every word
 #pragma unroll
             for (int k = 0; k < kWords; ++k) {
-                const uint32_t e = first + (uint32_t)(k * kWave * 64) + (uint32_t)__builtin_ctzll(w[k]);
+                // (of a word of nothing the last place, which nobody takes: there is no first one)
+                const uint32_t e = first + (uint32_t)(k * kWave * 64) + (uint32_t)__builtin_ctzll(w[k] | (1ull << 63));
                 bool mine = w[k] != 0;
                 if (trial_tiles > 1) mine = mine && (unsigned)((int)(e - div_by(e, by_batch) * (uint32_t)batch) - b0) < (unsigned)trials;
                 w[k] &= w[k] - 1;
