@@ -600,20 +600,28 @@ __device__ __forceinline__ void chain(ChainShared<V> &sh, const Chain &ch, const
     __syncthreads();
     // the blocks before this one, and the whole stretch
     float pp[V], pe[V], wp[V], we[V];
+    auto join = [&](auto product_of) {
 #pragma unroll
-    for (int c = 0; c < V; ++c) wp[c] = 1.0f, we[c] = 0.0f;
+        for (int c = 0; c < V; ++c) wp[c] = 1.0f, we[c] = 0.0f;
 #pragma unroll
-    for (int w = 0; w < kChainWaves; ++w) {
-        if (w == wave)
+        for (int w = 0; w < kChainWaves; ++w) {
+            if (w == wave)
 #pragma unroll
-            for (int c = 0; c < V; ++c) pp[c] = wp[c], pe[c] = we[c];
+                for (int c = 0; c < V; ++c) pp[c] = wp[c], pe[c] = we[c];
 #pragma unroll
-        for (int c = 0; c < V; ++c) {
-            const float bp = sh.block[w][0][c][lane];
-            we[c] = passed(bp, we[c]) + sh.block[w][1][c][lane];
-            wp[c] = times(wp[c], bp);
+            for (int c = 0; c < V; ++c) {
+                const float bp = sh.block[w][0][c][lane];
+                we[c] = passed(bp, we[c]) + sh.block[w][1][c][lane];
+                wp[c] = product_of(wp[c], bp);
+            }
         }
-    }
+    };
+    // (every stretch waits for this: products are looked at one by one only where they come out as 0, 4,096 x 8 x 2,048 bf16 75 us against 81)
+    join([](float p, float q) { return p * q; });
+    bool none = false;
+#pragma unroll
+    for (int c = 0; c < V; ++c) none = none || wp[c] == 0.0f;
+    if (__ballot(none) != 0) join([](float p, float q) { return times(p, q); });
     if (wave == 0 && l.in) say<V>(ch.stretch + order * columns + l.col, wp, we);
     // a part of the group's stretches before
     constexpr int kPart = kGroup / kChainWaves;
