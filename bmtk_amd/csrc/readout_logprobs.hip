@@ -518,7 +518,7 @@ __global__ void __launch_bounds__(kBlock) logprobs_bwd_short_kernel(const RowBwd
     }
 }
 
-// Slices of a row: enough workgroups to fill the chip, two loads a lane at least (4 x 131,072, top 20, both launches: four 15.8 us, two 14.2, one 15.0)
+// Slices of a row: enough workgroups to fill the chip, but no more than one for every two loads a lane (begun ones too: 4,097 bf16 are two slices; 4 x 131,072, top 20, both launches: four 15.8 us, two 14.2, one 15.0)
 void slices_of(int64_t rows, int32_t vocab, int32_t dtype, Slices &sl)
 {
     const int64_t unit = 2 * kBlock * (16 / (int64_t)type_size(dtype));

@@ -521,8 +521,8 @@ __global__ void __launch_bounds__(kMaxWaves * kWave) scan_sums_kernel(const Scan
 // the state that entered the group, which the last workgroup of the group before tells.  So every sum is made in an order that is
 // fixed, and the way from one group to the next is all that happens one after the other.
 //
-// 65,536 x 1,000 bf16, a gate per channel: 112 us forward (393 MB, 3.5 TB/s; two passes 156).  4,096 x 8 x 2,048 bf16, a gate per 64 channels, ragged: 77 us
-// forward and 111 back.  Three workgroups on a compute unit in the place of two change nothing: what is left is memory that is read and written by turns.
+// 65,536 x 1,000 bf16, a gate per channel: 114 us forward (393 MB, 3.5 TB/s; two passes 156).  4,096 x 8 x 2,048 bf16, a gate per 64 channels, ragged: 71 us
+// forward and 113 back.  Three workgroups on a compute unit in the place of two change nothing: what is left is memory that is read and written by turns.
 //
 // Workgroups take their stretches by a counter, in the order in which the state passes: what one waits for comes from workgroups that have begun before
 // it and wait for earlier ones only, so every wait ends, however few run at once.  Values are told as 64 bits at a time, all ones being none yet.
@@ -913,6 +913,9 @@ Plan plan_of(int64_t n_steps, int64_t batch, int32_t dim, int32_t groups, int32_
     // One round of more wavefronts in the place of stretches: 150 x 32 x 64 fp32 4.9 / 8.3 us forward, 7.8 / 10.7 back; two such rounds would take 10.1 / 8.0
     // and 13.4 / 11.2 (500 x 32 x 64)
     if (p.splits > 1 && w <= kRoundWaves) p.splits = 1, p.waves = (int)w, p.split_steps = w * kSteps;
+    // A shared gate's gradient is summed over neighbouring lanes, a power of two of them that divides the gate's channels; what that leaves is written as
+    // partial sums, 4 bytes each, and joined.  Gates of 32, 64 and 128 channels leave one sum or few; an odd number of channels one for every channel and step:
+    // 4,096 x 8 x 2,046 bf16, gates of 33, back 1,340 us and 268 MB of workspace; 2,000 channels in gates of 100 238 us; 2,048 in gates of 32 or 64 117 us.
     p.seg_lanes = p.parts = 0;
     if (groups > 0 && groups != dim) {
         const int seg = gcd(channels, kWave * p.v);

@@ -317,8 +317,9 @@ spike_bwd_weight_kernel(const uint64_t *__restrict__ bits, int64_t stride, int64
 // the matrix instructions take them, while those before are multiplied.
 //
 // fp32: the matrix instructions take 16-bit operands sixteen times as fast as 32-bit ones.  Each operand is the sum of three bf16 numbers of 8 bits each
-// (what the one before leaves, rounded), exact to 2^-27 of it; of the nine products the six that are not below 2^-24 of the whole
-// are made and added up in fp32.
+// (what the one before leaves, rounded), exact to 2^-27 of it, and to 2^-134 of anything, where bf16 ends: below 1e-34 that is more, an operand around 1e-36 is
+// off by 3e-5 of itself, one around 1e-39 by 3 %.  Of the nine products the six that are not below 2^-24 of the whole are made and added up in fp32.
+// fp16: the matrix instructions lose what a product with an operand below 2^-14 has below about 2^-35 (of operands around 2e-7 4e-6 of the sum).
 //
 // 600 steps of 51,978 x 32 x 64 fp32: 936 us at the median, 755 at best, for 3.99 GB of results (4.3 to 5.3 TB/s).  Writing them alone, in this order, takes 710 to
 // 760 us, a fill of as much memory from front to back 583.
@@ -693,8 +694,8 @@ int lane_channels(int dim, int dtype, const void *p)
     return vw;
 }
 
-// Slices of a step's words: enough workgroups that those left over at the end are few,
-// two loads of words for every wavefront at least.  600 steps of 51,978 x 32 x 64: one slice 152 us, two 127 and 6 for their sum.  Two loads against
+// Slices of a step's words: enough workgroups that those left over at the end are few, but no more than one for every two loads of words of its wavefronts
+// (begun ones too: 1,025 words are two slices).  600 steps of 51,978 x 32 x 64: one slice 152 us, two 127 and 6 for their sum.  Two loads against
 // one: 100 steps of 3,001 x 12 x 17 6.8 / 8.3 us, 1 of 51,978 x 32 x 64 14.9 / 19.1, 200 of 6,000 x 16 x 10 11.2 / 12.2; many spikes would have more
 // slices, 50 of 5,000 x 32 x 64 at 2 % 19.3 / 15.0, but nobody knows them here.
 int64_t fwd_slices(int64_t n_steps, int64_t words, int64_t tiles)
@@ -719,8 +720,10 @@ FwdPlan fwd_plan(int64_t n_steps, int64_t n, int batch, int dim, int vw)
     const int64_t words = (n * batch + 63) / 64;
     p.slices = fwd_slices(n_steps, words, p.tiles);
     p.waves = kManyWaves;
-    // one step of one trial whose words one workgroup has on their way at once: no slices to join (230,924 neurons, 64 channels: 9.3 us in 8 slices
-    // and their sum, 8.3 in one launch)
+    // one step of one trial, up to four words a lane of one workgroup: no slices to join.  A word a lane at a time, where not all
+    // wavefronts have four: four at once take longer.  64 channels fp32 at 0.3 %, in one workgroup / that with four words at once / in the slices
+    // from above and their sum: 230,924 neurons 7.0 / 7.5 / 8.7 us, 100,000 4.8 / 5.6 / 8.8, 262,144 8.3 / 8.3 / 8.8.  At 2 %, which nobody knows here, slices
+    // would be better, 230,924 neurons 21.1 / 24.2 / 12.8.
     if (batch == 1 && p.slices > 1 && words <= kOneBlockWaves * kWave * kWordsPerLane) p.slices = 1, p.waves = kOneBlockWaves;
     p.slice_words = div_up(div_up(words, p.slices), kWave) * kWave;
     p.slices = div_up(words, p.slice_words);
