@@ -306,3 +306,54 @@ def test_negated_views_are_refused():
         with pytest.raises(ValueError, match="resolve_neg"):
             call(x)
         call(x.resolve_neg())
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+# captured
+
+def odd_case(odd):
+    """Inputs of one shape, ordinary or with infinities, NaN and logits far from zero among them."""
+    g = gen(7)
+    x, a, state, _, dh, d_last = scan_case(700, 4, 64, 64, torch.float32, torch.float32, seed=5)
+    z = raster(50, 24, 4, 0.1, 6)
+    s = dict(w=torch.randn(9001, 64, generator=g).cuda(), dy=torch.randn(20, 32, 64, generator=g).cuda(), x=x, a=torch.copysign(0.3 + 0.2 * a.abs(), a), state=state, dh=dh, d_last=d_last,
+             logits=torch.randn(5, 20000, generator=g).cuda(), few=torch.randn(60, 12, generator=g).cuda(), d_logp=torch.randn(60, generator=g).cuda(),
+             bits=pack(z), weight=torch.randn(24, 6, generator=g).half().cuda())
+    if odd:
+        s["w"][3, 5], s["dy"][2, 1, 0], s["state"][0, 0], s["x"][90, 1, 1], s["dh"][600, 2, 2] = math.inf, math.nan, math.inf, -math.inf, math.nan
+        s["logits"][1:3], s["few"][::2], s["few"][1::4] = torch.finfo(torch.float32).min, torch.finfo(torch.float32).max, s["few"][1::4] + 700
+        s["weight"] *= 100
+    return s
+
+
+def odd_pass(s):
+    none = torch.zeros(20, 9001 * 32 // 64 + 1, dtype=torch.int64, device="cuda")
+    h, last, saved = readout.gated_scan(s["x"], s["a"], s["state"], save_state=True)
+    tokens, few = (torch.arange(n, device="cuda") % 12 for n in (5, 60))
+    r, q = readout.token_logprobs(s["logits"], tokens), readout.token_logprobs(s["few"], few)
+    loss, dl_dz, grads, _ = training.label_loss(s["bits"], 4, s["weight"], torch.full((6,), 0.9, device="cuda"), torch.arange(200, device="cuda").view(50, 4) % 6)
+    return [*readout.spike_readout_bwd(none, s["w"], s["dy"], 32), h, last, *readout.gated_scan_bwd(s["x"], s["a"], saved, s["dh"], s["d_last"]),
+            readout.token_logprobs_bwd(s["logits"], tokens, r, s["d_logp"][:5].clone(), r.entropy), readout.token_logprobs_bwd(s["few"], few, q, s["d_logp"], q.entropy),
+            loss, dl_dz, *grads.values()]
+
+
+def test_captured_and_replayed_on_odd_inputs():
+    """A graph captured on ordinary inputs, replayed on odd ones and on ordinary ones in turn, with eager work between."""
+    cases = [odd_case(False), odd_case(True)]
+    want = [[torch.nan_to_num(t, nan=12345.0) for t in odd_pass(c)] for c in cases]
+    held = {name: t.clone() for name, t in cases[0].items()}
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    with torch.cuda.stream(side):
+        odd_pass(held)
+    torch.cuda.current_stream().wait_stream(side)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        out = odd_pass(held)
+    for turn in (1, 0, 1, 1, 0):
+        for name, t in cases[turn].items():
+            held[name].copy_(t)
+        graph.replay()
+        odd_pass(cases[1 - turn])
+        torch.cuda.synchronize()
+        assert all(torch.equal(torch.nan_to_num(p, nan=12345.0), q) for p, q in zip(out, want[turn]))
