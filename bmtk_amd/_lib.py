@@ -68,7 +68,7 @@ class Glif3Bwd(C.Structure):
 
 
 EVENTS_INCONSISTENT = 1     # BMTK_EVENTS_INCONSISTENT
-ABI_VERSION = 38  # BMTK_AMD_ABI_VERSION of include/bmtk_amd.h that the mirrors above were written for
+ABI_VERSION = 39  # BMTK_AMD_ABI_VERSION of include/bmtk_amd.h that the mirrors above were written for
 
 # name -> (restype, argtypes); every symbol include/bmtk_amd.h declares
 SIGNATURES = {
@@ -140,6 +140,13 @@ SIGNATURES = {
     "bmtk_token_logprobs_workspace_bytes": (c_int64, [c_int64, c_int32, c_int32, c_int32]),
     "bmtk_token_logprobs_fwd": (c_int32, [c_int64, c_int32, c_int32, c_void_p, c_int64, c_void_p, c_int64, c_int32] + [c_void_p] * 7),
     "bmtk_token_logprobs_bwd": (c_int32, [c_int64, c_int32, c_int32, c_void_p, c_int64, c_void_p, c_int64] + [c_void_p] * 5 + [c_int64, c_void_p]),
+    "bmtk_short_conv_workspace_bytes": (c_int64, [c_int64, c_int64] + [c_int32] * 3),
+    "bmtk_short_conv_fwd": (c_int32, [c_int64, c_int64] + [c_int32] * 5 + [c_void_p, c_int64, c_int64] + [c_void_p] * 7),
+    "bmtk_short_conv_bwd": (c_int32, [c_int64, c_int64] + [c_int32] * 5 + [c_void_p, c_int64, c_int64] + [c_void_p] * 4 + [c_void_p, c_int64, c_int64] + [c_void_p] * 7),
+    "bmtk_selective_scan_workspace_bytes": (c_int64, [c_int64, c_int64] + [c_int32] * 4),
+    "bmtk_selective_scan_fwd": (c_int32, [c_int64, c_int64] + [c_int32] * 6 + [c_void_p, c_int64, c_int64] * 4 + [c_void_p] * 10),
+    "bmtk_selective_scan_bwd": (c_int32, [c_int64, c_int64] + [c_int32] * 6 + [c_void_p, c_int64, c_int64] * 4 + [c_void_p] * 5 + [c_void_p, c_int64, c_int64] +
+                                [c_void_p] * 11),
     "bmtk_rate_mse": (c_int32, [c_void_p, c_int64, c_int32, c_int64, c_void_p, c_int64] + [c_void_p] * 5),
 }
 
@@ -150,6 +157,8 @@ RECORD_COUNT_STRIDE = 16
 RES_FIRED_SLOTS = 16              # BMTK_RES_FIRED_SLOTS
 SCAN_MARK = 16                    # BMTK_SCAN_MARK
 LOGPROBS_MAX_TOP = 64             # BMTK_LOGPROBS_MAX_TOP
+CONV_MAX_WIDTH = 8                # BMTK_CONV_MAX_WIDTH
+SELECTIVE_MAX_STATES = 64         # BMTK_SELECTIVE_MAX_STATES
 
 
 class LibraryMissing(RuntimeError):

@@ -24,7 +24,8 @@ _CODE = {torch.float32: 0, torch.bfloat16: 1, torch.float16: 2}
 
 class _Native:
     """The same calls in native code for arguments that are as they should be, where that has been built for this torch and library; None for all others."""
-    NAMES = ("spike_readout", "spike_readout_bwd", "gated_scan", "gated_scan_bwd", "token_logprobs", "token_logprobs_bwd")
+    NAMES = ("spike_readout", "spike_readout_bwd", "gated_scan", "gated_scan_bwd", "token_logprobs", "token_logprobs_bwd", "short_conv", "short_conv_bwd", "selective_scan",
+             "selective_scan_bwd", "projected_logprobs", "projected_logprobs_bwd")
     LIBRARY = ("spike_readout_workspace_bytes", "spike_readout_fwd", "spike_readout_bwd_weight", "spike_readout_bwd_spikes", "gated_scan_workspace_bytes",
                "gated_scan_fwd", "gated_scan_bwd", "token_logprobs_workspace_bytes", "token_logprobs_fwd", "token_logprobs_bwd")
 
@@ -243,6 +244,208 @@ def gated_scan_bwd(x, decay, saved, dh, d_last=None, lengths=None):
     else:
         d_state.zero_()
     return dx, d_decay, d_state
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+
+def _ptr(t):
+    return None if t is None else t.data_ptr()
+
+
+def _sequences(x, name="x"):
+    if x.dim() != 3 or x.shape[1] == 0 or x.shape[2] == 0:
+        raise ValueError("{} must be [steps, sequences, channels]".format(name))
+    return x.shape
+
+
+def _conv(x, weight, bias, state, lengths, silu):
+    """(steps, sequences, channels, width, sizes and what both directions point to)"""
+    _given(x, "x")
+    _contiguous(weight, "weight")
+    steps, batch, dim = _sequences(x)
+    if weight.dim() != 2 or weight.shape[0] != dim or not 2 <= weight.shape[1] <= _lib.CONV_MAX_WIDTH:
+        raise ValueError("weight must be [{}, 2..{}], got {}".format(dim, _lib.CONV_MAX_WIDTH, tuple(weight.shape)))
+    if weight.dtype != torch.float32 and weight.dtype != x.dtype:
+        raise TypeError("weight must be float32 or of the type of x, {}, got {}".format(x.dtype, weight.dtype))
+    width = weight.shape[1]
+    if bias is not None:
+        _contiguous(bias, "bias", weight.dtype, (dim,))
+    if state is not None:
+        _contiguous(state, "state", x.dtype, (width - 1, batch, dim))
+    if lengths is not None:
+        _contiguous(lengths, "lengths", torch.int32, (batch,))
+    return steps, batch, dim, width, ((steps, batch, dim, width, _CODE[x.dtype], _CODE[weight.dtype], int(bool(silu))) + _rows(x, "x")
+                                      + (weight.data_ptr(), _ptr(bias), _ptr(state), _ptr(lengths)))
+
+
+def short_conv(x, weight, bias=None, state=None, lengths=None, silu=False):
+    """y[t] = bias + the sum of the last few x, each with a weight of its channel, and with ``silu`` that times its sigmoid: (y, last).
+
+    x       [steps, sequences, channels]; steps and sequences at any distance in memory, the channels next to one another
+    weight  [channels, width], width 2 to 8; weight[:, width - 1] is for the present step.  Of the type of ``x`` or float32
+    bias    [channels], of the type of ``weight`` (None: zero)
+    state   [width - 1, sequences, channels], of the type of ``x``: the inputs before the first step (None: zero)
+    lengths int32 [sequences]: steps of each sequence (None: all).  y is 0 behind them and nothing of x counts there; values outside
+            0..steps count as the nearer of the two
+    y has the type and shape of ``x``; last, of the state's shape: the last inputs of each sequence, the ``state`` of the next call, of a single step or
+    of many."""
+    r = _native.short_conv(x, weight, bias, state, lengths, silu)
+    if r is not None:
+        return r
+    steps, batch, dim, width, args = _conv(x, weight, bias, state, lengths, silu)
+    y = torch.empty(steps, batch, dim, dtype=x.dtype, device=x.device)
+    last = torch.empty(width - 1, batch, dim, dtype=x.dtype, device=x.device)
+    if steps:
+        _lib.check(_lib.load().bmtk_short_conv_fwd(*args, y.data_ptr(), last.data_ptr(), _stream()))
+    elif state is not None:
+        last.copy_(state)
+    else:
+        last.zero_()
+    return y, last
+
+
+def short_conv_bwd(x, weight, dy, bias=None, state=None, d_last=None, lengths=None, silu=False):
+    """(dx, d_weight, d_bias, d_state) from the gradients of ``short_conv``'s y, ``dy`` (the type of ``x``, strides as ``x`` may have), and last, ``d_last``
+    (of last's type and shape, None: zero).  x, weight, bias, state, lengths, silu: as they were.
+
+    dx: as ``x``, 0 behind a sequence's end; d_weight, d_bias: as ``weight`` and ``bias``, summed over steps and sequences; d_state: as ``state``.  All four are
+    returned, where there was no bias or state too."""
+    r = _native.short_conv_bwd(x, weight, dy, bias, state, d_last, lengths, silu)
+    if r is not None:
+        return r
+    steps, batch, dim, width, args = _conv(x, weight, bias, state, lengths, silu)
+    if _given(dy, "dy", x.dtype).shape != x.shape:
+        raise ValueError("dy must be {}, got {}".format(tuple(x.shape), tuple(dy.shape)))
+    if d_last is not None:
+        _contiguous(d_last, "d_last", x.dtype, (width - 1, batch, dim))
+    dev = x.device
+    dx = torch.empty(steps, batch, dim, dtype=x.dtype, device=dev)
+    make = torch.empty if steps else torch.zeros
+    d_weight, d_bias = make(dim, width, dtype=weight.dtype, device=dev), make(dim, dtype=weight.dtype, device=dev)
+    d_state = torch.empty(width - 1, batch, dim, dtype=x.dtype, device=dev)
+    if steps:
+        lib = _lib.load()
+        ws = _Workspace(lib.bmtk_short_conv_workspace_bytes(steps, batch, dim, width, _CODE[x.dtype]), dev)
+        _lib.check(lib.bmtk_short_conv_bwd(*args, *_rows(dy, "dy"), _ptr(d_last), dx.data_ptr(), d_weight.data_ptr(), d_bias.data_ptr(), d_state.data_ptr(), ws.ptr, _stream()))
+    elif d_last is not None:
+        d_state.copy_(d_last)
+    else:
+        d_state.zero_()
+    return dx, d_weight, d_bias, d_state
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+
+class SelectiveGrads(NamedTuple):
+    """What ``selective_scan_bwd`` returns: gradients of the types and shapes of the inputs that they are named for."""
+    dx: torch.Tensor
+    d_dt: torch.Tensor
+    d_rate: torch.Tensor
+    d_write: torch.Tensor
+    d_read: torch.Tensor
+    d_skip: torch.Tensor
+    d_dt_bias: torch.Tensor
+    d_state: torch.Tensor
+
+
+def _selective(x, dt, rate, write, read, skip, dt_bias, softplus, lengths):
+    """(steps, sequences, channels, groups, states, sizes and what both directions point to)"""
+    _given(x, "x")
+    _given(dt, "dt")
+    _contiguous(rate, "rate", torch.float32)
+    steps, batch, dim = _sequences(x)
+    if dt.dtype != torch.float32 and dt.dtype != x.dtype:
+        raise TypeError("dt must be float32 or of the type of x, {}, got {}".format(x.dtype, dt.dtype))
+    if tuple(dt.shape) != tuple(x.shape):
+        raise ValueError("dt must be {}, got {}".format(tuple(x.shape), tuple(dt.shape)))
+    if rate.dim() != 2 or rate.shape[0] != dim or not 1 <= rate.shape[1] <= _lib.SELECTIVE_MAX_STATES:
+        raise ValueError("rate must be [{}, 1..{}], got {}".format(dim, _lib.SELECTIVE_MAX_STATES, tuple(rate.shape)))
+    states = rate.shape[1]
+    _given(write, "write", x.dtype)
+    if write.dim() != 4 or tuple(write.shape[:2]) != (steps, batch) or write.shape[3] != states or not write.shape[2] or dim % write.shape[2]:
+        raise ValueError("write must be [{}, {}, groups, {}] with a number of groups that divides the channels; got {}".format(steps, batch, states, tuple(write.shape)))
+    groups = write.shape[2]
+    _given(read, "read", x.dtype, write.shape)
+    shared = ()
+    for t, name in ((write, "write"), (read, "read")):
+        if (states > 1 and t.stride(3) != 1) or (groups > 1 and t.stride(2) != states):
+            raise ValueError("the groups' states of {} must lie next to one another".format(name))
+        shared += (t.data_ptr(), t.stride(0), t.stride(1))
+    for t, name in ((skip, "skip"), (dt_bias, "dt_bias")):
+        if t is not None:
+            _contiguous(t, name, torch.float32, (dim,))
+    if lengths is not None:
+        _contiguous(lengths, "lengths", torch.int32, (batch,))
+    return steps, batch, dim, groups, states, ((steps, batch, dim, groups, states, _CODE[x.dtype], _CODE[dt.dtype], int(bool(softplus))) + _rows(x, "x") + _rows(dt, "dt")
+                                               + shared + (rate.data_ptr(), _ptr(skip), _ptr(dt_bias)))
+
+
+def selective_scan(x, dt, rate, write, read, skip=None, dt_bias=None, softplus=False, state=None, lengths=None, save_state=False):
+    """A memory of several states a channel whose step size and whose input and output weights come with every step: (y, last), with ``save_state`` (y, last, saved).
+    With delta = dt + dt_bias, or with ``softplus`` log(1 + e^(dt + dt_bias)),
+
+        h[t, c, n] = e^(delta[t, c] rate[c, n]) h[t - 1, c, n] + delta[t, c] x[t, c] write[t, n]
+        y[t, c]    = sum over n of read[t, n] h[t, c, n] + skip[c] x[t, c]
+
+    x       [steps, sequences, channels]; steps and sequences at any distance in memory, the channels next to one another; dt likewise, of the type of ``x``
+            or float32
+    rate    float32 [channels, states], up to 64 states; delta * rate is meant to be 0 or less
+    write, read  [steps, sequences, groups, states], of the type of ``x``, the states of a step next to one another; each group is for
+            channels / groups neighbouring channels
+    skip, dt_bias  float32 [channels] (None: zero)
+    state   float32 [sequences, channels, states]: the state before the first step (None: zero)
+    lengths int32 [sequences]: steps of each sequence (None: all).  y is 0 behind them and nothing of the inputs counts there; values outside
+            0..steps count as the nearer of the two
+    y has the type and shape of ``x``; last is float32 and of the state's shape: the ``state`` of the next call, of a single step or of many.
+    saved: what ``selective_scan_bwd`` takes, float32 [steps / 16, sequences, channels, states]."""
+    r = _native.selective_scan(x, dt, rate, write, read, skip, dt_bias, softplus, state, lengths, save_state)
+    if r is not None:
+        return r
+    steps, batch, dim, groups, states, args = _selective(x, dt, rate, write, read, skip, dt_bias, softplus, lengths)
+    if state is not None:
+        _contiguous(state, "state", torch.float32, (batch, dim, states))
+    dev = x.device
+    y = torch.empty(steps, batch, dim, dtype=x.dtype, device=dev)
+    last = torch.empty(batch, dim, states, dtype=torch.float32, device=dev)
+    saved = torch.empty(-(-steps // _lib.SCAN_MARK), batch, dim, states, dtype=torch.float32, device=dev) if save_state else None
+    if steps:
+        lib = _lib.load()
+        ws = _Workspace(lib.bmtk_selective_scan_workspace_bytes(steps, batch, dim, groups, states, 0), dev)
+        _lib.check(lib.bmtk_selective_scan_fwd(*args, _ptr(state), _ptr(lengths), y.data_ptr(), last.data_ptr(), _ptr(saved), ws.ptr, _stream()))
+    elif state is not None:
+        last.copy_(state)
+    else:
+        last.zero_()
+    return (y, last, saved) if save_state else (y, last)
+
+
+def selective_scan_bwd(x, dt, rate, write, read, saved, dy, skip=None, dt_bias=None, softplus=False, d_last=None, lengths=None):
+    """``SelectiveGrads`` from the gradients of ``selective_scan``'s y, ``dy`` (the type of ``x``, strides as ``x`` may have), and last, ``d_last`` (float32, None:
+    zero).  The other arguments as they were; saved: what the forward pass returned.  The states are computed again from it in 32 bits.
+
+    Gradients behind a sequence's end are 0.  d_write and d_read are summed over the channels of a group, d_rate, d_skip and d_dt_bias over steps and sequences.  All
+    are returned, where there was no skip, dt_bias or state too."""
+    r = _native.selective_scan_bwd(x, dt, rate, write, read, saved, dy, skip, dt_bias, softplus, d_last, lengths)
+    if r is not None:
+        return SelectiveGrads(*r)
+    steps, batch, dim, groups, states, args = _selective(x, dt, rate, write, read, skip, dt_bias, softplus, lengths)
+    if _given(dy, "dy", x.dtype).shape != x.shape:
+        raise ValueError("dy must be {}, got {}".format(tuple(x.shape), tuple(dy.shape)))
+    _contiguous(saved, "saved", torch.float32, (-(-steps // _lib.SCAN_MARK), batch, dim, states))
+    if d_last is not None:
+        _contiguous(d_last, "d_last", torch.float32, (batch, dim, states))
+    dev = x.device
+    make = lambda like, shape: (torch.empty if steps else torch.zeros)(shape, dtype=like.dtype, device=dev)  # noqa: E731
+    d = SelectiveGrads(make(x, x.shape), make(dt, dt.shape), make(rate, rate.shape), make(write, write.shape), make(read, read.shape), make(rate, (dim,)),
+                       make(rate, (dim,)), make(rate, (batch, dim, states)))
+    if steps:
+        lib = _lib.load()
+        ws = _Workspace(lib.bmtk_selective_scan_workspace_bytes(steps, batch, dim, groups, states, 1), dev)
+        _lib.check(lib.bmtk_selective_scan_bwd(*args, saved.data_ptr(), _ptr(lengths), *_rows(dy, "dy"), _ptr(d_last), d.dx.data_ptr(), d.d_dt.data_ptr(), d.d_write.data_ptr(),
+                                               d.d_read.data_ptr(), d.d_rate.data_ptr(), d.d_skip.data_ptr(), d.d_dt_bias.data_ptr(), d.d_state.data_ptr(), ws.ptr, _stream()))
+    elif d_last is not None:
+        d.d_state.copy_(d_last)
+    return d
 
 
 # ---------------------------------------------------------------------------------------------------------------------

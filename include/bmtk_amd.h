@@ -49,7 +49,7 @@ extern "C" {
 
 /* Bumped whenever a struct layout or a signature below changes; bmtk_amd_abi_version() returns the value the
  * library was built with. */
-#define BMTK_AMD_ABI_VERSION 38
+#define BMTK_AMD_ABI_VERSION 39
 int bmtk_amd_abi_version(void);
 const char *bmtk_amd_last_error(void);
 /* sizeof(bmtk_glif3_sim) as the library was compiled, for bindings that mirror the struct */
@@ -755,6 +755,47 @@ int bmtk_token_logprobs_fwd(int64_t rows, int32_t vocab, int32_t dtype, const vo
 int bmtk_token_logprobs_bwd(int64_t rows, int32_t vocab, int32_t dtype, const void *logits, int64_t row_stride, const int64_t *tokens, int64_t ignore,
                             const float *lse, const float *entropy, const float *d_logp, const float *d_entropy, void *d_logits, int64_t out_stride,
                             void *stream);
+
+/* y[t][b][c] = f(bias[c] + sum_j weight[c][j] x[t - (width - 1) + j][b][c]) for the steps t < lengths[b] (NULL: all n_steps), f the identity or, with
+ * silu, z / (1 + e^-z); y is 0 behind a sequence's end and nothing of x counts there.  state [width - 1][batch][dim] (NULL: zero): the inputs before
+ * step 0; last, of the same shape: those before the step behind each sequence's end, the state of the next call.
+ * weight [dim][width], bias [dim] (NULL: zero): of weight_dtype, BMTK_F32 or dtype.  x_t, x_b, dy_t, dy_b: distance of steps and of sequences in
+ * x and dy, in elements (a channel's neighbour is next to it); everything else is contiguous and, where its type is not said, of dtype.
+ * Limits: width in 2 .. BMTK_CONV_MAX_WIDTH, batch * dim < 2^31, n_steps < 2^31 - 4096. */
+#define BMTK_CONV_MAX_WIDTH 8
+int bmtk_short_conv_fwd(int64_t n_steps, int64_t batch, int32_t dim, int32_t width, int32_t dtype, int32_t weight_dtype, int32_t silu, const void *x, int64_t x_t,
+                        int64_t x_b, const void *weight, const void *bias, const void *state, const int32_t *lengths, void *y, void *last, void *stream);
+/* dy, d_last (NULL: zero): gradients of y and last; dx, d_weight, d_bias, d_state (either NULL: not wanted): of x, weight, bias and state.  workspace:
+ * bmtk_short_conv_workspace_bytes, of the backward pass only */
+int64_t bmtk_short_conv_workspace_bytes(int64_t n_steps, int64_t batch, int32_t dim, int32_t width, int32_t dtype);
+int bmtk_short_conv_bwd(int64_t n_steps, int64_t batch, int32_t dim, int32_t width, int32_t dtype, int32_t weight_dtype, int32_t silu, const void *x, int64_t x_t,
+                        int64_t x_b, const void *weight, const void *bias, const void *state, const int32_t *lengths, const void *dy, int64_t dy_t, int64_t dy_b,
+                        const void *d_last, void *dx, void *d_weight, void *d_bias, void *d_state, float *workspace, void *stream);
+
+/* A memory of n_states numbers a channel whose step size, input and output weights come with every step: with delta = dt + dt_bias[c], or with
+ * softplus log(1 + e^(dt + dt_bias[c])), for the steps t < lengths[b] (NULL: all n_steps),
+ *     h[c][n] = e^(delta rate[c][n]) h[c][n] + delta x[t][b][c] write[t][b][g][n],   y[t][b][c] = sum_n read[t][b][g][n] h[c][n] + skip[c] x[t][b][c],
+ * from state [batch][dim][n_states] (NULL: zero), g = c / (dim / groups); y is 0 behind a sequence's end and nothing of the inputs counts there.  last, of
+ * the state's shape: the state behind each sequence's last step.
+ * x, write, read, y: of dtype; dt: of dt_dtype, BMTK_F32 or dtype; rate [dim][n_states], skip, dt_bias [dim] (NULL: zero), state, last, marks: 32 bits.
+ * x_t .. read_b: distance of steps and of sequences, in elements; the channels of a step, and its groups' states, lie next to one another; everything else
+ * is contiguous.  marks (NULL: not kept): the state before every BMTK_SCAN_MARK-th step, [ceil(n_steps / BMTK_SCAN_MARK)][batch][dim][n_states],
+ * which the backward pass needs.  delta * rate of up to 0, or such that e to its sums over any steps in a row stays in 32 bits; of a state that decays to less,
+ * up to 2^-126 of what it was may be left.
+ * Limits: n_states in 1 .. BMTK_SELECTIVE_MAX_STATES, batch * dim < 2^31, n_steps < 2^31 - 4096. */
+#define BMTK_SELECTIVE_MAX_STATES 64
+int64_t bmtk_selective_scan_workspace_bytes(int64_t n_steps, int64_t batch, int32_t dim, int32_t groups, int32_t n_states, int32_t backward);
+int bmtk_selective_scan_fwd(int64_t n_steps, int64_t batch, int32_t dim, int32_t groups, int32_t n_states, int32_t dtype, int32_t dt_dtype, int32_t softplus, const void *x,
+                            int64_t x_t, int64_t x_b, const void *dt, int64_t dt_t, int64_t dt_b, const void *write, int64_t write_t, int64_t write_b, const void *read,
+                            int64_t read_t, int64_t read_b, const float *rate, const float *skip, const float *dt_bias, const float *state, const int32_t *lengths,
+                            void *y, float *last, float *marks, float *workspace, void *stream);
+/* dy, d_last (NULL: zero): gradients of y and last.  dx, d_dt, d_write, d_read, d_rate, d_skip, d_dt_bias, d_state: of the inputs of those names, contiguous, of
+ * their types and shapes; d_skip, d_dt_bias and d_state may be NULL: not wanted. */
+int bmtk_selective_scan_bwd(int64_t n_steps, int64_t batch, int32_t dim, int32_t groups, int32_t n_states, int32_t dtype, int32_t dt_dtype, int32_t softplus, const void *x,
+                            int64_t x_t, int64_t x_b, const void *dt, int64_t dt_t, int64_t dt_b, const void *write, int64_t write_t, int64_t write_b, const void *read,
+                            int64_t read_t, int64_t read_b, const float *rate, const float *skip, const float *dt_bias, const float *marks, const int32_t *lengths,
+                            const void *dy, int64_t dy_t, int64_t dy_b, const float *d_last, void *dx, void *d_dt, void *d_write, void *d_read, float *d_rate, float *d_skip,
+                            float *d_dt_bias, float *d_state, float *workspace, void *stream);
 
 /* ---------------------------------------------------------------------------
  * Three measurements the kernels' design rests on, kept in the library so that they can be repeated
