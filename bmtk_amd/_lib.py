@@ -147,6 +147,9 @@ SIGNATURES = {
     "bmtk_selective_scan_fwd": (c_int32, [c_int64, c_int64] + [c_int32] * 6 + [c_void_p, c_int64, c_int64] * 4 + [c_void_p] * 10),
     "bmtk_selective_scan_bwd": (c_int32, [c_int64, c_int64] + [c_int32] * 6 + [c_void_p, c_int64, c_int64] * 4 + [c_void_p] * 5 + [c_void_p, c_int64, c_int64] +
                                 [c_void_p] * 11),
+    "bmtk_projected_logprobs_workspace_bytes": (c_int64, [c_int64] + [c_int32] * 3 + [c_void_p, c_int64] * 2 + [c_int32]),
+    "bmtk_projected_logprobs_fwd": (c_int32, [c_int64] + [c_int32] * 3 + [c_void_p, c_int64] * 2 + [c_void_p, c_int64] + [c_void_p] * 6),
+    "bmtk_projected_logprobs_bwd": (c_int32, [c_int64] + [c_int32] * 3 + [c_void_p, c_int64] * 2 + [c_void_p, c_int64] + [c_void_p] * 7),
     "bmtk_rate_mse": (c_int32, [c_void_p, c_int64, c_int32, c_int64, c_void_p, c_int64] + [c_void_p] * 5),
 }
 

@@ -1,0 +1,919 @@
+// Log probabilities of tokens under the softmax of x @ weight^T, and their gradients by x and weight, without the logits in memory.
+//
+// Forward: tiles of logits are made on the matrix cores and reduced where they are, to each row's maximum and sum over the tile's vocabulary;
+// tiles are joined by a second kernel.  Backward: with p = e^logit / sum, G = p - delta, dx = -d_logp G weight and d_weight = -(G^T (d_logp x)): the logits are
+// made again, a piece of the vocabulary at a time, G of the piece is written in 16 bits, and two more products read it.  All of that is one kernel,
+// D[i][j] = sum_k A[i][k] B[j][k], whose operands lie in memory with k contiguous or with i (j) contiguous.
+//
+// fp32 operands are taken as three bf16 parts each (8 bits of mantissa a part, 24 in all), whose six largest products are added up: what is left out is below 2^-24
+// of a term.
+#include <type_traits>
+
+#include "readout.hpp"
+
+namespace bmtk {
+namespace {
+
+constexpr int kTile = 32;          // of a matrix instruction
+constexpr int kDepth = 64;         // k of a step: 128 bytes a row
+constexpr float kLog2e = 1.44269504f;
+
+typedef float Acc __attribute__((ext_vector_type(16)));
+typedef float Acc4 __attribute__((ext_vector_type(4)));
+template <typename E>
+struct Vec;
+template <>
+struct Vec<bf16> {
+    typedef __bf16 V8 __attribute__((ext_vector_type(8)));
+    typedef __bf16 V4 __attribute__((ext_vector_type(4)));
+    static __device__ __forceinline__ Acc mfma(V8 a, V8 b, Acc c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ Acc4 mfma16(V8 a, V8 b, Acc4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+};
+template <>
+struct Vec<f16> {
+    typedef _Float16 V8 __attribute__((ext_vector_type(8)));
+    typedef _Float16 V4 __attribute__((ext_vector_type(4)));
+    static __device__ __forceinline__ Acc mfma(V8 a, V8 b, Acc c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ Acc4 mfma16(V8 a, V8 b, Acc4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+};
+
+// three bf16 parts of v; of what is not finite the first is it (so that its products are not either), and a number that rounds to infinity is cut
+__device__ __forceinline__ void split(float v, bf16 (&p)[3])
+{
+    p[0] = (bf16)v;
+    if (fabsf((float)p[0]) == INFINITY) {
+        const uint16_t top = (uint16_t)(__float_as_uint(v) >> 16);
+        __builtin_memcpy(&p[0], &top, 2);
+    }
+    const float r = v - (float)p[0];
+    const bool finite = fabsf(v) < INFINITY;
+    p[1] = (bf16)(finite ? r : 0.0f);
+    p[2] = (bf16)(finite ? r - (float)p[1] : 0.0f);
+}
+// of the products of parts, in this order: 0 0, 0 1, 1 0, 1 1, 0 2, 2 0
+__device__ __forceinline__ int part_a(int combination) { return 0x201100 >> combination * 4 & 3; }
+__device__ __forceinline__ int part_b(int combination) { return 0x021010 >> combination * 4 & 3; }
+
+// e^(v - m) with m = -inf (nothing yet) as 0.  (The difference first: it is exact where it matters, and a rounded m would be in every term.)
+__device__ __forceinline__ float exp_below(float v, float m) { return __builtin_amdgcn_exp2f((v - (m == -INFINITY ? 0.0f : m)) * kLog2e); }
+
+// maxima and sums of e^(logit - maximum), joined
+__device__ __forceinline__ float2 join(float2 u, float2 v)
+{
+    const float m = fmaxf(u.x, v.x);
+    return make_float2(m, u.y * exp_below(u.x, m) + v.y * exp_below(v.x, m));
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// the product
+
+enum { kStats = 0, kGradient = 1, kSlab = 2, kOut = 3 };
+
+struct Product {
+    const char *a, *b;
+    int64_t a_stride, b_stride, a_part, b_part;   // bytes from row to row, from part to part.  A row is an i (j), or a k where i (j) is contiguous
+    int32_t ni, nj, nk;                           // sizes; nk: rows of an operand that has k rows, beyond which its last one is read again
+    int32_t a_last, b_last;                       // bytes of a row that may be read
+    int32_t steps, combinations;                  // steps of kDepth in k; 1 or 6
+    int32_t tiles_i, tiles_j, slices;             // slices: parts of the steps, each to a slab of its own
+    // kStats, kGradient: i is the vocabulary from first on, j the rows
+    int32_t first, vocab;
+    const int64_t *tokens;
+    int64_t ignore;
+    float2 *stats;                                // [tiles_i of all pieces][rows]: maximum, sum of e^(logit - maximum)
+    float *label;                                 // [rows]: logit of the row's token
+    const float *peak, *total;
+    void *g;                                      // [parts][rows, to a whole tile][piece, to a whole tile]
+    int64_t g_stride, g_part;                     // in numbers
+    float g_scale;
+    // kSlab: [slices][nj][slab_stride]; kOut: [nj][ni] of T
+    float *slab;
+    int64_t slab_stride, slab_size;
+    int32_t add;                                  // to what is in the slab
+    void *out;
+    const float *factor;                          // (one number) kOut: results times this and out_scale
+    float out_scale;
+};
+
+typedef __attribute__((address_space(1))) const uint32_t GlobalWord;
+typedef __attribute__((address_space(3))) uint32_t LdsWord;
+
+// One operand's tile of N rows (i or j) and kDepth k on its way through LDS, 16 bytes a lane straight from memory.
+// K rows of 128 bytes, k contiguous: the 16 bytes c of row r lie at c ^ (r & 7), so that eight rows' same c are in different banks.
+// Otherwise N * 2 bytes of a k: their 32 bytes s lie at s ^ (k & 3), so that four rows' same s are; fragments are transposed as they are read.
+template <typename E, int N, int Waves, bool KRows>
+struct Operand {
+    static constexpr int kBytes = N * kDepth * 2, kLoads = kBytes / 1024 / Waves;
+    static_assert(kLoads >= 1, "a load for every wavefront");
+    typedef typename Vec<E>::V8 V8;
+    typedef typename Vec<E>::V4 V4;
+    uint32_t from[kLoads];   // K rows: of every load, the row's bytes from the tile's first one, and the chunk's; else the column's bytes alone
+    const char *base;        // the tile's first row (K rows), or column
+    int64_t stride, part;
+    int32_t last, nk;
+    __device__ __forceinline__ void start(const char *p, int64_t stride_, int64_t part_, int32_t last_, int32_t row0, int32_t rows, int32_t nk_, int lane, int wave)
+    {
+        stride = stride_, part = part_, last = last_, nk = nk_;
+        if constexpr (!KRows) {
+            base = p + (int64_t)row0 * stride;
+#pragma unroll
+            for (int n = 0; n < kLoads; ++n) {
+                const int row = (wave * kLoads + n) * 8 + lane / 8;
+                from[n] = (uint32_t)(min(row, rows - 1 - row0) * (int32_t)stride);
+            }
+        } else {
+            base = p;
+#pragma unroll
+            for (int n = 0; n < kLoads; ++n) {
+                constexpr int kChunks = N / 8;   // of 16 bytes in a row
+                const int at = (wave * kLoads + n) * 64 + lane, k = at / kChunks, slot = at % kChunks;
+                const int chunk = slot ^ ((k & 3) * 2);
+                from[n] = (uint32_t)min(row0 * 2 + chunk * 16, last - 16);
+            }
+        }
+    }
+    __device__ __forceinline__ void load(char *lds, int32_t step, int which, int lane, int wave) const
+    {
+        const char *p = base + which * part;
+#pragma unroll
+        for (int n = 0; n < kLoads; ++n) {
+            const char *q;
+            if constexpr (!KRows) {
+                const int chunk = (lane & 7) ^ (lane / 8 & 7);
+                q = p + (from[n] + (uint32_t)min(step * (kDepth * 2) + chunk * 16, last - 16));
+            } else {
+                constexpr int kChunks = N / 8;
+                const int k = ((wave * kLoads + n) * 64 + lane) / kChunks;
+                q = p + (int64_t)min(step * kDepth + k, nk - 1) * stride + from[n];
+            }
+            __builtin_amdgcn_global_load_lds((GlobalWord *)q, (LdsWord *)(lds + (wave * kLoads + n) * 1024), 16, 0, 0);
+        }
+    }
+    // the fragment of 32 rows from `row` (a multiple of 32) on, sixteen k from s * 16 on
+    __device__ __forceinline__ V8 fragment(const char *lds, int row, int s, int lane) const
+    {
+        if constexpr (!KRows) {
+            const int r = row + (lane & 31), chunk = (s * 2 + lane / 32) ^ (lane & 7);
+            return *reinterpret_cast<const V8 *>(lds + r * 128 + chunk * 16);
+        } else {
+            // sixteen lanes read four k of sixteen columns, 8 bytes each, and get a column's four k each
+            const int group = lane / 16, l = lane & 15;
+            typedef short S4 __attribute__((ext_vector_type(4)));
+            typedef __attribute__((address_space(3))) S4 *P;
+            union {
+                S4 half[2];
+                V8 v;
+            } r;
+#pragma unroll
+            for (int q = 0; q < 2; ++q) {
+                const int k = s * 16 + (group >> 1) * 8 + q * 4 + l / 4, seg = (row / 16 + (group & 1)) ^ (l / 4);
+                r.half[q] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(lds + k * (N * 2) + seg * 32 + (l & 3) * 8));
+            }
+            return r.v;
+        }
+    }
+};
+
+// The order of tiles: workgroups go round the eight XCDs; each XCD gets neighbouring tiles, in blocks of 8 tiles of j by tiles of i, so that what its
+// compute units read at one time stays in its L2.
+__device__ __forceinline__ void place(int32_t block, int32_t blocks, int32_t tiles_i, int32_t tiles_j, int32_t &ti, int32_t &tj)
+{
+    const int32_t x = block & 7, each = blocks >> 3, rest = blocks & 7;
+    const int32_t id = x * each + min(x, rest) + (block >> 3);
+    constexpr int32_t kBand = 8;
+    const int32_t band = id / (kBand * tiles_i), in_band = id - band * kBand * tiles_i, height = min(kBand, tiles_j - band * kBand);
+    ti = in_band / height;
+    tj = band * kBand + in_band % height;
+}
+
+// W: tiles of 32 each way that a wavefront has; a workgroup is 2 x 2 wavefronts
+template <typename E, typename T, int W, bool AK, bool BK, int Mode>
+__global__ __launch_bounds__(256, W == 4 ? 1 : 2) void product_kernel(Product p)
+{
+    constexpr int N = W * 2 * kTile;
+    typedef Operand<E, N, 4, AK> OpA;
+    typedef Operand<E, N, 4, BK> OpB;
+    constexpr int kStage = OpA::kBytes + OpB::kBytes;
+    __shared__ __align__(1024) char lds[2 * kStage];
+    const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), wi = wave >> 1, wj = wave & 1;
+    const int32_t tiles = p.tiles_i * p.tiles_j, slice = blockIdx.x / tiles;
+    int32_t ti, tj;
+    place(blockIdx.x - slice * tiles, tiles, p.tiles_i, p.tiles_j, ti, tj);
+    const int32_t i0 = ti * N, j0 = tj * N;
+    const int32_t all = p.steps * p.combinations, s0 = (int32_t)((int64_t)all * slice / p.slices), s1 = (int32_t)((int64_t)all * (slice + 1) / p.slices);
+    OpA a;
+    OpB b;
+    a.start(p.a, p.a_stride, p.a_part, p.a_last, i0, p.ni, p.nk, lane, wave);
+    b.start(p.b, p.b_stride, p.b_part, p.b_last, j0, p.nj, p.nk, lane, wave);
+    Acc acc[W][W];
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+#pragma unroll
+        for (int j = 0; j < W; ++j)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+    const auto fetch = [&](int32_t s, char *to) {
+        int32_t step = s, c = 0;
+        if (p.combinations > 1) step = s / 6, c = s - step * 6;
+        a.load(to, step, part_a(c), lane, wave);
+        b.load(to + OpA::kBytes, step, part_b(c), lane, wave);
+    };
+    typename Vec<E>::V8 fa[2][W], fb[2][W];
+    const auto take = [&](int to, const char *from, int k) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) fa[to][i] = a.fragment(from, (wi * W + i) * kTile, k, lane);
+#pragma unroll
+        for (int j = 0; j < W; ++j) fb[to][j] = b.fragment(from + OpA::kBytes, (wj * W + j) * kTile, k, lane);
+    };
+    const auto multiply = [&](int from) {
+#pragma unroll
+        for (int i = 0; i < W; ++i)
+#pragma unroll
+            for (int j = 0; j < W; ++j) acc[i][j] = Vec<E>::mfma(fa[from][i], fb[from][j], acc[i][j]);
+    };
+    // Of a quarter's products, the next one's fragments are read beside the first eight, a load to LDS goes out beside each.
+    const auto in_turn = [&](bool loads) {
+#pragma unroll
+        for (int n = 0; n < W * W; ++n) {
+            if (n < 2 * W * (AK ? 2 : 1)) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
+            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+            if (loads) __builtin_amdgcn_sched_group_barrier(0x020, (OpA::kLoads + OpB::kLoads) / (W * W), 0);
+        }
+    };
+    // Two stages in LDS.  Before the last quarter of a step's products the next step's tile is waited for, and the one after it is asked for into the
+    // stage that nobody reads any more: it has the time of a whole step's products to come.
+    if (s0 < s1) {
+        fetch(s0, lds);
+        if (s0 + 1 < s1) fetch(s0 + 1, lds + kStage);
+        // (the first stage's loads came first, and loads to LDS return in order)
+        if (s0 + 1 < s1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(OpA::kLoads + OpB::kLoads) : "memory");
+        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        take(0, lds, 0);
+        for (int32_t s = s0; s < s1; ++s) {
+            char *now = lds + ((s - s0) & 1) * kStage, *next = lds + ((s - s0 + 1) & 1) * kStage;
+#pragma unroll
+            for (int k = 0; k < kDepth / 16; ++k) {
+                if (k + 1 < kDepth / 16) {
+                    take((k + 1) & 1, now, k + 1);
+                } else if (s + 1 < s1) {
+                    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
+                    __builtin_amdgcn_s_barrier();
+                    if (s + 2 < s1) fetch(s + 2, now);
+                    take((k + 1) & 1, next, 0);
+                }
+                multiply(k & 1);
+            }
+        }
+    }
+
+    // lane l has column j = l % 32 of a tile and its rows i = 8 (r / 4) + 4 (l / 32) + r % 4
+    const int half = lane / 32;
+    if constexpr (Mode == kStats) {
+        __syncthreads();
+        float2 *joined = reinterpret_cast<float2 *>(lds);   // [2][N]
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+            const int32_t jj = (wj * W + j) * kTile + (lane & 31), row = j0 + jj;
+            float m = -INFINITY;
+#pragma unroll
+            for (int i = 0; i < W; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) {
+                    const int32_t v = i0 + (wi * W + i) * kTile + 8 * (r / 4) + 4 * half + r % 4;
+                    if (v >= p.ni) acc[i][j][r] = -INFINITY;
+                    m = fmaxf(m, acc[i][j][r]);
+                }
+            m = fmaxf(m, __shfl_xor(m, 32));
+            float s = 0.0f;
+#pragma unroll
+            for (int i = 0; i < W; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) s += exp_below(acc[i][j][r], m);
+            s += __shfl_xor(s, 32);
+            if (half == 0) joined[wi * N + jj] = make_float2(m, s);
+            // the token's logit, where it is in this tile
+            const int64_t token = row < p.nj ? p.tokens[row] : -1;
+            const int64_t at = token - p.first - i0 - wi * W * kTile;
+            const bool here = token >= 0 && token < p.vocab && at >= 0 && at < W * kTile && (int)(at >> 2 & 1) == half;
+            if (__ballot(here)) {
+#pragma unroll
+                for (int i = 0; i < W; ++i)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r)
+                        if (here && at == i * kTile + 8 * (r / 4) + 4 * half + r % 4) p.label[row] = acc[i][j][r];
+            }
+        }
+        __syncthreads();
+        for (int jj = threadIdx.x; jj < N; jj += 256) {
+            if (j0 + jj >= p.nj) continue;
+            p.stats[(int64_t)ti * p.nj + j0 + jj] = join(joined[jj], joined[N + jj]);
+        }
+    } else if constexpr (Mode == kGradient) {
+        typedef typename Vec<E>::V4 V4;
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+            const int32_t row = j0 + (wj * W + j) * kTile + (lane & 31);
+            const bool there = row < p.nj;
+            const int64_t token = there ? p.tokens[row] : p.ignore;
+            const float peak = there ? p.peak[row] : 0.0f, total = there ? p.total[row] : 1.0f;
+            const bool none = !there || token == p.ignore || peak == -INFINITY;
+            const float inverse = p.g_scale / total;
+            E *to = static_cast<E *>(p.g) + row * p.g_stride + i0 + wi * W * kTile;
+            const int64_t at = token - p.first - i0 - wi * W * kTile;
+#pragma unroll
+            for (int i = 0; i < W; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    float v[4];
+#pragma unroll
+                    for (int r = 0; r < 4; ++r) {
+                        const int in = i * kTile + 8 * q + 4 * half + r;
+                        const float e = __builtin_amdgcn_exp2f((acc[i][j][q * 4 + r] - peak) * kLog2e);
+                        v[r] = fmaf(e, inverse, at == in ? -p.g_scale : 0.0f);
+                        if (none || i0 + wi * W * kTile + in >= p.ni) v[r] = 0.0f;
+                    }
+                    if constexpr (std::is_same<T, float>::value) {
+                        V4 parts[3];
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            bf16 s[3];
+                            split(v[r], s);
+#pragma unroll
+                            for (int k = 0; k < 3; ++k) parts[k][r] = s[k];
+                        }
+#pragma unroll
+                        for (int k = 0; k < 3; ++k) *reinterpret_cast<V4 *>(to + k * p.g_part + i * kTile + 8 * q + 4 * half) = parts[k];
+                    } else {
+                        V4 w;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) w[r] = (E)v[r];
+                        *reinterpret_cast<V4 *>(to + i * kTile + 8 * q + 4 * half) = w;
+                    }
+                }
+        }
+    } else {
+        const float scale = Mode == kOut ? p.out_scale * (p.factor ? *p.factor : 1.0f) : 1.0f;
+#pragma unroll
+        for (int j = 0; j < W; ++j) {
+            const int32_t row = j0 + (wj * W + j) * kTile + (lane & 31);
+            if (row >= p.nj) continue;
+#pragma unroll
+            for (int i = 0; i < W; ++i)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int32_t col = i0 + (wi * W + i) * kTile + 8 * q + 4 * half;
+                    if (col >= p.ni) continue;
+                    if constexpr (Mode == kSlab) {   // (rows of a slab are whole fours)
+                        Acc4 *to = reinterpret_cast<Acc4 *>(p.slab + slice * p.slab_size + row * p.slab_stride + col);
+                        Acc4 v;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) v[r] = acc[i][j][q * 4 + r];
+                        *to = p.add ? *to + v : v;
+                    } else {
+                        T *to = static_cast<T *>(p.out) + (int64_t)row * p.ni + col;
+#pragma unroll
+                        for (int r = 0; r < 4; ++r)
+                            if (col + r < p.ni) to[r] = (T)(acc[i][j][q * 4 + r] * scale);
+                    }
+                }
+        }
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// what goes before and after
+
+// Rows of n numbers, `width` (n or more, with zeros) apart, of T or as the three parts of float; with `by`, times by[row], and rows that have no token are 0
+template <typename T, typename E>
+__global__ __launch_bounds__(256) void lay_kernel(const T *from, int64_t stride, int64_t rows, int32_t n, int32_t width, int64_t padded_rows, E *to, const float *by)
+{
+    const int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x, row = k / width;
+    const int32_t c = (int32_t)(k - row * width);
+    if (row >= padded_rows) return;
+    float v = 0.0f;
+    if (row < rows && c < n) {
+        v = (float)from[row * stride + c];
+        if (by) {
+            const float f = by[row];
+            v = f == 0.0f ? 0.0f : v * f;
+        }
+    }
+    if constexpr (std::is_same<T, float>::value) {
+        bf16 s[3];
+        split(v, s);
+#pragma unroll
+        for (int i = 0; i < 3; ++i) to[i * padded_rows * width + k] = s[i];
+    } else {
+        to[k] = (E)v;
+    }
+}
+
+// weights[row] = d_logp over a power of two that leaves the largest at 1 to 2 (for fp16; else itself), 0 for rows without a token, NaN for tokens outside
+// the vocabulary; *factor: that power of two
+__global__ __launch_bounds__(1024) void weigh_kernel(const float *d_logp, const int64_t *tokens, int64_t ignore, int64_t rows, int32_t vocab, int32_t normal, float *weights,
+                                                     float *factor)
+{
+    __shared__ float most[16];
+    float c = 1.0f;
+    if (normal) {
+        float m = 0.0f;
+        for (int64_t r = threadIdx.x; r < rows; r += 1024)
+            if (tokens[r] != ignore && fabsf(d_logp[r]) < INFINITY) m = fmaxf(m, fabsf(d_logp[r]));
+#pragma unroll
+        for (int k = 32; k; k >>= 1) m = fmaxf(m, __shfl_xor(m, k));
+        if (lane_id() == 0) most[threadIdx.x / kWave] = m;
+        __syncthreads();
+        m = 0.0f;
+        for (int k = 0; k < 16; ++k) m = fmaxf(m, most[k]);
+        // (the exponent alone; powers of two from 2^-120 to 2^120, so that neither it nor its inverse is lost)
+        const int e = m > 0.0f ? min(max((int)(__float_as_uint(m) >> 23) - 127, -120), 120) : 0;
+        c = __uint_as_float((uint32_t)(e + 127) << 23);
+    }
+    if (threadIdx.x == 0) *factor = c;
+    for (int64_t r = threadIdx.x; r < rows; r += 1024) {
+        const int64_t token = tokens[r];
+        weights[r] = token == ignore ? 0.0f : token < 0 || token >= vocab ? NAN : d_logp[r] / c;
+    }
+}
+
+// each row's tiles joined: a workgroup takes 64 rows, each of its 16 wavefronts every sixteenth tile
+__global__ __launch_bounds__(1024) void stats_join_kernel(const float2 *stats, int32_t tiles, int32_t rows, const float *label, const int64_t *tokens, int64_t ignore, int32_t vocab,
+                                                          float *logp, float *lse, float *peak, float *total)
+{
+    __shared__ float2 parts[16][64];
+    const int wave = threadIdx.x / kWave, lane = lane_id();
+    const int32_t row = blockIdx.x * 64 + lane;
+    float2 sum = make_float2(-INFINITY, 0.0f);
+    if (row < rows) {
+        for (int k = wave; k < tiles; k += 16 * 4) {
+            float2 q[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) q[i] = stats[(int64_t)min(k + 16 * i, tiles - 1) * rows + row];
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (k + 16 * i < tiles) sum = join(sum, q[i]);
+        }
+    }
+    parts[wave][lane] = sum;
+    __syncthreads();
+    if (wave != 0 || row >= rows) return;
+    for (int k = 1; k < 16; ++k) sum = join(sum, parts[k][lane]);
+    const float m = sum.x, s = sum.y;
+    const float log_total = logf(s);
+    const float l = m == -INFINITY && s == 0.0f ? -INFINITY : m + log_total;
+    const int64_t token = tokens[row];
+    peak[row] = m;
+    total[row] = s;
+    lse[row] = m == INFINITY ? NAN : l;
+    logp[row] = token == ignore ? 0.0f : token < 0 || token >= vocab || m == INFINITY ? NAN : l == -INFINITY ? -INFINITY : (label[row] - m) - log_total;
+}
+
+// results from their slabs: rows of `width` numbers, n of them there
+template <typename T>
+__global__ __launch_bounds__(256) void slab_join_kernel(const float *slab, int32_t slabs, int64_t slab_size, int64_t rows, int32_t n, int32_t width, const float *by, const float *factor,
+                                                        float scale, T *out)
+{
+    const int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x, row = k / (width / 4);
+    const int32_t c = (int32_t)(k - row * (width / 4)) * 4;
+    if (row >= rows || c >= n) return;
+    Acc4 v = *reinterpret_cast<const Acc4 *>(slab + row * width + c);
+    for (int i = 1; i < slabs; ++i) v += *reinterpret_cast<const Acc4 *>(slab + i * slab_size + row * width + c);
+    const float w = by ? by[row] : 1.0f, f = scale * (factor ? *factor : 1.0f) * w;
+#pragma unroll
+    for (int r = 0; r < 4; ++r)
+        if (c + r < n) out[row * n + c + r] = (T)(w == 0.0f ? 0.0f : v[r] * f);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// few rows: a wavefront takes 32 rows of the weights straight from memory into matrix instructions of 16 x 16, against J times 16 rows of x from the
+// caches.  Bound by the weights' bytes.
+
+template <typename T>
+struct Loose8 {
+    typedef uint32_t Words __attribute__((ext_vector_type(4)));
+    typedef Words Loose __attribute__((aligned(2)));
+    union {
+        Words w[sizeof(T) / 2];
+        T v[8];
+    };
+    __device__ __forceinline__ Loose8() {}
+    __device__ __forceinline__ void load(const T *p)
+    {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = reinterpret_cast<const Loose *>(p)[i];
+    }
+    __device__ __forceinline__ void load_some(const T *p, int n)   // n of them; 0 for the others
+    {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : (T)0.0f;
+    }
+};
+
+struct Few {
+    const void *x, *weight;
+    const int64_t *tokens;
+    int64_t x_stride, w_stride;   // in numbers
+    int32_t rows, vocab, dim;
+    float2 *stats;
+    float *label;
+};
+
+template <typename T, typename E, int J>
+__global__ __launch_bounds__(256) void few_rows_kernel(Few a)
+{
+    constexpr bool kParts = std::is_same<T, float>::value;
+    typedef typename Vec<E>::V8 V8;
+    __shared__ float2 parts[4][J * 16];
+    const int lane = lane_id(), wave = threadIdx.x / kWave, r16 = lane & 15, quarter = lane >> 4;
+    const int32_t v0 = (blockIdx.x * 4 + wave) * 32;
+    const T *w_row[2], *x_row[J];
+#pragma unroll
+    for (int i = 0; i < 2; ++i) w_row[i] = static_cast<const T *>(a.weight) + (int64_t)min(v0 + i * 16 + r16, a.vocab - 1) * a.w_stride + quarter * 8;
+#pragma unroll
+    for (int j = 0; j < J; ++j) x_row[j] = static_cast<const T *>(a.x) + (int64_t)min(j * 16 + r16, a.rows - 1) * a.x_stride + quarter * 8;
+    Acc4 acc[2][J];
+#pragma unroll
+    for (int i = 0; i < 2; ++i)
+#pragma unroll
+        for (int j = 0; j < J; ++j) acc[i][j] = Acc4{0.0f, 0.0f, 0.0f, 0.0f};
+    const auto multiply = [&](const Loose8<T> (&w)[2], const Loose8<T> (&x)[J]) {
+        if constexpr (kParts) {
+            V8 wp[2][3], xp[J][3];
+            const auto parts_of = [&](const Loose8<T> &from, V8 (&to)[3]) {
+#pragma unroll
+                for (int k = 0; k < 8; ++k) {
+                    bf16 s[3];
+                    split(from.v[k], s);
+#pragma unroll
+                    for (int i = 0; i < 3; ++i) to[i][k] = s[i];
+                }
+            };
+#pragma unroll
+            for (int i = 0; i < 2; ++i) parts_of(w[i], wp[i]);
+#pragma unroll
+            for (int j = 0; j < J; ++j) parts_of(x[j], xp[j]);
+            constexpr int pa[6] = {0, 0, 1, 1, 0, 2}, pb[6] = {0, 1, 0, 1, 2, 0};
+#pragma unroll
+            for (int c = 0; c < 6; ++c)
+#pragma unroll
+                for (int i = 0; i < 2; ++i)
+#pragma unroll
+                    for (int j = 0; j < J; ++j) acc[i][j] = Vec<E>::mfma16(wp[i][pa[c]], xp[j][pb[c]], acc[i][j]);
+        } else {
+            V8 wv[2], xv[J];
+#pragma unroll
+            for (int i = 0; i < 2; ++i) __builtin_memcpy(&wv[i], &w[i], 16);
+#pragma unroll
+            for (int j = 0; j < J; ++j) __builtin_memcpy(&xv[j], &x[j], 16);
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < J; ++j) acc[i][j] = Vec<E>::mfma16(wv[i], xv[j], acc[i][j]);
+        }
+    };
+    constexpr int kAhead = kParts ? 2 : 4;   // steps of 32 k that are asked for at once
+    const int32_t whole = a.dim / 32;
+    int32_t k = 0;
+    for (; k + kAhead <= whole; k += kAhead) {
+        Loose8<T> w[kAhead][2], x[kAhead][J];
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i) w[u][i].load(w_row[i] + (k + u) * 32);
+#pragma unroll
+            for (int j = 0; j < J; ++j) x[u][j].load(x_row[j] + (k + u) * 32);
+        }
+#pragma unroll
+        for (int u = 0; u < kAhead; ++u) multiply(w[u], x[u]);
+    }
+    for (; k * 32 < a.dim; ++k) {
+        Loose8<T> w[2], x[J];
+        const int n = a.dim - k * 32 - quarter * 8;
+#pragma unroll
+        for (int i = 0; i < 2; ++i) w[i].load_some(w_row[i] + k * 32, n);
+#pragma unroll
+        for (int j = 0; j < J; ++j) x[j].load_some(x_row[j] + k * 32, n);
+        multiply(w, x);
+    }
+    // lane l has column j = l % 16 of a tile and its rows i = 4 (l / 16) + r
+#pragma unroll
+    for (int j = 0; j < J; ++j) {
+        const int32_t row = j * 16 + r16;
+        const int64_t token = row < a.rows ? a.tokens[row] : -1;
+        float m = -INFINITY;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) {
+                const int32_t v = v0 + i * 16 + quarter * 4 + r;
+                if (v >= a.vocab) acc[i][j][r] = -INFINITY;
+                else if (v == token) a.label[row] = acc[i][j][r];
+                m = fmaxf(m, acc[i][j][r]);
+            }
+        m = fmaxf(m, __shfl_xor(m, 16));
+        m = fmaxf(m, __shfl_xor(m, 32));
+        float s = 0.0f;
+#pragma unroll
+        for (int i = 0; i < 2; ++i)
+#pragma unroll
+            for (int r = 0; r < 4; ++r) s += exp_below(acc[i][j][r], m);
+        s += __shfl_xor(s, 16);
+        s += __shfl_xor(s, 32);
+        if (quarter == 0) parts[wave][row] = make_float2(m, s);
+    }
+    __syncthreads();
+    if ((int)threadIdx.x < a.rows) {
+        float2 sum = parts[0][threadIdx.x];
+#pragma unroll
+        for (int w = 1; w < 4; ++w) sum = join(sum, parts[w][threadIdx.x]);
+        a.stats[(int64_t)blockIdx.x * a.rows + threadIdx.x] = sum;
+    }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+
+constexpr int32_t kFewRows = 64;
+constexpr int64_t kPieceBytes = int64_t{512} << 20;   // of G: pieces of the vocabulary are as large as that allows
+
+int64_t up(int64_t n, int64_t to) { return div_up(n, to) * to; }
+
+// tiles of 256 or 128 a workgroup: the large ones need half the reads for a product, and at least as many as three quarters of the chip's compute units
+int32_t tile_of(int64_t ni, int64_t nj, int64_t slices = 1) { return div_up(ni, 256) * div_up(nj, 256) * slices >= 192 ? 256 : 128; }
+
+struct Plan {
+    int32_t parts, combinations, depth;          // depth: dim to whole steps
+    bool copy_x, copy_w;                         // operands that are laid out anew
+    int64_t piece, pieces, g_rows, g_width, out_width;
+    int32_t dx_tile, dx_slices, dw_tile, dw_slices, logit_tile;
+    int64_t x_copy, w_copy, x_weighted, g, dx_slab, dw_slab, stats, label, weights;   // bytes
+    Plan(int64_t rows, int64_t vocab, int32_t dim, int32_t dtype, bool x_fits, bool w_fits, bool backward)
+    {
+        parts = dtype == BMTK_F32 ? 3 : 1;
+        combinations = parts == 3 ? 6 : 1;
+        depth = (int32_t)up(dim, kDepth);
+        copy_x = parts == 3 || !x_fits || dim % kDepth != 0;
+        copy_w = parts == 3 || !w_fits;
+        x_copy = w_copy = x_weighted = g = dx_slab = dw_slab = stats = label = weights = 0;
+        pieces = 1, piece = vocab, g_rows = g_width = out_width = 0;
+        dx_tile = dx_slices = dw_tile = dw_slices = 0;
+        if (!backward) {
+            logit_tile = tile_of(vocab, rows);
+            label = up(rows * 4, 256);
+            if (rows <= kFewRows) {
+                stats = up(div_up(vocab, 128) * rows * 8, 256);
+                return;
+            }
+            stats = up(div_up(vocab, logit_tile) * rows * 8, 256);
+            x_copy = copy_x ? up(parts * rows * depth * 2, 256) : 0;
+            w_copy = copy_w ? up(parts * vocab * depth * 2, 256) : 0;
+            return;
+        }
+        x_copy = copy_x ? up(parts * rows * depth * 2, 256) : 0;
+        w_copy = copy_w ? up(parts * vocab * depth * 2, 256) : 0;
+        g_rows = up(rows, 256);
+        const int64_t most = kPieceBytes / (parts * g_rows * 2) / 256 * 256;
+        piece = most < 256 ? 256 : most;
+        if (piece > vocab) piece = vocab;
+        pieces = div_up(vocab, piece);
+        piece = up(div_up(vocab, pieces), 256);
+        pieces = div_up(vocab, piece);
+        g_width = piece;
+        logit_tile = tile_of(piece < vocab ? piece : vocab, rows);
+        g = up(parts * g_rows * g_width * 2, 256);
+        out_width = up(dim, 8);
+        x_weighted = up(parts * up(rows, kDepth) * out_width * 2, 256);
+        const auto slices_of = [](int64_t ni, int64_t nj, int64_t steps, int32_t &tile, int32_t &slices) {
+            // the sum over k in as many parts as fill the chip, of eight steps at least
+            const auto wanted = [&](int64_t t, int64_t fill) {
+                const int64_t tiles = div_up(ni, t) * div_up(nj, t), s = fill / tiles;
+                const int64_t most = div_up(steps, 8);
+                return s < 1 ? 1 : s > most ? most : s;
+            };
+            const int64_t large = wanted(256, 256);
+            tile = tile_of(ni, nj, large);
+            slices = (int32_t)(tile == 256 ? large : wanted(128, 512));
+        };
+        const int64_t columns = piece < vocab ? piece : vocab;
+        slices_of(dim, rows, div_up(columns, kDepth) * combinations, dx_tile, dx_slices);
+        slices_of(dim, columns, div_up(rows, kDepth) * combinations, dw_tile, dw_slices);
+        dx_slab = up(dx_slices * rows * out_width * 4, 256);
+        dw_slab = dw_slices > 1 ? up(dw_slices * columns * out_width * 4, 256) : 0;
+        weights = up(rows * 4 + 4, 256);
+    }
+    int64_t bytes() const { return x_copy + w_copy + x_weighted + g + dx_slab + dw_slab + stats + label + weights; }
+};
+
+bool sizes_fit(int64_t rows, int64_t vocab, int64_t dim, int32_t dtype)
+{
+    return rows > 0 && vocab > 0 && dim > 0 && dtype >= 0 && dtype <= 2 && rows < (1 << 24) && vocab < (1 << 28) && dim <= 65536;
+}
+
+// whether rows can be read 16 bytes at a time
+bool fits(const void *p, int64_t stride, int32_t dim, int32_t dtype) { return dtype != BMTK_F32 && dim % 8 == 0 && aligned(p, 16) && stride % 8 == 0; }
+
+template <typename T>
+struct Element {
+    typedef T type;
+};
+template <>
+struct Element<float> {
+    typedef bf16 type;
+};
+
+template <typename E, typename T, bool AK, bool BK, int Mode>
+void multiply(Product &p, int32_t tile, hipStream_t s)
+{
+    p.tiles_i = (int32_t)div_up(p.ni, tile);
+    p.tiles_j = (int32_t)div_up(p.nj, tile);
+    const uint32_t blocks = (uint32_t)p.tiles_i * p.tiles_j * p.slices;
+    if (tile == 256) product_kernel<E, T, 4, AK, BK, Mode><<<blocks, 256, 0, s>>>(p);
+    else product_kernel<E, T, 2, AK, BK, Mode><<<blocks, 256, 0, s>>>(p);
+}
+
+template <typename T>
+void lay(const void *from, int64_t stride, int64_t rows, int32_t n, int64_t width, int64_t padded_rows, void *to, const float *by, hipStream_t s)
+{
+    typedef typename Element<T>::type E;
+    lay_kernel<T, E><<<(uint32_t)div_up(padded_rows * width, 256), 256, 0, s>>>(static_cast<const T *>(from), stride, rows, n, (int32_t)width, padded_rows, static_cast<E *>(to), by);
+}
+
+struct Call {
+    int64_t rows, vocab, x_stride, w_stride, ignore;
+    int32_t dim, dtype;
+    const void *x, *weight;
+    const int64_t *tokens;
+    char *ws;
+    hipStream_t stream;
+    char *next(int64_t bytes)
+    {
+        char *p = ws;
+        ws += bytes;
+        return p;
+    }
+};
+
+// logits as a product: i the vocabulary from `first` on, j the rows
+template <typename T>
+Product logits(const Call &c, const Plan &plan, const char *x, const char *w, int64_t first, int64_t count)
+{
+    Product p{};
+    p.a_stride = plan.copy_w ? plan.depth * 2 : c.w_stride * 2;
+    p.a_part = plan.copy_w ? c.vocab * plan.depth * 2 : 0;
+    p.a_last = plan.copy_w ? plan.depth * 2 : c.dim * 2;
+    p.a = w + first * p.a_stride;
+    p.b = x;
+    p.b_stride = plan.copy_x ? plan.depth * 2 : c.x_stride * 2;
+    p.b_part = plan.copy_x ? c.rows * plan.depth * 2 : 0;
+    p.b_last = plan.depth * 2;
+    p.ni = (int32_t)count, p.nj = (int32_t)c.rows, p.nk = 0;
+    p.steps = plan.depth / kDepth, p.combinations = plan.combinations, p.slices = 1;
+    p.first = (int32_t)first, p.vocab = (int32_t)c.vocab, p.tokens = c.tokens, p.ignore = c.ignore;
+    return p;
+}
+
+template <typename T>
+void forward(Call c, float *logp, float *lse, float *peak, float *total)
+{
+    typedef typename Element<T>::type E;
+    const bool x_fits = fits(c.x, c.x_stride, c.dim, c.dtype), w_fits = fits(c.weight, c.w_stride, c.dim, c.dtype);
+    const Plan plan(c.rows, c.vocab, c.dim, c.dtype, x_fits, w_fits, false);
+    float2 *stats = reinterpret_cast<float2 *>(c.next(plan.stats));
+    float *label = reinterpret_cast<float *>(c.next(plan.label));
+    int32_t tiles;
+    if (c.rows <= kFewRows) {
+        Few f{c.x, c.weight, c.tokens, c.x_stride, c.w_stride, (int32_t)c.rows, (int32_t)c.vocab, c.dim, stats, label};
+        tiles = (int32_t)div_up(c.vocab, 128);
+        if (c.rows <= 16) few_rows_kernel<T, E, 1><<<tiles, 256, 0, c.stream>>>(f);
+        else if (c.rows <= 32) few_rows_kernel<T, E, 2><<<tiles, 256, 0, c.stream>>>(f);
+        else few_rows_kernel<T, E, 4><<<tiles, 256, 0, c.stream>>>(f);
+    } else {
+        const char *x = static_cast<const char *>(c.x), *w = static_cast<const char *>(c.weight);
+        if (plan.copy_x) {
+            char *to = c.next(plan.x_copy);
+            lay<T>(c.x, c.x_stride, c.rows, c.dim, plan.depth, c.rows, to, nullptr, c.stream);
+            x = to;
+        }
+        if (plan.copy_w) {
+            char *to = c.next(plan.w_copy);
+            lay<T>(c.weight, c.w_stride, c.vocab, c.dim, plan.depth, c.vocab, to, nullptr, c.stream);
+            w = to;
+        }
+        Product p = logits<T>(c, plan, x, w, 0, c.vocab);
+        p.stats = stats, p.label = label;
+        multiply<E, T, false, false, kStats>(p, plan.logit_tile, c.stream);
+        tiles = p.tiles_i;
+    }
+    stats_join_kernel<<<(uint32_t)div_up(c.rows, 64), 1024, 0, c.stream>>>(stats, tiles, (int32_t)c.rows, label, c.tokens, c.ignore, (int32_t)c.vocab, logp, lse, peak, total);
+}
+
+template <typename T>
+void backward(Call c, const float *peak, const float *total, const float *d_logp, void *dx, void *d_weight)
+{
+    typedef typename Element<T>::type E;
+    const bool x_fits = fits(c.x, c.x_stride, c.dim, c.dtype), w_fits = fits(c.weight, c.w_stride, c.dim, c.dtype);
+    const Plan plan(c.rows, c.vocab, c.dim, c.dtype, x_fits, w_fits, true);
+    const bool half = std::is_same<T, f16>::value;
+    // fp16: p down to 2^-39 keeps bits (its subnormals are not lost in the matrix instructions), and d_logp is divided by a power of two
+    const float g_scale = half ? 32768.0f : 1.0f;
+    float *weights = reinterpret_cast<float *>(c.next(plan.weights)), *factor = weights + c.rows;
+    char *g = c.next(plan.g), *x_weighted = c.next(plan.x_weighted);
+    float *dx_slab = reinterpret_cast<float *>(c.next(plan.dx_slab)), *dw_slab = reinterpret_cast<float *>(c.next(plan.dw_slab));
+    weigh_kernel<<<1, 1024, 0, c.stream>>>(d_logp, c.tokens, c.ignore, c.rows, (int32_t)c.vocab, half, weights, factor);
+    const char *x = static_cast<const char *>(c.x), *w = static_cast<const char *>(c.weight);
+    if (plan.copy_x) {
+        char *to = c.next(plan.x_copy);
+        lay<T>(c.x, c.x_stride, c.rows, c.dim, plan.depth, c.rows, to, nullptr, c.stream);
+        x = to;
+    }
+    if (plan.copy_w) {
+        char *to = c.next(plan.w_copy);
+        lay<T>(c.weight, c.w_stride, c.vocab, c.dim, plan.depth, c.vocab, to, nullptr, c.stream);
+        w = to;
+    }
+    const int64_t k_rows = up(c.rows, kDepth);
+    lay<T>(c.x, c.x_stride, c.rows, c.dim, plan.out_width, k_rows, x_weighted, weights, c.stream);
+    for (int64_t q = 0; q < plan.pieces; ++q) {
+        const int64_t first = q * plan.piece, count = c.vocab - first < plan.piece ? c.vocab - first : plan.piece;
+        Product p = logits<T>(c, plan, x, w, first, count);
+        p.peak = peak, p.total = total, p.g = g, p.g_stride = plan.g_width, p.g_part = plan.g_rows * plan.g_width, p.g_scale = g_scale;
+        multiply<E, T, false, false, kGradient>(p, plan.logit_tile, c.stream);
+
+        // dx: i a channel, j a row, k the vocabulary
+        Product d{};
+        d.a = p.a, d.a_stride = p.a_stride, d.a_part = p.a_part, d.a_last = p.a_last;
+        d.b = g, d.b_stride = plan.g_width * 2, d.b_part = p.g_part * 2, d.b_last = (int32_t)(plan.g_width * 2);
+        d.ni = c.dim, d.nj = (int32_t)c.rows, d.nk = (int32_t)count;
+        d.steps = (int32_t)div_up(count, kDepth), d.combinations = plan.combinations, d.slices = plan.dx_slices;
+        d.slab = dx_slab, d.slab_stride = plan.out_width, d.slab_size = c.rows * plan.out_width, d.add = q > 0;
+        multiply<E, T, true, false, kSlab>(d, plan.dx_tile, c.stream);
+
+        // d_weight: i a channel, j the vocabulary, k a row
+        Product e{};
+        e.a = x_weighted, e.a_stride = plan.out_width * 2, e.a_part = k_rows * plan.out_width * 2, e.a_last = (int32_t)(plan.out_width * 2);
+        e.b = g, e.b_stride = plan.g_width * 2, e.b_part = p.g_part * 2, e.b_last = (int32_t)(plan.g_width * 2);
+        e.ni = c.dim, e.nj = (int32_t)count, e.nk = (int32_t)k_rows;
+        e.steps = (int32_t)(k_rows / kDepth), e.combinations = plan.combinations, e.slices = plan.dw_slices;
+        T *out = static_cast<T *>(d_weight) + first * c.dim;
+        e.out = out, e.factor = factor, e.out_scale = -1.0f / g_scale;
+        e.slab = dw_slab, e.slab_stride = plan.out_width, e.slab_size = count * plan.out_width;
+        if (plan.dw_slices == 1) {
+            multiply<E, T, true, true, kOut>(e, plan.dw_tile, c.stream);
+        } else {
+            multiply<E, T, true, true, kSlab>(e, plan.dw_tile, c.stream);
+            slab_join_kernel<T><<<(uint32_t)div_up(count * (plan.out_width / 4), 256), 256, 0, c.stream>>>(dw_slab, plan.dw_slices, e.slab_size, count, c.dim, (int32_t)plan.out_width, nullptr,
+                                                                                                         factor, e.out_scale, out);
+        }
+    }
+    slab_join_kernel<T><<<(uint32_t)div_up(c.rows * (plan.out_width / 4), 256), 256, 0, c.stream>>>(dx_slab, plan.dx_slices, c.rows * plan.out_width, c.rows, c.dim, (int32_t)plan.out_width,
+                                                                                                  weights, factor, -1.0f / g_scale, static_cast<T *>(dx));
+}
+
+int check(const char *name, const Call &c)
+{
+    BMTK_REQUIRE(c.rows > 0 && c.vocab > 0 && c.dim > 0, "%s: sizes must be positive", name);
+    BMTK_REQUIRE(c.dtype >= 0 && c.dtype <= 2, "%s: unknown type %d", name, c.dtype);
+    BMTK_REQUIRE(c.rows < (1 << 24), "%s: rows must be below 2^24", name);
+    BMTK_REQUIRE(c.vocab < (1 << 28), "%s: vocab must be below 2^28", name);
+    BMTK_REQUIRE(c.dim <= 65536, "%s: up to 65,536 channels", name);
+    // (offsets within a tile of 256 rows and launches of one dimension are in 32 bits)
+    BMTK_REQUIRE(c.x_stride >= 0 && c.w_stride >= 0 && (c.x_stride < (1 << 21) || c.rows <= 1) && (c.w_stride < (1 << 21) || c.vocab <= 1), "%s: rows further apart than 2^21 numbers", name);
+    BMTK_REQUIRE(up(c.vocab, 256) * up(c.dim, 64) < (int64_t{1} << 39) && up(c.rows, 256) * up(c.dim, 64) < (int64_t{1} << 39), "%s: too many numbers for a launch", name);
+    BMTK_REQUIRE(c.ws, "%s: needs a workspace", name);
+    return 0;
+}
+
+}  // namespace
+}  // namespace bmtk
+
+using namespace bmtk;
+
+extern "C" int64_t bmtk_projected_logprobs_workspace_bytes(int64_t rows, int32_t vocab, int32_t dim, int32_t dtype, const void *x, int64_t x_stride, const void *weight,
+                                                           int64_t weight_stride, int32_t backward)
+{
+    if (!sizes_fit(rows, vocab, dim, dtype)) return 0;
+    return Plan(rows, vocab, dim, dtype, fits(x, x_stride, dim, dtype), fits(weight, weight_stride, dim, dtype), backward != 0).bytes();
+}
+
+extern "C" int bmtk_projected_logprobs_fwd(int64_t rows, int32_t vocab, int32_t dim, int32_t dtype, const void *x, int64_t x_stride, const void *weight, int64_t weight_stride,
+                                           const int64_t *tokens, int64_t ignore, float *logp, float *lse, float *peak, float *total, void *workspace, void *stream)
+{
+    BMTK_REQUIRE(x && weight && tokens && logp && lse && peak && total, "projected_logprobs_fwd: null pointer");
+    const Call c{rows, vocab, x_stride, weight_stride, ignore, dim, dtype, x, weight, tokens, static_cast<char *>(workspace), static_cast<hipStream_t>(stream)};
+    if (const int failed = check("projected_logprobs_fwd", c)) return failed;
+    BMTK_BY_TYPE(dtype, T, { forward<T>(c, logp, lse, peak, total); });
+    BMTK_CHECK_LAUNCH("projected_logprobs_fwd");
+    return 0;
+}
+
+extern "C" int bmtk_projected_logprobs_bwd(int64_t rows, int32_t vocab, int32_t dim, int32_t dtype, const void *x, int64_t x_stride, const void *weight, int64_t weight_stride,
+                                           const int64_t *tokens, int64_t ignore, const float *peak, const float *total, const float *d_logp, void *dx, void *d_weight, void *workspace,
+                                           void *stream)
+{
+    BMTK_REQUIRE(x && weight && tokens && peak && total && d_logp && dx && d_weight, "projected_logprobs_bwd: null pointer");
+    const Call c{rows, vocab, x_stride, weight_stride, ignore, dim, dtype, x, weight, tokens, static_cast<char *>(workspace), static_cast<hipStream_t>(stream)};
+    if (const int failed = check("projected_logprobs_bwd", c)) return failed;
+    BMTK_BY_TYPE(dtype, T, { backward<T>(c, peak, total, d_logp, dx, d_weight); });
+    BMTK_CHECK_LAUNCH("projected_logprobs_bwd");
+    return 0;
+}

@@ -540,3 +540,79 @@ def _overlap(a, b):
     first = [t.data_ptr() for t in (a, b)]
     end = [p + ((t.shape[0] - 1) * t.stride(0) + t.shape[1]) * t.element_size() for p, t in zip(first, (a, b))]
     return first[0] < end[1] and first[1] < end[0]
+
+
+# ---------------------------------------------------------------------------------------------------------------------
+
+class ProjectedLogProbs(NamedTuple):
+    """What ``projected_logprobs`` returns, float32 and of the shape of the tokens.  peak and total: the row's largest logit, and the sum of e^(logit - peak)."""
+    logp: torch.Tensor
+    lse: torch.Tensor
+    peak: torch.Tensor
+    total: torch.Tensor
+
+
+def _projected(x, weight, tokens):
+    """x as rows, (rows, vocabulary, channels, what both directions point to)."""
+    _given(x, "x")
+    _given(weight, "weight", x.dtype)
+    _given(tokens, "tokens", torch.int64)
+    if x.dim() < 1 or x.shape[-1] == 0:
+        raise ValueError("x must be [..., channels]")
+    dim = x.shape[-1]
+    if weight.dim() != 2 or weight.shape[0] == 0 or weight.shape[1] != dim:
+        raise ValueError("weight must be [vocabulary, {}], got {}".format(dim, tuple(weight.shape)))
+    if tuple(tokens.shape) != tuple(x.shape[:-1]):
+        raise ValueError("tokens must be {}, got {}".format(tuple(x.shape[:-1]), tuple(tokens.shape)))
+    flat = x if x.dim() == 2 else x.reshape(-1, dim)
+    strides = []
+    for t, name in ((flat, "x"), (weight, "weight")):
+        if dim > 1 and t.stride(1) != 1:
+            raise ValueError("the channels of {} must lie next to one another".format(name))
+        strides.append(t.stride(0) if t.shape[0] > 1 else dim)
+    rows, vocab = flat.shape[0], weight.shape[0]
+    return flat, rows, vocab, dim, (flat.data_ptr(), strides[0], weight.data_ptr(), strides[1])
+
+
+def projected_logprobs(x, weight, tokens, ignore=-100):
+    """Log probability of each row's token under the softmax of ``x @ weight.T``, without the logits in memory: ``ProjectedLogProbs``.
+
+    x       [..., channels], the channels of a row next to one another
+    weight  [vocabulary, channels], of the type of ``x``: a row for each token, the channels next to one another
+    tokens  int64 [...]; ``ignore`` where a row has none (padding): its logp is 0.  A token outside the vocabulary has logp NaN
+    Rows whose logits hold NaN or +inf have lse and logp NaN.  float32 arguments are multiplied in parts of 16 bits that hold all their bits; what is not finite in
+    them makes the rows that meet it NaN."""
+    r = _native.projected_logprobs(x, weight, tokens, ignore)
+    if r is not None:
+        return ProjectedLogProbs(*r)
+    flat, rows, vocab, dim, at = _projected(x, weight, tokens)
+    r = ProjectedLogProbs(*(torch.empty(tokens.shape, dtype=torch.float32, device=x.device) for _ in range(4)))
+    if rows:
+        lib, code = _lib.load(), _CODE[x.dtype]
+        tokens = tokens.contiguous()
+        ws = _Workspace(lib.bmtk_projected_logprobs_workspace_bytes(rows, vocab, dim, code, *at, 0), x.device)
+        _lib.check(lib.bmtk_projected_logprobs_fwd(rows, vocab, dim, code, *at, tokens.data_ptr(), ignore, *(t.data_ptr() for t in r), ws.ptr, _stream()))
+    return r
+
+
+def projected_logprobs_bwd(x, weight, tokens, fwd, d_logp, ignore=-100):
+    """(dx, d_weight), of the types and shapes of ``x`` and ``weight``, from the gradient of logp, ``d_logp`` (float32, of the shape of the tokens).
+
+    x, weight, tokens, ignore: as they were; fwd: what ``projected_logprobs`` returned.  Rows without a token have a gradient of 0 and no part in d_weight, whatever
+    they hold.  The logits are made again, in pieces of up to 512 MB of the vocabulary, with p rounded to 16 bits (of float32: in three parts); float16
+    holds no gradient below 6e-8: give it a scaled d_logp, as a mean over many rows needs."""
+    r = _native.projected_logprobs_bwd(x, weight, tokens, fwd.peak, fwd.total, d_logp, ignore)
+    if r is not None:
+        return r
+    flat, rows, vocab, dim, at = _projected(x, weight, tokens)
+    for t, name in ((fwd.peak, "peak"), (fwd.total, "total"), (d_logp, "d_logp")):
+        _contiguous(t, name, torch.float32, tokens.shape)
+    dx = torch.empty(x.shape, dtype=x.dtype, device=x.device)
+    d_weight = (torch.empty if rows else torch.zeros)(vocab, dim, dtype=x.dtype, device=x.device)
+    if rows:
+        lib, code = _lib.load(), _CODE[x.dtype]
+        tokens = tokens.contiguous()
+        ws = _Workspace(lib.bmtk_projected_logprobs_workspace_bytes(rows, vocab, dim, code, *at, 1), x.device)
+        _lib.check(lib.bmtk_projected_logprobs_bwd(rows, vocab, dim, code, *at, tokens.data_ptr(), ignore, fwd.peak.data_ptr(), fwd.total.data_ptr(), d_logp.data_ptr(), dx.data_ptr(),
+                                                   d_weight.data_ptr(), ws.ptr, _stream()))
+    return dx, d_weight

@@ -797,6 +797,21 @@ int bmtk_selective_scan_bwd(int64_t n_steps, int64_t batch, int32_t dim, int32_t
                             const void *dy, int64_t dy_t, int64_t dy_b, const float *d_last, void *dx, void *d_dt, void *d_write, void *d_read, float *d_rate, float *d_skip,
                             float *d_dt_bias, float *d_state, float *workspace, void *stream);
 
+/* Of each of `rows` rows of x (x_stride numbers apart), with logits l[v] = x . weight[v] over `dim` channels: lse = log of the sum of e^l, logp = l[token] - lse (0 where
+ * the token is `ignore`, NaN where it lies outside 0 .. vocab - 1), peak = the largest logit, total = the sum of e^(l - peak).  The logits are not kept.
+ * weight: vocab rows, weight_stride numbers apart.  Rows whose logits hold NaN or +inf have lse and logp NaN.  Sums are in 32 bits; fp32 operands are taken as three
+ * bf16 parts each, six of their products (a row that meets an fp32 operand that is not finite is NaN).
+ * Limits: rows < 2^24, vocab < 2^28, dim up to 65,536, strides below 2^21. */
+int64_t bmtk_projected_logprobs_workspace_bytes(int64_t rows, int32_t vocab, int32_t dim, int32_t dtype, const void *x, int64_t x_stride, const void *weight,
+                                                int64_t weight_stride, int32_t backward);
+int bmtk_projected_logprobs_fwd(int64_t rows, int32_t vocab, int32_t dim, int32_t dtype, const void *x, int64_t x_stride, const void *weight, int64_t weight_stride,
+                                const int64_t *tokens, int64_t ignore, float *logp, float *lse, float *peak, float *total, void *workspace, void *stream);
+/* dx [rows][dim], d_weight [vocab][dim], contiguous and of dtype, from d_logp [rows]; peak and total are the forward pass's.  Rows without a token have dx 0 and no part in
+ * d_weight, whatever they hold.  Logits are made again in pieces of the vocabulary of up to 512 MB. */
+int bmtk_projected_logprobs_bwd(int64_t rows, int32_t vocab, int32_t dim, int32_t dtype, const void *x, int64_t x_stride, const void *weight, int64_t weight_stride,
+                                const int64_t *tokens, int64_t ignore, const float *peak, const float *total, const float *d_logp, void *dx, void *d_weight, void *workspace,
+                                void *stream);
+
 /* ---------------------------------------------------------------------------
  * Three measurements the kernels' design rests on, kept in the library so that they can be repeated
  * (bench.py --kernels lds).  No counterpart in the reference.
