@@ -16,6 +16,7 @@ namespace {
 
 constexpr int kTile = 32;          // of a matrix instruction
 constexpr int kDepth = 64;         // k of a step: 128 bytes a row
+constexpr int kWaitAll = 0x70;     // s_waitcnt of all loads and all LDS operations
 constexpr float kLog2e = 1.44269504f;
 
 typedef float Acc __attribute__((ext_vector_type(16)));
@@ -212,11 +213,13 @@ __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void product_kernel(Product p)
         for (int j = 0; j < W; ++j)
 #pragma unroll
             for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
-    const auto fetch = [&](int32_t s, char *to) {
-        int32_t step = s, c = 0;
-        if (p.combinations > 1) step = s / 6, c = s - step * 6;
-        a.load(to, step, part_a(c), lane, wave);
-        b.load(to + OpA::kBytes, step, part_b(c), lane, wave);
+    int32_t step = s0 / p.combinations, combination = s0 - step * p.combinations;   // of the next tile
+    const auto fetch = [&](char *to) {
+        a.load(to, step, part_a(combination), lane, wave);
+        b.load(to + OpA::kBytes, step, part_b(combination), lane, wave);
+        const bool more = combination + 1 < p.combinations;
+        step = min(more ? step : step + 1, p.steps - 1);   // (behind the last step it is asked for again, for nothing)
+        combination = more ? combination + 1 : 0;
     };
     typename Vec<E>::V8 fa[2][W], fb[2][W];
     const auto take = [&](int to, const char *from, int k) {
@@ -231,40 +234,55 @@ __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void product_kernel(Product p)
 #pragma unroll
             for (int j = 0; j < W; ++j) acc[i][j] = Vec<E>::mfma(fa[from][i], fb[from][j], acc[i][j]);
     };
-    // Of a quarter's products, the next one's fragments are read beside the first eight, a load to LDS goes out beside each.
+    // Of a quarter's products, beside the first half the next one's fragments are read, beside the second the loads to LDS go out.
+    constexpr int kReads = W * (AK ? 2 : 1) + W * (BK ? 2 : 1), kHalf = W * W / 2;
     const auto in_turn = [&](bool loads) {
 #pragma unroll
         for (int n = 0; n < W * W; ++n) {
-            if (n < 2 * W * (AK ? 2 : 1)) __builtin_amdgcn_sched_group_barrier(0x100, 1, 0);
             __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            if (loads) __builtin_amdgcn_sched_group_barrier(0x020, (OpA::kLoads + OpB::kLoads) / (W * W), 0);
+            if (n < kHalf) __builtin_amdgcn_sched_group_barrier(0x100, (kReads + kHalf - 1) / kHalf, 0);
+            else if (loads) __builtin_amdgcn_sched_group_barrier(0x020, (OpA::kLoads + OpB::kLoads) / kHalf, 0);
         }
     };
     // Two stages in LDS.  Before the last quarter of a step's products the next step's tile is waited for, and the one after it is asked for into the
     // stage that nobody reads any more: it has the time of a whole step's products to come.
+    constexpr int kQuarters = kDepth / 16;
     if (s0 < s1) {
-        fetch(s0, lds);
-        if (s0 + 1 < s1) fetch(s0 + 1, lds + kStage);
+        fetch(lds);
+        fetch(lds + kStage);
         // (the first stage's loads came first, and loads to LDS return in order)
-        if (s0 + 1 < s1) asm volatile("s_waitcnt vmcnt(%0)" ::"n"(OpA::kLoads + OpB::kLoads) : "memory");
-        else asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(OpA::kLoads + OpB::kLoads) : "memory");
         __builtin_amdgcn_s_barrier();
         take(0, lds, 0);
-        for (int32_t s = s0; s < s1; ++s) {
+        int32_t s = s0;
+        for (; s + 1 < s1; ++s) {
             char *now = lds + ((s - s0) & 1) * kStage, *next = lds + ((s - s0 + 1) & 1) * kStage;
 #pragma unroll
-            for (int k = 0; k < kDepth / 16; ++k) {
-                if (k + 1 < kDepth / 16) {
-                    take((k + 1) & 1, now, k + 1);
-                } else if (s + 1 < s1) {
-                    asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)" ::: "memory");
-                    __builtin_amdgcn_s_barrier();
-                    if (s + 2 < s1) fetch(s + 2, now);
-                    take((k + 1) & 1, next, 0);
-                }
+            for (int k = 0; k + 1 < kQuarters; ++k) {
+                take((k + 1) & 1, now, k + 1);
                 multiply(k & 1);
+                in_turn(false);
+                __builtin_amdgcn_sched_barrier(0);
             }
+            __builtin_amdgcn_s_waitcnt(kWaitAll);
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            take(0, next, 0);
+            fetch(now);
+            multiply((kQuarters - 1) & 1);
+            in_turn(true);
+            __builtin_amdgcn_sched_barrier(0);
         }
+        const char *now = lds + ((s - s0) & 1) * kStage;
+#pragma unroll
+        for (int k = 0; k < kQuarters; ++k) {
+            if (k + 1 < kQuarters) take((k + 1) & 1, now, k + 1);
+            multiply(k & 1);
+            if (k + 1 < kQuarters) in_turn(false);
+            __builtin_amdgcn_sched_barrier(0);
+        }
+        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
     }
 
     // lane l has column j = l % 32 of a tile and its rows i = 8 (r / 4) + 4 (l / 32) + r % 4
