@@ -16,8 +16,8 @@ namespace {
 
 constexpr int kTile = 32;          // of a matrix instruction
 constexpr int kDepth = 64;         // k of a step: 128 bytes a row
-constexpr int kWaitAll = 0x70;     // s_waitcnt of all loads and all LDS operations
-constexpr float kLog2e = 1.44269504f;
+constexpr int kWaitReads = 0xc07f, kWaitLoads = 0x0f70, kWaitAll = 0x70;   // s_waitcnt of all LDS operations, of all loads, of both
+constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
 
 typedef float Acc __attribute__((ext_vector_type(16)));
 typedef float Acc4 __attribute__((ext_vector_type(4)));
@@ -55,14 +55,43 @@ __device__ __forceinline__ void split(float v, bf16 (&p)[3])
 __device__ __forceinline__ int part_a(int combination) { return 0x201100 >> combination * 4 & 3; }
 __device__ __forceinline__ int part_b(int combination) { return 0x021010 >> combination * 4 & 3; }
 
-// e^(v - m) with m = -inf (nothing yet) as 0.  (The difference first: it is exact where it matters, and a rounded m would be in every term.)
-__device__ __forceinline__ float exp_below(float v, float m) { return __builtin_amdgcn_exp2f((v - (m == -INFINITY ? 0.0f : m)) * kLog2e); }
+// Exponentials are of base 2, against a base that is a number of eighths near the largest logit times log2 e: it is exact, so that 2^(v log2e - base) is rounded
+// in the exponent once, and what log2 e itself is off by is the same in the logit of a token.
+__device__ __forceinline__ float base_of(float m) { return rintf(m * (kLog2e * 8.0f)) * 0.125f; }
+__device__ __forceinline__ float exp_over(float v, float base) { return __builtin_amdgcn_exp2f(fmaf(v, kLog2e, -base)); }
 
-// maxima and sums of e^(logit - maximum), joined
+// bases and sums over them, joined; -inf: nothing yet
 __device__ __forceinline__ float2 join(float2 u, float2 v)
 {
-    const float m = fmaxf(u.x, v.x);
-    return make_float2(m, u.y * exp_below(u.x, m) + v.y * exp_below(v.x, m));
+    const float m = fmaxf(u.x, v.x), from = m == -INFINITY ? 0.0f : m;
+    return make_float2(m, u.y * __builtin_amdgcn_exp2f(u.x - from) + v.y * __builtin_amdgcn_exp2f(v.x - from));
+}
+
+// the order of a stretch of code: beside each of N products their share of R LDS reads and of L loads to LDS
+template <int N, int R, int L, int At>
+__device__ __forceinline__ void beside()
+{
+    if constexpr (At < N) {
+        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
+        constexpr int r = R * (At + 1) / N - R * At / N, l = L * (At + 1) / N - L * At / N;
+        if constexpr (r > 0) __builtin_amdgcn_sched_group_barrier(0x100, r, 0);
+        if constexpr (l > 0) __builtin_amdgcn_sched_group_barrier(0x020, l, 0);
+        beside<N, R, L, At + 1>();
+    }
+}
+
+// four numbers to where they begin anywhere
+template <typename T>
+__device__ __forceinline__ void put4(T *p, const Acc4 &v)
+{
+    typedef uint32_t Words __attribute__((ext_vector_type(sizeof(T))));
+    typedef Words Loose __attribute__((aligned(2)));
+    T q[4];
+#pragma unroll
+    for (int r = 0; r < 4; ++r) q[r] = (T)v[r];
+    Words w;
+    __builtin_memcpy(&w, q, sizeof(w));
+    *reinterpret_cast<Loose *>(p) = w;
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -187,7 +216,8 @@ __device__ __forceinline__ void place(int32_t block, int32_t blocks, int32_t til
     tj = band * kBand + in_band % height;
 }
 
-// W: tiles of 32 each way that a wavefront has; a workgroup is 2 x 2 wavefronts
+// W: tiles of 32 each way that a wavefront has; a workgroup is 2 x 2 wavefronts.  Workgroups take tiles in turn: the next tile's first two stages are on their way
+// while a tile's results are looked after.
 template <typename E, typename T, int W, bool AK, bool BK, int Mode>
 __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void product_kernel(Product p)
 {
@@ -195,25 +225,12 @@ __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void product_kernel(Product p)
     typedef Operand<E, N, 4, AK> OpA;
     typedef Operand<E, N, 4, BK> OpB;
     constexpr int kStage = OpA::kBytes + OpB::kBytes;
-    __shared__ __align__(1024) char lds[2 * kStage];
+    __shared__ __align__(1024) char lds[2 * kStage + (Mode == kStats ? 2 * N * 8 : 0)];
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), wi = wave >> 1, wj = wave & 1;
-    const int32_t tiles = p.tiles_i * p.tiles_j, slice = blockIdx.x / tiles;
-    int32_t ti, tj;
-    place(blockIdx.x - slice * tiles, tiles, p.tiles_i, p.tiles_j, ti, tj);
-    const int32_t i0 = ti * N, j0 = tj * N;
-    const int32_t all = p.steps * p.combinations, s0 = (int32_t)((int64_t)all * slice / p.slices), s1 = (int32_t)((int64_t)all * (slice + 1) / p.slices);
+    const int32_t tiles = p.tiles_i * p.tiles_j, jobs = tiles * p.slices, all = p.steps * p.combinations;
     OpA a;
     OpB b;
-    a.start(p.a, p.a_stride, p.a_part, p.a_last, i0, p.ni, p.nk, lane, wave);
-    b.start(p.b, p.b_stride, p.b_part, p.b_last, j0, p.nj, p.nk, lane, wave);
-    Acc acc[W][W];
-#pragma unroll
-    for (int i = 0; i < W; ++i)
-#pragma unroll
-        for (int j = 0; j < W; ++j)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
-    int32_t step = s0 / p.combinations, combination = s0 - step * p.combinations;   // of the next tile
+    int32_t ti, tj, slice, s0, s1, step, combination;
     const auto fetch = [&](char *to) {
         a.load(to, step, part_a(combination), lane, wave);
         b.load(to + OpA::kBytes, step, part_b(combination), lane, wave);
@@ -221,182 +238,249 @@ __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void product_kernel(Product p)
         step = min(more ? step : step + 1, p.steps - 1);   // (behind the last step it is asked for again, for nothing)
         combination = more ? combination + 1 : 0;
     };
-    typename Vec<E>::V8 fa[2][W], fb[2][W];
-    const auto take = [&](int to, const char *from, int k) {
-#pragma unroll
-        for (int i = 0; i < W; ++i) fa[to][i] = a.fragment(from, (wi * W + i) * kTile, k, lane);
-#pragma unroll
-        for (int j = 0; j < W; ++j) fb[to][j] = b.fragment(from + OpA::kBytes, (wj * W + j) * kTile, k, lane);
+    const auto begin = [&](int32_t job) {
+        slice = job / tiles;
+        place(job - slice * tiles, tiles, p.tiles_i, p.tiles_j, ti, tj);
+        s0 = (int32_t)((int64_t)all * slice / p.slices), s1 = (int32_t)((int64_t)all * (slice + 1) / p.slices);
+        step = s0 / p.combinations, combination = s0 - step * p.combinations;
+        a.start(p.a, p.a_stride, p.a_part, p.a_last, ti * N, p.ni, p.nk, lane, wave);
+        b.start(p.b, p.b_stride, p.b_part, p.b_last, tj * N, p.nj, p.nk, lane, wave);
+        fetch(lds);
+        fetch(lds + kStage);
     };
-    const auto multiply = [&](int from) {
+    Acc acc[W][W];
+    typename Vec<E>::V8 fa[4][W], fb[4][W];
+    const auto take_a = [&](int k, const char *from) {
+#pragma unroll
+        for (int i = 0; i < W; ++i) fa[k][i] = a.fragment(from, (wi * W + i) * kTile, k, lane);
+    };
+    const auto take_b = [&](int k, const char *from) {
+#pragma unroll
+        for (int j = 0; j < W; ++j) fb[k][j] = b.fragment(from + OpA::kBytes, (wj * W + j) * kTile, k, lane);
+    };
+    // products of half a quarter
+    const auto multiply = [&](int k, int h) {
+#pragma unroll
+        for (int i = h * W / 2; i < (h + 1) * W / 2; ++i)
+#pragma unroll
+            for (int j = 0; j < W; ++j) acc[i][j] = Vec<E>::mfma(fa[k][i], fb[k][j], acc[i][j]);
+    };
+    // beside each of `products` products `reads` LDS reads in all, spread evenly, and `loads` loads to LDS in all
+    constexpr int kReadsA = W * (AK ? 2 : 1), kReadsB = W * (BK ? 2 : 1), kLoads = OpA::kLoads + OpB::kLoads, kHalf = W * W / 2;
+    const auto in_turn = [&](auto products, auto reads, auto loads) {
+        constexpr int n = decltype(products)::value, r = decltype(reads)::value, l = decltype(loads)::value;
+        beside<n, r, l, 0>();
+        __builtin_amdgcn_sched_barrier(0);
+    };
+#define BMTK_N(v) std::integral_constant<int, (v)>()
+    // the products of the first two quarters, and the fragments of the others
+    const auto first_half = [&](const char *now) {
+        take_a(1, now);
+        take_b(1, now);
+        multiply(0, 0);
+        in_turn(BMTK_N(kHalf), BMTK_N(kReadsA + kReadsB), BMTK_N(0));
+        take_a(2, now);
+        multiply(0, 1);
+        in_turn(BMTK_N(kHalf / 2), BMTK_N(kReadsA), BMTK_N(0));
+        take_b(2, now);
+        take_a(3, now);
+        multiply(1, 0);
+        in_turn(BMTK_N(kHalf), BMTK_N(kReadsA + kReadsB), BMTK_N(0));
+        take_b(3, now);
+        multiply(1, 1);
+        in_turn(BMTK_N(kHalf / 2), BMTK_N(kReadsB), BMTK_N(0));
+    };
+
+    if ((int32_t)blockIdx.x >= jobs) return;
+    begin(blockIdx.x);
+    for (int32_t job = blockIdx.x; job < jobs; job += gridDim.x) {
+        const int32_t i0 = ti * N, j0 = tj * N, out_slice = slice;
+        // what the results will be asked for, of this lane's column of each tile
+        int64_t token[W];
+        float peak[W], total[W];
+        if constexpr (Mode == kStats || Mode == kGradient) {
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                const int32_t row = min(j0 + (wj * W + j) * kTile + (lane & 31), p.nj - 1);
+                token[j] = p.tokens[row];
+                if constexpr (Mode == kGradient) peak[j] = p.peak[row], total[j] = p.total[row];
+            }
+        }
 #pragma unroll
         for (int i = 0; i < W; ++i)
 #pragma unroll
-            for (int j = 0; j < W; ++j) acc[i][j] = Vec<E>::mfma(fa[from][i], fb[from][j], acc[i][j]);
-    };
-    // Of a quarter's products, beside the first half the next one's fragments are read, beside the second the loads to LDS go out.
-    constexpr int kReads = W * (AK ? 2 : 1) + W * (BK ? 2 : 1), kHalf = W * W / 2;
-    const auto in_turn = [&](bool loads) {
+            for (int j = 0; j < W; ++j)
 #pragma unroll
-        for (int n = 0; n < W * W; ++n) {
-            __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-            if (n < kHalf) __builtin_amdgcn_sched_group_barrier(0x100, (kReads + kHalf - 1) / kHalf, 0);
-            else if (loads) __builtin_amdgcn_sched_group_barrier(0x020, (OpA::kLoads + OpB::kLoads) / kHalf, 0);
-        }
-    };
-    // Two stages in LDS.  Before the last quarter of a step's products the next step's tile is waited for, and the one after it is asked for into the
-    // stage that nobody reads any more: it has the time of a whole step's products to come.
-    constexpr int kQuarters = kDepth / 16;
-    if (s0 < s1) {
-        fetch(lds);
-        fetch(lds + kStage);
-        // (the first stage's loads came first, and loads to LDS return in order)
-        asm volatile("s_waitcnt vmcnt(%0)" ::"n"(OpA::kLoads + OpB::kLoads) : "memory");
+                for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
+        // Two stages in LDS, a step's products in quarters.  A step's fragments are all in registers well before its products are done, so that from the middle of
+        // the third quarter on the tile after the next is asked for into the same stage: it has the time of a step's products to come.
+        static_assert(kDepth == 64, "four quarters");
+        __builtin_amdgcn_s_waitcnt(kWaitLoads);
+        asm volatile("" ::: "memory");
         __builtin_amdgcn_s_barrier();
-        take(0, lds, 0);
+        asm volatile("" ::: "memory");
+        take_a(0, lds);
+        take_b(0, lds);
         int32_t s = s0;
         for (; s + 1 < s1; ++s) {
             char *now = lds + ((s - s0) & 1) * kStage, *next = lds + ((s - s0 + 1) & 1) * kStage;
-#pragma unroll
-            for (int k = 0; k + 1 < kQuarters; ++k) {
-                take((k + 1) & 1, now, k + 1);
-                multiply(k & 1);
-                in_turn(false);
-                __builtin_amdgcn_sched_barrier(0);
-            }
+            first_half(now);
+            multiply(2, 0);
+            in_turn(BMTK_N(kHalf), BMTK_N(0), BMTK_N(0));
             __builtin_amdgcn_s_waitcnt(kWaitAll);
             asm volatile("" ::: "memory");
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
-            take(0, next, 0);
             fetch(now);
-            multiply((kQuarters - 1) & 1);
-            in_turn(true);
-            __builtin_amdgcn_sched_barrier(0);
+            multiply(2, 1);
+            in_turn(BMTK_N(kHalf), BMTK_N(0), BMTK_N(kLoads));
+            take_a(0, next);
+            take_b(0, next);
+            multiply(3, 0);
+            in_turn(BMTK_N(kHalf), BMTK_N(kReadsA + kReadsB), BMTK_N(0));
+            multiply(3, 1);
+            in_turn(BMTK_N(kHalf), BMTK_N(0), BMTK_N(0));
         }
         const char *now = lds + ((s - s0) & 1) * kStage;
-#pragma unroll
-        for (int k = 0; k < kQuarters; ++k) {
-            if (k + 1 < kQuarters) take((k + 1) & 1, now, k + 1);
-            multiply(k & 1);
-            if (k + 1 < kQuarters) in_turn(false);
-            __builtin_amdgcn_sched_barrier(0);
-        }
-        asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
-    }
+        first_half(now);
+        // (what was asked for behind the last step has come, and everybody has read what there was)
+        __builtin_amdgcn_s_waitcnt(kWaitAll);
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
+        if (job + (int32_t)gridDim.x < jobs) begin(job + gridDim.x);
+        multiply(2, 0);
+        multiply(2, 1);
+        multiply(3, 0);
+        multiply(3, 1);
 
-    // lane l has column j = l % 32 of a tile and its rows i = 8 (r / 4) + 4 (l / 32) + r % 4
-    const int half = lane / 32;
-    if constexpr (Mode == kStats) {
-        __syncthreads();
-        float2 *joined = reinterpret_cast<float2 *>(lds);   // [2][N]
+        // lane l has column j = l % 32 of a tile and its rows i = 8 (r / 4) + 4 (l / 32) + r % 4
+        const int half = lane / 32, ii0 = i0 + wi * W * kTile;
+        const bool edge = i0 + N > p.ni;
+        if constexpr (Mode == kStats) {
+            float2 *joined = reinterpret_cast<float2 *>(lds + 2 * kStage);   // [2][N]
 #pragma unroll
-        for (int j = 0; j < W; ++j) {
-            const int32_t jj = (wj * W + j) * kTile + (lane & 31), row = j0 + jj;
-            float m = -INFINITY;
+            for (int j = 0; j < W; ++j) {
+                const int32_t jj = (wj * W + j) * kTile + (lane & 31), row = j0 + jj;
+                if (edge) {
 #pragma unroll
-            for (int i = 0; i < W; ++i)
+                    for (int i = 0; i < W; ++i)
 #pragma unroll
-                for (int r = 0; r < 16; ++r) {
-                    const int32_t v = i0 + (wi * W + i) * kTile + 8 * (r / 4) + 4 * half + r % 4;
-                    if (v >= p.ni) acc[i][j][r] = -INFINITY;
-                    m = fmaxf(m, acc[i][j][r]);
+                        for (int r = 0; r < 16; ++r)
+                            if (ii0 + i * kTile + 8 * (r / 4) + 4 * half + r % 4 >= p.ni) acc[i][j][r] = -INFINITY;
                 }
-            m = fmaxf(m, __shfl_xor(m, 32));
-            float s = 0.0f;
-#pragma unroll
-            for (int i = 0; i < W; ++i)
-#pragma unroll
-                for (int r = 0; r < 16; ++r) s += exp_below(acc[i][j][r], m);
-            s += __shfl_xor(s, 32);
-            if (half == 0) joined[wi * N + jj] = make_float2(m, s);
-            // the token's logit, where it is in this tile
-            const int64_t token = row < p.nj ? p.tokens[row] : -1;
-            const int64_t at = token - p.first - i0 - wi * W * kTile;
-            const bool here = token >= 0 && token < p.vocab && at >= 0 && at < W * kTile && (int)(at >> 2 & 1) == half;
-            if (__ballot(here)) {
+                float m = acc[0][j][0];
 #pragma unroll
                 for (int i = 0; i < W; ++i)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r)
-                        if (here && at == i * kTile + 8 * (r / 4) + 4 * half + r % 4) p.label[row] = acc[i][j][r];
+                    for (int r = 0; r < 16; ++r) m = fmaxf(m, acc[i][j][r]);
+                m = fmaxf(m, __shfl_xor(m, 32));
+                const float base = base_of(m), from = base == -INFINITY ? 0.0f : base;
+                float s4[4] = {0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+                for (int i = 0; i < W; ++i)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) s4[r & 3] += exp_over(acc[i][j][r], from);
+                float sum = (s4[0] + s4[1]) + (s4[2] + s4[3]);
+                sum += __shfl_xor(sum, 32);
+                if (half == 0) joined[wi * N + jj] = make_float2(base, sum);
+                // the token's logit, where it is in this tile
+                const int64_t far = token[j] - p.first - ii0 - 4 * half;
+                const int at = row < p.nj && token[j] < p.vocab && far >= 0 && far < W * kTile && !(far & 4) ? (int)far : -1;
+                if (__ballot(at >= 0)) {
+                    float logit = 0.0f;
+#pragma unroll
+                    for (int i = 0; i < W; ++i)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) logit = at == i * kTile + 8 * (r / 4) + r % 4 ? acc[i][j][r] : logit;
+                    if (at >= 0) p.label[row] = logit;
+                }
             }
-        }
-        __syncthreads();
-        for (int jj = threadIdx.x; jj < N; jj += 256) {
-            if (j0 + jj >= p.nj) continue;
-            p.stats[(int64_t)ti * p.nj + j0 + jj] = join(joined[jj], joined[N + jj]);
-        }
-    } else if constexpr (Mode == kGradient) {
-        typedef typename Vec<E>::V4 V4;
+            __builtin_amdgcn_s_waitcnt(kWaitReads);
+            asm volatile("" ::: "memory");
+            __builtin_amdgcn_s_barrier();
+            asm volatile("" ::: "memory");
+            for (int jj = threadIdx.x; jj < N; jj += 256)
+                if (j0 + jj < p.nj) p.stats[(int64_t)(i0 / N) * p.nj + j0 + jj] = join(joined[jj], joined[N + jj]);
+            // (the next tile's barriers are between these reads and what it writes there)
+        } else if constexpr (Mode == kGradient) {
+            typedef typename Vec<E>::V4 V4;
 #pragma unroll
-        for (int j = 0; j < W; ++j) {
-            const int32_t row = j0 + (wj * W + j) * kTile + (lane & 31);
-            const bool there = row < p.nj;
-            const int64_t token = there ? p.tokens[row] : p.ignore;
-            const float peak = there ? p.peak[row] : 0.0f, total = there ? p.total[row] : 1.0f;
-            const bool none = !there || token == p.ignore || peak == -INFINITY;
-            const float inverse = p.g_scale / total;
-            E *to = static_cast<E *>(p.g) + row * p.g_stride + i0 + wi * W * kTile;
-            const int64_t at = token - p.first - i0 - wi * W * kTile;
+            for (int j = 0; j < W; ++j) {
+                const int32_t row = j0 + (wj * W + j) * kTile + (lane & 31);
+                const bool none = row >= p.nj || token[j] == p.ignore || peak[j] == -INFINITY;
+                const float inverse = p.g_scale / total[j];
+                E *to = static_cast<E *>(p.g) + row * p.g_stride + ii0 + 4 * half;
+                const int64_t far = token[j] - p.first - ii0 - 4 * half;
+                const int at = far >= 0 && far < W * kTile ? (int)far : -1;   // (one of the other half's rows is none of this one's)
+                const bool any = __ballot(at >= 0) != 0;
 #pragma unroll
-            for (int i = 0; i < W; ++i)
+                for (int i = 0; i < W; ++i)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    float v[4];
+                    for (int q = 0; q < 4; ++q) {
+                        float v[4];
 #pragma unroll
-                    for (int r = 0; r < 4; ++r) {
-                        const int in = i * kTile + 8 * q + 4 * half + r;
-                        const float e = __builtin_amdgcn_exp2f((acc[i][j][q * 4 + r] - peak) * kLog2e);
-                        v[r] = fmaf(e, inverse, at == in ? -p.g_scale : 0.0f);
-                        if (none || i0 + wi * W * kTile + in >= p.ni) v[r] = 0.0f;
-                    }
-                    if constexpr (std::is_same<T, float>::value) {
-                        V4 parts[3];
+                        for (int r = 0; r < 4; ++r) v[r] = exp_over(acc[i][j][q * 4 + r], peak[j]) * inverse;
+                        if (any) {
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) {
-                            bf16 s[3];
-                            split(v[r], s);
-#pragma unroll
-                            for (int k = 0; k < 3; ++k) parts[k][r] = s[k];
+                            for (int r = 0; r < 4; ++r)
+                                if (at == i * kTile + 8 * q + r) v[r] = fmaf(exp_over(acc[i][j][q * 4 + r], peak[j]), inverse, -p.g_scale);
                         }
 #pragma unroll
-                        for (int k = 0; k < 3; ++k) *reinterpret_cast<V4 *>(to + k * p.g_part + i * kTile + 8 * q + 4 * half) = parts[k];
-                    } else {
-                        V4 w;
+                        for (int r = 0; r < 4; ++r)
+                            if (none || (edge && ii0 + 4 * half + i * kTile + 8 * q + r >= p.ni)) v[r] = 0.0f;
+                        if constexpr (std::is_same<T, float>::value) {
+                            V4 parts[3];
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) w[r] = (E)v[r];
-                        *reinterpret_cast<V4 *>(to + i * kTile + 8 * q + 4 * half) = w;
+                            for (int r = 0; r < 4; ++r) {
+                                bf16 part[3];
+                                split(v[r], part);
+#pragma unroll
+                                for (int k = 0; k < 3; ++k) parts[k][r] = part[k];
+                            }
+#pragma unroll
+                            for (int k = 0; k < 3; ++k) *reinterpret_cast<V4 *>(to + k * p.g_part + i * kTile + 8 * q) = parts[k];
+                        } else {
+                            V4 w;
+#pragma unroll
+                            for (int r = 0; r < 4; ++r) w[r] = (E)v[r];
+                            *reinterpret_cast<V4 *>(to + i * kTile + 8 * q) = w;
+                        }
                     }
-                }
-        }
-    } else {
-        const float scale = Mode == kOut ? p.out_scale * (p.factor ? *p.factor : 1.0f) : 1.0f;
+            }
+        } else {
+            const float scale = Mode == kOut ? p.out_scale * *p.factor : 1.0f;
 #pragma unroll
-        for (int j = 0; j < W; ++j) {
-            const int32_t row = j0 + (wj * W + j) * kTile + (lane & 31);
-            if (row >= p.nj) continue;
+            for (int j = 0; j < W; ++j) {
+                const int32_t row = j0 + (wj * W + j) * kTile + (lane & 31);
+                if (row >= p.nj) continue;
 #pragma unroll
-            for (int i = 0; i < W; ++i)
+                for (int i = 0; i < W; ++i)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    const int32_t col = i0 + (wi * W + i) * kTile + 8 * q + 4 * half;
-                    if (col >= p.ni) continue;
-                    if constexpr (Mode == kSlab) {   // (rows of a slab are whole fours)
-                        Acc4 *to = reinterpret_cast<Acc4 *>(p.slab + slice * p.slab_size + row * p.slab_stride + col);
+                    for (int q = 0; q < 4; ++q) {
+                        const int32_t col = ii0 + i * kTile + 8 * q + 4 * half;
+                        if (col >= p.ni) continue;
                         Acc4 v;
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) v[r] = acc[i][j][q * 4 + r];
-                        *to = p.add ? *to + v : v;
-                    } else {
-                        T *to = static_cast<T *>(p.out) + (int64_t)row * p.ni + col;
+                        for (int r = 0; r < 4; ++r) v[r] = acc[i][j][q * 4 + r] * scale;
+                        if constexpr (Mode == kSlab) {   // (rows of a slab are whole fours)
+                            Acc4 *to = reinterpret_cast<Acc4 *>(p.slab + out_slice * p.slab_size + row * p.slab_stride + col);
+                            *to = p.add ? *to + v : v;
+                        } else {
+                            T *to = static_cast<T *>(p.out) + (int64_t)row * p.ni + col;
+                            if (col + 4 <= p.ni) {
+                                put4<T>(to, v);
+                            } else {
 #pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (col + r < p.ni) to[r] = (T)(acc[i][j][q * 4 + r] * scale);
+                                for (int r = 0; r < 4; ++r)
+                                    if (col + r < p.ni) to[r] = (T)v[r];
+                            }
+                        }
                     }
-                }
+            }
         }
     }
+#undef BMTK_N
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -479,12 +563,12 @@ __global__ __launch_bounds__(1024) void stats_join_kernel(const float2 *stats, i
     for (int k = 1; k < 16; ++k) sum = join(sum, parts[k][lane]);
     const float m = sum.x, s = sum.y;
     const float log_total = logf(s);
-    const float l = m == -INFINITY && s == 0.0f ? -INFINITY : m + log_total;
+    const float l = m == -INFINITY && s == 0.0f ? -INFINITY : fmaf(m, kLn2, log_total);
     const int64_t token = tokens[row];
     peak[row] = m;
     total[row] = s;
     lse[row] = m == INFINITY ? NAN : l;
-    logp[row] = token == ignore ? 0.0f : token < 0 || token >= vocab || m == INFINITY ? NAN : l == -INFINITY ? -INFINITY : (label[row] - m) - log_total;
+    logp[row] = token == ignore ? 0.0f : token < 0 || token >= vocab || m == INFINITY ? NAN : l == -INFINITY ? -INFINITY : fmaf(fmaf(label[row], kLog2e, -m), kLn2, -log_total);
 }
 
 // results from their slabs: rows of `width` numbers, n of them there
@@ -631,14 +715,15 @@ __global__ __launch_bounds__(256) void few_rows_kernel(Few a)
             }
         m = fmaxf(m, __shfl_xor(m, 16));
         m = fmaxf(m, __shfl_xor(m, 32));
+        const float base = base_of(m), from = base == -INFINITY ? 0.0f : base;
         float s = 0.0f;
 #pragma unroll
         for (int i = 0; i < 2; ++i)
 #pragma unroll
-            for (int r = 0; r < 4; ++r) s += exp_below(acc[i][j][r], m);
+            for (int r = 0; r < 4; ++r) s += exp_over(acc[i][j][r], from);
         s += __shfl_xor(s, 16);
         s += __shfl_xor(s, 32);
-        if (quarter == 0) parts[wave][row] = make_float2(m, s);
+        if (quarter == 0) parts[wave][row] = make_float2(base, s);
     }
     __syncthreads();
     if ((int)threadIdx.x < a.rows) {
@@ -744,9 +829,10 @@ void multiply(Product &p, int32_t tile, hipStream_t s)
 {
     p.tiles_i = (int32_t)div_up(p.ni, tile);
     p.tiles_j = (int32_t)div_up(p.nj, tile);
-    const uint32_t blocks = (uint32_t)p.tiles_i * p.tiles_j * p.slices;
-    if (tile == 256) product_kernel<E, T, 4, AK, BK, Mode><<<blocks, 256, 0, s>>>(p);
-    else product_kernel<E, T, 2, AK, BK, Mode><<<blocks, 256, 0, s>>>(p);
+    const uint32_t jobs = (uint32_t)p.tiles_i * p.tiles_j * p.slices;
+    // (a compute unit holds one workgroup of the large tiles, two of the small ones)
+    if (tile == 256) product_kernel<E, T, 4, AK, BK, Mode><<<jobs < 256 ? jobs : 256, 256, 0, s>>>(p);
+    else product_kernel<E, T, 2, AK, BK, Mode><<<jobs < 512 ? jobs : 512, 256, 0, s>>>(p);
 }
 
 template <typename T>
