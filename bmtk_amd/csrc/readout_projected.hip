@@ -38,6 +38,28 @@ struct Vec<f16> {
     static __device__ __forceinline__ Acc4 mfma16(V8 a, V8 b, Acc4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
 
+// eight numbers from where they begin anywhere
+template <typename T>
+struct Loose8 {
+    typedef uint32_t Words __attribute__((ext_vector_type(4)));
+    typedef Words Loose __attribute__((aligned(2)));
+    union {
+        Words w[sizeof(T) / 2];
+        T v[8];
+    };
+    __device__ __forceinline__ Loose8() {}
+    __device__ __forceinline__ void load(const T *p)
+    {
+#pragma unroll
+        for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = reinterpret_cast<const Loose *>(p)[i];
+    }
+    __device__ __forceinline__ void load_some(const T *p, int n)   // n of them; 0 for the others
+    {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : (T)0.0f;
+    }
+};
+
 // three bf16 parts of v; of what is not finite the first is it (so that its products are not either), and a number that rounds to infinity is cut
 __device__ __forceinline__ void split(float v, bf16 (&p)[3])
 {
@@ -99,11 +121,15 @@ __device__ __forceinline__ void put4(T *p, const Acc4 &v)
 
 enum { kStats = 0, kGradient = 1, kSlab = 2, kOut = 3 };
 
+struct Source {
+    const char *p;
+    int64_t stride, part, step, total;   // bytes from row to row, from part to part, from step to step, of a part
+    int64_t block;                       // of i (j) contiguous: bytes from 64 numbers of a row to the next 64
+};
+
 struct Product {
-    const char *a, *b;
-    int64_t a_stride, b_stride, a_part, b_part;   // bytes from row to row, from part to part.  A row is an i (j), or a k where i (j) is contiguous
-    int32_t ni, nj, nk;                           // sizes; nk: rows of an operand that has k rows, beyond which its last one is read again
-    int32_t a_last, b_last;                       // bytes of a row that may be read
+    Source a, b;
+    int32_t ni, nj;                               // sizes
     int32_t steps, combinations;                  // steps of kDepth in k; 1 or 6
     int32_t tiles_i, tiles_j, slices;             // slices: parts of the steps, each to a slab of its own
     // kStats, kGradient: i is the vocabulary from first on, j the rows
@@ -113,8 +139,8 @@ struct Product {
     float2 *stats;                                // [tiles_i of all pieces][rows]: maximum, sum of e^(logit - maximum)
     float *label;                                 // [rows]: logit of the row's token
     const float *peak, *total;
-    void *g;                                      // [parts][rows, to a whole tile][piece, to a whole tile]
-    int64_t g_stride, g_part;                     // in numbers
+    void *g;                                      // [parts][piece / 64][rows, to a whole tile][64]: a step's operands lie next to one another in both products that read it
+    int64_t g_block, g_part;                      // in numbers
     float g_scale;
     // kSlab: [slices][nj][slab_stride]; kOut: [nj][ni] of T
     float *slab;
@@ -125,65 +151,70 @@ struct Product {
     float out_scale;
 };
 
-typedef __attribute__((address_space(1))) const uint32_t GlobalWord;
 typedef __attribute__((address_space(3))) uint32_t LdsWord;
 
 // One operand's tile of N rows (i or j) and kDepth k on its way through LDS, 16 bytes a lane straight from memory.
-// K rows of 128 bytes, k contiguous: the 16 bytes c of row r lie at c ^ (r & 7), so that eight rows' same c are in different banks.
-// Otherwise N * 2 bytes of a k: their 32 bytes s lie at s ^ (k & 3), so that four rows' same s are; fragments are transposed as they are read.
+// LDS gives 256 bytes at a time.  Rows of 128 bytes, k contiguous: the 16 bytes c of row r lie at c ^ (r / 2 & 7), so that sixteen rows' same c are in different banks.
+// Otherwise N * 2 bytes of a k: their 32 bytes s lie at s ^ 2 (k & 3), so that four rows' s and s ^ 1 are; fragments are transposed as they are read.
+// Loads are of a buffer that ends with the operand: what a tile has beyond it is 0, and nothing outside is read.
 template <typename E, int N, int Waves, bool KRows>
 struct Operand {
     static constexpr int kBytes = N * kDepth * 2, kLoads = kBytes / 1024 / Waves;
-    static_assert(kLoads >= 1, "a load for every wavefront");
+    static constexpr int kLoadRows = KRows ? 512 / N : 8;                    // rows that a load of a wavefront takes
+    static constexpr int kVary = KRows && kLoadRows != 2 ? 1 : 2;            // loads in a row that differ by their swizzle
+    static_assert(kLoads >= 1 && kLoads % kVary == 0, "a load for every wavefront");
     typedef typename Vec<E>::V8 V8;
-    typedef typename Vec<E>::V4 V4;
-    uint32_t from[kLoads];   // K rows: of every load, the row's bytes from the tile's first one, and the chunk's; else the column's bytes alone
-    const char *base;        // the tile's first row (K rows), or column
-    int64_t stride, part;
-    int32_t last, nk;
-    __device__ __forceinline__ void start(const char *p, int64_t stride_, int64_t part_, int32_t last_, int32_t row0, int32_t rows, int32_t nk_, int lane, int wave)
+    uint32_t from[kVary];    // this lane's bytes of a wavefront's first loads
+    uint32_t each;           // bytes from one load's rows to the next one's
+    const char *at;          // what the tile begins with, at the step that is to be loaded
+    int64_t left;            // bytes from there to the operand's end
+    __device__ __forceinline__ void start(const Source &s, int32_t row0, int lane, int wave)
     {
-        stride = stride_, part = part_, last = last_, nk = nk_;
-        if constexpr (!KRows) {
-            base = p + (int64_t)row0 * stride;
+        const int64_t skip = KRows ? row0 / 64 * s.block : row0 * s.stride;
+        at = s.p + skip;
+        left = s.total - skip;
+        each = (uint32_t)(kLoadRows * s.stride);
 #pragma unroll
-            for (int n = 0; n < kLoads; ++n) {
-                const int row = (wave * kLoads + n) * 8 + lane / 8;
-                from[n] = (uint32_t)(min(row, rows - 1 - row0) * (int32_t)stride);
-            }
-        } else {
-            base = p;
-#pragma unroll
-            for (int n = 0; n < kLoads; ++n) {
+        for (int n = 0; n < kVary; ++n) {
+            if constexpr (!KRows) {
+                const int row = (wave * kLoads + n) * kLoadRows + lane / 8;
+                from[n] = (uint32_t)(row - n * kLoadRows) * (uint32_t)s.stride + (uint32_t)((lane & 7) ^ (row / 2 & 7)) * 16;
+            } else {
                 constexpr int kChunks = N / 8;   // of 16 bytes in a row
-                const int at = (wave * kLoads + n) * 64 + lane, k = at / kChunks, slot = at % kChunks;
-                const int chunk = slot ^ ((k & 3) * 2);
-                from[n] = (uint32_t)min(row0 * 2 + chunk * 16, last - 16);
+                const int k = (wave * kLoads + n) * kLoadRows + lane / kChunks, byte = ((lane % kChunks) ^ ((k & 3) * 4)) * 16;
+                from[n] = (uint32_t)(k - n * kLoadRows) * (uint32_t)s.stride + (uint32_t)(byte / 128) * (uint32_t)s.block + (uint32_t)(byte % 128);
             }
         }
     }
-    __device__ __forceinline__ void load(char *lds, int32_t step, int which, int lane, int wave) const
+    // load n of step `step` of a part, to where the tile's stage begins in LDS
+    __device__ __forceinline__ void load(int n, uint32_t lds, const Source &s, int32_t step, int which, int wave) const
     {
-        const char *p = base + which * part;
-#pragma unroll
-        for (int n = 0; n < kLoads; ++n) {
-            const char *q;
-            if constexpr (!KRows) {
-                const int chunk = (lane & 7) ^ (lane / 8 & 7);
-                q = p + (from[n] + (uint32_t)min(step * (kDepth * 2) + chunk * 16, last - 16));
-            } else {
-                constexpr int kChunks = N / 8;
-                const int k = ((wave * kLoads + n) * 64 + lane) / kChunks;
-                q = p + (int64_t)min(step * kDepth + k, nk - 1) * stride + from[n];
-            }
-            __builtin_amdgcn_global_load_lds((GlobalWord *)q, (LdsWord *)(lds + (wave * kLoads + n) * 1024), 16, 0, 0);
-        }
+#ifdef __HIP_DEVICE_COMPILE__   // (types and registers that the host's compiler does not know)
+        const int64_t skip = step * s.step;
+        const int64_t records = left - skip;
+        const __amdgpu_buffer_rsrc_t rsrc = __builtin_amdgcn_make_buffer_rsrc(const_cast<char *>(at + which * s.part + skip), 0, (int)(uint32_t)(records < 0xfffffff0ll ? records : 0xfffffff0ll), 0x00020000);
+        __builtin_amdgcn_raw_ptr_buffer_load_lds(rsrc, (LdsWord *)(uintptr_t)(lds + (wave * kLoads + n) * 1024), 16, from[n % kVary] + n * each, 0, 0, 0);
+#endif
+    }
+    // The same where fragments are transposed as they are read: before such a read the compiler would wait for every load to LDS that it knows of, also for those of
+    // the other stage.  (The load has no register for a result, it has read those that say where when it is issued, and the kernel waits for it by itself;
+    // nothing else in such a kernel uses m0.  Five wait states: of a scalar register that a vector instruction may just have written.)
+    __device__ __forceinline__ void load_untold(int n, uint32_t lds, const Source &s, int32_t step, int which, int wave) const
+    {
+#ifdef __HIP_DEVICE_COMPILE__
+        typedef uint32_t Words __attribute__((ext_vector_type(4)));
+        const int64_t skip = step * s.step;
+        const int64_t records = left - skip;
+        const uintptr_t p = reinterpret_cast<uintptr_t>(at + which * s.part + skip);
+        const Words rsrc = {(uint32_t)p, (uint32_t)(p >> 32), (uint32_t)(records < 0xfffffff0ll ? records : 0xfffffff0ll), 0x00020000u};
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds + (wave * kLoads + n) * 1024), "v"(from[n % kVary] + n * each), "s"(rsrc) : "memory");
+#endif
     }
     // the fragment of 32 rows from `row` (a multiple of 32) on, sixteen k from s * 16 on
     __device__ __forceinline__ V8 fragment(const char *lds, int row, int s, int lane) const
     {
         if constexpr (!KRows) {
-            const int r = row + (lane & 31), chunk = (s * 2 + lane / 32) ^ (lane & 7);
+            const int r = row + (lane & 31), chunk = (s * 2 + lane / 32) ^ (lane / 2 & 7);
             return *reinterpret_cast<const V8 *>(lds + r * 128 + chunk * 16);
         } else {
             // sixteen lanes read four k of sixteen columns, 8 bytes each, and get a column's four k each
@@ -196,7 +227,7 @@ struct Operand {
             } r;
 #pragma unroll
             for (int q = 0; q < 2; ++q) {
-                const int k = s * 16 + (group >> 1) * 8 + q * 4 + l / 4, seg = (row / 16 + (group & 1)) ^ (l / 4);
+                const int k = s * 16 + (group >> 1) * 8 + q * 4 + l / 4, seg = (row / 16 + (group & 1)) ^ (l / 4 * 2);
                 r.half[q] = __builtin_amdgcn_ds_read_tr16_b64_v4i16((P)(lds + k * (N * 2) + seg * 32 + (l & 3) * 8));
             }
             return r.v;
@@ -204,16 +235,41 @@ struct Operand {
     }
 };
 
-// The order of tiles: workgroups go round the eight XCDs; each XCD gets neighbouring tiles, in blocks of 8 tiles of j by tiles of i, so that what its
+// The order of jobs: workgroups go round the eight XCDs; each XCD gets neighbouring tiles of a slice, in blocks of 8 tiles of j by tiles of i, so that what its
 // compute units read at one time stays in its L2.
-__device__ __forceinline__ void place(int32_t block, int32_t blocks, int32_t tiles_i, int32_t tiles_j, int32_t &ti, int32_t &tj)
+__device__ __forceinline__ void place(int32_t job, int32_t jobs, int32_t tiles_i, int32_t tiles_j, int32_t &slice, int32_t &ti, int32_t &tj)
 {
-    const int32_t x = block & 7, each = blocks >> 3, rest = blocks & 7;
-    const int32_t id = x * each + min(x, rest) + (block >> 3);
+    const int32_t x = job & 7, each = jobs >> 3, rest = jobs & 7, tiles = tiles_i * tiles_j;
+    int32_t id = x * each + min(x, rest) + (job >> 3);
+    slice = id / tiles;
+    id -= slice * tiles;
     constexpr int32_t kBand = 8;
     const int32_t band = id / (kBand * tiles_i), in_band = id - band * kBand * tiles_i, height = min(kBand, tiles_j - band * kBand);
     ti = in_band / height;
     tj = band * kBand + in_band % height;
+}
+
+// 16-bit results of 32 columns (v[i][q]: four of a lane's column) as rows of W * 64 bytes, each written 16 bytes a lane: through a part of LDS of the wavefront's own,
+// where the 16 bytes c of a column lie at c ^ column, of as many bits as c has.  `to(r, c)`: where byte c of column r goes, or null.
+template <int W, typename V4, typename To>
+__device__ __forceinline__ void columns_out(char *lds, const V4 (&v)[W][4], int lane, const To &to)
+{
+    constexpr int kRow = W * kTile * 2, kChunks = kRow / 16;
+    char *mine = lds + (lane & 31) * kRow;
+#pragma unroll
+    for (int i = 0; i < W; ++i)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) *reinterpret_cast<V4 *>(mine + (((i * 4 + q) ^ (lane & (kChunks - 1))) * 16 + lane / 32 * 8)) = v[i][q];
+    __builtin_amdgcn_wave_barrier();   // (the wavefront's own LDS operations are done in order)
+#pragma unroll
+    for (int n = 0; n < kTile * kChunks / 64; ++n) {
+        const int at = n * 64 + lane, r = at / kChunks, c = at % kChunks;
+        typedef uint32_t Words __attribute__((ext_vector_type(4)));
+        const Words w = *reinterpret_cast<const Words *>(lds + r * kRow + ((c ^ (r & (kChunks - 1))) * 16));
+        char *p = to(r, c * 16);
+        if (p) *reinterpret_cast<Words *>(p) = w;
+    }
+    __builtin_amdgcn_wave_barrier();
 }
 
 // W: tiles of 32 each way that a wavefront has; a workgroup is 2 x 2 wavefronts.  Workgroups take tiles in turn: the next tile's first two stages are on their way
@@ -225,28 +281,51 @@ __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void product_kernel(Product p)
     typedef Operand<E, N, 4, AK> OpA;
     typedef Operand<E, N, 4, BK> OpB;
     constexpr int kStage = OpA::kBytes + OpB::kBytes;
-    __shared__ __align__(1024) char lds[2 * kStage + (Mode == kStats ? 2 * N * 8 : 0)];
+    // beside the stages: of kStats, the two halves of a tile's sums; of the 16-bit results, a wavefront's 32 columns, to be written row by row
+    constexpr int kRow = W * kTile * 2, kBeside = Mode == kStats ? 2 * N * 8 : Mode == kSlab || (Mode == kOut && std::is_same<T, float>::value) ? 0 : 4 * kTile * kRow;
+    __shared__ __align__(1024) char lds[2 * kStage + kBeside];
     const int lane = lane_id(), wave = __builtin_amdgcn_readfirstlane(threadIdx.x / kWave), wi = wave >> 1, wj = wave & 1;
-    const int32_t tiles = p.tiles_i * p.tiles_j, jobs = tiles * p.slices, all = p.steps * p.combinations;
+    const int32_t jobs = p.tiles_i * p.tiles_j * p.slices, all = p.steps * p.combinations;
     OpA a;
     OpB b;
     int32_t ti, tj, slice, s0, s1, step, combination;
-    const auto fetch = [&](char *to) {
-        a.load(to, step, part_a(combination), lane, wave);
-        b.load(to + OpA::kBytes, step, part_b(combination), lane, wave);
+    const auto fetch_one = [&](int n, int stage) {
+        const uint32_t to = (uint32_t)(uintptr_t)(LdsWord *)lds + stage * kStage;
+        if constexpr (AK || BK) {
+            if (n < OpA::kLoads) a.load_untold(n, to, p.a, step, part_a(combination), wave);
+            else b.load_untold(n - OpA::kLoads, to + OpA::kBytes, p.b, step, part_b(combination), wave);
+        } else {
+            if (n < OpA::kLoads) a.load(n, to, p.a, step, part_a(combination), wave);
+            else b.load(n - OpA::kLoads, to + OpA::kBytes, p.b, step, part_b(combination), wave);
+        }
+    };
+    // offsets of loads are made where they are needed: sixteen registers for them, or thirty-two, are not there
+    const auto make_here = [&]() {
+#pragma unroll
+        for (int n = 0; n < OpA::kVary; ++n) asm volatile("" : "+v"(a.from[n]));
+#pragma unroll
+        for (int n = 0; n < OpB::kVary; ++n) asm volatile("" : "+v"(b.from[n]));
+    };
+    const auto fetch_next = [&]() {
+        make_here();
         const bool more = combination + 1 < p.combinations;
         step = min(more ? step : step + 1, p.steps - 1);   // (behind the last step it is asked for again, for nothing)
         combination = more ? combination + 1 : 0;
     };
+    constexpr int kLoads = OpA::kLoads + OpB::kLoads;
     const auto begin = [&](int32_t job) {
-        slice = job / tiles;
-        place(job - slice * tiles, tiles, p.tiles_i, p.tiles_j, ti, tj);
+        place(job, jobs, p.tiles_i, p.tiles_j, slice, ti, tj);
         s0 = (int32_t)((int64_t)all * slice / p.slices), s1 = (int32_t)((int64_t)all * (slice + 1) / p.slices);
         step = s0 / p.combinations, combination = s0 - step * p.combinations;
-        a.start(p.a, p.a_stride, p.a_part, p.a_last, ti * N, p.ni, p.nk, lane, wave);
-        b.start(p.b, p.b_stride, p.b_part, p.b_last, tj * N, p.nj, p.nk, lane, wave);
-        fetch(lds);
-        fetch(lds + kStage);
+        a.start(p.a, ti * N, lane, wave);
+        b.start(p.b, tj * N, lane, wave);
+        make_here();
+#pragma unroll
+        for (int stage = 0; stage < 2; ++stage) {
+#pragma unroll
+            for (int n = 0; n < kLoads; ++n) fetch_one(n, stage);
+            fetch_next();
+        }
     };
     Acc acc[W][W];
     typename Vec<E>::V8 fa[4][W], fb[4][W];
@@ -266,7 +345,7 @@ __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void product_kernel(Product p)
             for (int j = 0; j < W; ++j) acc[i][j] = Vec<E>::mfma(fa[k][i], fb[k][j], acc[i][j]);
     };
     // beside each of `products` products `reads` LDS reads in all, spread evenly, and `loads` loads to LDS in all
-    constexpr int kReadsA = W * (AK ? 2 : 1), kReadsB = W * (BK ? 2 : 1), kLoads = OpA::kLoads + OpB::kLoads, kHalf = W * W / 2;
+    constexpr int kReadsA = W * (AK ? 2 : 1), kReadsB = W * (BK ? 2 : 1), kHalf = W * W / 2;
     const auto in_turn = [&](auto products, auto reads, auto loads) {
         constexpr int n = decltype(products)::value, r = decltype(reads)::value, l = decltype(loads)::value;
         beside<n, r, l, 0>();
@@ -293,19 +372,9 @@ __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void product_kernel(Product p)
 
     if ((int32_t)blockIdx.x >= jobs) return;
     begin(blockIdx.x);
+    __builtin_amdgcn_s_waitcnt(kWaitLoads);
     for (int32_t job = blockIdx.x; job < jobs; job += gridDim.x) {
         const int32_t i0 = ti * N, j0 = tj * N, out_slice = slice;
-        // what the results will be asked for, of this lane's column of each tile
-        int64_t token[W];
-        float peak[W], total[W];
-        if constexpr (Mode == kStats || Mode == kGradient) {
-#pragma unroll
-            for (int j = 0; j < W; ++j) {
-                const int32_t row = min(j0 + (wj * W + j) * kTile + (lane & 31), p.nj - 1);
-                token[j] = p.tokens[row];
-                if constexpr (Mode == kGradient) peak[j] = p.peak[row], total[j] = p.total[row];
-            }
-        }
 #pragma unroll
         for (int i = 0; i < W; ++i)
 #pragma unroll
@@ -315,7 +384,6 @@ __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void product_kernel(Product p)
         // Two stages in LDS, a step's products in quarters.  A step's fragments are all in registers well before its products are done, so that from the middle of
         // the third quarter on the tile after the next is asked for into the same stage: it has the time of a step's products to come.
         static_assert(kDepth == 64, "four quarters");
-        __builtin_amdgcn_s_waitcnt(kWaitLoads);
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
@@ -331,9 +399,17 @@ __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void product_kernel(Product p)
             asm volatile("" ::: "memory");
             __builtin_amdgcn_s_barrier();
             asm volatile("" ::: "memory");
-            fetch(now);
-            multiply(2, 1);
-            in_turn(BMTK_N(kHalf), BMTK_N(0), BMTK_N(kLoads));
+#pragma unroll
+            for (int i = W / 2; i < W; ++i)
+#pragma unroll
+                for (int j = 0; j < W; ++j) {
+                    acc[i][j] = Vec<E>::mfma(fa[2][i], fb[2][j], acc[i][j]);
+                    constexpr int kEach = kLoads / kHalf;
+#pragma unroll
+                    for (int n = 0; n < kEach; ++n) fetch_one(((i - W / 2) * W + j) * kEach + n, (s - s0) & 1);
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            fetch_next();
             take_a(0, next);
             take_b(0, next);
             multiply(3, 0);
@@ -348,27 +424,39 @@ __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void product_kernel(Product p)
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
+        // what the results will be asked for, of this lane's column of each tile: before the next tile's loads, so that it is not waited for behind them
+        int64_t token[W];
+        float peak[W], total[W];
+        if constexpr (Mode == kStats || Mode == kGradient) {
+#pragma unroll
+            for (int j = 0; j < W; ++j) {
+                const int32_t row = min(j0 + (wj * W + j) * kTile + (lane & 31), p.nj - 1);
+                token[j] = p.tokens[row];
+                if constexpr (Mode == kGradient) peak[j] = p.peak[row], total[j] = p.total[row];
+            }
+        }
         if (job + (int32_t)gridDim.x < jobs) begin(job + gridDim.x);
         multiply(2, 0);
         multiply(2, 1);
         multiply(3, 0);
         multiply(3, 1);
+        __builtin_amdgcn_sched_barrier(0);
 
         // lane l has column j = l % 32 of a tile and its rows i = 8 (r / 4) + 4 (l / 32) + r % 4
         const int half = lane / 32, ii0 = i0 + wi * W * kTile;
         const bool edge = i0 + N > p.ni;
+        const auto cut = [&](int j) {   // logits behind the vocabulary
+#pragma unroll
+            for (int i = 0; i < W; ++i)
+#pragma unroll
+                for (int r = 0; r < 16; ++r) acc[i][j][r] = ii0 + i * kTile + 8 * (r / 4) + 4 * half + r % 4 >= p.ni ? -INFINITY : acc[i][j][r];
+        };
         if constexpr (Mode == kStats) {
             float2 *joined = reinterpret_cast<float2 *>(lds + 2 * kStage);   // [2][N]
 #pragma unroll
             for (int j = 0; j < W; ++j) {
                 const int32_t jj = (wj * W + j) * kTile + (lane & 31), row = j0 + jj;
-                if (edge) {
-#pragma unroll
-                    for (int i = 0; i < W; ++i)
-#pragma unroll
-                        for (int r = 0; r < 16; ++r)
-                            if (ii0 + i * kTile + 8 * (r / 4) + 4 * half + r % 4 >= p.ni) acc[i][j][r] = -INFINITY;
-                }
+                if (edge) cut(j);
                 float m = acc[0][j][0];
 #pragma unroll
                 for (int i = 0; i < W; ++i)
@@ -395,6 +483,7 @@ __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void product_kernel(Product p)
                         for (int r = 0; r < 16; ++r) logit = at == i * kTile + 8 * (r / 4) + r % 4 ? acc[i][j][r] : logit;
                     if (at >= 0) p.label[row] = logit;
                 }
+                __builtin_amdgcn_sched_barrier(0);
             }
             __builtin_amdgcn_s_waitcnt(kWaitReads);
             asm volatile("" ::: "memory");
@@ -410,49 +499,68 @@ __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void product_kernel(Product p)
                 const int32_t row = j0 + (wj * W + j) * kTile + (lane & 31);
                 const bool none = row >= p.nj || token[j] == p.ignore || peak[j] == -INFINITY;
                 const float inverse = p.g_scale / total[j];
-                E *to = static_cast<E *>(p.g) + row * p.g_stride + ii0 + 4 * half;
                 const int64_t far = token[j] - p.first - ii0 - 4 * half;
-                const int at = far >= 0 && far < W * kTile ? (int)far : -1;   // (one of the other half's rows is none of this one's)
-                const bool any = __ballot(at >= 0) != 0;
+                const int at = far >= 0 && far < W * kTile && !(far & 4) ? (int)far : -1;
+                if (edge) cut(j);
 #pragma unroll
                 for (int i = 0; i < W; ++i)
 #pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        float v[4];
+                    for (int r = 0; r < 16; ++r) acc[i][j][r] = none ? 0.0f : exp_over(acc[i][j][r], peak[j]) * inverse;
+                if (__ballot(at >= 0 && !none)) {
 #pragma unroll
-                        for (int r = 0; r < 4; ++r) v[r] = exp_over(acc[i][j][q * 4 + r], peak[j]) * inverse;
-                        if (any) {
+                    for (int i = 0; i < W; ++i)
 #pragma unroll
-                            for (int r = 0; r < 4; ++r)
-                                if (at == i * kTile + 8 * q + r) v[r] = fmaf(exp_over(acc[i][j][q * 4 + r], peak[j]), inverse, -p.g_scale);
-                        }
+                        for (int r = 0; r < 16; ++r) acc[i][j][r] -= at == i * kTile + 8 * (r / 4) + r % 4 && !none ? p.g_scale : 0.0f;
+                }
+                V4 out[std::is_same<T, float>::value ? 3 : 1][W][4];
 #pragma unroll
-                        for (int r = 0; r < 4; ++r)
-                            if (none || (edge && ii0 + 4 * half + i * kTile + 8 * q + r >= p.ni)) v[r] = 0.0f;
-                        if constexpr (std::is_same<T, float>::value) {
-                            V4 parts[3];
+                for (int i = 0; i < W; ++i)
 #pragma unroll
-                            for (int r = 0; r < 4; ++r) {
+                    for (int q = 0; q < 4; ++q)
+#pragma unroll
+                        for (int r = 0; r < 4; ++r) {
+                            if constexpr (std::is_same<T, float>::value) {
                                 bf16 part[3];
-                                split(v[r], part);
+                                split(acc[i][j][q * 4 + r], part);
 #pragma unroll
-                                for (int k = 0; k < 3; ++k) parts[k][r] = part[k];
+                                for (int k = 0; k < 3; ++k) out[k][i][q][r] = part[k];
+                            } else {
+                                out[0][i][q][r] = (E)acc[i][j][q * 4 + r];
                             }
-#pragma unroll
-                            for (int k = 0; k < 3; ++k) *reinterpret_cast<V4 *>(to + k * p.g_part + i * kTile + 8 * q) = parts[k];
-                        } else {
-                            V4 w;
-#pragma unroll
-                            for (int r = 0; r < 4; ++r) w[r] = (E)v[r];
-                            *reinterpret_cast<V4 *>(to + i * kTile + 8 * q) = w;
                         }
-                    }
+                const int32_t row0 = j0 + (wj * W + j) * kTile;
+#pragma unroll
+                for (int k = 0; k < (std::is_same<T, float>::value ? 3 : 1); ++k) {
+                    char *to = reinterpret_cast<char *>(static_cast<E *>(p.g) + k * p.g_part);
+                    columns_out<W>(lds + 2 * kStage + wave * kTile * kRow, out[k], lane, [&](int r, int c) {
+                        const int32_t byte = (ii0 * 2 + c) / 128;
+                        return to + byte * p.g_block * 2 + (int64_t)(row0 + r) * 128 + (ii0 * 2 + c) % 128;
+                    });
+                }
             }
         } else {
             const float scale = Mode == kOut ? p.out_scale * *p.factor : 1.0f;
+            // (rows of whole 16 bytes can go out in those)
+            const bool rows_fit = Mode == kOut && sizeof(T) == 2 && p.ni % 8 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
 #pragma unroll
             for (int j = 0; j < W; ++j) {
-                const int32_t row = j0 + (wj * W + j) * kTile + (lane & 31);
+                const int32_t row0 = j0 + (wj * W + j) * kTile, row = row0 + (lane & 31);
+                if constexpr (Mode == kOut && sizeof(T) == 2) {
+                    if (rows_fit) {
+                        typename Vec<E>::V4 out[W][4];
+#pragma unroll
+                        for (int i = 0; i < W; ++i)
+#pragma unroll
+                            for (int q = 0; q < 4; ++q)
+#pragma unroll
+                                for (int r = 0; r < 4; ++r) out[i][q][r] = (E)(acc[i][j][q * 4 + r] * scale);
+                        columns_out<W>(lds + 2 * kStage + wave * kTile * kRow, out, lane, [&](int r, int c) {
+                            char *to = static_cast<char *>(p.out) + ((int64_t)(row0 + r) * p.ni + ii0) * 2 + c;
+                            return row0 + r < p.nj && ii0 + c / 2 < p.ni ? to : nullptr;
+                        });
+                        continue;
+                    }
+                }
                 if (row >= p.nj) continue;
 #pragma unroll
                 for (int i = 0; i < W; ++i)
@@ -479,6 +587,10 @@ __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void product_kernel(Product p)
                     }
             }
         }
+        // The next tile's loads have come; the results that were written after them need not have arrived.  (Memory operations are counted in order.)
+        constexpr int kWritten = Mode == kGradient ? W * (kTile * kRow / 1024) * (std::is_same<T, float>::value ? 3 : 1) : 0, kMayWait = kWritten < 63 ? kWritten : 63;
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_waitcnt(kWaitLoads | kMayWait % 16 | kMayWait / 16 << 14);
     }
 #undef BMTK_N
 }
@@ -486,29 +598,36 @@ __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void product_kernel(Product p)
 // ---------------------------------------------------------------------------------------------------------------------
 // what goes before and after
 
-// Rows of n numbers, `width` (n or more, with zeros) apart, of T or as the three parts of float; with `by`, times by[row], and rows that have no token are 0
+// Rows of n numbers, `width` (n or more, with zeros; a multiple of 8) apart, of T or as the three parts of float; with `by`, times by[row], and rows that have no
+// token are 0.  Eight numbers a lane.
 template <typename T, typename E>
 __global__ __launch_bounds__(256) void lay_kernel(const T *from, int64_t stride, int64_t rows, int32_t n, int32_t width, int64_t padded_rows, E *to, const float *by)
 {
-    const int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x, row = k / width;
-    const int32_t c = (int32_t)(k - row * width);
+    const int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x, row = k / (width / 8);
+    const int32_t c = (int32_t)(k - row * (width / 8)) * 8;
     if (row >= padded_rows) return;
-    float v = 0.0f;
-    if (row < rows && c < n) {
-        v = (float)from[row * stride + c];
-        if (by) {
-            const float f = by[row];
-            v = f == 0.0f ? 0.0f : v * f;
+    Loose8<T> in;
+    const int some = row < rows ? n - c : 0;
+    if (some >= 8) in.load(from + row * stride + c);
+    else in.load_some(from + row * stride + c, some);
+    const float f = by && row < rows ? by[row] : 1.0f;
+    typedef typename Vec<E>::V8 V8;
+    V8 out[std::is_same<T, float>::value ? 3 : 1];
+#pragma unroll
+    for (int i = 0; i < 8; ++i) {
+        float v = (float)in.v[i];
+        if (by) v = f == 0.0f ? 0.0f : v * f;
+        if constexpr (std::is_same<T, float>::value) {
+            bf16 s[3];
+            split(v, s);
+#pragma unroll
+            for (int j = 0; j < 3; ++j) out[j][i] = s[j];
+        } else {
+            out[0][i] = (E)v;
         }
     }
-    if constexpr (std::is_same<T, float>::value) {
-        bf16 s[3];
-        split(v, s);
 #pragma unroll
-        for (int i = 0; i < 3; ++i) to[i * padded_rows * width + k] = s[i];
-    } else {
-        to[k] = (E)v;
-    }
+    for (int j = 0; j < (std::is_same<T, float>::value ? 3 : 1); ++j) *reinterpret_cast<V8 *>(to + j * padded_rows * width + k * 8) = out[j];
 }
 
 // weights[row] = d_logp over a power of two that leaves the largest at 1 to 2 (for fp16; else itself), 0 for rows without a token, NaN for tokens outside
@@ -590,27 +709,6 @@ __global__ __launch_bounds__(256) void slab_join_kernel(const float *slab, int32
 // ---------------------------------------------------------------------------------------------------------------------
 // few rows: a wavefront takes 32 rows of the weights straight from memory into matrix instructions of 16 x 16, against J times 16 rows of x from the
 // caches.  Bound by the weights' bytes.
-
-template <typename T>
-struct Loose8 {
-    typedef uint32_t Words __attribute__((ext_vector_type(4)));
-    typedef Words Loose __attribute__((aligned(2)));
-    union {
-        Words w[sizeof(T) / 2];
-        T v[8];
-    };
-    __device__ __forceinline__ Loose8() {}
-    __device__ __forceinline__ void load(const T *p)
-    {
-#pragma unroll
-        for (int i = 0; i < (int)sizeof(T) / 2; ++i) w[i] = reinterpret_cast<const Loose *>(p)[i];
-    }
-    __device__ __forceinline__ void load_some(const T *p, int n)   // n of them; 0 for the others
-    {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : (T)0.0f;
-    }
-};
 
 struct Few {
     const void *x, *weight;
@@ -809,7 +907,7 @@ struct Plan {
 
 bool sizes_fit(int64_t rows, int64_t vocab, int64_t dim, int32_t dtype)
 {
-    return rows > 0 && vocab > 0 && dim > 0 && dtype >= 0 && dtype <= 2 && rows < (1 << 24) && vocab < (1 << 28) && dim <= 65536;
+    return rows > 0 && vocab > 0 && dim > 0 && dtype >= 0 && dtype <= 2 && rows < (1 << 22) && vocab < (1 << 28) && dim <= 65536;
 }
 
 // whether rows can be read 16 bytes at a time
@@ -839,7 +937,7 @@ template <typename T>
 void lay(const void *from, int64_t stride, int64_t rows, int32_t n, int64_t width, int64_t padded_rows, void *to, const float *by, hipStream_t s)
 {
     typedef typename Element<T>::type E;
-    lay_kernel<T, E><<<(uint32_t)div_up(padded_rows * width, 256), 256, 0, s>>>(static_cast<const T *>(from), stride, rows, n, (int32_t)width, padded_rows, static_cast<E *>(to), by);
+    lay_kernel<T, E><<<(uint32_t)div_up(padded_rows * width / 8, 256), 256, 0, s>>>(static_cast<const T *>(from), stride, rows, n, (int32_t)width, padded_rows, static_cast<E *>(to), by);
 }
 
 struct Call {
@@ -857,20 +955,19 @@ struct Call {
     }
 };
 
+// rows of n numbers, `stride` apart, as an operand: their numbers as k, or the rows
+Source by_numbers(const char *p, int64_t stride, int64_t part, int64_t rows, int64_t n) { return {p, stride * 2, part * 2, kDepth * 2, ((rows - 1) * stride + n) * 2, 128}; }
+Source by_rows(const char *p, int64_t stride, int64_t part, int64_t rows, int64_t n) { return {p, stride * 2, part * 2, kDepth * stride * 2, ((rows - 1) * stride + n) * 2, 128}; }
+
 // logits as a product: i the vocabulary from `first` on, j the rows
 template <typename T>
 Product logits(const Call &c, const Plan &plan, const char *x, const char *w, int64_t first, int64_t count)
 {
     Product p{};
-    p.a_stride = plan.copy_w ? plan.depth * 2 : c.w_stride * 2;
-    p.a_part = plan.copy_w ? c.vocab * plan.depth * 2 : 0;
-    p.a_last = plan.copy_w ? plan.depth * 2 : c.dim * 2;
-    p.a = w + first * p.a_stride;
-    p.b = x;
-    p.b_stride = plan.copy_x ? plan.depth * 2 : c.x_stride * 2;
-    p.b_part = plan.copy_x ? c.rows * plan.depth * 2 : 0;
-    p.b_last = plan.depth * 2;
-    p.ni = (int32_t)count, p.nj = (int32_t)c.rows, p.nk = 0;
+    const int64_t w_stride = plan.copy_w ? plan.depth : c.w_stride, x_stride = plan.copy_x ? plan.depth : c.x_stride;
+    p.a = by_numbers(w + first * w_stride * 2, w_stride, c.vocab * plan.depth, count, plan.copy_w ? plan.depth : c.dim);
+    p.b = by_numbers(x, x_stride, c.rows * plan.depth, c.rows, plan.depth);
+    p.ni = (int32_t)count, p.nj = (int32_t)c.rows;
     p.steps = plan.depth / kDepth, p.combinations = plan.combinations, p.slices = 1;
     p.first = (int32_t)first, p.vocab = (int32_t)c.vocab, p.tokens = c.tokens, p.ignore = c.ignore;
     return p;
@@ -940,23 +1037,23 @@ void backward(Call c, const float *peak, const float *total, const float *d_logp
     for (int64_t q = 0; q < plan.pieces; ++q) {
         const int64_t first = q * plan.piece, count = c.vocab - first < plan.piece ? c.vocab - first : plan.piece;
         Product p = logits<T>(c, plan, x, w, first, count);
-        p.peak = peak, p.total = total, p.g = g, p.g_stride = plan.g_width, p.g_part = plan.g_rows * plan.g_width, p.g_scale = g_scale;
+        p.peak = peak, p.total = total, p.g = g, p.g_block = plan.g_rows * 64, p.g_part = plan.g_rows * plan.g_width, p.g_scale = g_scale;
         multiply<E, T, false, false, kGradient>(p, plan.logit_tile, c.stream);
 
         // dx: i a channel, j a row, k the vocabulary
         Product d{};
-        d.a = p.a, d.a_stride = p.a_stride, d.a_part = p.a_part, d.a_last = p.a_last;
-        d.b = g, d.b_stride = plan.g_width * 2, d.b_part = p.g_part * 2, d.b_last = (int32_t)(plan.g_width * 2);
-        d.ni = c.dim, d.nj = (int32_t)c.rows, d.nk = (int32_t)count;
+        d.a = by_rows(p.a.p, p.a.stride / 2, p.a.part / 2, count, plan.copy_w ? plan.depth : c.dim);
+        d.b = {g, 128, p.g_part * 2, plan.g_rows * 128, p.g_part * 2, 0};
+        d.ni = c.dim, d.nj = (int32_t)c.rows;
         d.steps = (int32_t)div_up(count, kDepth), d.combinations = plan.combinations, d.slices = plan.dx_slices;
         d.slab = dx_slab, d.slab_stride = plan.out_width, d.slab_size = c.rows * plan.out_width, d.add = q > 0;
         multiply<E, T, true, false, kSlab>(d, plan.dx_tile, c.stream);
 
         // d_weight: i a channel, j the vocabulary, k a row
         Product e{};
-        e.a = x_weighted, e.a_stride = plan.out_width * 2, e.a_part = k_rows * plan.out_width * 2, e.a_last = (int32_t)(plan.out_width * 2);
-        e.b = g, e.b_stride = plan.g_width * 2, e.b_part = p.g_part * 2, e.b_last = (int32_t)(plan.g_width * 2);
-        e.ni = c.dim, e.nj = (int32_t)count, e.nk = (int32_t)k_rows;
+        e.a = by_rows(x_weighted, plan.out_width, k_rows * plan.out_width, k_rows, plan.out_width);
+        e.b = {g, 128, p.g_part * 2, kDepth * 128, p.g_part * 2, plan.g_rows * 128};
+        e.ni = c.dim, e.nj = (int32_t)count;
         e.steps = (int32_t)(k_rows / kDepth), e.combinations = plan.combinations, e.slices = plan.dw_slices;
         T *out = static_cast<T *>(d_weight) + first * c.dim;
         e.out = out, e.factor = factor, e.out_scale = -1.0f / g_scale;
@@ -977,7 +1074,7 @@ int check(const char *name, const Call &c)
 {
     BMTK_REQUIRE(c.rows > 0 && c.vocab > 0 && c.dim > 0, "%s: sizes must be positive", name);
     BMTK_REQUIRE(c.dtype >= 0 && c.dtype <= 2, "%s: unknown type %d", name, c.dtype);
-    BMTK_REQUIRE(c.rows < (1 << 24), "%s: rows must be below 2^24", name);
+    BMTK_REQUIRE(c.rows < (1 << 22), "%s: rows must be below 2^22", name);
     BMTK_REQUIRE(c.vocab < (1 << 28), "%s: vocab must be below 2^28", name);
     BMTK_REQUIRE(c.dim <= 65536, "%s: up to 65,536 channels", name);
     // (offsets within a tile of 256 rows and launches of one dimension are in 32 bits)

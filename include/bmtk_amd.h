@@ -801,7 +801,7 @@ int bmtk_selective_scan_bwd(int64_t n_steps, int64_t batch, int32_t dim, int32_t
  * the token is `ignore`, NaN where it lies outside 0 .. vocab - 1), peak = the largest logit, total = the sum of e^(l - peak).  The logits are not kept.
  * weight: vocab rows, weight_stride numbers apart.  Rows whose logits hold NaN or +inf have lse and logp NaN.  Sums are in 32 bits; fp32 operands are taken as three
  * bf16 parts each, six of their products (a row that meets an fp32 operand that is not finite is NaN).
- * Limits: rows < 2^24, vocab < 2^28, dim up to 65,536, strides below 2^21. */
+ * Limits: rows < 2^22, vocab < 2^28, dim up to 65,536, strides below 2^21. */
 int64_t bmtk_projected_logprobs_workspace_bytes(int64_t rows, int32_t vocab, int32_t dim, int32_t dtype, const void *x, int64_t x_stride, const void *weight,
                                                 int64_t weight_stride, int32_t backward);
 int bmtk_projected_logprobs_fwd(int64_t rows, int32_t vocab, int32_t dim, int32_t dtype, const void *x, int64_t x_stride, const void *weight, int64_t weight_stride,
