@@ -89,19 +89,6 @@ __device__ __forceinline__ float2 join(float2 u, float2 v)
     return make_float2(m, u.y * __builtin_amdgcn_exp2f(u.x - from) + v.y * __builtin_amdgcn_exp2f(v.x - from));
 }
 
-// the order of a stretch of code: beside each of N products their share of R LDS reads and of L loads to LDS
-template <int N, int R, int L, int At>
-__device__ __forceinline__ void beside()
-{
-    if constexpr (At < N) {
-        __builtin_amdgcn_sched_group_barrier(0x008, 1, 0);
-        constexpr int r = R * (At + 1) / N - R * At / N, l = L * (At + 1) / N - L * At / N;
-        if constexpr (r > 0) __builtin_amdgcn_sched_group_barrier(0x100, r, 0);
-        if constexpr (l > 0) __builtin_amdgcn_sched_group_barrier(0x020, l, 0);
-        beside<N, R, L, At + 1>();
-    }
-}
-
 // four numbers to where they begin anywhere
 template <typename T>
 __device__ __forceinline__ void put4(T *p, const Acc4 &v)
@@ -207,7 +194,7 @@ struct Operand {
         const int64_t records = left - skip;
         const uintptr_t p = reinterpret_cast<uintptr_t>(at + which * s.part + skip);
         const Words rsrc = {(uint32_t)p, (uint32_t)(p >> 32), (uint32_t)(records < 0xfffffff0ll ? records : 0xfffffff0ll), 0x00020000u};
-        asm volatile("s_mov_b32 m0, %0\n\ts_nop 4\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds + (wave * kLoads + n) * 1024), "v"(from[n % kVary] + n * each), "s"(rsrc) : "memory");
+        asm volatile("s_mov_b32 m0, %0\n\ts_nop 3\n\tbuffer_load_dwordx4 %1, %2, 0 offen lds" ::"s"(lds + (wave * kLoads + n) * 1024), "v"(from[n % kVary] + n * each), "s"(rsrc) : "memory");
 #endif
     }
     // the fragment of 32 rows from `row` (a multiple of 32) on, sixteen k from s * 16 on
@@ -329,45 +316,35 @@ __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void product_kernel(Product p)
     };
     Acc acc[W][W];
     typename Vec<E>::V8 fa[4][W], fb[4][W];
-    const auto take_a = [&](int k, const char *from) {
-#pragma unroll
-        for (int i = 0; i < W; ++i) fa[k][i] = a.fragment(from, (wi * W + i) * kTile, k, lane);
+    // A step is kSlots products of 32 x 32 x 16, a quarter of them for each sixteen k.  Beside them go, one at a time, the reads of the fragments of the other quarters,
+    // which are done when kMiddle slots are; then everybody has read this stage, the next one has come, and the tile after it is asked for into this one, beside the
+    // reads of the next stage's first fragments.  The order is given: the compiler would read all at once.
+    static_assert(kDepth == 64, "four quarters");
+    constexpr int kSlots = 4 * W * W, kMiddle = kSlots * 5 / 8, kPerQuarter = 2 * W;
+    const auto read = [&](int f, const char *from) {   // fragment f of a step: a's first, then those of b, then the others of a
+        const int k = f / kPerQuarter, n = f % kPerQuarter;
+        if (n >= 1 && n <= W) fb[k][n - 1] = b.fragment(from + OpA::kBytes, (wj * W + n - 1) * kTile, k, lane);
+        else fa[k][n ? n - W : 0] = a.fragment(from, (wi * W + (n ? n - W : 0)) * kTile, k, lane);
     };
-    const auto take_b = [&](int k, const char *from) {
-#pragma unroll
-        for (int j = 0; j < W; ++j) fb[k][j] = b.fragment(from + OpA::kBytes, (wj * W + j) * kTile, k, lane);
+    const auto product = [&](int slot) {
+        const int k = slot / (W * W), i = slot % (W * W) / W, j = slot % W;
+        acc[i][j] = Vec<E>::mfma(fa[k][i], fb[k][j], acc[i][j]);
     };
-    // products of half a quarter
-    const auto multiply = [&](int k, int h) {
+    const auto up_to_the_middle = [&](const char *now) {
+        constexpr int kReads = 3 * kPerQuarter, kOver = kMiddle - kMiddle / 10;
 #pragma unroll
-        for (int i = h * W / 2; i < (h + 1) * W / 2; ++i)
+        for (int slot = 0; slot < kMiddle; ++slot) {
+            product(slot);
 #pragma unroll
-            for (int j = 0; j < W; ++j) acc[i][j] = Vec<E>::mfma(fa[k][i], fb[k][j], acc[i][j]);
+            for (int f = kReads * min(slot, kOver) / kOver; f < kReads * min(slot + 1, kOver) / kOver; ++f) read(kPerQuarter + f, now);
+            __builtin_amdgcn_sched_barrier(0);
+        }
     };
-    // beside each of `products` products `reads` LDS reads in all, spread evenly, and `loads` loads to LDS in all
-    constexpr int kReadsA = W * (AK ? 2 : 1), kReadsB = W * (BK ? 2 : 1), kHalf = W * W / 2;
-    const auto in_turn = [&](auto products, auto reads, auto loads) {
-        constexpr int n = decltype(products)::value, r = decltype(reads)::value, l = decltype(loads)::value;
-        beside<n, r, l, 0>();
-        __builtin_amdgcn_sched_barrier(0);
-    };
-#define BMTK_N(v) std::integral_constant<int, (v)>()
-    // the products of the first two quarters, and the fragments of the others
-    const auto first_half = [&](const char *now) {
-        take_a(1, now);
-        take_b(1, now);
-        multiply(0, 0);
-        in_turn(BMTK_N(kHalf), BMTK_N(kReadsA + kReadsB), BMTK_N(0));
-        take_a(2, now);
-        multiply(0, 1);
-        in_turn(BMTK_N(kHalf / 2), BMTK_N(kReadsA), BMTK_N(0));
-        take_b(2, now);
-        take_a(3, now);
-        multiply(1, 0);
-        in_turn(BMTK_N(kHalf), BMTK_N(kReadsA + kReadsB), BMTK_N(0));
-        take_b(3, now);
-        multiply(1, 1);
-        in_turn(BMTK_N(kHalf / 2), BMTK_N(kReadsB), BMTK_N(0));
+    const auto everybody = [&]() {
+        __builtin_amdgcn_s_waitcnt(kWaitAll);
+        asm volatile("" ::: "memory");
+        __builtin_amdgcn_s_barrier();
+        asm volatile("" ::: "memory");
     };
 
     if ((int32_t)blockIdx.x >= jobs) return;
@@ -381,49 +358,33 @@ __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void product_kernel(Product p)
             for (int j = 0; j < W; ++j)
 #pragma unroll
                 for (int r = 0; r < 16; ++r) acc[i][j][r] = 0.0f;
-        // Two stages in LDS, a step's products in quarters.  A step's fragments are all in registers well before its products are done, so that from the middle of
-        // the third quarter on the tile after the next is asked for into the same stage: it has the time of a step's products to come.
-        static_assert(kDepth == 64, "four quarters");
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_barrier();
         asm volatile("" ::: "memory");
-        take_a(0, lds);
-        take_b(0, lds);
+#pragma unroll
+        for (int f = 0; f < kPerQuarter; ++f) read(f, lds);
         int32_t s = s0;
         for (; s + 1 < s1; ++s) {
-            char *now = lds + ((s - s0) & 1) * kStage, *next = lds + ((s - s0 + 1) & 1) * kStage;
-            first_half(now);
-            multiply(2, 0);
-            in_turn(BMTK_N(kHalf), BMTK_N(0), BMTK_N(0));
-            __builtin_amdgcn_s_waitcnt(kWaitAll);
-            asm volatile("" ::: "memory");
-            __builtin_amdgcn_s_barrier();
-            asm volatile("" ::: "memory");
+            const int stage = (s - s0) & 1;
+            up_to_the_middle(lds + stage * kStage);
+            everybody();
+            constexpr int kLoadsOver = (kSlots - kMiddle) * 2 / 3, kFirst = kMiddle + 2;
 #pragma unroll
-            for (int i = W / 2; i < W; ++i)
+            for (int slot = kMiddle; slot < kSlots; ++slot) {
+                product(slot);
+                const int n = slot - kMiddle, r = slot - kFirst;
 #pragma unroll
-                for (int j = 0; j < W; ++j) {
-                    acc[i][j] = Vec<E>::mfma(fa[2][i], fb[2][j], acc[i][j]);
-                    constexpr int kEach = kLoads / kHalf;
+                for (int l = kLoads * min(n, kLoadsOver) / kLoadsOver; l < kLoads * min(n + 1, kLoadsOver) / kLoadsOver; ++l) fetch_one(l, stage);
+                constexpr int kReadsOver = kSlots - kFirst - kSlots / 16;
+                if (r >= 0)
 #pragma unroll
-                    for (int n = 0; n < kEach; ++n) fetch_one(((i - W / 2) * W + j) * kEach + n, (s - s0) & 1);
-                    __builtin_amdgcn_sched_barrier(0);
-                }
+                    for (int f = kPerQuarter * min(r, kReadsOver) / kReadsOver; f < kPerQuarter * min(r + 1, kReadsOver) / kReadsOver; ++f) read(f, lds + (stage ^ 1) * kStage);
+                __builtin_amdgcn_sched_barrier(0);
+            }
             fetch_next();
-            take_a(0, next);
-            take_b(0, next);
-            multiply(3, 0);
-            in_turn(BMTK_N(kHalf), BMTK_N(kReadsA + kReadsB), BMTK_N(0));
-            multiply(3, 1);
-            in_turn(BMTK_N(kHalf), BMTK_N(0), BMTK_N(0));
         }
-        const char *now = lds + ((s - s0) & 1) * kStage;
-        first_half(now);
-        // (what was asked for behind the last step has come, and everybody has read what there was)
-        __builtin_amdgcn_s_waitcnt(kWaitAll);
-        asm volatile("" ::: "memory");
-        __builtin_amdgcn_s_barrier();
-        asm volatile("" ::: "memory");
+        up_to_the_middle(lds + ((s - s0) & 1) * kStage);
+        everybody();   // (what was asked for behind the last step has come, too)
         // what the results will be asked for, of this lane's column of each tile: before the next tile's loads, so that it is not waited for behind them
         int64_t token[W];
         float peak[W], total[W];
@@ -436,10 +397,8 @@ __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void product_kernel(Product p)
             }
         }
         if (job + (int32_t)gridDim.x < jobs) begin(job + gridDim.x);
-        multiply(2, 0);
-        multiply(2, 1);
-        multiply(3, 0);
-        multiply(3, 1);
+#pragma unroll
+        for (int slot = kMiddle; slot < kSlots; ++slot) product(slot);
         __builtin_amdgcn_sched_barrier(0);
 
         // lane l has column j = l % 32 of a tile and its rows i = 8 (r / 4) + 4 (l / 32) + r % 4
@@ -592,7 +551,6 @@ __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void product_kernel(Product p)
         asm volatile("" ::: "memory");
         __builtin_amdgcn_s_waitcnt(kWaitLoads | kMayWait % 16 | kMayWait / 16 << 14);
     }
-#undef BMTK_N
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
