@@ -38,6 +38,16 @@ struct Vec<f16> {
     static __device__ __forceinline__ Acc4 mfma16(V8 a, V8 b, Acc4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 };
 
+// what a type's products are made of
+template <typename T>
+struct Element {
+    typedef T type;
+};
+template <>
+struct Element<float> {
+    typedef bf16 type;
+};
+
 // eight numbers from where they begin anywhere
 template <typename T>
 struct Loose8 {
@@ -57,6 +67,27 @@ struct Loose8 {
     {
 #pragma unroll
         for (int i = 0; i < 8; ++i) v[i] = i < n ? p[i] : (T)0.0f;
+    }
+};
+
+// four numbers, `some` of them there, the others 0
+template <typename T>
+struct Loose4 {
+    typedef uint32_t Words __attribute__((ext_vector_type(sizeof(T))));
+    typedef Words Loose __attribute__((aligned(2)));
+    union {
+        Words w;
+        T v[4];
+    };
+    __device__ __forceinline__ Loose4() {}
+    __device__ __forceinline__ void load(const T *p, int some)
+    {
+        if (some >= 4) {
+            w = *reinterpret_cast<const Loose *>(p);
+        } else {
+#pragma unroll
+            for (int q = 0; q < 4; ++q) v[q] = q < some ? p[q] : (T)0.0f;
+        }
     }
 };
 
@@ -81,6 +112,8 @@ __device__ __forceinline__ int part_b(int combination) { return 0x021010 >> comb
 // in the exponent once, and what log2 e itself is off by is the same in the logit of a token.
 __device__ __forceinline__ float base_of(float m) { return rintf(m * (kLog2e * 8.0f)) * 0.125f; }
 __device__ __forceinline__ float exp_over(float v, float base) { return __builtin_amdgcn_exp2f(fmaf(v, kLog2e, -base)); }
+
+__device__ __forceinline__ int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
 
 // bases and sums over them, joined; -inf: nothing yet
 __device__ __forceinline__ float2 join(float2 u, float2 v)
@@ -117,6 +150,7 @@ struct Source {
 struct Product {
     Source a, b;
     int32_t ni, nj;                               // sizes
+    int32_t tail;                                 // k of the last step that b's rows have; what lies behind them is not theirs
     int32_t steps, combinations;                  // steps of kDepth in k; 1 or 6
     int32_t tiles_i, tiles_j, slices;             // slices: parts of the steps, each to a slab of its own
     // kStats, kGradient: i is the vocabulary from first on, j the rows
@@ -330,10 +364,17 @@ __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void product_kernel(Product p)
         const int k = slot / (W * W), i = slot % (W * W) / W, j = slot % W;
         acc[i][j] = Vec<E>::mfma(fa[k][i], fb[k][j], acc[i][j]);
     };
-    const auto up_to_the_middle = [&](const char *now) {
+    const auto cut_fragments = [&](int k) {   // b's numbers behind its rows, in the last step
+        if (Mode == kSlab || Mode == kOut || p.tail == kDepth) return;
+#pragma unroll
+        for (int j = 0; j < W; ++j)
+            if (k * 16 + lane / 32 * 8 >= p.tail) fb[k][j] = typename Vec<E>::V8{};
+    };
+    const auto up_to_the_middle = [&](const char *now, bool last) {
         constexpr int kReads = 3 * kPerQuarter, kOver = kMiddle - kMiddle / 10;
 #pragma unroll
         for (int slot = 0; slot < kMiddle; ++slot) {
+            if (last && slot % (W * W) == 0) cut_fragments(slot / (W * W));
             product(slot);
 #pragma unroll
             for (int f = kReads * min(slot, kOver) / kOver; f < kReads * min(slot + 1, kOver) / kOver; ++f) read(kPerQuarter + f, now);
@@ -366,7 +407,7 @@ __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void product_kernel(Product p)
         int32_t s = s0;
         for (; s + 1 < s1; ++s) {
             const int stage = (s - s0) & 1;
-            up_to_the_middle(lds + stage * kStage);
+            up_to_the_middle(lds + stage * kStage, false);
             everybody();
             constexpr int kLoadsOver = (kSlots - kMiddle) * 2 / 3, kFirst = kMiddle + 2;
 #pragma unroll
@@ -383,7 +424,7 @@ __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void product_kernel(Product p)
             }
             fetch_next();
         }
-        up_to_the_middle(lds + ((s - s0) & 1) * kStage);
+        up_to_the_middle(lds + ((s - s0) & 1) * kStage, true);
         everybody();   // (what was asked for behind the last step has come, too)
         // what the results will be asked for, of this lane's column of each tile: before the next tile's loads, so that it is not waited for behind them
         int64_t token[W];
@@ -398,7 +439,10 @@ __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void product_kernel(Product p)
         }
         if (job + (int32_t)gridDim.x < jobs) begin(job + gridDim.x);
 #pragma unroll
-        for (int slot = kMiddle; slot < kSlots; ++slot) product(slot);
+        for (int slot = kMiddle; slot < kSlots; ++slot) {
+            if (slot % (W * W) == 0) cut_fragments(slot / (W * W));
+            product(slot);
+        }
         __builtin_amdgcn_sched_barrier(0);
 
         // lane l has column j = l % 32 of a tile and its rows i = 8 (r / 4) + 4 (l / 32) + r % 4
@@ -596,9 +640,19 @@ __global__ __launch_bounds__(1024) void weigh_kernel(const float *d_logp, const 
     __shared__ float most[16];
     float c = 1.0f;
     if (normal) {
+        // (every workgroup looks at all rows, eight at a time)
         float m = 0.0f;
-        for (int64_t r = threadIdx.x; r < rows; r += 1024)
-            if (tokens[r] != ignore && fabsf(d_logp[r]) < INFINITY) m = fmaxf(m, fabsf(d_logp[r]));
+        for (int64_t r = threadIdx.x; r < rows; r += 8 * 1024) {
+            float d[8];
+            int64_t t[8];
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const int64_t at = r + i * 1024 < rows ? r + i * 1024 : r;
+                d[i] = fabsf(d_logp[at]), t[i] = tokens[at];
+            }
+#pragma unroll
+            for (int i = 0; i < 8; ++i) m = t[i] != ignore && d[i] < INFINITY ? fmaxf(m, d[i]) : m;
+        }
 #pragma unroll
         for (int k = 32; k; k >>= 1) m = fmaxf(m, __shfl_xor(m, k));
         if (lane_id() == 0) most[threadIdx.x / kWave] = m;
@@ -609,11 +663,24 @@ __global__ __launch_bounds__(1024) void weigh_kernel(const float *d_logp, const 
         const int e = m > 0.0f ? min(max((int)(__float_as_uint(m) >> 23) - 127, -120), 120) : 0;
         c = __uint_as_float((uint32_t)(e + 127) << 23);
     }
-    if (threadIdx.x == 0) *factor = c;
-    for (int64_t r = threadIdx.x; r < rows; r += 1024) {
+    if (blockIdx.x == 0 && threadIdx.x == 0) *factor = c;
+    const int64_t r = (int64_t)blockIdx.x * 1024 + threadIdx.x;
+    if (r < rows) {
         const int64_t token = tokens[r];
         weights[r] = token == ignore ? 0.0f : token < 0 || token >= vocab ? NAN : d_logp[r] / c;
     }
+}
+
+// a row's results from its base and sum
+__device__ __forceinline__ void finish(float2 sum, int32_t row, const float *label, const int64_t *tokens, int64_t ignore, int32_t vocab, float *logp, float *lse, float *peak, float *total)
+{
+    const float m = sum.x, s = sum.y, log_total = logf(s);
+    const float l = m == -INFINITY && s == 0.0f ? -INFINITY : fmaf(m, kLn2, log_total);
+    const int64_t token = tokens[row];
+    peak[row] = m;
+    total[row] = s;
+    lse[row] = m == INFINITY ? NAN : l;
+    logp[row] = token == ignore ? 0.0f : token < 0 || token >= vocab || m == INFINITY ? NAN : l == -INFINITY ? -INFINITY : fmaf(fmaf(label[row], kLog2e, -m), kLn2, -log_total);
 }
 
 // each row's tiles joined: a workgroup takes 64 rows, each of its 16 wavefronts every sixteenth tile
@@ -638,30 +705,48 @@ __global__ __launch_bounds__(1024) void stats_join_kernel(const float2 *stats, i
     __syncthreads();
     if (wave != 0 || row >= rows) return;
     for (int k = 1; k < 16; ++k) sum = join(sum, parts[k][lane]);
-    const float m = sum.x, s = sum.y;
-    const float log_total = logf(s);
-    const float l = m == -INFINITY && s == 0.0f ? -INFINITY : fmaf(m, kLn2, log_total);
-    const int64_t token = tokens[row];
-    peak[row] = m;
-    total[row] = s;
-    lse[row] = m == INFINITY ? NAN : l;
-    logp[row] = token == ignore ? 0.0f : token < 0 || token >= vocab || m == INFINITY ? NAN : l == -INFINITY ? -INFINITY : fmaf(fmaf(label[row], kLog2e, -m), kLn2, -log_total);
+    finish(sum, row, label, tokens, ignore, vocab, logp, lse, peak, total);
 }
-
-// results from their slabs: rows of `width` numbers, n of them there
+// Results from their slabs: rows of `width` numbers, n of them there.  `ways` wavefronts of a workgroup share 64 times four numbers, each takes every so manieth slab.
 template <typename T>
-__global__ __launch_bounds__(256) void slab_join_kernel(const float *slab, int32_t slabs, int64_t slab_size, int64_t rows, int32_t n, int32_t width, const float *by, const float *factor,
-                                                        float scale, T *out)
+__global__ __launch_bounds__(1024) void slab_join_kernel(const float *slab, int32_t slabs, int64_t slab_size, int64_t rows, int32_t n, int32_t width, int32_t ways, const float *by,
+                                                         const float *factor, float scale, T *out)
 {
-    const int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x, row = k / (width / 4);
+    __shared__ Acc4 parts[16][64];
+    const int wave = threadIdx.x / kWave, lane = lane_id(), way = wave % ways;
+    const int64_t k = ((int64_t)blockIdx.x * (blockDim.x / kWave / ways) + wave / ways) * 64 + lane, row = k / (width / 4);
     const int32_t c = (int32_t)(k - row * (width / 4)) * 4;
-    if (row >= rows || c >= n) return;
-    Acc4 v = *reinterpret_cast<const Acc4 *>(slab + row * width + c);
-    for (int i = 1; i < slabs; ++i) v += *reinterpret_cast<const Acc4 *>(slab + i * slab_size + row * width + c);
-    const float w = by ? by[row] : 1.0f, f = scale * (factor ? *factor : 1.0f) * w;
+    const bool there = row < rows && c < n;
+    Acc4 v = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (there) {
+        const float *p = slab + row * width + c;
+        int32_t i = way;
+        for (; i + 3 * ways < slabs; i += 4 * ways) {
+            Acc4 q[4];
 #pragma unroll
-    for (int r = 0; r < 4; ++r)
-        if (c + r < n) out[row * n + c + r] = (T)(w == 0.0f ? 0.0f : v[r] * f);
+            for (int u = 0; u < 4; ++u) q[u] = *reinterpret_cast<const Acc4 *>(p + (i + u * ways) * slab_size);
+#pragma unroll
+            for (int u = 0; u < 4; ++u) v += q[u];
+        }
+        for (; i < slabs; i += ways) v += *reinterpret_cast<const Acc4 *>(p + i * slab_size);
+    }
+    if (ways > 1) {
+        parts[wave][lane] = v;
+        __syncthreads();
+        if (way != 0) return;
+        for (int w = 1; w < ways; ++w) v += parts[wave + w][lane];
+    }
+    if (!there) return;
+    const float w = by ? by[row] : 1.0f, f = scale * (factor ? *factor : 1.0f) * w;
+    const Acc4 r = {w == 0.0f ? 0.0f : v[0] * f, w == 0.0f ? 0.0f : v[1] * f, w == 0.0f ? 0.0f : v[2] * f, w == 0.0f ? 0.0f : v[3] * f};
+    T *to = out + row * n + c;
+    if (c + 4 <= n) {
+        put4<T>(to, r);
+    } else {
+#pragma unroll
+        for (int q = 0; q < 3; ++q)
+            if (c + q < n) to[q] = (T)r[q];
+    }
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -675,16 +760,26 @@ struct Few {
     int32_t rows, vocab, dim;
     float2 *stats;
     float *label;
+    // backward
+    const float *peak, *total, *weights;   // weights: see weigh_kernel
+    int64_t ignore;
+    float *g;                              // [vocab, to a whole 128][rows, to a whole 16]: p - delta
+    void *d_weight;
+    float *slab;                           // [slices][rows][dim, to a whole 8]
+    int32_t slices, slice_rows;            // slices of the vocabulary, of so many of its rows (a multiple of 16)
 };
 
-template <typename T, typename E, int J>
-__global__ __launch_bounds__(256) void few_rows_kernel(Few a)
+// Split: wavefronts of a workgroup that share 32 rows of the weights, each a part of the channels.
+template <typename T, int J, int Split, bool Gradient>
+__global__ __launch_bounds__(Split == 8 ? 512 : 256) void few_rows_kernel(Few a)
 {
-    constexpr bool kParts = std::is_same<T, float>::value;
+    typedef typename Element<T>::type E;
     typedef typename Vec<E>::V8 V8;
-    __shared__ float2 parts[4][J * 16];
+    constexpr int kBlocks = Split == 1 ? 4 : 1;   // of 32 rows
+    __shared__ float2 parts[kBlocks][J * 16];
+    __shared__ Acc4 sums[Split == 1 ? 1 : Split - 1][2][J][64];
     const int lane = lane_id(), wave = threadIdx.x / kWave, r16 = lane & 15, quarter = lane >> 4;
-    const int32_t v0 = (blockIdx.x * 4 + wave) * 32;
+    const int32_t v0 = (blockIdx.x * kBlocks + (Split == 1 ? wave : 0)) * 32;
     const T *w_row[2], *x_row[J];
 #pragma unroll
     for (int i = 0; i < 2; ++i) w_row[i] = static_cast<const T *>(a.weight) + (int64_t)min(v0 + i * 16 + r16, a.vocab - 1) * a.w_stride + quarter * 8;
@@ -696,28 +791,14 @@ __global__ __launch_bounds__(256) void few_rows_kernel(Few a)
 #pragma unroll
         for (int j = 0; j < J; ++j) acc[i][j] = Acc4{0.0f, 0.0f, 0.0f, 0.0f};
     const auto multiply = [&](const Loose8<T> (&w)[2], const Loose8<T> (&x)[J]) {
-        if constexpr (kParts) {
-            V8 wp[2][3], xp[J][3];
-            const auto parts_of = [&](const Loose8<T> &from, V8 (&to)[3]) {
+        if constexpr (std::is_same<T, float>::value) {
+            // (fp32 operands in fp32 instructions, one k of a lane's eight each: at so few rows they keep up with memory)
 #pragma unroll
-                for (int k = 0; k < 8; ++k) {
-                    bf16 s[3];
-                    split(from.v[k], s);
-#pragma unroll
-                    for (int i = 0; i < 3; ++i) to[i][k] = s[i];
-                }
-            };
-#pragma unroll
-            for (int i = 0; i < 2; ++i) parts_of(w[i], wp[i]);
-#pragma unroll
-            for (int j = 0; j < J; ++j) parts_of(x[j], xp[j]);
-            constexpr int pa[6] = {0, 0, 1, 1, 0, 2}, pb[6] = {0, 1, 0, 1, 2, 0};
-#pragma unroll
-            for (int c = 0; c < 6; ++c)
+            for (int k = 0; k < 8; ++k)
 #pragma unroll
                 for (int i = 0; i < 2; ++i)
 #pragma unroll
-                    for (int j = 0; j < J; ++j) acc[i][j] = Vec<E>::mfma16(wp[i][pa[c]], xp[j][pb[c]], acc[i][j]);
+                    for (int j = 0; j < J; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[i].v[k], x[j].v[k], acc[i][j], 0, 0, 0);
         } else {
             V8 wv[2], xv[J];
 #pragma unroll
@@ -730,11 +811,10 @@ __global__ __launch_bounds__(256) void few_rows_kernel(Few a)
                 for (int j = 0; j < J; ++j) acc[i][j] = Vec<E>::mfma16(wv[i], xv[j], acc[i][j]);
         }
     };
-    constexpr int kAhead = kParts ? 2 : 4;   // steps of 32 k that are asked for at once
-    const int32_t whole = a.dim / 32;
-    int32_t k = 0;
-    for (; k + kAhead <= whole; k += kAhead) {
-        Loose8<T> w[kAhead][2], x[kAhead][J];
+    constexpr int kAhead = (std::is_same<T, float>::value ? 2 : 4) / (J == 4 ? 2 : 1);   // steps of 32 k that are asked for at once
+    const int32_t steps = (a.dim + 31) / 32, part = Split == 1 ? 0 : wave;
+    const int32_t first = steps * part / Split, end = steps * (part + 1) / Split, whole = min(end, a.dim / 32);
+    const auto ask = [&](int32_t k, Loose8<T> (&w)[kAhead][2], Loose8<T> (&x)[kAhead][J]) {
 #pragma unroll
         for (int u = 0; u < kAhead; ++u) {
 #pragma unroll
@@ -742,10 +822,26 @@ __global__ __launch_bounds__(256) void few_rows_kernel(Few a)
 #pragma unroll
             for (int j = 0; j < J; ++j) x[u][j].load(x_row[j] + (k + u) * 32);
         }
+    };
+    int32_t k = first;
+    if (k + kAhead <= whole) {
+        Loose8<T> w_next[kAhead][2], x_next[kAhead][J];
+        ask(k, w_next, x_next);
+        for (; k + kAhead <= whole; k += kAhead) {
+            Loose8<T> w[kAhead][2], x[kAhead][J];
 #pragma unroll
-        for (int u = 0; u < kAhead; ++u) multiply(w[u], x[u]);
+            for (int u = 0; u < kAhead; ++u) {
+#pragma unroll
+                for (int i = 0; i < 2; ++i) w[u][i] = w_next[u][i];
+#pragma unroll
+                for (int j = 0; j < J; ++j) x[u][j] = x_next[u][j];
+            }
+            if (k + 2 * kAhead <= whole) ask(k + kAhead, w_next, x_next);
+#pragma unroll
+            for (int u = 0; u < kAhead; ++u) multiply(w[u], x[u]);
+        }
     }
-    for (; k * 32 < a.dim; ++k) {
+    for (; k < end; ++k) {
         Loose8<T> w[2], x[J];
         const int n = a.dim - k * 32 - quarter * 8;
 #pragma unroll
@@ -754,11 +850,39 @@ __global__ __launch_bounds__(256) void few_rows_kernel(Few a)
         for (int j = 0; j < J; ++j) x[j].load_some(x_row[j] + k * 32, n);
         multiply(w, x);
     }
+    if constexpr (Split > 1) {
+        if (wave > 0) {
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < J; ++j) sums[wave - 1][i][j][lane] = acc[i][j];
+        }
+        __syncthreads();
+        if (wave > 0) return;
+        for (int w = 0; w < Split - 1; ++w)
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int j = 0; j < J; ++j) acc[i][j] += sums[w][i][j][lane];
+    }
     // lane l has column j = l % 16 of a tile and its rows i = 4 (l / 16) + r
 #pragma unroll
     for (int j = 0; j < J; ++j) {
         const int32_t row = j * 16 + r16;
         const int64_t token = row < a.rows ? a.tokens[row] : -1;
+        if constexpr (Gradient) {
+            const float peak = row < a.rows ? a.peak[row] : -INFINITY, inverse = row < a.rows ? 1.0f / a.total[row] : 0.0f;
+            const bool none = row >= a.rows || token == a.ignore || peak == -INFINITY;
+#pragma unroll
+            for (int i = 0; i < 2; ++i)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int32_t v = v0 + i * 16 + quarter * 4 + r;
+                    const float p = exp_over(acc[i][j][r], peak) * inverse;
+                    a.g[(int64_t)v * (J * 16) + row] = none || v >= a.vocab ? 0.0f : v == token ? p - 1.0f : p;
+                }
+            continue;
+        }
         float m = -INFINITY;
 #pragma unroll
         for (int i = 0; i < 2; ++i)
@@ -779,20 +903,129 @@ __global__ __launch_bounds__(256) void few_rows_kernel(Few a)
             for (int r = 0; r < 4; ++r) s += exp_over(acc[i][j][r], from);
         s += __shfl_xor(s, 16);
         s += __shfl_xor(s, 32);
-        if (quarter == 0) parts[wave][row] = make_float2(base, s);
+        if (Split > 1 && quarter == 0 && row < a.rows) a.stats[(int64_t)blockIdx.x * a.rows + row] = make_float2(base, s);
+        if (Split == 1 && quarter == 0) parts[wave][row] = make_float2(base, s);
     }
+    if constexpr (Gradient || Split > 1) return;
     __syncthreads();
     if ((int)threadIdx.x < a.rows) {
         float2 sum = parts[0][threadIdx.x];
 #pragma unroll
-        for (int w = 1; w < 4; ++w) sum = join(sum, parts[w][threadIdx.x]);
+        for (int w = 1; w < kBlocks; ++w) sum = join(sum, parts[w][threadIdx.x]);
         a.stats[(int64_t)blockIdx.x * a.rows + threadIdx.x] = sum;
     }
 }
 
+// The two products of G for few rows, in one pass over the weights: a wavefront takes 64 channels (a lane four) of a slice of the vocabulary, and per 16 of its rows
+//     dx[r][d] -= G[v][r] w[v][d]   and   d_weight[v][d] = -sum_r G[v][r] d_logp[r] x[r][d]
+// in matrix instructions of 32 bits, which take one k a lane: nothing has to be transposed, and a lane's four channels are four tiles.  Bound by memory: the weights
+// read, their gradient written.
+template <typename T, int J>
+__global__ __launch_bounds__(256) void few_back_kernel(Few a)
+{
+    typedef Loose4<T> In;
+    const int lane = lane_id(), wave = threadIdx.x / kWave, r16 = lane & 15, kk = lane >> 4;
+    const int32_t d = (blockIdx.x * 4 + wave) * 64 + r16 * 4;
+    const int32_t some = a.dim - d;   // this lane's channels that are there, if fewer than four
+    if ((blockIdx.x * 4 + wave) * 64 >= a.dim) return;
+    // x d_logp, 4 kk + m of each 16 rows: what a lane's k is in product m
+    float xw[J][4][4];
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+        for (int m = 0; m < 4; ++m) {
+            const int32_t row = j * 16 + kk * 4 + m;
+            const float by = row < a.rows ? a.weights[row] : 0.0f;
+            In x;
+            x.load(static_cast<const T *>(a.x) + (int64_t)min(row, a.rows - 1) * a.x_stride + d, some);
+#pragma unroll
+            for (int q = 0; q < 4; ++q) xw[j][m][q] = by == 0.0f ? 0.0f : -by * (float)x.v[q];
+        }
+    Acc4 dx[J][4];
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) dx[j][q] = Acc4{0.0f, 0.0f, 0.0f, 0.0f};
+    const int32_t v_first = blockIdx.y * a.slice_rows, v_end = min(v_first + a.slice_rows, a.vocab);
+    const auto ask = [&](int32_t v, In (&w)[4]) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u) w[u].load(static_cast<const T *>(a.weight) + (int64_t)min(v + u * 4 + kk, a.vocab - 1) * a.w_stride + d, some);
+    };
+    In next[4];
+    ask(v_first, next);
+    for (int32_t v = v_first; v < v_end; v += 16) {
+        In w[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u) w[u] = next[u];
+        float by_row[J][4];
+        Acc4 by_vocab[J];
+#pragma unroll
+        for (int j = 0; j < J; ++j) {
+#pragma unroll
+            for (int u = 0; u < 4; ++u) by_row[j][u] = a.g[(int64_t)(v + u * 4 + kk) * (J * 16) + j * 16 + r16];
+            by_vocab[j] = *reinterpret_cast<const Acc4 *>(a.g + (int64_t)(v + r16) * (J * 16) + j * 16 + kk * 4);
+        }
+        if (v + 16 < v_end) ask(v + 16, next);
+        Acc4 dw[4];
+#pragma unroll
+        for (int q = 0; q < 4; ++q) dw[q] = Acc4{0.0f, 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < J; ++j)
+#pragma unroll
+            for (int m = 0; m < 4; ++m)
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    dx[j][q] = __builtin_amdgcn_mfma_f32_16x16x4f32(by_row[j][m], (float)w[m].v[q], dx[j][q], 0, 0, 0);
+                    dw[q] = __builtin_amdgcn_mfma_f32_16x16x4f32(by_vocab[j][m], xw[j][m][q], dw[q], 0, 0, 0);
+                }
+        // lane l has column l % 16, four channels, and its rows 4 (l / 16) + r
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int32_t at = v + kk * 4 + r;
+            if (at >= v_end || some <= 0) continue;
+            T *to = static_cast<T *>(a.d_weight) + (int64_t)at * a.dim + d;
+            const Acc4 out = {dw[0][r], dw[1][r], dw[2][r], dw[3][r]};
+            if (some >= 4) {
+                put4<T>(to, out);
+            } else {
+#pragma unroll
+                for (int q = 0; q < 3; ++q)
+                    if (q < some) to[q] = (T)out[q];
+            }
+        }
+    }
+    const int64_t width = up8(a.dim);
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+        for (int r = 0; r < 4; ++r) {
+            const int32_t row = j * 16 + kk * 4 + r;
+            if (row < a.rows && some > 0)
+                *reinterpret_cast<Acc4 *>(a.slab + ((int64_t)blockIdx.y * a.rows + row) * width + d) = Acc4{dx[j][0][r], dx[j][1][r], dx[j][2][r], dx[j][3][r]};
+        }
+}
+
+// the same of few rows: a workgroup to a row, its threads each every 256th tile
+__global__ __launch_bounds__(256) void few_join_kernel(const float2 *stats, int32_t tiles, int32_t rows, const float *label, const int64_t *tokens, int64_t ignore, int32_t vocab,
+                                                       float *logp, float *lse, float *peak, float *total)
+{
+    __shared__ float2 parts[4];
+    const int32_t row = blockIdx.x;
+    float2 sum = make_float2(-INFINITY, 0.0f);
+    for (int k = threadIdx.x; k < tiles; k += 256) sum = join(sum, stats[(int64_t)k * rows + row]);
+#pragma unroll
+    for (int k = 32; k; k >>= 1) sum = join(sum, make_float2(__shfl_xor(sum.x, k), __shfl_xor(sum.y, k)));
+    if (lane_id() == 0) parts[threadIdx.x / kWave] = sum;
+    __syncthreads();
+    if (threadIdx.x == 0) finish(join(join(parts[0], parts[1]), join(parts[2], parts[3])), row, label, tokens, ignore, vocab, logp, lse, peak, total);
+}
+
 // ---------------------------------------------------------------------------------------------------------------------
 
-constexpr int32_t kFewRows = 64;
+// Up to how many rows the kernels for few rows take.  us of 100,000 x 2,000, forward and both ways, few / large tiles: bf16 12 rows 112/148, 507/555; 17: 133/150, 618/556; 33:
+// 144/152, 857/560; 64: 170/152, 1003/564; fp32 12: 201/883, 787/2539; 64: 603/895, 1896/2565.  Large tiles of 16-bit weights whose rows do not
+// begin at whole 16 bytes copy them first, 170 us each way here.
+int32_t few_most(int32_t dtype, bool w_fits, bool backward) { return dtype == BMTK_F32 ? 64 : w_fits ? (backward ? 16 : 32) : (backward ? 32 : 64); }
 constexpr int64_t kPieceBytes = int64_t{512} << 20;   // of G: pieces of the vocabulary are as large as that allows
 
 int64_t up(int64_t n, int64_t to) { return div_up(n, to) * to; }
@@ -802,7 +1035,7 @@ int32_t tile_of(int64_t ni, int64_t nj, int64_t slices = 1) { return div_up(ni, 
 
 struct Plan {
     int32_t parts, combinations, depth;          // depth: dim to whole steps
-    bool copy_x, copy_w;                         // operands that are laid out anew
+    bool few, copy_x, copy_w;                    // the kernels for few rows; operands that are laid out anew
     int64_t piece, pieces, g_rows, g_width, out_width;
     int32_t dx_tile, dx_slices, dw_tile, dw_slices, logit_tile;
     int64_t x_copy, w_copy, x_weighted, g, dx_slab, dw_slab, stats, label, weights;   // bytes
@@ -811,7 +1044,8 @@ struct Plan {
         parts = dtype == BMTK_F32 ? 3 : 1;
         combinations = parts == 3 ? 6 : 1;
         depth = (int32_t)up(dim, kDepth);
-        copy_x = parts == 3 || !x_fits || dim % kDepth != 0;
+        few = rows <= few_most(dtype, w_fits, backward);
+        copy_x = parts == 3 || !x_fits;
         copy_w = parts == 3 || !w_fits;
         x_copy = w_copy = x_weighted = g = dx_slab = dw_slab = stats = label = weights = 0;
         pieces = 1, piece = vocab, g_rows = g_width = out_width = 0;
@@ -819,13 +1053,27 @@ struct Plan {
         if (!backward) {
             logit_tile = tile_of(vocab, rows);
             label = up(rows * 4, 256);
-            if (rows <= kFewRows) {
-                stats = up(div_up(vocab, 128) * rows * 8, 256);
+            if (few) {
+                stats = up(div_up(vocab, 32) * rows * 8, 256);
                 return;
             }
             stats = up(div_up(vocab, logit_tile) * rows * 8, 256);
             x_copy = copy_x ? up(parts * rows * depth * 2, 256) : 0;
             w_copy = copy_w ? up(parts * vocab * depth * 2, 256) : 0;
+            return;
+        }
+        out_width = up(dim, 8);
+        weights = up(rows * 4 + 4, 256);
+        if (few) {
+            // slices of the vocabulary, each with sums of its own for dx: as many workgroups as fill the chip some times, slabs of up to 64 MB
+            g = up(up(vocab, 128) * (rows <= 16 ? 16 : rows <= 32 ? 32 : 64) * 4, 256);
+            int64_t s = div_up(2048, div_up(dim, 256));
+            const int64_t most = (int64_t{64} << 20) / (rows * out_width * 4);
+            s = s > most ? most : s;
+            s = s < 1 ? 1 : s;
+            piece = up(div_up(vocab, s), 16);
+            dx_slices = (int32_t)div_up(vocab, piece);
+            dx_slab = up(dx_slices * rows * out_width * 4, 256);
             return;
         }
         x_copy = copy_x ? up(parts * rows * depth * 2, 256) : 0;
@@ -840,7 +1088,6 @@ struct Plan {
         g_width = piece;
         logit_tile = tile_of(piece < vocab ? piece : vocab, rows);
         g = up(parts * g_rows * g_width * 2, 256);
-        out_width = up(dim, 8);
         x_weighted = up(parts * up(rows, kDepth) * out_width * 2, 256);
         const auto slices_of = [](int64_t ni, int64_t nj, int64_t steps, int32_t &tile, int32_t &slices) {
             // the sum over k in as many parts as fill the chip, of eight steps at least
@@ -858,7 +1105,6 @@ struct Plan {
         slices_of(dim, columns, div_up(rows, kDepth) * combinations, dw_tile, dw_slices);
         dx_slab = up(dx_slices * rows * out_width * 4, 256);
         dw_slab = dw_slices > 1 ? up(dw_slices * columns * out_width * 4, 256) : 0;
-        weights = up(rows * 4 + 4, 256);
     }
     int64_t bytes() const { return x_copy + w_copy + x_weighted + g + dx_slab + dw_slab + stats + label + weights; }
 };
@@ -870,15 +1116,6 @@ bool sizes_fit(int64_t rows, int64_t vocab, int64_t dim, int32_t dtype)
 
 // whether rows can be read 16 bytes at a time
 bool fits(const void *p, int64_t stride, int32_t dim, int32_t dtype) { return dtype != BMTK_F32 && dim % 8 == 0 && aligned(p, 16) && stride % 8 == 0; }
-
-template <typename T>
-struct Element {
-    typedef T type;
-};
-template <>
-struct Element<float> {
-    typedef bf16 type;
-};
 
 template <typename E, typename T, bool AK, bool BK, int Mode>
 void multiply(Product &p, int32_t tile, hipStream_t s)
@@ -896,6 +1133,21 @@ void lay(const void *from, int64_t stride, int64_t rows, int32_t n, int64_t widt
 {
     typedef typename Element<T>::type E;
     lay_kernel<T, E><<<(uint32_t)div_up(padded_rows * width / 8, 256), 256, 0, s>>>(static_cast<const T *>(from), stride, rows, n, (int32_t)width, padded_rows, static_cast<E *>(to), by);
+}
+
+// Few rows of the weights leave the chip empty where a wavefront takes 32 of them: then a workgroup's wavefronts share them, four or eight.
+int32_t few_split(int64_t vocab) { return vocab >= 32 * 2048 ? 1 : vocab >= 32 * 512 ? 4 : 8; }
+int32_t few_tiles(int64_t vocab) { return (int32_t)div_up(vocab, few_split(vocab) == 1 ? 128 : 32); }
+
+template <typename T, int J, bool Gradient>
+void few_rows(const Few &f, hipStream_t s)
+{
+    const uint32_t tiles = (uint32_t)few_tiles(f.vocab);
+    switch (few_split(f.vocab)) {
+        case 1: few_rows_kernel<T, J, 1, Gradient><<<tiles, 256, 0, s>>>(f); break;
+        case 4: few_rows_kernel<T, J, 4, Gradient><<<tiles, 256, 0, s>>>(f); break;
+        default: few_rows_kernel<T, J, 8, Gradient><<<tiles, 512, 0, s>>>(f);
+    }
 }
 
 struct Call {
@@ -924,7 +1176,8 @@ Product logits(const Call &c, const Plan &plan, const char *x, const char *w, in
     Product p{};
     const int64_t w_stride = plan.copy_w ? plan.depth : c.w_stride, x_stride = plan.copy_x ? plan.depth : c.x_stride;
     p.a = by_numbers(w + first * w_stride * 2, w_stride, c.vocab * plan.depth, count, plan.copy_w ? plan.depth : c.dim);
-    p.b = by_numbers(x, x_stride, c.rows * plan.depth, c.rows, plan.depth);
+    p.b = by_numbers(x, x_stride, c.rows * plan.depth, c.rows, plan.copy_x ? plan.depth : c.dim);
+    p.tail = plan.copy_x ? kDepth : c.dim - (plan.depth - kDepth);
     p.ni = (int32_t)count, p.nj = (int32_t)c.rows;
     p.steps = plan.depth / kDepth, p.combinations = plan.combinations, p.slices = 1;
     p.first = (int32_t)first, p.vocab = (int32_t)c.vocab, p.tokens = c.tokens, p.ignore = c.ignore;
@@ -940,12 +1193,16 @@ void forward(Call c, float *logp, float *lse, float *peak, float *total)
     float2 *stats = reinterpret_cast<float2 *>(c.next(plan.stats));
     float *label = reinterpret_cast<float *>(c.next(plan.label));
     int32_t tiles;
-    if (c.rows <= kFewRows) {
-        Few f{c.x, c.weight, c.tokens, c.x_stride, c.w_stride, (int32_t)c.rows, (int32_t)c.vocab, c.dim, stats, label};
-        tiles = (int32_t)div_up(c.vocab, 128);
-        if (c.rows <= 16) few_rows_kernel<T, E, 1><<<tiles, 256, 0, c.stream>>>(f);
-        else if (c.rows <= 32) few_rows_kernel<T, E, 2><<<tiles, 256, 0, c.stream>>>(f);
-        else few_rows_kernel<T, E, 4><<<tiles, 256, 0, c.stream>>>(f);
+    if (plan.few) {
+        Few f{};
+        f.x = c.x, f.weight = c.weight, f.tokens = c.tokens, f.x_stride = c.x_stride, f.w_stride = c.w_stride, f.rows = (int32_t)c.rows, f.vocab = (int32_t)c.vocab, f.dim = c.dim;
+        f.stats = stats, f.label = label;
+        tiles = few_tiles(c.vocab);
+        if (c.rows <= 16) few_rows<T, 1, false>(f, c.stream);
+        else if (c.rows <= 32) few_rows<T, 2, false>(f, c.stream);
+        else few_rows<T, 4, false>(f, c.stream);
+        few_join_kernel<<<(uint32_t)c.rows, 256, 0, c.stream>>>(stats, tiles, (int32_t)c.rows, label, c.tokens, c.ignore, (int32_t)c.vocab, logp, lse, peak, total);
+        return;
     } else {
         const char *x = static_cast<const char *>(c.x), *w = static_cast<const char *>(c.weight);
         if (plan.copy_x) {
@@ -967,6 +1224,22 @@ void forward(Call c, float *logp, float *lse, float *peak, float *total)
 }
 
 template <typename T>
+void join_slabs(const float *slab, int32_t slabs, int64_t slab_size, int64_t rows, int32_t n, int64_t width, const float *by, const float *factor, float scale, void *out, hipStream_t s)
+{
+    const int32_t ways = slabs <= 4 ? 1 : slabs < 64 ? 4 : 16;
+    const uint32_t waves = ways == 16 ? 16 : 4;
+    slab_join_kernel<T><<<(uint32_t)div_up(rows * (width / 4), 64 * (waves / ways)), waves * kWave, 0, s>>>(slab, slabs, slab_size, rows, n, (int32_t)width, ways, by, factor, scale,
+                                                                                                          static_cast<T *>(out));
+}
+
+template <typename T, int J>
+void few_backward(const Few &f, hipStream_t s)
+{
+    few_rows<T, J, true>(f, s);
+    few_back_kernel<T, J><<<dim3((uint32_t)div_up(f.dim, 256), (uint32_t)f.slices), 256, 0, s>>>(f);
+}
+
+template <typename T>
 void backward(Call c, const float *peak, const float *total, const float *d_logp, void *dx, void *d_weight)
 {
     typedef typename Element<T>::type E;
@@ -978,7 +1251,18 @@ void backward(Call c, const float *peak, const float *total, const float *d_logp
     float *weights = reinterpret_cast<float *>(c.next(plan.weights)), *factor = weights + c.rows;
     char *g = c.next(plan.g), *x_weighted = c.next(plan.x_weighted);
     float *dx_slab = reinterpret_cast<float *>(c.next(plan.dx_slab)), *dw_slab = reinterpret_cast<float *>(c.next(plan.dw_slab));
-    weigh_kernel<<<1, 1024, 0, c.stream>>>(d_logp, c.tokens, c.ignore, c.rows, (int32_t)c.vocab, half, weights, factor);
+    weigh_kernel<<<(uint32_t)div_up(c.rows, 1024), 1024, 0, c.stream>>>(d_logp, c.tokens, c.ignore, c.rows, (int32_t)c.vocab, half && !plan.few, weights, factor);
+    if (plan.few) {
+        Few f{};
+        f.x = c.x, f.weight = c.weight, f.tokens = c.tokens, f.x_stride = c.x_stride, f.w_stride = c.w_stride, f.rows = (int32_t)c.rows, f.vocab = (int32_t)c.vocab, f.dim = c.dim;
+        f.peak = peak, f.total = total, f.weights = weights, f.ignore = c.ignore, f.g = reinterpret_cast<float *>(g), f.d_weight = d_weight, f.slab = dx_slab;
+        f.slices = plan.dx_slices, f.slice_rows = (int32_t)plan.piece;
+        if (c.rows <= 16) few_backward<T, 1>(f, c.stream);
+        else if (c.rows <= 32) few_backward<T, 2>(f, c.stream);
+        else few_backward<T, 4>(f, c.stream);
+        join_slabs<T>(dx_slab, plan.dx_slices, c.rows * plan.out_width, c.rows, c.dim, plan.out_width, weights, nullptr, -1.0f, dx, c.stream);
+        return;
+    }
     const char *x = static_cast<const char *>(c.x), *w = static_cast<const char *>(c.weight);
     if (plan.copy_x) {
         char *to = c.next(plan.x_copy);
@@ -1020,12 +1304,10 @@ void backward(Call c, const float *peak, const float *total, const float *d_logp
             multiply<E, T, true, true, kOut>(e, plan.dw_tile, c.stream);
         } else {
             multiply<E, T, true, true, kSlab>(e, plan.dw_tile, c.stream);
-            slab_join_kernel<T><<<(uint32_t)div_up(count * (plan.out_width / 4), 256), 256, 0, c.stream>>>(dw_slab, plan.dw_slices, e.slab_size, count, c.dim, (int32_t)plan.out_width, nullptr,
-                                                                                                         factor, e.out_scale, out);
+            join_slabs<T>(dw_slab, plan.dw_slices, e.slab_size, count, c.dim, plan.out_width, nullptr, factor, e.out_scale, out, c.stream);
         }
     }
-    slab_join_kernel<T><<<(uint32_t)div_up(c.rows * (plan.out_width / 4), 256), 256, 0, c.stream>>>(dx_slab, plan.dx_slices, c.rows * plan.out_width, c.rows, c.dim, (int32_t)plan.out_width,
-                                                                                                  weights, factor, -1.0f / g_scale, static_cast<T *>(dx));
+    join_slabs<T>(dx_slab, plan.dx_slices, c.rows * plan.out_width, c.rows, c.dim, plan.out_width, weights, factor, -1.0f / g_scale, dx, c.stream);
 }
 
 int check(const char *name, const Call &c)
