@@ -152,6 +152,7 @@ struct Product {
     int32_t ni, nj;                               // sizes
     int32_t tail;                                 // k of the last step that b's rows have; what lies behind them is not theirs
     int32_t steps, combinations;                  // steps of kDepth in k; 1 or 6
+    int32_t rotate;                               // whether the steps may be begun anywhere: all of them are taken, and none is cut
     int32_t tiles_i, tiles_j, slices;             // slices: parts of the steps, each to a slab of its own
     // kStats, kGradient: i is the vocabulary from first on, j the rows
     int32_t first, vocab;
@@ -330,7 +331,7 @@ __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void product_kernel(Product p)
     const auto fetch_next = [&]() {
         make_here();
         const bool more = combination + 1 < p.combinations;
-        step = min(more ? step : step + 1, p.steps - 1);   // (behind the last step it is asked for again, for nothing)
+        step = more ? step : step + 1 < p.steps ? step + 1 : 0;   // (behind the last one others are asked for, for nothing)
         combination = more ? combination + 1 : 0;
     };
     constexpr int kLoads = OpA::kLoads + OpB::kLoads;
@@ -338,6 +339,8 @@ __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void product_kernel(Product p)
         place(job, jobs, p.tiles_i, p.tiles_j, slice, ti, tj);
         s0 = (int32_t)((int64_t)all * slice / p.slices), s1 = (int32_t)((int64_t)all * (slice + 1) / p.slices);
         step = s0 / p.combinations, combination = s0 - step * p.combinations;
+        // (each XCD begins elsewhere in k, where that can be: rows some power of two apart have the same numbers in the same channels of memory)
+        if (p.rotate) step = (int32_t)((int64_t)p.steps * (blockIdx.x & 7) / 8);
         a.start(p.a, ti * N, lane, wave);
         b.start(p.b, tj * N, lane, wave);
         make_here();
@@ -1180,6 +1183,7 @@ Product logits(const Call &c, const Plan &plan, const char *x, const char *w, in
     p.tail = plan.copy_x ? kDepth : c.dim - (plan.depth - kDepth);
     p.ni = (int32_t)count, p.nj = (int32_t)c.rows;
     p.steps = plan.depth / kDepth, p.combinations = plan.combinations, p.slices = 1;
+    p.rotate = p.tail == kDepth;
     p.first = (int32_t)first, p.vocab = (int32_t)c.vocab, p.tokens = c.tokens, p.ignore = c.ignore;
     return p;
 }
