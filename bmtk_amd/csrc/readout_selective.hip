@@ -26,16 +26,20 @@ struct SelArgs {
     const int32_t *lengths;
     void *y, *dx, *d_dt, *d_write, *d_read;
     float *last, *marks, *d_rate, *d_skip, *d_dt_bias, *d_state;
-    float *spread;            // [batch][groups][waves][n_steps][2][kOwn]: write and read in 32 bits, 0 behind a sequence's end
+    float *spread;            // [batch][groups][waves][padded_steps][2][kOwn]: write and read in 32 bits, 0 behind a sequence's end
     float *ends;              // [stretches][batch][dim][padded]: a stretch's end from zero, then what enters it
     float *deltas;            // [stretches][batch][dim]: sum of a stretch's deltas
     float *part_write, *part_read;   // [tiles][batch][groups][waves][n_steps][kOwn]: sums over a tile's channels
     float *part_rate;         // [stretches][batch][dim][padded]
     float *part_skip, *part_bias;    // [stretches][batch][dim]
     int64_t n_steps, batch, x_t, x_b, dt_t, dt_b, write_t, write_b, read_t, read_b, dy_t, dy_b;
+    int64_t padded_steps;     // n_steps, to whole blocks
     int64_t stretch_steps;    // a multiple of kSteps
     int32_t dim, groups, n_states, waves, padded, channels, tiles, stretches, softplus;   // padded: waves * kOwn; channels, tiles: of a group
 };
+
+// write and read as the main kernels see them: of the constant address space, so that they come through scalar loads (an earlier kernel has written them)
+typedef __attribute__((address_space(4))) const float Shared;
 
 __device__ __forceinline__ float exp2_of(float v) { return __builtin_amdgcn_exp2f(v); }
 
@@ -74,13 +78,13 @@ __global__ __launch_bounds__(256) void spread_kernel(SelArgs a, int64_t rows)
     const int64_t tb = row / a.groups;
     const int32_t g = (int32_t)(row - tb * a.groups);
     const int64_t t = tb / a.batch, b = tb - t * a.batch;
-    const bool there = n < a.n_states && (!a.lengths || t < a.lengths[b]);
+    const bool there = n < a.n_states && t < (a.lengths ? min((int64_t)a.lengths[b], a.n_steps) : a.n_steps);
     float w = 0.0f, r = 0.0f;
     if (there) {
         w = (float)static_cast<const T *>(a.write)[t * a.write_t + b * a.write_b + (int64_t)g * a.n_states + n];
         r = (float)static_cast<const T *>(a.read)[t * a.read_t + b * a.read_b + (int64_t)g * a.n_states + n];
     }
-    float *to = a.spread + ((((b * a.groups + g) * a.waves + n / kOwn) * a.n_steps + t) * 2) * kOwn + n % kOwn;
+    float *to = a.spread + ((((b * a.groups + g) * a.waves + n / kOwn) * a.padded_steps + t) * 2) * kOwn + n % kOwn;
     to[0] = w;
     to[kOwn] = r;
 }
@@ -99,7 +103,9 @@ struct Tile {
         const int32_t tile = blockIdx.x % a.tiles;
         const int32_t gb = blockIdx.x / a.tiles;
         g = gb % a.groups;
-        b = gb / a.groups;
+        // (the sequences in another order in every stretch: workgroups whose numbers are some power of two apart share a compute unit, and sequences end early)
+        b = gb / a.groups + blockIdx.y % a.batch;
+        b -= b >= a.batch ? a.batch : 0;
         const int32_t in_group = tile * kWave + lane;
         there = in_group < a.channels;
         c = g * a.channels + min(in_group, a.channels - 1);
@@ -182,7 +188,7 @@ __global__ __launch_bounds__(Waves * kWave) void selective_fwd_kernel(SelArgs a)
         else if (a.state) get_states(a.state + column * a.n_states, n0, a.n_states, whole_states(a, a.state), h);
     }
     const float bias = a.dt_bias ? a.dt_bias[at.c] : 0.0f, skip = a.skip ? a.skip[at.c] : 0.0f;
-    const float *spread = a.spread + ((at.b * a.groups + at.g) * a.waves + at.wave) * a.n_steps * 2 * kOwn;
+    const Shared *spread = (const Shared *)(a.spread + ((at.b * a.groups + at.g) * a.waves + at.wave) * a.padded_steps * 2 * kOwn);
     Inputs<T, TD, Rows, false> in;
     in.ask(a, at, at.t0);
     float total = 0.0f;
@@ -201,31 +207,18 @@ __global__ __launch_bounds__(Waves * kWave) void selective_fwd_kernel(SelArgs a)
         if (t + kSteps < at.t1) in.ask(a, at, t + kSteps);
         if (!Sums && a.marks && at.there) put_states(a.marks + (t / kSteps * a.batch * a.dim + column) * a.n_states, n0, a.n_states, whole_states(a, a.marks), h);
         if (t < at.end) {
-            const float *wr = spread + t * 2 * kOwn;
-            const int steps = (int)min(at.t1 - t, (int64_t)kSteps);
-            if (steps == kSteps) {
+            const Shared *wr = spread + t * 2 * kOwn;
+            // (a step behind the stretch's last one has delta and delta x 0, and changes nothing)
 #pragma unroll
-                for (int k = 0; k < kSteps; ++k) {
-                    const float2 d = staged[k * kWave + at.lane];
-                    float y = 0.0f;
+            for (int k = 0; k < kSteps; ++k) {
+                const float2 d = staged[k * kWave + at.lane];
+                float y = 0.0f;
 #pragma unroll
-                    for (int i = 0; i < kOwn; ++i) {
-                        h[i] = fmaf(exp2_of(d.x * rate[i]), h[i], d.y * wr[k * 2 * kOwn + i]);
-                        if (!Sums) y = fmaf(wr[k * 2 * kOwn + kOwn + i], h[i], y);
-                    }
-                    if (!Sums) parts[(at.wave * kSteps + k) * kWave + at.lane] = y;
+                for (int i = 0; i < kOwn; ++i) {
+                    h[i] = fmaf(exp2_of(d.x * rate[i]), h[i], d.y * wr[k * 2 * kOwn + i]);
+                    if (!Sums) y = fmaf(wr[k * 2 * kOwn + kOwn + i], h[i], y);
                 }
-            } else {
-                for (int k = 0; k < steps; ++k) {
-                    const float2 d = staged[k * kWave + at.lane];
-                    float y = 0.0f;
-#pragma unroll
-                    for (int i = 0; i < kOwn; ++i) {
-                        h[i] = fmaf(exp2_of(d.x * rate[i]), h[i], d.y * wr[k * 2 * kOwn + i]);
-                        if (!Sums) y = fmaf(wr[k * 2 * kOwn + kOwn + i], h[i], y);
-                    }
-                    if (!Sums) parts[(at.wave * kSteps + k) * kWave + at.lane] = y;
-                }
+                if (!Sums) parts[(at.wave * kSteps + k) * kWave + at.lane] = y;
             }
         }
         __syncthreads();
@@ -356,7 +349,7 @@ __global__ __launch_bounds__(Waves * kWave) void selective_bwd_kernel(SelArgs a)
         else if (a.d_last) get_states(a.d_last + column * a.n_states, n0, a.n_states, whole_states(a, a.d_last), back);
     }
     const float bias = a.dt_bias ? a.dt_bias[at.c] : 0.0f, skip = a.skip ? a.skip[at.c] : 0.0f;
-    const float *spread = a.spread + ((at.b * a.groups + at.g) * a.waves + at.wave) * a.n_steps * 2 * kOwn;
+    const Shared *spread = (const Shared *)(a.spread + ((at.b * a.groups + at.g) * a.waves + at.wave) * a.padded_steps * 2 * kOwn);
     const int64_t part_row = (((int64_t)(blockIdx.x % a.tiles) * a.batch + at.b) * a.groups + at.g) * a.waves + at.wave;
     Inputs<T, TD, Rows, true> in;
     const int64_t t_last = at.t0 + (at.t1 - at.t0 - 1) / kSteps * kSteps;
@@ -381,15 +374,14 @@ __global__ __launch_bounds__(Waves * kWave) void selective_bwd_kernel(SelArgs a)
         }
         __syncthreads();
         if (t > at.t0) in.ask(a, at, t - kSteps);
-        // (steps behind the stretch's last one have delta, x and dy 0; their write and read are the last step's, whatever they are)
+        // (steps behind the stretch's last one have delta, x and dy 0)
         if (t < at.end) {
-            const float *wr = spread + t * 2 * kOwn;
-            const int most = (int)min(at.t1 - t, (int64_t)kSteps) - 1;
+            const Shared *wr = spread + t * 2 * kOwn;
             if constexpr (Sums) {
 #pragma unroll
                 for (int k = kSteps - 1; k >= 0; --k) {
                     const float d = staged[k * kWave + at.lane].x, dy_k = dys[k * kWave + at.lane];
-                    const float *w = wr + min(k, most) * 2 * kOwn;
+                    const Shared *w = wr + k * 2 * kOwn;
 #pragma unroll
                     for (int i = 0; i < kOwn; ++i) back[i] = exp2_of(d * rate2[i]) * fmaf(dy_k, w[kOwn + i], back[i]);
                 }
@@ -401,8 +393,9 @@ __global__ __launch_bounds__(Waves * kWave) void selective_bwd_kernel(SelArgs a)
                     for (int i = 0; i < kOwn; ++i) h[i] = 0.0f;
 #pragma unroll
                 for (int k = 0; k < kSteps; ++k) {
+                    if (k % 4 == 0) asm volatile("" : "+s"(wr), "+v"(h[0]));
                     const float2 d = staged[k * kWave + at.lane];
-                    const float *w = wr + min(k, most) * 2 * kOwn;
+                    const Shared *w = wr + k * 2 * kOwn;
 #pragma unroll
                     for (int i = 0; i < kOwn; ++i) {
                         e[k][i] = exp2_of(d.x * rate2[i]);
@@ -413,9 +406,11 @@ __global__ __launch_bounds__(Waves * kWave) void selective_bwd_kernel(SelArgs a)
                 float sum_read[kSteps], sum_write[kSteps];
 #pragma unroll
                 for (int k = kSteps - 1; k >= 0; --k) {
+                    // (write and read are asked for again, four steps at a time: there are no scalar registers to keep those of the block in)
+                    if (k % 4 == 3) asm volatile("" : "+s"(wr), "+v"(back[0]));
                     const float2 d = staged[k * kWave + at.lane];
                     const float dy_k = dys[k * kWave + at.lane];
-                    const float *w = wr + min(k, most) * 2 * kOwn;
+                    const Shared *w = wr + k * 2 * kOwn;
                     float s1 = 0.0f, s2 = 0.0f, by_read[kOwn], by_write[kOwn];
 #pragma unroll
                     for (int i = 0; i < kOwn; ++i) {
@@ -575,7 +570,7 @@ __global__ __launch_bounds__(1024) void selective_join_channels_kernel(SelArgs a
 
 struct Plan {
     int32_t waves, padded, channels, tiles, stretches;
-    int64_t stretch_steps, spread, ends, deltas, shared, rate, per_dim;   // sizes in numbers
+    int64_t stretch_steps, padded_steps, spread, ends, deltas, shared, rate, per_dim;   // sizes in numbers
     Plan(int64_t n_steps, int64_t batch, int32_t dim, int32_t groups, int32_t n_states, bool backward)
     {
         waves = (int32_t)div_up(n_states, kOwn);
@@ -591,7 +586,8 @@ struct Plan {
         const int64_t each = div_up(blocks, s);
         stretch_steps = each * kSteps;
         stretches = (int32_t)div_up(blocks, each);
-        spread = batch * groups * waves * n_steps * 2 * kOwn;
+        padded_steps = blocks * kSteps;
+        spread = batch * groups * waves * padded_steps * 2 * kOwn;
         ends = stretches > 1 ? stretches * batch * dim * padded : 0;
         deltas = stretches > 1 ? stretches * batch * dim : 0;
         shared = backward ? (int64_t)tiles * batch * groups * waves * n_steps * kOwn : 0;
@@ -609,7 +605,7 @@ struct Plan {
         };
         a.spread = next(spread), a.ends = next(ends), a.deltas = next(deltas), a.part_write = next(shared), a.part_read = next(shared), a.part_rate = next(rate);
         a.part_skip = next(per_dim), a.part_bias = next(per_dim);
-        a.waves = waves, a.padded = padded, a.channels = channels, a.tiles = tiles, a.stretches = stretches, a.stretch_steps = stretch_steps;
+        a.waves = waves, a.padded = padded, a.channels = channels, a.tiles = tiles, a.stretches = stretches, a.stretch_steps = stretch_steps, a.padded_steps = padded_steps;
     }
 };
 
@@ -679,7 +675,7 @@ int run(const char *name, SelArgs &a, int32_t dtype, int32_t dt_dtype, bool back
     BMTK_REQUIRE(dt_dtype == BMTK_F32 || dt_dtype == dtype, "%s: dt must be float32 or of the type of x", name);
     BMTK_REQUIRE(sizes_fit(a.n_steps, a.batch, a.dim, a.groups, a.n_states), "%s: too many steps or columns", name);
     const Plan plan(a.n_steps, a.batch, a.dim, a.groups, a.n_states, backward);
-    const int64_t across = a.batch * a.groups * plan.tiles, rows = a.n_steps * a.batch * a.groups, columns = a.batch * a.dim;
+    const int64_t across = a.batch * a.groups * plan.tiles, rows = plan.padded_steps * a.batch * a.groups, columns = a.batch * a.dim;
     BMTK_REQUIRE(across * plan.waves * kWave < (int64_t{1} << 32) && rows * plan.padded < (int64_t{1} << 32) && columns * plan.padded < (int64_t{1} << 32),
                  "%s: too many states for a launch", name);
     BMTK_REQUIRE(workspace, "%s: needs a workspace", name);
