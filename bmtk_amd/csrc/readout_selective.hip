@@ -17,6 +17,7 @@ namespace {
 
 constexpr int kSteps = BMTK_SCAN_MARK;   // steps of a block: what a workgroup stages at once, and of which a state is kept
 constexpr int kOwn = 4;                  // states of a wavefront
+constexpr int64_t kFewSteps = 8;         // up to which the steps are taken one by one
 constexpr float kLog2e = 1.44269504f;
 constexpr float kLeast = 1.17549435e-38f;   // a stretch's decay is at least this, so that an infinite state stays infinite
 
@@ -249,6 +250,46 @@ __global__ __launch_bounds__(Waves * kWave) void selective_fwd_kernel(SelArgs a)
     } else if (at.there && (int32_t)blockIdx.y == a.stretches - 1) {
         put_states(a.last + column * a.n_states, n0, a.n_states, whole_states(a, a.last), h);
     }
+}
+
+// A few steps, with the states as they lie in memory: a lane has four of a channel's, Lanes neighbouring lanes the channel's all, and y is summed over those.  Bound
+// by the states, read and written.
+template <typename T, typename TD, int Lanes>
+__global__ __launch_bounds__(256) void selective_step_kernel(SelArgs a, FastDiv by_dim, FastDiv by_channels)
+{
+    const uint32_t q = blockIdx.x * 256u + threadIdx.x, column = q / Lanes;
+    const int32_t n0 = (int32_t)(q % Lanes) * kOwn;
+    if (column >= (uint32_t)(a.batch * a.dim)) return;   // (Lanes divides a wavefront: a channel's lanes leave together)
+    const uint32_t b = div_by(column, by_dim), c = column - b * (uint32_t)a.dim, g = div_by(c, by_channels);
+    const bool whole = whole_states(a, a.rate) && whole_states(a, a.last) && (!a.state || whole_states(a, a.state)) && n0 < a.n_states;
+    const int64_t end = a.lengths ? min(max((int64_t)a.lengths[b], (int64_t)0), a.n_steps) : a.n_steps;
+    float rate[kOwn], h[kOwn];
+    get_states(a.rate + (int64_t)c * a.n_states, n0, a.n_states, whole, rate);
+#pragma unroll
+    for (int i = 0; i < kOwn; ++i) rate[i] *= kLog2e, h[i] = 0.0f;
+    if (a.state) get_states(a.state + (int64_t)column * a.n_states, n0, a.n_states, whole, h);
+    const float bias = a.dt_bias ? a.dt_bias[c] : 0.0f, skip = a.skip ? a.skip[c] : 0.0f;
+    for (int64_t t = 0; t < a.n_steps; ++t) {
+        if (t % kSteps == 0 && a.marks) put_states(a.marks + (t / kSteps * a.batch * a.dim + column) * a.n_states, n0, a.n_states, false, h);
+        float y = 0.0f;
+        if (t < end) {
+            const float x = (float)static_cast<const T *>(a.x)[t * a.x_t + b * a.x_b + c];
+            const float delta = delta_of(a, (float)static_cast<const TD *>(a.dt)[t * a.dt_t + b * a.dt_b + c] + bias), u = delta * x;
+            const T *write = static_cast<const T *>(a.write) + t * a.write_t + b * a.write_b + (int64_t)g * a.n_states;
+            const T *read = static_cast<const T *>(a.read) + t * a.read_t + b * a.read_b + (int64_t)g * a.n_states;
+#pragma unroll
+            for (int i = 0; i < kOwn; ++i) {
+                if (n0 + i >= a.n_states) continue;
+                h[i] = fmaf(exp2_of(delta * rate[i]), h[i], u * (float)write[n0 + i]);
+                y = fmaf((float)read[n0 + i], h[i], y);
+            }
+#pragma unroll
+            for (int k = 1; k < Lanes; k *= 2) y += __shfl_xor(y, k);
+            y = fmaf(skip, x, y);
+        }
+        if (n0 == 0) static_cast<T *>(a.y)[(t * a.batch + b) * a.dim + c] = (T)y;
+    }
+    put_states(a.last + (int64_t)column * a.n_states, n0, a.n_states, whole, h);
 }
 
 // What enters each stretch, from its neighbour's: in the order of time from the state, or (Back) against it from the last state's gradient
@@ -577,11 +618,13 @@ struct Plan {
         padded = waves * kOwn;
         channels = dim / groups;
         tiles = (int32_t)div_up(channels, kWave);
-        // Stretches cost their sums beforehand, which are about as much again: only where the chip would stay half empty.  A stretch has at least 64 steps.
+        // Stretches cost their sums beforehand, which are about as much again, but a workgroup waits for its own wavefronts twice a block: from some 4,096 wavefronts on
+        // (back, where a block is three times as long, 2,048) one stretch does.  us of 2,000 x 8 x 4,096 x 16, 2,048 wavefronts: forward 624 in one stretch, 490 in eight;
+        // back 1,240 and 1,430.  Otherwise as many as make 16,384, down to a block each: 65,536 x 1 x 1,024 x 16 forward 688 with 4,096, 580 with 12,288, 562 with 16,384;
+        // 600 x 32 x 64 x 8 fp32 both ways 153 with stretches of four blocks, 113 of two, 98 of one.
         const int64_t across = batch * groups * tiles * waves, blocks = div_up(n_steps, kSteps);
-        int64_t s = across >= 2048 ? 1 : div_up(4096, across);
-        if (s > blocks / 4) s = blocks / 4;
-        if (s < 1) s = 1;
+        int64_t s = across >= (backward ? 2048 : 4096) ? 1 : div_up(16384, across);
+        if (s > blocks) s = blocks;
         if (s > 65535) s = 65535;
         const int64_t each = div_up(blocks, s);
         stretch_steps = each * kSteps;
@@ -666,6 +709,28 @@ int launch_rows(const char *name, const SelArgs &a, dim3 grid, bool backward, hi
     return launch<T, TD, 16, 2>(name, a, grid, backward, s);
 }
 
+template <typename T, typename TD>
+int launch_step(const char *name, const SelArgs &a, hipStream_t s)
+{
+    int lanes = 1;
+    while (lanes * kOwn < a.n_states) lanes *= 2;
+    const int64_t threads = a.batch * a.dim * lanes;
+    const uint32_t blocks = (uint32_t)div_up(threads, 256);
+    const FastDiv by_dim = fast_div((uint32_t)a.dim), by_channels = fast_div((uint32_t)(a.dim / a.groups));
+    switch (lanes) {
+        case 1: selective_step_kernel<T, TD, 1><<<blocks, 256, 0, s>>>(a, by_dim, by_channels); break;
+        case 2: selective_step_kernel<T, TD, 2><<<blocks, 256, 0, s>>>(a, by_dim, by_channels); break;
+        case 4: selective_step_kernel<T, TD, 4><<<blocks, 256, 0, s>>>(a, by_dim, by_channels); break;
+        case 8: selective_step_kernel<T, TD, 8><<<blocks, 256, 0, s>>>(a, by_dim, by_channels); break;
+        default: selective_step_kernel<T, TD, 16><<<blocks, 256, 0, s>>>(a, by_dim, by_channels);
+    }
+    BMTK_CHECK_LAUNCH(name);
+    return 0;
+}
+
+// Whether the steps are few enough for the kernel that takes them one by one: it has one launch instead of two
+bool few_steps(int64_t n_steps, int64_t batch, int32_t dim) { return n_steps <= kFewSteps && batch * dim < (int64_t{1} << 27); }
+
 int run(const char *name, SelArgs &a, int32_t dtype, int32_t dt_dtype, bool backward, float *workspace, hipStream_t s)
 {
     BMTK_REQUIRE(a.n_steps > 0 && a.batch > 0 && a.dim > 0 && a.groups > 0 && a.n_states > 0, "%s: sizes must be positive", name);
@@ -674,6 +739,9 @@ int run(const char *name, SelArgs &a, int32_t dtype, int32_t dt_dtype, bool back
     BMTK_REQUIRE(dtype >= 0 && dtype <= 2, "%s: unknown type %d", name, dtype);
     BMTK_REQUIRE(dt_dtype == BMTK_F32 || dt_dtype == dtype, "%s: dt must be float32 or of the type of x", name);
     BMTK_REQUIRE(sizes_fit(a.n_steps, a.batch, a.dim, a.groups, a.n_states), "%s: too many steps or columns", name);
+    if (!backward && few_steps(a.n_steps, a.batch, a.dim)) {
+        BMTK_BY_TYPE(dtype, T, { return dt_dtype == BMTK_F32 ? launch_step<T, float>(name, a, s) : launch_step<T, T>(name, a, s); });
+    }
     const Plan plan(a.n_steps, a.batch, a.dim, a.groups, a.n_states, backward);
     const int64_t across = a.batch * a.groups * plan.tiles, rows = plan.padded_steps * a.batch * a.groups, columns = a.batch * a.dim;
     BMTK_REQUIRE(across * plan.waves * kWave < (int64_t{1} << 32) && rows * plan.padded < (int64_t{1} << 32) && columns * plan.padded < (int64_t{1} << 32),
@@ -703,7 +771,7 @@ using namespace bmtk;
 
 extern "C" int64_t bmtk_selective_scan_workspace_bytes(int64_t n_steps, int64_t batch, int32_t dim, int32_t groups, int32_t n_states, int32_t backward)
 {
-    if (!sizes_fit(n_steps, batch, dim, groups, n_states)) return 0;
+    if (!sizes_fit(n_steps, batch, dim, groups, n_states) || (!backward && few_steps(n_steps, batch, dim))) return 0;
     return Plan(n_steps, batch, dim, groups, n_states, backward != 0).numbers() * 4;
 }
 
