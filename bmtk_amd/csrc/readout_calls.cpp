@@ -26,6 +26,15 @@ decltype(&bmtk_gated_scan_bwd) scan_bwd;
 decltype(&bmtk_token_logprobs_workspace_bytes) logprobs_workspace;
 decltype(&bmtk_token_logprobs_fwd) logprobs_fwd;
 decltype(&bmtk_token_logprobs_bwd) logprobs_bwd;
+decltype(&bmtk_short_conv_workspace_bytes) conv_workspace;
+decltype(&bmtk_short_conv_fwd) conv_fwd;
+decltype(&bmtk_short_conv_bwd) conv_bwd;
+decltype(&bmtk_selective_scan_workspace_bytes) selective_workspace;
+decltype(&bmtk_selective_scan_fwd) selective_fwd;
+decltype(&bmtk_selective_scan_bwd) selective_bwd;
+decltype(&bmtk_projected_logprobs_workspace_bytes) projected_workspace;
+decltype(&bmtk_projected_logprobs_fwd) projected_fwd;
+decltype(&bmtk_projected_logprobs_bwd) projected_bwd;
 PyObject *raw_stream = nullptr;   // torch._C._cuda_getCurrentRawStream
 bool ready = false;
 
@@ -327,6 +336,205 @@ PyObject *token_logprobs_bwd(PyObject *, PyObject *const *args, Py_ssize_t nargs
     });
 }
 
+// steps, sequences and channels that the C ABI takes, the channels next to one another
+bool sequences(const at::Tensor &t) { return t.dim() == 3 && t.numel() > 0 && t.stride(2) == 1 && t.size(0) < (int64_t{1} << 31) - 4096 && t.size(1) * t.size(2) < (int64_t{1} << 31); }
+
+struct Conv {
+    const at::Tensor *x, *weight, *bias = nullptr, *state = nullptr, *lengths = nullptr;
+    int64_t steps = 0, batch = 0, dim = 0, width = 0;
+    int code = -1, weight_code = -1;
+    bool silu = false;
+    Conv(Call &c, PyObject *x_obj, PyObject *weight_obj, PyObject *bias_obj, PyObject *state_obj, PyObject *lengths_obj, PyObject *silu_obj)
+    {
+        x = c.tensor(x_obj);
+        weight = c.tensor(weight_obj);
+        silu = c.truth(silu_obj);
+        if (!c.fine) return;
+        code = code_of(*x), weight_code = code_of(*weight);
+        c.fine = code >= 0 && (weight_code == BMTK_F32 || weight_code == code) && sequences(*x) && weight->dim() == 2 && weight->is_contiguous() && weight->size(0) == x->size(2) &&
+                 weight->size(1) >= 2 && weight->size(1) <= BMTK_CONV_MAX_WIDTH;
+        if (!c.fine) return;
+        steps = x->size(0), batch = x->size(1), dim = x->size(2), width = weight->size(1);
+        bias = c.optional(bias_obj, weight->scalar_type(), {dim});
+        if (c.fine) state = c.optional(state_obj, x->scalar_type(), {width - 1, batch, dim});
+        if (c.fine) lengths = c.optional(lengths_obj, at::kInt, {batch});
+    }
+};
+
+PyObject *short_conv(PyObject *, PyObject *const *args, Py_ssize_t nargs)
+{
+    return guarded([&]() -> PyObject * {
+        Call c(nargs, 6);
+        if (!c.fine) return nullptr;
+        const Conv v(c, args[0], args[1], args[2], args[3], args[4], args[5]);
+        void *stream = c.stream();
+        if (!c.fine) return nullptr;
+        const at::Tensor y = c.empty({v.steps, v.batch, v.dim}, v.x->scalar_type()), last = c.empty({v.width - 1, v.batch, v.dim}, v.x->scalar_type());
+        if (conv_fwd(v.steps, v.batch, (int32_t)v.dim, (int32_t)v.width, v.code, v.weight_code, v.silu, ptr(v.x), v.x->stride(0), v.x->stride(1), ptr(v.weight), ptr(v.bias), ptr(v.state),
+                     (const int32_t *)ptr(v.lengths), ptr(y), ptr(last), stream) != 0)
+            return nullptr;
+        return results({y, last});
+    });
+}
+
+PyObject *short_conv_bwd(PyObject *, PyObject *const *args, Py_ssize_t nargs)
+{
+    return guarded([&]() -> PyObject * {
+        Call c(nargs, 8);   // x, weight, dy, bias, state, d_last, lengths, silu
+        if (!c.fine) return nullptr;
+        const Conv v(c, args[0], args[1], args[3], args[4], args[6], args[7]);
+        if (!c.fine) return nullptr;
+        const at::Tensor *dy = c.tensor(args[2]);
+        const at::Tensor *d_last = c.optional(args[5], v.x->scalar_type(), {v.width - 1, v.batch, v.dim});
+        void *stream = c.stream();
+        if (!c.fine || dy->scalar_type() != v.x->scalar_type() || dy->sizes() != v.x->sizes() || dy->stride(2) != 1) return nullptr;
+        const at::Tensor dx = c.empty({v.steps, v.batch, v.dim}, v.x->scalar_type()), d_weight = c.empty({v.dim, v.width}, v.weight->scalar_type());
+        const at::Tensor d_bias = c.empty({v.dim}, v.weight->scalar_type()), d_state = c.empty({v.width - 1, v.batch, v.dim}, v.x->scalar_type());
+        const at::Tensor ws = c.bytes(conv_workspace(v.steps, v.batch, (int32_t)v.dim, (int32_t)v.width, v.code));
+        if (conv_bwd(v.steps, v.batch, (int32_t)v.dim, (int32_t)v.width, v.code, v.weight_code, v.silu, ptr(v.x), v.x->stride(0), v.x->stride(1), ptr(v.weight), ptr(v.bias), ptr(v.state),
+                     (const int32_t *)ptr(v.lengths), ptr(dy), dy->stride(0), dy->stride(1), ptr(d_last), ptr(dx), ptr(d_weight), ptr(d_bias), ptr(d_state), (float *)ptr(ws), stream) != 0)
+            return nullptr;
+        return results({dx, d_weight, d_bias, d_state});
+    });
+}
+
+struct Selective {
+    const at::Tensor *x, *dt, *rate, *write, *read, *skip = nullptr, *dt_bias = nullptr, *lengths = nullptr;
+    int64_t steps = 0, batch = 0, dim = 0, groups = 0, states = 0;
+    int code = -1, dt_code = -1;
+    bool softplus = false;
+    Selective(Call &c, PyObject *const *first, PyObject *skip_obj, PyObject *dt_bias_obj, PyObject *softplus_obj, PyObject *lengths_obj)
+    {
+        x = c.tensor(first[0]);
+        dt = c.tensor(first[1]);
+        rate = c.tensor(first[2]);
+        write = c.tensor(first[3]);
+        read = c.tensor(first[4]);
+        softplus = c.truth(softplus_obj);
+        if (!c.fine) return;
+        code = code_of(*x), dt_code = code_of(*dt);
+        c.fine = code >= 0 && (dt_code == BMTK_F32 || dt_code == code) && sequences(*x) && dt->sizes() == x->sizes() && dt->stride(2) == 1 && rate->scalar_type() == at::kFloat &&
+                 rate->dim() == 2 && rate->is_contiguous() && rate->size(0) == x->size(2) && rate->size(1) >= 1 && rate->size(1) <= BMTK_SELECTIVE_MAX_STATES && write->dim() == 4;
+        if (!c.fine) return;
+        steps = x->size(0), batch = x->size(1), dim = x->size(2), states = rate->size(1), groups = write->size(2);
+        c.fine = groups > 0 && dim % groups == 0 && write->sizes() == at::IntArrayRef({steps, batch, groups, states}) && read->sizes() == write->sizes();
+        for (const at::Tensor *t : {write, read}) c.fine = c.fine && t->scalar_type() == x->scalar_type() && t->stride(3) == 1 && t->stride(2) == states;
+        if (c.fine) skip = c.optional(skip_obj, at::kFloat, {dim});
+        if (c.fine) dt_bias = c.optional(dt_bias_obj, at::kFloat, {dim});
+        if (c.fine) lengths = c.optional(lengths_obj, at::kInt, {batch});
+    }
+};
+
+PyObject *selective_scan(PyObject *, PyObject *const *args, Py_ssize_t nargs)
+{
+    return guarded([&]() -> PyObject * {
+        Call c(nargs, 11);   // x, dt, rate, write, read, skip, dt_bias, softplus, state, lengths, save_state
+        if (!c.fine) return nullptr;
+        const Selective s(c, args, args[5], args[6], args[7], args[9]);
+        if (!c.fine) return nullptr;
+        const at::Tensor *state = c.optional(args[8], at::kFloat, {s.batch, s.dim, s.states});
+        const bool save = c.truth(args[10]);
+        void *stream = c.stream();
+        if (!c.fine) return nullptr;
+        const at::Tensor y = c.empty({s.steps, s.batch, s.dim}, s.x->scalar_type()), last = c.empty({s.batch, s.dim, s.states}, at::kFloat);
+        const at::Tensor saved = save ? c.empty({(s.steps + BMTK_SCAN_MARK - 1) / BMTK_SCAN_MARK, s.batch, s.dim, s.states}, at::kFloat) : at::Tensor();
+        const at::Tensor ws = c.bytes(selective_workspace(s.steps, s.batch, (int32_t)s.dim, (int32_t)s.groups, (int32_t)s.states, 0));
+        if (selective_fwd(s.steps, s.batch, (int32_t)s.dim, (int32_t)s.groups, (int32_t)s.states, s.code, s.dt_code, s.softplus, ptr(s.x), s.x->stride(0), s.x->stride(1), ptr(s.dt),
+                          s.dt->stride(0), s.dt->stride(1), ptr(s.write), s.write->stride(0), s.write->stride(1), ptr(s.read), s.read->stride(0), s.read->stride(1),
+                          (const float *)ptr(s.rate), (const float *)ptr(s.skip), (const float *)ptr(s.dt_bias), (const float *)ptr(state), (const int32_t *)ptr(s.lengths), ptr(y),
+                          (float *)ptr(last), (float *)ptr(saved), (float *)ptr(ws), stream) != 0)
+            return nullptr;
+        if (save) return results({y, last, saved});
+        return results({y, last});
+    });
+}
+
+PyObject *selective_scan_bwd(PyObject *, PyObject *const *args, Py_ssize_t nargs)
+{
+    return guarded([&]() -> PyObject * {
+        Call c(nargs, 12);   // x, dt, rate, write, read, saved, dy, skip, dt_bias, softplus, d_last, lengths
+        if (!c.fine) return nullptr;
+        const Selective s(c, args, args[7], args[8], args[9], args[11]);
+        if (!c.fine) return nullptr;
+        const at::Tensor *saved = c.tensor(args[5], at::kFloat, {(s.steps + BMTK_SCAN_MARK - 1) / BMTK_SCAN_MARK, s.batch, s.dim, s.states});
+        const at::Tensor *dy = c.tensor(args[6]);
+        const at::Tensor *d_last = c.optional(args[10], at::kFloat, {s.batch, s.dim, s.states});
+        void *stream = c.stream();
+        if (!c.fine || dy->scalar_type() != s.x->scalar_type() || dy->sizes() != s.x->sizes() || dy->stride(2) != 1) return nullptr;
+        const at::ScalarType type = s.x->scalar_type();
+        const at::Tensor dx = c.empty({s.steps, s.batch, s.dim}, type), d_dt = c.empty({s.steps, s.batch, s.dim}, s.dt->scalar_type()), d_rate = c.empty({s.dim, s.states}, at::kFloat);
+        const at::Tensor d_write = c.empty({s.steps, s.batch, s.groups, s.states}, type), d_read = c.empty({s.steps, s.batch, s.groups, s.states}, type);
+        const at::Tensor d_skip = c.empty({s.dim}, at::kFloat), d_dt_bias = c.empty({s.dim}, at::kFloat), d_state = c.empty({s.batch, s.dim, s.states}, at::kFloat);
+        const at::Tensor ws = c.bytes(selective_workspace(s.steps, s.batch, (int32_t)s.dim, (int32_t)s.groups, (int32_t)s.states, 1));
+        if (selective_bwd(s.steps, s.batch, (int32_t)s.dim, (int32_t)s.groups, (int32_t)s.states, s.code, s.dt_code, s.softplus, ptr(s.x), s.x->stride(0), s.x->stride(1), ptr(s.dt),
+                          s.dt->stride(0), s.dt->stride(1), ptr(s.write), s.write->stride(0), s.write->stride(1), ptr(s.read), s.read->stride(0), s.read->stride(1),
+                          (const float *)ptr(s.rate), (const float *)ptr(s.skip), (const float *)ptr(s.dt_bias), (const float *)ptr(saved), (const int32_t *)ptr(s.lengths), ptr(dy),
+                          dy->stride(0), dy->stride(1), (const float *)ptr(d_last), ptr(dx), ptr(d_dt), ptr(d_write), ptr(d_read), (float *)ptr(d_rate), (float *)ptr(d_skip),
+                          (float *)ptr(d_dt_bias), (float *)ptr(d_state), (float *)ptr(ws), stream) != 0)
+            return nullptr;
+        return results({dx, d_dt, d_rate, d_write, d_read, d_skip, d_dt_bias, d_state});
+    });
+}
+
+// two dimensions: rows of x and a token for each
+struct Projected {
+    const at::Tensor *x, *weight, *tokens;
+    int64_t rows = 0, vocab = 0, dim = 0, x_stride = 0, w_stride = 0;
+    int code = -1;
+    Projected(Call &c, PyObject *x_obj, PyObject *weight_obj, PyObject *tokens_obj)
+    {
+        x = c.tensor(x_obj);
+        weight = c.tensor(weight_obj);
+        tokens = c.tensor(tokens_obj);
+        if (!c.fine) return;
+        code = code_of(*x);
+        c.fine = code >= 0 && code_of(*weight) == code && x->dim() == 2 && x->numel() > 0 && x->stride(1) == 1 && weight->dim() == 2 && weight->numel() > 0 && weight->stride(1) == 1 &&
+                 weight->size(1) == x->size(1) && tokens->scalar_type() == at::kLong && tokens->dim() == 1 && tokens->is_contiguous() && tokens->size(0) == x->size(0) &&
+                 x->size(0) < (1 << 22) && weight->size(0) < (1 << 28) && x->size(1) <= 65536;
+        if (!c.fine) return;
+        rows = x->size(0), vocab = weight->size(0), dim = x->size(1);
+        x_stride = rows > 1 ? x->stride(0) : dim, w_stride = vocab > 1 ? weight->stride(0) : dim;
+    }
+};
+
+PyObject *projected_logprobs(PyObject *, PyObject *const *args, Py_ssize_t nargs)
+{
+    return guarded([&]() -> PyObject * {
+        Call c(nargs, 4);
+        if (!c.fine) return nullptr;
+        const Projected p(c, args[0], args[1], args[2]);
+        const int64_t ignore = c.whole(args[3], INT64_MIN, INT64_MAX);
+        void *stream = c.stream();
+        if (!c.fine) return nullptr;
+        const at::Tensor logp = c.empty({p.rows}, at::kFloat), lse = c.empty({p.rows}, at::kFloat), peak = c.empty({p.rows}, at::kFloat), total = c.empty({p.rows}, at::kFloat);
+        const at::Tensor ws = c.bytes(projected_workspace(p.rows, (int32_t)p.vocab, (int32_t)p.dim, p.code, ptr(p.x), p.x_stride, ptr(p.weight), p.w_stride, 0));
+        if (projected_fwd(p.rows, (int32_t)p.vocab, (int32_t)p.dim, p.code, ptr(p.x), p.x_stride, ptr(p.weight), p.w_stride, (const int64_t *)ptr(p.tokens), ignore, (float *)ptr(logp),
+                          (float *)ptr(lse), (float *)ptr(peak), (float *)ptr(total), ptr(ws), stream) != 0)
+            return nullptr;
+        return results({logp, lse, peak, total});
+    });
+}
+
+PyObject *projected_logprobs_bwd(PyObject *, PyObject *const *args, Py_ssize_t nargs)
+{
+    return guarded([&]() -> PyObject * {
+        Call c(nargs, 7);   // x, weight, tokens, peak, total, d_logp, ignore
+        if (!c.fine) return nullptr;
+        const Projected p(c, args[0], args[1], args[2]);
+        if (!c.fine) return nullptr;
+        const at::Tensor *peak = c.tensor(args[3], at::kFloat, {p.rows}), *total = c.tensor(args[4], at::kFloat, {p.rows}), *d_logp = c.tensor(args[5], at::kFloat, {p.rows});
+        const int64_t ignore = c.whole(args[6], INT64_MIN, INT64_MAX);
+        void *stream = c.stream();
+        if (!c.fine) return nullptr;
+        const at::Tensor dx = c.empty({p.rows, p.dim}, p.x->scalar_type()), d_weight = c.empty({p.vocab, p.dim}, p.x->scalar_type());
+        const at::Tensor ws = c.bytes(projected_workspace(p.rows, (int32_t)p.vocab, (int32_t)p.dim, p.code, ptr(p.x), p.x_stride, ptr(p.weight), p.w_stride, 1));
+        if (projected_bwd(p.rows, (int32_t)p.vocab, (int32_t)p.dim, p.code, ptr(p.x), p.x_stride, ptr(p.weight), p.w_stride, (const int64_t *)ptr(p.tokens), ignore, (const float *)ptr(peak),
+                          (const float *)ptr(total), (const float *)ptr(d_logp), ptr(dx), ptr(d_weight), ptr(ws), stream) != 0)
+            return nullptr;
+        return results({dx, d_weight});
+    });
+}
+
 template <typename F>
 bool take(PyObject *addresses, Py_ssize_t k, F &f)
 {
@@ -339,8 +547,8 @@ PyObject *set_library(PyObject *, PyObject *args)
 {
     PyObject *addresses, *stream;
     if (!PyArg_ParseTuple(args, "O!O", &PyTuple_Type, &addresses, &stream)) return nullptr;
-    if (PyTuple_GET_SIZE(addresses) != 10) {
-        PyErr_SetString(PyExc_TypeError, "set_library takes ten addresses");
+    if (PyTuple_GET_SIZE(addresses) != 19) {
+        PyErr_SetString(PyExc_TypeError, "set_library takes nineteen addresses");
         return nullptr;
     }
     Py_INCREF(stream);
@@ -348,14 +556,17 @@ PyObject *set_library(PyObject *, PyObject *args)
     raw_stream = stream;
     ready = take(addresses, 0, spike_workspace) && take(addresses, 1, spike_fwd) && take(addresses, 2, spike_bwd_weight) && take(addresses, 3, spike_bwd_spikes) &&
             take(addresses, 4, scan_workspace) && take(addresses, 5, scan_fwd) && take(addresses, 6, scan_bwd) && take(addresses, 7, logprobs_workspace) &&
-            take(addresses, 8, logprobs_fwd) && take(addresses, 9, logprobs_bwd);
+            take(addresses, 8, logprobs_fwd) && take(addresses, 9, logprobs_bwd) && take(addresses, 10, conv_workspace) && take(addresses, 11, conv_fwd) &&
+            take(addresses, 12, conv_bwd) && take(addresses, 13, selective_workspace) && take(addresses, 14, selective_fwd) && take(addresses, 15, selective_bwd) &&
+            take(addresses, 16, projected_workspace) && take(addresses, 17, projected_fwd) && take(addresses, 18, projected_bwd);
     if (PyErr_Occurred()) return nullptr;
     return PyBool_FromLong(ready);
 }
 
 #define BMTK_METHOD(name) {#name, reinterpret_cast<PyCFunction>(reinterpret_cast<void (*)(void)>(name)), METH_FASTCALL, "as bmtk_amd.readout." #name ", or None"}
 PyMethodDef methods[] = {BMTK_METHOD(spike_readout), BMTK_METHOD(spike_readout_bwd), BMTK_METHOD(gated_scan), BMTK_METHOD(gated_scan_bwd), BMTK_METHOD(token_logprobs),
-                         BMTK_METHOD(token_logprobs_bwd), {"set_library", set_library, METH_VARARGS, "addresses of the C functions, and what says the current stream of a device"}, {nullptr, nullptr, 0, nullptr}};
+                         BMTK_METHOD(token_logprobs_bwd), BMTK_METHOD(short_conv), BMTK_METHOD(short_conv_bwd), BMTK_METHOD(selective_scan), BMTK_METHOD(selective_scan_bwd),
+                         BMTK_METHOD(projected_logprobs), BMTK_METHOD(projected_logprobs_bwd), {"set_library", set_library, METH_VARARGS, "addresses of the C functions, and what says the current stream of a device"}, {nullptr, nullptr, 0, nullptr}};
 
 PyModuleDef module = {PyModuleDef_HEAD_INIT, "_readout", nullptr, -1, methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -27,7 +27,9 @@ class _Native:
     NAMES = ("spike_readout", "spike_readout_bwd", "gated_scan", "gated_scan_bwd", "token_logprobs", "token_logprobs_bwd", "short_conv", "short_conv_bwd", "selective_scan",
              "selective_scan_bwd", "projected_logprobs", "projected_logprobs_bwd")
     LIBRARY = ("spike_readout_workspace_bytes", "spike_readout_fwd", "spike_readout_bwd_weight", "spike_readout_bwd_spikes", "gated_scan_workspace_bytes",
-               "gated_scan_fwd", "gated_scan_bwd", "token_logprobs_workspace_bytes", "token_logprobs_fwd", "token_logprobs_bwd")
+               "gated_scan_fwd", "gated_scan_bwd", "token_logprobs_workspace_bytes", "token_logprobs_fwd", "token_logprobs_bwd", "short_conv_workspace_bytes", "short_conv_fwd",
+               "short_conv_bwd", "selective_scan_workspace_bytes", "selective_scan_fwd", "selective_scan_bwd", "projected_logprobs_workspace_bytes", "projected_logprobs_fwd",
+               "projected_logprobs_bwd")
 
     def __init__(self):
         for name in self.NAMES:
