@@ -150,7 +150,7 @@ struct Source {
 struct Product {
     Source a, b;
     int32_t ni, nj;                               // sizes
-    int32_t tail;                                 // k of the last step that b's rows have; what lies behind them is not theirs
+    int32_t tail;                                 // k of the last step that the rows have; what lies behind them is not theirs
     int32_t steps, combinations;                  // steps of kDepth in k; 1 or 6
     int32_t rotate;                               // whether the steps may be begun anywhere: all of them are taken, and none is cut
     int32_t tiles_i, tiles_j, slices;             // slices: parts of the steps, each to a slab of its own
@@ -367,11 +367,11 @@ __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void product_kernel(Product p)
         const int k = slot / (W * W), i = slot % (W * W) / W, j = slot % W;
         acc[i][j] = Vec<E>::mfma(fa[k][i], fb[k][j], acc[i][j]);
     };
-    const auto cut_fragments = [&](int k) {   // b's numbers behind its rows, in the last step
+    const auto cut_fragments = [&](int k) {   // numbers behind the rows, in the last step: of both operands, since what lies there may be NaN
         if (Mode == kSlab || Mode == kOut || p.tail == kDepth) return;
 #pragma unroll
         for (int j = 0; j < W; ++j)
-            if (k * 16 + lane / 32 * 8 >= p.tail) fb[k][j] = typename Vec<E>::V8{};
+            if (k * 16 + lane / 32 * 8 >= p.tail) fa[k][j] = fb[k][j] = typename Vec<E>::V8{};
     };
     const auto up_to_the_middle = [&](const char *now, bool last) {
         constexpr int kReads = 3 * kPerQuarter, kOver = kMiddle - kMiddle / 10;
@@ -503,7 +503,7 @@ __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void product_kernel(Product p)
 #pragma unroll
             for (int j = 0; j < W; ++j) {
                 const int32_t row = j0 + (wj * W + j) * kTile + (lane & 31);
-                const bool none = row >= p.nj || token[j] == p.ignore || peak[j] == -INFINITY;
+                const bool none = row >= p.nj || token[j] == p.ignore || (peak[j] == -INFINITY && total[j] == 0.0f);
                 const float inverse = p.g_scale / total[j];
                 const int64_t far = token[j] - p.first - ii0 - 4 * half;
                 const int at = far >= 0 && far < W * kTile && !(far & 4) ? (int)far : -1;
@@ -874,8 +874,8 @@ __global__ __launch_bounds__(Split == 8 ? 512 : 256) void few_rows_kernel(Few a)
         const int32_t row = j * 16 + r16;
         const int64_t token = row < a.rows ? a.tokens[row] : -1;
         if constexpr (Gradient) {
-            const float peak = row < a.rows ? a.peak[row] : -INFINITY, inverse = row < a.rows ? 1.0f / a.total[row] : 0.0f;
-            const bool none = row >= a.rows || token == a.ignore || peak == -INFINITY;
+            const float peak = row < a.rows ? a.peak[row] : -INFINITY, total = row < a.rows ? a.total[row] : 0.0f, inverse = 1.0f / total;
+            const bool none = row >= a.rows || token == a.ignore || (peak == -INFINITY && total == 0.0f);
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll
@@ -1323,7 +1323,9 @@ int check(const char *name, const Call &c)
     BMTK_REQUIRE(c.dim <= 65536, "%s: up to 65,536 channels", name);
     // (offsets within a tile of 256 rows and launches of one dimension are in 32 bits)
     BMTK_REQUIRE(c.x_stride >= 0 && c.w_stride >= 0 && (c.x_stride < (1 << 21) || c.rows <= 1) && (c.w_stride < (1 << 21) || c.vocab <= 1), "%s: rows further apart than 2^21 numbers", name);
-    BMTK_REQUIRE(up(c.vocab, 256) * up(c.dim, 64) < (int64_t{1} << 39) && up(c.rows, 256) * up(c.dim, 64) < (int64_t{1} << 39), "%s: too many numbers for a launch", name);
+    // (a launch has up to 2^32 threads: of eight numbers where operands are laid out anew, of four where dx is put together)
+    BMTK_REQUIRE(up(c.vocab, 256) * up(c.dim, 64) < (int64_t{1} << 35) && up(c.rows, 256) * up(c.dim, 64) < (int64_t{1} << 34), "%s: too many numbers for a launch", name);
+    BMTK_REQUIRE(div_up(c.rows, 128) * div_up(c.vocab, 128) < (int64_t{1} << 31), "%s: too many logits for a launch", name);
     BMTK_REQUIRE(c.ws, "%s: needs a workspace", name);
     return 0;
 }

@@ -391,7 +391,7 @@ def selective_scan(x, dt, rate, write, read, skip=None, dt_bias=None, softplus=F
 
     x       [steps, sequences, channels]; steps and sequences at any distance in memory, the channels next to one another; dt likewise, of the type of ``x``
             or float32
-    rate    float32 [channels, states], up to 64 states; delta * rate is meant to be 0 or less
+    rate    float32 [channels, states], finite, up to 64 states; delta * rate is meant to be 0 or less
     write, read  [steps, sequences, groups, states], of the type of ``x``, the states of a step next to one another; each group is for
             channels / groups neighbouring channels
     skip, dt_bias  float32 [channels] (None: zero)
@@ -547,7 +547,8 @@ def _overlap(a, b):
 # ---------------------------------------------------------------------------------------------------------------------
 
 class ProjectedLogProbs(NamedTuple):
-    """What ``projected_logprobs`` returns, float32 and of the shape of the tokens.  peak and total: the row's largest logit, and the sum of e^(logit - peak)."""
+    """What ``projected_logprobs`` returns, float32 and of the shape of the tokens.  peak and total are for the backward pass: a multiple of 1/8 next to the row's
+    largest logit times log2(e), and the sum of 2^(logit log2(e) - peak)."""
     logp: torch.Tensor
     lse: torch.Tensor
     peak: torch.Tensor
@@ -582,8 +583,8 @@ def projected_logprobs(x, weight, tokens, ignore=-100):
     x       [..., channels], the channels of a row next to one another
     weight  [vocabulary, channels], of the type of ``x``: a row for each token, the channels next to one another
     tokens  int64 [...]; ``ignore`` where a row has none (padding): its logp is 0.  A token outside the vocabulary has logp NaN
-    Rows whose logits hold NaN or +inf have lse and logp NaN.  float32 arguments are multiplied in parts of 16 bits that hold all their bits; what is not finite in
-    them makes the rows that meet it NaN."""
+    Rows whose logits hold NaN or +inf have lse and logp NaN.  Weights are meant to be finite: one that is not makes every row NaN.  float32 arguments of more than
+    64 rows are multiplied in three parts of 16 bits that hold all their bits."""
     r = _native.projected_logprobs(x, weight, tokens, ignore)
     if r is not None:
         return ProjectedLogProbs(*r)
@@ -601,7 +602,7 @@ def projected_logprobs_bwd(x, weight, tokens, fwd, d_logp, ignore=-100):
     """(dx, d_weight), of the types and shapes of ``x`` and ``weight``, from the gradient of logp, ``d_logp`` (float32, of the shape of the tokens).
 
     x, weight, tokens, ignore: as they were; fwd: what ``projected_logprobs`` returned.  Rows without a token have a gradient of 0 and no part in d_weight, whatever
-    they hold.  The logits are made again, in pieces of up to 512 MB of the vocabulary, with p rounded to 16 bits (of float32: in three parts); float16
+    they hold; a row whose token lies outside the vocabulary, or whose logits hold NaN or +inf, makes its own gradient and all of d_weight NaN.  The logits are made again, in pieces of up to 512 MB of the vocabulary, with p rounded to 16 bits (of float32: in three parts); float16
     holds no gradient below 6e-8: give it a scaled d_logp, as a mean over many rows needs."""
     r = _native.projected_logprobs_bwd(x, weight, tokens, fwd.peak, fwd.total, d_logp, ignore)
     if r is not None:

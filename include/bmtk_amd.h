@@ -781,8 +781,9 @@ int bmtk_short_conv_bwd(int64_t n_steps, int64_t batch, int32_t dim, int32_t wid
  * x_t .. read_b: distance of steps and of sequences, in elements; the channels of a step, and its groups' states, lie next to one another; everything else
  * is contiguous.  marks (NULL: not kept): the state before every BMTK_SCAN_MARK-th step, [ceil(n_steps / BMTK_SCAN_MARK)][batch][dim][n_states],
  * which the backward pass needs.  delta * rate of up to 0, or such that e to its sums over any steps in a row stays in 32 bits; of a state that decays to less,
- * up to 2^-126 of what it was may be left.
- * Limits: n_states in 1 .. BMTK_SELECTIVE_MAX_STATES, batch * dim < 2^31, n_steps < 2^31 - 4096. */
+ * up to 2^-126 of what it was may be left.  Rates are meant to be finite.
+ * Limits: n_states in 1 .. BMTK_SELECTIVE_MAX_STATES, batch * dim < 2^31, n_steps < 2^31 - 4096; with P n_states to a multiple of four, n_steps * batch * groups * P,
+ * batch * dim * P and 16 dim P below 2^32, channels of a group counted in 64s. */
 #define BMTK_SELECTIVE_MAX_STATES 64
 int64_t bmtk_selective_scan_workspace_bytes(int64_t n_steps, int64_t batch, int32_t dim, int32_t groups, int32_t n_states, int32_t backward);
 int bmtk_selective_scan_fwd(int64_t n_steps, int64_t batch, int32_t dim, int32_t groups, int32_t n_states, int32_t dtype, int32_t dt_dtype, int32_t softplus, const void *x,
@@ -798,16 +799,17 @@ int bmtk_selective_scan_bwd(int64_t n_steps, int64_t batch, int32_t dim, int32_t
                             float *d_dt_bias, float *d_state, float *workspace, void *stream);
 
 /* Of each of `rows` rows of x (x_stride numbers apart), with logits l[v] = x . weight[v] over `dim` channels: lse = log of the sum of e^l, logp = l[token] - lse (0 where
- * the token is `ignore`, NaN where it lies outside 0 .. vocab - 1), peak = the largest logit, total = the sum of e^(l - peak).  The logits are not kept.
+ * the token is `ignore`, NaN where it lies outside 0 .. vocab - 1), peak = a multiple of 1/8 next to the largest logit times log2(e), total = the sum
+ * of 2^(l log2(e) - peak).  The logits are not kept.
  * weight: vocab rows, weight_stride numbers apart.  Rows whose logits hold NaN or +inf have lse and logp NaN.  Sums are in 32 bits; fp32 operands are taken as three
- * bf16 parts each, six of their products (a row that meets an fp32 operand that is not finite is NaN).
- * Limits: rows < 2^22, vocab < 2^28, dim up to 65,536, strides below 2^21. */
+ * bf16 parts each, six of their products, or, of few rows, by fp32 instructions.  Weights are meant to be finite: one that is not makes every row NaN.
+ * Limits: rows < 2^22, vocab < 2^28, dim up to 65,536, strides below 2^21; vocab * dim < 2^35, rows * dim < 2^34, and 2^31 squares of 128 x 128 logits. */
 int64_t bmtk_projected_logprobs_workspace_bytes(int64_t rows, int32_t vocab, int32_t dim, int32_t dtype, const void *x, int64_t x_stride, const void *weight,
                                                 int64_t weight_stride, int32_t backward);
 int bmtk_projected_logprobs_fwd(int64_t rows, int32_t vocab, int32_t dim, int32_t dtype, const void *x, int64_t x_stride, const void *weight, int64_t weight_stride,
                                 const int64_t *tokens, int64_t ignore, float *logp, float *lse, float *peak, float *total, void *workspace, void *stream);
 /* dx [rows][dim], d_weight [vocab][dim], contiguous and of dtype, from d_logp [rows]; peak and total are the forward pass's.  Rows without a token have dx 0 and no part in
- * d_weight, whatever they hold.  Logits are made again in pieces of the vocabulary of up to 512 MB. */
+ * d_weight, whatever they hold; a row whose token lies outside the vocabulary, or whose logits hold NaN or +inf, makes its dx and all of d_weight NaN.  Logits are made again in pieces of the vocabulary of up to 512 MB. */
 int bmtk_projected_logprobs_bwd(int64_t rows, int32_t vocab, int32_t dim, int32_t dtype, const void *x, int64_t x_stride, const void *weight, int64_t weight_stride,
                                 const int64_t *tokens, int64_t ignore, const float *peak, const float *total, const float *d_logp, void *dx, void *d_weight, void *workspace,
                                 void *stream);
