@@ -399,6 +399,8 @@ int run(const char *name, int32_t dtype, int32_t weight_dtype, ConvArgs &a, bool
     a.stretch = stretch_of(a.n_steps, a.batch, a.dim, v);
     const int64_t across = div_up(a.batch * a.vectors, 256), down = div_up(a.n_steps, a.stretch);
     BMTK_REQUIRE(across * 256 < (int64_t{1} << 31), "%s: too many columns", name);
+    // (sixteen threads of the sums' launch for each weight and bias)
+    BMTK_REQUIRE(!backward || (int64_t)a.dim * (a.width + 1) < (int64_t{1} << 28), "%s: too many weights for a launch", name);
     // (stretches are a launch's second size, so that 2^32 threads are never asked for in one)
     const hipStream_t s = static_cast<hipStream_t>(stream);
     const dim3 grid((uint32_t)across, (uint32_t)down);

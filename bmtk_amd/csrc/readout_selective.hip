@@ -654,8 +654,13 @@ struct Plan {
 
 bool sizes_fit(int64_t n_steps, int64_t batch, int32_t dim, int32_t groups, int32_t n_states)
 {
-    return n_steps > 0 && batch > 0 && dim > 0 && groups > 0 && dim % groups == 0 && n_states > 0 && n_states <= BMTK_SELECTIVE_MAX_STATES && n_steps < (int64_t{1} << 31) - 4096 &&
-           batch < (int64_t{1} << 31) && batch * dim < (int64_t{1} << 31);
+    if (!(n_steps > 0 && batch > 0 && dim > 0 && groups > 0 && dim % groups == 0 && n_states > 0 && n_states <= BMTK_SELECTIVE_MAX_STATES && n_steps < (int64_t{1} << 31) - 4096 &&
+          batch < (int64_t{1} << 31) && batch * dim < (int64_t{1} << 31)))
+        return false;
+    // 2^32 threads a launch: one for each state of a step, of a channel; sixteen where a channel's sums are put together, lanes without a channel with the others
+    const int64_t most = int64_t{1} << 32, padded = div_up(n_states, kOwn) * kOwn, rows = div_up(n_steps, kSteps) * kSteps * batch * groups;
+    const int64_t lanes = batch * groups * div_up(dim / groups, kWave) * kWave;
+    return rows < most && rows * padded < most && batch * dim * padded < most && (int64_t)dim * padded < most / 16 - 4096 && lanes < most && lanes * (padded / kOwn) < most;
 }
 
 template <typename T, typename TD, int Waves, int Rows>
@@ -738,14 +743,12 @@ int run(const char *name, SelArgs &a, int32_t dtype, int32_t dt_dtype, bool back
     BMTK_REQUIRE(a.n_states <= BMTK_SELECTIVE_MAX_STATES, "%s: up to %d states, got %d", name, BMTK_SELECTIVE_MAX_STATES, a.n_states);
     BMTK_REQUIRE(dtype >= 0 && dtype <= 2, "%s: unknown type %d", name, dtype);
     BMTK_REQUIRE(dt_dtype == BMTK_F32 || dt_dtype == dtype, "%s: dt must be float32 or of the type of x", name);
-    BMTK_REQUIRE(sizes_fit(a.n_steps, a.batch, a.dim, a.groups, a.n_states), "%s: too many steps or columns", name);
+    BMTK_REQUIRE(sizes_fit(a.n_steps, a.batch, a.dim, a.groups, a.n_states), "%s: too many steps, columns or states", name);
     if (!backward && few_steps(a.n_steps, a.batch, a.dim)) {
         BMTK_BY_TYPE(dtype, T, { return dt_dtype == BMTK_F32 ? launch_step<T, float>(name, a, s) : launch_step<T, T>(name, a, s); });
     }
     const Plan plan(a.n_steps, a.batch, a.dim, a.groups, a.n_states, backward);
-    const int64_t across = a.batch * a.groups * plan.tiles, rows = plan.padded_steps * a.batch * a.groups, columns = a.batch * a.dim;
-    BMTK_REQUIRE(across * plan.waves * kWave < (int64_t{1} << 32) && rows * plan.padded < (int64_t{1} << 32) && columns * plan.padded < (int64_t{1} << 32),
-                 "%s: too many states for a launch", name);
+    const int64_t across = a.batch * a.groups * plan.tiles, rows = plan.padded_steps * a.batch * a.groups;
     BMTK_REQUIRE(workspace, "%s: needs a workspace", name);
     plan.place(a, workspace);
     BMTK_BY_TYPE(dtype, T, { spread_kernel<T><<<(uint32_t)div_up(rows * plan.padded, 256), 256, 0, s>>>(a, rows); });
