@@ -109,6 +109,53 @@ def label_loss(bits, batch, weight, decay, labels, ignore=-100, state=None, top=
     return loss, dl_dz, {"weight": d_weight.to(given[0].dtype), "decay": d_decay.to(given[1].dtype), "state": d_state}, answer
 
 
+def sequence_loss(bits, batch, weight, conv_weight, rate, out_weight, labels, conv_bias=None, skip=None, dt_bias=None, groups=1, ignore=-100, memory=None):
+    """Cross entropy of the labels (tokens) that a trained readout with a memory should answer, and its derivatives.
+
+    bits    int64 [steps, words] spike bits of a run of ``batch`` trials (``fwd["bits"]``)
+    weight  [neurons, channels + 2 * groups * states + channels]: the weights of a spike for the memory's input, for what it writes and reads, and for the
+            step sizes, in this order (``readout.spike_readout``)
+    conv_weight  [channels + 2 * groups * states, width], conv_bias: the short convolution with a sigmoid gate that input, write and read pass (``readout.short_conv``)
+    rate    float32 [channels, states], skip, dt_bias float32 [channels]: the memory, its step sizes through softplus (``readout.selective_scan``)
+    out_weight  [vocabulary, channels], of the type of ``weight``: the classes' probabilities are the softmax of the memory's output times these, which never are in
+            memory at once (``readout.projected_logprobs``).  What lies between the stages and its gradients have the type of ``weight``, rounded once each; of
+            float16 weights float32: a mean over many labels leaves each a gradient below what float16 holds
+    labels  int64 [steps, batch]: the class wanted in each step and trial, ``ignore`` where none is
+    memory  (convolution's last inputs, state) of the steps before, as returned (None: zero)
+    Returns (loss, dl_dz, gradients, answer, memory): the mean of -log p(label) over the steps and trials that have one; dl_dz float32 [steps, neurons * batch], what
+    ``Glif3Bptt.backward`` takes; a dict of the gradients by the arguments' names, "conv_state" and "state"; the ``readout.ProjectedLogProbs`` of every step and
+    trial; and the memory behind the last step, which takes no part in the loss.  Nothing synchronises."""
+    given = dict(weight=weight, conv_weight=conv_weight, conv_bias=conv_bias, rate=rate, out_weight=out_weight, skip=skip, dt_bias=dt_bias)
+    for name in ("rate", "weight"):
+        if not isinstance(given[name], torch.Tensor) or given[name].dim() != 2:
+            raise ValueError("{} must be a tensor of two dimensions".format(name))
+    wide = lambda t: t.float() if isinstance(t, torch.Tensor) and t.dtype == torch.float16 else t  # noqa: E731
+    conv_state, state = (None, None) if memory is None else memory
+    weight, conv_weight, conv_bias, out_weight, conv_state = wide(weight), wide(conv_weight), wide(conv_bias), wide(out_weight), wide(conv_state)
+    channels, states = rate.shape
+    shared = groups * states
+    mixed = channels + 2 * shared
+    if groups < 1 or weight.shape[1] != mixed + channels:
+        raise ValueError("weight must be [neurons, {}] for {} channels of {} states in {} groups, got {}".format(mixed + channels, channels, states, groups, tuple(weight.shape)))
+    y = readout.spike_readout(bits, weight, batch)
+    conv_in, dt = y[:, :, :mixed], y[:, :, mixed:]
+    m, conv_last = readout.short_conv(conv_in, conv_weight, conv_bias, conv_state, silu=True)
+    per_group = lambda t: t.unflatten(2, (groups, states))  # noqa: E731
+    inputs = m[:, :, :channels], dt, rate, per_group(m[:, :, channels:channels + shared]), per_group(m[:, :, channels + shared:])
+    h, last, saved = readout.selective_scan(*inputs, skip=skip, dt_bias=dt_bias, softplus=True, state=state, save_state=True)
+    answer = readout.projected_logprobs(h, out_weight, labels, ignore=ignore)
+    share = 1.0 / _total(labels != ignore).clamp_(min=1).to(torch.float32)
+    loss = -_total(answer.logp) * share
+    dh, d_out = readout.projected_logprobs_bwd(h, out_weight, labels, answer, (-share).expand(labels.shape).contiguous(), ignore=ignore)
+    d = readout.selective_scan_bwd(*inputs, saved, dh, skip=skip, dt_bias=dt_bias, softplus=True)
+    dm = torch.cat([d.dx, d.d_write.flatten(2), d.d_read.flatten(2)], 2)
+    d_in, d_conv, d_bias, d_conv_state = readout.short_conv_bwd(conv_in, conv_weight, dm, conv_bias, conv_state, silu=True)
+    d_weight, dl_dz = readout.spike_readout_bwd(bits, weight, torch.cat([d_in, d.d_dt], 2), batch)
+    gradients = dict(weight=d_weight, conv_weight=d_conv, conv_bias=d_bias, rate=d.d_rate, out_weight=d_out, skip=d.d_skip, dt_bias=d.d_dt_bias)
+    gradients = {name: g if given[name] is None else g.to(given[name].dtype) for name, g in gradients.items()}
+    return loss, dl_dz, dict(gradients, conv_state=d_conv_state, state=d.d_state), answer, (conv_last, last)
+
+
 class Glif3Bptt:
     """Reverse-time adjoint over a recorded forward run of a ``Glif3Simulator``: of a batch, or of a single trial
     built with ``resident=False``.  (A batch whose simulator leaves ``resident`` at "auto" runs the forward part with
