@@ -17,6 +17,7 @@ namespace {
 constexpr int kTile = 32;          // of a matrix instruction
 constexpr int kDepth = 64;         // k of a step: 128 bytes a row
 constexpr int kWaitReads = 0xc07f, kWaitLoads = 0x0f70, kWaitAll = 0x70;   // s_waitcnt of all LDS operations, of all loads, of both
+constexpr int kSmallMost = 128;    // of a small vocabulary
 constexpr float kLog2e = 1.44269504f, kLn2 = 0.693147181f;
 
 typedef float Acc __attribute__((ext_vector_type(16)));
@@ -70,23 +71,23 @@ struct Loose8 {
     }
 };
 
-// four numbers, `some` of them there, the others 0
-template <typename T>
-struct Loose4 {
-    typedef uint32_t Words __attribute__((ext_vector_type(sizeof(T))));
+// C numbers (two or four), `some` of them there, the others 0
+template <typename T, int C>
+struct LooseFew {
+    typedef uint32_t Words __attribute__((ext_vector_type(C * sizeof(T) / 4)));
     typedef Words Loose __attribute__((aligned(2)));
     union {
         Words w;
-        T v[4];
+        T v[C];
     };
-    __device__ __forceinline__ Loose4() {}
+    __device__ __forceinline__ LooseFew() {}
     __device__ __forceinline__ void load(const T *p, int some)
     {
-        if (some >= 4) {
+        if (some >= C) {
             w = *reinterpret_cast<const Loose *>(p);
         } else {
 #pragma unroll
-            for (int q = 0; q < 4; ++q) v[q] = q < some ? p[q] : (T)0.0f;
+            for (int q = 0; q < C; ++q) v[q] = q < some ? p[q] : (T)0.0f;
         }
     }
 };
@@ -122,18 +123,24 @@ __device__ __forceinline__ float2 join(float2 u, float2 v)
     return make_float2(m, u.y * __builtin_amdgcn_exp2f(u.x - from) + v.y * __builtin_amdgcn_exp2f(v.x - from));
 }
 
-// four numbers to where they begin anywhere
-template <typename T>
-__device__ __forceinline__ void put4(T *p, const Acc4 &v)
+// the first `some` of C numbers (two or four) to where they begin anywhere
+template <typename T, int C>
+__device__ __forceinline__ void put(T *p, const float (&v)[C], int some)
 {
-    typedef uint32_t Words __attribute__((ext_vector_type(sizeof(T))));
+    typedef uint32_t Words __attribute__((ext_vector_type(C * sizeof(T) / 4)));
     typedef Words Loose __attribute__((aligned(2)));
-    T q[4];
+    T q[C];
 #pragma unroll
-    for (int r = 0; r < 4; ++r) q[r] = (T)v[r];
-    Words w;
-    __builtin_memcpy(&w, q, sizeof(w));
-    *reinterpret_cast<Loose *>(p) = w;
+    for (int r = 0; r < C; ++r) q[r] = (T)v[r];
+    if (some >= C) {
+        Words w;
+        __builtin_memcpy(&w, q, sizeof(w));
+        *reinterpret_cast<Loose *>(p) = w;
+    } else {
+#pragma unroll
+        for (int r = 0; r < C - 1; ++r)
+            if (r < some) p[r] = q[r];
+    }
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -574,21 +581,15 @@ __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void product_kernel(Product p)
                     for (int q = 0; q < 4; ++q) {
                         const int32_t col = ii0 + i * kTile + 8 * q + 4 * half;
                         if (col >= p.ni) continue;
-                        Acc4 v;
+                        float v[4];
 #pragma unroll
                         for (int r = 0; r < 4; ++r) v[r] = acc[i][j][q * 4 + r] * scale;
                         if constexpr (Mode == kSlab) {   // (rows of a slab are whole fours)
                             Acc4 *to = reinterpret_cast<Acc4 *>(p.slab + out_slice * p.slab_size + row * p.slab_stride + col);
-                            *to = p.add ? *to + v : v;
+                            const Acc4 sum = {v[0], v[1], v[2], v[3]};
+                            *to = p.add ? *to + sum : sum;
                         } else {
-                            T *to = static_cast<T *>(p.out) + (int64_t)row * p.ni + col;
-                            if (col + 4 <= p.ni) {
-                                put4<T>(to, v);
-                            } else {
-#pragma unroll
-                                for (int r = 0; r < 4; ++r)
-                                    if (col + r < p.ni) to[r] = (T)v[r];
-                            }
+                            put<T, 4>(static_cast<T *>(p.out) + (int64_t)row * p.ni + col, v, p.ni - col);
                         }
                     }
             }
@@ -675,7 +676,7 @@ __global__ __launch_bounds__(1024) void weigh_kernel(const float *d_logp, const 
 }
 
 // a row's results from its base and sum
-__device__ __forceinline__ void finish(float2 sum, int32_t row, const float *label, const int64_t *tokens, int64_t ignore, int32_t vocab, float *logp, float *lse, float *peak, float *total)
+__device__ __forceinline__ void finish(float2 sum, int32_t row, float label, const int64_t *tokens, int64_t ignore, int32_t vocab, float *logp, float *lse, float *peak, float *total)
 {
     const float m = sum.x, s = sum.y, log_total = logf(s);
     const float l = m == -INFINITY && s == 0.0f ? -INFINITY : fmaf(m, kLn2, log_total);
@@ -683,7 +684,7 @@ __device__ __forceinline__ void finish(float2 sum, int32_t row, const float *lab
     peak[row] = m;
     total[row] = s;
     lse[row] = m == INFINITY ? NAN : l;
-    logp[row] = token == ignore ? 0.0f : token < 0 || token >= vocab || m == INFINITY ? NAN : l == -INFINITY ? -INFINITY : fmaf(fmaf(label[row], kLog2e, -m), kLn2, -log_total);
+    logp[row] = token == ignore ? 0.0f : token < 0 || token >= vocab || m == INFINITY ? NAN : l == -INFINITY ? -INFINITY : fmaf(fmaf(label, kLog2e, -m), kLn2, -log_total);
 }
 
 // each row's tiles joined: a workgroup takes 64 rows, each of its 16 wavefronts every sixteenth tile
@@ -708,7 +709,7 @@ __global__ __launch_bounds__(1024) void stats_join_kernel(const float2 *stats, i
     __syncthreads();
     if (wave != 0 || row >= rows) return;
     for (int k = 1; k < 16; ++k) sum = join(sum, parts[k][lane]);
-    finish(sum, row, label, tokens, ignore, vocab, logp, lse, peak, total);
+    finish(sum, row, label[row], tokens, ignore, vocab, logp, lse, peak, total);
 }
 // Results from their slabs: rows of `width` numbers, n of them there.  `ways` wavefronts of a workgroup share 64 times four numbers, each takes every so manieth slab.
 template <typename T>
@@ -741,15 +742,8 @@ __global__ __launch_bounds__(1024) void slab_join_kernel(const float *slab, int3
     }
     if (!there) return;
     const float w = by ? by[row] : 1.0f, f = scale * (factor ? *factor : 1.0f) * w;
-    const Acc4 r = {w == 0.0f ? 0.0f : v[0] * f, w == 0.0f ? 0.0f : v[1] * f, w == 0.0f ? 0.0f : v[2] * f, w == 0.0f ? 0.0f : v[3] * f};
-    T *to = out + row * n + c;
-    if (c + 4 <= n) {
-        put4<T>(to, r);
-    } else {
-#pragma unroll
-        for (int q = 0; q < 3; ++q)
-            if (c + q < n) to[q] = (T)r[q];
-    }
+    const float r[4] = {w == 0.0f ? 0.0f : v[0] * f, w == 0.0f ? 0.0f : v[1] * f, w == 0.0f ? 0.0f : v[2] * f, w == 0.0f ? 0.0f : v[3] * f};
+    put<T, 4>(out + row * n + c, r, n - c);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -772,15 +766,98 @@ struct Few {
     int32_t slices, slice_rows;            // slices of the vocabulary, of so many of its rows (a multiple of 16)
 };
 
+// acc[i][j] += the products of 16 rows of I tiles by 16 rows of J tiles, over the steps of 32 k from first to end; p, q: where this lane's rows have their first eight k
+template <typename T, int I, int J>
+__device__ __forceinline__ void multiply_rows(const T *const (&p)[I], const T *const (&q)[J], int32_t first, int32_t end, int32_t dim, int quarter, Acc4 (&acc)[I][J])
+{
+    typedef typename Element<T>::type E;
+    typedef typename Vec<E>::V8 V8;
+    const auto multiply = [&](const Loose8<T> (&u)[I], const Loose8<T> (&v)[J]) {
+        if constexpr (std::is_same<T, float>::value) {
+            // (fp32 operands in fp32 instructions, one k of a lane's eight each: at so few rows they keep up with memory)
+#pragma unroll
+            for (int k = 0; k < 8; ++k)
+#pragma unroll
+                for (int i = 0; i < I; ++i)
+#pragma unroll
+                    for (int j = 0; j < J; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(u[i].v[k], v[j].v[k], acc[i][j], 0, 0, 0);
+        } else {
+            V8 uv[I], vv[J];
+#pragma unroll
+            for (int i = 0; i < I; ++i) __builtin_memcpy(&uv[i], &u[i], 16);
+#pragma unroll
+            for (int j = 0; j < J; ++j) __builtin_memcpy(&vv[j], &v[j], 16);
+#pragma unroll
+            for (int i = 0; i < I; ++i)
+#pragma unroll
+                for (int j = 0; j < J; ++j) acc[i][j] = Vec<E>::mfma16(uv[i], vv[j], acc[i][j]);
+        }
+    };
+    constexpr int kAhead = (std::is_same<T, float>::value ? 2 : 4) / (I + J > 4 ? 2 : 1);   // steps of 32 k that are asked for at once
+    const int32_t whole = min(end, dim / 32);
+    const auto ask = [&](int32_t k, Loose8<T> (&u)[kAhead][I], Loose8<T> (&v)[kAhead][J]) {
+#pragma unroll
+        for (int s = 0; s < kAhead; ++s) {
+#pragma unroll
+            for (int i = 0; i < I; ++i) u[s][i].load(p[i] + (k + s) * 32);
+#pragma unroll
+            for (int j = 0; j < J; ++j) v[s][j].load(q[j] + (k + s) * 32);
+        }
+    };
+    int32_t k = first;
+    if (k + kAhead <= whole) {
+        Loose8<T> u_next[kAhead][I], v_next[kAhead][J];
+        ask(k, u_next, v_next);
+        for (; k + kAhead <= whole; k += kAhead) {
+            Loose8<T> u[kAhead][I], v[kAhead][J];
+#pragma unroll
+            for (int s = 0; s < kAhead; ++s) {
+#pragma unroll
+                for (int i = 0; i < I; ++i) u[s][i] = u_next[s][i];
+#pragma unroll
+                for (int j = 0; j < J; ++j) v[s][j] = v_next[s][j];
+            }
+            if (k + 2 * kAhead <= whole) ask(k + kAhead, u_next, v_next);
+#pragma unroll
+            for (int s = 0; s < kAhead; ++s) multiply(u[s], v[s]);
+        }
+    }
+    for (; k < end; ++k) {
+        Loose8<T> u[I], v[J];
+        const int n = dim - k * 32 - quarter * 8;
+#pragma unroll
+        for (int i = 0; i < I; ++i) u[i].load_some(p[i] + k * 32, n);
+#pragma unroll
+        for (int j = 0; j < J; ++j) v[j].load_some(q[j] + k * 32, n);
+        multiply(u, v);
+    }
+}
+
+// where the wavefronts of a workgroup share a sum: all of it in the first one's registers
+template <int Split, int I, int J>
+__device__ __forceinline__ void add_up(Acc4 (&acc)[I][J], Acc4 (&sums)[Split - 1][I][J][64], int wave, int lane)
+{
+    if (wave > 0) {
+#pragma unroll
+        for (int i = 0; i < I; ++i)
+#pragma unroll
+            for (int j = 0; j < J; ++j) sums[wave - 1][i][j][lane] = acc[i][j];
+    }
+    __syncthreads();
+    if (wave > 0) return;
+    for (int w = 0; w < Split - 1; ++w)
+#pragma unroll
+        for (int i = 0; i < I; ++i)
+#pragma unroll
+            for (int j = 0; j < J; ++j) acc[i][j] += sums[w][i][j][lane];
+}
+
 // Split: wavefronts of a workgroup that share 32 rows of the weights, each a part of the channels.
 template <typename T, int J, int Split, bool Gradient>
 __global__ __launch_bounds__(Split == 8 ? 512 : 256) void few_rows_kernel(Few a)
 {
-    typedef typename Element<T>::type E;
-    typedef typename Vec<E>::V8 V8;
     constexpr int kBlocks = Split == 1 ? 4 : 1;   // of 32 rows
     __shared__ float2 parts[kBlocks][J * 16];
-    __shared__ Acc4 sums[Split == 1 ? 1 : Split - 1][2][J][64];
     const int lane = lane_id(), wave = threadIdx.x / kWave, r16 = lane & 15, quarter = lane >> 4;
     const int32_t v0 = (blockIdx.x * kBlocks + (Split == 1 ? wave : 0)) * 32;
     const T *w_row[2], *x_row[J];
@@ -793,80 +870,12 @@ __global__ __launch_bounds__(Split == 8 ? 512 : 256) void few_rows_kernel(Few a)
     for (int i = 0; i < 2; ++i)
 #pragma unroll
         for (int j = 0; j < J; ++j) acc[i][j] = Acc4{0.0f, 0.0f, 0.0f, 0.0f};
-    const auto multiply = [&](const Loose8<T> (&w)[2], const Loose8<T> (&x)[J]) {
-        if constexpr (std::is_same<T, float>::value) {
-            // (fp32 operands in fp32 instructions, one k of a lane's eight each: at so few rows they keep up with memory)
-#pragma unroll
-            for (int k = 0; k < 8; ++k)
-#pragma unroll
-                for (int i = 0; i < 2; ++i)
-#pragma unroll
-                    for (int j = 0; j < J; ++j) acc[i][j] = __builtin_amdgcn_mfma_f32_16x16x4f32(w[i].v[k], x[j].v[k], acc[i][j], 0, 0, 0);
-        } else {
-            V8 wv[2], xv[J];
-#pragma unroll
-            for (int i = 0; i < 2; ++i) __builtin_memcpy(&wv[i], &w[i], 16);
-#pragma unroll
-            for (int j = 0; j < J; ++j) __builtin_memcpy(&xv[j], &x[j], 16);
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < J; ++j) acc[i][j] = Vec<E>::mfma16(wv[i], xv[j], acc[i][j]);
-        }
-    };
-    constexpr int kAhead = (std::is_same<T, float>::value ? 2 : 4) / (J == 4 ? 2 : 1);   // steps of 32 k that are asked for at once
     const int32_t steps = (a.dim + 31) / 32, part = Split == 1 ? 0 : wave;
-    const int32_t first = steps * part / Split, end = steps * (part + 1) / Split, whole = min(end, a.dim / 32);
-    const auto ask = [&](int32_t k, Loose8<T> (&w)[kAhead][2], Loose8<T> (&x)[kAhead][J]) {
-#pragma unroll
-        for (int u = 0; u < kAhead; ++u) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i) w[u][i].load(w_row[i] + (k + u) * 32);
-#pragma unroll
-            for (int j = 0; j < J; ++j) x[u][j].load(x_row[j] + (k + u) * 32);
-        }
-    };
-    int32_t k = first;
-    if (k + kAhead <= whole) {
-        Loose8<T> w_next[kAhead][2], x_next[kAhead][J];
-        ask(k, w_next, x_next);
-        for (; k + kAhead <= whole; k += kAhead) {
-            Loose8<T> w[kAhead][2], x[kAhead][J];
-#pragma unroll
-            for (int u = 0; u < kAhead; ++u) {
-#pragma unroll
-                for (int i = 0; i < 2; ++i) w[u][i] = w_next[u][i];
-#pragma unroll
-                for (int j = 0; j < J; ++j) x[u][j] = x_next[u][j];
-            }
-            if (k + 2 * kAhead <= whole) ask(k + kAhead, w_next, x_next);
-#pragma unroll
-            for (int u = 0; u < kAhead; ++u) multiply(w[u], x[u]);
-        }
-    }
-    for (; k < end; ++k) {
-        Loose8<T> w[2], x[J];
-        const int n = a.dim - k * 32 - quarter * 8;
-#pragma unroll
-        for (int i = 0; i < 2; ++i) w[i].load_some(w_row[i] + k * 32, n);
-#pragma unroll
-        for (int j = 0; j < J; ++j) x[j].load_some(x_row[j] + k * 32, n);
-        multiply(w, x);
-    }
+    multiply_rows<T, 2, J>(w_row, x_row, steps * part / Split, steps * (part + 1) / Split, a.dim, quarter, acc);
     if constexpr (Split > 1) {
-        if (wave > 0) {
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < J; ++j) sums[wave - 1][i][j][lane] = acc[i][j];
-        }
-        __syncthreads();
+        __shared__ Acc4 sums[Split - 1][2][J][64];
+        add_up<Split>(acc, sums, wave, lane);
         if (wave > 0) return;
-        for (int w = 0; w < Split - 1; ++w)
-#pragma unroll
-            for (int i = 0; i < 2; ++i)
-#pragma unroll
-                for (int j = 0; j < J; ++j) acc[i][j] += sums[w][i][j][lane];
     }
     // lane l has column j = l % 16 of a tile and its rows i = 4 (l / 16) + r
 #pragma unroll
@@ -919,47 +928,57 @@ __global__ __launch_bounds__(Split == 8 ? 512 : 256) void few_rows_kernel(Few a)
     }
 }
 
-// The two products of G for few rows, in one pass over the weights: a wavefront takes 64 channels (a lane four) of a slice of the vocabulary, and per 16 of its rows
+// The two products of G for few rows, in one pass over the weights: a wavefront takes 16 C channels (a lane C) of a slice of the vocabulary, and per 16 of its rows
 //     dx[r][d] -= G[v][r] w[v][d]   and   d_weight[v][d] = -sum_r G[v][r] d_logp[r] x[r][d]
-// in matrix instructions of 32 bits, which take one k a lane: nothing has to be transposed, and a lane's four channels are four tiles.  Bound by memory: the weights
+// in matrix instructions of 32 bits, which take one k a lane: nothing has to be transposed, and a lane's C channels are C tiles.  Bound by memory: the weights
 // read, their gradient written.
-template <typename T, int J>
+// Classes: a small vocabulary and many rows, the two in each other's place, with G times d_logp already; rows that have no part (weights of 0) may hold anything.  A workgroup's
+// wavefronts share a slice of the rows and add up.
+template <typename T, int J, int C, bool Classes>
 __global__ __launch_bounds__(256) void few_back_kernel(Few a)
 {
-    typedef Loose4<T> In;
+    typedef LooseFew<T, C> In;
     const int lane = lane_id(), wave = threadIdx.x / kWave, r16 = lane & 15, kk = lane >> 4;
-    const int32_t d = (blockIdx.x * 4 + wave) * 64 + r16 * 4;
-    const int32_t some = a.dim - d;   // this lane's channels that are there, if fewer than four
-    if ((blockIdx.x * 4 + wave) * 64 >= a.dim) return;
+    const int32_t d0 = (Classes ? blockIdx.x : blockIdx.x * 4 + wave) * (16 * C), d = d0 + r16 * C;
+    const int32_t some = a.dim - d;   // this lane's channels that are there, if fewer than C
+    if (d0 >= a.dim) return;
     // x d_logp, 4 kk + m of each 16 rows: what a lane's k is in product m
-    float xw[J][4][4];
+    float xw[J][4][C];
 #pragma unroll
     for (int j = 0; j < J; ++j)
 #pragma unroll
         for (int m = 0; m < 4; ++m) {
             const int32_t row = j * 16 + kk * 4 + m;
-            const float by = row < a.rows ? a.weights[row] : 0.0f;
+            const float by = row >= a.rows ? 0.0f : Classes ? 1.0f : a.weights[row];
             In x;
             x.load(static_cast<const T *>(a.x) + (int64_t)min(row, a.rows - 1) * a.x_stride + d, some);
 #pragma unroll
-            for (int q = 0; q < 4; ++q) xw[j][m][q] = by == 0.0f ? 0.0f : -by * (float)x.v[q];
+            for (int q = 0; q < C; ++q) xw[j][m][q] = by == 0.0f ? 0.0f : -by * (float)x.v[q];
         }
-    Acc4 dx[J][4];
+    Acc4 dx[J][C];
 #pragma unroll
     for (int j = 0; j < J; ++j)
 #pragma unroll
-        for (int q = 0; q < 4; ++q) dx[j][q] = Acc4{0.0f, 0.0f, 0.0f, 0.0f};
-    const int32_t v_first = blockIdx.y * a.slice_rows, v_end = min(v_first + a.slice_rows, a.vocab);
-    const auto ask = [&](int32_t v, In (&w)[4]) {
+        for (int q = 0; q < C; ++q) dx[j][q] = Acc4{0.0f, 0.0f, 0.0f, 0.0f};
+    constexpr int kEach = Classes ? 64 : 16;   // rows that a workgroup, or a wavefront of its own, goes on by
+    const int32_t v_end = min((int32_t)(blockIdx.y + 1) * a.slice_rows, a.vocab), v_first = blockIdx.y * a.slice_rows + (Classes ? wave * 16 : 0);
+    const auto ask = [&](int32_t v, In (&w)[4], float (&part)[4]) {
 #pragma unroll
-        for (int u = 0; u < 4; ++u) w[u].load(static_cast<const T *>(a.weight) + (int64_t)min(v + u * 4 + kk, a.vocab - 1) * a.w_stride + d, some);
+        for (int u = 0; u < 4; ++u) {
+            const int32_t at = min(v + u * 4 + kk, a.vocab - 1);
+            w[u].load(static_cast<const T *>(a.weight) + (int64_t)at * a.w_stride + d, some);
+            if (Classes) part[u] = a.weights[at];
+        }
     };
     In next[4];
-    ask(v_first, next);
-    for (int32_t v = v_first; v < v_end; v += 16) {
-        In w[4];
+    float next_part[4];
+    ask(v_first, next, next_part);
+    for (int32_t v = v_first; v < v_end; v += kEach) {
+        float w[4][C];
 #pragma unroll
-        for (int u = 0; u < 4; ++u) w[u] = next[u];
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int q = 0; q < C; ++q) w[u][q] = Classes && next_part[u] == 0.0f ? 0.0f : (float)next[u].v[q];
         float by_row[J][4];
         Acc4 by_vocab[J];
 #pragma unroll
@@ -968,34 +987,34 @@ __global__ __launch_bounds__(256) void few_back_kernel(Few a)
             for (int u = 0; u < 4; ++u) by_row[j][u] = a.g[(int64_t)(v + u * 4 + kk) * (J * 16) + j * 16 + r16];
             by_vocab[j] = *reinterpret_cast<const Acc4 *>(a.g + (int64_t)(v + r16) * (J * 16) + j * 16 + kk * 4);
         }
-        if (v + 16 < v_end) ask(v + 16, next);
-        Acc4 dw[4];
+        if (v + kEach < v_end) ask(v + kEach, next, next_part);
+        Acc4 dw[C];
 #pragma unroll
-        for (int q = 0; q < 4; ++q) dw[q] = Acc4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int q = 0; q < C; ++q) dw[q] = Acc4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
         for (int j = 0; j < J; ++j)
 #pragma unroll
             for (int m = 0; m < 4; ++m)
 #pragma unroll
-                for (int q = 0; q < 4; ++q) {
-                    dx[j][q] = __builtin_amdgcn_mfma_f32_16x16x4f32(by_row[j][m], (float)w[m].v[q], dx[j][q], 0, 0, 0);
+                for (int q = 0; q < C; ++q) {
+                    dx[j][q] = __builtin_amdgcn_mfma_f32_16x16x4f32(by_row[j][m], w[m][q], dx[j][q], 0, 0, 0);
                     dw[q] = __builtin_amdgcn_mfma_f32_16x16x4f32(by_vocab[j][m], xw[j][m][q], dw[q], 0, 0, 0);
                 }
-        // lane l has column l % 16, four channels, and its rows 4 (l / 16) + r
+        // lane l has column l % 16, C channels, and its rows 4 (l / 16) + r
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int32_t at = v + kk * 4 + r;
             if (at >= v_end || some <= 0) continue;
-            T *to = static_cast<T *>(a.d_weight) + (int64_t)at * a.dim + d;
-            const Acc4 out = {dw[0][r], dw[1][r], dw[2][r], dw[3][r]};
-            if (some >= 4) {
-                put4<T>(to, out);
-            } else {
+            float out[C];
 #pragma unroll
-                for (int q = 0; q < 3; ++q)
-                    if (q < some) to[q] = (T)out[q];
-            }
+            for (int q = 0; q < C; ++q) out[q] = dw[q][r];
+            put<T, C>(static_cast<T *>(a.d_weight) + (int64_t)at * a.dim + d, out, some);
         }
+    }
+    if constexpr (Classes) {
+        __shared__ Acc4 sums[3][J][C][64];
+        add_up<4>(dx, sums, wave, lane);
+        if (wave > 0) return;
     }
     const int64_t width = up8(a.dim);
 #pragma unroll
@@ -1003,9 +1022,99 @@ __global__ __launch_bounds__(256) void few_back_kernel(Few a)
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
             const int32_t row = j * 16 + kk * 4 + r;
-            if (row < a.rows && some > 0)
-                *reinterpret_cast<Acc4 *>(a.slab + ((int64_t)blockIdx.y * a.rows + row) * width + d) = Acc4{dx[j][0][r], dx[j][1][r], dx[j][2][r], dx[j][3][r]};
+            typedef float Out __attribute__((ext_vector_type(C)));
+            Out out;
+#pragma unroll
+            for (int q = 0; q < C; ++q) out[q] = dx[j][q][r];
+            if (row < a.rows && some > 0) *reinterpret_cast<Out *>(a.slab + ((int64_t)blockIdx.y * a.rows + row) * width + d) = out;
         }
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// a small vocabulary: a wavefront takes R times 16 rows of x straight from memory against J times 16 rows of weights from the caches, and has all of a row's logits, four of each tile in
+// each of four lanes.  Bound by the bytes of x.
+
+struct Small {
+    const void *x, *weight;
+    const int64_t *tokens;
+    int64_t x_stride, w_stride, ignore;
+    int32_t rows, vocab, dim;
+    float *logp, *lse, *peak, *total;   // (peak and total: read by the backward pass)
+    const float *d_logp;
+    float *g, *weights;                 // [rows, to a whole 32][vocab, to a whole 16]: (p - delta) d_logp; d_logp, 0 of rows without a token, NaN of tokens outside the vocabulary
+};
+
+// Split: wavefronts of a workgroup that share rows, each a part of the channels
+template <typename T, int J, int Split, bool Gradient>
+__global__ __launch_bounds__(Split == 8 ? 512 : 256) void small_kernel(Small a)
+{
+    constexpr int R = Split == 8 ? 1 : 2;
+    const int lane = lane_id(), wave = threadIdx.x / kWave, r16 = lane & 15, quarter = lane >> 4;
+    const int32_t row0 = (Split == 1 ? blockIdx.x * 4 + wave : blockIdx.x) * (R * 16);
+    if (row0 >= a.rows) return;   // (of workgroups that share rows, all or none)
+    const T *w_row[J], *x_row[R];
+#pragma unroll
+    for (int j = 0; j < J; ++j) w_row[j] = static_cast<const T *>(a.weight) + (int64_t)min(j * 16 + r16, a.vocab - 1) * a.w_stride + quarter * 8;
+#pragma unroll
+    for (int i = 0; i < R; ++i) x_row[i] = static_cast<const T *>(a.x) + (int64_t)min(row0 + i * 16 + r16, a.rows - 1) * a.x_stride + quarter * 8;
+    Acc4 acc[J][R];
+#pragma unroll
+    for (int j = 0; j < J; ++j)
+#pragma unroll
+        for (int i = 0; i < R; ++i) acc[j][i] = Acc4{0.0f, 0.0f, 0.0f, 0.0f};
+    const int32_t steps = (a.dim + 31) / 32, part = Split == 1 ? 0 : wave;
+    multiply_rows<T, J, R>(w_row, x_row, steps * part / Split, steps * (part + 1) / Split, a.dim, quarter, acc);
+    if constexpr (Split > 1) {
+        __shared__ Acc4 sums[Split - 1][J][R][64];
+        add_up<Split>(acc, sums, wave, lane);
+        if (wave > 0) return;
+    }
+#pragma unroll
+    for (int i = 0; i < R; ++i) {
+        const int32_t row = row0 + i * 16 + r16;
+        const bool there = row < a.rows;
+        const int64_t token = there ? a.tokens[row] : -1;
+        if constexpr (Gradient) {
+            const float peak = there ? a.peak[row] : 0.0f, total = there ? a.total[row] : 1.0f, inverse = 1.0f / total;
+            const float weight = !there || token == a.ignore ? 0.0f : token < 0 || token >= a.vocab ? NAN : a.d_logp[row];
+            const bool none = !there || token == a.ignore || (peak == -INFINITY && total == 0.0f);
+            if (there && quarter == 0) a.weights[row] = weight;
+#pragma unroll
+            for (int j = 0; j < J; ++j) {
+                Acc4 g;
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int32_t v = j * 16 + quarter * 4 + r;
+                    const float p = exp_over(acc[j][i][r], peak) * inverse;
+                    g[r] = none || v >= a.vocab ? 0.0f : weight * (v == token ? p - 1.0f : p);
+                }
+                *reinterpret_cast<Acc4 *>(a.g + (int64_t)row * (J * 16) + j * 16 + quarter * 4) = g;
+            }
+        } else {
+            float m = -INFINITY, label = 0.0f, s = 0.0f;
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) {
+                    const int32_t v = j * 16 + quarter * 4 + r;
+                    if (v >= a.vocab) acc[j][i][r] = -INFINITY;
+                    else if (v == token) label = acc[j][i][r];
+                    m = fmaxf(m, acc[j][i][r]);
+                }
+            m = fmaxf(m, __shfl_xor(m, 16));
+            m = fmaxf(m, __shfl_xor(m, 32));
+            const float base = base_of(m), from = base == -INFINITY ? 0.0f : base;
+#pragma unroll
+            for (int j = 0; j < J; ++j)
+#pragma unroll
+                for (int r = 0; r < 4; ++r) s += exp_over(acc[j][i][r], from);
+            s += __shfl_xor(s, 16);
+            s += __shfl_xor(s, 32);
+            label += __shfl_xor(label, 16);   // (one lane has it, the others 0)
+            label += __shfl_xor(label, 32);
+            if (there && quarter == 0) finish(make_float2(base, s), row, label, a.tokens, a.ignore, a.vocab, a.logp, a.lse, a.peak, a.total);
+        }
+    }
 }
 
 // the same of few rows: a workgroup to a row, its threads each every 256th tile
@@ -1020,7 +1129,7 @@ __global__ __launch_bounds__(256) void few_join_kernel(const float2 *stats, int3
     for (int k = 32; k; k >>= 1) sum = join(sum, make_float2(__shfl_xor(sum.x, k), __shfl_xor(sum.y, k)));
     if (lane_id() == 0) parts[threadIdx.x / kWave] = sum;
     __syncthreads();
-    if (threadIdx.x == 0) finish(join(join(parts[0], parts[1]), join(parts[2], parts[3])), row, label, tokens, ignore, vocab, logp, lse, peak, total);
+    if (threadIdx.x == 0) finish(join(join(parts[0], parts[1]), join(parts[2], parts[3])), row, label[row], tokens, ignore, vocab, logp, lse, peak, total);
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
@@ -1029,6 +1138,11 @@ __global__ __launch_bounds__(256) void few_join_kernel(const float2 *stats, int3
 // 144/152, 857/560; 64: 170/152, 1003/564; fp32 12: 201/883, 787/2539; 64: 603/895, 1896/2565.  Large tiles of 16-bit weights whose rows do not
 // begin at whole 16 bytes copy them first, 170 us each way here.
 int32_t few_most(int32_t dtype, bool w_fits, bool backward) { return dtype == BMTK_F32 ? 64 : w_fits ? (backward ? 16 : 32) : (backward ? 32 : 64); }
+// Up to which vocabulary the kernels for a small one take it, where rows are more than that or more than few
+bool small_vocab(int64_t rows, int64_t vocab, int32_t dtype, bool w_fits, bool backward) { return vocab <= kSmallMost && (vocab <= rows || rows > few_most(dtype, w_fits, backward)); }
+int32_t small_tiles(int64_t vocab) { return vocab <= 16 ? 1 : vocab <= 32 ? 2 : vocab <= 64 ? 4 : 8; }
+// wavefronts that share rows: where those would leave the chip empty and channels are enough
+int32_t small_split(int64_t rows, int32_t dim) { return rows >= 32 * 2048 || dim < 256 ? 1 : rows >= 32 * 256 || dim < 1024 ? 4 : 8; }
 constexpr int64_t kPieceBytes = int64_t{512} << 20;   // of G: pieces of the vocabulary are as large as that allows
 
 int64_t up(int64_t n, int64_t to) { return div_up(n, to) * to; }
@@ -1038,7 +1152,7 @@ int32_t tile_of(int64_t ni, int64_t nj, int64_t slices = 1) { return div_up(ni, 
 
 struct Plan {
     int32_t parts, combinations, depth;          // depth: dim to whole steps
-    bool few, copy_x, copy_w;                    // the kernels for few rows; operands that are laid out anew
+    bool small, few, copy_x, copy_w;             // the kernels for a small vocabulary, for few rows; operands that are laid out anew
     int64_t piece, pieces, g_rows, g_width, out_width;
     int32_t dx_tile, dx_slices, dw_tile, dw_slices, logit_tile;
     int64_t x_copy, w_copy, x_weighted, g, dx_slab, dw_slab, stats, label, weights;   // bytes
@@ -1047,12 +1161,29 @@ struct Plan {
         parts = dtype == BMTK_F32 ? 3 : 1;
         combinations = parts == 3 ? 6 : 1;
         depth = (int32_t)up(dim, kDepth);
-        few = rows <= few_most(dtype, w_fits, backward);
+        small = small_vocab(rows, vocab, dtype, w_fits, backward);
+        few = !small && rows <= few_most(dtype, w_fits, backward);
         copy_x = parts == 3 || !x_fits;
         copy_w = parts == 3 || !w_fits;
         x_copy = w_copy = x_weighted = g = dx_slab = dw_slab = stats = label = weights = 0;
         pieces = 1, piece = vocab, g_rows = g_width = out_width = 0;
-        dx_tile = dx_slices = dw_tile = dw_slices = 0;
+        dx_tile = dx_slices = dw_tile = dw_slices = logit_tile = 0;
+        if (small) {
+            if (!backward) return;
+            out_width = up(dim, 8);
+            weights = up(rows * 4, 256);
+            const int32_t j = small_tiles(vocab);
+            g = up(up(rows, 64) * j * 16 * 4, 256);
+            // slices of the rows, each with sums of its own for d_weight: some thousand workgroups, slabs of up to 64 MB
+            int64_t s = div_up(1024, div_up(dim, j == 8 ? 32 : 64));
+            const int64_t most = (int64_t{64} << 20) / (vocab * out_width * 4);
+            s = s > most ? most : s;
+            s = s < 1 ? 1 : s;
+            piece = up(div_up(rows, s), 64);
+            dw_slices = (int32_t)div_up(rows, piece);
+            dw_slab = up(dw_slices * vocab * out_width * 4, 256);
+            return;
+        }
         if (!backward) {
             logit_tile = tile_of(vocab, rows);
             label = up(rows * 4, 256);
@@ -1153,6 +1284,27 @@ void few_rows(const Few &f, hipStream_t s)
     }
 }
 
+template <typename T, int J, bool Gradient>
+void small_rows(const Small &m, hipStream_t s)
+{
+    switch (small_split(m.rows, m.dim)) {
+        case 1: small_kernel<T, J, 1, Gradient><<<(uint32_t)div_up(m.rows, 128), 256, 0, s>>>(m); break;
+        case 4: small_kernel<T, J, 4, Gradient><<<(uint32_t)div_up(m.rows, 32), 256, 0, s>>>(m); break;
+        default: small_kernel<T, J, 8, Gradient><<<(uint32_t)div_up(m.rows, 16), 512, 0, s>>>(m);
+    }
+}
+
+template <typename T, bool Gradient>
+void small_any(const Small &m, hipStream_t s)
+{
+    switch (small_tiles(m.vocab)) {
+        case 1: return small_rows<T, 1, Gradient>(m, s);
+        case 2: return small_rows<T, 2, Gradient>(m, s);
+        case 4: return small_rows<T, 4, Gradient>(m, s);
+        default: return small_rows<T, 8, Gradient>(m, s);
+    }
+}
+
 struct Call {
     int64_t rows, vocab, x_stride, w_stride, ignore;
     int32_t dim, dtype;
@@ -1194,6 +1346,12 @@ void forward(Call c, float *logp, float *lse, float *peak, float *total)
     typedef typename Element<T>::type E;
     const bool x_fits = fits(c.x, c.x_stride, c.dim, c.dtype), w_fits = fits(c.weight, c.w_stride, c.dim, c.dtype);
     const Plan plan(c.rows, c.vocab, c.dim, c.dtype, x_fits, w_fits, false);
+    if (plan.small) {
+        Small m{};
+        m.x = c.x, m.weight = c.weight, m.tokens = c.tokens, m.x_stride = c.x_stride, m.w_stride = c.w_stride, m.ignore = c.ignore;
+        m.rows = (int32_t)c.rows, m.vocab = (int32_t)c.vocab, m.dim = c.dim, m.logp = logp, m.lse = lse, m.peak = peak, m.total = total;
+        return small_any<T, false>(m, c.stream);
+    }
     float2 *stats = reinterpret_cast<float2 *>(c.next(plan.stats));
     float *label = reinterpret_cast<float *>(c.next(plan.label));
     int32_t tiles;
@@ -1240,7 +1398,7 @@ template <typename T, int J>
 void few_backward(const Few &f, hipStream_t s)
 {
     few_rows<T, J, true>(f, s);
-    few_back_kernel<T, J><<<dim3((uint32_t)div_up(f.dim, 256), (uint32_t)f.slices), 256, 0, s>>>(f);
+    few_back_kernel<T, J, 4, false><<<dim3((uint32_t)div_up(f.dim, 256), (uint32_t)f.slices), 256, 0, s>>>(f);
 }
 
 template <typename T>
@@ -1255,6 +1413,25 @@ void backward(Call c, const float *peak, const float *total, const float *d_logp
     float *weights = reinterpret_cast<float *>(c.next(plan.weights)), *factor = weights + c.rows;
     char *g = c.next(plan.g), *x_weighted = c.next(plan.x_weighted);
     float *dx_slab = reinterpret_cast<float *>(c.next(plan.dx_slab)), *dw_slab = reinterpret_cast<float *>(c.next(plan.dw_slab));
+    if (plan.small) {
+        Small m{};
+        m.x = c.x, m.weight = c.weight, m.tokens = c.tokens, m.x_stride = c.x_stride, m.w_stride = c.w_stride, m.ignore = c.ignore;
+        m.rows = (int32_t)c.rows, m.vocab = (int32_t)c.vocab, m.dim = c.dim, m.peak = const_cast<float *>(peak), m.total = const_cast<float *>(total);
+        m.d_logp = d_logp, m.g = reinterpret_cast<float *>(g), m.weights = weights;
+        small_any<T, true>(m, c.stream);
+        Few f{};
+        f.x = c.weight, f.weight = c.x, f.x_stride = c.w_stride, f.w_stride = c.x_stride, f.rows = (int32_t)c.vocab, f.vocab = (int32_t)c.rows, f.dim = c.dim;
+        f.weights = weights, f.g = m.g, f.d_weight = dx, f.slab = dw_slab, f.slices = plan.dw_slices, f.slice_rows = (int32_t)plan.piece;
+        const int32_t j = small_tiles(c.vocab);
+        const dim3 grid((uint32_t)div_up(c.dim, j == 8 ? 32 : 64), (uint32_t)f.slices);
+        // (a lane has two channels instead of four where there are eight tiles of the vocabulary: registers)
+        if (j == 1) few_back_kernel<T, 1, 4, true><<<grid, 256, 0, c.stream>>>(f);
+        else if (j == 2) few_back_kernel<T, 2, 4, true><<<grid, 256, 0, c.stream>>>(f);
+        else if (j == 4) few_back_kernel<T, 4, 4, true><<<grid, 256, 0, c.stream>>>(f);
+        else few_back_kernel<T, 8, 2, true><<<grid, 256, 0, c.stream>>>(f);
+        join_slabs<T>(dw_slab, plan.dw_slices, c.vocab * plan.out_width, c.vocab, c.dim, plan.out_width, nullptr, nullptr, -1.0f, d_weight, c.stream);
+        return;
+    }
     weigh_kernel<<<(uint32_t)div_up(c.rows, 1024), 1024, 0, c.stream>>>(d_logp, c.tokens, c.ignore, c.rows, (int32_t)c.vocab, half && !plan.few, weights, factor);
     if (plan.few) {
         Few f{};
@@ -1314,7 +1491,7 @@ void backward(Call c, const float *peak, const float *total, const float *d_logp
     join_slabs<T>(dx_slab, plan.dx_slices, c.rows * plan.out_width, c.rows, c.dim, plan.out_width, weights, factor, -1.0f / g_scale, dx, c.stream);
 }
 
-int check(const char *name, const Call &c)
+int check(const char *name, const Call &c, bool backward)
 {
     BMTK_REQUIRE(c.rows > 0 && c.vocab > 0 && c.dim > 0, "%s: sizes must be positive", name);
     BMTK_REQUIRE(c.dtype >= 0 && c.dtype <= 2, "%s: unknown type %d", name, c.dtype);
@@ -1326,7 +1503,8 @@ int check(const char *name, const Call &c)
     // (a launch has up to 2^32 threads: of eight numbers where operands are laid out anew, of four where dx is put together)
     BMTK_REQUIRE(up(c.vocab, 256) * up(c.dim, 64) < (int64_t{1} << 35) && up(c.rows, 256) * up(c.dim, 64) < (int64_t{1} << 34), "%s: too many numbers for a launch", name);
     BMTK_REQUIRE(div_up(c.rows, 128) * div_up(c.vocab, 128) < (int64_t{1} << 31), "%s: too many logits for a launch", name);
-    BMTK_REQUIRE(c.ws, "%s: needs a workspace", name);
+    BMTK_REQUIRE(c.ws || !Plan(c.rows, c.vocab, c.dim, c.dtype, fits(c.x, c.x_stride, c.dim, c.dtype), fits(c.weight, c.w_stride, c.dim, c.dtype), backward).bytes(),
+                 "%s: needs a workspace", name);
     return 0;
 }
 
@@ -1347,7 +1525,7 @@ extern "C" int bmtk_projected_logprobs_fwd(int64_t rows, int32_t vocab, int32_t 
 {
     BMTK_REQUIRE(x && weight && tokens && logp && lse && peak && total, "projected_logprobs_fwd: null pointer");
     const Call c{rows, vocab, x_stride, weight_stride, ignore, dim, dtype, x, weight, tokens, static_cast<char *>(workspace), static_cast<hipStream_t>(stream)};
-    if (const int failed = check("projected_logprobs_fwd", c)) return failed;
+    if (const int failed = check("projected_logprobs_fwd", c, false)) return failed;
     BMTK_BY_TYPE(dtype, T, { forward<T>(c, logp, lse, peak, total); });
     BMTK_CHECK_LAUNCH("projected_logprobs_fwd");
     return 0;
@@ -1359,7 +1537,7 @@ extern "C" int bmtk_projected_logprobs_bwd(int64_t rows, int32_t vocab, int32_t 
 {
     BMTK_REQUIRE(x && weight && tokens && peak && total && d_logp && dx && d_weight, "projected_logprobs_bwd: null pointer");
     const Call c{rows, vocab, x_stride, weight_stride, ignore, dim, dtype, x, weight, tokens, static_cast<char *>(workspace), static_cast<hipStream_t>(stream)};
-    if (const int failed = check("projected_logprobs_bwd", c)) return failed;
+    if (const int failed = check("projected_logprobs_bwd", c, true)) return failed;
     BMTK_BY_TYPE(dtype, T, { backward<T>(c, peak, total, d_logp, dx, d_weight); });
     BMTK_CHECK_LAUNCH("projected_logprobs_bwd");
     return 0;

@@ -11,8 +11,8 @@ from test_gpu_readout import DTYPES, U, close, gen
 
 pytestmark = pytest.mark.gpu
 
-# few rows of every class, and tiles; vocabularies of one, four and eight wavefronts a tile of few rows
-FEW_AND_MANY = [(7, 1000, 96), (20, 40000, 40), (50, 66000, 24), (130, 700, 72), (300, 129, 200)]
+# few rows of every class, and tiles; vocabularies of one, four and eight wavefronts a tile of few rows; small vocabularies, rows of one, four and eight wavefronts
+FEW_AND_MANY = [(7, 1000, 96), (20, 40000, 40), (50, 66000, 24), (130, 700, 72), (300, 129, 200), (90, 7, 300), (9, 8, 1100), (2100, 100, 271), (66000, 40, 24)]
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
@@ -62,6 +62,17 @@ def test_rows_that_are_not_finite_leave_the_others_as_they_are(rows, vocab, dim,
 @pytest.mark.parametrize("rows,vocab,dim", [(9, 3000, 40), (200, 3000, 40)])
 def test_logits_far_from_zero_and_all_alike(rows, vocab, dim, dtype, scale):
     check(case(rows, vocab, dim, dtype, scale=scale))
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("rows,vocab,dim", [(40, 2, 9), (40, 16, 70), (33, 17, 1030), (300, 128, 1100), (100, 32, 264), (9000, 100, 270), (8200, 65, 64), (8191, 64, 1025), (130, 128, 33),
+                                            (65, 128, 2050)])
+def test_small_vocabularies(rows, vocab, dim, dtype):
+    check(case(rows, vocab, dim, dtype))
+
+
+def test_small_vocabulary_of_very_many_rows():
+    check(case(65600, 33, 300, torch.bfloat16))
 
 
 @pytest.mark.parametrize("rows,vocab,dim", [(1, 1, 1), (1, 1, 64), (70, 1, 5), (1, 300, 1), (65, 2, 3), (400, 3, 1)])

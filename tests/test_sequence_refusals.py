@@ -74,7 +74,7 @@ def test_selective_scan_bwd():
         assert size(*wrong, 0) == size(*wrong, 1) == 0
 
 
-def projected(backward, rows=100, vocab=50, dim=8, dtype=0, x=P, x_stride=8, weight=P, w_stride=8, tokens=P, logp=P, lse=P, peak=P, total=P, ws=P):
+def projected(backward, rows=100, vocab=500, dim=8, dtype=0, x=P, x_stride=8, weight=P, w_stride=8, tokens=P, logp=P, lse=P, peak=P, total=P, ws=P):
     given = rows, vocab, dim, dtype, x, x_stride, weight, w_stride, tokens, -100
     if backward:
         return _lib.load().bmtk_projected_logprobs_bwd(*given, peak, total, P, logp, lse, ws, None)
@@ -93,7 +93,7 @@ def test_projected_logprobs(backward, change, word):
 
 def test_projected_logprobs_workspace():
     size = lambda *sizes: [_lib.load().bmtk_projected_logprobs_workspace_bytes(*sizes, P, 8, P, 8, way) for way in (0, 1)]  # noqa: E731
-    assert min(size(100, 50, 8, 0)) >= 100 * 4
+    assert min(size(100, 500, 8, 0)) >= 100 * 4 and size(100, 50, 8, 0)[0] == 0 < size(100, 50, 8, 0)[1]   # (a small vocabulary's logits are whole in registers)
     for wrong in ((0, 50, 8, 0), (100, 0, 8, 0), (100, 50, 0, 0), (100, 50, 8, 3), (1 << 22, 50, 8, 0), (100, 1 << 28, 8, 0), (100, 50, 65537, 0)):
         assert size(*wrong) == [0, 0]
 
