@@ -30,6 +30,11 @@ struct Vec<bf16> {
     typedef __bf16 V4 __attribute__((ext_vector_type(4)));
     static __device__ __forceinline__ Acc mfma(V8 a, V8 b, Acc c) { return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ Acc4 mfma16(V8 a, V8 b, Acc4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ Acc4 mfma16(V4 a, V4 b, Acc4 c)
+    {
+        typedef short S4 __attribute__((ext_vector_type(4)));
+        return __builtin_amdgcn_mfma_f32_16x16x16bf16_1k(__builtin_bit_cast(S4, a), __builtin_bit_cast(S4, b), c, 0, 0, 0);
+    }
 };
 template <>
 struct Vec<f16> {
@@ -37,6 +42,7 @@ struct Vec<f16> {
     typedef _Float16 V4 __attribute__((ext_vector_type(4)));
     static __device__ __forceinline__ Acc mfma(V8 a, V8 b, Acc c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
     static __device__ __forceinline__ Acc4 mfma16(V8 a, V8 b, Acc4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+    static __device__ __forceinline__ Acc4 mfma16(V4 a, V4 b, Acc4 c) { return __builtin_amdgcn_mfma_f32_16x16x16f16(a, b, c, 0, 0, 0); }
 };
 
 // what a type's products are made of
@@ -764,6 +770,8 @@ struct Few {
     void *d_weight;
     float *slab;                           // [slices][rows][dim, to a whole 8]
     int32_t slices, slice_rows;            // slices of the vocabulary, of so many of its rows (a multiple of 16)
+    const float *factor;                   // small vocabulary: weights are d_logp over this number (none: 1), and G is (p - delta) / g_unit
+    float g_unit;
 };
 
 // acc[i][j] += the products of 16 rows of I tiles by 16 rows of J tiles, over the steps of 32 k from first to end; p, q: where this lane's rows have their first eight k
@@ -821,6 +829,14 @@ __device__ __forceinline__ void multiply_rows(const T *const (&p)[I], const T *c
 #pragma unroll
             for (int s = 0; s < kAhead; ++s) multiply(u[s], v[s]);
         }
+    }
+    for (; k < whole; ++k) {
+        Loose8<T> u[I], v[J];
+#pragma unroll
+        for (int i = 0; i < I; ++i) u[i].load(p[i] + k * 32);
+#pragma unroll
+        for (int j = 0; j < J; ++j) v[j].load(q[j] + k * 32);
+        multiply(u, v);
     }
     for (; k < end; ++k) {
         Loose8<T> u[I], v[J];
@@ -928,22 +944,51 @@ __global__ __launch_bounds__(Split == 8 ? 512 : 256) void few_rows_kernel(Few a)
     }
 }
 
+// four numbers of a lane's k, one of each, or sixteen k's in one instruction
+__device__ __forceinline__ Acc4 multiply_fours(const Acc4 &a, const Acc4 &b, Acc4 c)
+{
+#pragma unroll
+    for (int m = 0; m < 4; ++m) c = __builtin_amdgcn_mfma_f32_16x16x4f32(a[m], b[m], c, 0, 0, 0);
+    return c;
+}
+__device__ __forceinline__ Acc4 multiply_fours(const Vec<bf16>::V4 &a, const Vec<bf16>::V4 &b, Acc4 c) { return Vec<bf16>::mfma16(a, b, c); }
+__device__ __forceinline__ Acc4 multiply_fours(const Vec<f16>::V4 &a, const Vec<f16>::V4 &b, Acc4 c) { return Vec<f16>::mfma16(a, b, c); }
+
+// what G is kept in
+template <typename T, bool Classes>
+struct Kept {
+    typedef float type;
+    typedef Acc4 V4;
+};
+template <>
+struct Kept<bf16, true> {
+    typedef bf16 type;
+    typedef Vec<bf16>::V4 V4;
+};
+template <>
+struct Kept<f16, true> {
+    typedef f16 type;
+    typedef Vec<f16>::V4 V4;
+};
+
 // The two products of G for few rows, in one pass over the weights: a wavefront takes 16 C channels (a lane C) of a slice of the vocabulary, and per 16 of its rows
 //     dx[r][d] -= G[v][r] w[v][d]   and   d_weight[v][d] = -sum_r G[v][r] d_logp[r] x[r][d]
-// in matrix instructions of 32 bits, which take one k a lane: nothing has to be transposed, and a lane's C channels are C tiles.  Bound by memory: the weights
-// read, their gradient written.
-// Classes: a small vocabulary and many rows, the two in each other's place, with G times d_logp already; rows that have no part (weights of 0) may hold anything.  A workgroup's
-// wavefronts share a slice of the rows and add up.
+// in matrix instructions of 32 bits.  A lane's k are 4 (l / 16) .. 4 (l / 16) + 3, of rows as of the vocabulary, which nothing has to be transposed for, and its C channels are C tiles.
+// Bound by memory: the weights read, their gradient written.
+// Classes: a small vocabulary and many rows, the two in each other's place: of each 16 rows d_weight -= G^T (d_logp x) and dx = -d_logp G weight, in 16 bits where the type has them
+// (G and d_logp x are rounded to it).  Rows that have no part, of weights 0, may hold anything.  A workgroup's wavefronts share a slice of the rows and add up.
 template <typename T, int J, int C, bool Classes>
 __global__ __launch_bounds__(256) void few_back_kernel(Few a)
 {
     typedef LooseFew<T, C> In;
+    typedef typename Kept<T, Classes>::type G;
+    typedef typename Kept<T, Classes>::V4 V4;
     const int lane = lane_id(), wave = threadIdx.x / kWave, r16 = lane & 15, kk = lane >> 4;
     const int32_t d0 = (Classes ? blockIdx.x : blockIdx.x * 4 + wave) * (16 * C), d = d0 + r16 * C;
     const int32_t some = a.dim - d;   // this lane's channels that are there, if fewer than C
     if (d0 >= a.dim) return;
-    // x d_logp, 4 kk + m of each 16 rows: what a lane's k is in product m
-    float xw[J][4][C];
+    const G *g = reinterpret_cast<const G *>(a.g);
+    V4 xw[J][C];   // x d_logp; Classes: weights
 #pragma unroll
     for (int j = 0; j < J; ++j)
 #pragma unroll
@@ -953,7 +998,7 @@ __global__ __launch_bounds__(256) void few_back_kernel(Few a)
             In x;
             x.load(static_cast<const T *>(a.x) + (int64_t)min(row, a.rows - 1) * a.x_stride + d, some);
 #pragma unroll
-            for (int q = 0; q < C; ++q) xw[j][m][q] = by == 0.0f ? 0.0f : -by * (float)x.v[q];
+            for (int q = 0; q < C; ++q) xw[j][q][m] = (G)(by == 0.0f ? 0.0f : -by * (float)x.v[q]);
         }
     Acc4 dx[J][C];
 #pragma unroll
@@ -962,44 +1007,49 @@ __global__ __launch_bounds__(256) void few_back_kernel(Few a)
         for (int q = 0; q < C; ++q) dx[j][q] = Acc4{0.0f, 0.0f, 0.0f, 0.0f};
     constexpr int kEach = Classes ? 64 : 16;   // rows that a workgroup, or a wavefront of its own, goes on by
     const int32_t v_end = min((int32_t)(blockIdx.y + 1) * a.slice_rows, a.vocab), v_first = blockIdx.y * a.slice_rows + (Classes ? wave * 16 : 0);
-    const auto ask = [&](int32_t v, In (&w)[4], float (&part)[4]) {
+    const float factor = !Classes ? 1.0f : a.factor ? *a.factor * a.g_unit : a.g_unit;
+    struct Block {
+        In w[4];
+        float part[4];
+        G by_row[J][4];
+        V4 by_vocab[J];
+    };
+    const auto ask = [&](int32_t v, Block &to) {
 #pragma unroll
         for (int u = 0; u < 4; ++u) {
-            const int32_t at = min(v + u * 4 + kk, a.vocab - 1);
-            w[u].load(static_cast<const T *>(a.weight) + (int64_t)at * a.w_stride + d, some);
-            if (Classes) part[u] = a.weights[at];
+            const int32_t at = min(v + kk * 4 + u, a.vocab - 1);
+            to.w[u].load(static_cast<const T *>(a.weight) + (int64_t)at * a.w_stride + d, some);
+            if (Classes) to.part[u] = a.weights[at];
         }
-    };
-    In next[4];
-    float next_part[4];
-    ask(v_first, next, next_part);
-    for (int32_t v = v_first; v < v_end; v += kEach) {
-        float w[4][C];
-#pragma unroll
-        for (int u = 0; u < 4; ++u)
-#pragma unroll
-            for (int q = 0; q < C; ++q) w[u][q] = Classes && next_part[u] == 0.0f ? 0.0f : (float)next[u].v[q];
-        float by_row[J][4];
-        Acc4 by_vocab[J];
 #pragma unroll
         for (int j = 0; j < J; ++j) {
 #pragma unroll
-            for (int u = 0; u < 4; ++u) by_row[j][u] = a.g[(int64_t)(v + u * 4 + kk) * (J * 16) + j * 16 + r16];
-            by_vocab[j] = *reinterpret_cast<const Acc4 *>(a.g + (int64_t)(v + r16) * (J * 16) + j * 16 + kk * 4);
+            for (int u = 0; u < 4; ++u) to.by_row[j][u] = g[(int64_t)(v + kk * 4 + u) * (J * 16) + j * 16 + r16];
+            to.by_vocab[j] = *reinterpret_cast<const V4 *>(g + (int64_t)(v + r16) * (J * 16) + j * 16 + kk * 4);
         }
-        if (v + kEach < v_end) ask(v + kEach, next, next_part);
+    };
+    Block next;
+    if (v_first < v_end) ask(v_first, next);
+    for (int32_t v = v_first; v < v_end; v += kEach) {
+        const Block now = next;
+        if (v + kEach < v_end) ask(v + kEach, next);
+        V4 w[C];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+#pragma unroll
+            for (int q = 0; q < C; ++q) w[q][u] = (G)(!Classes ? (float)now.w[u].v[q] : now.part[u] == 0.0f ? 0.0f : (float)now.w[u].v[q] * now.part[u]);
         Acc4 dw[C];
 #pragma unroll
         for (int q = 0; q < C; ++q) dw[q] = Acc4{0.0f, 0.0f, 0.0f, 0.0f};
 #pragma unroll
-        for (int j = 0; j < J; ++j)
+        for (int j = 0; j < J; ++j) {
+            const V4 by_row = {now.by_row[j][0], now.by_row[j][1], now.by_row[j][2], now.by_row[j][3]};
 #pragma unroll
-            for (int m = 0; m < 4; ++m)
-#pragma unroll
-                for (int q = 0; q < C; ++q) {
-                    dx[j][q] = __builtin_amdgcn_mfma_f32_16x16x4f32(by_row[j][m], w[m][q], dx[j][q], 0, 0, 0);
-                    dw[q] = __builtin_amdgcn_mfma_f32_16x16x4f32(by_vocab[j][m], xw[j][m][q], dw[q], 0, 0, 0);
-                }
+            for (int q = 0; q < C; ++q) {
+                dx[j][q] = multiply_fours(by_row, w[q], dx[j][q]);
+                dw[q] = multiply_fours(now.by_vocab[j], xw[j][q], dw[q]);
+            }
+        }
         // lane l has column l % 16, C channels, and its rows 4 (l / 16) + r
 #pragma unroll
         for (int r = 0; r < 4; ++r) {
@@ -1007,7 +1057,7 @@ __global__ __launch_bounds__(256) void few_back_kernel(Few a)
             if (at >= v_end || some <= 0) continue;
             float out[C];
 #pragma unroll
-            for (int q = 0; q < C; ++q) out[q] = dw[q][r];
+            for (int q = 0; q < C; ++q) out[q] = !Classes ? dw[q][r] : now.part[r] == 0.0f ? 0.0f : dw[q][r] * (now.part[r] * factor);
             put<T, C>(static_cast<T *>(a.d_weight) + (int64_t)at * a.dim + d, out, some);
         }
     }
@@ -1041,7 +1091,9 @@ struct Small {
     int32_t rows, vocab, dim;
     float *logp, *lse, *peak, *total;   // (peak and total: read by the backward pass)
     const float *d_logp;
-    float *g, *weights;                 // [rows, to a whole 32][vocab, to a whole 16]: (p - delta) d_logp; d_logp, 0 of rows without a token, NaN of tokens outside the vocabulary
+    void *g;                            // [rows, to a whole 32][vocab, to a whole 16]: (p - delta) g_scale
+    float g_scale;
+    float *weights;                     // as weigh_kernel's, if that has not made them; else none
 };
 
 // Split: wavefronts of a workgroup that share rows, each a part of the channels
@@ -1076,19 +1128,18 @@ __global__ __launch_bounds__(Split == 8 ? 512 : 256) void small_kernel(Small a)
         const int64_t token = there ? a.tokens[row] : -1;
         if constexpr (Gradient) {
             const float peak = there ? a.peak[row] : 0.0f, total = there ? a.total[row] : 1.0f, inverse = 1.0f / total;
-            const float weight = !there || token == a.ignore ? 0.0f : token < 0 || token >= a.vocab ? NAN : a.d_logp[row];
             const bool none = !there || token == a.ignore || (peak == -INFINITY && total == 0.0f);
-            if (there && quarter == 0) a.weights[row] = weight;
+            if (a.weights && there && quarter == 0) a.weights[row] = token == a.ignore ? 0.0f : token < 0 || token >= a.vocab ? NAN : a.d_logp[row];
 #pragma unroll
             for (int j = 0; j < J; ++j) {
-                Acc4 g;
+                typename Kept<T, true>::V4 g;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int32_t v = j * 16 + quarter * 4 + r;
                     const float p = exp_over(acc[j][i][r], peak) * inverse;
-                    g[r] = none || v >= a.vocab ? 0.0f : weight * (v == token ? p - 1.0f : p);
+                    g[r] = (typename Kept<T, true>::type)(none || v >= a.vocab ? 0.0f : (v == token ? p - 1.0f : p) * a.g_scale);
                 }
-                *reinterpret_cast<Acc4 *>(a.g + (int64_t)row * (J * 16) + j * 16 + quarter * 4) = g;
+                *reinterpret_cast<typename Kept<T, true>::V4 *>(static_cast<typename Kept<T, true>::type *>(a.g) + (int64_t)row * (J * 16) + j * 16 + quarter * 4) = g;
             }
         } else {
             float m = -INFINITY, label = 0.0f, s = 0.0f;
@@ -1138,8 +1189,17 @@ __global__ __launch_bounds__(256) void few_join_kernel(const float2 *stats, int3
 // 144/152, 857/560; 64: 170/152, 1003/564; fp32 12: 201/883, 787/2539; 64: 603/895, 1896/2565.  Large tiles of 16-bit weights whose rows do not
 // begin at whole 16 bytes copy them first, 170 us each way here.
 int32_t few_most(int32_t dtype, bool w_fits, bool backward) { return dtype == BMTK_F32 ? 64 : w_fits ? (backward ? 16 : 32) : (backward ? 32 : 64); }
-// Up to which vocabulary the kernels for a small one take it, where rows are more than that or more than few
-bool small_vocab(int64_t rows, int64_t vocab, int32_t dtype, bool w_fits, bool backward) { return vocab <= kSmallMost && (vocab <= rows || rows > few_most(dtype, w_fits, backward)); }
+// Whether a vocabulary is taken by the kernels for a small one.  Not where there are fewer rows than that, and few.  Of fp32 always: the large tiles copy it in parts first (us forward, both
+// ways, small / large: 20,000 x 128 x 2,000 fp32 129/210, 545/768; 18,124 x 2 x 1,930 30/195, 138/660).  Of 16 bits up to 64 (20,000 x 30 x 4,000 36/49, 163/416; 20,000 x 64 x 2,000 32/31,
+// 137/238); above, where each workgroup's weights weigh less than what the large tiles cost (20,000 x 100 x 250 13/22; 5,000 x 100 x 1,000 12/16, 89/75; 20,000 x 128 x 2,000 60/35, 322/257;
+// 2,000 x 100 x 2,000 16/23, 76/88); and of long rows that do not begin at whole 16 bytes up to 32 (5,000 x 50 x 3,001 67/50, 176/151).
+bool small_vocab(int64_t rows, int64_t vocab, int32_t dim, int32_t dtype, bool x_fits, bool w_fits, bool backward)
+{
+    if (vocab > kSmallMost || (vocab > rows && rows <= few_most(dtype, w_fits, backward))) return false;
+    if (dtype == BMTK_F32 || vocab <= 32) return true;
+    if (dim > 512 && !(x_fits && w_fits)) return false;
+    return vocab <= 64 || (backward ? rows <= 4096 : rows * dim <= (5 << 20));
+}
 int32_t small_tiles(int64_t vocab) { return vocab <= 16 ? 1 : vocab <= 32 ? 2 : vocab <= 64 ? 4 : 8; }
 // wavefronts that share rows: where those would leave the chip empty and channels are enough
 int32_t small_split(int64_t rows, int32_t dim) { return rows >= 32 * 2048 || dim < 256 ? 1 : rows >= 32 * 256 || dim < 1024 ? 4 : 8; }
@@ -1161,7 +1221,7 @@ struct Plan {
         parts = dtype == BMTK_F32 ? 3 : 1;
         combinations = parts == 3 ? 6 : 1;
         depth = (int32_t)up(dim, kDepth);
-        small = small_vocab(rows, vocab, dtype, w_fits, backward);
+        small = small_vocab(rows, vocab, dim, dtype, x_fits, w_fits, backward);
         few = !small && rows <= few_most(dtype, w_fits, backward);
         copy_x = parts == 3 || !x_fits;
         copy_w = parts == 3 || !w_fits;
@@ -1171,7 +1231,7 @@ struct Plan {
         if (small) {
             if (!backward) return;
             out_width = up(dim, 8);
-            weights = up(rows * 4, 256);
+            weights = up(rows * 4 + 4, 256);
             const int32_t j = small_tiles(vocab);
             g = up(up(rows, 64) * j * 16 * 4, 256);
             // slices of the rows, each with sums of its own for d_weight: some thousand workgroups, slabs of up to 64 MB
@@ -1413,15 +1473,18 @@ void backward(Call c, const float *peak, const float *total, const float *d_logp
     float *weights = reinterpret_cast<float *>(c.next(plan.weights)), *factor = weights + c.rows;
     char *g = c.next(plan.g), *x_weighted = c.next(plan.x_weighted);
     float *dx_slab = reinterpret_cast<float *>(c.next(plan.dx_slab)), *dw_slab = reinterpret_cast<float *>(c.next(plan.dw_slab));
+    // (a small vocabulary's weights are made beside G, but where they are first divided by what the largest of them needs)
+    if (!plan.small || half) weigh_kernel<<<(uint32_t)div_up(c.rows, 1024), 1024, 0, c.stream>>>(d_logp, c.tokens, c.ignore, c.rows, (int32_t)c.vocab, half && !plan.few, weights, factor);
     if (plan.small) {
         Small m{};
         m.x = c.x, m.weight = c.weight, m.tokens = c.tokens, m.x_stride = c.x_stride, m.w_stride = c.w_stride, m.ignore = c.ignore;
         m.rows = (int32_t)c.rows, m.vocab = (int32_t)c.vocab, m.dim = c.dim, m.peak = const_cast<float *>(peak), m.total = const_cast<float *>(total);
-        m.d_logp = d_logp, m.g = reinterpret_cast<float *>(g), m.weights = weights;
+        m.d_logp = d_logp, m.g = g, m.g_scale = g_scale, m.weights = half ? nullptr : weights;
         small_any<T, true>(m, c.stream);
         Few f{};
         f.x = c.weight, f.weight = c.x, f.x_stride = c.w_stride, f.w_stride = c.x_stride, f.rows = (int32_t)c.vocab, f.vocab = (int32_t)c.rows, f.dim = c.dim;
-        f.weights = weights, f.g = m.g, f.d_weight = dx, f.slab = dw_slab, f.slices = plan.dw_slices, f.slice_rows = (int32_t)plan.piece;
+        f.weights = weights, f.g = reinterpret_cast<float *>(g), f.d_weight = dx, f.slab = dw_slab, f.slices = plan.dw_slices, f.slice_rows = (int32_t)plan.piece;
+        f.factor = half ? factor : nullptr, f.g_unit = 1.0f / g_scale;
         const int32_t j = small_tiles(c.vocab);
         const dim3 grid((uint32_t)div_up(c.dim, j == 8 ? 32 : 64), (uint32_t)f.slices);
         // (a lane has two channels instead of four where there are eight tiles of the vocabulary: registers)
@@ -1429,10 +1492,9 @@ void backward(Call c, const float *peak, const float *total, const float *d_logp
         else if (j == 2) few_back_kernel<T, 2, 4, true><<<grid, 256, 0, c.stream>>>(f);
         else if (j == 4) few_back_kernel<T, 4, 4, true><<<grid, 256, 0, c.stream>>>(f);
         else few_back_kernel<T, 8, 2, true><<<grid, 256, 0, c.stream>>>(f);
-        join_slabs<T>(dw_slab, plan.dw_slices, c.vocab * plan.out_width, c.vocab, c.dim, plan.out_width, nullptr, nullptr, -1.0f, d_weight, c.stream);
+        join_slabs<T>(dw_slab, plan.dw_slices, c.vocab * plan.out_width, c.vocab, c.dim, plan.out_width, nullptr, f.factor, -f.g_unit, d_weight, c.stream);
         return;
     }
-    weigh_kernel<<<(uint32_t)div_up(c.rows, 1024), 1024, 0, c.stream>>>(d_logp, c.tokens, c.ignore, c.rows, (int32_t)c.vocab, half && !plan.few, weights, factor);
     if (plan.few) {
         Few f{};
         f.x = c.x, f.weight = c.weight, f.tokens = c.tokens, f.x_stride = c.x_stride, f.w_stride = c.w_stride, f.rows = (int32_t)c.rows, f.vocab = (int32_t)c.vocab, f.dim = c.dim;
