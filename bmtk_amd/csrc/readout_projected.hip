@@ -1234,8 +1234,11 @@ struct Plan {
             weights = up(rows * 4 + 4, 256);
             const int32_t j = small_tiles(vocab);
             g = up(up(rows, 64) * j * 16 * 4, 256);
-            // slices of the rows, each with sums of its own for d_weight: some thousand workgroups, slabs of up to 64 MB
-            int64_t s = div_up(1024, div_up(dim, j == 8 ? 32 : 64));
+            // slices of the rows, each with sums of its own for d_weight: as many workgroups as the chip holds at once, one or two a compute unit of eight or four tiles of the
+            // vocabulary (us both ways of 1,024, 512, 256 workgroups: 19,200 x 100 x 64 fp32 60, 56, 47; 20,000 x 64 x 2,000 303, 292, 294), but of eight tiles and many channels
+            // (20,000 x 128 x 2,000 fp32 546, 605, 692); slabs of up to 64 MB
+            const int64_t fill = j == 8 ? (dim <= 512 ? 256 : 1024) : j == 4 ? 512 : 1024;
+            int64_t s = div_up(fill, div_up(dim, j == 8 ? 32 : 64));
             const int64_t most = (int64_t{64} << 20) / (vocab * out_width * 4);
             s = s > most ? most : s;
             s = s < 1 ? 1 : s;
