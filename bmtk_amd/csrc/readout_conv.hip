@@ -352,11 +352,12 @@ int32_t stretch_of(int64_t n_steps, int64_t batch, int32_t dim, int32_t v)
     return (int32_t)s;
 }
 
-int32_t vector_of(int32_t dim, int32_t dtype, int32_t width, bool backward)
+// Channels of a thread.  Back, where a thread has twice as much to keep, eight of 16 bits only with four taps or fewer (eight taps are 250 registers with eight channels), rows that begin
+// at whole 16 bytes, and enough of them: us of eight and four, 4,096 x 8 x 2,048 88/103; 3,000 x 16 x 641 fp16, two taps 91/79; 30,000 x 1 x 100 75/50.
+int32_t vector_of(int64_t n_steps, int64_t batch, int32_t dim, int32_t dtype, int32_t width, bool backward, bool whole)
 {
-    // (eight taps both ways are 250 registers a thread with eight channels)
-    const int32_t v = dtype == BMTK_F32 ? 4 : backward && width > 4 ? 4 : 8;
-    return dim >= v ? v : 1;
+    const bool eight = dtype != BMTK_F32 && (!backward || (width <= 4 && whole && div_up(n_steps, 8) * batch * (dim / 8) >= 2048 * 64));
+    return dim >= 8 && eight ? 8 : dim >= 4 ? 4 : 1;
 }
 
 template <typename T, typename TW, int W, int V>
@@ -393,7 +394,8 @@ int run(const char *name, int32_t dtype, int32_t weight_dtype, ConvArgs &a, bool
     BMTK_REQUIRE(dtype >= 0 && dtype <= 2, "%s: unknown type %d", name, dtype);
     BMTK_REQUIRE(weight_dtype == BMTK_F32 || weight_dtype == dtype, "%s: weights must be float32 or of the type of x", name);
     BMTK_REQUIRE(a.n_steps < (int64_t{1} << 31) - 4096 && a.batch < (int64_t{1} << 31) && a.batch * a.dim < (int64_t{1} << 31), "%s: too many steps or columns", name);
-    const int32_t v = vector_of(a.dim, dtype, a.width, backward);
+    const auto whole = [](const void *p, int64_t t, int64_t b) { return t % 8 == 0 && b % 8 == 0 && aligned(p, 16); };
+    const int32_t v = vector_of(a.n_steps, a.batch, a.dim, dtype, a.width, backward, a.dim % 8 == 0 && whole(a.x, a.x_t, a.x_b) && whole(a.dy, a.dy_t, a.dy_b) && aligned(a.dx, 16));
     a.vectors = (int32_t)div_up(a.dim, v);
     a.by_vectors = fast_div((uint32_t)a.vectors);
     a.stretch = stretch_of(a.n_steps, a.batch, a.dim, v);
@@ -428,8 +430,12 @@ extern "C" int64_t bmtk_short_conv_workspace_bytes(int64_t n_steps, int64_t batc
     if (n_steps <= 0 || batch <= 0 || dim <= 0 || width < 2 || width > BMTK_CONV_MAX_WIDTH || dtype < 0 || dtype > 2 || batch >= (int64_t{1} << 31) ||
         batch * dim >= (int64_t{1} << 31) || n_steps >= (int64_t{1} << 31) - 4096)
         return 0;
-    const int32_t s = stretch_of(n_steps, batch, dim, vector_of(dim, dtype, width, true));
-    return div_up(n_steps, s) * batch * dim * (width + 1) * 4;
+    int64_t stretches = 0;   // (of the call's strides, which decide, nothing is known here)
+    for (const bool whole : {false, true}) {
+        const int64_t n = div_up(n_steps, stretch_of(n_steps, batch, dim, vector_of(n_steps, batch, dim, dtype, width, true, whole)));
+        stretches = n > stretches ? n : stretches;
+    }
+    return stretches * batch * dim * (width + 1) * 4;
 }
 
 extern "C" int bmtk_short_conv_fwd(int64_t n_steps, int64_t batch, int32_t dim, int32_t width, int32_t dtype, int32_t weight_dtype, int32_t silu, const void *x, int64_t x_t,
