@@ -371,13 +371,15 @@ __device__ __forceinline__ float sum_rows(float (&v)[kSteps], int lane)
     return add_pairs<0>(v[0], v[1], lane);
 }
 
+// (two wavefronts a SIMD, where a workgroup has no more: of a few states, whose wavefronts stage many rows, the compiler would take more registers than that leaves)
 template <typename T, typename TD, int Waves, int Rows, bool Sums>
-__global__ __launch_bounds__(Waves * kWave) void selective_bwd_kernel(SelArgs a)
+__global__ __launch_bounds__(Waves * kWave, Waves == 16 ? 4 : 2) void selective_bwd_kernel(SelArgs a)
 {
+    // A block's decays and states are kept in registers, 128 of them; of 16 wavefronts, which have no more, by halves, the first half made twice
+    constexpr int kParts = Waves == 16 ? 2 : 1, kEach = kSteps / kParts;
     extern __shared__ float lds[];
-    float2 *staged = reinterpret_cast<float2 *>(lds);                        // [kSteps][kWave]: delta, delta x
-    float *dys = lds + 2 * kSteps * kWave;                                   // [kSteps][kWave]
-    float2 *parts = reinterpret_cast<float2 *>(lds + 3 * kSteps * kWave);    // [waves][kSteps][kWave]: s1, s2 of a wavefront's states
+    float4 *staged = reinterpret_cast<float4 *>(lds);                        // [kSteps][kWave]: delta, x, dy, slope of delta
+    float2 *parts = reinterpret_cast<float2 *>(lds + 4 * kSteps * kWave);    // [waves][kSteps][kWave]: s1, s2 of a wavefront's states
     const Tile at(a);
     const int32_t n0 = at.wave * kOwn;
     const int64_t column = at.column(a);
@@ -397,21 +399,13 @@ __global__ __launch_bounds__(Waves * kWave) void selective_bwd_kernel(SelArgs a)
     in.ask(a, at, t_last);
     float total = 0.0f, d_skip = 0.0f, d_bias = 0.0f;
     for (int64_t t = t_last; t >= at.t0; t -= kSteps) {
-        float x[Rows], delta[Rows], slope[Rows], dy[Rows];
 #pragma unroll
         for (int r = 0; r < Rows; ++r) {
             const int row = at.wave + r * a.waves;
             const bool there = at.there && t + row < at.end && t + row < at.t1 && row < kSteps;
-            const float v = (float)in.dt[r] + bias;
-            x[r] = there ? (float)in.x[r] : 0.0f;
-            dy[r] = there ? (float)in.dy[r] : 0.0f;
-            delta[r] = there ? delta_of(a, v) : 0.0f;
-            if (!Sums) slope[r] = !there ? 0.0f : a.softplus ? softplus_slope(v) : 1.0f;
-            if (row < kSteps) {
-                staged[row * kWave + at.lane] = make_float2(delta[r], there ? delta[r] * x[r] : 0.0f);
-                dys[row * kWave + at.lane] = dy[r];
-            }
-            if (Sums) total += delta[r];
+            const float v = (float)in.dt[r] + bias, delta = there ? delta_of(a, v) : 0.0f, slope = Sums || !there ? 0.0f : a.softplus ? softplus_slope(v) : 1.0f;
+            if (row < kSteps) staged[row * kWave + at.lane] = make_float4(delta, there ? (float)in.x[r] : 0.0f, there ? (float)in.dy[r] : 0.0f, slope);
+            if (Sums) total += delta;
         }
         __syncthreads();
         if (t > at.t0) in.ask(a, at, t - kSteps);
@@ -421,53 +415,73 @@ __global__ __launch_bounds__(Waves * kWave) void selective_bwd_kernel(SelArgs a)
             if constexpr (Sums) {
 #pragma unroll
                 for (int k = kSteps - 1; k >= 0; --k) {
-                    const float d = staged[k * kWave + at.lane].x, dy_k = dys[k * kWave + at.lane];
+                    const float d = staged[k * kWave + at.lane].x, dy_k = staged[k * kWave + at.lane].z;
                     const Shared *w = wr + k * 2 * kOwn;
 #pragma unroll
                     for (int i = 0; i < kOwn; ++i) back[i] = exp2_of(d * rate2[i]) * fmaf(dy_k, w[kOwn + i], back[i]);
                 }
             } else {
-                float e[kSteps][kOwn], eh[kSteps][kOwn], h[kOwn];
-                get_states(a.marks + (t / kSteps * a.batch * a.dim + column) * a.n_states, n0, a.n_states, whole_states(a, a.marks), h);
+                float first[kOwn], middle[kOwn];
+                get_states(a.marks + (t / kSteps * a.batch * a.dim + column) * a.n_states, n0, a.n_states, whole_states(a, a.marks), first);
                 if (!at.there)   // (a neighbour's may be infinite, and is not this lane's to add up)
 #pragma unroll
-                    for (int i = 0; i < kOwn; ++i) h[i] = 0.0f;
+                    for (int i = 0; i < kOwn; ++i) first[i] = 0.0f;
 #pragma unroll
-                for (int k = 0; k < kSteps; ++k) {
-                    if (k % 4 == 0) asm volatile("" : "+s"(wr), "+v"(h[0]));
-                    const float2 d = staged[k * kWave + at.lane];
-                    const Shared *w = wr + k * 2 * kOwn;
+                for (int i = 0; i < kOwn; ++i) middle[i] = first[i];
+                if constexpr (kParts == 2) {
 #pragma unroll
-                    for (int i = 0; i < kOwn; ++i) {
-                        e[k][i] = exp2_of(d.x * rate2[i]);
-                        eh[k][i] = e[k][i] * h[i];
-                        h[i] = fmaf(d.y, w[i], eh[k][i]);
+                    for (int k = 0; k < kEach; ++k) {
+                        if (k % 4 == 0) asm volatile("" : "+s"(wr), "+v"(middle[0]));
+                        const float4 d = staged[k * kWave + at.lane];
+                        const float u = d.x * d.y;
+#pragma unroll
+                        for (int i = 0; i < kOwn; ++i) middle[i] = fmaf(u, wr[k * 2 * kOwn + i], exp2_of(d.x * rate2[i]) * middle[i]);
                     }
                 }
                 float sum_read[kSteps], sum_write[kSteps];
 #pragma unroll
-                for (int k = kSteps - 1; k >= 0; --k) {
-                    // (write and read are asked for again, four steps at a time: there are no scalar registers to keep those of the block in)
-                    if (k % 4 == 3) asm volatile("" : "+s"(wr), "+v"(back[0]));
-                    const float2 d = staged[k * kWave + at.lane];
-                    const float dy_k = dys[k * kWave + at.lane];
-                    const Shared *w = wr + k * 2 * kOwn;
-                    float s1 = 0.0f, s2 = 0.0f, by_read[kOwn], by_write[kOwn];
+                for (int part = kParts - 1; part >= 0; --part) {
+                    float e[kEach][kOwn], eh[kEach][kOwn], h[kOwn];
 #pragma unroll
-                    for (int i = 0; i < kOwn; ++i) {
-                        const float g = fmaf(dy_k, w[kOwn + i], back[i]);
-                        by_read[i] = dy_k * fmaf(d.y, w[i], eh[k][i]);
-                        by_write[i] = g * d.y;
-                        s1 = fmaf(g, w[i], s1);
-                        const float q = g * eh[k][i];
-                        s2 = fmaf(q, rate[i], s2);
-                        d_rate[i] = fmaf(q, d.x, d_rate[i]);
-                        back[i] = e[k][i] * g;
+                    for (int i = 0; i < kOwn; ++i) h[i] = part ? middle[i] : first[i];
+#pragma unroll
+                    for (int k = 0; k < kEach; ++k) {
+                        if (k % 4 == 0) asm volatile("" : "+s"(wr), "+v"(h[0]));
+                        const float4 d = staged[(part * kEach + k) * kWave + at.lane];
+                        const float u = d.x * d.y;
+                        const Shared *w = wr + (part * kEach + k) * 2 * kOwn;
+#pragma unroll
+                        for (int i = 0; i < kOwn; ++i) {
+                            e[k][i] = exp2_of(d.x * rate2[i]);
+                            eh[k][i] = e[k][i] * h[i];
+                            h[i] = fmaf(u, w[i], eh[k][i]);
+                        }
                     }
-                    parts[(at.wave * kSteps + k) * kWave + at.lane] = make_float2(s1, s2);
-                    // states 0 and 2, 1 and 3 share a register, in halves; then all four, in rows of 16 lanes: 0, 1, 2, 3
-                    sum_read[k] = add_rows(add_halves(by_read[0], by_read[2]), add_halves(by_read[1], by_read[3]));
-                    sum_write[k] = add_rows(add_halves(by_write[0], by_write[2]), add_halves(by_write[1], by_write[3]));
+#pragma unroll
+                    for (int q = kEach - 1; q >= 0; --q) {
+                        const int k = part * kEach + q;
+                        // (write and read are asked for again, four steps at a time: there are no scalar registers to keep those of the block in)
+                        if (k % 4 == 3) asm volatile("" : "+s"(wr), "+v"(back[0]));
+                        const float4 d = staged[k * kWave + at.lane];
+                        const float u = d.x * d.y, dy_k = d.z;
+                        const Shared *w = wr + k * 2 * kOwn;
+                        float s1 = 0.0f, s2 = 0.0f, by_read[kOwn], by_write[kOwn];
+#pragma unroll
+                        for (int i = 0; i < kOwn; ++i) {
+                            const float g = fmaf(dy_k, w[kOwn + i], back[i]);
+                            by_read[i] = dy_k * fmaf(u, w[i], eh[q][i]);
+                            by_write[i] = g * u;
+                            s1 = fmaf(g, w[i], s1);
+                            const float by_decay = g * eh[q][i];
+                            s2 = fmaf(by_decay, rate[i], s2);
+                            d_rate[i] = fmaf(by_decay, d.x, d_rate[i]);
+                            back[i] = e[q][i] * g;
+                        }
+                        parts[(at.wave * kSteps + k) * kWave + at.lane] = make_float2(s1, s2);
+                        // states 0 and 2, 1 and 3 share a register, in halves; then all four, in rows of 16 lanes: 0, 1, 2, 3
+                        sum_read[k] = add_rows(add_halves(by_read[0], by_read[2]), add_halves(by_read[1], by_read[3]));
+                        sum_write[k] = add_rows(add_halves(by_write[0], by_write[2]), add_halves(by_write[1], by_write[3]));
+                    }
                 }
                 const float r = sum_rows(sum_read, at.lane), w = sum_rows(sum_write, at.lane);
                 // lane l of a row of 16: the step whose bits were told apart in the order 8, 4, 2, 1
@@ -499,11 +513,12 @@ __global__ __launch_bounds__(Waves * kWave) void selective_bwd_kernel(SelArgs a)
                         s2 += p.y;
                     }
                 const bool there = t + row < at.end;
-                const float dx = there ? fmaf(delta[r], s1, skip * dy[r]) : 0.0f, d_dt = there ? fmaf(x[r], s1, s2) * slope[r] : 0.0f;
+                const float4 d = staged[row * kWave + at.lane];   // (this wavefront's own)
+                const float dx = there ? fmaf(d.x, s1, skip * d.z) : 0.0f, d_dt = there ? fmaf(d.y, s1, s2) * d.w : 0.0f;
                 const int64_t to = ((t + row) * a.batch + at.b) * a.dim + at.c;
                 static_cast<T *>(a.dx)[to] = (T)dx;
                 static_cast<TD *>(a.d_dt)[to] = (TD)d_dt;
-                d_skip = fmaf(dy[r], x[r], d_skip);
+                d_skip = fmaf(d.z, d.y, d_skip);
                 d_bias += d_dt;
             }
         }
@@ -523,11 +538,13 @@ __global__ __launch_bounds__(Waves * kWave) void selective_bwd_kernel(SelArgs a)
         put_states(a.part_rate + stretch_column * a.padded, n0, a.padded, true, d_rate);
         if (blockIdx.y == 0 && a.d_state) put_states(a.d_state + column * a.n_states, n0, a.n_states, whole_states(a, a.d_state), back);
     }
-    staged[at.wave * kWave + at.lane] = make_float2(d_skip, d_bias);
+    float2 *sums = reinterpret_cast<float2 *>(lds);
+    __syncthreads();
+    sums[at.wave * kWave + at.lane] = make_float2(d_skip, d_bias);
     __syncthreads();
     if (at.wave == 0 && at.there) {
         for (int w = 1; w < a.waves; ++w) {
-            const float2 p = staged[w * kWave + at.lane];
+            const float2 p = sums[w * kWave + at.lane];
             d_skip += p.x;
             d_bias += p.y;
         }
@@ -669,7 +686,7 @@ int launch(const char *name, const SelArgs &a, dim3 grid, bool backward, hipStre
     const uint32_t threads = (uint32_t)a.waves * kWave;
     const int64_t columns = a.batch * a.dim;
     const uint32_t joins = (uint32_t)div_up(columns * a.padded, 256);
-    const int32_t unit = kSteps * kWave * 4, lds = (backward ? 3 + 2 * a.waves : 2 + a.waves) * unit;
+    const int32_t unit = kSteps * kWave * 4, lds = (backward ? 4 + 2 * a.waves : 2 + a.waves) * unit;
     if constexpr (Waves > 4) {
         // more than 64 KB of LDS (of 160) has to be asked for, once per kernel and device
         static bool asked[2][64];
@@ -678,7 +695,7 @@ int launch(const char *name, const SelArgs &a, dim3 grid, bool backward, hipStre
         if (err == hipSuccess && !(dev >= 0 && dev < 64 && asked[backward][dev])) {
             const void *kernel = backward ? reinterpret_cast<const void *>(selective_bwd_kernel<T, TD, Waves, Rows, false>)
                                           : reinterpret_cast<const void *>(selective_fwd_kernel<T, TD, Waves, Rows, false>);
-            err = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (backward ? 3 + 2 * Waves : 2 + Waves) * unit);
+            err = hipFuncSetAttribute(kernel, hipFuncAttributeMaxDynamicSharedMemorySize, (backward ? 4 + 2 * Waves : 2 + Waves) * unit);
             if (err == hipSuccess && dev >= 0 && dev < 64) asked[backward][dev] = true;
         }
         if (err != hipSuccess) {
@@ -695,7 +712,7 @@ int launch(const char *name, const SelArgs &a, dim3 grid, bool backward, hipStre
         selective_fwd_kernel<T, TD, Waves, Rows, false><<<grid, threads, lds, s>>>(a);
     } else {
         if (a.stretches > 1) {
-            selective_bwd_kernel<T, TD, Waves, Rows, true><<<grid, threads, 3 * unit, s>>>(a);
+            selective_bwd_kernel<T, TD, Waves, Rows, true><<<grid, threads, 4 * unit, s>>>(a);
             selective_join_kernel<true><<<joins, 256, 0, s>>>(a, columns);
         }
         selective_bwd_kernel<T, TD, Waves, Rows, false><<<grid, threads, lds, s>>>(a);
