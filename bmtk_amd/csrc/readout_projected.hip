@@ -1,8 +1,8 @@
 // Log probabilities of tokens under the softmax of x @ weight^T, and their gradients by x and weight, without the logits in memory.
 //
 // Forward: tiles of logits are made on the matrix cores and reduced where they are, to each row's maximum and sum over the tile's vocabulary;
-// tiles are joined by a second kernel.  Backward: with p = e^logit / sum, G = p - delta, dx = -d_logp G weight and d_weight = -(G^T (d_logp x)): the logits are
-// made again, a piece of the vocabulary at a time, G of the piece is written in 16 bits, and two more products read it.  All of that is one kernel,
+// tiles are joined by a second kernel.  Backward: with p = e^logit / sum and d_logp = m size, size a power of two, G = m (p - delta), dx = -size G weight and d_weight =
+// -(G^T (size x)): the logits are made again, a piece of the vocabulary at a time, G of the piece is written in 16 bits, and two more products read it.  All of that is one kernel,
 // D[i][j] = sum_k A[i][k] B[j][k], whose operands lie in memory with k contiguous or with i (j) contiguous.
 //
 // fp32 operands are taken as three bf16 parts each (8 bits of mantissa a part, 24 in all), whose six largest products are added up: what is left out is below 2^-24
@@ -120,6 +120,23 @@ __device__ __forceinline__ int part_b(int combination) { return 0x021010 >> comb
 __device__ __forceinline__ float base_of(float m) { return rintf(m * (kLog2e * 8.0f)) * 0.125f; }
 __device__ __forceinline__ float exp_over(float v, float base) { return __builtin_amdgcn_exp2f(fmaf(v, kLog2e, -base)); }
 
+// What a row's d_logp (over what is common to all rows) does to its gradient: it is m size with size a power of two.  m is in G, so that G is rounded once and x, times size, not at all;
+// whole is the scale of G times m, by_total that over the row's sum.  All 0 for rows that have no part; a token outside the vocabulary makes everything NaN.
+struct Share {
+    float size, by_total, whole;
+    __device__ __forceinline__ Share(float d, int64_t token, int64_t ignore, int32_t vocab, float peak, float total, float g_scale)
+    {
+        size = by_total = whole = 0.0f;
+        if (token == ignore || (peak == -INFINITY && total == 0.0f)) return;
+        if (token < 0 || token >= vocab) d = NAN;
+        if (d == 0.0f) return;
+        const uint32_t exponent = __float_as_uint(d) & 0x7f800000u;
+        size = exponent == 0x7f800000u ? 1.0f : __uint_as_float(exponent ? exponent : 0x00800000u);
+        whole = g_scale * (d / size);
+        by_total = whole / total;
+    }
+};
+
 __device__ __forceinline__ int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
 
 // bases and sums over them, joined; -inf: nothing yet
@@ -173,10 +190,10 @@ struct Product {
     int64_t ignore;
     float2 *stats;                                // [tiles_i of all pieces][rows]: maximum, sum of e^(logit - maximum)
     float *label;                                 // [rows]: logit of the row's token
-    const float *peak, *total;
+    const float *peak;
+    const float2 *shares;                         // by_total and whole of each row's Share
     void *g;                                      // [parts][piece / 64][rows, to a whole tile][64]: a step's operands lie next to one another in both products that read it
     int64_t g_block, g_part;                      // in numbers
-    float g_scale;
     // kSlab: [slices][nj][slab_stride]; kOut: [nj][ni] of T
     float *slab;
     int64_t slab_stride, slab_size;
@@ -444,13 +461,14 @@ __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void product_kernel(Product p)
         everybody();   // (what was asked for behind the last step has come, too)
         // what the results will be asked for, of this lane's column of each tile: before the next tile's loads, so that it is not waited for behind them
         int64_t token[W];
-        float peak[W], total[W];
+        float peak[W];
+        float2 share[W];
         if constexpr (Mode == kStats || Mode == kGradient) {
 #pragma unroll
             for (int j = 0; j < W; ++j) {
                 const int32_t row = min(j0 + (wj * W + j) * kTile + (lane & 31), p.nj - 1);
                 token[j] = p.tokens[row];
-                if constexpr (Mode == kGradient) peak[j] = p.peak[row], total[j] = p.total[row];
+                if constexpr (Mode == kGradient) peak[j] = p.peak[row], share[j] = p.shares[row];
             }
         }
         if (job + (int32_t)gridDim.x < jobs) begin(job + gridDim.x);
@@ -516,20 +534,20 @@ __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void product_kernel(Product p)
 #pragma unroll
             for (int j = 0; j < W; ++j) {
                 const int32_t row = j0 + (wj * W + j) * kTile + (lane & 31);
-                const bool none = row >= p.nj || token[j] == p.ignore || (peak[j] == -INFINITY && total[j] == 0.0f);
-                const float inverse = p.g_scale / total[j];
+                const float by_total = share[j].x, whole = share[j].y;
+                const bool none = row >= p.nj || whole == 0.0f;
                 const int64_t far = token[j] - p.first - ii0 - 4 * half;
                 const int at = far >= 0 && far < W * kTile && !(far & 4) ? (int)far : -1;
                 if (edge) cut(j);
 #pragma unroll
                 for (int i = 0; i < W; ++i)
 #pragma unroll
-                    for (int r = 0; r < 16; ++r) acc[i][j][r] = none ? 0.0f : exp_over(acc[i][j][r], peak[j]) * inverse;
+                    for (int r = 0; r < 16; ++r) acc[i][j][r] = none ? 0.0f : exp_over(acc[i][j][r], peak[j]) * by_total;
                 if (__ballot(at >= 0 && !none)) {
 #pragma unroll
                     for (int i = 0; i < W; ++i)
 #pragma unroll
-                        for (int r = 0; r < 16; ++r) acc[i][j][r] -= at == i * kTile + 8 * (r / 4) + r % 4 && !none ? p.g_scale : 0.0f;
+                        for (int r = 0; r < 16; ++r) acc[i][j][r] -= at == i * kTile + 8 * (r / 4) + r % 4 && !none ? whole : 0.0f;
                 }
                 V4 out[std::is_same<T, float>::value ? 3 : 1][W][4];
 #pragma unroll
@@ -642,10 +660,10 @@ __global__ __launch_bounds__(256) void lay_kernel(const T *from, int64_t stride,
     for (int j = 0; j < (std::is_same<T, float>::value ? 3 : 1); ++j) *reinterpret_cast<V8 *>(to + j * padded_rows * width + k * 8) = out[j];
 }
 
-// weights[row] = d_logp over a power of two that leaves the largest at 1 to 2 (for fp16; else itself), 0 for rows without a token, NaN for tokens outside
-// the vocabulary; *factor: that power of two
-__global__ __launch_bounds__(1024) void weigh_kernel(const float *d_logp, const int64_t *tokens, int64_t ignore, int64_t rows, int32_t vocab, int32_t normal, float *weights,
-                                                     float *factor)
+// For few rows weights[row] = d_logp, 0 for rows without a token, NaN for tokens outside the vocabulary.  Otherwise, with shares, each row's Share, its size as weight; of fp16 d_logp is over
+// a power of two, *factor, that leaves the largest at 1 to 2
+__global__ __launch_bounds__(1024) void weigh_kernel(const float *d_logp, const int64_t *tokens, int64_t ignore, int64_t rows, int32_t vocab, int32_t normal, const float *peak,
+                                                     const float *total, float g_scale, float *weights, float2 *shares, float *factor)
 {
     __shared__ float most[16];
     float c = 1.0f;
@@ -677,7 +695,13 @@ __global__ __launch_bounds__(1024) void weigh_kernel(const float *d_logp, const 
     const int64_t r = (int64_t)blockIdx.x * 1024 + threadIdx.x;
     if (r < rows) {
         const int64_t token = tokens[r];
-        weights[r] = token == ignore ? 0.0f : token < 0 || token >= vocab ? NAN : d_logp[r] / c;
+        if (shares) {
+            const Share share(d_logp[r] / c, token, ignore, vocab, peak[r], total[r], g_scale);
+            weights[r] = share.size;
+            shares[r] = make_float2(share.by_total, share.whole);
+        } else {
+            weights[r] = token == ignore ? 0.0f : token < 0 || token >= vocab ? NAN : d_logp[r];
+        }
     }
 }
 
@@ -770,7 +794,7 @@ struct Few {
     void *d_weight;
     float *slab;                           // [slices][rows][dim, to a whole 8]
     int32_t slices, slice_rows;            // slices of the vocabulary, of so many of its rows (a multiple of 16)
-    const float *factor;                   // small vocabulary: weights are d_logp over this number (none: 1), and G is (p - delta) / g_unit
+    const float *factor;                   // small vocabulary: the Shares are of d_logp over this number (none: 1), and their scale is 1 / g_unit
     float g_unit;
 };
 
@@ -975,8 +999,8 @@ struct Kept<f16, true> {
 //     dx[r][d] -= G[v][r] w[v][d]   and   d_weight[v][d] = -sum_r G[v][r] d_logp[r] x[r][d]
 // in matrix instructions of 32 bits.  A lane's k are 4 (l / 16) .. 4 (l / 16) + 3, of rows as of the vocabulary, which nothing has to be transposed for, and its C channels are C tiles.
 // Bound by memory: the weights read, their gradient written.
-// Classes: a small vocabulary and many rows, the two in each other's place: of each 16 rows d_weight -= G^T (d_logp x) and dx = -d_logp G weight, in 16 bits where the type has them
-// (G and d_logp x are rounded to it).  Rows that have no part, of weights 0, may hold anything.  A workgroup's wavefronts share a slice of the rows and add up.
+// Classes: a small vocabulary and many rows, the two in each other's place: of each 16 rows d_weight -= G^T (size x) and dx = -size G weight, in 16 bits where the type has them
+// (G is rounded to it; size: see Share).  Rows that have no part, of size 0, may hold anything.  A workgroup's wavefronts share a slice of the rows and add up.
 template <typename T, int J, int C, bool Classes>
 __global__ __launch_bounds__(256) void few_back_kernel(Few a)
 {
@@ -1091,9 +1115,9 @@ struct Small {
     int32_t rows, vocab, dim;
     float *logp, *lse, *peak, *total;   // (peak and total: read by the backward pass)
     const float *d_logp;
-    void *g;                            // [rows, to a whole 32][vocab, to a whole 16]: (p - delta) g_scale
-    float g_scale;
-    float *weights;                     // as weigh_kernel's, if that has not made them; else none
+    void *g;                            // [rows, to a whole 32][vocab, to a whole 16]: p - delta times the Share's whole
+    float *weights;                     // the Shares' sizes
+    const float2 *shares;               // where weigh_kernel has made them, and the sizes; else none
 };
 
 // Split: wavefronts of a workgroup that share rows, each a part of the channels
@@ -1127,17 +1151,23 @@ __global__ __launch_bounds__(Split == 8 ? 512 : 256) void small_kernel(Small a)
         const bool there = row < a.rows;
         const int64_t token = there ? a.tokens[row] : -1;
         if constexpr (Gradient) {
-            const float peak = there ? a.peak[row] : 0.0f, total = there ? a.total[row] : 1.0f, inverse = 1.0f / total;
-            const bool none = !there || token == a.ignore || (peak == -INFINITY && total == 0.0f);
-            if (a.weights && there && quarter == 0) a.weights[row] = token == a.ignore ? 0.0f : token < 0 || token >= a.vocab ? NAN : a.d_logp[row];
+            const float peak = there ? a.peak[row] : 0.0f;
+            float by_total = 0.0f, whole = 0.0f;
+            if (there && a.shares) {
+                by_total = a.shares[row].x, whole = a.shares[row].y;
+            } else if (there) {
+                const Share share(a.d_logp[row], token, a.ignore, a.vocab, peak, a.total[row], 1.0f);
+                by_total = share.by_total, whole = share.whole;
+                if (quarter == 0) a.weights[row] = share.size;
+            }
 #pragma unroll
             for (int j = 0; j < J; ++j) {
                 typename Kept<T, true>::V4 g;
 #pragma unroll
                 for (int r = 0; r < 4; ++r) {
                     const int32_t v = j * 16 + quarter * 4 + r;
-                    const float p = exp_over(acc[j][i][r], peak) * inverse;
-                    g[r] = (typename Kept<T, true>::type)(none || v >= a.vocab ? 0.0f : (v == token ? p - 1.0f : p) * a.g_scale);
+                    const float p = exp_over(acc[j][i][r], peak) * by_total;
+                    g[r] = (typename Kept<T, true>::type)(whole == 0.0f || v >= a.vocab ? 0.0f : v == token ? p - whole : p);
                 }
                 *reinterpret_cast<typename Kept<T, true>::V4 *>(static_cast<typename Kept<T, true>::type *>(a.g) + (int64_t)row * (J * 16) + j * 16 + quarter * 4) = g;
             }
@@ -1231,7 +1261,7 @@ struct Plan {
         if (small) {
             if (!backward) return;
             out_width = up(dim, 8);
-            weights = up(rows * 4 + 4, 256);
+            weights = up(rows * 12 + 4, 256);
             const int32_t j = small_tiles(vocab);
             g = up(up(rows, 64) * j * 16 * 4, 256);
             // slices of the rows, each with sums of its own for d_weight: as many workgroups as the chip holds at once, one or two a compute unit of eight or four tiles of the
@@ -1260,7 +1290,7 @@ struct Plan {
             return;
         }
         out_width = up(dim, 8);
-        weights = up(rows * 4 + 4, 256);
+        weights = up(rows * 12 + 4, 256);
         if (few) {
             // slices of the vocabulary, each with sums of its own for dx: as many workgroups as fill the chip some times, slabs of up to 64 MB
             g = up(up(vocab, 128) * (rows <= 16 ? 16 : rows <= 32 ? 32 : 64) * 4, 256);
@@ -1471,18 +1501,21 @@ void backward(Call c, const float *peak, const float *total, const float *d_logp
     const bool x_fits = fits(c.x, c.x_stride, c.dim, c.dtype), w_fits = fits(c.weight, c.w_stride, c.dim, c.dtype);
     const Plan plan(c.rows, c.vocab, c.dim, c.dtype, x_fits, w_fits, true);
     const bool half = std::is_same<T, f16>::value;
-    // fp16: p down to 2^-39 keeps bits (its subnormals are not lost in the matrix instructions), and d_logp is divided by a power of two
-    const float g_scale = half ? 32768.0f : 1.0f;
-    float *weights = reinterpret_cast<float *>(c.next(plan.weights)), *factor = weights + c.rows;
+    // fp16: p down to 2^-38 keeps bits (its subnormals are not lost in the matrix instructions), and d_logp is divided by a power of two
+    const float g_scale = half ? 16384.0f : 1.0f;
+    float2 *shares = reinterpret_cast<float2 *>(c.next(plan.weights));
+    float *weights = reinterpret_cast<float *>(shares + c.rows), *factor = weights + c.rows;
     char *g = c.next(plan.g), *x_weighted = c.next(plan.x_weighted);
     float *dx_slab = reinterpret_cast<float *>(c.next(plan.dx_slab)), *dw_slab = reinterpret_cast<float *>(c.next(plan.dw_slab));
-    // (a small vocabulary's weights are made beside G, but where they are first divided by what the largest of them needs)
-    if (!plan.small || half) weigh_kernel<<<(uint32_t)div_up(c.rows, 1024), 1024, 0, c.stream>>>(d_logp, c.tokens, c.ignore, c.rows, (int32_t)c.vocab, half && !plan.few, weights, factor);
+    // (a small vocabulary's shares are made beside G, but where they need the largest d_logp first)
+    if (!plan.small || half)
+        weigh_kernel<<<(uint32_t)div_up(c.rows, 1024), 1024, 0, c.stream>>>(d_logp, c.tokens, c.ignore, c.rows, (int32_t)c.vocab, half && !plan.few, peak, total, g_scale, weights,
+                                                                            plan.few ? nullptr : shares, factor);
     if (plan.small) {
         Small m{};
         m.x = c.x, m.weight = c.weight, m.tokens = c.tokens, m.x_stride = c.x_stride, m.w_stride = c.w_stride, m.ignore = c.ignore;
         m.rows = (int32_t)c.rows, m.vocab = (int32_t)c.vocab, m.dim = c.dim, m.peak = const_cast<float *>(peak), m.total = const_cast<float *>(total);
-        m.d_logp = d_logp, m.g = g, m.g_scale = g_scale, m.weights = half ? nullptr : weights;
+        m.d_logp = d_logp, m.g = g, m.weights = weights, m.shares = half ? shares : nullptr;
         small_any<T, true>(m, c.stream);
         Few f{};
         f.x = c.weight, f.weight = c.x, f.x_stride = c.w_stride, f.w_stride = c.x_stride, f.rows = (int32_t)c.vocab, f.vocab = (int32_t)c.rows, f.dim = c.dim;
@@ -1525,7 +1558,7 @@ void backward(Call c, const float *peak, const float *total, const float *d_logp
     for (int64_t q = 0; q < plan.pieces; ++q) {
         const int64_t first = q * plan.piece, count = c.vocab - first < plan.piece ? c.vocab - first : plan.piece;
         Product p = logits<T>(c, plan, x, w, first, count);
-        p.peak = peak, p.total = total, p.g = g, p.g_block = plan.g_rows * 64, p.g_part = plan.g_rows * plan.g_width, p.g_scale = g_scale;
+        p.peak = peak, p.shares = shares, p.g = g, p.g_block = plan.g_rows * 64, p.g_part = plan.g_rows * plan.g_width;
         multiply<E, T, false, false, kGradient>(p, plan.logit_tile, c.stream);
 
         // dx: i a channel, j a row, k the vocabulary

@@ -39,10 +39,10 @@ def reference(c):
     out = dict(lse=(lse, e_lse), logp=(torch.where(given, lp.gather(1, at).squeeze(1), 0.0), torch.where(given, e_logp, 0.0)))
     p = torch.exp(lp)
     g = p.scatter_add(1, at, torch.full_like(at, -1.0, dtype=torch.float64)) * given.unsqueeze(1)
-    # p - delta: p's own error, then half a step of the 16 bits that it is rounded to (fp32: of 24)
+    # p - delta: p's own error, then half a step of the 16 bits that it, or it times up to 2, is rounded to (fp32: of 24); of fp16, in units of 2^-14, half of the smallest step, 2^-25
     half = torch.finfo(dtype).eps / 2 if dtype != torch.float32 else U
     e_p = (p * torch.expm1(e_l + e_lse.unsqueeze(1)) + 8 * U * p) * given.unsqueeze(1)
-    e_g = e_p + half * (g.abs() + e_p) + (2.0 ** -40 if dtype == torch.float16 else 0.0)
+    e_g = e_p + half * (g.abs() + e_p) + (2.0 ** -39 if dtype == torch.float16 else 0.0)
     gm = g.abs() + e_g
     k = 6 if dtype == torch.float32 else 1
     dx = -(d_logp * given).unsqueeze(1) * (g @ w)
