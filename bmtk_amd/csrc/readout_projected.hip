@@ -120,8 +120,8 @@ __device__ __forceinline__ int part_b(int combination) { return 0x021010 >> comb
 __device__ __forceinline__ float base_of(float m) { return rintf(m * (kLog2e * 8.0f)) * 0.125f; }
 __device__ __forceinline__ float exp_over(float v, float base) { return __builtin_amdgcn_exp2f(fmaf(v, kLog2e, -base)); }
 
-// What a row's d_logp (over what is common to all rows) does to its gradient: it is m size with size a power of two.  m is in G, so that G is rounded once and x, times size, not at all;
-// whole is the scale of G times m, by_total that over the row's sum.  All 0 for rows that have no part; a token outside the vocabulary makes everything NaN.
+// What a row's d_logp, over the largest of all rows, does to its gradient: it is m size with size a power of two.  m is in G, so that G is rounded once and x, times size, not at all; of
+// a mean, with one d_logp for all rows, m is 1, and G of a row's token is next to -1, which rounding changes by p at most.  whole is the scale of G times m, by_total that over the row's sum.  All 0 for rows that have no part; a token outside the vocabulary makes everything NaN.
 struct Share {
     float size, by_total, whole;
     __device__ __forceinline__ Share(float d, int64_t token, int64_t ignore, int32_t vocab, float peak, float total, float g_scale)
@@ -662,14 +662,14 @@ __global__ __launch_bounds__(256) void lay_kernel(const T *from, int64_t stride,
     for (int j = 0; j < (std::is_same<T, float>::value ? 3 : 1); ++j) *reinterpret_cast<V8 *>(to + j * padded_rows * width + k * 8) = out[j];
 }
 
-// For few rows weights[row] = d_logp, 0 for rows without a token, NaN for tokens outside the vocabulary.  Otherwise, with shares, each row's Share, its size as weight; of fp16 d_logp is over
-// a power of two, *factor, that leaves the largest at 1 to 2
-__global__ __launch_bounds__(1024) void weigh_kernel(const float *d_logp, const int64_t *tokens, int64_t ignore, int64_t rows, int32_t vocab, int32_t normal, const float *peak,
+// For few rows weights[row] = d_logp, 0 for rows without a token, NaN for tokens outside the vocabulary.  Otherwise, with shares, each row's Share of d_logp over the largest, *factor, and
+// its size as weight
+__global__ __launch_bounds__(1024) void weigh_kernel(const float *d_logp, const int64_t *tokens, int64_t ignore, int64_t rows, int32_t vocab, const float *peak,
                                                      const float *total, float g_scale, float *weights, float2 *shares, float *factor)
 {
     __shared__ float most[16];
     float c = 1.0f;
-    if (normal) {
+    if (shares) {
         // (every workgroup looks at all rows, eight at a time)
         float m = 0.0f;
         for (int64_t r = threadIdx.x; r < rows; r += 8 * 1024) {
@@ -689,9 +689,7 @@ __global__ __launch_bounds__(1024) void weigh_kernel(const float *d_logp, const 
         __syncthreads();
         m = 0.0f;
         for (int k = 0; k < 16; ++k) m = fmaxf(m, most[k]);
-        // (the exponent alone; powers of two from 2^-120 to 2^120, so that neither it nor its inverse is lost)
-        const int e = m > 0.0f ? min(max((int)(__float_as_uint(m) >> 23) - 127, -120), 120) : 0;
-        c = __uint_as_float((uint32_t)(e + 127) << 23);
+        c = m > 0.0f ? fmaxf(m, 0x1p-120f) : 1.0f;   // (so that quotients are not lost)
     }
     if (blockIdx.x == 0 && threadIdx.x == 0) *factor = c;
     const int64_t r = (int64_t)blockIdx.x * 1024 + threadIdx.x;
@@ -1218,8 +1216,8 @@ __global__ __launch_bounds__(256) void few_join_kernel(const float2 *stats, int3
 
 // ---------------------------------------------------------------------------------------------------------------------
 
-// Up to how many rows the kernels for few rows take.  us of 100,000 x 2,000, forward and both ways, few / large tiles: bf16 12 rows 112/148, 507/555; 17: 133/150, 618/556; 33:
-// 144/152, 857/560; 64: 170/152, 1003/564; fp32 12: 201/883, 787/2539; 64: 603/895, 1896/2565.  Large tiles of 16-bit weights whose rows do not
+// Up to how many rows the kernels for few rows take.  us of 100,000 x 2,000, forward and both ways, few / large tiles: bf16 12 rows 100/148, 484/560; 17: 118/150, 603/561; 33:
+// 143/152, 1021/566; 64: 171/152, 1191/571; fp32 12: 203/889, 785/2553; 64: 514/900, 1928/2691.  Large tiles of 16-bit weights whose rows do not
 // begin at whole 16 bytes copy them first, 170 us each way here.
 int32_t few_most(int32_t dtype, bool w_fits, bool backward) { return dtype == BMTK_F32 ? 64 : w_fits ? (backward ? 16 : 32) : (backward ? 32 : 64); }
 // Whether a vocabulary is taken by the kernels for a small one.  Not where there are fewer rows than that, and few.  Of fp32 always: the large tiles copy it in parts first (us forward, both
@@ -1504,26 +1502,27 @@ void backward(Call c, const float *peak, const float *total, const float *d_logp
     const bool x_fits = fits(c.x, c.x_stride, c.dim, c.dtype), w_fits = fits(c.weight, c.w_stride, c.dim, c.dtype);
     const Plan plan(c.rows, c.vocab, c.dim, c.dtype, x_fits, w_fits, true);
     const bool half = std::is_same<T, f16>::value;
-    // fp16: p down to 2^-38 keeps bits (its subnormals are not lost in the matrix instructions), and d_logp is divided by a power of two
+    // fp16: p down to 2^-38 keeps bits (its subnormals are not lost in the matrix instructions), and G, up to 2, stays below the largest
     const float g_scale = half ? 16384.0f : 1.0f;
     float2 *shares = reinterpret_cast<float2 *>(c.next(plan.weights));
     float *weights = reinterpret_cast<float *>(shares + c.rows), *factor = weights + c.rows;
     char *g = c.next(plan.g), *x_weighted = c.next(plan.x_weighted);
     float *dx_slab = reinterpret_cast<float *>(c.next(plan.dx_slab)), *dw_slab = reinterpret_cast<float *>(c.next(plan.dw_slab));
-    // (a small vocabulary's shares are made beside G, but where they need the largest d_logp first)
-    if (!plan.small || half)
-        weigh_kernel<<<(uint32_t)div_up(c.rows, 1024), 1024, 0, c.stream>>>(d_logp, c.tokens, c.ignore, c.rows, (int32_t)c.vocab, half && !plan.few, peak, total, g_scale, weights,
+    // (nothing of fp32 is rounded by which the largest d_logp would matter: of a small vocabulary its shares are made beside G)
+    const bool beside = plan.small && c.dtype == BMTK_F32;
+    if (!beside)
+        weigh_kernel<<<(uint32_t)div_up(c.rows, 1024), 1024, 0, c.stream>>>(d_logp, c.tokens, c.ignore, c.rows, (int32_t)c.vocab, peak, total, g_scale, weights,
                                                                             plan.few ? nullptr : shares, factor);
     if (plan.small) {
         Small m{};
         m.x = c.x, m.weight = c.weight, m.tokens = c.tokens, m.x_stride = c.x_stride, m.w_stride = c.w_stride, m.ignore = c.ignore;
         m.rows = (int32_t)c.rows, m.vocab = (int32_t)c.vocab, m.dim = c.dim, m.peak = const_cast<float *>(peak), m.total = const_cast<float *>(total);
-        m.d_logp = d_logp, m.g = g, m.weights = weights, m.shares = half ? shares : nullptr;
+        m.d_logp = d_logp, m.g = g, m.weights = weights, m.shares = beside ? nullptr : shares;
         small_any<T, true>(m, c.stream);
         Few f{};
         f.x = c.weight, f.weight = c.x, f.x_stride = c.w_stride, f.w_stride = c.x_stride, f.rows = (int32_t)c.vocab, f.vocab = (int32_t)c.rows, f.dim = c.dim;
         f.weights = weights, f.g = reinterpret_cast<float *>(g), f.d_weight = dx, f.slab = dw_slab, f.slices = plan.dw_slices, f.slice_rows = (int32_t)plan.piece;
-        f.factor = half ? factor : nullptr, f.g_unit = 1.0f / g_scale;
+        f.factor = beside ? nullptr : factor, f.g_unit = 1.0f / g_scale;
         const int32_t j = small_tiles(c.vocab);
         const dim3 grid((uint32_t)div_up(c.dim, j == 8 ? 32 : 64), (uint32_t)f.slices);
         // (a lane has two channels instead of four where there are eight tiles of the vocabulary: registers)
