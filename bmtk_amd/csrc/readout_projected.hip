@@ -120,8 +120,9 @@ __device__ __forceinline__ int part_b(int combination) { return 0x021010 >> comb
 __device__ __forceinline__ float base_of(float m) { return rintf(m * (kLog2e * 8.0f)) * 0.125f; }
 __device__ __forceinline__ float exp_over(float v, float base) { return __builtin_amdgcn_exp2f(fmaf(v, kLog2e, -base)); }
 
-// What a row's d_logp, over the largest of all rows, does to its gradient: it is m size with size a power of two.  m is in G, so that G is rounded once and x, times size, not at all; of
-// a mean, with one d_logp for all rows, m is 1, and G of a row's token is next to -1, which rounding changes by p at most.  whole is the scale of G times m, by_total that over the row's sum.  All 0 for rows that have no part; a token outside the vocabulary makes everything NaN.
+// What a row's d_logp, over the largest of all rows, does to its gradient: it is m size with size a power of two.  m is in G, so that G is rounded once and x, times size, not at all;
+// of a mean, with one d_logp for all rows, m is 1, and G of a row's token is next to -1, which rounding changes by p at most.  whole is the scale of G times m, by_total that over the
+// row's sum.  All 0 for rows that have no part; a token outside the vocabulary makes everything NaN.
 struct Share {
     float size, by_total, whole;
     __device__ __forceinline__ Share(float d, int64_t token, int64_t ignore, int32_t vocab, float peak, float total, float g_scale)
@@ -1342,8 +1343,8 @@ bool sizes_fit(int64_t rows, int64_t vocab, int64_t dim, int32_t dtype)
     return rows > 0 && vocab > 0 && dim > 0 && dtype >= 0 && dtype <= 2 && rows < (1 << 22) && vocab < (1 << 28) && dim <= 65536;
 }
 
-// whether rows can be read 16 bytes at a time
-bool fits(const void *p, int64_t stride, int32_t dim, int32_t dtype) { return dtype != BMTK_F32 && dim % 8 == 0 && aligned(p, 16) && stride % 8 == 0; }
+// whether rows can be read 16 bytes at a time, and offsets within a tile of 256 of them are in 32 bits
+bool fits(const void *p, int64_t stride, int32_t dim, int32_t dtype) { return dtype != BMTK_F32 && dim % 8 == 0 && aligned(p, 16) && stride % 8 == 0 && stride < (1 << 21); }
 
 template <typename E, typename T, bool AK, bool BK, int Mode>
 void multiply(Product &p, int32_t tile, hipStream_t s)
@@ -1598,8 +1599,7 @@ int check(const char *name, const Call &c, bool backward)
     BMTK_REQUIRE(c.rows < (1 << 22), "%s: rows must be below 2^22", name);
     BMTK_REQUIRE(c.vocab < (1 << 28), "%s: vocab must be below 2^28", name);
     BMTK_REQUIRE(c.dim <= 65536, "%s: up to 65,536 channels", name);
-    // (offsets within a tile of 256 rows and launches of one dimension are in 32 bits)
-    BMTK_REQUIRE(c.x_stride >= 0 && c.w_stride >= 0 && (c.x_stride < (1 << 21) || c.rows <= 1) && (c.w_stride < (1 << 21) || c.vocab <= 1), "%s: rows further apart than 2^21 numbers", name);
+    BMTK_REQUIRE(c.x_stride >= 0 && c.w_stride >= 0, "%s: strides must not be negative", name);
     // (a launch has up to 2^32 threads: of eight numbers where operands are laid out anew, of four where dx is put together)
     BMTK_REQUIRE(up(c.vocab, 256) * up(c.dim, 64) < (int64_t{1} << 35) && up(c.rows, 256) * up(c.dim, 64) < (int64_t{1} << 34), "%s: too many numbers for a launch", name);
     BMTK_REQUIRE(div_up(c.rows, 128) * div_up(c.vocab, 128) < (int64_t{1} << 31), "%s: too many logits for a launch", name);

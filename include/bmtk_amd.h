@@ -803,7 +803,7 @@ int bmtk_selective_scan_bwd(int64_t n_steps, int64_t batch, int32_t dim, int32_t
  * of 2^(l log2(e) - peak).  The logits are not kept.
  * weight: vocab rows, weight_stride numbers apart.  Rows whose logits hold NaN or +inf have lse and logp NaN.  Sums are in 32 bits; fp32 operands are taken as three
  * bf16 parts each, six of their products, or, of few rows, by fp32 instructions.  Weights are meant to be finite: one that is not makes every row NaN.
- * Limits: rows < 2^22, vocab < 2^28, dim up to 65,536, strides below 2^21; vocab * dim < 2^35, rows * dim < 2^34, and 2^31 squares of 128 x 128 logits. */
+ * Limits: rows < 2^22, vocab < 2^28, dim up to 65,536; vocab * dim < 2^35, rows * dim < 2^34, and 2^31 squares of 128 x 128 logits. */
 int64_t bmtk_projected_logprobs_workspace_bytes(int64_t rows, int32_t vocab, int32_t dim, int32_t dtype, const void *x, int64_t x_stride, const void *weight,
                                                 int64_t weight_stride, int32_t backward);
 int bmtk_projected_logprobs_fwd(int64_t rows, int32_t vocab, int32_t dim, int32_t dtype, const void *x, int64_t x_stride, const void *weight, int64_t weight_stride,

@@ -95,6 +95,50 @@ def test_views_of_anything(rows, dim, dtype):
     check(dict(c, weight=c["weight"][:1].expand(500, dim)))
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("rows", [5, 150])
+def test_rows_far_apart(rows, dtype):
+    """The last step of each of some sequences: rows 2^22 numbers apart."""
+    c = case(rows, 300, 64, dtype)
+    far = torch.empty(rows, 1 << 22, dtype=dtype, device="cuda")[:, -64:]
+    far.copy_(c["x"])
+    check(dict(c, x=far))
+
+
+@pytest.mark.parametrize("rows", [3, 70])
+def test_weights_of_more_than_32_bits_of_offsets(rows):
+    """The last rows of 2.5 billion weights, the others 0: sums over the vocabulary known in closed form."""
+    vocab, dim, used = 1_200_003, 2080, 5
+    g = gen(rows)
+    weight = torch.zeros(vocab, dim, dtype=torch.bfloat16, device="cuda")
+    last = (2.0 / math.sqrt(dim) * torch.randn(used, dim, generator=g)).bfloat16().cuda()
+    weight[-used:] = last
+    x = torch.randn(rows, dim, generator=g).bfloat16().cuda()
+    tokens = vocab - 1 - torch.arange(rows, device="cuda") % used
+    r = readout.projected_logprobs(x, weight, tokens)
+    logits = x.double() @ last.double().t()
+    mag = x.double().abs() @ last.double().abs().t()
+    lse = torch.log(torch.exp(logits).sum(1) + (vocab - used))
+    at = (tokens - (vocab - used)).unsqueeze(1)
+    # as in the other checks: dim + 8 roundings of a logit's terms; a sum of positive terms in additions of 256 and vocab / 256 tiles
+    e_l = (dim + 8) * U * mag
+    e_lse = e_l.amax(1) + (2 * 40 + 8 + 256 + vocab / 256) * U + 4 * U * lse.abs()
+    want = logits.gather(1, at).squeeze(1) - lse
+    close(r.lse, lse, e_lse, "lse")
+    close(r.logp, want, e_lse + e_l.gather(1, at).squeeze(1) + 4 * U * logits.gather(1, at).squeeze(1).abs(), "logp")
+    dx, dw = readout.projected_logprobs_bwd(x, weight, tokens, r, torch.ones(rows, device="cuda"))
+    p = torch.exp(logits - lse.unsqueeze(1))
+    d = torch.zeros_like(p).scatter(1, at, 1.0) - p
+    # d_logp of 1 for all: p - delta is rounded to 16 bits once, and the result once (close's own)
+    e_d = 2.0 ** -8 * d.abs() + p * (e_l + e_lse.unsqueeze(1)) * 2
+    close(dx, d @ last.double(), e_d @ last.double().abs() + (vocab + 16) * U * (d.abs() @ last.double().abs()), "dx")
+    close(dw[-used:], d.t().contiguous() @ x.double(), (e_d + (rows + 16) * U * d.abs()).t().contiguous() @ x.double().abs(), "d_weight")
+    rest = torch.exp(-lse)
+    # (all other rows have the same gradient: minus the sum of x e^-lse)
+    close(dw[0], -(rest @ x.double()), (2.0 ** -8 + 2 * e_lse.max() + (rows + 16) * U) * (rest @ x.double().abs()), "d_weight of weights of 0")
+    assert all(torch.equal(dw[k], dw[0]) for k in (1, 127, 70_000, vocab // 2, vocab - used - 1))
+
+
 def test_shapes_of_more_and_fewer_dimensions():
     c = case(24, 50, 16, torch.bfloat16)
     want = run(c)
