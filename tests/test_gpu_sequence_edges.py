@@ -4,8 +4,9 @@ import math
 
 import pytest
 import torch
+import torch.autograd.forward_ad as forward_ad
 
-from bmtk_amd import readout
+from bmtk_amd import readout, training
 from test_gpu_readout import DTYPES, close, gen
 from test_gpu_sequence import conv_case, conv_run, selective_case, selective_check, selective_reference, selective_run
 
@@ -99,3 +100,45 @@ def test_the_same_bits_again(dtype):
         first = run(case)
         for _ in range(3):
             assert all(torch.equal(first[k], q) for k, q in run(case).items())
+
+
+def calls():
+    """Every call with its tensors by name, float32 on the device."""
+    ones = lambda *shape: torch.full(shape, 0.5, device="cuda")  # noqa: E731
+    conv = dict(x=ones(5, 2, 4), weight=ones(4, 3), bias=ones(4), state=ones(2, 2, 4))
+    scan = dict(x=ones(5, 2, 4), dt=ones(5, 2, 4), rate=-ones(4, 3), write=ones(5, 2, 1, 3), read=ones(5, 2, 1, 3), skip=ones(4), dt_bias=ones(4))
+    rows, tokens = dict(x=ones(5, 4), weight=ones(7, 4)), torch.zeros(5, dtype=torch.int64, device="cuda")
+    loss = dict(weight=ones(10, 14), conv_weight=ones(10, 4), rate=-ones(4, 3), out_weight=ones(7, 4), conv_bias=ones(10), skip=ones(4), dt_bias=ones(4))
+    bits, labels = torch.zeros(5, 1, dtype=torch.int64, device="cuda"), torch.zeros(5, 2, dtype=torch.int64, device="cuda")
+    back = lambda x, weight, peak, total, d_logp: readout.projected_logprobs_bwd(  # noqa: E731
+        x, weight, tokens, readout.ProjectedLogProbs(None, None, peak, total), d_logp)
+    return [(readout.short_conv, conv), (readout.short_conv_bwd, dict(conv, dy=ones(5, 2, 4), d_last=ones(2, 2, 4))), (readout.selective_scan, dict(scan, state=ones(2, 4, 3))),
+            (readout.selective_scan_bwd, dict(scan, saved=ones(1, 2, 4, 3), dy=ones(5, 2, 4), d_last=ones(2, 4, 3))),
+            (lambda **k: readout.projected_logprobs(tokens=tokens, **k), rows), (back, dict(rows, peak=ones(5), total=ones(5), d_logp=ones(5))),
+            (lambda **k: training.sequence_loss(bits, 2, labels=labels, **k), loss)]
+
+
+def test_tensors_that_are_not_what_they_look_like():
+    """Each argument of each call in turn: with a tangent, recorded by autograd, or a view of numbers with the other sign."""
+    for call, given in calls():
+        call(**given)
+        for name, t in given.items():
+            with forward_ad.dual_level():
+                for recording in (True, False):
+                    with torch.set_grad_enabled(recording), pytest.raises(ValueError, match="tangent"):
+                        call(**dict(given, **{name: forward_ad.make_dual(t, torch.ones_like(t))}))
+            with pytest.raises(ValueError, match="requires gradients"):
+                call(**dict(given, **{name: t.clone().requires_grad_()}))
+            with torch.no_grad():
+                call(**dict(given, **{name: t.clone().requires_grad_()}))
+            negated = torch.complex(t, -t).conj().imag
+            if negated.is_neg():
+                with pytest.raises(ValueError, match="resolve_neg|next to one another|contiguous"):
+                    call(**dict(given, **{name: negated}))
+        for name, t in given.items():
+            with pytest.raises(ValueError, match="current device"):
+                call(**dict(given, **{name: t.cpu()}))
+            with pytest.raises(TypeError):
+                call(**dict(given, **{name: t.double()}))
+            with pytest.raises((TypeError, ValueError)):
+                call(**dict(given, **{name: t[..., :-1]}))
