@@ -663,33 +663,50 @@ __global__ __launch_bounds__(256) void lay_kernel(const T *from, int64_t stride,
     for (int j = 0; j < (std::is_same<T, float>::value ? 3 : 1); ++j) *reinterpret_cast<V8 *>(to + j * padded_rows * width + k * 8) = out[j];
 }
 
-// For few rows weights[row] = d_logp, 0 for rows without a token, NaN for tokens outside the vocabulary.  Otherwise, with shares, each row's Share of d_logp over the largest, *factor, and
-// its size as weight
-__global__ __launch_bounds__(1024) void weigh_kernel(const float *d_logp, const int64_t *tokens, int64_t ignore, int64_t rows, int32_t vocab, const float *peak,
-                                                     const float *total, float g_scale, float *weights, float2 *shares, float *factor)
+// The largest finite |d_logp| of the rows that have a token, of those that a workgroup's threads look at: first, first + step, ..., eight at a time
+__device__ __forceinline__ float largest(const float *d_logp, const int64_t *tokens, int64_t ignore, int64_t rows, int64_t first, int64_t step)
 {
     __shared__ float most[16];
-    float c = 1.0f;
-    if (shares) {
-        // (every workgroup looks at all rows, eight at a time)
-        float m = 0.0f;
-        for (int64_t r = threadIdx.x; r < rows; r += 8 * 1024) {
-            float d[8];
-            int64_t t[8];
+    float m = 0.0f;
+    for (int64_t r = first; r < rows; r += 8 * step) {
+        float d[8];
+        int64_t t[8];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const int64_t at = r + i * 1024 < rows ? r + i * 1024 : r;
-                d[i] = fabsf(d_logp[at]), t[i] = tokens[at];
-            }
-#pragma unroll
-            for (int i = 0; i < 8; ++i) m = t[i] != ignore && d[i] < INFINITY ? fmaxf(m, d[i]) : m;
+        for (int i = 0; i < 8; ++i) {
+            const int64_t at = r + i * step < rows ? r + i * step : r;
+            d[i] = fabsf(d_logp[at]), t[i] = tokens[at];
         }
 #pragma unroll
-        for (int k = 32; k; k >>= 1) m = fmaxf(m, __shfl_xor(m, k));
-        if (lane_id() == 0) most[threadIdx.x / kWave] = m;
-        __syncthreads();
-        m = 0.0f;
-        for (int k = 0; k < 16; ++k) m = fmaxf(m, most[k]);
+        for (int i = 0; i < 8; ++i) m = t[i] != ignore && d[i] < INFINITY ? fmaxf(m, d[i]) : m;
+    }
+#pragma unroll
+    for (int k = 32; k; k >>= 1) m = fmaxf(m, __shfl_xor(m, k));
+    if (lane_id() == 0) most[threadIdx.x / kWave] = m;
+    __syncthreads();
+    m = 0.0f;
+    for (int k = 0; k < 16; ++k) m = fmaxf(m, most[k]);
+    return m;
+}
+constexpr int kLargest = 256;   // workgroups, of more than 32,768 rows
+__global__ __launch_bounds__(1024) void largest_kernel(const float *d_logp, const int64_t *tokens, int64_t ignore, int64_t rows, float *out)
+{
+    const float m = largest(d_logp, tokens, ignore, rows, (int64_t)blockIdx.x * 1024 + threadIdx.x, kLargest * 1024);
+    if (threadIdx.x == 0) out[blockIdx.x] = m;
+}
+
+// For few rows weights[row] = d_logp, 0 for rows without a token, NaN for tokens outside the vocabulary.  Otherwise, with shares, each row's Share of d_logp over the largest, *factor, and
+// its size as weight.  The largest: that of largest_kernel's, or, without those, of all rows, which every workgroup looks at
+__global__ __launch_bounds__(1024) void weigh_kernel(const float *d_logp, const int64_t *tokens, int64_t ignore, int64_t rows, int32_t vocab, const float *peak,
+                                                     const float *total, float g_scale, float *weights, float2 *shares, float *factor, const float *parts)
+{
+    float c = 1.0f;
+    if (shares) {
+        float m = 0.0f;
+        if (parts) {
+            for (int k = 0; k < kLargest; ++k) m = fmaxf(m, parts[k]);
+        } else {
+            m = largest(d_logp, tokens, ignore, rows, threadIdx.x, 1024);
+        }
         c = m > 0.0f ? fmaxf(m, 0x1p-120f) : 1.0f;   // (so that quotients are not lost)
     }
     if (blockIdx.x == 0 && threadIdx.x == 0) *factor = c;
@@ -1263,7 +1280,7 @@ struct Plan {
         if (small) {
             if (!backward) return;
             out_width = up(dim, 8);
-            weights = up(rows * 12 + 4, 256);
+            weights = up(rows * 12 + 4 + kLargest * 4, 256);
             const int32_t j = small_tiles(vocab);
             g = up(up(rows, 64) * j * 16 * 4, 256);
             // slices of the rows, each with sums of its own for d_weight: as many workgroups as the chip holds at once, one or two a compute unit of eight or four tiles of the
@@ -1292,7 +1309,7 @@ struct Plan {
             return;
         }
         out_width = up(dim, 8);
-        weights = up(rows * 12 + 4, 256);
+        weights = up(rows * 12 + 4 + kLargest * 4, 256);
         if (few) {
             // slices of the vocabulary, each with sums of its own for dx: as many workgroups as fill the chip some times, slabs of up to 64 MB
             g = up(up(vocab, 128) * (rows <= 16 ? 16 : rows <= 32 ? 32 : 64) * 4, 256);
@@ -1511,9 +1528,11 @@ void backward(Call c, const float *peak, const float *total, const float *d_logp
     float *dx_slab = reinterpret_cast<float *>(c.next(plan.dx_slab)), *dw_slab = reinterpret_cast<float *>(c.next(plan.dw_slab));
     // (nothing of fp32 is rounded by which the largest d_logp would matter: of a small vocabulary its shares are made beside G)
     const bool beside = plan.small && c.dtype == BMTK_F32;
+    float *parts = !beside && !plan.few && c.rows > 32768 ? factor + 1 : nullptr;
+    if (parts) largest_kernel<<<kLargest, 1024, 0, c.stream>>>(d_logp, c.tokens, c.ignore, c.rows, parts);
     if (!beside)
         weigh_kernel<<<(uint32_t)div_up(c.rows, 1024), 1024, 0, c.stream>>>(d_logp, c.tokens, c.ignore, c.rows, (int32_t)c.vocab, peak, total, g_scale, weights,
-                                                                            plan.few ? nullptr : shares, factor);
+                                                                            plan.few ? nullptr : shares, factor, parts);
     if (plan.small) {
         Small m{};
         m.x = c.x, m.weight = c.weight, m.tokens = c.tokens, m.x_stride = c.x_stride, m.w_stride = c.w_stride, m.ignore = c.ignore;

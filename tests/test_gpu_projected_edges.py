@@ -71,8 +71,14 @@ def test_small_vocabularies(rows, vocab, dim, dtype):
     check(case(rows, vocab, dim, dtype))
 
 
-def test_small_vocabulary_of_very_many_rows():
-    check(case(65600, 33, 300, torch.bfloat16))
+@pytest.mark.parametrize("vocab", [33, 130])
+def test_very_many_rows(vocab):
+    """One row's d_logp is far larger than all others', and the last one's."""
+    c = case(65600, vocab, 300, torch.bfloat16)
+    check(c)
+    c["tokens"][65599] = 1
+    c["d_logp"][65599] = 1e6
+    check(c)
 
 
 @pytest.mark.parametrize("rows,vocab,dim", [(1, 1, 1), (1, 1, 64), (70, 1, 5), (1, 300, 1), (65, 2, 3), (400, 3, 1)])
