@@ -130,6 +130,15 @@ def test_goes_on_from_its_memory():
         assert (got - wanted).abs().max() <= tolerance * (1 + wanted.abs().max())
 
 
+def test_no_steps_and_no_labels():
+    d = on_device(case(5, 2, 40, 16, 8, 1, 20, torch.bfloat16))
+    loss, dl_dz, grads, answer, memory = run(dict(d, bits=d["bits"][:0], labels=d["labels"][:0]))
+    assert loss == 0 and dl_dz.shape == (0, 80) and answer.logp.shape == (0, 2) and not any(g.any() for g in grads.values())
+    assert all(torch.equal(p, q) for p, q in zip(memory, d["memory"]))
+    loss, dl_dz, grads, answer, memory = run(dict(d, labels=torch.full_like(d["labels"], -100)))
+    assert loss == 0 and not dl_dz.any() and not any(g.any() for g in grads.values()) and not answer.logp.any() and answer.lse.isfinite().all()
+
+
 def tensors(r):
     loss, dl_dz, grads, answer, memory = r
     return [loss, dl_dz, *grads.values(), *answer, *memory]
