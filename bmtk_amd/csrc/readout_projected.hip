@@ -1588,7 +1588,10 @@ void backward(Call c, const float *peak, const float *total, const float *d_logp
         d.a = by_rows(p.a.p, p.a.stride / 2, p.a.part / 2, count, plan.copy_w ? plan.depth : c.dim);
         d.b = {g, 128, p.g_part * 2, plan.g_rows * 128, p.g_part * 2, 0};
         d.ni = c.dim, d.nj = (int32_t)c.rows;
-        d.steps = (int32_t)div_up(count, kDepth), d.combinations = plan.combinations, d.slices = plan.dx_slices;
+        d.steps = (int32_t)div_up(count, kDepth), d.combinations = plan.combinations;
+        // (a last piece may have fewer steps than there are slabs, and a slice without one would take its neighbour's: the other slabs keep the sums that they have)
+        const int64_t steps = (int64_t)d.steps * d.combinations;
+        d.slices = (int32_t)(steps < plan.dx_slices ? steps : plan.dx_slices);
         d.slab = dx_slab, d.slab_stride = plan.out_width, d.slab_size = c.rows * plan.out_width, d.add = q > 0;
         multiply<E, T, true, false, kSlab>(d, plan.dx_tile, c.stream);
 
