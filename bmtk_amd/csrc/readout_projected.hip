@@ -1444,7 +1444,8 @@ Product logits(const Call &c, const Plan &plan, const char *x, const char *w, in
     const int64_t w_stride = plan.copy_w ? plan.depth : c.w_stride, x_stride = plan.copy_x ? plan.depth : c.x_stride;
     p.a = by_numbers(w + first * w_stride * 2, w_stride, c.vocab * plan.depth, count, plan.copy_w ? plan.depth : c.dim);
     p.b = by_numbers(x, x_stride, c.rows * plan.depth, c.rows, plan.copy_x ? plan.depth : c.dim);
-    p.tail = plan.copy_x ? kDepth : c.dim - (plan.depth - kDepth);
+    // (copies have zeros behind the rows' channels; what lies there of an operand that is read as it is may be NaN, whatever the other one has)
+    p.tail = plan.copy_x && plan.copy_w ? kDepth : c.dim - (plan.depth - kDepth);
     p.ni = (int32_t)count, p.nj = (int32_t)c.rows;
     p.steps = plan.depth / kDepth, p.combinations = plan.combinations, p.slices = 1;
     p.rotate = p.tail == kDepth;
