@@ -122,14 +122,16 @@ __device__ __forceinline__ float exp_over(float v, float base) { return __builti
 
 // What a row's d_logp, over the largest of all rows, does to its gradient: it is m size with size a power of two.  m is in G, so that G is rounded once and x, times size, not at all;
 // of a mean, with one d_logp for all rows, m is 1, and G of a row's token is next to -1, which rounding changes by p at most.  whole is the scale of G times m, by_total that over the
-// row's sum.  All 0 for rows that have no part; a token outside the vocabulary makes everything NaN.
+// row's sum.  All 0 for rows that have no part; a token outside the vocabulary, or logits that are NaN or +inf (whose sum is NaN), makes everything NaN, with a d_logp of 0 too.
+__device__ __forceinline__ bool no_part(int64_t token, int64_t ignore, float peak, float total) { return token == ignore || (peak == -INFINITY && total == 0.0f); }
+__device__ __forceinline__ bool undefined(int64_t token, int32_t vocab, float total) { return token < 0 || token >= vocab || total != total; }
 struct Share {
     float size, by_total, whole;
     __device__ __forceinline__ Share(float d, int64_t token, int64_t ignore, int32_t vocab, float peak, float total, float g_scale)
     {
         size = by_total = whole = 0.0f;
-        if (token == ignore || (peak == -INFINITY && total == 0.0f)) return;
-        if (token < 0 || token >= vocab) d = NAN;
+        if (no_part(token, ignore, peak, total)) return;
+        if (undefined(token, vocab, total)) d = NAN;
         if (d == 0.0f) return;
         const uint32_t exponent = __float_as_uint(d) & 0x7f800000u;
         size = exponent == 0x7f800000u ? 1.0f : __uint_as_float(exponent ? exponent : 0x00800000u);
@@ -694,7 +696,7 @@ __global__ __launch_bounds__(1024) void largest_kernel(const float *d_logp, cons
     if (threadIdx.x == 0) out[blockIdx.x] = m;
 }
 
-// For few rows weights[row] = d_logp, 0 for rows without a token, NaN for tokens outside the vocabulary.  Otherwise, with shares, each row's Share of d_logp over the largest, *factor, and
+// For few rows weights[row] = d_logp, 0 for rows that have no part, NaN where Share has that.  Otherwise, with shares, each row's Share of d_logp over the largest, *factor, and
 // its size as weight.  The largest: that of largest_kernel's, or, without those, of all rows, which every workgroup looks at
 __global__ __launch_bounds__(1024) void weigh_kernel(const float *d_logp, const int64_t *tokens, int64_t ignore, int64_t rows, int32_t vocab, const float *peak,
                                                      const float *total, float g_scale, float *weights, float2 *shares, float *factor, const float *parts)
@@ -718,7 +720,7 @@ __global__ __launch_bounds__(1024) void weigh_kernel(const float *d_logp, const 
             weights[r] = share.size;
             shares[r] = make_float2(share.by_total, share.whole);
         } else {
-            weights[r] = token == ignore ? 0.0f : token < 0 || token >= vocab ? NAN : d_logp[r];
+            weights[r] = no_part(token, ignore, peak[r], total[r]) ? 0.0f : undefined(token, vocab, total[r]) ? NAN : d_logp[r];
         }
     }
 }
@@ -942,7 +944,7 @@ __global__ __launch_bounds__(Split == 8 ? 512 : 256) void few_rows_kernel(Few a)
         const int64_t token = row < a.rows ? a.tokens[row] : -1;
         if constexpr (Gradient) {
             const float peak = row < a.rows ? a.peak[row] : -INFINITY, total = row < a.rows ? a.total[row] : 0.0f, inverse = 1.0f / total;
-            const bool none = row >= a.rows || token == a.ignore || (peak == -INFINITY && total == 0.0f);
+            const bool none = row >= a.rows || no_part(token, a.ignore, peak, total);
 #pragma unroll
             for (int i = 0; i < 2; ++i)
 #pragma unroll

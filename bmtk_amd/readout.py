@@ -586,8 +586,8 @@ def projected_logprobs(x, weight, tokens, ignore=-100):
     x       [..., channels], the channels of a row next to one another
     weight  [vocabulary, channels], of the type of ``x``: a row for each token, the channels next to one another
     tokens  int64 [...]; ``ignore`` where a row has none (padding): its logp is 0.  A token outside the vocabulary has logp NaN
-    Rows whose logits hold NaN or +inf have lse and logp NaN.  Weights are meant to be finite: one that is not makes every row NaN.  float32 arguments of more than
-    64 rows, with more than 128 in the vocabulary, are multiplied in three parts of 16 bits that hold all their bits."""
+    Rows whose logits hold NaN or +inf have lse and logp NaN, rows of nothing but -inf -inf.  Weights are meant to be finite: one that is not makes every row NaN.  float32 arguments of more than
+    64 rows, with more than 128 in the vocabulary, are multiplied in three parts of 16 bits that hold all their bits; a row of those that holds an infinity has NaN where its logits would be -inf."""
     r = _native.projected_logprobs(x, weight, tokens, ignore)
     if r is not None:
         return ProjectedLogProbs(*r)
@@ -604,9 +604,9 @@ def projected_logprobs(x, weight, tokens, ignore=-100):
 def projected_logprobs_bwd(x, weight, tokens, fwd, d_logp, ignore=-100):
     """(dx, d_weight), of the types and shapes of ``x`` and ``weight``, from the gradient of logp, ``d_logp`` (float32, of the shape of the tokens).
 
-    x, weight, tokens, ignore: as they were; fwd: what ``projected_logprobs`` returned.  Rows without a token have a gradient of 0 and no part in d_weight, whatever
-    they hold; a row whose token lies outside the vocabulary, or whose logits hold NaN or +inf, makes its own gradient and all of d_weight
-    NaN.  The logits are made again, in pieces of up to 512 MB of the vocabulary, and p - delta, times the mantissa of d_logp over the largest, is rounded to 16 bits (of float32: kept);
+    x, weight, tokens, ignore: as they were; fwd: what ``projected_logprobs`` returned.  Rows without a token, and rows of nothing but -inf, have a
+    gradient of 0 and no part in d_weight, whatever they hold; a row whose token lies outside the vocabulary, or whose logits hold NaN or +inf, makes its own gradient and all of
+    d_weight NaN, with a d_logp of 0 too.  The logits are made again, in pieces of up to 512 MB of the vocabulary, and p - delta, times the mantissa of d_logp over the largest, is rounded to 16 bits (of float32: kept);
     float16 holds no gradient below 6e-8: give it a scaled d_logp, as a mean over many rows needs."""
     r = _native.projected_logprobs_bwd(x, weight, tokens, fwd.peak, fwd.total, d_logp, ignore)
     if r is not None:

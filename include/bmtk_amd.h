@@ -801,15 +801,15 @@ int bmtk_selective_scan_bwd(int64_t n_steps, int64_t batch, int32_t dim, int32_t
 /* Of each of `rows` rows of x (x_stride numbers apart), with logits l[v] = x . weight[v] over `dim` channels: lse = log of the sum of e^l, logp = l[token] - lse (0 where
  * the token is `ignore`, NaN where it lies outside 0 .. vocab - 1), peak = a multiple of 1/8 next to the largest logit times log2(e), total = the sum
  * of 2^(l log2(e) - peak).  The logits are not kept.
- * weight: vocab rows, weight_stride numbers apart.  Rows whose logits hold NaN or +inf have lse and logp NaN.  Sums are in 32 bits; fp32 operands are taken as three
- * bf16 parts each, six of their products, or, of few rows and small vocabularies, by fp32 instructions.  Weights are meant to be finite: one that is not makes every row NaN.
+ * weight: vocab rows, weight_stride numbers apart.  Rows whose logits hold NaN or +inf have lse and logp NaN, rows of nothing but -inf -inf.  Sums are in 32 bits; fp32 operands are taken as three
+ * bf16 parts each, six of their products (logits of an infinity are NaN there), or, of few rows and small vocabularies, by fp32 instructions.  Weights are meant to be finite: one that is not makes every row NaN.
  * Limits: rows < 2^22, vocab < 2^28, dim up to 65,536; vocab * dim < 2^35, rows * dim < 2^34, and 2^31 squares of 128 x 128 logits. */
 int64_t bmtk_projected_logprobs_workspace_bytes(int64_t rows, int32_t vocab, int32_t dim, int32_t dtype, const void *x, int64_t x_stride, const void *weight,
                                                 int64_t weight_stride, int32_t backward);
 int bmtk_projected_logprobs_fwd(int64_t rows, int32_t vocab, int32_t dim, int32_t dtype, const void *x, int64_t x_stride, const void *weight, int64_t weight_stride,
                                 const int64_t *tokens, int64_t ignore, float *logp, float *lse, float *peak, float *total, void *workspace, void *stream);
-/* dx [rows][dim], d_weight [vocab][dim], contiguous and of dtype, from d_logp [rows]; peak and total are the forward pass's.  Rows without a token have dx 0 and no part in
- * d_weight, whatever they hold; a row whose token lies outside the vocabulary, or whose logits hold NaN or +inf, makes its dx and all of d_weight NaN.  Logits are made
+/* dx [rows][dim], d_weight [vocab][dim], contiguous and of dtype, from d_logp [rows]; peak and total are the forward pass's.  Rows without a token, and rows of nothing but -inf, have dx 0 and no part in
+ * d_weight, whatever they hold; a row whose token lies outside the vocabulary, or whose logits hold NaN or +inf, makes its dx and all of d_weight NaN, with a d_logp of 0 too.  Logits are made
  * again, in pieces of the vocabulary of up to 512 MB; p - delta, times the mantissa of d_logp over the largest, is rounded to dtype's 16 bits (fp32: in three parts, or not). */
 int bmtk_projected_logprobs_bwd(int64_t rows, int32_t vocab, int32_t dim, int32_t dtype, const void *x, int64_t x_stride, const void *weight, int64_t weight_stride,
                                 const int64_t *tokens, int64_t ignore, const float *peak, const float *total, const float *d_logp, void *dx, void *d_weight, void *workspace,
