@@ -140,6 +140,14 @@ struct Share {
     }
 };
 
+// fp16: x times size would be among the subnormals, or lost, where one row's d_logp is some 2^14 times another's.  reach is the largest |x| size of the call, and x size is kept times the power of
+// two that takes that to 2^14 or more, below 2^15: what is rounded then is 2^-28 of the largest or less.  (Of bf16 and fp32, whose smallest numbers are far away, there is none.)
+__device__ __forceinline__ float lift_of(const float *reach)
+{
+    if (!reach || !(*reach > 0.0f)) return 1.0f;
+    return __uint_as_float((127u + 14u + 127u - (__float_as_uint(fmaxf(*reach, 0x1p-100f)) >> 23)) << 23);
+}
+
 __device__ __forceinline__ int64_t up8(int64_t n) { return (n + 7) / 8 * 8; }
 
 // bases and sums over them, joined; -inf: nothing yet
@@ -202,7 +210,7 @@ struct Product {
     int64_t slab_stride, slab_size;
     int32_t add;                                  // to what is in the slab
     void *out;
-    const float *factor;                          // (one number) kOut: results times this and out_scale
+    const float *factor, *reach;                  // (one number each) kOut: results times this and out_scale, over lift_of the other
     float out_scale;
 };
 
@@ -581,7 +589,7 @@ __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void product_kernel(Product p)
                 }
             }
         } else {
-            const float scale = Mode == kOut ? p.out_scale * *p.factor : 1.0f;
+            const float scale = Mode == kOut ? p.out_scale * *p.factor / lift_of(p.reach) : 1.0f;
             // (rows of whole 16 bytes can go out in those)
             const bool rows_fit = Mode == kOut && sizeof(T) == 2 && p.ni % 8 == 0 && (reinterpret_cast<uintptr_t>(p.out) & 15) == 0;
 #pragma unroll
@@ -633,10 +641,10 @@ __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void product_kernel(Product p)
 // ---------------------------------------------------------------------------------------------------------------------
 // what goes before and after
 
-// Rows of n numbers, `width` (n or more, with zeros; a multiple of 8) apart, of T or as the three parts of float; with `by`, times by[row], and rows that have no
-// token are 0.  Eight numbers a lane.
+// Rows of n numbers, `width` (n or more, with zeros; a multiple of 8) apart, of T or as the three parts of float; with `by`, times by[row] and lift_of(reach), and
+// rows that have no part are 0.  Eight numbers a lane.
 template <typename T, typename E>
-__global__ __launch_bounds__(256) void lay_kernel(const T *from, int64_t stride, int64_t rows, int32_t n, int32_t width, int64_t padded_rows, E *to, const float *by)
+__global__ __launch_bounds__(256) void lay_kernel(const T *from, int64_t stride, int64_t rows, int32_t n, int32_t width, int64_t padded_rows, E *to, const float *by, const float *reach)
 {
     const int64_t k = (int64_t)blockIdx.x * 256 + threadIdx.x, row = k / (width / 8);
     const int32_t c = (int32_t)(k - row * (width / 8)) * 8;
@@ -645,7 +653,7 @@ __global__ __launch_bounds__(256) void lay_kernel(const T *from, int64_t stride,
     const int some = row < rows ? n - c : 0;
     if (some >= 8) in.load(from + row * stride + c);
     else in.load_some(from + row * stride + c, some);
-    const float f = by && row < rows ? by[row] : 1.0f;
+    const float f = by && row < rows ? by[row] * lift_of(reach) : 1.0f;
     typedef typename Vec<E>::V8 V8;
     V8 out[std::is_same<T, float>::value ? 3 : 1];
 #pragma unroll
@@ -696,10 +704,39 @@ __global__ __launch_bounds__(1024) void largest_kernel(const float *d_logp, cons
     if (threadIdx.x == 0) out[blockIdx.x] = m;
 }
 
+// reach (see lift_of) of finite numbers; weigh_kernel has made it 0.  The largest of all does not depend on who comes first.
+__global__ __launch_bounds__(1024) void reach_kernel(const f16 *x, int64_t stride, int64_t rows, int32_t n, const float *sizes, float *reach)
+{
+    __shared__ float most[16];
+    const int32_t each = (n + 7) / 8;
+    float m = 0.0f;
+#pragma unroll 4
+    for (int64_t k = (int64_t)blockIdx.x * 1024 + threadIdx.x; k < rows * each; k += (int64_t)gridDim.x * 1024) {
+        const int64_t row = k / each;
+        const int32_t c = (int32_t)(k - row * each) * 8;
+        Loose8<f16> in;
+        if (c + 8 <= n) in.load(x + row * stride + c);
+        else in.load_some(x + row * stride + c, n - c);
+        const float size = sizes[row];   // (0: the row may hold anything)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float v = fabsf((float)in.v[i]);
+            m = v < INFINITY ? fmaxf(m, v * size) : m;
+        }
+    }
+#pragma unroll
+    for (int k = 32; k; k >>= 1) m = fmaxf(m, __shfl_xor(m, k));
+    if (lane_id() == 0) most[threadIdx.x / kWave] = m;
+    __syncthreads();
+    if (threadIdx.x != 0) return;
+    for (int k = 1; k < 16; ++k) m = fmaxf(m, most[k]);
+    atomicMax(reinterpret_cast<uint32_t *>(reach), __float_as_uint(m));   // (0 or more: their bits are in their order)
+}
+
 // For few rows weights[row] = d_logp, 0 for rows that have no part, NaN where Share has that.  Otherwise, with shares, each row's Share of d_logp over the largest, *factor, and
 // its size as weight.  The largest: that of largest_kernel's, or, without those, of all rows, which every workgroup looks at
 __global__ __launch_bounds__(1024) void weigh_kernel(const float *d_logp, const int64_t *tokens, int64_t ignore, int64_t rows, int32_t vocab, const float *peak,
-                                                     const float *total, float g_scale, float *weights, float2 *shares, float *factor, const float *parts)
+                                                     const float *total, float g_scale, float *weights, float2 *shares, float *factor, float *reach, const float *parts)
 {
     float c = 1.0f;
     if (shares) {
@@ -711,7 +748,7 @@ __global__ __launch_bounds__(1024) void weigh_kernel(const float *d_logp, const 
         }
         c = m > 0.0f ? fmaxf(m, 0x1p-120f) : 1.0f;   // (so that quotients are not lost)
     }
-    if (blockIdx.x == 0 && threadIdx.x == 0) *factor = c;
+    if (blockIdx.x == 0 && threadIdx.x == 0) *factor = c, *reach = 0.0f;
     const int64_t r = (int64_t)blockIdx.x * 1024 + threadIdx.x;
     if (r < rows) {
         const int64_t token = tokens[r];
@@ -764,7 +801,7 @@ __global__ __launch_bounds__(1024) void stats_join_kernel(const float2 *stats, i
 // Results from their slabs: rows of `width` numbers, n of them there.  `ways` wavefronts of a workgroup share 64 times four numbers, each takes every so manieth slab.
 template <typename T>
 __global__ __launch_bounds__(1024) void slab_join_kernel(const float *slab, int32_t slabs, int64_t slab_size, int64_t rows, int32_t n, int32_t width, int32_t ways, const float *by,
-                                                         const float *factor, float scale, T *out)
+                                                         const float *factor, const float *reach, float scale, T *out)
 {
     __shared__ Acc4 parts[16][64];
     const int wave = threadIdx.x / kWave, lane = lane_id(), way = wave % ways;
@@ -791,7 +828,7 @@ __global__ __launch_bounds__(1024) void slab_join_kernel(const float *slab, int3
         for (int w = 1; w < ways; ++w) v += parts[wave + w][lane];
     }
     if (!there) return;
-    const float w = by ? by[row] : 1.0f, f = scale * (factor ? *factor : 1.0f) * w;
+    const float w = by ? by[row] : 1.0f, f = scale * (factor ? *factor : 1.0f) / lift_of(reach) * w;
     const float r[4] = {w == 0.0f ? 0.0f : v[0] * f, w == 0.0f ? 0.0f : v[1] * f, w == 0.0f ? 0.0f : v[2] * f, w == 0.0f ? 0.0f : v[3] * f};
     put<T, 4>(out + row * n + c, r, n - c);
 }
@@ -814,7 +851,7 @@ struct Few {
     void *d_weight;
     float *slab;                           // [slices][rows][dim, to a whole 8]
     int32_t slices, slice_rows;            // slices of the vocabulary, of so many of its rows (a multiple of 16)
-    const float *factor;                   // small vocabulary: the Shares are of d_logp over this number (none: 1), and their scale is 1 / g_unit
+    const float *factor, *reach;           // small vocabulary: the Shares are of d_logp over this number (none: 1), and their scale is 1 / g_unit; see lift_of
     float g_unit;
 };
 
@@ -1020,7 +1057,7 @@ struct Kept<f16, true> {
 // in matrix instructions of 32 bits.  A lane's k are 4 (l / 16) .. 4 (l / 16) + 3, of rows as of the vocabulary, which nothing has to be transposed for, and its C channels are C tiles.
 // Bound by memory: the weights read, their gradient written (16 x 194,675 x 3,999 fp32 1.86 ms, 3.35 TB/s).
 // Classes: a small vocabulary and many rows, the two in each other's place: of each 16 rows d_weight -= G^T (size x) and dx = -size G weight, in 16 bits where the type has them
-// (G is rounded to it; size: see Share).  Rows that have no part, of size 0, may hold anything.  A workgroup's wavefronts share a slice of the rows and add up.
+// (G is rounded to it; size: see Share, and lift_of).  Rows that have no part, of size 0, may hold anything.  A workgroup's wavefronts share a slice of the rows and add up.
 template <typename T, int J, int C, bool Classes>
 __global__ __launch_bounds__(256) void few_back_kernel(Few a)
 {
@@ -1051,7 +1088,7 @@ __global__ __launch_bounds__(256) void few_back_kernel(Few a)
         for (int q = 0; q < C; ++q) dx[j][q] = Acc4{0.0f, 0.0f, 0.0f, 0.0f};
     constexpr int kEach = Classes ? 64 : 16;   // rows that a workgroup, or a wavefront of its own, goes on by
     const int32_t v_end = min((int32_t)(blockIdx.y + 1) * a.slice_rows, a.vocab), v_first = blockIdx.y * a.slice_rows + (Classes ? wave * 16 : 0);
-    const float factor = !Classes ? 1.0f : a.factor ? *a.factor * a.g_unit : a.g_unit;
+    const float factor = !Classes ? 1.0f : a.factor ? *a.factor * a.g_unit : a.g_unit, lift = Classes ? lift_of(a.reach) : 1.0f;
     struct Block {
         In w[4];
         float part[4];
@@ -1081,7 +1118,7 @@ __global__ __launch_bounds__(256) void few_back_kernel(Few a)
 #pragma unroll
         for (int u = 0; u < 4; ++u)
 #pragma unroll
-            for (int q = 0; q < C; ++q) w[q][u] = (G)(!Classes ? (float)now.w[u].v[q] : now.part[u] == 0.0f ? 0.0f : (float)now.w[u].v[q] * now.part[u]);
+            for (int q = 0; q < C; ++q) w[q][u] = (G)(!Classes ? (float)now.w[u].v[q] : now.part[u] == 0.0f ? 0.0f : (float)now.w[u].v[q] * (now.part[u] * lift));
         Acc4 dw[C];
 #pragma unroll
         for (int q = 0; q < C; ++q) dw[q] = Acc4{0.0f, 0.0f, 0.0f, 0.0f};
@@ -1282,7 +1319,7 @@ struct Plan {
         if (small) {
             if (!backward) return;
             out_width = up(dim, 8);
-            weights = up(rows * 12 + 4 + kLargest * 4, 256);
+            weights = up(rows * 12 + 8 + kLargest * 4, 256);
             const int32_t j = small_tiles(vocab);
             g = up(up(rows, 64) * j * 16 * 4, 256);
             // slices of the rows, each with sums of its own for d_weight: as many workgroups as the chip holds at once, one or two a compute unit of eight or four tiles of the
@@ -1311,7 +1348,7 @@ struct Plan {
             return;
         }
         out_width = up(dim, 8);
-        weights = up(rows * 12 + 4 + kLargest * 4, 256);
+        weights = up(rows * 12 + 8 + kLargest * 4, 256);
         if (few) {
             // slices of the vocabulary, each with sums of its own for dx: as many workgroups as fill the chip some times, slabs of up to 64 MB
             g = up(up(vocab, 128) * (rows <= 16 ? 16 : rows <= 32 ? 32 : 64) * 4, 256);
@@ -1377,10 +1414,10 @@ void multiply(Product &p, int32_t tile, hipStream_t s)
 }
 
 template <typename T>
-void lay(const void *from, int64_t stride, int64_t rows, int32_t n, int64_t width, int64_t padded_rows, void *to, const float *by, hipStream_t s)
+void lay(const void *from, int64_t stride, int64_t rows, int32_t n, int64_t width, int64_t padded_rows, void *to, const float *by, const float *reach, hipStream_t s)
 {
     typedef typename Element<T>::type E;
-    lay_kernel<T, E><<<(uint32_t)div_up(padded_rows * width / 8, 256), 256, 0, s>>>(static_cast<const T *>(from), stride, rows, n, (int32_t)width, padded_rows, static_cast<E *>(to), by);
+    lay_kernel<T, E><<<(uint32_t)div_up(padded_rows * width / 8, 256), 256, 0, s>>>(static_cast<const T *>(from), stride, rows, n, (int32_t)width, padded_rows, static_cast<E *>(to), by, reach);
 }
 
 // Few rows of the weights leave the chip empty where a wavefront takes 32 of them: then a workgroup's wavefronts share them, four or eight.
@@ -1484,12 +1521,12 @@ void forward(Call c, float *logp, float *lse, float *peak, float *total)
         const char *x = static_cast<const char *>(c.x), *w = static_cast<const char *>(c.weight);
         if (plan.copy_x) {
             char *to = c.next(plan.x_copy);
-            lay<T>(c.x, c.x_stride, c.rows, c.dim, plan.depth, c.rows, to, nullptr, c.stream);
+            lay<T>(c.x, c.x_stride, c.rows, c.dim, plan.depth, c.rows, to, nullptr, nullptr, c.stream);
             x = to;
         }
         if (plan.copy_w) {
             char *to = c.next(plan.w_copy);
-            lay<T>(c.weight, c.w_stride, c.vocab, c.dim, plan.depth, c.vocab, to, nullptr, c.stream);
+            lay<T>(c.weight, c.w_stride, c.vocab, c.dim, plan.depth, c.vocab, to, nullptr, nullptr, c.stream);
             w = to;
         }
         Product p = logits<T>(c, plan, x, w, 0, c.vocab);
@@ -1501,11 +1538,11 @@ void forward(Call c, float *logp, float *lse, float *peak, float *total)
 }
 
 template <typename T>
-void join_slabs(const float *slab, int32_t slabs, int64_t slab_size, int64_t rows, int32_t n, int64_t width, const float *by, const float *factor, float scale, void *out, hipStream_t s)
+void join_slabs(const float *slab, int32_t slabs, int64_t slab_size, int64_t rows, int32_t n, int64_t width, const float *by, const float *factor, const float *reach, float scale, void *out, hipStream_t s)
 {
     const int32_t ways = slabs <= 4 ? 1 : slabs < 64 ? 4 : 16;
     const uint32_t waves = ways == 16 ? 16 : 4;
-    slab_join_kernel<T><<<(uint32_t)div_up(rows * (width / 4), 64 * (waves / ways)), waves * kWave, 0, s>>>(slab, slabs, slab_size, rows, n, (int32_t)width, ways, by, factor, scale,
+    slab_join_kernel<T><<<(uint32_t)div_up(rows * (width / 4), 64 * (waves / ways)), waves * kWave, 0, s>>>(slab, slabs, slab_size, rows, n, (int32_t)width, ways, by, factor, reach, scale,
                                                                                                           static_cast<T *>(out));
 }
 
@@ -1526,16 +1563,24 @@ void backward(Call c, const float *peak, const float *total, const float *d_logp
     // fp16: p down to 2^-38 keeps bits (its subnormals are not lost in the matrix instructions), and G, up to 2, stays below the largest
     const float g_scale = half ? 16384.0f : 1.0f;
     float2 *shares = reinterpret_cast<float2 *>(c.next(plan.weights));
-    float *weights = reinterpret_cast<float *>(shares + c.rows), *factor = weights + c.rows;
+    float *weights = reinterpret_cast<float *>(shares + c.rows), *factor = weights + c.rows, *reach = factor + 1;
     char *g = c.next(plan.g), *x_weighted = c.next(plan.x_weighted);
     float *dx_slab = reinterpret_cast<float *>(c.next(plan.dx_slab)), *dw_slab = reinterpret_cast<float *>(c.next(plan.dw_slab));
     // (nothing of fp32 is rounded by which the largest d_logp would matter: of a small vocabulary its shares are made beside G)
     const bool beside = plan.small && c.dtype == BMTK_F32;
-    float *parts = !beside && !plan.few && c.rows > 32768 ? factor + 1 : nullptr;
+    float *parts = !beside && !plan.few && c.rows > 32768 ? factor + 2 : nullptr;
     if (parts) largest_kernel<<<kLargest, 1024, 0, c.stream>>>(d_logp, c.tokens, c.ignore, c.rows, parts);
     if (!beside)
         weigh_kernel<<<(uint32_t)div_up(c.rows, 1024), 1024, 0, c.stream>>>(d_logp, c.tokens, c.ignore, c.rows, (int32_t)c.vocab, peak, total, g_scale, weights,
-                                                                            plan.few ? nullptr : shares, factor, parts);
+                                                                            plan.few ? nullptr : shares, factor, reach, parts);
+    if constexpr (std::is_same<T, f16>::value) {
+        if (!plan.few) {
+            const int64_t groups = div_up(c.rows * div_up(c.dim, 8), 1024);
+            reach_kernel<<<(uint32_t)(groups < 256 ? groups : 256), 1024, 0, c.stream>>>(static_cast<const f16 *>(c.x), c.x_stride, c.rows, c.dim, weights, reach);
+        }
+    } else {
+        reach = nullptr;
+    }
     if (plan.small) {
         Small m{};
         m.x = c.x, m.weight = c.weight, m.tokens = c.tokens, m.x_stride = c.x_stride, m.w_stride = c.w_stride, m.ignore = c.ignore;
@@ -1545,7 +1590,7 @@ void backward(Call c, const float *peak, const float *total, const float *d_logp
         Few f{};
         f.x = c.weight, f.weight = c.x, f.x_stride = c.w_stride, f.w_stride = c.x_stride, f.rows = (int32_t)c.vocab, f.vocab = (int32_t)c.rows, f.dim = c.dim;
         f.weights = weights, f.g = reinterpret_cast<float *>(g), f.d_weight = dx, f.slab = dw_slab, f.slices = plan.dw_slices, f.slice_rows = (int32_t)plan.piece;
-        f.factor = beside ? nullptr : factor, f.g_unit = 1.0f / g_scale;
+        f.factor = beside ? nullptr : factor, f.reach = reach, f.g_unit = 1.0f / g_scale;
         const int32_t j = small_tiles(c.vocab);
         const dim3 grid((uint32_t)div_up(c.dim, j == 8 ? 32 : 64), (uint32_t)f.slices);
         // (a lane has two channels instead of four where there are eight tiles of the vocabulary: registers)
@@ -1553,7 +1598,7 @@ void backward(Call c, const float *peak, const float *total, const float *d_logp
         else if (j == 2) few_back_kernel<T, 2, 4, true><<<grid, 256, 0, c.stream>>>(f);
         else if (j == 4) few_back_kernel<T, 4, 4, true><<<grid, 256, 0, c.stream>>>(f);
         else few_back_kernel<T, 8, 2, true><<<grid, 256, 0, c.stream>>>(f);
-        join_slabs<T>(dw_slab, plan.dw_slices, c.vocab * plan.out_width, c.vocab, c.dim, plan.out_width, nullptr, f.factor, -f.g_unit, d_weight, c.stream);
+        join_slabs<T>(dw_slab, plan.dw_slices, c.vocab * plan.out_width, c.vocab, c.dim, plan.out_width, nullptr, f.factor, reach, -f.g_unit, d_weight, c.stream);
         return;
     }
     if (plan.few) {
@@ -1564,22 +1609,22 @@ void backward(Call c, const float *peak, const float *total, const float *d_logp
         if (c.rows <= 16) few_backward<T, 1>(f, c.stream);
         else if (c.rows <= 32) few_backward<T, 2>(f, c.stream);
         else few_backward<T, 4>(f, c.stream);
-        join_slabs<T>(dx_slab, plan.dx_slices, c.rows * plan.out_width, c.rows, c.dim, plan.out_width, weights, nullptr, -1.0f, dx, c.stream);
+        join_slabs<T>(dx_slab, plan.dx_slices, c.rows * plan.out_width, c.rows, c.dim, plan.out_width, weights, nullptr, nullptr, -1.0f, dx, c.stream);
         return;
     }
     const char *x = static_cast<const char *>(c.x), *w = static_cast<const char *>(c.weight);
     if (plan.copy_x) {
         char *to = c.next(plan.x_copy);
-        lay<T>(c.x, c.x_stride, c.rows, c.dim, plan.depth, c.rows, to, nullptr, c.stream);
+        lay<T>(c.x, c.x_stride, c.rows, c.dim, plan.depth, c.rows, to, nullptr, nullptr, c.stream);
         x = to;
     }
     if (plan.copy_w) {
         char *to = c.next(plan.w_copy);
-        lay<T>(c.weight, c.w_stride, c.vocab, c.dim, plan.depth, c.vocab, to, nullptr, c.stream);
+        lay<T>(c.weight, c.w_stride, c.vocab, c.dim, plan.depth, c.vocab, to, nullptr, nullptr, c.stream);
         w = to;
     }
     const int64_t k_rows = up(c.rows, kDepth);
-    lay<T>(c.x, c.x_stride, c.rows, c.dim, plan.out_width, k_rows, x_weighted, weights, c.stream);
+    lay<T>(c.x, c.x_stride, c.rows, c.dim, plan.out_width, k_rows, x_weighted, weights, reach, c.stream);
     for (int64_t q = 0; q < plan.pieces; ++q) {
         const int64_t first = q * plan.piece, count = c.vocab - first < plan.piece ? c.vocab - first : plan.piece;
         Product p = logits<T>(c, plan, x, w, first, count);
@@ -1605,16 +1650,16 @@ void backward(Call c, const float *peak, const float *total, const float *d_logp
         e.ni = c.dim, e.nj = (int32_t)count;
         e.steps = (int32_t)(k_rows / kDepth), e.combinations = plan.combinations, e.slices = plan.dw_slices;
         T *out = static_cast<T *>(d_weight) + first * c.dim;
-        e.out = out, e.factor = factor, e.out_scale = -1.0f / g_scale;
+        e.out = out, e.factor = factor, e.reach = reach, e.out_scale = -1.0f / g_scale;
         e.slab = dw_slab, e.slab_stride = plan.out_width, e.slab_size = count * plan.out_width;
         if (plan.dw_slices == 1) {
             multiply<E, T, true, true, kOut>(e, plan.dw_tile, c.stream);
         } else {
             multiply<E, T, true, true, kSlab>(e, plan.dw_tile, c.stream);
-            join_slabs<T>(dw_slab, plan.dw_slices, e.slab_size, count, c.dim, plan.out_width, nullptr, factor, e.out_scale, out, c.stream);
+            join_slabs<T>(dw_slab, plan.dw_slices, e.slab_size, count, c.dim, plan.out_width, nullptr, factor, reach, e.out_scale, out, c.stream);
         }
     }
-    join_slabs<T>(dx_slab, plan.dx_slices, c.rows * plan.out_width, c.rows, c.dim, plan.out_width, weights, factor, -1.0f / g_scale, dx, c.stream);
+    join_slabs<T>(dx_slab, plan.dx_slices, c.rows * plan.out_width, c.rows, c.dim, plan.out_width, weights, factor, nullptr, -1.0f / g_scale, dx, c.stream);
 }
 
 int check(const char *name, const Call &c, bool backward)

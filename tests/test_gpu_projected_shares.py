@@ -1,4 +1,4 @@
-"""projected_logprobs_bwd of rows that are not finite and have no gradient."""
+"""projected_logprobs_bwd of rows whose d_logp, or whose x, are far apart in size, or that are not finite and have no gradient."""
 import math
 
 import pytest
@@ -7,9 +7,47 @@ import torch
 from bmtk_amd import readout
 from test_gpu_projected import case, run
 from test_gpu_projected_edges import FEW_AND_MANY
-from test_gpu_readout import DTYPES
+from test_gpu_readout import DTYPES, U, close, gen
 
 pytestmark = pytest.mark.gpu
+
+
+@pytest.mark.parametrize("aligned", [True, False])
+@pytest.mark.parametrize("rows,vocab,dim", [(9, 200, 64), (40, 200, 64), (300, 40, 64), (300, 120, 72), (700, 1000, 72), (40000, 20, 64), (33000, 200, 64)])
+@pytest.mark.parametrize("large,size", [(1.0, 1.0), (2.0 ** 9, 2.0 ** -9), (2.0 ** -7, 1.0)])
+def test_fp16_rows_of_far_smaller_gradients(rows, vocab, dim, aligned, large, size):
+    """One row's d_logp is 2^14, and its label one of the two words that it takes for likely; the others' are 2^-10 to 2^-26 of that, and their labels among the other words, of whose
+    gradient they have all but channel 0.  large: that row's x; size: of the other rows' x, which have less or more of d_logp by as much."""
+    g = gen(rows)
+    weight = torch.randn(vocab, dim, generator=g) / 8
+    weight[:2], weight[:, 0] = 0.0, 0.0
+    weight[:2, 0] = 28.0 / large   # (of up to 3,584: e^28, so that all other words have 2^-40 of the row's probability)
+    x = torch.randn(rows, dim, generator=g) * size
+    x[:, 0] = 0.0
+    at = rows // 2
+    x[at] = 0.0
+    x[at, 0] = large
+    tokens = torch.randint(2, vocab, (rows,), generator=g)
+    tokens[at] = 1
+    d_logp = 2.0 ** (4.0 - 16.0 * torch.rand(rows, generator=g)) / size
+    d_logp[at] = 2.0 ** 14 / max(large, 1.0)
+    x, weight, tokens, d_logp = x.half().cuda(), weight.half().cuda(), tokens.cuda(), d_logp.cuda()
+    if not aligned:
+        x, weight = (torch.cat([torch.zeros(len(t), 1, dtype=t.dtype, device="cuda"), t], 1)[:, 1:] for t in (x, weight))
+    got = run(dict(x=x, weight=weight, tokens=tokens, d_logp=d_logp))["d_weight"]
+    xd, wd, dd = x.double(), weight.double(), d_logp.double().unsqueeze(1)
+    logits, mag = xd @ wd.t().contiguous(), xd.abs() @ wd.abs().t().contiguous()
+    p = torch.softmax(logits, 1)
+    gr = p.scatter_add(1, tokens.unsqueeze(1), torch.full_like(tokens.unsqueeze(1), -1.0, dtype=torch.float64))
+    # p: its logit's and its sum's errors; G: half a step of 16 bits, of a smallest step of 2^-24 in units of 2^-14; x times d_logp: half a step of 24 bits for each of three roundings, and half of
+    # the smallest step where the largest product of the call is 2^14 or more of them, twice that for d_logp's mantissa
+    e_p = p * torch.expm1(2 * (dim + 8) * U * mag.amax(1, keepdim=True) + (vocab + 80) * U) + 8 * U * p
+    e_g = e_p + 2.0 ** -11 * (gr.abs() + e_p) + 2.0 ** -39
+    xw = (xd * dd).abs()
+    e_xw = 3 * U * xw + 2.0 ** -38 * xw.max()
+    gm = gr.abs() + e_g
+    error = e_g.t().contiguous() @ (xw + e_xw) + gm.t().contiguous() @ e_xw + (rows + 16) * U * (gm.t().contiguous() @ xw)
+    close(got, -(gr.t().contiguous() @ (xd * dd)), error, "d_weight")
 
 
 @pytest.mark.parametrize("dtype", DTYPES)
