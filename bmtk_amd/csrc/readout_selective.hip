@@ -682,10 +682,11 @@ bool sizes_fit(int64_t n_steps, int64_t batch, int32_t dim, int32_t groups, int3
     if (!(n_steps > 0 && batch > 0 && dim > 0 && groups > 0 && dim % groups == 0 && n_states > 0 && n_states <= BMTK_SELECTIVE_MAX_STATES && n_steps < (int64_t{1} << 31) - 4096 &&
           batch < (int64_t{1} << 31) && batch * dim < (int64_t{1} << 31)))
         return false;
-    // 2^32 threads a launch: one for each state of a step, of a channel; sixteen where a channel's sums are put together, lanes without a channel with the others
-    const int64_t most = int64_t{1} << 32, padded = div_up(n_states, kOwn) * kOwn, rows = div_up(n_steps, kSteps) * kSteps * batch * groups;
-    const int64_t lanes = batch * groups * div_up(dim / groups, kWave) * kWave;
-    return rows < most && rows * padded < most && batch * dim * padded < most && (int64_t)dim * padded < most / 16 - 4096 && lanes < most && lanes * (padded / kOwn) < most;
+    // 2^32 threads a launch, whole workgroups: one for each state of a step, of a channel; sixteen where a channel's sums are put together, which are P and two, lanes without a channel with the
+    // others
+    const int64_t most = (int64_t{1} << 32) - 256, padded = div_up(n_states, kOwn) * kOwn, rows = div_up(n_steps, kSteps) * kSteps * batch * groups;
+    const int64_t lanes = batch * groups * div_up(dim / groups, kWave) * kWave, sums = (div_up(dim * padded, 64) + 2 * div_up(dim, 64)) * 1024;
+    return rows < most && rows * padded < most && batch * dim * padded < most && sums < most && lanes < most && lanes * (padded / kOwn) < most;
 }
 
 template <typename T, typename TD, int Waves, int Rows>

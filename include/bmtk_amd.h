@@ -783,7 +783,7 @@ int bmtk_short_conv_bwd(int64_t n_steps, int64_t batch, int32_t dim, int32_t wid
  * which the backward pass needs.  delta * rate of up to 0, or such that e to its sums over any steps in a row stays in 32 bits; of a state that decays to less,
  * up to 2^-126 of what it was may be left.  Rates are meant to be finite.
  * Limits: n_states in 1 .. BMTK_SELECTIVE_MAX_STATES, batch * dim < 2^31, n_steps < 2^31 - 4096; with P n_states to a multiple of four, n_steps * batch * groups * P,
- * batch * dim * P and 16 dim P below 2^32, channels of a group counted in 64s. */
+ * batch * dim * P and 16 dim (P + 2) below 2^32, less a workgroup, channels of a group counted in 64s. */
 #define BMTK_SELECTIVE_MAX_STATES 64
 int64_t bmtk_selective_scan_workspace_bytes(int64_t n_steps, int64_t batch, int32_t dim, int32_t groups, int32_t n_states, int32_t backward);
 int bmtk_selective_scan_fwd(int64_t n_steps, int64_t batch, int32_t dim, int32_t groups, int32_t n_states, int32_t dtype, int32_t dt_dtype, int32_t softplus, const void *x,

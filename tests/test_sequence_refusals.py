@@ -143,3 +143,12 @@ def test_sequence_loss():
                                 (dict(groups=0), ValueError, "groups"), (dict(weight=[[1.0]]), ValueError, "weight"), (dict(rate=torch.zeros(4)), ValueError, "rate")):
         with pytest.raises(error, match=word):
             training.sequence_loss(**given(**change)[0])
+
+
+@pytest.mark.parametrize("dim,states", [((1 << 26) - 2048, 4), (44_800_000, 1), (44_740_000, 3), ((1 << 24) - 1024, 16)])
+def test_selective_scan_sums_of_too_many_channels(dim, states):
+    """The launch that adds up d_rate, d_skip and d_dt_bias has sixteen threads for each number of a channel, of which there are P and two: 2^32 of them or more are refused."""
+    assert 16 * dim * (-(-states // 4) * 4 + 2) >= 1 << 32 > 16 * dim * (-(-states // 4) * 4)
+    for backward in (False, True):
+        refused(selective(backward, batch=1, dim=dim, states=states), "selective_scan_" + ("bwd" if backward else "fwd"), "too many")
+        assert _lib.load().bmtk_selective_scan_workspace_bytes(20, 1, dim, 1, states, backward) == 0
