@@ -261,7 +261,7 @@ struct Operand {
     }
     // The same where fragments are transposed as they are read: before such a read the compiler would wait for every load to LDS that it knows of, also for those of
     // the other stage.  (The load has no register for a result, it has read those that say where when it is issued, and the kernel waits for it by itself;
-    // nothing else in such a kernel uses m0.  Five wait states: of a scalar register that a vector instruction may just have written.)
+    // nothing else in such a kernel uses m0, which the compiler takes for its own and would warn of here: tests/test_projected_registers.py looks at what it made.  Five wait states: of a scalar register that a vector instruction may just have written.)
     __device__ __forceinline__ void load_untold(int n, uint32_t lds, const Source &s, int32_t step, int which, int wave) const
     {
 #ifdef __HIP_DEVICE_COMPILE__
