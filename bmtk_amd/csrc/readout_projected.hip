@@ -574,7 +574,7 @@ __global__ __launch_bounds__(256, W == 4 ? 1 : 2) void product_kernel(Product p)
                                 split(acc[i][j][q * 4 + r], part);
 #pragma unroll
                                 for (int k = 0; k < 3; ++k) out[k][i][q][r] = part[k];
-                            } else {
+                            } else {   // (what both products read in 16 bits: gradients are off by 1.3 times what rounding them alone would be, 2.2e-3 of 1.7e-3 in bf16)
                                 out[0][i][q][r] = (E)acc[i][j][q * 4 + r];
                             }
                         }
@@ -704,7 +704,8 @@ __global__ __launch_bounds__(1024) void largest_kernel(const float *d_logp, cons
     if (threadIdx.x == 0) out[blockIdx.x] = m;
 }
 
-// reach (see lift_of) of finite numbers; weigh_kernel has made it 0.  The largest of all does not depend on who comes first.
+// reach (see lift_of) of finite numbers; weigh_kernel has made it 0.  The largest of all does not depend on who comes first.  Bound by memory, and a launch: 20,000 x 2,000 17 us of the 122 that
+// the gradient of 64 words takes, 1,000 x 777 6 of 273 of 32,003 words.
 __global__ __launch_bounds__(1024) void reach_kernel(const f16 *x, int64_t stride, int64_t rows, int32_t n, const float *sizes, float *reach)
 {
     __shared__ float most[16];
@@ -1291,7 +1292,7 @@ bool small_vocab(int64_t rows, int64_t vocab, int32_t dim, int32_t dtype, bool x
 int32_t small_tiles(int64_t vocab) { return vocab <= 16 ? 1 : vocab <= 32 ? 2 : vocab <= 64 ? 4 : 8; }
 // wavefronts that share rows: where those would leave the chip empty and channels are enough
 int32_t small_split(int64_t rows, int32_t dim) { return rows >= 32 * 2048 || dim < 256 ? 1 : rows >= 32 * 256 || dim < 1024 ? 4 : 8; }
-constexpr int64_t kPieceBytes = int64_t{512} << 20;   // of G: pieces of the vocabulary are as large as that allows
+constexpr int64_t kPieceBytes = int64_t{512} << 20;   // of G: pieces of the vocabulary are as large as that allows, of 256 words at least
 
 int64_t up(int64_t n, int64_t to) { return div_up(n, to) * to; }
 

@@ -394,14 +394,16 @@ def selective_scan(x, dt, rate, write, read, skip=None, dt_bias=None, softplus=F
 
     x       [steps, sequences, channels]; steps and sequences at any distance in memory, the channels next to one another; dt likewise, of the type of ``x``
             or float32
-    rate    float32 [channels, states], finite, up to 64 states; delta * rate is meant to be 0 or less
+    rate    float32 [channels, states], finite, up to 64 states; delta * rate is meant to be 0 or less, or at least such that e to its sum over any steps in a row
+            stays in 32 bits: the decay of many steps is one exponential, and what it cannot hold makes NaN of a state that is still 0
     write, read  [steps, sequences, groups, states], of the type of ``x``, the states of a step next to one another; each group is for
             channels / groups neighbouring channels
     skip, dt_bias  float32 [channels] (None: zero)
     state   float32 [sequences, channels, states]: the state before the first step (None: zero)
     lengths int32 [sequences]: steps of each sequence (None: all).  y is 0 behind them and nothing of the inputs counts there; values outside
             0..steps count as the nearer of the two
-    y has the type and shape of ``x``; last is float32 and of the state's shape: the ``state`` of the next call, of a single step or of many.
+    y has the type and shape of ``x``; last is float32 and of the state's shape: the ``state`` of the next call, of a single step or of many.  Where delta * x is infinite, y is
+    NaN or infinite: NaN where the states are no multiple of four, too.
     saved: what ``selective_scan_bwd`` takes, float32 [steps / 16, sequences, channels, states]."""
     r = _native.selective_scan(x, dt, rate, write, read, skip, dt_bias, softplus, state, lengths, save_state)
     if r is not None:
@@ -586,7 +588,7 @@ def projected_logprobs(x, weight, tokens, ignore=-100):
     x       [..., channels], the channels of a row next to one another
     weight  [vocabulary, channels], of the type of ``x``: a row for each token, the channels next to one another
     tokens  int64 [...]; ``ignore`` where a row has none (padding): its logp is 0.  A token outside the vocabulary has logp NaN
-    Rows whose logits hold NaN or +inf have lse and logp NaN, rows of nothing but -inf -inf.  Weights are meant to be finite: one that is not makes every row NaN.  float32 arguments of more than
+    Rows whose logits hold NaN or +inf have lse and logp NaN, rows of nothing but -inf -inf; 2^124 and more counts as infinite.  Weights are meant to be finite: one that is not makes every row NaN.  float32 arguments of more than
     64 rows, with more than 128 in the vocabulary, are multiplied in three parts of 16 bits that hold all their bits; a row of those that holds an infinity has NaN where its logits would be -inf."""
     r = _native.projected_logprobs(x, weight, tokens, ignore)
     if r is not None:
@@ -606,7 +608,8 @@ def projected_logprobs_bwd(x, weight, tokens, fwd, d_logp, ignore=-100):
 
     x, weight, tokens, ignore: as they were; fwd: what ``projected_logprobs`` returned.  Rows without a token, and rows of nothing but -inf, have a
     gradient of 0 and no part in d_weight, whatever they hold; a row whose token lies outside the vocabulary, or whose logits hold NaN or +inf, makes its own gradient and all of
-    d_weight NaN, with a d_logp of 0 too.  The logits are made again, in pieces of up to 512 MB of the vocabulary, and p - delta, times the mantissa of d_logp over the largest, is rounded to 16 bits (of float32: kept);
+    d_weight NaN, with a d_logp of 0 too.  The logits are made again, in pieces of the vocabulary of up to 512 MB of p - delta (or of 256 words for all rows, where that is
+    more: 2 GB of four million rows of 16 bits, 6 of float32), which, times the mantissa of d_logp over the largest, is rounded to 16 bits (of float32: kept);
     float16 holds no gradient below 6e-8: give it a scaled d_logp, as a mean over many rows needs."""
     r = _native.projected_logprobs_bwd(x, weight, tokens, fwd.peak, fwd.total, d_logp, ignore)
     if r is not None:

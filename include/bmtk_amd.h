@@ -781,7 +781,7 @@ int bmtk_short_conv_bwd(int64_t n_steps, int64_t batch, int32_t dim, int32_t wid
  * x_t .. read_b: distance of steps and of sequences, in elements; the channels of a step, and its groups' states, lie next to one another; everything else
  * is contiguous.  marks (NULL: not kept): the state before every BMTK_SCAN_MARK-th step, [ceil(n_steps / BMTK_SCAN_MARK)][batch][dim][n_states],
  * which the backward pass needs.  delta * rate of up to 0, or such that e to its sums over any steps in a row stays in 32 bits; of a state that decays to less,
- * up to 2^-126 of what it was may be left.  Rates are meant to be finite.
+ * up to 2^-126 of what it was may be left.  Rates are meant to be finite.  Where delta x is infinite, y is NaN or infinite: NaN where n_states is no multiple of four, too.
  * Limits: n_states in 1 .. BMTK_SELECTIVE_MAX_STATES, batch * dim < 2^31, n_steps < 2^31 - 4096; with P n_states to a multiple of four, n_steps * batch * groups * P,
  * batch * dim * P and 16 dim (P + 2) below 2^32, less a workgroup, channels of a group counted in 64s. */
 #define BMTK_SELECTIVE_MAX_STATES 64
@@ -801,7 +801,7 @@ int bmtk_selective_scan_bwd(int64_t n_steps, int64_t batch, int32_t dim, int32_t
 /* Of each of `rows` rows of x (x_stride numbers apart), with logits l[v] = x . weight[v] over `dim` channels: lse = log of the sum of e^l, logp = l[token] - lse (0 where
  * the token is `ignore`, NaN where it lies outside 0 .. vocab - 1), peak = a multiple of 1/8 next to the largest logit times log2(e), total = the sum
  * of 2^(l log2(e) - peak).  The logits are not kept.
- * weight: vocab rows, weight_stride numbers apart.  Rows whose logits hold NaN or +inf have lse and logp NaN, rows of nothing but -inf -inf.  Sums are in 32 bits; fp32 operands are taken as three
+ * weight: vocab rows, weight_stride numbers apart.  Rows whose logits hold NaN or +inf have lse and logp NaN, rows of nothing but -inf -inf; 2^124 and more counts as infinite.  Sums are in 32 bits; fp32 operands are taken as three
  * bf16 parts each, six of their products (logits of an infinity are NaN there), or, of few rows and small vocabularies, by fp32 instructions.  Weights are meant to be finite: one that is not makes every row NaN.
  * Limits: rows < 2^22, vocab < 2^28, dim up to 65,536; vocab * dim < 2^35, rows * dim < 2^34, and 2^31 squares of 128 x 128 logits. */
 int64_t bmtk_projected_logprobs_workspace_bytes(int64_t rows, int32_t vocab, int32_t dim, int32_t dtype, const void *x, int64_t x_stride, const void *weight,
@@ -810,7 +810,8 @@ int bmtk_projected_logprobs_fwd(int64_t rows, int32_t vocab, int32_t dim, int32_
                                 const int64_t *tokens, int64_t ignore, float *logp, float *lse, float *peak, float *total, void *workspace, void *stream);
 /* dx [rows][dim], d_weight [vocab][dim], contiguous and of dtype, from d_logp [rows]; peak and total are the forward pass's.  Rows without a token, and rows of nothing but -inf, have dx 0 and no part in
  * d_weight, whatever they hold; a row whose token lies outside the vocabulary, or whose logits hold NaN or +inf, makes its dx and all of d_weight NaN, with a d_logp of 0 too.  Logits are made
- * again, in pieces of the vocabulary of up to 512 MB; p - delta, times the mantissa of d_logp over the largest, is rounded to dtype's 16 bits (fp32: in three parts, or not). */
+ * again, in pieces of the vocabulary of up to 512 MB of p - delta (or of 256 words for all rows, where that is more); it, times the mantissa of d_logp over the largest, is rounded to dtype's 16
+ * bits (fp32: in three parts, or not). */
 int bmtk_projected_logprobs_bwd(int64_t rows, int32_t vocab, int32_t dim, int32_t dtype, const void *x, int64_t x_stride, const void *weight, int64_t weight_stride,
                                 const int64_t *tokens, int64_t ignore, const float *peak, const float *total, const float *d_logp, void *dx, void *d_weight, void *workspace,
                                 void *stream);
