@@ -84,3 +84,34 @@ def test_a_row_of_nothing_but_minus_infinity_has_no_part(rows, vocab, dim, dtype
     else:
         assert r.lse[2] == -math.inf and r.logp[2] == -math.inf
         assert not got["dx"][2].any() and torch.equal(got["d_weight"], want["d_weight"])
+
+
+@pytest.mark.parametrize("rows,vocab,dim", [(300, 40, 64), (200, 500, 72)])
+def test_fp16_captured_and_replayed_on_rows_of_other_sizes(rows, vocab, dim):
+    """Two graphs, replayed in turn, whose rows and d_logp are larger or smaller each time; eager work and synchronizations in between."""
+    cases = [case(rows, vocab, dim, torch.float16, seed=s) for s in range(3)]
+    for k, c in enumerate(cases):
+        c["x"], c["weight"] = c["x"] * (1.0, 2.0 ** 6, 2.0 ** -9)[k], c["weight"] / (1.0, 2.0 ** 6, 2.0 ** -5)[k]
+        c["d_logp"] = c["d_logp"] * 2.0 ** -(20.0 * torch.rand(rows, generator=gen(k))).cuda() / (1.0, 2.0 ** 6, 2.0 ** -9)[k]
+    want = [run(c) for c in cases]
+    graphs = []
+    for k in (0, 1):
+        held = {name: t.clone() for name, t in cases[k].items()}
+        side = torch.cuda.Stream()
+        side.wait_stream(torch.cuda.current_stream())
+        with torch.cuda.stream(side):
+            run(held)
+        torch.cuda.current_stream().wait_stream(side)
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            out = run(held)
+        graphs.append((graph, held, out))
+    for turn in range(5):
+        for k, (graph, held, _) in enumerate(graphs):
+            for name, t in cases[(turn + k) % 3].items():
+                held[name].copy_(t)
+            graph.replay()
+        run(cases[2])
+        torch.cuda.synchronize()
+        for k, (_, _, out) in enumerate(graphs):
+            assert all(torch.equal(out[name], t) for name, t in want[(turn + k) % 3].items()), (turn, k)
